@@ -281,6 +281,10 @@ int CheckInputs(const mnb_desc *desc, const void *B, const void *scales, const v
 
 namespace mnb {
 
+void SetLastHipError(const char *what, hipError_t e) { SetLastError(what, e); }
+int CurrentGfx950(int *device) { return CheckDevice(device); }
+int DeviceComputeUnits(int device) { return DeviceCUs(device); }
+
 __global__ __launch_bounds__(256) void SiluMulKernel(const float *__restrict__ Y,
                                                      float *__restrict__ H, int64_t half_mn) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;

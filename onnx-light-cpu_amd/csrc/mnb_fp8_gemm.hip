@@ -1,0 +1,424 @@
+// The 8-bit product on CDNA4's e4m3 MFMA (16x16x128: one instruction per
+// block of 128 values of K).
+//
+// A block's scales are one weight scale s_w (shared by 128 columns) and one
+// row scale s_a, so each block's partial product p = a . w starts from zero
+// in the MFMA and joins the fp32 sum as acc += p * (s_a s_w). The weights are
+// the MFMA's row operand: a lane's four results are four columns of Y for one
+// row, so s_a s_w is one value per lane and fragment.
+//
+// The e4m3 MFMA adds its products in groups of eight, each product cut off
+// 13 bits below the group's largest (measured; between groups it adds in
+// fp32): about 1.4e-5 of Y on normal values. That is a hundredth of bfloat16's
+// rounding and a twentieth of float16's, so a 16-bit Y takes it. An fp32 Y does
+// not (EXACT): both operands are widened to fp16, where e4m3 values and their
+// products are exact, for four fp16 MFMAs (16x16x32) at twice the matrix time.
+#include "mnb_fp8.h"
+
+#include <utility>
+
+namespace mnb {
+namespace fp8 {
+namespace {
+
+typedef int intx4 __attribute__((ext_vector_type(4)));
+typedef int intx8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+
+// One lane's 32 values of a fragment: as codes, or widened to fp16 (EXACT).
+template <bool EXACT>
+struct Fragment;
+
+template <>
+struct Fragment<false> {
+  intx8 v;
+  __device__ __forceinline__ Fragment(intx4 lo, intx4 hi)
+      : v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]} {}
+};
+
+__device__ __forceinline__ halfx8 Widen(int lo, int hi) {
+  const halfx2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
+  const halfx2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
+  const halfx2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false);
+  const halfx2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
+  return halfx8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+template <>
+struct Fragment<true> {
+  halfx8 v[4];
+  __device__ __forceinline__ Fragment(intx4 lo, intx4 hi)
+      : v{Widen(lo[0], lo[1]), Widen(lo[2], lo[3]), Widen(hi[0], hi[1]), Widen(hi[2], hi[3])} {}
+};
+
+__device__ __forceinline__ floatx4 Mfma(const Fragment<false> &w, const Fragment<false> &a) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+      w.v, a.v, floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+}
+
+__device__ __forceinline__ floatx4 Mfma(const Fragment<true> &w, const Fragment<true> &a) {
+  floatx4 p{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    p = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.v[i], a.v[i], p, 0, 0, 0);
+  return p;
+}
+
+// n (up to C) consecutive values of a row of Y; whole: all C, at an address
+// that 16 bytes (or the C values) divide.
+template <typename T, int C>
+__device__ __forceinline__ void StoreRow(T *p, const float *v, int64_t n, bool whole) {
+  if (whole) {
+    constexpr int kPer = C * sizeof(T) >= 16 ? 16 / sizeof(T) : C;
+    typedef T Vec __attribute__((ext_vector_type(kPer)));
+#pragma unroll
+    for (int i = 0; i < C; i += kPer) {
+      Vec q;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) q[j] = static_cast<T>(v[i + j]);
+      *reinterpret_cast<Vec *>(p + i) = q;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (i < n) p[i] = static_cast<T>(v[i]);
+  }
+}
+
+// ---- few rows: the weights streamed once ------------------------------------
+//
+// A workgroup takes RG fragments (16 columns each) and all rows (MC fragments
+// of 16); its wavefronts take the blocks of K in turn and add up in LDS.
+template <int MC, int RG, int WAVES, bool EXACT, typename T>
+__global__ __launch_bounds__(64 * WAVES) void Fp8StreamKernel(
+    const uint8_t *__restrict__ W, const float *__restrict__ SW, const uint8_t *__restrict__ A,
+    const float *__restrict__ SA, T *__restrict__ Y, int M, int64_t N, int64_t lda, int nb) {
+  extern __shared__ floatx4 red[];  // [WAVES][MC * RG][64]
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int c = lane & 15, qd = lane >> 4;
+  const int64_t f0 = static_cast<int64_t>(blockIdx.x) * RG;
+  const int64_t g = f0 >> 2;
+  const int j0 = static_cast<int>(f0 & 3);
+  const uint8_t *w = W + (g * nb * 8 + 2 * j0) * kRec + lane * 16;
+  const float *sw = SW + (g >> 1) * nb;
+  const uint8_t *a[MC];
+  const float *sa[MC];
+#pragma unroll
+  for (int m = 0; m < MC; ++m) {
+    const int64_t row = min(16 * m + c, M - 1);
+    a[m] = A + row * lda + 16 * qd;
+    sa[m] = SA + row * nb;
+  }
+  struct Block {
+    intx4 w[RG][2], a[MC][2];
+    float s[MC];
+  };
+  auto load = [&](int b, Block &o) __attribute__((always_inline)) {
+    b = min(b, nb - 1);
+#pragma unroll
+    for (int r = 0; r < RG; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        o.w[r][h] = *reinterpret_cast<const intx4 *>(
+            w + (static_cast<int64_t>(b) * 8 + 2 * r + h) * kRec);
+    const float scale = sw[b];
+#pragma unroll
+    for (int m = 0; m < MC; ++m) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        o.a[m][h] = *reinterpret_cast<const intx4 *>(a[m] + static_cast<int64_t>(b) * kBlock + 64 * h);
+      o.s[m] = sa[m][b] * scale;
+    }
+  };
+  floatx4 acc[MC][RG];
+#pragma unroll
+  for (int m = 0; m < MC; ++m)
+#pragma unroll
+    for (int r = 0; r < RG; ++r) acc[m][r] = floatx4{0.f, 0.f, 0.f, 0.f};
+  auto multiply = [&](const Block &o) __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = 0; r < RG; ++r) {
+      const Fragment<EXACT> w(o.w[r][0], o.w[r][1]);
+#pragma unroll
+      for (int m = 0; m < MC; ++m) {
+        const floatx4 p = Mfma(w, Fragment<EXACT>(o.a[m][0], o.a[m][1]));
+#pragma unroll
+        for (int v = 0; v < 4; ++v) acc[m][r][v] = fmaf(p[v], o.s[m], acc[m][r][v]);
+      }
+    }
+  };
+  Block x, y;
+  if (wave < nb) load(wave, x);
+  for (int b = wave; b < nb; b += 2 * WAVES) {
+    load(b + WAVES, y);
+    multiply(x);
+    if (b + WAVES < nb) {
+      load(b + 2 * WAVES, x);
+      multiply(y);
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MC; ++m)
+#pragma unroll
+    for (int r = 0; r < RG; ++r) red[(wave * MC * RG + m * RG + r) * 64 + lane] = acc[m][r];
+  __syncthreads();
+  for (int t = wave; t < MC * RG; t += WAVES) {
+    floatx4 sum = red[t * 64 + lane];
+    for (int u = 1; u < WAVES; ++u) sum += red[(u * MC * RG + t) * 64 + lane];
+    const int m = t / RG * 16 + c, r = t % RG;
+    const int64_t n = 64 * g + 16 * qd + 4 * (j0 + r);
+    if (m < M && n < N) {
+      const float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+      StoreRow<T, 4>(Y + m * N + n, v, N - n, N % 4 == 0);
+    }
+  }
+}
+
+// ---- many rows: tiles in LDS --------------------------------------------------
+//
+// WM x WN wavefronts of MI x NJ fragments: a tile of 16 MI WM rows and
+// 16 NJ WN columns. A and W reach LDS by direct copies in the fragments' own
+// order (the lanes of a copy gather the rows of A), so an LDS read is 1 KiB in
+// a row; NS tiles of 128 values of K are in flight.
+template <int MI, int NJ, int WM, int WN, int NS, bool EXACT, typename T>
+__global__ __launch_bounds__(64 * WM *WN) void Fp8TileKernel(
+    const uint8_t *__restrict__ W, const float *__restrict__ SW, const uint8_t *__restrict__ A,
+    const float *__restrict__ SA, T *__restrict__ Y, int64_t M, int64_t N, int64_t lda, int nb,
+    int tiles_m, int tiles_n, int groups, int per_split) {
+  static_assert(NJ == 4, "a wavefront takes one group of 64 columns");
+  constexpr int kWaves = WM * WN;
+  constexpr int kARecs = 2 * MI * WM, kWRecs = 8 * WN;
+  static_assert(kARecs % kWaves == 0 && kWRecs % kWaves == 0, "copies");
+  static_assert(64 * kWaves >= 16 * MI * WM, "one row scale per thread");
+  constexpr int kStage = (kARecs + kWRecs) * kRec + 256 * kWaves;  // bytes; row scales last
+  extern __shared__ uint8_t lds[];
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int c = lane & 15, qd = lane >> 4;
+  const int wm = wave % WM, wn = wave / WM;
+
+  // Workgroup -> tile: an XCD (blockIdx % 8) takes a contiguous run of an order
+  // that walks groups of 4 row tiles column tile by column tile.
+  int tm, tn;
+  {
+    const int tiles = tiles_m * tiles_n;
+    int L = static_cast<int>(blockIdx.x);
+    if (tiles % 8 == 0) L = (L & 7) * (tiles / 8) + (L >> 3);
+    constexpr int kGM = 4;
+    const int group = L / (kGM * tiles_n);
+    const int gm = min(kGM, tiles_m - group * kGM);
+    const int rem = L - group * kGM * tiles_n;
+    tm = group * kGM + rem % gm;
+    tn = rem / gm;
+  }
+  const int b0 = static_cast<int>(blockIdx.y) * per_split;
+  const int b1 = min(nb, b0 + per_split);
+  Y += static_cast<int64_t>(blockIdx.y) * M * N;
+  const int64_t m0 = static_cast<int64_t>(tm) * 16 * MI * WM;
+  const int64_t rows = min(M - m0, static_cast<int64_t>(16 * MI * WM));
+  const int last_row = static_cast<int>(rows) - 1;
+
+  // Copy sources: per-lane offsets from a base that walks K.
+  constexpr int kAC = kARecs / kWaves, kWC = kWRecs / kWaves;
+  uint32_t a_off[kAC];
+  int64_t w_off[kWC];
+#pragma unroll
+  for (int i = 0; i < kAC; ++i) {
+    const int rec = i * kWaves + wave;  // fragment rec / 2, half rec % 2
+    const int row = min(16 * (rec >> 1) + c, last_row);
+    a_off[i] = static_cast<uint32_t>(row * lda + 64 * (rec & 1) + 16 * qd);
+  }
+#pragma unroll
+  for (int i = 0; i < kWC; ++i) {
+    const int rec = i * kWaves + wave;  // group rec / 8 of the tile
+    const int64_t g = min(static_cast<int64_t>(tn) * WN + (rec >> 3), static_cast<int64_t>(groups) - 1);
+    w_off[i] = (g * nb * 8 + (rec & 7)) * kRec;
+  }
+  const uint8_t *a_base = A + m0 * lda;
+  const float *sa_base = SA + (m0 + min(static_cast<int>(threadIdx.x), last_row)) * nb;
+  const uint32_t l16 = static_cast<uint32_t>(lane) * 16;
+  auto issue = [&](int b, int stage) __attribute__((always_inline)) {
+    const uint32_t st = lds0 + stage * kStage;
+#pragma unroll
+    for (int i = 0; i < kAC; ++i)
+      CopyToLds16S(a_base + static_cast<int64_t>(b) * kBlock, a_off[i],
+                   st + (i * kWaves + wave) * kRec);
+#pragma unroll
+    for (int i = 0; i < kWC; ++i)
+      CopyToLds16S(W + w_off[i] + static_cast<int64_t>(b) * 8 * kRec, l16,
+                   st + (kARecs + i * kWaves + wave) * kRec);
+    CopyToLds4(sa_base + b, st + (kARecs + kWRecs) * kRec + wave * 256);
+  };
+  constexpr int kOps = kAC + kWC + 1;
+
+  floatx4 acc[MI][NJ];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+#pragma unroll
+  for (int p = 0; p < NS - 1; ++p) issue(min(b0 + p, b1 - 1), p);
+  const float *sw = SW + (min(static_cast<int64_t>(tn) * WN + wn, static_cast<int64_t>(groups) - 1) >> 1) * nb;
+  int stage = 0;
+  for (int b = b0; b < b1; ++b) {
+    const float scale = sw[b];
+    WaitBarrier<kOps *(NS - 2)>();
+    issue(min(b + NS - 1, b1 - 1), stage == 0 ? NS - 1 : stage - 1);
+    const uint8_t *st = lds + stage * kStage;
+    const intx4 *la = reinterpret_cast<const intx4 *>(st) + wm * MI * 128 + lane;
+    const intx4 *lw = reinterpret_cast<const intx4 *>(st + kARecs * kRec) + wn * 512 + lane;
+    const float *ls = reinterpret_cast<const float *>(st + (kARecs + kWRecs) * kRec) + wm * MI * 16 + c;
+    const Fragment<EXACT> wf[NJ] = {{lw[0], lw[64]},
+                                    {lw[128], lw[192]},
+                                    {lw[256], lw[320]},
+                                    {lw[384], lw[448]}};
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const Fragment<EXACT> af(la[128 * i], la[128 * i + 64]);
+      const float f = ls[16 * i] * scale;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const floatx4 p = Mfma(wf[j], af);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) acc[i][j][v] = fmaf(p[v], f, acc[i][j][v]);
+      }
+    }
+    stage = stage + 1 == NS ? 0 : stage + 1;
+  }
+  WaitBarrier<0>();  // no copy may land after this workgroup
+
+  const int64_t n = (static_cast<int64_t>(tn) * WN + wn) * 64 + 16 * qd;
+  const bool whole = n + 16 <= N && (N * static_cast<int64_t>(sizeof(T))) % 16 == 0;
+  if (n < N) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int64_t row = 16 * (wm * MI + i) + c;
+      float v[16];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[4 * j + u] = acc[i][j][u];
+      if (row < rows) StoreRow<T, 16>(Y + (m0 + row) * N + n, v, N - n, whole);
+    }
+  }
+}
+
+// Y = the sum of S partial products, in order.
+template <typename T>
+__global__ __launch_bounds__(256) void Fp8SumKernel(const float *__restrict__ P, T *__restrict__ Y,
+                                                    int64_t mn, int S) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < mn; i += step) {
+    float v = P[i];
+    for (int s = 1; s < S; ++s) v += P[s * mn + i];
+    Y[i] = static_cast<T>(v);
+  }
+}
+
+constexpr int64_t kStreamRows = 64;
+
+struct TileShape {
+  int rows, cols;
+  int splits, per_split;
+};
+
+// Large tiles where they fill the chip, else 128 x 128 ones with K split so that
+// every CU has work (at least four blocks each).
+TileShape PickTile(const Weight &w, int64_t M) {
+  TileShape t{256, 256, 1, static_cast<int>(w.nb)};
+  if (CeilDiv(M, 256) * CeilDiv(w.N, 256) >= w.num_cus) return t;
+  t.rows = t.cols = 128;
+  const int64_t tiles = CeilDiv(M, 128) * CeilDiv(w.N, 128);
+  int64_t s = std::max<int64_t>(1, w.num_cus / tiles);
+  s = std::min<int64_t>(s, std::max<int64_t>(1, w.nb / 4));
+  s = std::min<int64_t>(s, 8);
+  t.per_split = static_cast<int>(CeilDiv(w.nb, s));
+  t.splits = static_cast<int>(CeilDiv(w.nb, t.per_split));
+  return t;
+}
+
+template <int MC, typename T>
+hipError_t StreamT(const Weight &w, int M, const uint8_t *A, int64_t lda, const float *sa, void *Y,
+                   hipStream_t s) {
+  constexpr int kWaves = 8, kRG = 1;
+  const size_t lds = static_cast<size_t>(kWaves) * MC * kRG * 1024;
+  hipLaunchKernelGGL((Fp8StreamKernel<MC, kRG, kWaves, sizeof(T) == 4, T>),
+                     dim3(static_cast<unsigned>(w.groups * 4 / kRG)), dim3(64 * kWaves), lds, s, w.W,
+                     w.scales, A, sa, static_cast<T *>(Y), M, w.N, lda, static_cast<int>(w.nb));
+  return hipGetLastError();
+}
+
+template <int MI, int WM, int WN, int NS, bool EXACT, typename T>
+hipError_t TileLaunch(const Weight &w, const TileShape &t, int64_t M, const uint8_t *A, int64_t lda,
+                      const float *sa, T *Y, hipStream_t s) {
+  const int64_t tiles_m = CeilDiv(M, 16 * MI * WM), tiles_n = CeilDiv(w.N, 64 * WN);
+  const size_t lds = static_cast<size_t>(NS) * ((2 * MI * WM + 8 * WN) * kRec + 256 * WM * WN);
+  hipLaunchKernelGGL((Fp8TileKernel<MI, 4, WM, WN, NS, EXACT, T>),
+                     dim3(static_cast<unsigned>(tiles_m * tiles_n), t.splits), dim3(64 * WM * WN),
+                     lds, s, w.W, w.scales, A, sa, Y, M, w.N, lda, static_cast<int>(w.nb),
+                     static_cast<int>(tiles_m), static_cast<int>(tiles_n),
+                     static_cast<int>(w.groups), t.per_split);
+  return hipGetLastError();
+}
+
+template <bool EXACT, typename T>
+hipError_t TileT(const Weight &w, const TileShape &t, int64_t M, const uint8_t *A, int64_t lda,
+                 const float *sa, T *Y, hipStream_t s) {
+  if (t.rows == 256) return TileLaunch<8, 2, 4, 2, EXACT, T>(w, t, M, A, lda, sa, Y, s);
+  return TileLaunch<4, 2, 2, 3, EXACT, T>(w, t, M, A, lda, sa, Y, s);
+}
+
+template <typename T>
+hipError_t ProductT(const Weight &w, int64_t M, const uint8_t *A, int64_t lda, const float *sa,
+                    void *Y, void *work, hipStream_t s) {
+  if (M <= kStreamRows) {
+    const int m = static_cast<int>(M);
+    switch ((M + 15) / 16) {
+    case 1: return StreamT<1, T>(w, m, A, lda, sa, Y, s);
+    case 2: return StreamT<2, T>(w, m, A, lda, sa, Y, s);
+    case 3: return StreamT<3, T>(w, m, A, lda, sa, Y, s);
+    default: return StreamT<4, T>(w, m, A, lda, sa, Y, s);
+    }
+  }
+  const TileShape t = PickTile(w, M);
+  constexpr bool kExact = sizeof(T) == 4;
+  if (t.splits == 1) return TileT<kExact, T>(w, t, M, A, lda, sa, static_cast<T *>(Y), s);
+  float *parts = static_cast<float *>(work);
+  hipError_t e = TileT<kExact, float>(w, t, M, A, lda, sa, parts, s);
+  if (e != hipSuccess) return e;
+  const int64_t mn = M * w.N;
+  hipLaunchKernelGGL((Fp8SumKernel<T>),
+                     dim3(static_cast<unsigned>(std::min<int64_t>(CeilDiv(mn, 256), 1 << 16))),
+                     dim3(256), 0, s, parts, static_cast<T *>(Y), mn, t.splits);
+  return hipGetLastError();
+}
+
+} // namespace
+
+size_t WorkBytes(const Weight &w, int64_t M) {
+  if (M <= kStreamRows) return 0;
+  const TileShape t = PickTile(w, M);
+  return t.splits == 1 ? 0 : static_cast<size_t>(t.splits) * M * w.N * sizeof(float);
+}
+
+const char *ProductKernelName(const Weight &w, int64_t M) {
+  if (M <= kStreamRows) return "Fp8StreamKernel";
+  return "Fp8TileKernel";
+}
+
+hipError_t LaunchProduct(const Weight &w, int64_t M, const uint8_t *A, int64_t lda,
+                         const float *sa, int32_t y_type, void *Y, void *work, hipStream_t s) {
+  switch (y_type) {
+  case MNB_TYPE_FLOAT16: return ProductT<_Float16>(w, M, A, lda, sa, Y, work, s);
+  case MNB_TYPE_BFLOAT16: return ProductT<__bf16>(w, M, A, lda, sa, Y, work, s);
+  default: return ProductT<float>(w, M, A, lda, sa, Y, work, s);
+  }
+}
+
+} // namespace fp8
+} // namespace mnb

@@ -8,6 +8,13 @@
 
 namespace mnb {
 
+// Shared by the C ABI's translation units: records the text of mnb_last_error
+// for this thread; the current device's number if it is a gfx950 (MNB_OK or
+// MNB_ERR_NO_DEVICE); its number of CUs.
+void SetLastHipError(const char *what, hipError_t e);
+int CurrentGfx950(int *device);
+int DeviceComputeUnits(int device);
+
 // Global -> LDS copy of 16 bytes per lane: lane L's 16 bytes at gsrc land at
 // LDS byte lds_base + 16 L (global_load_lds_dwordx4). Issued through inline
 // asm on purpose: the compiler cannot tell which LDS bytes such a copy writes,
