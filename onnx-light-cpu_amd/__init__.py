@@ -646,3 +646,4 @@ class NodeKernel:
 
 
 from .fp8 import MatMulFp8, quantize_fp8  # noqa: E402,F401  (they use the names above)
+from .moe import MatMulNBitsMoE  # noqa: E402,F401

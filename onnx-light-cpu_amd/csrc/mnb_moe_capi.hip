@@ -1,0 +1,249 @@
+// C ABI of the mixture-of-experts layer: validation, plan lifetime.
+#include "mnb_moe.h"
+
+#include <algorithm>
+#include <new>
+
+struct mnb_moe_plan {
+  mnb::moe::Layer layer;
+  int device;
+  void *mem[7];  // gate/up records, scales, zeros; down's; router
+  size_t bytes;
+};
+
+namespace {
+
+using mnb::moe::CeilDiv;
+using mnb::moe::kMaxTokens;
+using mnb::moe::kRec;
+using mnb::moe::kUnit;
+
+bool FloatType(int32_t t) {
+  return t == MNB_TYPE_FLOAT || t == MNB_TYPE_FLOAT16 || t == MNB_TYPE_BFLOAT16;
+}
+
+bool Aligned(const void *p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+int Fail(const char *what, hipError_t e, int status) {
+  mnb::SetLastHipError(what, e);
+  return status;
+}
+
+void FreePlan(mnb_moe_plan *p) {
+  for (void *m : p->mem)
+    if (m) (void)hipFree(m);
+  delete p;
+}
+
+constexpr int64_t kMaxWidth = int64_t{1} << 20;
+constexpr int64_t kMaxMatrix = int64_t{1} << 34;
+constexpr int64_t kMaxRun = int64_t{1} << 24;
+
+int CheckPlanInputs(const mnb_moe_desc *d, const mnb_moe_weight *gate, const mnb_moe_weight *up,
+                    const mnb_moe_weight *down, mnb_moe_plan **out_plan) {
+  if (out_plan == nullptr) return MNB_ERR_NULL_POINTER;
+  *out_plan = nullptr;
+  if (d == nullptr) return MNB_ERR_NULL_POINTER;
+  if (d->bits != 4) return MNB_ERR_UNSUPPORTED;
+  if (d->block_size < 16 || (d->block_size & (d->block_size - 1)) != 0)
+    return MNB_ERR_BAD_ATTRIBUTE;
+  if ((d->normalize != 0 && d->normalize != 1) ||
+      (d->has_zero_points != 0 && d->has_zero_points != 1))
+    return MNB_ERR_BAD_ATTRIBUTE;
+  if (d->hidden <= 0 || d->intermediate <= 0 || d->hidden > kMaxWidth ||
+      d->intermediate > kMaxWidth || d->hidden * d->intermediate > kMaxMatrix || d->experts < 1 ||
+      d->experts > mnb::moe::kMaxExperts)
+    return MNB_ERR_BAD_SHAPE;
+  if (d->top_k < 1 || d->top_k > mnb::moe::kMaxTopK || d->top_k > d->experts)
+    return MNB_ERR_BAD_ATTRIBUTE;
+  for (const mnb_moe_weight *w : {gate, up, down}) {
+    if (w == nullptr || w->B == nullptr || w->scales == nullptr) return MNB_ERR_NULL_POINTER;
+    if (d->has_zero_points && w->zero_points == nullptr) return MNB_ERR_NULL_POINTER;
+    if (!d->has_zero_points && w->zero_points != nullptr) return MNB_ERR_UNSUPPORTED;
+  }
+  return MNB_OK;
+}
+
+int Create(const mnb_moe_desc *d, const float *router, const mnb_moe_weight *gate,
+           const mnb_moe_weight *up, const mnb_moe_weight *down, bool device,
+           mnb_moe_plan **out_plan) {
+  int dev = -1;
+  const int st = mnb::CurrentGfx950(&dev);
+  if (st != MNB_OK) return st;
+  mnb_moe_plan *p = new (std::nothrow) mnb_moe_plan();
+  if (p == nullptr) return MNB_ERR_ALLOC;
+  p->device = dev;
+  mnb::moe::Layer &l = p->layer;
+  l.hidden = d->hidden;
+  l.intermediate = d->intermediate;
+  l.experts = d->experts;
+  l.top_k = d->top_k;
+  l.block_size = d->block_size;
+  l.folds = std::max(1, kUnit / d->block_size);
+  l.normalize = d->normalize != 0;
+  l.zeros = d->has_zero_points != 0;
+  l.num_cus = mnb::DeviceComputeUnits(dev);
+  // The last unit of the experts' rows is whole: the gate/up kernel works by
+  // blocks of 128 channels.
+  l.gate_up.groups = CeilDiv(d->intermediate, kUnit) * (kUnit / 16);
+  l.gate_up.units = CeilDiv(d->hidden, kUnit);
+  l.down.groups = CeilDiv(d->hidden, 16);
+  l.down.units = CeilDiv(d->intermediate, kUnit);
+  const size_t up_recs = static_cast<size_t>(d->experts) * l.gate_up.groups * l.gate_up.units * 2;
+  const size_t down_recs = static_cast<size_t>(d->experts) * l.down.groups * l.down.units;
+  const size_t per_scales = static_cast<size_t>(l.folds) * 16 * sizeof(float);
+  const size_t per_zeros = l.zeros ? static_cast<size_t>(l.folds) * 16 : 0;
+  const size_t sizes[7] = {up_recs * kRec,   up_recs * per_scales,   up_recs * per_zeros,
+                           down_recs * kRec, down_recs * per_scales, down_recs * per_zeros,
+                           router ? static_cast<size_t>(d->experts) * d->hidden * sizeof(float) : 0};
+  hipError_t e = hipSuccess;
+  for (int i = 0; i < 7 && e == hipSuccess; ++i) {
+    p->bytes += sizes[i];
+    if (sizes[i] > 0) e = hipMalloc(&p->mem[i], sizes[i]);
+  }
+  // Host sources pass through a buffer that the largest weight fills.
+  const size_t nb_h = CeilDiv(d->hidden, d->block_size), nb_i = CeilDiv(d->intermediate, d->block_size);
+  const size_t rows_h = static_cast<size_t>(d->experts) * d->hidden,
+               rows_i = static_cast<size_t>(d->experts) * d->intermediate;
+  void *staged[3] = {nullptr, nullptr, nullptr};
+  if (!device && e == hipSuccess) {
+    const size_t blocks = std::max(rows_i * nb_h, rows_h * nb_i);
+    e = hipMalloc(&staged[0], blocks * (d->block_size / 2));
+    if (e == hipSuccess) e = hipMalloc(&staged[1], blocks * sizeof(float));
+    if (e == hipSuccess && l.zeros) e = hipMalloc(&staged[2], blocks);
+  }
+  auto done = [&](const char *what, int status) -> int {
+    for (void *m : staged)
+      if (m) (void)hipFree(m);
+    if (status != MNB_OK) {
+      if (status == MNB_ERR_ALLOC) (void)hipGetLastError();  // the failed allocation's
+      FreePlan(p);
+      return Fail(what, e, status);
+    }
+    *out_plan = p;
+    return MNB_OK;
+  };
+  if (e != hipSuccess) return done("hipMalloc", MNB_ERR_ALLOC);
+  // The copies run on the null stream, which does not wait for non-blocking
+  // streams: every write to the sources must have landed first.
+  if (device) e = hipDeviceSynchronize();
+  struct Part {
+    const mnb_moe_weight *w;
+    int64_t N, K;
+    int r, R, mem;
+  };
+  const Part parts[3] = {{gate, d->intermediate, d->hidden, 0, 2, 0},
+                         {up, d->intermediate, d->hidden, 1, 2, 0},
+                         {down, d->hidden, d->intermediate, 0, 1, 3}};
+  for (const Part &part : parts) {
+    mnb_moe_weight w = *part.w;
+    const size_t rows = static_cast<size_t>(d->experts) * part.N;
+    const size_t nb = CeilDiv(part.K, d->block_size);
+    if (!device && e == hipSuccess) {
+      e = hipMemcpy(staged[0], w.B, rows * nb * (d->block_size / 2), hipMemcpyHostToDevice);
+      if (e == hipSuccess)
+        e = hipMemcpy(staged[1], w.scales, rows * nb * sizeof(float), hipMemcpyHostToDevice);
+      if (e == hipSuccess && l.zeros)
+        e = hipMemcpy(staged[2], w.zero_points, rows * ((nb + 1) / 2), hipMemcpyHostToDevice);
+      w.B = static_cast<const uint8_t *>(staged[0]);
+      w.scales = static_cast<const float *>(staged[1]);
+      w.zero_points = static_cast<const uint8_t *>(staged[2]);
+    }
+    if (e == hipSuccess)
+      e = mnb::moe::LaunchRelayout(w, part.N, part.K, d->block_size, d->experts, part.r, part.R,
+                                   static_cast<uint8_t *>(p->mem[part.mem]),
+                                   static_cast<float *>(p->mem[part.mem + 1]),
+                                   static_cast<int8_t *>(p->mem[part.mem + 2]), nullptr);
+    if (e == hipSuccess) e = hipStreamSynchronize(nullptr);
+  }
+  if (e == hipSuccess && router) {
+    e = hipMemcpy(p->mem[6], router, sizes[6],
+                  device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice);
+    if (e == hipSuccess) e = hipStreamSynchronize(nullptr);
+  }
+  if (e != hipSuccess) return done("expert weight layout", MNB_ERR_HIP);
+  l.gate_up.rec = static_cast<const uint8_t *>(p->mem[0]);
+  l.gate_up.scales = static_cast<const float *>(p->mem[1]);
+  l.gate_up.zeros = static_cast<const int8_t *>(p->mem[2]);
+  l.down.rec = static_cast<const uint8_t *>(p->mem[3]);
+  l.down.scales = static_cast<const float *>(p->mem[4]);
+  l.down.zeros = static_cast<const int8_t *>(p->mem[5]);
+  l.router = static_cast<const float *>(p->mem[6]);
+  return done("", MNB_OK);
+}
+
+} // namespace
+
+extern "C" {
+
+int mnb_moe_plan_create(const mnb_moe_desc *desc, const float *router, const mnb_moe_weight *gate,
+                        const mnb_moe_weight *up, const mnb_moe_weight *down,
+                        mnb_moe_plan **out_plan) {
+  const int st = CheckPlanInputs(desc, gate, up, down, out_plan);
+  return st != MNB_OK ? st : Create(desc, router, gate, up, down, false, out_plan);
+}
+
+int mnb_moe_plan_create_device(const mnb_moe_desc *desc, const float *dRouter,
+                               const mnb_moe_weight *dGate, const mnb_moe_weight *dUp,
+                               const mnb_moe_weight *dDown, mnb_moe_plan **out_plan) {
+  const int st = CheckPlanInputs(desc, dGate, dUp, dDown, out_plan);
+  if (st != MNB_OK) return st;
+  for (const mnb_moe_weight *w : {dGate, dUp, dDown})
+    if (!Aligned(w->B, 4) || !Aligned(w->scales, 4)) return MNB_ERR_BAD_SHAPE;
+  if (!Aligned(dRouter, 4)) return MNB_ERR_BAD_SHAPE;
+  return Create(desc, dRouter, dGate, dUp, dDown, true, out_plan);
+}
+
+int mnb_moe_plan_destroy(mnb_moe_plan *plan) {
+  if (plan != nullptr) FreePlan(plan);
+  return MNB_OK;
+}
+
+int mnb_moe_plan_device_bytes(const mnb_moe_plan *plan, size_t *bytes) {
+  if (plan == nullptr || bytes == nullptr) return MNB_ERR_NULL_POINTER;
+  *bytes = plan->bytes;
+  return MNB_OK;
+}
+
+int mnb_moe_workspace_bytes(const mnb_moe_plan *plan, int64_t T, int32_t x_type, size_t *bytes) {
+  if (plan == nullptr || bytes == nullptr) return MNB_ERR_NULL_POINTER;
+  if (!FloatType(x_type)) return MNB_ERR_BAD_ATTRIBUTE;
+  if (T < 0 || T > kMaxRun) return MNB_ERR_BAD_SHAPE;
+  *bytes = T == 0 ? 0
+                  : mnb::moe::WorkBytes(plan->layer,
+                                        static_cast<int>(std::min<int64_t>(T, kMaxTokens)), x_type);
+  return MNB_OK;
+}
+
+int mnb_moe_run(const mnb_moe_plan *plan, int64_t T, int32_t x_type, const void *dX,
+                const float *dLogits, void *dY, int32_t *dIds, float *dWeights, void *dWorkspace,
+                size_t workspace_bytes, void *stream) {
+  if (plan == nullptr) return MNB_ERR_NULL_POINTER;
+  if (!FloatType(x_type)) return MNB_ERR_BAD_ATTRIBUTE;
+  if (T < 0 || T > kMaxRun) return MNB_ERR_BAD_SHAPE;
+  if (T == 0) return MNB_OK;
+  const mnb::moe::Layer &l = plan->layer;
+  if (dX == nullptr || dY == nullptr || (dLogits == nullptr && l.router == nullptr))
+    return MNB_ERR_NULL_POINTER;
+  const size_t size = x_type == MNB_TYPE_FLOAT ? 4 : 2;
+  if (!Aligned(dX, size) || !Aligned(dY, size) || !Aligned(dLogits, 4) || !Aligned(dIds, 4) ||
+      !Aligned(dWeights, 4) || !Aligned(dWorkspace, 16))
+    return MNB_ERR_BAD_SHAPE;
+  const int most = static_cast<int>(std::min<int64_t>(T, kMaxTokens));
+  if (dWorkspace == nullptr || workspace_bytes < mnb::moe::WorkBytes(l, most, x_type))
+    return MNB_ERR_WORKSPACE;
+  int cur = -1;
+  if (hipGetDevice(&cur) != hipSuccess || cur != plan->device) return MNB_ERR_NO_DEVICE;
+  for (int64_t t = 0; t < T; t += kMaxTokens) {
+    const int n = static_cast<int>(std::min<int64_t>(kMaxTokens, T - t));
+    const hipError_t e = mnb::moe::LaunchLayer(
+        l, n, x_type, static_cast<const char *>(dX) + t * l.hidden * size,
+        dLogits ? dLogits + t * l.experts : nullptr, static_cast<char *>(dY) + t * l.hidden * size,
+        dIds ? dIds + t * l.top_k : nullptr, dWeights ? dWeights + t * l.top_k : nullptr,
+        dWorkspace, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return Fail("expert layer", e, MNB_ERR_HIP);
+  }
+  return MNB_OK;
+}
+
+} // extern "C"
