@@ -36,21 +36,33 @@ constexpr int kTokens = ND == 3 ? 5 : 8;
 
 // ---- fixed point ---------------------------------------------------------------
 
-// Eight values of a unit, k = 8 i .. 8 i + 7 for lane i of 16, into digits: row
-// d at dig + d * stride (the unit's 128 bytes; the eight of lane i lie at
-// 32 (i % 4) + 8 (i / 4), the order in which the weight layout takes them), the
-// unit's power of two at *xs, and per digit and weight block the sum of its
-// digits, times 16, at sd + d * sd_stride (folds words).
+// Rows in fixed point: digits [rows][ND][units * 128] and for each row, digit
+// and unit a column record of `words` words: the powers of two of the unit's
+// `scales` parts, then (zero points) for each of its `folds` parts -64 times the
+// sum of the digits, which the products start from.
+struct Fixed {
+  int8_t *dig;
+  int32_t *col;
+  int64_t units;
+  int scales, folds, words;
+};
+
+constexpr int ColumnWords(int scales, int folds, bool zeros) {
+  return (scales + (zeros ? folds : 0) + 3) / 4 * 4;
+}
+
+// Eight values of a unit of row `row`, k = 8 i .. 8 i + 7, by thread i (% 16) of
+// 16, or of the 16 / scales that share a part. The unit's 128 bytes of a digit
+// lie as the weight layout takes them: the eight of i at 32 (i % 4) + 8 (i / 4).
 template <int ND>
-__device__ __forceinline__ void StoreDigits(const float (&x)[8], int8_t *dig, int64_t stride,
-                                            float *xs, float *sd, int64_t sd_stride, int folds) {
-  const int i = threadIdx.x & 15;
+__device__ __forceinline__ void StoreUnit(const Fixed &f, int64_t row, int64_t unit, int i,
+                                          bool zeros, const float (&x)[8]) {
   // As integers, magnitudes order like their values, infinity above them and NaN on top.
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[j]) & 0x7FFFFFFFu);
-#pragma unroll
-  for (int off = 8; off >= 1; off >>= 1)
+  const int part = 16 / f.scales;
+  for (int off = part >> 1; off >= 1; off >>= 1)
     top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 16)));
   const bool finite = top < 0x7F800000u;
   // 2^e <= amax < 2^(e + 1), at least 2^-90: smaller values count against that.
@@ -62,7 +74,8 @@ __device__ __forceinline__ void StoreDigits(const float (&x)[8], int8_t *dig, in
 #pragma unroll
   for (int j = 0; j < 8; ++j)
     n[j] = finite ? static_cast<int>(rintf(ldexpf(x[j], kBits - e))) : 0;
-  const int lanes = 16 / folds;  // per weight block
+  const int lanes = 16 / f.folds;
+  const float power = finite ? ldexpf(1.0f, e - kBits) : __uint_as_float(0x7FC00000u);
 #pragma unroll
   for (int d = 0; d < ND; ++d) {
     uint32_t lo = 0, hi = 0;
@@ -76,29 +89,16 @@ __device__ __forceinline__ void StoreDigits(const float (&x)[8], int8_t *dig, in
       if (j < 4) lo |= b << (8 * j);
       else hi |= b << (8 * (j - 4));
     }
-    *reinterpret_cast<uint2 *>(dig + d * stride + 32 * (i & 3) + 8 * (i >> 2)) =
+    const int64_t at = (row * ND + d) * f.units + unit;
+    *reinterpret_cast<uint2 *>(f.dig + at * kUnit + 32 * (i & 3) + 8 * (i >> 2)) =
         make_uint2(lo, hi);
-    for (int off = 1; off < lanes; off <<= 1) sum += __shfl_xor(sum, off, 16);
-    if (i % lanes == 0) sd[d * sd_stride + i / lanes] = 16.0f * static_cast<float>(sum);
+    int32_t *col = f.col + at * f.words;
+    if (i % part == 0) col[i / part] = __float_as_int(power);
+    if (zeros) {
+      for (int off = 1; off < lanes; off <<= 1) sum += __shfl_xor(sum, off, 16);
+      if (i % lanes == 0) col[f.scales + i / lanes] = -64 * sum;
+    }
   }
-  // Digit d counts 256^d units of 2^(e - kBits); the 16 of the weights' bytes is here too.
-  if (i == 0) *xs = finite ? ldexpf(1.0f, e - kBits - 4) : __uint_as_float(0x7FC00000u);
-}
-
-// Rows in fixed point: digits [rows][ND][units * 128], powers of two [rows][units],
-// digit sums [rows][ND][units * folds].
-struct Fixed {
-  int8_t *dig;
-  float *xs, *sd;
-  int64_t units;
-};
-
-template <int ND>
-__device__ __forceinline__ void StoreUnit(const Fixed &f, int64_t row, int64_t unit, int folds,
-                                          const float (&x)[8]) {
-  StoreDigits<ND>(x, f.dig + row * ND * f.units * kUnit + unit * kUnit, f.units * kUnit,
-                  f.xs + row * f.units + unit, f.sd + (row * ND * f.units + unit) * folds,
-                  f.units * folds, folds);
 }
 
 // ---- first launch: the tokens in fixed point and the logits ----------------------
@@ -110,7 +110,7 @@ template <int ND, int RT, typename T>
 __global__ __launch_bounds__(256) void MoePrepKernel(const T *__restrict__ X,
                                                      const float *__restrict__ R, float *logits,
                                                      Fixed fx, int tokens, int64_t H, int E,
-                                                     int folds, int router_wgs) {
+                                                     bool zeros, int router_wgs) {
   const int tid = threadIdx.x;
   if (static_cast<int>(blockIdx.x) < router_wgs) {
     const int e = static_cast<int>(blockIdx.x) % E, t0 = static_cast<int>(blockIdx.x) / E * RT;
@@ -147,7 +147,7 @@ __global__ __launch_bounds__(256) void MoePrepKernel(const T *__restrict__ X,
   float x[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) x[j] = k0 + j < H ? static_cast<float>(X[row * H + k0 + j]) : 0.0f;
-  StoreUnit<ND>(fx, row, unit, folds, x);
+  StoreUnit<ND>(fx, row, unit, tid & 15, zeros, x);
 }
 
 // ---- second launch: the choice ------------------------------------------------
@@ -206,129 +206,206 @@ __global__ __launch_bounds__(256) void MoeRouteKernel(const float *__restrict__ 
 
 // ---- the products ---------------------------------------------------------------
 
-// One unit of R records of a row group with GC column groups.
-template <int ND, int R, int GC, int F, bool ZP>
-struct Stream {
-  struct Unit {
-    uint4 w[R];
-    float4 s[R][F];
-    uint32_t z[R][F];
-    intx4 d[GC][2];
-    float xs[GC], sd[GC][F];
-  };
-  // Per lane: the record, scale and zero-point bytes of the first unit; per
-  // column group the digits, powers and sums of this lane's column.
-  const uint8_t *rec;
-  const float *scales;
-  const int8_t *zeros;
-  const int8_t *dig[GC];
-  const float *xs[GC], *sd[GC];
+// A pipe streams units through LDS: SHARE wavefronts, each with two records of
+// its own per unit, and one set of GC column groups for all of them (SHARE = 1: a
+// pipe of one wavefront, without barriers). NS units are in flight by direct
+// global -> LDS copies, so what keeps the memory busy needs no registers.
+// F weight blocks per unit, XB parts of it with powers of two of their own.
+template <int ND, int GC, int F, int XB, bool ZP, int SHARE, int NS>
+struct Pipe {
+  static constexpr int R = kRecords;
+  static constexpr int kT = kTokens<ND>;
+  static constexpr int kFolds = F > XB ? F : XB;
+  static constexpr int kWords = ColumnWords(XB, kFolds, ZP);
+  static constexpr int kMeta = MetaBytes(F, ZP);
+  static constexpr int kMetaCopies = (kMeta + kRec - 1) / kRec;
+  static constexpr int kColLanes = GC * 16 * (kWords / 4);
+  static constexpr int kShared = 2 * GC + (kColLanes + 63) / 64;
+  static constexpr int kSharedPer = (kShared + SHARE - 1) / SHARE;
+  static constexpr int kOps = R + kMetaCopies + kSharedPer;
+  static constexpr int kPrivate = R * kRec + kMeta;
+  static constexpr int kDigits = SHARE * kPrivate;  // offset in a stage
+  static constexpr int kColumns = kDigits + GC * 2 * kRec;
+  static constexpr int kStage = kColumns + kColLanes * 16;
+  static constexpr int kLds = NS * kStage;
+  static_assert(kMeta % 16 == 0 && kOps * (NS - 1) < 64, "copies");
 
-  __device__ __forceinline__ void Rows(const Matrix &m, int64_t matrix, int64_t group, int lane) {
-    const int64_t first = (matrix * m.groups + group) * m.units * R;
-    const int q = lane >> 4;
-    rec = m.rec + first * kRec + lane * 16;
-    scales = m.scales + (first * 4 + q) * F * 4;
-    if constexpr (ZP) zeros = m.zeros + (first * 4 + q) * F * 4;
+  const uint8_t *lds;  // this pipe's
+  uint32_t base;       // its LDS byte
+  int lane, ws;        // lane and wavefront of the pipe
+  // Sources at unit 0 of the current segment.
+  const uint8_t *w_src, *m_src;
+  const uint8_t *s_src[kSharedPer];
+
+  __device__ __forceinline__ Pipe(const uint8_t *at, int lane_, int ws_)
+      : lds(at), base(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(at))), lane(lane_), ws(ws_) {}
+
+  // Which of the shared copies this wavefront makes; past the last it repeats that.
+  __device__ __forceinline__ int SharedCopy(int i) const {
+    return min(i * SHARE + ws, kShared - 1);
   }
-  __device__ __forceinline__ void Column(int g, const Fixed &f, int64_t row, int d, int lane) {
-    dig[g] = f.dig + (row * ND + d) * f.units * kUnit + 32 * (lane >> 4);
-    xs[g] = f.xs + row * f.units;
-    if constexpr (ZP) sd[g] = f.sd + (row * ND + d) * f.units * F;
+  // A segment: row group `group` (of 32 rows) of a matrix, and n tokens (at
+  // most GC * kT) whose fixed-point rows row_of(0 .. n - 1) names.
+  template <typename RowOf>
+  __device__ __forceinline__ void Segment(const Matrix &m, int64_t matrix, int64_t group,
+                                          const Fixed &f, int n, RowOf row_of) {
+    const int64_t first = (matrix * m.groups + group) * m.units;
+    w_src = m.rec + first * (R * kRec);
+    m_src = m.meta + first * kMeta;
+#pragma unroll
+    for (int i = 0; i < kSharedPer; ++i) {
+      const int s = SharedCopy(i);
+      // The column (g, c) whose data this lane copies.
+      int column, part = 0;
+      if (s < 2 * GC) {
+        column = (s >> 1) * 16 + (lane & 15);
+      } else {
+        const int l = min((s - 2 * GC) * 64 + lane, kColLanes - 1);
+        column = l / (kWords / 4);
+        part = l % (kWords / 4);
+      }
+      const int c = column & 15, token = (column >> 4) * kT + c % kT;
+      const int digit = min(c / kT, ND - 1);
+      const int64_t at = (row_of(token < n ? token : 0) * ND + digit) * f.units;
+      s_src[i] = s < 2 * GC
+                     ? reinterpret_cast<const uint8_t *>(f.dig) + at * kUnit + 32 * (lane >> 4) +
+                           16 * (s & 1)
+                     : reinterpret_cast<const uint8_t *>(f.col) + at * (kWords * 4) + part * 16;
+    }
   }
-  __device__ __forceinline__ void Load(int64_t u, Unit &o) const {
+  __device__ __forceinline__ void Issue(int64_t u, int stage) const {
+    const uint32_t st = base + stage * kStage;
+    const uint32_t mine = st + ws * kPrivate;
+    const uint32_t l16 = static_cast<uint32_t>(lane) * 16;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      o.w[r] = *reinterpret_cast<const uint4 *>(rec + (u * R + r) * kRec);
+    for (int r = 0; r < R; ++r) CopyToLds16S(w_src + (u * R + r) * kRec, l16, mine + r * kRec);
 #pragma unroll
-      for (int f = 0; f < F; ++f) {
-        o.s[r][f] = *reinterpret_cast<const float4 *>(scales + ((u * R + r) * 4 * F + f) * 4);
-        if constexpr (ZP)
-          o.z[r][f] = *reinterpret_cast<const uint32_t *>(zeros + ((u * R + r) * 4 * F + f) * 4);
+    for (int i = 0; i < kMetaCopies; ++i)
+      if (i * 64 + lane < kMeta / 16)
+        CopyToLds16S(m_src + u * kMeta + i * kRec, l16, mine + (R + i) * kRec);
+#pragma unroll
+    for (int i = 0; i < kSharedPer; ++i) {
+      const int s = SharedCopy(i);
+      if (s < 2 * GC) {
+        CopyToLds16(s_src[i] + u * kUnit, st + kDigits + s * kRec);
+      } else if ((s - 2 * GC) * 64 + lane < kColLanes) {
+        CopyToLds16(s_src[i] + u * (kWords * 4), st + kColumns + (s - 2 * GC) * kRec);
       }
     }
-#pragma unroll
-    for (int g = 0; g < GC; ++g) {
-      const intx4 *p = reinterpret_cast<const intx4 *>(dig[g] + u * kUnit);
-      o.d[g][0] = p[0];
-      o.d[g][1] = p[1];
-      o.xs[g] = xs[g][u];
-      if constexpr (ZP) {
-#pragma unroll
-        for (int f = 0; f < F; ++f) o.sd[g][f] = sd[g][u * F + f];
-      }
-    }
+  }
+  // Waits until all but the newest N copies of this wavefront are in LDS (for
+  // every wavefront of the pipe).
+  template <int N>
+  static __device__ __forceinline__ void Wait() {
+    __asm__ volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | ((N >> 4) << 14));
+    if constexpr (SHARE > 1) __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    __asm__ volatile("" ::: "memory");
   }
   static __device__ __forceinline__ long Long(int lo, int hi) {
     return static_cast<long>((static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32) |
                              static_cast<uint32_t>(lo));
   }
-  // acc[r][g][v] += row 4 q + v, this lane's column.
-  static __device__ __forceinline__ void Multiply(const Unit &o, floatx4 (&acc)[R][GC], int lane) {
-    const bool low = lane < 32;  // lane groups of the first 16 values of each 32
+  // acc[r][g][v] += row 4 q + v of record r, this lane's column of group g
+  // (groups past `groups` are left out).
+  __device__ __forceinline__ void Multiply(int stage, int groups, floatx4 (&acc)[R][GC]) const {
+    const uint8_t *st = lds + stage * kStage, *mine = st + ws * kPrivate;
+    const int c = lane & 15, q = lane >> 4;
+    const bool low = q < 2;  // lane groups of the first 16 values of each 32
+    int a[R][8];
+    floatx4 scale[R][F];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const uint32_t w[4] = {o.w[r].x, o.w[r].y, o.w[r].z, o.w[r].w};
-      int a[8];
+      const uint4 wv = *reinterpret_cast<const uint4 *>(mine + r * kRec + lane * 16);
+      const uint32_t w[4] = {wv.x, wv.y, wv.z, wv.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        a[2 * i] = static_cast<int>((w[i] << 4) & 0xF0F0F0F0u);
-        a[2 * i + 1] = static_cast<int>(w[i] & 0xF0F0F0F0u);
+      for (int f = 0; f < F; ++f)
+        scale[r][f] = *reinterpret_cast<const floatx4 *>(mine + R * kRec + r * (64 * F) +
+                                                         (q * F + f) * 16);
+      if constexpr (ZP) {
+        // Bytes 64 + nibble - zero point: in 49 .. 79, so no byte borrows.
+        const uint8_t *zp = mine + R * kRec + R * 64 * F + (r * 16 + c) * F;
+        uint32_t z[2];
+        if constexpr (F == 1) z[0] = *zp;
+        else if constexpr (F == 2) z[0] = *reinterpret_cast<const uint16_t *>(zp);
+        else z[0] = *reinterpret_cast<const uint32_t *>(zp);
+        if constexpr (F == 8) z[1] = *reinterpret_cast<const uint32_t *>(zp + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t zz;
+          if constexpr (F == 8) {  // lane groups 0, 1: block 2 i, the others block 2 i + 1
+            const uint32_t pair = z[i >> 1] >> (16 * (i & 1));
+            zz = __builtin_amdgcn_perm(0, low ? pair : pair >> 8, 0u);
+          } else {
+            const int f = F == 4 ? i : F == 2 ? i / 2 : 0;
+            zz = __builtin_amdgcn_perm(0, z[0], 0x01010101u * f);
+          }
+          a[r][2 * i] = static_cast<int>(((w[i] & 0x0F0F0F0Fu) | 0x40404040u) - zz);
+          a[r][2 * i + 1] = static_cast<int>((((w[i] >> 4) & 0x0F0F0F0Fu) | 0x40404040u) - zz);
+        }
+      } else {
+        // Nibbles are two's complement here: 16 of them in the high half of a byte.
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          a[r][2 * i] = static_cast<int>((w[i] << 4) & 0xF0F0F0F0u);
+          a[r][2 * i + 1] = static_cast<int>(w[i] & 0xF0F0F0F0u);
+        }
       }
-      const intx4 a0{a[0], a[1], a[2], a[3]}, a1{a[4], a[5], a[6], a[7]};
+    }
 #pragma unroll
-      for (int g = 0; g < GC; ++g) {
-        const intx4 b0 = o.d[g][0], b1 = o.d[g][1];
+    for (int g = 0; g < GC; ++g) {
+      if (GC > 1 && g >= groups) break;
+      const intx4 b0 = *reinterpret_cast<const intx4 *>(st + kDigits + 2 * g * kRec + lane * 16);
+      const intx4 b1 =
+          *reinterpret_cast<const intx4 *>(st + kDigits + (2 * g + 1) * kRec + lane * 16);
+      int col[kWords];
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4) {
+        const intx4 v =
+            *reinterpret_cast<const intx4 *>(st + kColumns + ((g * 16 + c) * kWords + i) * 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) col[i + j] = v[j];
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const intx4 a0{a[r][0], a[r][1], a[r][2], a[r][3]}, a1{a[r][4], a[r][5], a[r][6], a[r][7]};
         floatx4 part{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-          intx4 sum{0, 0, 0, 0};
-          if constexpr (F == 1) {
+        for (int f = 0; f < kFolds; ++f) {
+          const int start = ZP ? col[XB + f] : 0;
+          intx4 sum{start, start, start, start};
+          if constexpr (kFolds == 1) {
             sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(a0, b0, sum, 0, 0, 0);
             sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(a1, b1, sum, 0, 0, 0);
-          } else if constexpr (F == 2) {
+          } else if constexpr (kFolds == 2) {
             sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(f == 0 ? a0 : a1, f == 0 ? b0 : b1, sum, 0,
                                                         0, 0);
           } else {
-            const int i = F == 4 ? f : f / 2;
+            const int i = kFolds == 4 ? f : f / 2;
             const intx4 b = i < 2 ? b0 : b1;
             int lo = b[2 * (i & 1)], hi = b[2 * (i & 1) + 1];
-            if constexpr (F == 8) {  // half of the 32 values
-              const bool mine = low == (f % 2 == 0);
-              lo = mine ? lo : 0;
-              hi = mine ? hi : 0;
+            if constexpr (kFolds == 8) {  // half of the 32 values
+              const bool use = low == (f % 2 == 0);
+              lo = use ? lo : 0;
+              hi = use ? hi : 0;
             }
-            sum = __builtin_amdgcn_mfma_i32_16x16x32_i8(Long(a[2 * i], a[2 * i + 1]), Long(lo, hi),
-                                                        sum, 0, 0, 0);
+            sum = __builtin_amdgcn_mfma_i32_16x16x32_i8(Long(a[r][2 * i], a[r][2 * i + 1]),
+                                                        Long(lo, hi), sum, 0, 0, 0);
           }
-          const float s[4] = {o.s[r][f].x, o.s[r][f].y, o.s[r][f].z, o.s[r][f].w};
+          const floatx4 s = scale[r][f * F / kFolds];
 #pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            float t = static_cast<float>(sum[v]);
-            if constexpr (ZP) {
-              const int z = static_cast<int8_t>(o.z[r][f] >> (8 * v));
-              t = fmaf(-static_cast<float>(z), o.sd[g][f], t);  // exact
+          for (int v = 0; v < 4; ++v) part[v] = fmaf(static_cast<float>(sum[v]), s[v], part[v]);
+          if ((f + 1) % (kFolds / XB) == 0) {  // the end of a part with its own power
+            const float power = __int_as_float(col[f / (kFolds / XB)]);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              acc[r][g][v] = fmaf(part[v], power, acc[r][g][v]);
+              part[v] = 0.0f;
             }
-            part[v] = fmaf(t, s[v], part[v]);
           }
         }
-#pragma unroll
-        for (int v = 0; v < 4; ++v) acc[r][g][v] = fmaf(part[v], o.xs[g], acc[r][g][v]);
-      }
-    }
-  }
-  // Units u0, u0 + step, .. below u1.
-  __device__ __forceinline__ void Run(int64_t u0, int64_t u1, int64_t step,
-                                      floatx4 (&acc)[R][GC], int lane) const {
-    if (u0 >= u1) return;
-    Unit x, y;
-    Load(u0, x);
-    for (int64_t u = u0; u < u1; u += 2 * step) {
-      Load(u + step < u1 ? u + step : u, y);
-      Multiply(x, acc, lane);
-      if (u + step < u1) {
-        Load(u + 2 * step < u1 ? u + 2 * step : u, x);
-        Multiply(y, acc, lane);
       }
     }
   }
@@ -348,52 +425,63 @@ __device__ __forceinline__ float JoinDigits(float v) {
   }
 }
 
-template <int ND>
-__device__ __forceinline__ float DigitWeight(int digit) {
-  return digit == 0 ? 1.0f : digit == 1 ? 256.0f : 65536.0f;
+// What a column's sum counts for: 256^digit, and 1/16 without zero points (the
+// weights' bytes hold 16 times their value there).
+template <int ND, bool ZP>
+__device__ __forceinline__ float ColumnWeight(int lane) {
+  const int c = lane & 15;
+  if (c >= ND * kTokens<ND>) return 0.0f;
+  const int digit = c / kTokens<ND>;
+  const float w = digit == 0 ? 1.0f : digit == 1 ? 256.0f : 65536.0f;
+  return ZP ? w : w * 0.0625f;
 }
 
 // What the choice gives each launch of experts: entry i of min(tokens * top_k,
-// experts) is an expert with the pairs (token * top_k + place) that chose it.
+// experts) is an expert with the pairs (token * top_k + place) that chose it, which
+// lie one after another in `pair`, with their weights.
 struct Entries {
-  int32_t *expert;  // [entries]
-  int32_t *count;   // 0: an expert that another entry has, or nobody chose
-  int32_t *pair;    // [entries][kMaxTokens]
+  int32_t *expert, *count, *offset;  // [entries]; count 0: another entry's, or nobody's
+  int32_t *pair;                     // [pairs], by expert and then in order
+  float *weight;
 };
 
-// The pairs that chose an expert, in order: every thread of the first wavefront.
+// The pairs that chose expert e, in order, and how many chose a lower one: by
+// every thread of one wavefront.
 __device__ __forceinline__ int CollectPairs(const int32_t *pair_expert, int pairs, int e,
-                                            int32_t *out) {
+                                            int32_t *out, int *before) {
   const int lane = threadIdx.x & 63;
-  int n = 0;
+  int n = 0, lower = 0;
   for (int p0 = 0; p0 < pairs; p0 += 64) {
     const int p = p0 + lane;
-    const bool mine = p < pairs && pair_expert[p] == e;
-    const uint64_t mask = __ballot(mine);
-    if (mine) out[n + __popcll(mask & ((uint64_t{1} << lane) - 1))] = p;
+    const int who = p < pairs ? pair_expert[p] : kMaxExperts;
+    const uint64_t mask = __ballot(who == e);
+    if (who == e) out[n + __popcll(mask & ((uint64_t{1} << lane) - 1))] = p;
     n += __popcll(mask);
+    lower += __popcll(__ballot(who < e));
   }
+  *before = lower;
   return n;
 }
 
-// Third launch: workgroup (b, i) the 128 channels of block b of entry i's
-// expert, KS runs of the units for each of 8 wavefronts' 16 channels.
-template <int ND, int GC, int F, bool ZP, int KS>
-__global__ __launch_bounds__(512 * KS) void MoeGateUpKernel(Matrix m, Fixed fx, Fixed fh,
-                                                            const int32_t *__restrict__ pair_expert,
-                                                            Entries entries, int pairs, int top_k,
-                                                            bool by_expert) {
-  constexpr int kT = kTokens<ND>;
+// Third launch: workgroup (b, i) the 16 * WAVES channels of block b of entry i's
+// expert, 16 channels (gate and up) per wavefront.
+template <int ND, int GC, int F, bool ZP, int WAVES, int NS>
+__global__ __launch_bounds__(64 * WAVES) void MoeGateUpKernel(
+    Matrix m, Fixed fx, Fixed fh, const int32_t *__restrict__ pair_expert,
+    const float *__restrict__ pair_weight, Entries entries, int pairs, int top_k, bool by_expert) {
+  using P = Pipe<ND, GC, F, 1, ZP, WAVES, NS>;
+  constexpr int kT = P::kT, kChannels = 16 * WAVES;
+  static_assert(GC * kT * kChannels * 4 <= P::kLds, "the activations reuse the pipe's LDS");
+  extern __shared__ uint4 dynamic[];
   __shared__ int32_t list[kMaxTokens];
   __shared__ int32_t shared_n;
-  __shared__ float part[KS > 1 ? (KS - 1) * 8 : 1][2 * GC][64][4];
-  __shared__ float hidden[GC * kT][kUnit];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int entry = blockIdx.y;
   const int e = by_expert ? entry : pair_expert[entry];
   if (wave == 0) {
-    int n = CollectPairs(pair_expert, pairs, e, list);
+    int before;
+    int n = CollectPairs(pair_expert, pairs, e, list, &before);
     // Of the pairs that share an expert the first one works.
     if (!by_expert && list[0] != entry) n = 0;
     if (lane == 0) shared_n = n;
@@ -401,168 +489,260 @@ __global__ __launch_bounds__(512 * KS) void MoeGateUpKernel(Matrix m, Fixed fx, 
       if (lane == 0) {
         entries.expert[entry] = e;
         entries.count[entry] = n;
+        entries.offset[entry] = before;
       }
-      if (lane < n) entries.pair[entry * kMaxTokens + lane] = list[lane];
+      if (lane < n) {
+        entries.pair[before + lane] = list[lane];
+        entries.weight[before + lane] = pair_weight[list[lane]];
+      }
     }
   }
   __syncthreads();
-  const int n = shared_n;
+  const int n = __builtin_amdgcn_readfirstlane(shared_n);
   if (n == 0) return;
-  const int cg = wave & 7, ks = wave >> 3;
   const int c = lane & 15, q = lane >> 4;
-  const int digit = min(c / kT, ND - 1), slot = c % kT;
-  const float weight = c < ND * kT ? DigitWeight<ND>(digit) : 0.0f;
-  Stream<ND, 2, GC, F, ZP> stream;
-  stream.Rows(m, e, static_cast<int64_t>(blockIdx.x) * 8 + cg, lane);
-  const int64_t run = CeilDiv(m.units, KS);
+  const float weight = ColumnWeight<ND, ZP>(lane);
+  P pipe(reinterpret_cast<const uint8_t *>(dynamic), lane, wave);
+  float *hidden = reinterpret_cast<float *>(dynamic);  // [GC * kT][kChannels]
+  const int units = static_cast<int>(m.units);
   for (int t0 = 0; t0 < n; t0 += GC * kT) {
-#pragma unroll
-    for (int g = 0; g < GC; ++g) {
-      const int i = t0 + g * kT + slot;
-      stream.Column(g, fx, list[i < n ? i : 0] / top_k, digit, lane);
-    }
+    const int left = min(n - t0, GC * kT), groups = (left + kT - 1) / kT;
+    pipe.Segment(m, e, static_cast<int64_t>(blockIdx.x) * WAVES + wave, fx, left,
+                 [&](int i) { return static_cast<int64_t>(list[t0 + i] / top_k); });
     floatx4 acc[2][GC];
 #pragma unroll
     for (int r = 0; r < 2; ++r)
 #pragma unroll
       for (int g = 0; g < GC; ++g) acc[r][g] = floatx4{0.f, 0.f, 0.f, 0.f};
-    stream.Run(ks * run, min(m.units, (ks + 1) * run), 1, acc, lane);
-    if constexpr (KS > 1) {
-      if (ks > 0) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int g = 0; g < GC; ++g)
-            *reinterpret_cast<floatx4 *>(part[(ks - 1) * 8 + cg][r * GC + g][lane]) = acc[r][g];
-      }
-      __syncthreads();
+    for (int p = 0; p < NS - 1; ++p) pipe.Issue(min(p, units - 1), p);
+    int stage = 0;
+    for (int u = 0; u < units; ++u) {
+      P::template Wait<P::kOps *(NS - 2)>();
+      pipe.Issue(min(u + NS - 1, units - 1), stage == 0 ? NS - 1 : stage - 1);
+      pipe.Multiply(stage, groups, acc);
+      stage = stage + 1 == NS ? 0 : stage + 1;
     }
-    if (ks == 0) {
+    P::template Wait<0>();
 #pragma unroll
-      for (int g = 0; g < GC; ++g) {
-        float4 h;
-        float *hv = &h.x;
+    for (int g = 0; g < GC; ++g) {
+      floatx4 h;
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
-          for (int s = 1; s < KS; ++s)
-            acc[r][g] += *reinterpret_cast<const floatx4 *>(part[(s - 1) * 8 + cg][r * GC + g][lane]);
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const float gate = JoinDigits<ND>(acc[0][g][v] * weight);
-          const float up = JoinDigits<ND>(acc[1][g][v] * weight);
-          hv[v] = SiluMul(gate, up);
-        }
-        if (c < kT) *reinterpret_cast<float4 *>(&hidden[g * kT + c][16 * cg + 4 * q]) = h;
-      }
+      for (int v = 0; v < 4; ++v)
+        h[v] = SiluMul(JoinDigits<ND>(acc[0][g][v] * weight), JoinDigits<ND>(acc[1][g][v] * weight));
+      if (c < kT)
+        *reinterpret_cast<floatx4 *>(hidden + (g * kT + c) * kChannels + 16 * wave + 4 * q) = h;
     }
     __syncthreads();
-    for (int i = tid / 16; i < GC * kT; i += 32 * KS) {
-      if (t0 + i < n) {
-        float x[8];
+    constexpr int kPer = kChannels / 8;  // threads of a token
+    for (int i = tid / kPer; i < GC * kT; i += 64 * WAVES / kPer) {
+      if (i >= left) continue;
+      const int k = tid % kPer;
+      float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = hidden[i][8 * (tid & 15) + j];
-        StoreUnit<ND>(fh, list[t0 + i], blockIdx.x, F, x);
-      }
+      for (int j = 0; j < 8; ++j) x[j] = hidden[i * kChannels + 8 * k + j];
+      const int64_t k0 = static_cast<int64_t>(blockIdx.x) * (kChannels / 8) + k;  // eights of the row
+      StoreUnit<ND>(fh, list[t0 + i], k0 >> 4, static_cast<int>(k0 & 15), ZP, x);
     }
     __syncthreads();
   }
 }
 
-// Fourth launch: a workgroup takes 16 columns of Y and all experts. Its wavefronts
-// share the list of (entry, unit) items in equal runs and keep sums of their own,
-// which join in order.
-constexpr int kDownWaves = 8;
+// A segment's place in the list of pairs and its tokens (12 and 8 bits, the
+// expert above).
+__device__ __forceinline__ int Offset(uint32_t segment) { return segment & 0xFFFu; }
+__device__ __forceinline__ int Count(uint32_t segment) { return (segment >> 12) & 0xFFu; }
 
-template <int ND, int GC, int F, bool ZP, typename T>
-__global__ __launch_bounds__(64 * kDownWaves) void MoeDownKernel(
-    Matrix m, Fixed fh, Entries entries, const float *__restrict__ pair_weight, T *__restrict__ Y,
-    int n_entries, int tokens, int top_k, int64_t H) {
-  constexpr int kT = kTokens<ND>;
-  extern __shared__ float sums[];  // [kDownWaves][tokens][16]
-  __shared__ int32_t active[kMaxExperts];
+// Fourth launch: Y, or partial sums of it. The list of (expert, up to GC * kT of
+// its tokens) segments of the layer, each `units` items long, is cut into equal
+// runs of items; a pipe goes through one run and adds each segment's rows, times
+// the tokens' weights, to sums in LDS.
+//   SHARE = 8: a workgroup takes 8 * R * 16 columns of Y and run blockIdx.y of
+//              gridDim.y; partial sums to parts [runs][tokens][H] if there are several.
+//   SHARE = 1: R * 16 columns; each of 8 wavefronts a run of its own, which join
+//              in order.
+template <int ND, int GC, int F, int XB, bool ZP, int SHARE, int NS, typename T>
+__global__ __launch_bounds__(512) void MoeDownKernel(Matrix m, Fixed fh, Entries entries,
+                                                     T *__restrict__ Y, float *__restrict__ parts,
+                                                     int n_entries, int pairs, int most_segments,
+                                                     int tokens, int top_k, int64_t H) {
+  constexpr int R = kRecords;
+  using P = Pipe<ND, GC, F, XB, ZP, SHARE, NS>;
+  constexpr int kT = P::kT, kPipes = 8 / SHARE;
+  // The pipes' LDS, then sums [8][tokens][32], the pairs' weights, the segments
+  // (offset in the list of pairs, n, expert) and that list.
+  extern __shared__ uint4 dynamic[];
   __shared__ int32_t shared_n;
+  uint8_t *lds = reinterpret_cast<uint8_t *>(dynamic);
+  float *sums = reinterpret_cast<float *>(lds + kPipes * P::kLds);
+  float *weights = sums + 8 * tokens * R * 16;
+  uint32_t *segments = reinterpret_cast<uint32_t *>(weights + pairs);
+  uint16_t *list = reinterpret_cast<uint16_t *>(segments + most_segments);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  for (int i = tid; i < pairs; i += 512) {
+    list[i] = static_cast<uint16_t>(entries.pair[i]);
+    weights[i] = entries.weight[i];
+  }
   if (wave == 0) {
-    int n = 0;
+    int total = 0;
     for (int i0 = 0; i0 < n_entries; i0 += 64) {
       const int i = i0 + lane;
-      const bool on = i < n_entries && entries.count[i] > 0;
-      const uint64_t mask = __ballot(on);
-      if (on) active[n + __popcll(mask & ((uint64_t{1} << lane) - 1))] = i;
-      n += __popcll(mask);
-    }
-    if (lane == 0) shared_n = n;
-  }
-  float *mine = sums + static_cast<int64_t>(wave) * tokens * 16;
-  for (int i = lane; i < tokens * 16; i += 64) mine[i] = 0.0f;
-  __syncthreads();
-  const int64_t items = shared_n * m.units;
-  const int64_t i0 = items * wave / kDownWaves, i1 = items * (wave + 1) / kDownWaves;
-  const int c = lane & 15, q = lane >> 4;
-  const int digit = min(c / kT, ND - 1), slot = c % kT;
-  const float weight = c < ND * kT ? DigitWeight<ND>(digit) : 0.0f;
-  for (int64_t i = i0; i < i1;) {
-    const int entry = active[i / m.units];
-    const int64_t u0 = i % m.units, u1 = min(m.units, u0 + (i1 - i));
-    const int32_t *list = entries.pair + entry * kMaxTokens;
-    const int n = entries.count[entry];
-    Stream<ND, 1, GC, F, ZP> stream;
-    stream.Rows(m, entries.expert[entry], blockIdx.x, lane);
-    for (int t0 = 0; t0 < n; t0 += GC * kT) {
-      int pair[GC];
+      const int n = i < n_entries ? entries.count[i] : 0;
+      const int cut = (n + GC * kT - 1) / (GC * kT);
+      int end = cut;  // inclusive sum over the lanes
 #pragma unroll
-      for (int g = 0; g < GC; ++g) {
-        const int j = t0 + g * kT + slot;
-        pair[g] = list[j < n ? j : 0];
-        stream.Column(g, fh, pair[g], digit, lane);
+      for (int off = 1; off < 64; off <<= 1) {
+        const int v = __shfl_up(end, off, 64);
+        if (lane >= off) end += v;
       }
-      floatx4 acc[1][GC];
+      if (n > 0) {
+        const int expert = entries.expert[i], offset = entries.offset[i];
+        for (int j = 0; j < cut; ++j)
+          segments[total + end - cut + j] =
+              (offset + j * GC * kT) | min(n - j * GC * kT, GC * kT) << 12 | expert << 20;
+      }
+      total += __shfl(end, 63, 64);
+    }
+    if (lane == 0) shared_n = total;
+  }
+  float *mine = sums + wave * tokens * (R * 16);
+  for (int i = lane; i < tokens * R * 16; i += 64) mine[i] = 0.0f;
+  __syncthreads();
+  const int units = static_cast<int>(m.units);
+  const int64_t items = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(shared_n)) * units;
+  const int64_t run = SHARE == 1 ? wave : blockIdx.y, runs = SHARE == 1 ? 8 : gridDim.y;
+  const int64_t i0 = items * run / runs, i1 = items * (run + 1) / runs;
+  const int c = lane & 15, q = lane >> 4;
+  const float weight = ColumnWeight<ND, ZP>(lane);
+  const int64_t group = min(SHARE == 1 ? static_cast<int64_t>(blockIdx.x)
+                                       : static_cast<int64_t>(blockIdx.x) * 8 + wave,
+                            m.groups - 1);
+  if (i0 < i1) {
+    P pipe(lds + (SHARE == 1 ? wave * P::kLds : 0), lane, SHARE == 1 ? 0 : wave);
+    // The next item to copy.
+    int next_seg = static_cast<int>(i0 / units), next_u = static_cast<int>(i0 % units);
+    const int last_seg = static_cast<int>((i1 - 1) / units);
+    const int last_u = static_cast<int>((i1 - 1) % units);
+    auto enter = [&](int seg) __attribute__((always_inline)) {
+      const uint32_t s = __builtin_amdgcn_readfirstlane(segments[seg]);
+      pipe.Segment(m, s >> 20, group, fh, Count(s),
+                   [&](int i) { return static_cast<int64_t>(list[Offset(s) + i]); });
+    };
+    auto issue = [&](int stage) __attribute__((always_inline)) {
+      pipe.Issue(next_u, stage);
+      if (next_seg == last_seg && next_u == last_u) return;  // past the end: the last again
+      if (++next_u == units) {
+        next_u = 0;
+        enter(++next_seg);
+      }
+    };
+    enter(next_seg);
+    int seg = next_seg, u = next_u;  // the item to multiply
 #pragma unroll
-      for (int g = 0; g < GC; ++g) acc[0][g] = floatx4{0.f, 0.f, 0.f, 0.f};
-      stream.Run(u0, u1, 1, acc, lane);
+    for (int p = 0; p < NS - 1; ++p) issue(p);
+    int stage = 0;
+    floatx4 acc[R][GC];
 #pragma unroll
-      for (int g = 0; g < GC; ++g) {
-        float y[4];
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) y[v] = JoinDigits<ND>(acc[0][g][v] * weight);
-        if (c < kT && t0 + g * kT + c < n) {
-          const float p = pair_weight[pair[g]];
-          float4 *at = reinterpret_cast<float4 *>(mine + (pair[g] / top_k) * 16 + 4 * q);
-          float4 s = *at;
-          s.x = fmaf(p, y[0], s.x);
-          s.y = fmaf(p, y[1], s.y);
-          s.z = fmaf(p, y[2], s.z);
-          s.w = fmaf(p, y[3], s.w);
-          *at = s;
+      for (int g = 0; g < GC; ++g) acc[r][g] = floatx4{0.f, 0.f, 0.f, 0.f};
+    uint32_t now = __builtin_amdgcn_readfirstlane(segments[seg]);
+    for (int64_t i = i0; i < i1; ++i) {
+      P::template Wait<P::kOps *(NS - 2)>();
+      issue(stage == 0 ? NS - 1 : stage - 1);
+      const int n = Count(now);
+      pipe.Multiply(stage, (n + kT - 1) / kT, acc);
+      stage = stage + 1 == NS ? 0 : stage + 1;
+      if (++u == units || i + 1 == i1) {
+        const int offset = Offset(now);
+#pragma unroll
+        for (int g = 0; g < GC; ++g) {
+          floatx4 y[R];
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              y[r][v] = JoinDigits<ND>(acc[r][g][v] * weight);
+              acc[r][g][v] = 0.0f;
+            }
+          const int j = g * kT + c;
+          if (c < kT && j < n) {
+            const float p = weights[offset + j];
+            float *to = mine + (list[offset + j] / top_k) * (R * 16) + 4 * q;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+              floatx4 s = *reinterpret_cast<floatx4 *>(to + 16 * r);
+#pragma unroll
+              for (int v = 0; v < 4; ++v) s[v] = fmaf(p, y[r][v], s[v]);
+              *reinterpret_cast<floatx4 *>(to + 16 * r) = s;
+            }
+          }
+        }
+        if (u == units && i + 1 < i1) {
+          u = 0;
+          ++seg;
+          now = __builtin_amdgcn_readfirstlane(segments[seg]);
         }
       }
     }
-    i += u1 - u0;
+    // No copy may land after the workgroup (every wavefront of a pipe is here).
+    P::template Wait<0>();
   }
   __syncthreads();
-  for (int i = tid; i < tokens * 16; i += 64 * kDownWaves) {
-    const int64_t n = static_cast<int64_t>(blockIdx.x) * 16 + (i & 15);
-    if (n >= H) continue;
-    float y = sums[i];
-    for (int w = 1; w < kDownWaves; ++w) y += sums[w * tokens * 16 + i];
-    Y[(i >> 4) * H + n] = static_cast<T>(y);
+  constexpr int kCols = R * 16;
+  if constexpr (SHARE == 1) {
+    for (int i = tid; i < tokens * kCols; i += 512) {
+      const int64_t n = static_cast<int64_t>(blockIdx.x) * kCols + i % kCols;
+      if (n >= H) continue;
+      float y = sums[i];
+      for (int w = 1; w < 8; ++w) y += sums[w * tokens * kCols + i];
+      Y[(i / kCols) * H + n] = static_cast<T>(y);
+    }
+  } else {
+    for (int i = tid; i < tokens * 8 * kCols; i += 512) {
+      const int t = i / (8 * kCols), w = i / kCols % 8;
+      const int64_t n = static_cast<int64_t>(blockIdx.x) * 8 * kCols + i % (8 * kCols);
+      if (n >= H) continue;
+      const float y = sums[(w * tokens + t) * kCols + i % kCols];
+      if (runs == 1) Y[t * H + n] = static_cast<T>(y);
+      else parts[(run * tokens + t) * H + n] = y;
+    }
   }
+}
+
+// Y = the runs' sums, in order.
+template <typename T>
+__global__ __launch_bounds__(256) void MoeSumKernel(const float *__restrict__ parts,
+                                                    T *__restrict__ Y, int64_t n, int runs) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= n) return;
+  float y = parts[i];
+  for (int r = 1; r < runs; ++r) y += parts[r * n + i];
+  Y[i] = static_cast<T>(y);
 }
 
 // ---- weight layout -----------------------------------------------------------------
+
+// The record of 16-row group `group` (of `groups` in a matrix) and unit u.
+__device__ __forceinline__ int64_t RecordOf(Half half, int64_t matrix, int64_t group, int64_t u,
+                                            int64_t groups, int64_t units) {
+  if (half == Half::kPair)
+    return ((matrix * groups + (group & ~int64_t{1})) / 2 * units + u) * 2 + (group & 1);
+  return ((matrix * groups + group) * units + u) * 2 + static_cast<int>(half);
+}
 
 // One thread per 16 bytes of a record.
 __global__ __launch_bounds__(256) void MoeRecordKernel(const uint8_t *__restrict__ B,
                                                        uint8_t *__restrict__ rec, int64_t N,
                                                        int64_t K, int64_t row_bytes, int64_t groups,
-                                                       int64_t units, int r, int R, int64_t total) {
+                                                       int64_t units, Half half, uint32_t flip,
+                                                       int64_t total) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= total) return;
   const int lane = static_cast<int>(i & 63);
-  const int64_t unit_id = i >> 6;  // (matrix, group, unit)
-  const int64_t u = unit_id % units, mg = unit_id / units, matrix = mg / groups,
-                group = mg - matrix * groups;
+  const int64_t id = i >> 6;  // (matrix, group of 16 rows, unit)
+  const int64_t u = id % units, mg = id / units, matrix = mg / groups, group = mg - matrix * groups;
   const int64_t n = group * 16 + (lane & 15);
   uint32_t out[4] = {0, 0, 0, 0};
   if (n < N) {
@@ -571,56 +751,79 @@ __global__ __launch_bounds__(256) void MoeRecordKernel(const uint8_t *__restrict
     for (int w = 0; w < 4; ++w) {
       const int64_t k = u * kUnit + 32 * w + 8 * (lane >> 4);
       if (k >= K) continue;
-      uint32_t v = *reinterpret_cast<const uint32_t *>(row + k / 2) ^ 0x88888888u;
-      if (k + 8 > K) v &= (1u << (4 * (K - k))) - 1u;
+      // Values past K are multiplied by zero digits.
+      const uint32_t v = *reinterpret_cast<const uint32_t *>(row + k / 2) ^ flip;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         out[w] |= ((v >> (4 * j)) & 15u) << (8 * j) | ((v >> (4 * j + 16)) & 15u) << (8 * j + 4);
     }
   }
-  reinterpret_cast<uint4 *>(rec)[(unit_id * R + r) * 64 + lane] =
+  reinterpret_cast<uint4 *>(rec)[RecordOf(half, matrix, group, u, groups, units) * 64 + lane] =
       make_uint4(out[0], out[1], out[2], out[3]);
 }
 
-// One thread per scale: [4 q][folds][4] of a record.
+// One thread per scale (and zero point) of a record.
 __global__ __launch_bounds__(256) void MoeScaleKernel(const float *__restrict__ S,
                                                       const uint8_t *__restrict__ Z,
-                                                      float *__restrict__ scales,
-                                                      int8_t *__restrict__ zeros, int64_t N,
+                                                      uint8_t *__restrict__ meta, int64_t N,
                                                       int64_t nb, int64_t groups, int64_t units,
-                                                      int folds, int block_size, int r, int R,
+                                                      int folds, int block_size, Half half,
                                                       int64_t total) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= total) return;
   const int per = 16 * folds;
-  const int at = static_cast<int>(i % per);
-  const int v = at & 3, f = at / 4 % folds, q = at / (4 * folds);
-  const int64_t unit_id = i / per;
-  const int64_t u = unit_id % units, mg = unit_id / units, matrix = mg / groups,
-                group = mg - matrix * groups;
-  const int64_t n = group * 16 + 4 * q + v;
+  const int row = static_cast<int>(i % per) / folds, f = static_cast<int>(i % per) % folds;
+  const int64_t id = i / per;
+  const int64_t u = id % units, mg = id / units, matrix = mg / groups, group = mg - matrix * groups;
+  const int64_t n = group * 16 + row;
   const int64_t b = block_size >= kUnit ? u * kUnit / block_size : u * folds + f;
   float s = 0.0f;
-  int z = 8;
+  int z = 0;
   if (n < N && b < nb) {
     s = S[(matrix * N + n) * nb + b];
     if (Z) z = (Z[(matrix * N + n) * ((nb + 1) / 2) + b / 2] >> (4 * (b & 1))) & 15;
   }
-  const int64_t o = (unit_id * R + r) * per + at;
-  scales[o] = s;
-  if (Z) zeros[o] = static_cast<int8_t>(z - 8);
+  const int64_t record = RecordOf(half, matrix, group, u, groups, units);
+  constexpr int R = kRecords;
+  const int r = static_cast<int>(record % R);
+  uint8_t *m = meta + record / R * MetaBytes(folds, Z != nullptr);
+  reinterpret_cast<float *>(m)[r * per + ((row >> 2) * folds + f) * 4 + (row & 3)] = s;
+  if (Z) m[R * per * 4 + (r * 16 + row) * folds + f] = static_cast<uint8_t>(z);
 }
 
 // ---- launches ------------------------------------------------------------------------
 
 struct Work {
   Fixed fx, fh;
-  float *logits;
+  float *logits, *pair_weight, *parts;
   int32_t *pair_expert;
-  float *pair_weight;
   Entries entries;
   size_t bytes;
 };
+
+// Up to this many tokens the sums of down's eight wavefronts fit beside their pipes.
+constexpr int kNarrowTokens = 8;
+
+// How the experts' launches are cut.
+struct Shape {
+  int entries;
+  bool narrow;  // gate/up: 32 channels a workgroup, powers of two per 32 channels
+  int runs;     // down: 0: one workgroup for 32 columns; else runs of the items
+};
+
+Shape PickShape(const Layer &l, int tokens) {
+  Shape s;
+  s.entries = std::min(tokens * l.top_k, l.experts);
+  s.narrow = tokens <= kNarrowTokens && s.entries * CeilDiv(l.intermediate, 128) < 2 * l.num_cus;
+  s.runs = 0;
+  if (!s.narrow) {
+    const int64_t blocks = CeilDiv(l.hidden, 256);
+    s.runs = static_cast<int>(std::max<int64_t>(1, CeilDiv(2 * l.num_cus, blocks)));
+    s.runs = static_cast<int>(
+        std::min<int64_t>(s.runs, std::max<int64_t>(1, s.entries * l.down.units / 4)));
+  }
+  return s;
+}
 
 Work Split(const Layer &l, int T, int ND, void *base) {
   Work w;
@@ -631,45 +834,82 @@ Work Split(const Layer &l, int T, int ND, void *base) {
     return p;
   };
   const size_t pairs = static_cast<size_t>(T) * l.top_k;
-  auto fixed = [&](size_t rows, int64_t units) {
+  const Shape shape = PickShape(l, T);
+  auto fixed = [&](size_t rows, int64_t units, int scales) {
     Fixed f;
     f.units = units;
+    f.scales = scales;
+    f.folds = std::max(l.folds, scales);
+    f.words = ColumnWords(scales, f.folds, l.zeros);
     f.dig = reinterpret_cast<int8_t *>(take(rows * ND * units * kUnit));
-    f.xs = reinterpret_cast<float *>(take(rows * units * 4));
-    f.sd = reinterpret_cast<float *>(take(rows * ND * units * l.folds * 4));
+    f.col = reinterpret_cast<int32_t *>(take(rows * ND * units * f.words * 4));
     return f;
   };
-  w.fx = fixed(T, l.gate_up.units);
-  w.fh = fixed(pairs, l.down.units);
+  w.fx = fixed(T, l.gate_up.units, 1);
+  w.fh = fixed(pairs, l.down.units, shape.narrow ? 4 : 1);
   w.logits = reinterpret_cast<float *>(take(static_cast<size_t>(T) * l.experts * 4));
   w.pair_expert = reinterpret_cast<int32_t *>(take(pairs * 4));
   w.pair_weight = reinterpret_cast<float *>(take(pairs * 4));
-  const size_t entries = std::min<size_t>(pairs, l.experts);
-  w.entries.expert = reinterpret_cast<int32_t *>(take(entries * 4));
-  w.entries.count = reinterpret_cast<int32_t *>(take(entries * 4));
-  w.entries.pair = reinterpret_cast<int32_t *>(take(entries * kMaxTokens * 4));
+  w.entries.expert = reinterpret_cast<int32_t *>(take(shape.entries * 4));
+  w.entries.count = reinterpret_cast<int32_t *>(take(shape.entries * 4));
+  w.entries.offset = reinterpret_cast<int32_t *>(take(shape.entries * 4));
+  w.entries.pair = reinterpret_cast<int32_t *>(take(pairs * 4));
+  w.entries.weight = reinterpret_cast<float *>(take(pairs * 4));
+  w.parts = reinterpret_cast<float *>(
+      take(shape.runs > 1 ? static_cast<size_t>(shape.runs) * T * l.hidden * 4 : 0));
   w.bytes = at;
   return w;
 }
 
-template <int ND, int GC, int F, bool ZP, typename T>
-hipError_t LaunchExperts(const Layer &l, const Work &w, int tokens, void *Y, hipStream_t s) {
-  const int pairs = tokens * l.top_k;
-  const int entries = std::min(pairs, l.experts);
-  const dim3 grid(static_cast<unsigned>(l.gate_up.groups / 8), static_cast<unsigned>(entries));
-  hipLaunchKernelGGL((MoeGateUpKernel<ND, GC, F, ZP, 1>), grid, dim3(512), 0, s, l.gate_up, w.fx,
-                     w.fh, w.pair_expert, w.entries, pairs, l.top_k, pairs >= l.experts);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  const size_t lds = static_cast<size_t>(kDownWaves) * tokens * 16 * sizeof(float);
-  hipLaunchKernelGGL((MoeDownKernel<ND, GC, F, ZP, T>), dim3(static_cast<unsigned>(l.down.groups)),
-                     dim3(64 * kDownWaves), lds, s, l.down, w.fh, w.entries, w.pair_weight,
-                     static_cast<T *>(Y), entries, tokens, l.top_k, l.hidden);
+template <int ND, int GC, int F, bool ZP, int WAVES>
+hipError_t LaunchGateUp(const Layer &l, const Work &w, const Shape &shape, int pairs,
+                        hipStream_t s) {
+  constexpr int NS = 3;
+  const dim3 grid(static_cast<unsigned>(l.gate_up.groups / WAVES),
+                  static_cast<unsigned>(shape.entries));
+  hipLaunchKernelGGL((MoeGateUpKernel<ND, GC, F, ZP, WAVES, NS>), grid, dim3(64 * WAVES),
+                     (Pipe<ND, GC, F, 1, ZP, WAVES, NS>::kLds), s, l.gate_up, w.fx, w.fh,
+                     w.pair_expert, w.pair_weight, w.entries, pairs, l.top_k, pairs >= l.experts);
   return hipGetLastError();
 }
 
+template <int ND, int GC, int F, int XB, bool ZP, int SHARE, typename T>
+hipError_t LaunchDown(const Layer &l, const Work &w, const Shape &shape, int tokens, T *Y,
+                      hipStream_t s) {
+  constexpr int NS = SHARE == 1 || F == 8 ? 2 : 3;
+  const int pairs = tokens * l.top_k;
+  const int segments = shape.entries + pairs / (GC * kTokens<ND>);
+  const size_t lds = static_cast<size_t>(8 / SHARE) * Pipe<ND, GC, F, XB, ZP, SHARE, NS>::kLds +
+                     8 * tokens * 32 * sizeof(float) + pairs * 6 + segments * 4;
+  const int64_t blocks = CeilDiv(l.down.groups, SHARE);
+  hipLaunchKernelGGL((MoeDownKernel<ND, GC, F, XB, ZP, SHARE, NS, T>),
+                     dim3(static_cast<unsigned>(blocks), std::max(1, shape.runs)), dim3(512), lds, s,
+                     l.down, w.fh, w.entries, Y, w.parts, shape.entries, pairs, segments, tokens,
+                     l.top_k, l.hidden);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || shape.runs <= 1) return e;
+  const int64_t n = tokens * l.hidden;
+  hipLaunchKernelGGL((MoeSumKernel<T>), dim3(static_cast<unsigned>(CeilDiv(n, 256))), dim3(256), 0,
+                     s, w.parts, Y, n, shape.runs);
+  return hipGetLastError();
+}
+
+template <int ND, int GC, int F, bool ZP, typename T>
+hipError_t LaunchExperts(const Layer &l, const Work &w, int tokens, T *Y, hipStream_t s) {
+  const Shape shape = PickShape(l, tokens);
+  const int pairs = tokens * l.top_k;
+  if constexpr (GC == 1) {
+    if (shape.narrow) {
+      const hipError_t e = LaunchGateUp<ND, GC, F, ZP, 2>(l, w, shape, pairs, s);
+      return e != hipSuccess ? e : LaunchDown<ND, GC, F, 4, ZP, 1, T>(l, w, shape, tokens, Y, s);
+    }
+  }
+  const hipError_t e = LaunchGateUp<ND, GC, F, ZP, 8>(l, w, shape, pairs, s);
+  return e != hipSuccess ? e : LaunchDown<ND, GC, F, 1, ZP, 8, T>(l, w, shape, tokens, Y, s);
+}
+
 template <int ND, int GC, bool ZP, typename T>
-hipError_t LaunchFolds(const Layer &l, const Work &w, int tokens, void *Y, hipStream_t s) {
+hipError_t LaunchFolds(const Layer &l, const Work &w, int tokens, T *Y, hipStream_t s) {
   switch (l.folds) {
   case 1: return LaunchExperts<ND, GC, 1, ZP, T>(l, w, tokens, Y, s);
   case 2: return LaunchExperts<ND, GC, 2, ZP, T>(l, w, tokens, Y, s);
@@ -691,11 +931,11 @@ hipError_t LaunchLayerT(const Layer &l, int tokens, const void *X, const float *
   if (tokens == 1)
     hipLaunchKernelGGL((MoePrepKernel<ND, 1, T>), dim3(prep), dim3(256), 0, s,
                        static_cast<const T *>(X), l.router, w.logits, w.fx, tokens, l.hidden,
-                       l.experts, l.folds, router_wgs);
+                       l.experts, l.zeros, router_wgs);
   else
     hipLaunchKernelGGL((MoePrepKernel<ND, kRT, T>), dim3(prep), dim3(256), 0, s,
                        static_cast<const T *>(X), l.router, w.logits, w.fx, tokens, l.hidden,
-                       l.experts, l.folds, router_wgs);
+                       l.experts, l.zeros, router_wgs);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(MoeRouteKernel, dim3(static_cast<unsigned>(tokens)), dim3(256), 0, s,
@@ -703,25 +943,28 @@ hipError_t LaunchLayerT(const Layer &l, int tokens, const void *X, const float *
                      l.experts, l.top_k, l.normalize);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
+  T *y = static_cast<T *>(Y);
   // Column groups per pass over an expert's rows: what its share of the tokens fills.
-  const bool many = static_cast<int64_t>(tokens) * l.top_k > static_cast<int64_t>(l.experts) * kTokens<ND> / 2;
+  const bool many =
+      tokens > kNarrowTokens &&
+      static_cast<int64_t>(tokens) * l.top_k > static_cast<int64_t>(l.experts) * kTokens<ND> / 2;
   if (l.zeros)
-    return many ? LaunchFolds<ND, 2, true, T>(l, w, tokens, Y, s)
-                : LaunchFolds<ND, 1, true, T>(l, w, tokens, Y, s);
-  return many ? LaunchFolds<ND, 2, false, T>(l, w, tokens, Y, s)
-              : LaunchFolds<ND, 1, false, T>(l, w, tokens, Y, s);
+    return many ? LaunchFolds<ND, 2, true, T>(l, w, tokens, y, s)
+                : LaunchFolds<ND, 1, true, T>(l, w, tokens, y, s);
+  return many ? LaunchFolds<ND, 2, false, T>(l, w, tokens, y, s)
+              : LaunchFolds<ND, 1, false, T>(l, w, tokens, y, s);
 }
 
 } // namespace
 
 hipError_t LaunchRelayout(const mnb_moe_weight &src, int64_t N, int64_t K, int block_size,
-                          int experts, int r, int R, uint8_t *rec, float *scales, int8_t *zeros,
+                          int experts, Half half, const Matrix &m, uint8_t *rec, uint8_t *meta,
                           hipStream_t s) {
-  const int64_t units = CeilDiv(K, kUnit);
-  const int64_t groups = R == 2 ? CeilDiv(N, kUnit) * (kUnit / 16) : CeilDiv(N, 16);
+  const int64_t groups = half == Half::kPair ? 2 * m.groups : m.groups, units = m.units;
   const int64_t nb = CeilDiv(K, block_size);
   const int64_t row_bytes = nb * (block_size / 2);
   const int folds = std::max(1, kUnit / block_size);
+  const bool zeros = src.zero_points != nullptr;
   // Experts at a time, so that a grid's threads stay below 2^32 (one expert's
   // are at most 2^31: hidden * intermediate <= 2^34).
   const int64_t one = groups * units * std::max(64, 16 * folds);
@@ -729,17 +972,17 @@ hipError_t LaunchRelayout(const mnb_moe_weight &src, int64_t N, int64_t K, int b
   for (int64_t e = 0; e < experts; e += per) {
     const int64_t n = std::min<int64_t>(per, experts - e);
     const int64_t total = n * groups * units;
-    const int64_t first = e * groups * units * R;
+    const int64_t first = e * m.groups * units;
     hipLaunchKernelGGL(MoeRecordKernel, dim3(static_cast<unsigned>(CeilDiv(total * 64, 256))),
-                       dim3(256), 0, s, src.B + e * N * row_bytes, rec + first * kRec, N, K,
-                       row_bytes, groups, units, r, R, total * 64);
+                       dim3(256), 0, s, src.B + e * N * row_bytes, rec + first * kRecords * kRec, N,
+                       K, row_bytes, groups, units, half, zeros ? 0u : 0x88888888u, total * 64);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     hipLaunchKernelGGL(MoeScaleKernel, dim3(static_cast<unsigned>(CeilDiv(total * 16 * folds, 256))),
                        dim3(256), 0, s, src.scales + e * N * nb,
-                       src.zero_points ? src.zero_points + e * N * ((nb + 1) / 2) : nullptr,
-                       scales + first * 16 * folds, zeros ? zeros + first * 16 * folds : nullptr, N,
-                       nb, groups, units, folds, block_size, r, R, total * 16 * folds);
+                       zeros ? src.zero_points + e * N * ((nb + 1) / 2) : nullptr,
+                       meta + first * MetaBytes(folds, zeros), N, nb, groups, units, folds,
+                       block_size, half, total * 16 * folds);
     err = hipGetLastError();
     if (err != hipSuccess) return err;
   }

@@ -7,15 +7,17 @@
 struct mnb_moe_plan {
   mnb::moe::Layer layer;
   int device;
-  void *mem[7];  // gate/up records, scales, zeros; down's; router
+  void *mem[5];  // gate/up records and meta; down's; router
   size_t bytes;
 };
 
 namespace {
 
 using mnb::moe::CeilDiv;
+using mnb::moe::Half;
 using mnb::moe::kMaxTokens;
 using mnb::moe::kRec;
+using mnb::moe::kRecords;
 using mnb::moe::kUnit;
 
 bool FloatType(int32_t t) {
@@ -65,7 +67,7 @@ int CheckPlanInputs(const mnb_moe_desc *d, const mnb_moe_weight *gate, const mnb
 }
 
 int Create(const mnb_moe_desc *d, const float *router, const mnb_moe_weight *gate,
-           const mnb_moe_weight *up, const mnb_moe_weight *down, bool device,
+           const mnb_moe_weight *up_w, const mnb_moe_weight *down, bool device,
            mnb_moe_plan **out_plan) {
   int dev = -1;
   const int st = mnb::CurrentGfx950(&dev);
@@ -83,21 +85,19 @@ int Create(const mnb_moe_desc *d, const float *router, const mnb_moe_weight *gat
   l.normalize = d->normalize != 0;
   l.zeros = d->has_zero_points != 0;
   l.num_cus = mnb::DeviceComputeUnits(dev);
-  // The last unit of the experts' rows is whole: the gate/up kernel works by
-  // blocks of 128 channels.
+  // 16 channels of gate and up are a group; the last unit of the experts' rows is
+  // whole (the gate/up kernel works by blocks of 128 channels).
   l.gate_up.groups = CeilDiv(d->intermediate, kUnit) * (kUnit / 16);
   l.gate_up.units = CeilDiv(d->hidden, kUnit);
-  l.down.groups = CeilDiv(d->hidden, 16);
+  l.down.groups = CeilDiv(d->hidden, 32);
   l.down.units = CeilDiv(d->intermediate, kUnit);
-  const size_t up_recs = static_cast<size_t>(d->experts) * l.gate_up.groups * l.gate_up.units * 2;
-  const size_t down_recs = static_cast<size_t>(d->experts) * l.down.groups * l.down.units;
-  const size_t per_scales = static_cast<size_t>(l.folds) * 16 * sizeof(float);
-  const size_t per_zeros = l.zeros ? static_cast<size_t>(l.folds) * 16 : 0;
-  const size_t sizes[7] = {up_recs * kRec,   up_recs * per_scales,   up_recs * per_zeros,
-                           down_recs * kRec, down_recs * per_scales, down_recs * per_zeros,
+  const size_t up = static_cast<size_t>(d->experts) * l.gate_up.groups * l.gate_up.units;
+  const size_t dn = static_cast<size_t>(d->experts) * l.down.groups * l.down.units;
+  const size_t rec = kRecords * kRec, meta = mnb::moe::MetaBytes(l.folds, l.zeros);
+  const size_t sizes[5] = {up * rec, up * meta, dn * rec, dn * meta,
                            router ? static_cast<size_t>(d->experts) * d->hidden * sizeof(float) : 0};
   hipError_t e = hipSuccess;
-  for (int i = 0; i < 7 && e == hipSuccess; ++i) {
+  for (int i = 0; i < 5 && e == hipSuccess; ++i) {
     p->bytes += sizes[i];
     if (sizes[i] > 0) e = hipMalloc(&p->mem[i], sizes[i]);
   }
@@ -130,11 +130,13 @@ int Create(const mnb_moe_desc *d, const float *router, const mnb_moe_weight *gat
   struct Part {
     const mnb_moe_weight *w;
     int64_t N, K;
-    int r, R, mem;
+    Half half;
+    const mnb::moe::Matrix *m;
+    int mem;
   };
-  const Part parts[3] = {{gate, d->intermediate, d->hidden, 0, 2, 0},
-                         {up, d->intermediate, d->hidden, 1, 2, 0},
-                         {down, d->hidden, d->intermediate, 0, 1, 3}};
+  const Part parts[3] = {{gate, d->intermediate, d->hidden, Half::kGate, &l.gate_up, 0},
+                         {up_w, d->intermediate, d->hidden, Half::kUp, &l.gate_up, 0},
+                         {down, d->hidden, d->intermediate, Half::kPair, &l.down, 2}};
   for (const Part &part : parts) {
     mnb_moe_weight w = *part.w;
     const size_t rows = static_cast<size_t>(d->experts) * part.N;
@@ -150,25 +152,22 @@ int Create(const mnb_moe_desc *d, const float *router, const mnb_moe_weight *gat
       w.zero_points = static_cast<const uint8_t *>(staged[2]);
     }
     if (e == hipSuccess)
-      e = mnb::moe::LaunchRelayout(w, part.N, part.K, d->block_size, d->experts, part.r, part.R,
+      e = mnb::moe::LaunchRelayout(w, part.N, part.K, d->block_size, d->experts, part.half, *part.m,
                                    static_cast<uint8_t *>(p->mem[part.mem]),
-                                   static_cast<float *>(p->mem[part.mem + 1]),
-                                   static_cast<int8_t *>(p->mem[part.mem + 2]), nullptr);
+                                   static_cast<uint8_t *>(p->mem[part.mem + 1]), nullptr);
     if (e == hipSuccess) e = hipStreamSynchronize(nullptr);
   }
   if (e == hipSuccess && router) {
-    e = hipMemcpy(p->mem[6], router, sizes[6],
+    e = hipMemcpy(p->mem[4], router, sizes[4],
                   device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice);
     if (e == hipSuccess) e = hipStreamSynchronize(nullptr);
   }
   if (e != hipSuccess) return done("expert weight layout", MNB_ERR_HIP);
   l.gate_up.rec = static_cast<const uint8_t *>(p->mem[0]);
-  l.gate_up.scales = static_cast<const float *>(p->mem[1]);
-  l.gate_up.zeros = static_cast<const int8_t *>(p->mem[2]);
-  l.down.rec = static_cast<const uint8_t *>(p->mem[3]);
-  l.down.scales = static_cast<const float *>(p->mem[4]);
-  l.down.zeros = static_cast<const int8_t *>(p->mem[5]);
-  l.router = static_cast<const float *>(p->mem[6]);
+  l.gate_up.meta = static_cast<const uint8_t *>(p->mem[1]);
+  l.down.rec = static_cast<const uint8_t *>(p->mem[2]);
+  l.down.meta = static_cast<const uint8_t *>(p->mem[3]);
+  l.router = static_cast<const float *>(p->mem[4]);
   return done("", MNB_OK);
 }
 
