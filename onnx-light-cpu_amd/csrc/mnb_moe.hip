@@ -22,6 +22,8 @@
 #include "mnb_moe.h"
 
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 namespace mnb {
 namespace moe {
@@ -105,8 +107,9 @@ __device__ __forceinline__ void StoreUnit(const Fixed &f, int64_t row, int64_t u
 
 // Workgroups 0 .. router_wgs - 1: one expert and up to RT tokens each, sums in
 // 64 bits (the choice is a comparison of sums: it shall not hang on their
-// order). The others: 16 lanes per (token, unit).
-template <int ND, int RT, typename T>
+// order). The others: 16 lanes per (token, unit). VEC: H a multiple of 4, rows of
+// X and R aligned to four values.
+template <int ND, int RT, bool VEC, typename T>
 __global__ __launch_bounds__(256) void MoePrepKernel(const T *__restrict__ X,
                                                      const float *__restrict__ R, float *logits,
                                                      Fixed fx, int tokens, int64_t H, int E,
@@ -122,10 +125,28 @@ __global__ __launch_bounds__(256) void MoePrepKernel(const T *__restrict__ X,
       x[t] = X + static_cast<int64_t>(min(t0 + t, tokens - 1)) * H;
       sum[t] = 0.0;
     }
-    for (int64_t k = tid; k < H; k += 256) {
-      const double w = static_cast<double>(r[k]);
+    const int width = static_cast<int>(H);
+    if constexpr (VEC) {
+      typedef T Four __attribute__((ext_vector_type(4)));
+#pragma unroll 4
+      for (int k = 4 * tid; k < width; k += 1024) {
+        const floatx4 w = *reinterpret_cast<const floatx4 *>(r + k);
 #pragma unroll
-      for (int t = 0; t < RT; ++t) sum[t] = fma(w, static_cast<double>(static_cast<float>(x[t][k])), sum[t]);
+        for (int t = 0; t < RT; ++t) {
+          const Four v = *reinterpret_cast<const Four *>(x[t] + k);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            sum[t] = fma(static_cast<double>(w[j]),
+                         static_cast<double>(static_cast<float>(v[j])), sum[t]);
+        }
+      }
+    } else {
+      for (int k = tid; k < width; k += 256) {
+        const double w = static_cast<double>(r[k]);
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+          sum[t] = fma(w, static_cast<double>(static_cast<float>(x[t][k])), sum[t]);
+      }
     }
     __shared__ double red[RT][4];
 #pragma unroll
@@ -158,45 +179,68 @@ __device__ __forceinline__ uint32_t Key(float l) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// One workgroup per token: an expert's place is the number of experts before
-// it, by key and then by index.
-__global__ __launch_bounds__(256) void MoeRouteKernel(const float *__restrict__ logits,
-                                                      int32_t *pair_expert, float *pair_weight,
-                                                      int32_t *ids, float *weights, int E, int k,
-                                                      bool normalize) {
-  __shared__ uint32_t key[kMaxExperts];
-  __shared__ float best[kMaxTopK];
-  __shared__ int32_t who[kMaxTopK];
-  __shared__ float red[4];
-  const int tid = threadIdx.x, t = blockIdx.x;
-  const float *l = logits + static_cast<int64_t>(t) * E;
-  // -0 and 0 are equal logits.
-  for (int e = tid; e < E; e += 256) key[e] = Key(l[e] + 0.0f);
+// A token's choice, by all THREADS of a workgroup: best[i] and who[i] (i < k) the
+// i-th largest logit and its expert; returns what the weights expf(best[i] -
+// best[0]) are divided by. An expert's place is the number of experts before it, by
+// key and then by index.
+template <int THREADS>
+__device__ __forceinline__ float Choose(const float *__restrict__ l, int E, int k, bool normalize,
+                                        uint32_t *key, float *best, int32_t *who) {
+  __shared__ float red[THREADS / 64];
+  const int tid = threadIdx.x;
+  const int padded = (E + 3) & ~3;
+  // -0 and 0 are equal logits; key 0 is below every logit's.
+  for (int e = tid; e < padded; e += THREADS) key[e] = e < E ? Key(l[e] + 0.0f) : 0u;
   __syncthreads();
-  for (int e = tid; e < E; e += 256) {
+  const uint4 *key4 = reinterpret_cast<const uint4 *>(key);
+  for (int e = tid; e < E; e += THREADS) {
     const uint32_t me = key[e];
     int place = 0;
-    for (int j = 0; j < E; ++j) place += (key[j] > me || (key[j] == me && j < e)) ? 1 : 0;
+#pragma unroll 4
+    for (int j = 0; j < padded / 4; ++j) {
+      const uint4 v = key4[j];
+      // Before e equal keys count too: they exceed me - 1 (keys are above 0).
+      const int at = 4 * j;
+      place += v.x > me - (at < e ? 1u : 0u) ? 1 : 0;
+      place += v.y > me - (at + 1 < e ? 1u : 0u) ? 1 : 0;
+      place += v.z > me - (at + 2 < e ? 1u : 0u) ? 1 : 0;
+      place += v.w > me - (at + 3 < e ? 1u : 0u) ? 1 : 0;
+    }
     if (place < k) {
       best[place] = l[e] != l[e] ? -__builtin_inff() : l[e];
       who[place] = e;
     }
   }
   __syncthreads();
-  float total = 0.0f;
   const float top = best[0];
+  float total = 0.0f;
   if (normalize) {
     for (int j = 0; j < k; ++j) total += expf(best[j] - top);
   } else {
     float s = 0.0f;
-    for (int e = tid; e < E; e += 256) s += expf((l[e] != l[e] ? -__builtin_inff() : l[e]) - top);
+    for (int e = tid; e < E; e += THREADS)
+      s += expf((l[e] != l[e] ? -__builtin_inff() : l[e]) - top);
     for (int off = 32; off >= 1; off >>= 1) s += __shfl_xor(s, off, 64);
     if ((tid & 63) == 0) red[tid >> 6] = s;
     __syncthreads();
-    total = (red[0] + red[1]) + (red[2] + red[3]);
+    for (int w = 0; w < THREADS / 64; ++w) total += red[w];
   }
+  return total;
+}
+
+// One workgroup per token.
+__global__ __launch_bounds__(256) void MoeRouteKernel(const float *__restrict__ logits,
+                                                      int32_t *pair_expert, float *pair_weight,
+                                                      int32_t *ids, float *weights, int E, int k,
+                                                      bool normalize) {
+  __shared__ uint4 key[kMaxExperts / 4];
+  __shared__ float best[kMaxTopK];
+  __shared__ int32_t who[kMaxTopK];
+  const int tid = threadIdx.x, t = blockIdx.x;
+  const float total = Choose<256>(logits + static_cast<int64_t>(t) * E, E, k, normalize,
+                                  reinterpret_cast<uint32_t *>(key), best, who);
   if (tid < k) {
-    const float p = expf(best[tid] - top) / total;
+    const float p = expf(best[tid] - best[0]) / total;
     pair_expert[t * k + tid] = who[tid];
     pair_weight[t * k + tid] = p;
     if (ids) ids[t * k + tid] = who[tid];
@@ -206,14 +250,13 @@ __global__ __launch_bounds__(256) void MoeRouteKernel(const float *__restrict__ 
 
 // ---- the products ---------------------------------------------------------------
 
-// A pipe streams units through LDS: SHARE wavefronts, each with two records of
-// its own per unit, and one set of GC column groups for all of them (SHARE = 1: a
+// A pipe streams units through LDS: SHARE wavefronts, each with R records of its
+// own per unit (both of its row group, or one of them), and one set of GC column groups for all of them (SHARE = 1: a
 // pipe of one wavefront, without barriers). NS units are in flight by direct
 // global -> LDS copies, so what keeps the memory busy needs no registers.
 // F weight blocks per unit, XB parts of it with powers of two of their own.
-template <int ND, int GC, int F, int XB, bool ZP, int SHARE, int NS>
+template <int ND, int GC, int R, int F, int XB, bool ZP, int SHARE, int NS>
 struct Pipe {
-  static constexpr int R = kRecords;
   static constexpr int kT = kTokens<ND>;
   static constexpr int kFolds = F > XB ? F : XB;
   static constexpr int kWords = ColumnWords(XB, kFolds, ZP);
@@ -233,12 +276,15 @@ struct Pipe {
   const uint8_t *lds;  // this pipe's
   uint32_t base;       // its LDS byte
   int lane, ws;        // lane and wavefront of the pipe
+  int half;            // R = 1: which record
   // Sources at unit 0 of the current segment.
   const uint8_t *w_src, *m_src;
   const uint8_t *s_src[kSharedPer];
+  bool s_on[kSharedPer];  // this lane's column has a token
 
-  __device__ __forceinline__ Pipe(const uint8_t *at, int lane_, int ws_)
-      : lds(at), base(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(at))), lane(lane_), ws(ws_) {}
+  __device__ __forceinline__ Pipe(const uint8_t *at, int lane_, int ws_, int half_ = 0)
+      : lds(at), base(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(at))), lane(lane_), ws(ws_),
+        half(half_) {}
 
   // Which of the shared copies this wavefront makes; past the last it repeats that.
   __device__ __forceinline__ int SharedCopy(int i) const {
@@ -250,7 +296,7 @@ struct Pipe {
   __device__ __forceinline__ void Segment(const Matrix &m, int64_t matrix, int64_t group,
                                           const Fixed &f, int n, RowOf row_of) {
     const int64_t first = (matrix * m.groups + group) * m.units;
-    w_src = m.rec + first * (R * kRec);
+    w_src = m.rec + (first * kRecords + half) * kRec;
     m_src = m.meta + first * kMeta;
 #pragma unroll
     for (int i = 0; i < kSharedPer; ++i) {
@@ -260,12 +306,16 @@ struct Pipe {
       if (s < 2 * GC) {
         column = (s >> 1) * 16 + (lane & 15);
       } else {
-        const int l = min((s - 2 * GC) * 64 + lane, kColLanes - 1);
-        column = l / (kWords / 4);
+        const int l = (s - 2 * GC) * 64 + lane;
+        column = min(l, kColLanes - 1) / (kWords / 4);
         part = l % (kWords / 4);
       }
       const int c = column & 15, token = (column >> 4) * kT + c % kT;
       const int digit = min(c / kT, ND - 1);
+      // Columns without a token keep what LDS holds: nothing reads their sums. One
+      // lane is always on, so that every copy is issued and counted.
+      s_on[i] = (token < n && c < ND * kT && (s < 2 * GC || (s - 2 * GC) * 64 + lane < kColLanes)) ||
+                lane == 0;
       const int64_t at = (row_of(token < n ? token : 0) * ND + digit) * f.units;
       s_src[i] = s < 2 * GC
                      ? reinterpret_cast<const uint8_t *>(f.dig) + at * kUnit + 32 * (lane >> 4) +
@@ -278,7 +328,8 @@ struct Pipe {
     const uint32_t mine = st + ws * kPrivate;
     const uint32_t l16 = static_cast<uint32_t>(lane) * 16;
 #pragma unroll
-    for (int r = 0; r < R; ++r) CopyToLds16S(w_src + (u * R + r) * kRec, l16, mine + r * kRec);
+    for (int r = 0; r < R; ++r)
+      CopyToLds16S(w_src + (u * kRecords + r) * kRec, l16, mine + r * kRec);
 #pragma unroll
     for (int i = 0; i < kMetaCopies; ++i)
       if (i * 64 + lane < kMeta / 16)
@@ -286,11 +337,10 @@ struct Pipe {
 #pragma unroll
     for (int i = 0; i < kSharedPer; ++i) {
       const int s = SharedCopy(i);
-      if (s < 2 * GC) {
-        CopyToLds16(s_src[i] + u * kUnit, st + kDigits + s * kRec);
-      } else if ((s - 2 * GC) * 64 + lane < kColLanes) {
-        CopyToLds16(s_src[i] + u * (kWords * 4), st + kColumns + (s - 2 * GC) * kRec);
-      }
+      const uint32_t step = s < 2 * GC ? kUnit : kWords * 4;
+      if (s_on[i])
+        CopyToLds16(s_src[i] + static_cast<uint32_t>(u) * step,
+                    st + (s < 2 * GC ? kDigits + s * kRec : kColumns + (s - 2 * GC) * kRec));
     }
   }
   // Waits until all but the newest N copies of this wavefront are in LDS (for
@@ -314,19 +364,20 @@ struct Pipe {
     const uint8_t *st = lds + stage * kStage, *mine = st + ws * kPrivate;
     const int c = lane & 15, q = lane >> 4;
     const bool low = q < 2;  // lane groups of the first 16 values of each 32
-    int a[R][8];
-    floatx4 scale[R][F];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const uint4 wv = *reinterpret_cast<const uint4 *>(mine + r * kRec + lane * 16);
       const uint32_t w[4] = {wv.x, wv.y, wv.z, wv.w};
+      const int rr = r + half;
+      floatx4 scale[F];
 #pragma unroll
       for (int f = 0; f < F; ++f)
-        scale[r][f] = *reinterpret_cast<const floatx4 *>(mine + R * kRec + r * (64 * F) +
-                                                         (q * F + f) * 16);
+        scale[f] = *reinterpret_cast<const floatx4 *>(mine + R * kRec + rr * (64 * F) +
+                                                      (q * F + f) * 16);
+      int a[8];
       if constexpr (ZP) {
         // Bytes 64 + nibble - zero point: in 49 .. 79, so no byte borrows.
-        const uint8_t *zp = mine + R * kRec + R * 64 * F + (r * 16 + c) * F;
+        const uint8_t *zp = mine + R * kRec + kRecords * 64 * F + (rr * 16 + c) * F;
         uint32_t z[2];
         if constexpr (F == 1) z[0] = *zp;
         else if constexpr (F == 2) z[0] = *reinterpret_cast<const uint16_t *>(zp);
@@ -342,35 +393,32 @@ struct Pipe {
             const int f = F == 4 ? i : F == 2 ? i / 2 : 0;
             zz = __builtin_amdgcn_perm(0, z[0], 0x01010101u * f);
           }
-          a[r][2 * i] = static_cast<int>(((w[i] & 0x0F0F0F0Fu) | 0x40404040u) - zz);
-          a[r][2 * i + 1] = static_cast<int>((((w[i] >> 4) & 0x0F0F0F0Fu) | 0x40404040u) - zz);
+          a[2 * i] = static_cast<int>(((w[i] & 0x0F0F0F0Fu) | 0x40404040u) - zz);
+          a[2 * i + 1] = static_cast<int>((((w[i] >> 4) & 0x0F0F0F0Fu) | 0x40404040u) - zz);
         }
       } else {
         // Nibbles are two's complement here: 16 of them in the high half of a byte.
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          a[r][2 * i] = static_cast<int>((w[i] << 4) & 0xF0F0F0F0u);
-          a[r][2 * i + 1] = static_cast<int>(w[i] & 0xF0F0F0F0u);
+          a[2 * i] = static_cast<int>((w[i] << 4) & 0xF0F0F0F0u);
+          a[2 * i + 1] = static_cast<int>(w[i] & 0xF0F0F0F0u);
         }
       }
-    }
+      const intx4 a0{a[0], a[1], a[2], a[3]}, a1{a[4], a[5], a[6], a[7]};
 #pragma unroll
-    for (int g = 0; g < GC; ++g) {
-      if (GC > 1 && g >= groups) break;
-      const intx4 b0 = *reinterpret_cast<const intx4 *>(st + kDigits + 2 * g * kRec + lane * 16);
-      const intx4 b1 =
-          *reinterpret_cast<const intx4 *>(st + kDigits + (2 * g + 1) * kRec + lane * 16);
-      int col[kWords];
+      for (int g = 0; g < GC; ++g) {
+        if (GC > 1 && g >= groups) break;
+        const intx4 b0 = *reinterpret_cast<const intx4 *>(st + kDigits + 2 * g * kRec + lane * 16);
+        const intx4 b1 =
+            *reinterpret_cast<const intx4 *>(st + kDigits + (2 * g + 1) * kRec + lane * 16);
+        int col[kWords];
 #pragma unroll
-      for (int i = 0; i < kWords; i += 4) {
-        const intx4 v =
-            *reinterpret_cast<const intx4 *>(st + kColumns + ((g * 16 + c) * kWords + i) * 4);
+        for (int i = 0; i < kWords; i += 4) {
+          const intx4 v =
+              *reinterpret_cast<const intx4 *>(st + kColumns + ((g * 16 + c) * kWords + i) * 4);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) col[i + j] = v[j];
-      }
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const intx4 a0{a[r][0], a[r][1], a[r][2], a[r][3]}, a1{a[r][4], a[r][5], a[r][6], a[r][7]};
+          for (int j = 0; j < 4; ++j) col[i + j] = v[j];
+        }
         floatx4 part{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int f = 0; f < kFolds; ++f) {
@@ -391,10 +439,10 @@ struct Pipe {
               lo = use ? lo : 0;
               hi = use ? hi : 0;
             }
-            sum = __builtin_amdgcn_mfma_i32_16x16x32_i8(Long(a[r][2 * i], a[r][2 * i + 1]),
-                                                        Long(lo, hi), sum, 0, 0, 0);
+            sum = __builtin_amdgcn_mfma_i32_16x16x32_i8(Long(a[2 * i], a[2 * i + 1]), Long(lo, hi),
+                                                        sum, 0, 0, 0);
           }
-          const floatx4 s = scale[r][f * F / kFolds];
+          const floatx4 s = scale[f * F / kFolds];
 #pragma unroll
           for (int v = 0; v < 4; ++v) part[v] = fmaf(static_cast<float>(sum[v]), s[v], part[v]);
           if ((f + 1) % (kFolds / XB) == 0) {  // the end of a part with its own power
@@ -465,11 +513,21 @@ __device__ __forceinline__ int CollectPairs(const int32_t *pair_expert, int pair
 
 // Third launch: workgroup (b, i) the 16 * WAVES channels of block b of entry i's
 // expert, 16 channels (gate and up) per wavefront.
-template <int ND, int GC, int F, bool ZP, int WAVES, int NS>
+// CHOOSE: of one token, whose choice each workgroup makes from its logits.
+struct Choice {
+  const float *logits;
+  int32_t *ids;
+  float *weights;
+  int experts;
+  bool normalize;
+};
+
+template <int ND, int GC, int F, bool ZP, int WAVES, int NS, bool CHOOSE>
 __global__ __launch_bounds__(64 * WAVES) void MoeGateUpKernel(
     Matrix m, Fixed fx, Fixed fh, const int32_t *__restrict__ pair_expert,
-    const float *__restrict__ pair_weight, Entries entries, int pairs, int top_k, bool by_expert) {
-  using P = Pipe<ND, GC, F, 1, ZP, WAVES, NS>;
+    const float *__restrict__ pair_weight, Entries entries, int pairs, int top_k, bool by_expert,
+    Choice choice) {
+  using P = Pipe<ND, GC, 2, F, 1, ZP, WAVES, NS>;
   constexpr int kT = P::kT, kChannels = 16 * WAVES;
   static_assert(GC * kT * kChannels * 4 <= P::kLds, "the activations reuse the pipe's LDS");
   extern __shared__ uint4 dynamic[];
@@ -478,8 +536,32 @@ __global__ __launch_bounds__(64 * WAVES) void MoeGateUpKernel(
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int entry = blockIdx.y;
-  const int e = by_expert ? entry : pair_expert[entry];
-  if (wave == 0) {
+  int e;
+  if constexpr (CHOOSE) {
+    __shared__ float best[kMaxTopK];
+    __shared__ int32_t who[kMaxTopK];
+    static_assert(P::kLds >= kMaxExperts * 4, "the keys use the pipe's LDS");
+    const float total = Choose<64 * WAVES>(choice.logits, choice.experts, top_k, choice.normalize,
+                                           reinterpret_cast<uint32_t *>(dynamic), best, who);
+    e = __builtin_amdgcn_readfirstlane(who[entry]);
+    if (tid == 0) {
+      list[0] = entry;
+      shared_n = 1;
+      if (blockIdx.x == 0) {
+        const float p = expf(best[entry] - best[0]) / total;
+        entries.expert[entry] = e;
+        entries.count[entry] = 1;
+        entries.offset[entry] = entry;
+        entries.pair[entry] = entry;
+        entries.weight[entry] = p;
+        if (choice.ids) choice.ids[entry] = e;
+        if (choice.weights) choice.weights[entry] = p;
+      }
+    }
+  } else {
+    e = by_expert ? entry : pair_expert[entry];
+  }
+  if (!CHOOSE && wave == 0) {
     int before;
     int n = CollectPairs(pair_expert, pairs, e, list, &before);
     // Of the pairs that share an expert the first one works.
@@ -561,13 +643,13 @@ __device__ __forceinline__ int Count(uint32_t segment) { return (segment >> 12) 
 //              gridDim.y; partial sums to parts [runs][tokens][H] if there are several.
 //   SHARE = 1: R * 16 columns; each of 8 wavefronts a run of its own, which join
 //              in order.
-template <int ND, int GC, int F, int XB, bool ZP, int SHARE, int NS, typename T>
+// R = 2: the wavefront takes a group of 32 rows; R = 1: half of one.
+template <int ND, int GC, int R, int F, int XB, bool ZP, int SHARE, int NS, typename T>
 __global__ __launch_bounds__(512) void MoeDownKernel(Matrix m, Fixed fh, Entries entries,
                                                      T *__restrict__ Y, float *__restrict__ parts,
                                                      int n_entries, int pairs, int most_segments,
                                                      int tokens, int top_k, int64_t H) {
-  constexpr int R = kRecords;
-  using P = Pipe<ND, GC, F, XB, ZP, SHARE, NS>;
+  using P = Pipe<ND, GC, R, F, XB, ZP, SHARE, NS>;
   constexpr int kT = P::kT, kPipes = 8 / SHARE;
   // The pipes' LDS, then sums [8][tokens][32], the pairs' weights, the segments
   // (offset in the list of pairs, n, expert) and that list.
@@ -615,11 +697,12 @@ __global__ __launch_bounds__(512) void MoeDownKernel(Matrix m, Fixed fh, Entries
   const int64_t i0 = items * run / runs, i1 = items * (run + 1) / runs;
   const int c = lane & 15, q = lane >> 4;
   const float weight = ColumnWeight<ND, ZP>(lane);
-  const int64_t group = min(SHARE == 1 ? static_cast<int64_t>(blockIdx.x)
-                                       : static_cast<int64_t>(blockIdx.x) * 8 + wave,
-                            m.groups - 1);
+  const int64_t place = SHARE == 1 ? static_cast<int64_t>(blockIdx.x)
+                                   : static_cast<int64_t>(blockIdx.x) * 8 + wave;
+  const int64_t group = min(R == 2 ? place : place >> 1, m.groups - 1);
   if (i0 < i1) {
-    P pipe(lds + (SHARE == 1 ? wave * P::kLds : 0), lane, SHARE == 1 ? 0 : wave);
+    P pipe(lds + (SHARE == 1 ? wave * P::kLds : 0), lane, SHARE == 1 ? 0 : wave,
+           R == 2 ? 0 : static_cast<int>(place & 1));
     // The next item to copy.
     int next_seg = static_cast<int>(i0 / units), next_u = static_cast<int>(i0 % units);
     const int last_seg = static_cast<int>((i1 - 1) / units);
@@ -711,14 +794,20 @@ __global__ __launch_bounds__(512) void MoeDownKernel(Matrix m, Fixed fh, Entries
   }
 }
 
-// Y = the runs' sums, in order.
+// Y = the runs' sums, in order; a thread's loads of eight runs are in flight together.
 template <typename T>
 __global__ __launch_bounds__(256) void MoeSumKernel(const float *__restrict__ parts,
                                                     T *__restrict__ Y, int64_t n, int runs) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= n) return;
-  float y = parts[i];
-  for (int r = 1; r < runs; ++r) y += parts[r * n + i];
+  float y = 0.0f;
+  for (int r = 0; r < runs; r += 8) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = r + j < runs ? parts[(r + j) * n + i] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y += v[j];
+  }
   Y[i] = static_cast<T>(y);
 }
 
@@ -808,17 +897,20 @@ constexpr int kNarrowTokens = 8;
 struct Shape {
   int entries;
   bool narrow;  // gate/up: 32 channels a workgroup, powers of two per 32 channels
-  int runs;     // down: 0: one workgroup for 32 columns; else runs of the items
+  int runs;     // down: 0: one workgroup for 16 columns; else runs of the items
+  bool choose;  // one token: the gate/up kernel makes its choice
 };
 
 Shape PickShape(const Layer &l, int tokens) {
   Shape s;
   s.entries = std::min(tokens * l.top_k, l.experts);
   s.narrow = tokens <= kNarrowTokens && s.entries * CeilDiv(l.intermediate, 128) < 2 * l.num_cus;
+  // A workgroup's choice among more experts takes longer than a launch of its own.
+  s.choose = tokens == 1 && l.experts <= 256;
   s.runs = 0;
   if (!s.narrow) {
     const int64_t blocks = CeilDiv(l.hidden, 256);
-    s.runs = static_cast<int>(std::max<int64_t>(1, CeilDiv(2 * l.num_cus, blocks)));
+    s.runs = static_cast<int>(std::max<int64_t>(1, CeilDiv(l.num_cus, blocks)));
     s.runs = static_cast<int>(
         std::min<int64_t>(s.runs, std::max<int64_t>(1, s.entries * l.down.units / 4)));
   }
@@ -861,28 +953,30 @@ Work Split(const Layer &l, int T, int ND, void *base) {
   return w;
 }
 
-template <int ND, int GC, int F, bool ZP, int WAVES>
+template <int ND, int GC, int F, bool ZP, int WAVES, bool CHOOSE>
 hipError_t LaunchGateUp(const Layer &l, const Work &w, const Shape &shape, int pairs,
-                        hipStream_t s) {
-  constexpr int NS = 3;
+                        const Choice &choice, hipStream_t s) {
+  constexpr int NS = WAVES == 2 ? (F == 8 ? 5 : 8) : GC == 4 ? (F == 8 ? 3 : 4) : 3;
   const dim3 grid(static_cast<unsigned>(l.gate_up.groups / WAVES),
                   static_cast<unsigned>(shape.entries));
-  hipLaunchKernelGGL((MoeGateUpKernel<ND, GC, F, ZP, WAVES, NS>), grid, dim3(64 * WAVES),
-                     (Pipe<ND, GC, F, 1, ZP, WAVES, NS>::kLds), s, l.gate_up, w.fx, w.fh,
-                     w.pair_expert, w.pair_weight, w.entries, pairs, l.top_k, pairs >= l.experts);
+  hipLaunchKernelGGL((MoeGateUpKernel<ND, GC, F, ZP, WAVES, NS, CHOOSE>), grid, dim3(64 * WAVES),
+                     (Pipe<ND, GC, 2, F, 1, ZP, WAVES, NS>::kLds), s, l.gate_up, w.fx, w.fh,
+                     w.pair_expert, w.pair_weight, w.entries, pairs, l.top_k,
+                     pairs >= l.experts, choice);
   return hipGetLastError();
 }
 
 template <int ND, int GC, int F, int XB, bool ZP, int SHARE, typename T>
 hipError_t LaunchDown(const Layer &l, const Work &w, const Shape &shape, int tokens, T *Y,
                       hipStream_t s) {
-  constexpr int NS = SHARE == 1 || F == 8 ? 2 : 3;
+  constexpr int R = SHARE == 1 ? 1 : 2;
+  constexpr int NS = SHARE == 1 ? 3 : F == 8 || (GC == 4 && F == 4) ? 2 : 3;
   const int pairs = tokens * l.top_k;
   const int segments = shape.entries + pairs / (GC * kTokens<ND>);
-  const size_t lds = static_cast<size_t>(8 / SHARE) * Pipe<ND, GC, F, XB, ZP, SHARE, NS>::kLds +
-                     8 * tokens * 32 * sizeof(float) + pairs * 6 + segments * 4;
-  const int64_t blocks = CeilDiv(l.down.groups, SHARE);
-  hipLaunchKernelGGL((MoeDownKernel<ND, GC, F, XB, ZP, SHARE, NS, T>),
+  const size_t lds = static_cast<size_t>(8 / SHARE) * Pipe<ND, GC, R, F, XB, ZP, SHARE, NS>::kLds +
+                     8 * tokens * R * 16 * sizeof(float) + pairs * 6 + segments * 4;
+  const int64_t blocks = SHARE == 1 ? 2 * l.down.groups : CeilDiv(l.down.groups, SHARE);
+  hipLaunchKernelGGL((MoeDownKernel<ND, GC, R, F, XB, ZP, SHARE, NS, T>),
                      dim3(static_cast<unsigned>(blocks), std::max(1, shape.runs)), dim3(512), lds, s,
                      l.down, w.fh, w.entries, Y, w.parts, shape.entries, pairs, segments, tokens,
                      l.top_k, l.hidden);
@@ -895,26 +989,32 @@ hipError_t LaunchDown(const Layer &l, const Work &w, const Shape &shape, int tok
 }
 
 template <int ND, int GC, int F, bool ZP, typename T>
-hipError_t LaunchExperts(const Layer &l, const Work &w, int tokens, T *Y, hipStream_t s) {
-  const Shape shape = PickShape(l, tokens);
+hipError_t LaunchExperts(const Layer &l, const Work &w, const Shape &shape, int tokens, T *Y,
+                         const Choice &choice, hipStream_t s) {
   const int pairs = tokens * l.top_k;
+  hipError_t e;
   if constexpr (GC == 1) {
     if (shape.narrow) {
-      const hipError_t e = LaunchGateUp<ND, GC, F, ZP, 2>(l, w, shape, pairs, s);
+      e = shape.choose ? LaunchGateUp<ND, GC, F, ZP, 2, true>(l, w, shape, pairs, choice, s)
+                       : LaunchGateUp<ND, GC, F, ZP, 2, false>(l, w, shape, pairs, choice, s);
       return e != hipSuccess ? e : LaunchDown<ND, GC, F, 4, ZP, 1, T>(l, w, shape, tokens, Y, s);
     }
+    if (shape.choose) e = LaunchGateUp<ND, GC, F, ZP, 8, true>(l, w, shape, pairs, choice, s);
+    else e = LaunchGateUp<ND, GC, F, ZP, 8, false>(l, w, shape, pairs, choice, s);
+  } else {
+    e = LaunchGateUp<ND, GC, F, ZP, 8, false>(l, w, shape, pairs, choice, s);
   }
-  const hipError_t e = LaunchGateUp<ND, GC, F, ZP, 8>(l, w, shape, pairs, s);
   return e != hipSuccess ? e : LaunchDown<ND, GC, F, 1, ZP, 8, T>(l, w, shape, tokens, Y, s);
 }
 
 template <int ND, int GC, bool ZP, typename T>
-hipError_t LaunchFolds(const Layer &l, const Work &w, int tokens, T *Y, hipStream_t s) {
+hipError_t LaunchFolds(const Layer &l, const Work &w, const Shape &shape, int tokens, T *Y,
+                       const Choice &choice, hipStream_t s) {
   switch (l.folds) {
-  case 1: return LaunchExperts<ND, GC, 1, ZP, T>(l, w, tokens, Y, s);
-  case 2: return LaunchExperts<ND, GC, 2, ZP, T>(l, w, tokens, Y, s);
-  case 4: return LaunchExperts<ND, GC, 4, ZP, T>(l, w, tokens, Y, s);
-  default: return LaunchExperts<ND, GC, 8, ZP, T>(l, w, tokens, Y, s);
+  case 1: return LaunchExperts<ND, GC, 1, ZP, T>(l, w, shape, tokens, Y, choice, s);
+  case 2: return LaunchExperts<ND, GC, 2, ZP, T>(l, w, shape, tokens, Y, choice, s);
+  case 4: return LaunchExperts<ND, GC, 4, ZP, T>(l, w, shape, tokens, Y, choice, s);
+  default: return LaunchExperts<ND, GC, 8, ZP, T>(l, w, shape, tokens, Y, choice, s);
   }
 }
 
@@ -928,31 +1028,43 @@ hipError_t LaunchLayerT(const Layer &l, int tokens, const void *X, const float *
       logits ? 0 : l.experts * (tokens == 1 ? 1 : static_cast<int>(CeilDiv(tokens, kRT)));
   const unsigned prep =
       static_cast<unsigned>(router_wgs + CeilDiv(tokens * l.gate_up.units, 16));
-  if (tokens == 1)
-    hipLaunchKernelGGL((MoePrepKernel<ND, 1, T>), dim3(prep), dim3(256), 0, s,
-                       static_cast<const T *>(X), l.router, w.logits, w.fx, tokens, l.hidden,
-                       l.experts, l.zeros, router_wgs);
-  else
-    hipLaunchKernelGGL((MoePrepKernel<ND, kRT, T>), dim3(prep), dim3(256), 0, s,
-                       static_cast<const T *>(X), l.router, w.logits, w.fx, tokens, l.hidden,
-                       l.experts, l.zeros, router_wgs);
+  const bool vec = l.hidden % 4 == 0 && reinterpret_cast<uintptr_t>(X) % (4 * sizeof(T)) == 0;
+  auto launch_prep = [&](auto rt, auto v) {
+    hipLaunchKernelGGL((MoePrepKernel<ND, decltype(rt)::value, decltype(v)::value, T>), dim3(prep),
+                       dim3(256), 0, s, static_cast<const T *>(X), l.router, w.logits, w.fx, tokens,
+                       l.hidden, l.experts, l.zeros, router_wgs);
+  };
+  using One = std::integral_constant<int, 1>;
+  using Several = std::integral_constant<int, kRT>;
+  if (tokens == 1) vec ? launch_prep(One{}, std::true_type{}) : launch_prep(One{}, std::false_type{});
+  else vec ? launch_prep(Several{}, std::true_type{}) : launch_prep(Several{}, std::false_type{});
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(MoeRouteKernel, dim3(static_cast<unsigned>(tokens)), dim3(256), 0, s,
-                     logits ? logits : w.logits, w.pair_expert, w.pair_weight, ids, weights,
-                     l.experts, l.top_k, l.normalize);
-  e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  const Shape shape = PickShape(l, tokens);
+  const Choice choice{logits ? logits : w.logits, ids, weights, l.experts, l.normalize};
+  if (!shape.choose) {
+    hipLaunchKernelGGL(MoeRouteKernel, dim3(static_cast<unsigned>(tokens)), dim3(256), 0, s,
+                       choice.logits, w.pair_expert, w.pair_weight, ids, weights, l.experts,
+                       l.top_k, l.normalize);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
   T *y = static_cast<T *>(Y);
-  // Column groups per pass over an expert's rows: what its share of the tokens fills.
-  const bool many =
-      tokens > kNarrowTokens &&
-      static_cast<int64_t>(tokens) * l.top_k > static_cast<int64_t>(l.experts) * kTokens<ND> / 2;
-  if (l.zeros)
-    return many ? LaunchFolds<ND, 2, true, T>(l, w, tokens, y, s)
-                : LaunchFolds<ND, 1, true, T>(l, w, tokens, y, s);
-  return many ? LaunchFolds<ND, 2, false, T>(l, w, tokens, y, s)
-              : LaunchFolds<ND, 1, false, T>(l, w, tokens, y, s);
+  // Column groups per pass over an expert's rows: what most experts' tokens fill,
+  // their mean share and two standard deviations of even choices.
+  const double mean = static_cast<double>(tokens) * l.top_k / l.experts;
+  const double most = std::min<double>(tokens, mean + 2.0 * std::sqrt(mean));
+  const int gc = tokens <= kNarrowTokens || most <= kTokens<ND> ? 1 : most <= 2 * kTokens<ND> ? 2 : 4;
+  auto experts = [&](auto groups) {
+    constexpr int GC = decltype(groups)::value;
+    return l.zeros ? LaunchFolds<ND, GC, true, T>(l, w, shape, tokens, y, choice, s)
+                   : LaunchFolds<ND, GC, false, T>(l, w, shape, tokens, y, choice, s);
+  };
+  switch (gc) {
+  case 1: return experts(std::integral_constant<int, 1>{});
+  case 2: return experts(std::integral_constant<int, 2>{});
+  default: return experts(std::integral_constant<int, 4>{});
+  }
 }
 
 } // namespace
