@@ -26,17 +26,6 @@ struct Weight {
   int num_cus;
 };
 
-// Copies 4 bytes per lane from src to LDS byte lds_base + 4 lane (as CopyToLds16).
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void CopyToLds4(const void *src, uint32_t lds_base) {
-  __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
-                   :
-                   : "s"(lds_base), "v"(src)
-                   : "memory", "m0");
-}
-#pragma clang diagnostic pop
-
 // s_waitcnt vmcnt(N) lgkmcnt(0) and a workgroup barrier, nothing moved across.
 template <int N>
 __device__ __forceinline__ void WaitBarrier() {

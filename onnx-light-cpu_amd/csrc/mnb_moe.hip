@@ -6,15 +6,14 @@
 //
 //   x = 2^s (256^2 d2 + 256 d1 + d0), digits in [-128, 127] (two digits for
 //   16-bit activations), one power of two for each block of 128 values,
-//   w = scale (q - z), q - 8 in the high half of a byte: one mask per four
-//   weights and no conversion.
+//   w = scale (q - z), q - z in a byte by three or four operations on four
+//   weights at once, without conversions.
 //
-// A token's digits are neighbouring columns of one MFMA tile: 16 columns hold
-// five tokens of three digits or eight of two, so the digits cost no extra
-// matrix instruction, and the rows of a tile are 16 weight rows. A weight
-// block's sums S = 16 sum (q - 8) d are exact (below 2^21), as is S - 16 (z - 8)
-// sum d; they are scaled and added up in fp32, column by column, and the
-// columns of a token join after the last block.
+// A token's digits are columns of one MFMA tile: 16 columns hold five tokens of
+// three digits or eight of two, so the digits cost no extra matrix instruction,
+// and the rows of a tile are 16 weight rows. A weight block's sums are exact
+// integers (below 2^21); they are scaled and added up in fp32, column by column,
+// and the columns of a token join after the last block.
 //
 // Four launches: logits and the fixed-point tokens; the choice; gate/up with
 // the activation, whose rows leave in fixed point; down with the weighted sum
@@ -32,33 +31,28 @@ namespace {
 typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
-// Columns of a tile per digit: the tokens of one column group.
-template <int ND>
-constexpr int kTokens = ND == 3 ? 5 : 8;
+// Columns of a tile per digit: the tokens of one column group. ONE: a group of
+// one token, whose digits alone are kept and copied.
+template <int ND, bool ONE = false>
+constexpr int kTokens = ONE ? 1 : ND == 3 ? 5 : 8;
 
 // ---- fixed point ---------------------------------------------------------------
 
-// Rows in fixed point: digits [rows][ND][units * 128] and for each row, digit
-// and unit a column record of `words` words: the powers of two of the unit's
-// `scales` parts, then (zero points) for each of its `folds` parts -64 times the
-// sum of the digits, which the products start from.
+// Rows in fixed point: digits [rows][ND][units * 128] and the powers of two of
+// each unit's `scales` parts [rows][units][scales].
 struct Fixed {
   int8_t *dig;
-  int32_t *col;
+  float *power;
   int64_t units;
-  int scales, folds, words;
+  int scales;
 };
-
-constexpr int ColumnWords(int scales, int folds, bool zeros) {
-  return (scales + (zeros ? folds : 0) + 3) / 4 * 4;
-}
 
 // Eight values of a unit of row `row`, k = 8 i .. 8 i + 7, by thread i (% 16) of
 // 16, or of the 16 / scales that share a part. The unit's 128 bytes of a digit
 // lie as the weight layout takes them: the eight of i at 32 (i % 4) + 8 (i / 4).
 template <int ND>
 __device__ __forceinline__ void StoreUnit(const Fixed &f, int64_t row, int64_t unit, int i,
-                                          bool zeros, const float (&x)[8]) {
+                                          const float (&x)[8]) {
   // As integers, magnitudes order like their values, infinity above them and NaN on top.
   uint32_t top = 0;
 #pragma unroll
@@ -76,30 +70,22 @@ __device__ __forceinline__ void StoreUnit(const Fixed &f, int64_t row, int64_t u
 #pragma unroll
   for (int j = 0; j < 8; ++j)
     n[j] = finite ? static_cast<int>(rintf(ldexpf(x[j], kBits - e))) : 0;
-  const int lanes = 16 / f.folds;
-  const float power = finite ? ldexpf(1.0f, e - kBits) : __uint_as_float(0x7FC00000u);
+  if (i % part == 0)
+    f.power[(row * f.units + unit) * f.scales + i / part] =
+        finite ? ldexpf(1.0f, e - kBits) : __uint_as_float(0x7FC00000u);
 #pragma unroll
   for (int d = 0; d < ND; ++d) {
     uint32_t lo = 0, hi = 0;
-    int sum = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int digit = d + 1 < ND ? static_cast<int>(static_cast<int8_t>(n[j])) : n[j];
       n[j] = (n[j] - digit) >> 8;
-      sum += digit;
       const uint32_t b = static_cast<uint32_t>(digit) & 0xFFu;
       if (j < 4) lo |= b << (8 * j);
       else hi |= b << (8 * (j - 4));
     }
-    const int64_t at = (row * ND + d) * f.units + unit;
-    *reinterpret_cast<uint2 *>(f.dig + at * kUnit + 32 * (i & 3) + 8 * (i >> 2)) =
-        make_uint2(lo, hi);
-    int32_t *col = f.col + at * f.words;
-    if (i % part == 0) col[i / part] = __float_as_int(power);
-    if (zeros) {
-      for (int off = 1; off < lanes; off <<= 1) sum += __shfl_xor(sum, off, 16);
-      if (i % lanes == 0) col[f.scales + i / lanes] = -64 * sum;
-    }
+    *reinterpret_cast<uint2 *>(f.dig + ((row * ND + d) * f.units + unit) * kUnit + 32 * (i & 3) +
+                               8 * (i >> 2)) = make_uint2(lo, hi);
   }
 }
 
@@ -113,7 +99,7 @@ template <int ND, int RT, bool VEC, typename T>
 __global__ __launch_bounds__(256) void MoePrepKernel(const T *__restrict__ X,
                                                      const float *__restrict__ R, float *logits,
                                                      Fixed fx, int tokens, int64_t H, int E,
-                                                     bool zeros, int router_wgs) {
+                                                     int router_wgs) {
   const int tid = threadIdx.x;
   if (static_cast<int>(blockIdx.x) < router_wgs) {
     const int e = static_cast<int>(blockIdx.x) % E, t0 = static_cast<int>(blockIdx.x) / E * RT;
@@ -168,7 +154,7 @@ __global__ __launch_bounds__(256) void MoePrepKernel(const T *__restrict__ X,
   float x[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) x[j] = k0 + j < H ? static_cast<float>(X[row * H + k0 + j]) : 0.0f;
-  StoreUnit<ND>(fx, row, unit, tid & 15, zeros, x);
+  StoreUnit<ND>(fx, row, unit, tid & 15, x);
 }
 
 // ---- second launch: the choice ------------------------------------------------
@@ -251,27 +237,30 @@ __global__ __launch_bounds__(256) void MoeRouteKernel(const float *__restrict__ 
 // ---- the products ---------------------------------------------------------------
 
 // A pipe streams units through LDS: SHARE wavefronts, each with R records of its
-// own per unit (both of its row group, or one of them), and one set of GC column groups for all of them (SHARE = 1: a
-// pipe of one wavefront, without barriers). NS units are in flight by direct
-// global -> LDS copies, so what keeps the memory busy needs no registers.
-// F weight blocks per unit, XB parts of it with powers of two of their own.
-template <int ND, int GC, int R, int F, int XB, bool ZP, int SHARE, int NS>
+// own per unit (both of its row group, or one of them), and one set of GC column
+// groups for all of them (SHARE = 1: a pipe of one wavefront, without barriers).
+// NS units are in flight by direct global -> LDS copies, so what keeps the memory
+// busy needs no registers. F weight blocks per unit, XB parts of it with powers
+// of two of their own.
+template <int ND, bool ONE, int GC, int R, int F, int XB, bool ZP, int SHARE, int NS>
 struct Pipe {
-  static constexpr int kT = kTokens<ND>;
+  static_assert(!ONE || GC == 1, "one token, one column group");
+  static constexpr int kT = kTokens<ND, ONE>;
+  static constexpr int kCols = ONE ? 4 : 16;  // kept columns of a group
   static constexpr int kFolds = F > XB ? F : XB;
-  static constexpr int kWords = ColumnWords(XB, kFolds, ZP);
   static constexpr int kMeta = MetaBytes(F, ZP);
   static constexpr int kMetaCopies = (kMeta + kRec - 1) / kRec;
-  static constexpr int kColLanes = GC * 16 * (kWords / 4);
-  static constexpr int kShared = 2 * GC + (kColLanes + 63) / 64;
+  static constexpr int kDigitCopies = ONE ? 1 : 2 * GC;
+  static constexpr int kShared = kDigitCopies + 1;  // the last one the powers'
   static constexpr int kSharedPer = (kShared + SHARE - 1) / SHARE;
   static constexpr int kOps = R + kMetaCopies + kSharedPer;
   static constexpr int kPrivate = R * kRec + kMeta;
-  static constexpr int kDigits = SHARE * kPrivate;  // offset in a stage
-  static constexpr int kColumns = kDigits + GC * 2 * kRec;
-  static constexpr int kStage = kColumns + kColLanes * 16;
+  static constexpr int kDigits = SHARE * kPrivate;  // offsets in a stage
+  static constexpr int kPowers = kDigits + GC * 128 * kCols;
+  static constexpr int kStage = kPowers + (ONE ? 16 : GC * 16 * XB * 4);
   static constexpr int kLds = NS * kStage;
   static_assert(kMeta % 16 == 0 && kOps * (NS - 1) < 64, "copies");
+  static_assert(XB == 1 || GC == 1, "powers: one copy");
 
   const uint8_t *lds;  // this pipe's
   uint32_t base;       // its LDS byte
@@ -301,46 +290,40 @@ struct Pipe {
 #pragma unroll
     for (int i = 0; i < kSharedPer; ++i) {
       const int s = SharedCopy(i);
-      // The column (g, c) whose data this lane copies.
-      int column, part = 0;
-      if (s < 2 * GC) {
-        column = (s >> 1) * 16 + (lane & 15);
-      } else {
-        const int l = (s - 2 * GC) * 64 + lane;
-        column = min(l, kColLanes - 1) / (kWords / 4);
-        part = l % (kWords / 4);
-      }
-      const int c = column & 15, token = (column >> 4) * kT + c % kT;
-      const int digit = min(c / kT, ND - 1);
+      const bool powers = s == kDigitCopies;
+      // The column whose data this lane copies, and which 32 bytes of a digit's unit.
+      const int column = powers ? lane : ONE ? lane & 3 : (s >> 1) * 16 + (lane & 15);
+      const int part = ONE ? (lane >> 2) & 3 : lane >> 4, h = ONE ? lane >> 4 : s & 1;
+      const int c = column & 15, digit = c / kT, token = (column >> 4) * kT + c % kT;
       // Columns without a token keep what LDS holds: nothing reads their sums. One
       // lane is always on, so that every copy is issued and counted.
-      s_on[i] = (token < n && c < ND * kT && (s < 2 * GC || (s - 2 * GC) * 64 + lane < kColLanes)) ||
-                lane == 0;
-      const int64_t at = (row_of(token < n ? token : 0) * ND + digit) * f.units;
-      s_src[i] = s < 2 * GC
-                     ? reinterpret_cast<const uint8_t *>(f.dig) + at * kUnit + 32 * (lane >> 4) +
-                           16 * (s & 1)
-                     : reinterpret_cast<const uint8_t *>(f.col) + at * (kWords * 4) + part * 16;
+      s_on[i] = (token < n && digit < ND && column < 16 * GC && (!ONE || lane < 32) &&
+                 (!ONE || !powers || lane == 0)) || lane == 0;
+      const int64_t row = row_of(token < n ? token : 0);
+      s_src[i] = powers ? reinterpret_cast<const uint8_t *>(f.power + row * f.units * XB)
+                        : reinterpret_cast<const uint8_t *>(f.dig) +
+                              (row * ND + min(digit, ND - 1)) * f.units * kUnit + 32 * part + 16 * h;
     }
   }
-  __device__ __forceinline__ void Issue(int64_t u, int stage) const {
+  __device__ __forceinline__ void Issue(int u, int stage) const {
     const uint32_t st = base + stage * kStage;
     const uint32_t mine = st + ws * kPrivate;
     const uint32_t l16 = static_cast<uint32_t>(lane) * 16;
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      CopyToLds16S(w_src + (u * kRecords + r) * kRec, l16, mine + r * kRec);
+      CopyToLds16S(w_src + (static_cast<int64_t>(u) * kRecords + r) * kRec, l16, mine + r * kRec);
 #pragma unroll
     for (int i = 0; i < kMetaCopies; ++i)
       if (i * 64 + lane < kMeta / 16)
-        CopyToLds16S(m_src + u * kMeta + i * kRec, l16, mine + (R + i) * kRec);
+        CopyToLds16S(m_src + static_cast<int64_t>(u) * kMeta + i * kRec, l16, mine + (R + i) * kRec);
 #pragma unroll
     for (int i = 0; i < kSharedPer; ++i) {
       const int s = SharedCopy(i);
-      const uint32_t step = s < 2 * GC ? kUnit : kWords * 4;
-      if (s_on[i])
-        CopyToLds16(s_src[i] + static_cast<uint32_t>(u) * step,
-                    st + (s < 2 * GC ? kDigits + s * kRec : kColumns + (s - 2 * GC) * kRec));
+      if (s_on[i]) {
+        if (s < kDigitCopies) CopyToLds16(s_src[i] + u * kUnit, st + kDigits + s * kRec);
+        else if constexpr (XB == 1) CopyToLds4(s_src[i] + u * 4, st + kPowers);
+        else CopyToLds16(s_src[i] + u * (XB * 4), st + kPowers);
+      }
     }
   }
   // Waits until all but the newest N copies of this wavefront are in LDS (for
@@ -358,26 +341,25 @@ struct Pipe {
     return static_cast<long>((static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32) |
                              static_cast<uint32_t>(lo));
   }
+  // Four nibbles (in the low halves of the bytes) less the zero points zz: with
+  // the top bit set no byte borrows (128 + q - z is in 113 .. 143), and flipping it
+  // leaves the two's complement.
+  static __device__ __forceinline__ int Shift(uint32_t nibbles, uint32_t zz) {
+    return static_cast<int>((((nibbles & 0x0F0F0F0Fu) | 0x80808080u) - zz) ^ 0x80808080u);
+  }
   // acc[r][g][v] += row 4 q + v of record r, this lane's column of group g
   // (groups past `groups` are left out).
   __device__ __forceinline__ void Multiply(int stage, int groups, floatx4 (&acc)[R][GC]) const {
     const uint8_t *st = lds + stage * kStage, *mine = st + ws * kPrivate;
     const int c = lane & 15, q = lane >> 4;
     const bool low = q < 2;  // lane groups of the first 16 values of each 32
+    int a[R][8];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const uint4 wv = *reinterpret_cast<const uint4 *>(mine + r * kRec + lane * 16);
       const uint32_t w[4] = {wv.x, wv.y, wv.z, wv.w};
-      const int rr = r + half;
-      floatx4 scale[F];
-#pragma unroll
-      for (int f = 0; f < F; ++f)
-        scale[f] = *reinterpret_cast<const floatx4 *>(mine + R * kRec + rr * (64 * F) +
-                                                      (q * F + f) * 16);
-      int a[8];
       if constexpr (ZP) {
-        // Bytes 64 + nibble - zero point: in 49 .. 79, so no byte borrows.
-        const uint8_t *zp = mine + R * kRec + kRecords * 64 * F + (rr * 16 + c) * F;
+        const uint8_t *zp = mine + R * kRec + kRecords * 64 * F + ((r + half) * 16 + c) * F;
         uint32_t z[2];
         if constexpr (F == 1) z[0] = *zp;
         else if constexpr (F == 2) z[0] = *reinterpret_cast<const uint16_t *>(zp);
@@ -393,37 +375,47 @@ struct Pipe {
             const int f = F == 4 ? i : F == 2 ? i / 2 : 0;
             zz = __builtin_amdgcn_perm(0, z[0], 0x01010101u * f);
           }
-          a[2 * i] = static_cast<int>(((w[i] & 0x0F0F0F0Fu) | 0x40404040u) - zz);
-          a[2 * i + 1] = static_cast<int>((((w[i] >> 4) & 0x0F0F0F0Fu) | 0x40404040u) - zz);
+          a[r][2 * i] = Shift(w[i], zz);
+          a[r][2 * i + 1] = Shift(w[i] >> 4, zz);
         }
       } else {
         // Nibbles are two's complement here: 16 of them in the high half of a byte.
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          a[2 * i] = static_cast<int>((w[i] << 4) & 0xF0F0F0F0u);
-          a[2 * i + 1] = static_cast<int>(w[i] & 0xF0F0F0F0u);
+          a[r][2 * i] = static_cast<int>((w[i] << 4) & 0xF0F0F0F0u);
+          a[r][2 * i + 1] = static_cast<int>(w[i] & 0xF0F0F0F0u);
         }
       }
-      const intx4 a0{a[0], a[1], a[2], a[3]}, a1{a[4], a[5], a[6], a[7]};
+    }
+    floatx4 scale[R][F];
 #pragma unroll
-      for (int g = 0; g < GC; ++g) {
-        if (GC > 1 && g >= groups) break;
-        const intx4 b0 = *reinterpret_cast<const intx4 *>(st + kDigits + 2 * g * kRec + lane * 16);
-        const intx4 b1 =
-            *reinterpret_cast<const intx4 *>(st + kDigits + (2 * g + 1) * kRec + lane * 16);
-        int col[kWords];
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int i = 0; i < kWords; i += 4) {
-          const intx4 v =
-              *reinterpret_cast<const intx4 *>(st + kColumns + ((g * 16 + c) * kWords + i) * 4);
+      for (int f = 0; f < F; ++f)
+        scale[r][f] = *reinterpret_cast<const floatx4 *>(mine + R * kRec + (r + half) * (64 * F) +
+                                                         (q * F + f) * 16);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) col[i + j] = v[j];
-        }
+    for (int g = 0; g < GC; ++g) {
+      if (GC > 1 && g >= groups) break;
+      const uint8_t *dig = st + kDigits + 2 * g * kRec + (q * kCols + min(c, kCols - 1)) * 16;
+      const intx4 b0 = *reinterpret_cast<const intx4 *>(dig);
+      const intx4 b1 = *reinterpret_cast<const intx4 *>(dig + kCols * 64);
+      float power[XB];
+      const uint8_t *at = st + kPowers + (ONE ? 0 : (g * 16 + c) * XB * 4);
+      if constexpr (XB == 1) {
+        power[0] = *reinterpret_cast<const float *>(at);
+      } else {
+        const floatx4 p = *reinterpret_cast<const floatx4 *>(at);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) power[j] = p[j];
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const intx4 a0{a[r][0], a[r][1], a[r][2], a[r][3]}, a1{a[r][4], a[r][5], a[r][6], a[r][7]};
         floatx4 part{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int f = 0; f < kFolds; ++f) {
-          const int start = ZP ? col[XB + f] : 0;
-          intx4 sum{start, start, start, start};
+          intx4 sum{0, 0, 0, 0};
           if constexpr (kFolds == 1) {
             sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(a0, b0, sum, 0, 0, 0);
             sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(a1, b1, sum, 0, 0, 0);
@@ -439,19 +431,19 @@ struct Pipe {
               lo = use ? lo : 0;
               hi = use ? hi : 0;
             }
-            sum = __builtin_amdgcn_mfma_i32_16x16x32_i8(Long(a[2 * i], a[2 * i + 1]), Long(lo, hi),
-                                                        sum, 0, 0, 0);
+            sum = __builtin_amdgcn_mfma_i32_16x16x32_i8(Long(a[r][2 * i], a[r][2 * i + 1]),
+                                                        Long(lo, hi), sum, 0, 0, 0);
           }
-          const floatx4 s = scale[f * F / kFolds];
+          const floatx4 s = scale[r][f * F / kFolds];
 #pragma unroll
-          for (int v = 0; v < 4; ++v) part[v] = fmaf(static_cast<float>(sum[v]), s[v], part[v]);
+          for (int v = 0; v < 4; ++v) {
+            const float t = static_cast<float>(sum[v]);
+            part[v] = f % (kFolds / XB) == 0 ? t * s[v] : fmaf(t, s[v], part[v]);
+          }
           if ((f + 1) % (kFolds / XB) == 0) {  // the end of a part with its own power
-            const float power = __int_as_float(col[f / (kFolds / XB)]);
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              acc[r][g][v] = fmaf(part[v], power, acc[r][g][v]);
-              part[v] = 0.0f;
-            }
+            for (int v = 0; v < 4; ++v)
+              acc[r][g][v] = fmaf(part[v], power[f / (kFolds / XB)], acc[r][g][v]);
           }
         }
       }
@@ -459,27 +451,27 @@ struct Pipe {
   }
 };
 
-// The sum of a token's digit columns, in the column of digit 0 (garbage in the
-// others): v holds this lane's column times 256^digit.
-template <int ND>
+// The value `n` lanes up in the row of 16 (0 past its end).
+template <int N>
+__device__ __forceinline__ float LanesUp(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x100 + N, 0xF, 0xF, true));
+}
+
+// The sum of a token's digit columns (kTokens apart), in the column of digit 0
+// (garbage in the others): v holds this lane's column times 256^digit.
+template <int ND, bool ONE>
 __device__ __forceinline__ float JoinDigits(float v) {
-  const int b = __float_as_int(v);
-  if constexpr (ND == 2) {  // columns t and 8 + t
-    return v + __int_as_float(__builtin_amdgcn_mov_dpp(b, 0x128, 0xF, 0xF, true));  // row_ror:8
-  } else {  // columns t, 5 + t, 10 + t
-    const float m = __int_as_float(__builtin_amdgcn_mov_dpp(b, 0x105, 0xF, 0xF, true));  // row_shl:5
-    const float h = __int_as_float(__builtin_amdgcn_mov_dpp(b, 0x10A, 0xF, 0xF, true));  // row_shl:10
-    return (h + m) + v;
-  }
+  constexpr int kT = kTokens<ND, ONE>;
+  if constexpr (ND == 2) return LanesUp<kT>(v) + v;
+  else return (LanesUp<2 * kT>(v) + LanesUp<kT>(v)) + v;
 }
 
 // What a column's sum counts for: 256^digit, and 1/16 without zero points (the
 // weights' bytes hold 16 times their value there).
-template <int ND, bool ZP>
+template <int ND, bool ONE, bool ZP>
 __device__ __forceinline__ float ColumnWeight(int lane) {
-  const int c = lane & 15;
-  if (c >= ND * kTokens<ND>) return 0.0f;
-  const int digit = c / kTokens<ND>;
+  const int digit = (lane & 15) / kTokens<ND, ONE>;
+  if (digit >= ND) return 0.0f;
   const float w = digit == 0 ? 1.0f : digit == 1 ? 256.0f : 65536.0f;
   return ZP ? w : w * 0.0625f;
 }
@@ -511,8 +503,6 @@ __device__ __forceinline__ int CollectPairs(const int32_t *pair_expert, int pair
   return n;
 }
 
-// Third launch: workgroup (b, i) the 16 * WAVES channels of block b of entry i's
-// expert, 16 channels (gate and up) per wavefront.
 // CHOOSE: of one token, whose choice each workgroup makes from its logits.
 struct Choice {
   const float *logits;
@@ -522,14 +512,19 @@ struct Choice {
   bool normalize;
 };
 
-template <int ND, int GC, int F, bool ZP, int WAVES, int NS, bool CHOOSE>
-__global__ __launch_bounds__(64 * WAVES) void MoeGateUpKernel(
+// Third launch: workgroup (b, i) the channels of block b of entry i's expert, 16
+// (gate and up) for each of GROUPS wavefronts that share a pipe, or, with KS runs
+// of the units, for each of GROUPS * KS wavefronts with pipes of their own.
+template <int ND, bool ONE, int GC, int F, bool ZP, int GROUPS, int KS, int NS, bool CHOOSE>
+__global__ __launch_bounds__(64 * GROUPS *KS) void MoeGateUpKernel(
     Matrix m, Fixed fx, Fixed fh, const int32_t *__restrict__ pair_expert,
     const float *__restrict__ pair_weight, Entries entries, int pairs, int top_k, bool by_expert,
     Choice choice) {
-  using P = Pipe<ND, GC, 2, F, 1, ZP, WAVES, NS>;
-  constexpr int kT = P::kT, kChannels = 16 * WAVES;
-  static_assert(GC * kT * kChannels * 4 <= P::kLds, "the activations reuse the pipe's LDS");
+  using P = Pipe<ND, ONE, GC, 2, F, 1, ZP, KS == 1 ? GROUPS : 1, NS>;
+  constexpr int kT = P::kT, kChannels = 16 * GROUPS, kWaves = GROUPS * KS;
+  constexpr int kPipes = KS == 1 ? 1 : kWaves;
+  static_assert(kPipes * P::kLds >= GC * kT * kChannels * 4 + (KS - 1) * GROUPS * GC * 2048,
+                "the activations and the runs' sums reuse the pipes' LDS");
   extern __shared__ uint4 dynamic[];
   __shared__ int32_t list[kMaxTokens];
   __shared__ int32_t shared_n;
@@ -540,9 +535,9 @@ __global__ __launch_bounds__(64 * WAVES) void MoeGateUpKernel(
   if constexpr (CHOOSE) {
     __shared__ float best[kMaxTopK];
     __shared__ int32_t who[kMaxTopK];
-    static_assert(P::kLds >= kMaxExperts * 4, "the keys use the pipe's LDS");
-    const float total = Choose<64 * WAVES>(choice.logits, choice.experts, top_k, choice.normalize,
-                                           reinterpret_cast<uint32_t *>(dynamic), best, who);
+    static_assert(kPipes * P::kLds >= kMaxExperts * 4, "the keys use the pipes' LDS");
+    const float total = Choose<64 * kWaves>(choice.logits, choice.experts, top_k, choice.normalize,
+                                            reinterpret_cast<uint32_t *>(dynamic), best, who);
     e = __builtin_amdgcn_readfirstlane(who[entry]);
     if (tid == 0) {
       list[0] = entry;
@@ -560,22 +555,22 @@ __global__ __launch_bounds__(64 * WAVES) void MoeGateUpKernel(
     }
   } else {
     e = by_expert ? entry : pair_expert[entry];
-  }
-  if (!CHOOSE && wave == 0) {
-    int before;
-    int n = CollectPairs(pair_expert, pairs, e, list, &before);
-    // Of the pairs that share an expert the first one works.
-    if (!by_expert && list[0] != entry) n = 0;
-    if (lane == 0) shared_n = n;
-    if (blockIdx.x == 0) {
-      if (lane == 0) {
-        entries.expert[entry] = e;
-        entries.count[entry] = n;
-        entries.offset[entry] = before;
-      }
-      if (lane < n) {
-        entries.pair[before + lane] = list[lane];
-        entries.weight[before + lane] = pair_weight[list[lane]];
+    if (wave == 0) {
+      int before;
+      int n = CollectPairs(pair_expert, pairs, e, list, &before);
+      // Of the pairs that share an expert the first one works.
+      if (!by_expert && list[0] != entry) n = 0;
+      if (lane == 0) shared_n = n;
+      if (blockIdx.x == 0) {
+        if (lane == 0) {
+          entries.expert[entry] = e;
+          entries.count[entry] = n;
+          entries.offset[entry] = before;
+        }
+        if (lane < n) {
+          entries.pair[before + lane] = list[lane];
+          entries.weight[before + lane] = pair_weight[list[lane]];
+        }
       }
     }
   }
@@ -583,48 +578,75 @@ __global__ __launch_bounds__(64 * WAVES) void MoeGateUpKernel(
   const int n = __builtin_amdgcn_readfirstlane(shared_n);
   if (n == 0) return;
   const int c = lane & 15, q = lane >> 4;
-  const float weight = ColumnWeight<ND, ZP>(lane);
-  P pipe(reinterpret_cast<const uint8_t *>(dynamic), lane, wave);
+  const float weight = ColumnWeight<ND, ONE, ZP>(lane);
+  const int cg = wave % GROUPS, ks = wave / GROUPS;
+  P pipe(reinterpret_cast<const uint8_t *>(dynamic) + (KS == 1 ? 0 : wave * P::kLds), lane,
+         KS == 1 ? wave : 0);
   float *hidden = reinterpret_cast<float *>(dynamic);  // [GC * kT][kChannels]
+  floatx4 *sums = reinterpret_cast<floatx4 *>(hidden + GC * kT * kChannels);
   const int units = static_cast<int>(m.units);
+  const int u0 = units * ks / KS, u1 = units * (ks + 1) / KS;
   for (int t0 = 0; t0 < n; t0 += GC * kT) {
     const int left = min(n - t0, GC * kT), groups = (left + kT - 1) / kT;
-    pipe.Segment(m, e, static_cast<int64_t>(blockIdx.x) * WAVES + wave, fx, left,
-                 [&](int i) { return static_cast<int64_t>(list[t0 + i] / top_k); });
     floatx4 acc[2][GC];
 #pragma unroll
     for (int r = 0; r < 2; ++r)
 #pragma unroll
       for (int g = 0; g < GC; ++g) acc[r][g] = floatx4{0.f, 0.f, 0.f, 0.f};
+    if (u0 < u1) {
+      pipe.Segment(m, e, static_cast<int64_t>(blockIdx.x) * GROUPS + cg, fx, left,
+                   [&](int i) { return static_cast<int64_t>(list[t0 + i] / top_k); });
 #pragma unroll
-    for (int p = 0; p < NS - 1; ++p) pipe.Issue(min(p, units - 1), p);
-    int stage = 0;
-    for (int u = 0; u < units; ++u) {
-      P::template Wait<P::kOps *(NS - 2)>();
-      pipe.Issue(min(u + NS - 1, units - 1), stage == 0 ? NS - 1 : stage - 1);
-      pipe.Multiply(stage, groups, acc);
-      stage = stage + 1 == NS ? 0 : stage + 1;
+      for (int p = 0; p < NS - 1; ++p) pipe.Issue(min(u0 + p, u1 - 1), p);
+      int stage = 0;
+      for (int u = u0; u < u1; ++u) {
+        P::template Wait<P::kOps *(NS - 2)>();
+        pipe.Issue(min(u + NS - 1, u1 - 1), stage == 0 ? NS - 1 : stage - 1);
+        pipe.Multiply(stage, groups, acc);
+        stage = stage + 1 == NS ? 0 : stage + 1;
+      }
+      P::template Wait<0>();
     }
-    P::template Wait<0>();
+    if constexpr (KS > 1) {
+      __syncthreads();
+      if (ks > 0) {
 #pragma unroll
-    for (int g = 0; g < GC; ++g) {
-      floatx4 h;
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int v = 0; v < 4; ++v)
-        h[v] = SiluMul(JoinDigits<ND>(acc[0][g][v] * weight), JoinDigits<ND>(acc[1][g][v] * weight));
-      if (c < kT)
-        *reinterpret_cast<floatx4 *>(hidden + (g * kT + c) * kChannels + 16 * wave + 4 * q) = h;
+          for (int g = 0; g < GC; ++g)
+            sums[((wave - GROUPS) * 2 * GC + r * GC + g) * 64 + lane] = acc[r][g];
+      }
+      __syncthreads();
+    }
+    if (ks == 0) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int g = 0; g < GC; ++g)
+#pragma unroll
+          for (int s = 1; s < KS; ++s)
+            acc[r][g] += sums[(((s - 1) * GROUPS + cg) * 2 * GC + r * GC + g) * 64 + lane];
+#pragma unroll
+      for (int g = 0; g < GC; ++g) {
+        floatx4 h;
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          h[v] = SiluMul(JoinDigits<ND, ONE>(acc[0][g][v] * weight),
+                         JoinDigits<ND, ONE>(acc[1][g][v] * weight));
+        if (c < kT)
+          *reinterpret_cast<floatx4 *>(hidden + (g * kT + c) * kChannels + 16 * cg + 4 * q) = h;
+      }
     }
     __syncthreads();
     constexpr int kPer = kChannels / 8;  // threads of a token
-    for (int i = tid / kPer; i < GC * kT; i += 64 * WAVES / kPer) {
+    for (int i = tid / kPer; i < GC * kT; i += 64 * kWaves / kPer) {
       if (i >= left) continue;
       const int k = tid % kPer;
       float x[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = hidden[i * kChannels + 8 * k + j];
       const int64_t k0 = static_cast<int64_t>(blockIdx.x) * (kChannels / 8) + k;  // eights of the row
-      StoreUnit<ND>(fh, list[t0 + i], k0 >> 4, static_cast<int>(k0 & 15), ZP, x);
+      StoreUnit<ND>(fh, list[t0 + i], k0 >> 4, static_cast<int>(k0 & 15), x);
     }
     __syncthreads();
   }
@@ -644,12 +666,12 @@ __device__ __forceinline__ int Count(uint32_t segment) { return (segment >> 12) 
 //   SHARE = 1: R * 16 columns; each of 8 wavefronts a run of its own, which join
 //              in order.
 // R = 2: the wavefront takes a group of 32 rows; R = 1: half of one.
-template <int ND, int GC, int R, int F, int XB, bool ZP, int SHARE, int NS, typename T>
+template <int ND, bool ONE, int GC, int R, int F, int XB, bool ZP, int SHARE, int NS, typename T>
 __global__ __launch_bounds__(512) void MoeDownKernel(Matrix m, Fixed fh, Entries entries,
                                                      T *__restrict__ Y, float *__restrict__ parts,
                                                      int n_entries, int pairs, int most_segments,
                                                      int tokens, int top_k, int64_t H) {
-  using P = Pipe<ND, GC, R, F, XB, ZP, SHARE, NS>;
+  using P = Pipe<ND, ONE, GC, R, F, XB, ZP, SHARE, NS>;
   constexpr int kT = P::kT, kPipes = 8 / SHARE;
   // The pipes' LDS, then sums [8][tokens][32], the pairs' weights, the segments
   // (offset in the list of pairs, n, expert) and that list.
@@ -696,7 +718,7 @@ __global__ __launch_bounds__(512) void MoeDownKernel(Matrix m, Fixed fh, Entries
   const int64_t run = SHARE == 1 ? wave : blockIdx.y, runs = SHARE == 1 ? 8 : gridDim.y;
   const int64_t i0 = items * run / runs, i1 = items * (run + 1) / runs;
   const int c = lane & 15, q = lane >> 4;
-  const float weight = ColumnWeight<ND, ZP>(lane);
+  const float weight = ColumnWeight<ND, ONE, ZP>(lane);
   const int64_t place = SHARE == 1 ? static_cast<int64_t>(blockIdx.x)
                                    : static_cast<int64_t>(blockIdx.x) * 8 + wave;
   const int64_t group = min(R == 2 ? place : place >> 1, m.groups - 1);
@@ -746,7 +768,7 @@ __global__ __launch_bounds__(512) void MoeDownKernel(Matrix m, Fixed fh, Entries
           for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-              y[r][v] = JoinDigits<ND>(acc[r][g][v] * weight);
+              y[r][v] = JoinDigits<ND, ONE>(acc[r][g][v] * weight);
               acc[r][g][v] = 0.0f;
             }
           const int j = g * kT + c;
@@ -897,6 +919,7 @@ constexpr int kNarrowTokens = 8;
 struct Shape {
   int entries;
   bool narrow;  // gate/up: 32 channels a workgroup, powers of two per 32 channels
+  bool split;   // ... and the units over four wavefronts each
   int runs;     // down: 0: one workgroup for 16 columns; else runs of the items
   bool choose;  // one token: the gate/up kernel makes its choice
 };
@@ -904,13 +927,15 @@ struct Shape {
 Shape PickShape(const Layer &l, int tokens) {
   Shape s;
   s.entries = std::min(tokens * l.top_k, l.experts);
-  s.narrow = tokens <= kNarrowTokens && s.entries * CeilDiv(l.intermediate, 128) < 2 * l.num_cus;
+  const int64_t blocks = s.entries * CeilDiv(l.intermediate, 128);  // of 128 channels
+  s.narrow = tokens <= kNarrowTokens && blocks < 2 * l.num_cus;
+  s.split = s.narrow && 4 * blocks <= 2 * l.num_cus;
   // A workgroup's choice among more experts takes longer than a launch of its own.
   s.choose = tokens == 1 && l.experts <= 256;
   s.runs = 0;
   if (!s.narrow) {
-    const int64_t blocks = CeilDiv(l.hidden, 256);
-    s.runs = static_cast<int>(std::max<int64_t>(1, CeilDiv(l.num_cus, blocks)));
+    const int64_t columns = CeilDiv(l.hidden, 256);
+    s.runs = static_cast<int>(std::max<int64_t>(1, CeilDiv(l.num_cus, columns)));
     s.runs = static_cast<int>(
         std::min<int64_t>(s.runs, std::max<int64_t>(1, s.entries * l.down.units / 4)));
   }
@@ -931,10 +956,8 @@ Work Split(const Layer &l, int T, int ND, void *base) {
     Fixed f;
     f.units = units;
     f.scales = scales;
-    f.folds = std::max(l.folds, scales);
-    f.words = ColumnWords(scales, f.folds, l.zeros);
     f.dig = reinterpret_cast<int8_t *>(take(rows * ND * units * kUnit));
-    f.col = reinterpret_cast<int32_t *>(take(rows * ND * units * f.words * 4));
+    f.power = reinterpret_cast<float *>(take(rows * units * scales * 4));
     return f;
   };
   w.fx = fixed(T, l.gate_up.units, 1);
@@ -953,30 +976,32 @@ Work Split(const Layer &l, int T, int ND, void *base) {
   return w;
 }
 
-template <int ND, int GC, int F, bool ZP, int WAVES, bool CHOOSE>
+template <int ND, bool ONE, int GC, int F, bool ZP, int GROUPS, int KS, bool CHOOSE>
 hipError_t LaunchGateUp(const Layer &l, const Work &w, const Shape &shape, int pairs,
                         const Choice &choice, hipStream_t s) {
-  constexpr int NS = WAVES == 2 ? (F == 8 ? 5 : 8) : GC == 4 ? (F == 8 ? 3 : 4) : 3;
-  const dim3 grid(static_cast<unsigned>(l.gate_up.groups / WAVES),
+  constexpr int NS = KS > 1 ? (ONE ? 4 : 3) : GC == 4 ? (F == 8 ? 3 : 4) : 3;
+  using P = Pipe<ND, ONE, GC, 2, F, 1, ZP, KS == 1 ? GROUPS : 1, NS>;
+  const dim3 grid(static_cast<unsigned>(l.gate_up.groups / GROUPS),
                   static_cast<unsigned>(shape.entries));
-  hipLaunchKernelGGL((MoeGateUpKernel<ND, GC, F, ZP, WAVES, NS, CHOOSE>), grid, dim3(64 * WAVES),
-                     (Pipe<ND, GC, 2, F, 1, ZP, WAVES, NS>::kLds), s, l.gate_up, w.fx, w.fh,
-                     w.pair_expert, w.pair_weight, w.entries, pairs, l.top_k,
+  hipLaunchKernelGGL((MoeGateUpKernel<ND, ONE, GC, F, ZP, GROUPS, KS, NS, CHOOSE>), grid,
+                     dim3(64 * GROUPS * KS), (KS == 1 ? 1 : GROUPS * KS) * P::kLds, s, l.gate_up,
+                     w.fx, w.fh, w.pair_expert, w.pair_weight, w.entries, pairs, l.top_k,
                      pairs >= l.experts, choice);
   return hipGetLastError();
 }
 
-template <int ND, int GC, int F, int XB, bool ZP, int SHARE, typename T>
+template <int ND, bool ONE, int GC, int F, int XB, bool ZP, int SHARE, typename T>
 hipError_t LaunchDown(const Layer &l, const Work &w, const Shape &shape, int tokens, T *Y,
                       hipStream_t s) {
   constexpr int R = SHARE == 1 ? 1 : 2;
-  constexpr int NS = SHARE == 1 ? 3 : F == 8 || (GC == 4 && F == 4) ? 2 : 3;
+  constexpr int NS = SHARE == 1 ? (ONE ? 5 : 3) : F == 8 || (GC == 4 && F == 4) ? 2 : 3;
+  using P = Pipe<ND, ONE, GC, R, F, XB, ZP, SHARE, NS>;
   const int pairs = tokens * l.top_k;
-  const int segments = shape.entries + pairs / (GC * kTokens<ND>);
-  const size_t lds = static_cast<size_t>(8 / SHARE) * Pipe<ND, GC, R, F, XB, ZP, SHARE, NS>::kLds +
-                     8 * tokens * R * 16 * sizeof(float) + pairs * 6 + segments * 4;
+  const int segments = shape.entries + pairs / (GC * P::kT);
+  const size_t lds = static_cast<size_t>(8 / SHARE) * P::kLds + 8 * tokens * R * 16 * sizeof(float) +
+                     pairs * 6 + segments * 4;
   const int64_t blocks = SHARE == 1 ? 2 * l.down.groups : CeilDiv(l.down.groups, SHARE);
-  hipLaunchKernelGGL((MoeDownKernel<ND, GC, R, F, XB, ZP, SHARE, NS, T>),
+  hipLaunchKernelGGL((MoeDownKernel<ND, ONE, GC, R, F, XB, ZP, SHARE, NS, T>),
                      dim3(static_cast<unsigned>(blocks), std::max(1, shape.runs)), dim3(512), lds, s,
                      l.down, w.fh, w.entries, Y, w.parts, shape.entries, pairs, segments, tokens,
                      l.top_k, l.hidden);
@@ -988,33 +1013,40 @@ hipError_t LaunchDown(const Layer &l, const Work &w, const Shape &shape, int tok
   return hipGetLastError();
 }
 
-template <int ND, int GC, int F, bool ZP, typename T>
+template <int ND, bool ONE, int GC, int F, bool ZP, int GROUPS, int KS>
+hipError_t LaunchGateUpC(const Layer &l, const Work &w, const Shape &shape, int pairs,
+                         const Choice &choice, hipStream_t s) {
+  if constexpr (ONE) {
+    if (shape.choose)
+      return LaunchGateUp<ND, ONE, GC, F, ZP, GROUPS, KS, true>(l, w, shape, pairs, choice, s);
+  }
+  return LaunchGateUp<ND, ONE, GC, F, ZP, GROUPS, KS, false>(l, w, shape, pairs, choice, s);
+}
+
+template <int ND, bool ONE, int GC, int F, bool ZP, typename T>
 hipError_t LaunchExperts(const Layer &l, const Work &w, const Shape &shape, int tokens, T *Y,
                          const Choice &choice, hipStream_t s) {
   const int pairs = tokens * l.top_k;
   hipError_t e;
   if constexpr (GC == 1) {
     if (shape.narrow) {
-      e = shape.choose ? LaunchGateUp<ND, GC, F, ZP, 2, true>(l, w, shape, pairs, choice, s)
-                       : LaunchGateUp<ND, GC, F, ZP, 2, false>(l, w, shape, pairs, choice, s);
-      return e != hipSuccess ? e : LaunchDown<ND, GC, F, 4, ZP, 1, T>(l, w, shape, tokens, Y, s);
+      if (shape.split) e = LaunchGateUpC<ND, ONE, GC, F, ZP, 2, 4>(l, w, shape, pairs, choice, s);
+      else e = LaunchGateUpC<ND, ONE, GC, F, ZP, 2, 1>(l, w, shape, pairs, choice, s);
+      return e != hipSuccess ? e : LaunchDown<ND, ONE, GC, F, 4, ZP, 1, T>(l, w, shape, tokens, Y, s);
     }
-    if (shape.choose) e = LaunchGateUp<ND, GC, F, ZP, 8, true>(l, w, shape, pairs, choice, s);
-    else e = LaunchGateUp<ND, GC, F, ZP, 8, false>(l, w, shape, pairs, choice, s);
-  } else {
-    e = LaunchGateUp<ND, GC, F, ZP, 8, false>(l, w, shape, pairs, choice, s);
   }
-  return e != hipSuccess ? e : LaunchDown<ND, GC, F, 1, ZP, 8, T>(l, w, shape, tokens, Y, s);
+  e = LaunchGateUpC<ND, ONE, GC, F, ZP, 8, 1>(l, w, shape, pairs, choice, s);
+  return e != hipSuccess ? e : LaunchDown<ND, ONE, GC, F, 1, ZP, 8, T>(l, w, shape, tokens, Y, s);
 }
 
-template <int ND, int GC, bool ZP, typename T>
+template <int ND, bool ONE, int GC, bool ZP, typename T>
 hipError_t LaunchFolds(const Layer &l, const Work &w, const Shape &shape, int tokens, T *Y,
                        const Choice &choice, hipStream_t s) {
   switch (l.folds) {
-  case 1: return LaunchExperts<ND, GC, 1, ZP, T>(l, w, shape, tokens, Y, choice, s);
-  case 2: return LaunchExperts<ND, GC, 2, ZP, T>(l, w, shape, tokens, Y, choice, s);
-  case 4: return LaunchExperts<ND, GC, 4, ZP, T>(l, w, shape, tokens, Y, choice, s);
-  default: return LaunchExperts<ND, GC, 8, ZP, T>(l, w, shape, tokens, Y, choice, s);
+  case 1: return LaunchExperts<ND, ONE, GC, 1, ZP, T>(l, w, shape, tokens, Y, choice, s);
+  case 2: return LaunchExperts<ND, ONE, GC, 2, ZP, T>(l, w, shape, tokens, Y, choice, s);
+  case 4: return LaunchExperts<ND, ONE, GC, 4, ZP, T>(l, w, shape, tokens, Y, choice, s);
+  default: return LaunchExperts<ND, ONE, GC, 8, ZP, T>(l, w, shape, tokens, Y, choice, s);
   }
 }
 
@@ -1032,7 +1064,7 @@ hipError_t LaunchLayerT(const Layer &l, int tokens, const void *X, const float *
   auto launch_prep = [&](auto rt, auto v) {
     hipLaunchKernelGGL((MoePrepKernel<ND, decltype(rt)::value, decltype(v)::value, T>), dim3(prep),
                        dim3(256), 0, s, static_cast<const T *>(X), l.router, w.logits, w.fx, tokens,
-                       l.hidden, l.experts, l.zeros, router_wgs);
+                       l.hidden, l.experts, router_wgs);
   };
   using One = std::integral_constant<int, 1>;
   using Several = std::integral_constant<int, kRT>;
@@ -1055,15 +1087,17 @@ hipError_t LaunchLayerT(const Layer &l, int tokens, const void *X, const float *
   const double mean = static_cast<double>(tokens) * l.top_k / l.experts;
   const double most = std::min<double>(tokens, mean + 2.0 * std::sqrt(mean));
   const int gc = tokens <= kNarrowTokens || most <= kTokens<ND> ? 1 : most <= 2 * kTokens<ND> ? 2 : 4;
-  auto experts = [&](auto groups) {
+  auto experts = [&](auto groups, auto one) {
     constexpr int GC = decltype(groups)::value;
-    return l.zeros ? LaunchFolds<ND, GC, true, T>(l, w, shape, tokens, y, choice, s)
-                   : LaunchFolds<ND, GC, false, T>(l, w, shape, tokens, y, choice, s);
+    constexpr bool kOne = decltype(one)::value;
+    return l.zeros ? LaunchFolds<ND, kOne, GC, true, T>(l, w, shape, tokens, y, choice, s)
+                   : LaunchFolds<ND, kOne, GC, false, T>(l, w, shape, tokens, y, choice, s);
   };
+  if (tokens == 1) return experts(std::integral_constant<int, 1>{}, std::true_type{});
   switch (gc) {
-  case 1: return experts(std::integral_constant<int, 1>{});
-  case 2: return experts(std::integral_constant<int, 2>{});
-  default: return experts(std::integral_constant<int, 4>{});
+  case 1: return experts(std::integral_constant<int, 1>{}, std::false_type{});
+  case 2: return experts(std::integral_constant<int, 2>{}, std::false_type{});
+  default: return experts(std::integral_constant<int, 4>{}, std::false_type{});
   }
 }
 
