@@ -40,8 +40,8 @@ extern "C" {
 #endif
 
 typedef struct mnb_moe_desc {
-  int64_t hidden;           /* width of X and Y, at most 2^20 */
-  int64_t intermediate;     /* an expert's width, at most 2^20; the two multiplied at most 2^34 */
+  int64_t hidden;           /* width of X and Y, at most 2^18 */
+  int64_t intermediate;     /* an expert's width, at most 2^18; the two multiplied at most 2^34 */
   int32_t experts;          /* 1 .. 1024 */
   int32_t top_k;            /* 1 .. min(experts, 32) */
   int32_t bits;             /* 4 only */

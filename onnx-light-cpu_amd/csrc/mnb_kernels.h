@@ -53,6 +53,12 @@ __device__ __forceinline__ void CopyToLds4(const void *src, uint32_t lds_base) {
                    : "s"(lds_base), "v"(src)
                    : "memory", "m0");
 }
+__device__ __forceinline__ void CopyToLds4S(const void *sbase, uint32_t voff, uint32_t lds_base) {
+  __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+                   :
+                   : "s"(lds_base), "v"(voff), "s"(sbase)
+                   : "memory", "m0");
+}
 #pragma clang diagnostic pop
 
 // Gated-MLP activation of one gate/up pair, in the order of the ONNX subgraph

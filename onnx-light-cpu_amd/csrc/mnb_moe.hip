@@ -268,7 +268,7 @@ struct Pipe {
   int half;            // R = 1: which record
   // Sources at unit 0 of the current segment.
   const uint8_t *w_src, *m_src;
-  const uint8_t *s_src[kSharedPer];
+  uint32_t s_off[kSharedPer];  // bytes from the digits or the powers (below 2^31)
   bool s_on[kSharedPer];  // this lane's column has a token
 
   __device__ __forceinline__ Pipe(const uint8_t *at, int lane_, int ws_, int half_ = 0)
@@ -299,13 +299,12 @@ struct Pipe {
       // lane is always on, so that every copy is issued and counted.
       s_on[i] = (token < n && digit < ND && column < 16 * GC && (!ONE || lane < 32) &&
                  (!ONE || !powers || lane == 0)) || lane == 0;
-      const int64_t row = row_of(token < n ? token : 0);
-      s_src[i] = powers ? reinterpret_cast<const uint8_t *>(f.power + row * f.units * XB)
-                        : reinterpret_cast<const uint8_t *>(f.dig) +
-                              (row * ND + min(digit, ND - 1)) * f.units * kUnit + 32 * part + 16 * h;
+      const uint32_t row = row_of(token < n ? token : 0), units = static_cast<uint32_t>(f.units);
+      s_off[i] = powers ? row * units * (XB * 4)
+                        : (row * ND + min(digit, ND - 1)) * units * kUnit + 32 * part + 16 * h;
     }
   }
-  __device__ __forceinline__ void Issue(int u, int stage) const {
+  __device__ __forceinline__ void Issue(const Fixed &f, int u, int stage) const {
     const uint32_t st = base + stage * kStage;
     const uint32_t mine = st + ws * kPrivate;
     const uint32_t l16 = static_cast<uint32_t>(lane) * 16;
@@ -320,9 +319,9 @@ struct Pipe {
     for (int i = 0; i < kSharedPer; ++i) {
       const int s = SharedCopy(i);
       if (s_on[i]) {
-        if (s < kDigitCopies) CopyToLds16(s_src[i] + u * kUnit, st + kDigits + s * kRec);
-        else if constexpr (XB == 1) CopyToLds4(s_src[i] + u * 4, st + kPowers);
-        else CopyToLds16(s_src[i] + u * (XB * 4), st + kPowers);
+        if (s < kDigitCopies) CopyToLds16S(f.dig + u * kUnit, s_off[i], st + kDigits + s * kRec);
+        else if constexpr (XB == 1) CopyToLds4S(f.power + u, s_off[i], st + kPowers);
+        else CopyToLds16S(f.power + u * XB, s_off[i], st + kPowers);
       }
     }
   }
@@ -476,14 +475,53 @@ __device__ __forceinline__ float ColumnWeight(int lane) {
   return ZP ? w : w * 0.0625f;
 }
 
-// What the choice gives each launch of experts: entry i of min(tokens * top_k,
-// experts) is an expert with the pairs (token * top_k + place) that chose it, which
-// lie one after another in `pair`, with their weights.
-struct Entries {
-  int32_t *expert, *count, *offset;  // [entries]; count 0: another entry's, or nobody's
-  int32_t *pair;                     // [pairs], by expert and then in order
+// What the choice gives down: the pairs (token * top_k + place), those of an expert
+// one after another, with their weights, cut into segments of up to GC * kTokens
+// of one expert: place in that list, length and expert in 12, 8 and 12 bits.
+struct Plan {
+  int32_t *pair;      // [pairs], by expert and then in order
   float *weight;
+  uint32_t *segment;  // [0]: their number, then the segments
 };
+
+__device__ __forceinline__ uint32_t MakeSegment(int offset, int n, int expert) {
+  return static_cast<uint32_t>(offset) | static_cast<uint32_t>(n) << 12 |
+         static_cast<uint32_t>(expert) << 20;
+}
+__device__ __forceinline__ int Offset(uint32_t segment) { return segment & 0xFFFu; }
+__device__ __forceinline__ int Count(uint32_t segment) { return (segment >> 12) & 0xFFu; }
+__device__ __forceinline__ int Expert(uint32_t segment) { return segment >> 20; }
+
+// The segments of up to `most` pairs, by a whole workgroup; counts: LDS.
+__device__ __forceinline__ void CutSegments(const int32_t *pair_expert, int pairs, int experts,
+                                            int most, int32_t *counts, uint32_t *segment) {
+  const int tid = threadIdx.x, lane = tid & 63, threads = blockDim.x;
+  for (int e = tid; e < experts; e += threads) counts[e] = 0;
+  __syncthreads();
+  for (int p = tid; p < pairs; p += threads) atomicAdd(&counts[pair_expert[p]], 1);
+  __syncthreads();
+  if (tid >= 64) return;
+  int at = 0, offset = 0;
+  for (int e0 = 0; e0 < experts; e0 += 64) {
+    const int n = e0 + lane < experts ? counts[e0 + lane] : 0;
+    const int cut = (n + most - 1) / most;
+    int end = cut, last = n;  // inclusive sums over the lanes
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int a = __shfl_up(end, off, 64), b = __shfl_up(last, off, 64);
+      if (lane >= off) {
+        end += a;
+        last += b;
+      }
+    }
+    for (int j = 0; j < cut; ++j)
+      segment[1 + at + end - cut + j] =
+          MakeSegment(offset + last - n + j * most, min(n - j * most, most), e0 + lane);
+    at += __shfl(end, 63, 64);
+    offset += __shfl(last, 63, 64);
+  }
+  if (lane == 0) segment[0] = at;
+}
 
 // The pairs that chose expert e, in order, and how many chose a lower one: by
 // every thread of one wavefront.
@@ -518,7 +556,7 @@ struct Choice {
 template <int ND, bool ONE, int GC, int F, bool ZP, int GROUPS, int KS, int NS, bool CHOOSE>
 __global__ __launch_bounds__(64 * GROUPS *KS) void MoeGateUpKernel(
     Matrix m, Fixed fx, Fixed fh, const int32_t *__restrict__ pair_expert,
-    const float *__restrict__ pair_weight, Entries entries, int pairs, int top_k, bool by_expert,
+    const float *__restrict__ pair_weight, Plan plan, int pairs, int top_k, bool by_expert,
     Choice choice) {
   using P = Pipe<ND, ONE, GC, 2, F, 1, ZP, KS == 1 ? GROUPS : 1, NS>;
   constexpr int kT = P::kT, kChannels = 16 * GROUPS, kWaves = GROUPS * KS;
@@ -544,16 +582,22 @@ __global__ __launch_bounds__(64 * GROUPS *KS) void MoeGateUpKernel(
       shared_n = 1;
       if (blockIdx.x == 0) {
         const float p = expf(best[entry] - best[0]) / total;
-        entries.expert[entry] = e;
-        entries.count[entry] = 1;
-        entries.offset[entry] = entry;
-        entries.pair[entry] = entry;
-        entries.weight[entry] = p;
+        plan.pair[entry] = entry;
+        plan.weight[entry] = p;
+        plan.segment[1 + entry] = MakeSegment(entry, 1, e);
+        if (entry == 0) plan.segment[0] = top_k;
         if (choice.ids) choice.ids[entry] = e;
         if (choice.weights) choice.weights[entry] = p;
       }
     }
   } else {
+    if (entry == static_cast<int>(gridDim.y) - 1) {  // the last row's first workgroup
+      static_assert(kPipes * P::kLds >= kMaxExperts * 4, "the counts use the pipes' LDS");
+      if (blockIdx.x == 0)
+        CutSegments(pair_expert, pairs, choice.experts, GC * kT, reinterpret_cast<int32_t *>(dynamic),
+                    plan.segment);
+      return;
+    }
     e = by_expert ? entry : pair_expert[entry];
     if (wave == 0) {
       int before;
@@ -561,16 +605,9 @@ __global__ __launch_bounds__(64 * GROUPS *KS) void MoeGateUpKernel(
       // Of the pairs that share an expert the first one works.
       if (!by_expert && list[0] != entry) n = 0;
       if (lane == 0) shared_n = n;
-      if (blockIdx.x == 0) {
-        if (lane == 0) {
-          entries.expert[entry] = e;
-          entries.count[entry] = n;
-          entries.offset[entry] = before;
-        }
-        if (lane < n) {
-          entries.pair[before + lane] = list[lane];
-          entries.weight[before + lane] = pair_weight[list[lane]];
-        }
+      if (blockIdx.x == 0 && lane < n) {
+        plan.pair[before + lane] = list[lane];
+        plan.weight[before + lane] = pair_weight[list[lane]];
       }
     }
   }
@@ -595,13 +632,13 @@ __global__ __launch_bounds__(64 * GROUPS *KS) void MoeGateUpKernel(
       for (int g = 0; g < GC; ++g) acc[r][g] = floatx4{0.f, 0.f, 0.f, 0.f};
     if (u0 < u1) {
       pipe.Segment(m, e, static_cast<int64_t>(blockIdx.x) * GROUPS + cg, fx, left,
-                   [&](int i) { return static_cast<int64_t>(list[t0 + i] / top_k); });
+                   [&](int i) { return list[t0 + i] / top_k; });
 #pragma unroll
-      for (int p = 0; p < NS - 1; ++p) pipe.Issue(min(u0 + p, u1 - 1), p);
+      for (int p = 0; p < NS - 1; ++p) pipe.Issue(fx, min(u0 + p, u1 - 1), p);
       int stage = 0;
       for (int u = u0; u < u1; ++u) {
         P::template Wait<P::kOps *(NS - 2)>();
-        pipe.Issue(min(u + NS - 1, u1 - 1), stage == 0 ? NS - 1 : stage - 1);
+        pipe.Issue(fx, min(u + NS - 1, u1 - 1), stage == 0 ? NS - 1 : stage - 1);
         pipe.Multiply(stage, groups, acc);
         stage = stage + 1 == NS ? 0 : stage + 1;
       }
@@ -652,90 +689,53 @@ __global__ __launch_bounds__(64 * GROUPS *KS) void MoeGateUpKernel(
   }
 }
 
-// A segment's place in the list of pairs and its tokens (12 and 8 bits, the
-// expert above).
-__device__ __forceinline__ int Offset(uint32_t segment) { return segment & 0xFFFu; }
-__device__ __forceinline__ int Count(uint32_t segment) { return (segment >> 12) & 0xFFu; }
-
-// Fourth launch: Y, or partial sums of it. The list of (expert, up to GC * kT of
-// its tokens) segments of the layer, each `units` items long, is cut into equal
-// runs of items; a pipe goes through one run and adds each segment's rows, times
-// the tokens' weights, to sums in LDS.
-//   SHARE = 8: a workgroup takes 8 * R * 16 columns of Y and run blockIdx.y of
-//              gridDim.y; partial sums to parts [runs][tokens][H] if there are several.
-//   SHARE = 1: R * 16 columns; each of 8 wavefronts a run of its own, which join
-//              in order.
-// R = 2: the wavefront takes a group of 32 rows; R = 1: half of one.
-template <int ND, bool ONE, int GC, int R, int F, int XB, bool ZP, int SHARE, int NS, typename T>
-__global__ __launch_bounds__(512) void MoeDownKernel(Matrix m, Fixed fh, Entries entries,
-                                                     T *__restrict__ Y, float *__restrict__ parts,
-                                                     int n_entries, int pairs, int most_segments,
-                                                     int tokens, int top_k, int64_t H) {
-  using P = Pipe<ND, ONE, GC, R, F, XB, ZP, SHARE, NS>;
-  constexpr int kT = P::kT, kPipes = 8 / SHARE;
-  // The pipes' LDS, then sums [8][tokens][32], the pairs' weights, the segments
-  // (offset in the list of pairs, n, expert) and that list.
+// Fourth launch, few tokens on few experts: a workgroup takes 16 columns of Y. The
+// items (segment, unit) of the layer are cut into eight equal runs, one for each
+// wavefront and its pipe, which adds each segment's rows, times the tokens'
+// weights, to sums of its own; they join in order.
+template <int ND, bool ONE, int F, bool ZP, int NS, typename T>
+__global__ __launch_bounds__(512) void MoeDownNarrowKernel(Matrix m, Fixed fh, Plan plan,
+                                                           T *__restrict__ Y, int pairs,
+                                                           int most_segments, int tokens, int top_k,
+                                                           int64_t H) {
+  using P = Pipe<ND, ONE, 1, 1, F, 4, ZP, 1, NS>;
+  constexpr int kT = P::kT;
+  // The pipes' LDS, then sums [8][tokens][16], the pairs' weights, the segments and
+  // the list of pairs.
   extern __shared__ uint4 dynamic[];
-  __shared__ int32_t shared_n;
   uint8_t *lds = reinterpret_cast<uint8_t *>(dynamic);
-  float *sums = reinterpret_cast<float *>(lds + kPipes * P::kLds);
-  float *weights = sums + 8 * tokens * R * 16;
+  float *sums = reinterpret_cast<float *>(lds + 8 * P::kLds);
+  float *weights = sums + 8 * tokens * 16;
   uint32_t *segments = reinterpret_cast<uint32_t *>(weights + pairs);
-  uint16_t *list = reinterpret_cast<uint16_t *>(segments + most_segments);
+  uint16_t *list = reinterpret_cast<uint16_t *>(segments + most_segments + 1);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   for (int i = tid; i < pairs; i += 512) {
-    list[i] = static_cast<uint16_t>(entries.pair[i]);
-    weights[i] = entries.weight[i];
+    list[i] = static_cast<uint16_t>(plan.pair[i]);
+    weights[i] = plan.weight[i];
   }
-  if (wave == 0) {
-    int total = 0;
-    for (int i0 = 0; i0 < n_entries; i0 += 64) {
-      const int i = i0 + lane;
-      const int n = i < n_entries ? entries.count[i] : 0;
-      const int cut = (n + GC * kT - 1) / (GC * kT);
-      int end = cut;  // inclusive sum over the lanes
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const int v = __shfl_up(end, off, 64);
-        if (lane >= off) end += v;
-      }
-      if (n > 0) {
-        const int expert = entries.expert[i], offset = entries.offset[i];
-        for (int j = 0; j < cut; ++j)
-          segments[total + end - cut + j] =
-              (offset + j * GC * kT) | min(n - j * GC * kT, GC * kT) << 12 | expert << 20;
-      }
-      total += __shfl(end, 63, 64);
-    }
-    if (lane == 0) shared_n = total;
-  }
-  float *mine = sums + wave * tokens * (R * 16);
-  for (int i = lane; i < tokens * R * 16; i += 64) mine[i] = 0.0f;
+  for (int i = tid; i <= most_segments; i += 512) segments[i] = plan.segment[i];
+  float *mine = sums + wave * tokens * 16;
+  for (int i = lane; i < tokens * 16; i += 64) mine[i] = 0.0f;
   __syncthreads();
   const int units = static_cast<int>(m.units);
-  const int64_t items = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(shared_n)) * units;
-  const int64_t run = SHARE == 1 ? wave : blockIdx.y, runs = SHARE == 1 ? 8 : gridDim.y;
-  const int64_t i0 = items * run / runs, i1 = items * (run + 1) / runs;
+  const int items = __builtin_amdgcn_readfirstlane(segments[0]) * units;
+  ++segments;
+  const int i0 = items * wave / 8, i1 = items * (wave + 1) / 8;
   const int c = lane & 15, q = lane >> 4;
   const float weight = ColumnWeight<ND, ONE, ZP>(lane);
-  const int64_t place = SHARE == 1 ? static_cast<int64_t>(blockIdx.x)
-                                   : static_cast<int64_t>(blockIdx.x) * 8 + wave;
-  const int64_t group = min(R == 2 ? place : place >> 1, m.groups - 1);
   if (i0 < i1) {
-    P pipe(lds + (SHARE == 1 ? wave * P::kLds : 0), lane, SHARE == 1 ? 0 : wave,
-           R == 2 ? 0 : static_cast<int>(place & 1));
+    P pipe(lds + wave * P::kLds, lane, 0, blockIdx.x & 1);
     // The next item to copy.
-    int next_seg = static_cast<int>(i0 / units), next_u = static_cast<int>(i0 % units);
-    const int last_seg = static_cast<int>((i1 - 1) / units);
-    const int last_u = static_cast<int>((i1 - 1) % units);
+    int next_seg = i0 / units, next_u = i0 % units;
+    const int last_seg = (i1 - 1) / units, last_u = (i1 - 1) % units;
     auto enter = [&](int seg) __attribute__((always_inline)) {
       const uint32_t s = __builtin_amdgcn_readfirstlane(segments[seg]);
-      pipe.Segment(m, s >> 20, group, fh, Count(s),
-                   [&](int i) { return static_cast<int64_t>(list[Offset(s) + i]); });
+      pipe.Segment(m, Expert(s), blockIdx.x >> 1, fh, Count(s),
+                   [&](int i) { return list[Offset(s) + i]; });
     };
     auto issue = [&](int stage) __attribute__((always_inline)) {
-      pipe.Issue(next_u, stage);
+      pipe.Issue(fh, next_u, stage);
       if (next_seg == last_seg && next_u == last_u) return;  // past the end: the last again
       if (++next_u == units) {
         next_u = 0;
@@ -747,90 +747,144 @@ __global__ __launch_bounds__(512) void MoeDownKernel(Matrix m, Fixed fh, Entries
 #pragma unroll
     for (int p = 0; p < NS - 1; ++p) issue(p);
     int stage = 0;
-    floatx4 acc[R][GC];
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-      for (int g = 0; g < GC; ++g) acc[r][g] = floatx4{0.f, 0.f, 0.f, 0.f};
-    uint32_t now = __builtin_amdgcn_readfirstlane(segments[seg]);
-    for (int64_t i = i0; i < i1; ++i) {
+    floatx4 acc[1][1] = {{floatx4{0.f, 0.f, 0.f, 0.f}}};
+    for (int i = i0; i < i1; ++i) {
       P::template Wait<P::kOps *(NS - 2)>();
       issue(stage == 0 ? NS - 1 : stage - 1);
-      const int n = Count(now);
-      pipe.Multiply(stage, (n + kT - 1) / kT, acc);
+      pipe.Multiply(stage, 1, acc);
       stage = stage + 1 == NS ? 0 : stage + 1;
       if (++u == units || i + 1 == i1) {
-        const int offset = Offset(now);
+        const uint32_t now = __builtin_amdgcn_readfirstlane(segments[seg]);
+        floatx4 y;
 #pragma unroll
-        for (int g = 0; g < GC; ++g) {
-          floatx4 y[R];
+        for (int v = 0; v < 4; ++v) y[v] = JoinDigits<ND, ONE>(acc[0][0][v] * weight);
+        acc[0][0] = floatx4{0.f, 0.f, 0.f, 0.f};
+        if (c < kT && c < Count(now)) {
+          const float p = weights[Offset(now) + c];
+          floatx4 *to = reinterpret_cast<floatx4 *>(mine + list[Offset(now) + c] / top_k * 16 + 4 * q);
+          floatx4 s = *to;
 #pragma unroll
-          for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              y[r][v] = JoinDigits<ND, ONE>(acc[r][g][v] * weight);
-              acc[r][g][v] = 0.0f;
-            }
-          const int j = g * kT + c;
-          if (c < kT && j < n) {
-            const float p = weights[offset + j];
-            float *to = mine + (list[offset + j] / top_k) * (R * 16) + 4 * q;
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-              floatx4 s = *reinterpret_cast<floatx4 *>(to + 16 * r);
-#pragma unroll
-              for (int v = 0; v < 4; ++v) s[v] = fmaf(p, y[r][v], s[v]);
-              *reinterpret_cast<floatx4 *>(to + 16 * r) = s;
-            }
-          }
+          for (int v = 0; v < 4; ++v) s[v] = fmaf(p, y[v], s[v]);
+          *to = s;
         }
-        if (u == units && i + 1 < i1) {
-          u = 0;
-          ++seg;
-          now = __builtin_amdgcn_readfirstlane(segments[seg]);
-        }
+        u = 0;
+        ++seg;
       }
     }
-    // No copy may land after the workgroup (every wavefront of a pipe is here).
-    P::template Wait<0>();
+    P::template Wait<0>();  // no copy may land after the workgroup
   }
   __syncthreads();
-  constexpr int kCols = R * 16;
-  if constexpr (SHARE == 1) {
-    for (int i = tid; i < tokens * kCols; i += 512) {
-      const int64_t n = static_cast<int64_t>(blockIdx.x) * kCols + i % kCols;
-      if (n >= H) continue;
-      float y = sums[i];
-      for (int w = 1; w < 8; ++w) y += sums[w * tokens * kCols + i];
-      Y[(i / kCols) * H + n] = static_cast<T>(y);
-    }
-  } else {
-    for (int i = tid; i < tokens * 8 * kCols; i += 512) {
-      const int t = i / (8 * kCols), w = i / kCols % 8;
-      const int64_t n = static_cast<int64_t>(blockIdx.x) * 8 * kCols + i % (8 * kCols);
-      if (n >= H) continue;
-      const float y = sums[(w * tokens + t) * kCols + i % kCols];
-      if (runs == 1) Y[t * H + n] = static_cast<T>(y);
-      else parts[(run * tokens + t) * H + n] = y;
-    }
+  for (int i = tid; i < tokens * 16; i += 512) {
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * 16 + (i & 15);
+    if (n >= H) continue;
+    float y = sums[i];
+    for (int w = 1; w < 8; ++w) y += sums[w * tokens * 16 + i];
+    Y[(i >> 4) * H + n] = static_cast<T>(y);
   }
 }
 
-// Y = the runs' sums, in order; a thread's loads of eight runs are in flight together.
+// Fourth launch: a workgroup takes 256 columns of Y and one run of the items: part
+// blockIdx.y % cuts of the units of one segment, or `many` whole segments (cuts = 1).
+// Every pair's row, times its weight, goes to parts [cuts][pairs][width].
+template <int ND, bool ONE, int GC, int F, bool ZP, int NS>
+__global__ __launch_bounds__(512) void MoeDownKernel(Matrix m, Fixed fh, Plan plan,
+                                                     float *__restrict__ parts, int pairs, int cuts,
+                                                     int many, int64_t width) {
+  using P = Pipe<ND, ONE, GC, 2, F, 1, ZP, 8, NS>;
+  constexpr int kT = P::kT;
+  extern __shared__ uint4 dynamic[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int total = __builtin_amdgcn_readfirstlane(plan.segment[0]);
+  const int cut = blockIdx.y % cuts, units = static_cast<int>(m.units);
+  int seg = blockIdx.y / cuts * many;
+  const int end = min(total, seg + many);
+  if (seg >= end) return;
+  const int u0 = units * cut / cuts, u1 = units * (cut + 1) / cuts;
+  if (u0 >= u1) return;
+  const int c = lane & 15, q = lane >> 4;
+  const float weight = ColumnWeight<ND, ONE, ZP>(lane);
+  const int64_t group = min(static_cast<int64_t>(blockIdx.x) * 8 + wave, m.groups - 1);
+  float *out = parts + static_cast<int64_t>(cut) * pairs * width +
+               static_cast<int64_t>(blockIdx.x) * 256 + wave * 32 + 4 * q;
+  P pipe(reinterpret_cast<const uint8_t *>(dynamic), lane, wave);
+  auto enter = [&](int s) __attribute__((always_inline)) {
+    const uint32_t w = __builtin_amdgcn_readfirstlane(plan.segment[1 + s]);
+    pipe.Segment(m, Expert(w), group, fh, Count(w),
+                 [&](int i) { return plan.pair[Offset(w) + i]; });
+  };
+  // The next item to copy.
+  int next_seg = seg, next_u = u0;
+  auto issue = [&](int stage) __attribute__((always_inline)) {
+    pipe.Issue(fh, next_u, stage);
+    if (next_u + 1 < u1) {
+      ++next_u;
+    } else if (next_seg + 1 < end) {
+      next_u = u0;
+      enter(++next_seg);
+    }  // past the end: the last again
+  };
+  enter(seg);
+#pragma unroll
+  for (int p = 0; p < NS - 1; ++p) issue(p);
+  int stage = 0;
+  for (; seg < end; ++seg) {
+    const uint32_t now = __builtin_amdgcn_readfirstlane(plan.segment[1 + seg]);
+    const int n = Count(now), groups = (n + kT - 1) / kT;
+    floatx4 acc[2][GC];
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int g = 0; g < GC; ++g) acc[r][g] = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int u = u0; u < u1; ++u) {
+      P::template Wait<P::kOps *(NS - 2)>();
+      issue(stage == 0 ? NS - 1 : stage - 1);
+      pipe.Multiply(stage, groups, acc);
+      stage = stage + 1 == NS ? 0 : stage + 1;
+    }
+#pragma unroll
+    for (int g = 0; g < GC; ++g) {
+      const int j = g * kT + c;
+      const bool on = c < kT && j < n;
+      const int at = Offset(now) + (on ? j : 0);
+      const float p = plan.weight[at];
+      float *to = out + plan.pair[at] * width;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        floatx4 y;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) y[v] = p * JoinDigits<ND, ONE>(acc[r][g][v] * weight);
+        if (on) *reinterpret_cast<floatx4 *>(to + 16 * r) = y;
+      }
+    }
+  }
+  P::template Wait<0>();  // no copy may land after the workgroup
+}
+
+// Y[t] = the sum of the parts of t's top_k pairs, in order; a thread's loads of
+// eight of them are in flight together.
 template <typename T>
 __global__ __launch_bounds__(256) void MoeSumKernel(const float *__restrict__ parts,
-                                                    T *__restrict__ Y, int64_t n, int runs) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= n) return;
+                                                    T *__restrict__ Y, int64_t H, int64_t width,
+                                                    int top_k, int pairs, int cuts) {
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int t = blockIdx.y;
+  if (n >= H) return;
+  const int terms = top_k * cuts;
   float y = 0.0f;
-  for (int r = 0; r < runs; r += 8) {
+  for (int i = 0; i < terms; i += 8) {
     float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = r + j < runs ? parts[(r + j) * n + i] : 0.0f;
+    for (int j = 0; j < 8; ++j) {
+      const int at = min(i + j, terms - 1);
+      const int64_t row = static_cast<int64_t>(at / top_k) * pairs + t * top_k + at % top_k;
+      v[j] = parts[row * width + n];
+    }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y += v[j];
+    for (int j = 0; j < 8; ++j)
+      if (i + j < terms) y += v[j];
   }
-  Y[i] = static_cast<T>(y);
+  Y[t * H + n] = static_cast<T>(y);
 }
 
 // ---- weight layout -----------------------------------------------------------------
@@ -908,7 +962,7 @@ struct Work {
   Fixed fx, fh;
   float *logits, *pair_weight, *parts;
   int32_t *pair_expert;
-  Entries entries;
+  Plan plan;
   size_t bytes;
 };
 
@@ -920,11 +974,13 @@ struct Shape {
   int entries;
   bool narrow;  // gate/up: 32 channels a workgroup, powers of two per 32 channels
   bool split;   // ... and the units over four wavefronts each
-  int runs;     // down: 0: one workgroup for 16 columns; else runs of the items
   bool choose;  // one token: the gate/up kernel makes its choice
+  int groups;   // column groups per pass over an expert's rows
+  int segments; // at most
+  int cuts, many;  // down: runs of 1 / cuts of a segment, or of `many` segments
 };
 
-Shape PickShape(const Layer &l, int tokens) {
+Shape PickShape(const Layer &l, int tokens, int ND) {
   Shape s;
   s.entries = std::min(tokens * l.top_k, l.experts);
   const int64_t blocks = s.entries * CeilDiv(l.intermediate, 128);  // of 128 channels
@@ -932,15 +988,22 @@ Shape PickShape(const Layer &l, int tokens) {
   s.split = s.narrow && 4 * blocks <= 2 * l.num_cus;
   // A workgroup's choice among more experts takes longer than a launch of its own.
   s.choose = tokens == 1 && l.experts <= 256;
-  s.runs = 0;
-  if (!s.narrow) {
-    const int64_t columns = CeilDiv(l.hidden, 256);
-    s.runs = static_cast<int>(std::max<int64_t>(1, CeilDiv(l.num_cus, columns)));
-    s.runs = static_cast<int>(
-        std::min<int64_t>(s.runs, std::max<int64_t>(1, s.entries * l.down.units / 4)));
-  }
+  // What most experts' tokens fill: their mean share and two standard deviations
+  // of even choices.
+  const int group = tokens == 1 ? 1 : ND == 3 ? kTokens<3> : kTokens<2>;
+  const double mean = static_cast<double>(tokens) * l.top_k / l.experts;
+  const double most = std::min<double>(tokens, mean + 2.0 * std::sqrt(mean));
+  s.groups = tokens <= kNarrowTokens || most <= group ? 1 : most <= 2 * group ? 2 : 4;
+  s.segments = s.entries + tokens * l.top_k / (s.groups * group);
+  // Down: about two workgroups a CU, of at least four units.
+  const double met = l.experts * (1.0 - std::pow(1.0 - static_cast<double>(l.top_k) / l.experts, tokens));
+  const double blocks_down = std::max(1.0, met) * CeilDiv(l.hidden, 256);
+  s.cuts = s.many = 1;
+  while (blocks_down * s.cuts < 1.5 * l.num_cus && l.down.units >= 8 * s.cuts && s.cuts < 8) s.cuts *= 2;
   return s;
 }
+
+int64_t PartWidth(const Layer &l) { return CeilDiv(l.hidden, 256) * 256; }
 
 Work Split(const Layer &l, int T, int ND, void *base) {
   Work w;
@@ -951,7 +1014,7 @@ Work Split(const Layer &l, int T, int ND, void *base) {
     return p;
   };
   const size_t pairs = static_cast<size_t>(T) * l.top_k;
-  const Shape shape = PickShape(l, T);
+  const Shape shape = PickShape(l, T, ND);
   auto fixed = [&](size_t rows, int64_t units, int scales) {
     Fixed f;
     f.units = units;
@@ -965,13 +1028,11 @@ Work Split(const Layer &l, int T, int ND, void *base) {
   w.logits = reinterpret_cast<float *>(take(static_cast<size_t>(T) * l.experts * 4));
   w.pair_expert = reinterpret_cast<int32_t *>(take(pairs * 4));
   w.pair_weight = reinterpret_cast<float *>(take(pairs * 4));
-  w.entries.expert = reinterpret_cast<int32_t *>(take(shape.entries * 4));
-  w.entries.count = reinterpret_cast<int32_t *>(take(shape.entries * 4));
-  w.entries.offset = reinterpret_cast<int32_t *>(take(shape.entries * 4));
-  w.entries.pair = reinterpret_cast<int32_t *>(take(pairs * 4));
-  w.entries.weight = reinterpret_cast<float *>(take(pairs * 4));
+  w.plan.pair = reinterpret_cast<int32_t *>(take(pairs * 4));
+  w.plan.weight = reinterpret_cast<float *>(take(pairs * 4));
+  w.plan.segment = reinterpret_cast<uint32_t *>(take((shape.segments + 1) * 4));
   w.parts = reinterpret_cast<float *>(
-      take(shape.runs > 1 ? static_cast<size_t>(shape.runs) * T * l.hidden * 4 : 0));
+      take(shape.narrow ? 0 : static_cast<size_t>(shape.cuts) * pairs * PartWidth(l) * 4));
   w.bytes = at;
   return w;
 }
@@ -979,37 +1040,47 @@ Work Split(const Layer &l, int T, int ND, void *base) {
 template <int ND, bool ONE, int GC, int F, bool ZP, int GROUPS, int KS, bool CHOOSE>
 hipError_t LaunchGateUp(const Layer &l, const Work &w, const Shape &shape, int pairs,
                         const Choice &choice, hipStream_t s) {
-  constexpr int NS = KS > 1 ? (ONE ? 4 : 3) : GC == 4 ? (F == 8 ? 3 : 4) : 3;
+  constexpr int NS = KS > 1 && ONE ? 4 : 3;
   using P = Pipe<ND, ONE, GC, 2, F, 1, ZP, KS == 1 ? GROUPS : 1, NS>;
   const dim3 grid(static_cast<unsigned>(l.gate_up.groups / GROUPS),
-                  static_cast<unsigned>(shape.entries));
+                  static_cast<unsigned>(shape.entries + (CHOOSE ? 0 : 1)));
   hipLaunchKernelGGL((MoeGateUpKernel<ND, ONE, GC, F, ZP, GROUPS, KS, NS, CHOOSE>), grid,
                      dim3(64 * GROUPS * KS), (KS == 1 ? 1 : GROUPS * KS) * P::kLds, s, l.gate_up,
-                     w.fx, w.fh, w.pair_expert, w.pair_weight, w.entries, pairs, l.top_k,
+                     w.fx, w.fh, w.pair_expert, w.pair_weight, w.plan, pairs, l.top_k,
                      pairs >= l.experts, choice);
   return hipGetLastError();
 }
 
-template <int ND, bool ONE, int GC, int F, int XB, bool ZP, int SHARE, typename T>
+template <int ND, bool ONE, int F, bool ZP, typename T>
+hipError_t LaunchDownNarrow(const Layer &l, const Work &w, const Shape &shape, int tokens, T *Y,
+                            hipStream_t s) {
+  constexpr int NS = ONE ? 5 : 3;
+  using P = Pipe<ND, ONE, 1, 1, F, 4, ZP, 1, NS>;
+  const int pairs = tokens * l.top_k;
+  const size_t lds = static_cast<size_t>(8) * P::kLds + 8 * tokens * 16 * sizeof(float) + pairs * 6 +
+                     (shape.segments + 1) * 4;
+  hipLaunchKernelGGL((MoeDownNarrowKernel<ND, ONE, F, ZP, NS, T>),
+                     dim3(static_cast<unsigned>(2 * l.down.groups)), dim3(512), lds, s, l.down, w.fh,
+                     w.plan, Y, pairs, shape.segments, tokens, l.top_k, l.hidden);
+  return hipGetLastError();
+}
+
+template <int ND, bool ONE, int GC, int F, bool ZP, typename T>
 hipError_t LaunchDown(const Layer &l, const Work &w, const Shape &shape, int tokens, T *Y,
                       hipStream_t s) {
-  constexpr int R = SHARE == 1 ? 1 : 2;
-  constexpr int NS = SHARE == 1 ? (ONE ? 5 : 3) : F == 8 || (GC == 4 && F == 4) ? 2 : 3;
-  using P = Pipe<ND, ONE, GC, R, F, XB, ZP, SHARE, NS>;
+  constexpr int NS = 3;
+  using P = Pipe<ND, ONE, GC, 2, F, 1, ZP, 8, NS>;
   const int pairs = tokens * l.top_k;
-  const int segments = shape.entries + pairs / (GC * P::kT);
-  const size_t lds = static_cast<size_t>(8 / SHARE) * P::kLds + 8 * tokens * R * 16 * sizeof(float) +
-                     pairs * 6 + segments * 4;
-  const int64_t blocks = SHARE == 1 ? 2 * l.down.groups : CeilDiv(l.down.groups, SHARE);
-  hipLaunchKernelGGL((MoeDownKernel<ND, ONE, GC, R, F, XB, ZP, SHARE, NS, T>),
-                     dim3(static_cast<unsigned>(blocks), std::max(1, shape.runs)), dim3(512), lds, s,
-                     l.down, w.fh, w.entries, Y, w.parts, shape.entries, pairs, segments, tokens,
-                     l.top_k, l.hidden);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || shape.runs <= 1) return e;
-  const int64_t n = tokens * l.hidden;
-  hipLaunchKernelGGL((MoeSumKernel<T>), dim3(static_cast<unsigned>(CeilDiv(n, 256))), dim3(256), 0,
-                     s, w.parts, Y, n, shape.runs);
+  const int64_t width = PartWidth(l);
+  const dim3 grid(static_cast<unsigned>(width / 256),
+                  static_cast<unsigned>(CeilDiv(shape.segments, shape.many) * shape.cuts));
+  hipLaunchKernelGGL((MoeDownKernel<ND, ONE, GC, F, ZP, NS>), grid, dim3(512), P::kLds, s, l.down,
+                     w.fh, w.plan, w.parts, pairs, shape.cuts, shape.many, width);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((MoeSumKernel<T>),
+                     dim3(static_cast<unsigned>(CeilDiv(l.hidden, 256)), static_cast<unsigned>(tokens)),
+                     dim3(256), 0, s, w.parts, Y, l.hidden, width, l.top_k, pairs, shape.cuts);
   return hipGetLastError();
 }
 
@@ -1032,11 +1103,11 @@ hipError_t LaunchExperts(const Layer &l, const Work &w, const Shape &shape, int 
     if (shape.narrow) {
       if (shape.split) e = LaunchGateUpC<ND, ONE, GC, F, ZP, 2, 4>(l, w, shape, pairs, choice, s);
       else e = LaunchGateUpC<ND, ONE, GC, F, ZP, 2, 1>(l, w, shape, pairs, choice, s);
-      return e != hipSuccess ? e : LaunchDown<ND, ONE, GC, F, 4, ZP, 1, T>(l, w, shape, tokens, Y, s);
+      return e != hipSuccess ? e : LaunchDownNarrow<ND, ONE, F, ZP, T>(l, w, shape, tokens, Y, s);
     }
   }
   e = LaunchGateUpC<ND, ONE, GC, F, ZP, 8, 1>(l, w, shape, pairs, choice, s);
-  return e != hipSuccess ? e : LaunchDown<ND, ONE, GC, F, 1, ZP, 8, T>(l, w, shape, tokens, Y, s);
+  return e != hipSuccess ? e : LaunchDown<ND, ONE, GC, F, ZP, T>(l, w, shape, tokens, Y, s);
 }
 
 template <int ND, bool ONE, int GC, bool ZP, typename T>
@@ -1072,7 +1143,7 @@ hipError_t LaunchLayerT(const Layer &l, int tokens, const void *X, const float *
   else vec ? launch_prep(Several{}, std::true_type{}) : launch_prep(Several{}, std::false_type{});
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const Shape shape = PickShape(l, tokens);
+  const Shape shape = PickShape(l, tokens, ND);
   const Choice choice{logits ? logits : w.logits, ids, weights, l.experts, l.normalize};
   if (!shape.choose) {
     hipLaunchKernelGGL(MoeRouteKernel, dim3(static_cast<unsigned>(tokens)), dim3(256), 0, s,
@@ -1082,11 +1153,6 @@ hipError_t LaunchLayerT(const Layer &l, int tokens, const void *X, const float *
     if (e != hipSuccess) return e;
   }
   T *y = static_cast<T *>(Y);
-  // Column groups per pass over an expert's rows: what most experts' tokens fill,
-  // their mean share and two standard deviations of even choices.
-  const double mean = static_cast<double>(tokens) * l.top_k / l.experts;
-  const double most = std::min<double>(tokens, mean + 2.0 * std::sqrt(mean));
-  const int gc = tokens <= kNarrowTokens || most <= kTokens<ND> ? 1 : most <= 2 * kTokens<ND> ? 2 : 4;
   auto experts = [&](auto groups, auto one) {
     constexpr int GC = decltype(groups)::value;
     constexpr bool kOne = decltype(one)::value;
@@ -1094,7 +1160,7 @@ hipError_t LaunchLayerT(const Layer &l, int tokens, const void *X, const float *
                    : LaunchFolds<ND, kOne, GC, false, T>(l, w, shape, tokens, y, choice, s);
   };
   if (tokens == 1) return experts(std::integral_constant<int, 1>{}, std::true_type{});
-  switch (gc) {
+  switch (shape.groups) {
   case 1: return experts(std::integral_constant<int, 1>{}, std::false_type{});
   case 2: return experts(std::integral_constant<int, 2>{}, std::false_type{});
   default: return experts(std::integral_constant<int, 4>{}, std::false_type{});

@@ -37,7 +37,7 @@ void FreePlan(mnb_moe_plan *p) {
   delete p;
 }
 
-constexpr int64_t kMaxWidth = int64_t{1} << 20;
+constexpr int64_t kMaxWidth = int64_t{1} << 18;  // fixed-point offsets stay below 2^31
 constexpr int64_t kMaxMatrix = int64_t{1} << 34;
 constexpr int64_t kMaxRun = int64_t{1} << 24;
 
