@@ -165,14 +165,12 @@ __device__ __forceinline__ uint32_t Key(float l) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// A token's choice, by all THREADS of a workgroup: best[i] and who[i] (i < k) the
-// i-th largest logit and its expert; returns what the weights expf(best[i] -
-// best[0]) are divided by. An expert's place is the number of experts before it, by
-// key and then by index.
+// The first k experts of a token, by all THREADS of a workgroup: best[i] and who[i]
+// the i-th largest logit and its expert. An expert's place is the number of experts
+// before it, by key and then by index.
 template <int THREADS>
-__device__ __forceinline__ float Choose(const float *__restrict__ l, int E, int k, bool normalize,
-                                        uint32_t *key, float *best, int32_t *who) {
-  __shared__ float red[THREADS / 64];
+__device__ __forceinline__ void Choose(const float *__restrict__ l, int E, int k, uint32_t *key,
+                                       float *best, int32_t *who) {
   const int tid = threadIdx.x;
   const int padded = (E + 3) & ~3;
   // -0 and 0 are equal logits; key 0 is below every logit's.
@@ -182,7 +180,7 @@ __device__ __forceinline__ float Choose(const float *__restrict__ l, int E, int 
   for (int e = tid; e < E; e += THREADS) {
     const uint32_t me = key[e];
     int place = 0;
-#pragma unroll 4
+#pragma unroll 8
     for (int j = 0; j < padded / 4; ++j) {
       const uint4 v = key4[j];
       // Before e equal keys count too: they exceed me - 1 (keys are above 0).
@@ -193,24 +191,33 @@ __device__ __forceinline__ float Choose(const float *__restrict__ l, int E, int 
       place += v.w > me - (at + 3 < e ? 1u : 0u) ? 1 : 0;
     }
     if (place < k) {
-      best[place] = l[e] != l[e] ? -__builtin_inff() : l[e];
+      best[place] = __uint_as_float(me & 0x80000000u ? me & 0x7FFFFFFFu : ~me);
       who[place] = e;
     }
   }
   __syncthreads();
+}
+
+// What the weights expf(best[i] - best[0]) are divided by: the sum over the chosen,
+// or over all; by all THREADS.
+template <int THREADS>
+__device__ __forceinline__ float WeightSum(const float *__restrict__ l, int E, int k, bool normalize,
+                                           const float *best) {
+  __shared__ float red[THREADS / 64];
+  const int tid = threadIdx.x;
   const float top = best[0];
   float total = 0.0f;
   if (normalize) {
     for (int j = 0; j < k; ++j) total += expf(best[j] - top);
-  } else {
-    float s = 0.0f;
-    for (int e = tid; e < E; e += THREADS)
-      s += expf((l[e] != l[e] ? -__builtin_inff() : l[e]) - top);
-    for (int off = 32; off >= 1; off >>= 1) s += __shfl_xor(s, off, 64);
-    if ((tid & 63) == 0) red[tid >> 6] = s;
-    __syncthreads();
-    for (int w = 0; w < THREADS / 64; ++w) total += red[w];
+    return total;
   }
+  float s = 0.0f;
+  for (int e = tid; e < E; e += THREADS)
+    s += expf((l[e] != l[e] ? -__builtin_inff() : l[e]) - top);
+  for (int off = 32; off >= 1; off >>= 1) s += __shfl_xor(s, off, 64);
+  if ((tid & 63) == 0) red[tid >> 6] = s;
+  __syncthreads();
+  for (int w = 0; w < THREADS / 64; ++w) total += red[w];
   return total;
 }
 
@@ -223,8 +230,9 @@ __global__ __launch_bounds__(256) void MoeRouteKernel(const float *__restrict__ 
   __shared__ float best[kMaxTopK];
   __shared__ int32_t who[kMaxTopK];
   const int tid = threadIdx.x, t = blockIdx.x;
-  const float total = Choose<256>(logits + static_cast<int64_t>(t) * E, E, k, normalize,
-                                  reinterpret_cast<uint32_t *>(key), best, who);
+  const float *l = logits + static_cast<int64_t>(t) * E;
+  Choose<256>(l, E, k, reinterpret_cast<uint32_t *>(key), best, who);
+  const float total = WeightSum<256>(l, E, k, normalize, best);
   if (tid < k) {
     const float p = expf(best[tid] - best[0]) / total;
     pair_expert[t * k + tid] = who[tid];
@@ -395,7 +403,7 @@ struct Pipe {
                                                          (q * F + f) * 16);
 #pragma unroll
     for (int g = 0; g < GC; ++g) {
-      if (GC > 1 && g >= groups) break;
+      if (GC > 1 && g >= groups) continue;
       const uint8_t *dig = st + kDigits + 2 * g * kRec + (q * kCols + min(c, kCols - 1)) * 16;
       const intx4 b0 = *reinterpret_cast<const intx4 *>(dig);
       const intx4 b1 = *reinterpret_cast<const intx4 *>(dig + kCols * 64);
@@ -445,6 +453,8 @@ struct Pipe {
               acc[r][g][v] = fmaf(part[v], power[f / (kFolds / XB)], acc[r][g][v]);
           }
         }
+        // One record's sums at a time where all at once would cost a workgroup's registers.
+        if constexpr (GC > 1 && kFolds >= 2) __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -550,11 +560,17 @@ struct Choice {
   bool normalize;
 };
 
+// Wavefronts per SIMD that the registers are to leave room for: three workgroups of
+// eight a CU for one column group, two for several, one where two would spill.
+constexpr int WavesPerSimd(int gc, int folds) {
+  return gc * folds >= 16 ? 2 : gc > 1 || folds == 8 ? 4 : 6;
+}
+
 // Third launch: workgroup (b, i) the channels of block b of entry i's expert, 16
 // (gate and up) for each of GROUPS wavefronts that share a pipe, or, with KS runs
 // of the units, for each of GROUPS * KS wavefronts with pipes of their own.
 template <int ND, bool ONE, int GC, int F, bool ZP, int GROUPS, int KS, int NS, bool CHOOSE>
-__global__ __launch_bounds__(64 * GROUPS *KS) void MoeGateUpKernel(
+__global__ __launch_bounds__(64 * GROUPS *KS, GROUPS == 8 ? WavesPerSimd(GC, F) : 1) void MoeGateUpKernel(
     Matrix m, Fixed fx, Fixed fh, const int32_t *__restrict__ pair_expert,
     const float *__restrict__ pair_weight, Plan plan, int pairs, int top_k, bool by_expert,
     Choice choice) {
@@ -574,13 +590,13 @@ __global__ __launch_bounds__(64 * GROUPS *KS) void MoeGateUpKernel(
     __shared__ float best[kMaxTopK];
     __shared__ int32_t who[kMaxTopK];
     static_assert(kPipes * P::kLds >= kMaxExperts * 4, "the keys use the pipes' LDS");
-    const float total = Choose<64 * kWaves>(choice.logits, choice.experts, top_k, choice.normalize,
-                                            reinterpret_cast<uint32_t *>(dynamic), best, who);
+    Choose<64 * kWaves>(choice.logits, choice.experts, top_k, reinterpret_cast<uint32_t *>(dynamic),
+                        best, who);
     e = __builtin_amdgcn_readfirstlane(who[entry]);
-    if (tid == 0) {
-      list[0] = entry;
-      shared_n = 1;
-      if (blockIdx.x == 0) {
+    if (blockIdx.x == 0) {
+      const float total = WeightSum<64 * kWaves>(choice.logits, choice.experts, top_k,
+                                                 choice.normalize, best);
+      if (tid == 0) {
         const float p = expf(best[entry] - best[0]) / total;
         plan.pair[entry] = entry;
         plan.weight[entry] = p;
@@ -589,6 +605,10 @@ __global__ __launch_bounds__(64 * GROUPS *KS) void MoeGateUpKernel(
         if (choice.ids) choice.ids[entry] = e;
         if (choice.weights) choice.weights[entry] = p;
       }
+    }
+    if (tid == 0) {
+      list[0] = entry;
+      shared_n = 1;
     }
   } else {
     if (entry == static_cast<int>(gridDim.y) - 1) {  // the last row's first workgroup
@@ -787,7 +807,7 @@ __global__ __launch_bounds__(512) void MoeDownNarrowKernel(Matrix m, Fixed fh, P
 // blockIdx.y % cuts of the units of one segment, or `many` whole segments (cuts = 1).
 // Every pair's row, times its weight, goes to parts [cuts][pairs][width].
 template <int ND, bool ONE, int GC, int F, bool ZP, int NS>
-__global__ __launch_bounds__(512) void MoeDownKernel(Matrix m, Fixed fh, Plan plan,
+__global__ __launch_bounds__(512, WavesPerSimd(GC, F)) void MoeDownKernel(Matrix m, Fixed fh, Plan plan,
                                                      float *__restrict__ parts, int pairs, int cuts,
                                                      int many, int64_t width) {
   using P = Pipe<ND, ONE, GC, 2, F, 1, ZP, 8, NS>;
@@ -993,7 +1013,10 @@ Shape PickShape(const Layer &l, int tokens, int ND) {
   const int group = tokens == 1 ? 1 : ND == 3 ? kTokens<3> : kTokens<2>;
   const double mean = static_cast<double>(tokens) * l.top_k / l.experts;
   const double most = std::min<double>(tokens, mean + 2.0 * std::sqrt(mean));
-  s.groups = tokens <= kNarrowTokens || most <= group ? 1 : most <= 2 * group ? 2 : 4;
+  // Four groups of 16-wide blocks would not fit the registers.
+  s.groups = tokens <= kNarrowTokens || most <= group ? 1
+             : most <= 2 * group || l.folds == 8     ? 2
+                                                     : 4;
   s.segments = s.entries + tokens * l.top_k / (s.groups * group);
   // Down: about two workgroups a CU, of at least four units.
   const double met = l.experts * (1.0 - std::pow(1.0 - static_cast<double>(l.top_k) / l.experts, tokens));
@@ -1040,7 +1063,7 @@ Work Split(const Layer &l, int T, int ND, void *base) {
 template <int ND, bool ONE, int GC, int F, bool ZP, int GROUPS, int KS, bool CHOOSE>
 hipError_t LaunchGateUp(const Layer &l, const Work &w, const Shape &shape, int pairs,
                         const Choice &choice, hipStream_t s) {
-  constexpr int NS = KS > 1 && ONE ? 4 : 3;
+  constexpr int NS = KS > 1 && ONE ? 4 : GC == 1 && GROUPS == 8 ? 2 : 3;
   using P = Pipe<ND, ONE, GC, 2, F, 1, ZP, KS == 1 ? GROUPS : 1, NS>;
   const dim3 grid(static_cast<unsigned>(l.gate_up.groups / GROUPS),
                   static_cast<unsigned>(shape.entries + (CHOOSE ? 0 : 1)));
@@ -1068,7 +1091,7 @@ hipError_t LaunchDownNarrow(const Layer &l, const Work &w, const Shape &shape, i
 template <int ND, bool ONE, int GC, int F, bool ZP, typename T>
 hipError_t LaunchDown(const Layer &l, const Work &w, const Shape &shape, int tokens, T *Y,
                       hipStream_t s) {
-  constexpr int NS = 3;
+  constexpr int NS = GC == 1 ? 2 : 3;
   using P = Pipe<ND, ONE, GC, 2, F, 1, ZP, 8, NS>;
   const int pairs = tokens * l.top_k;
   const int64_t width = PartWidth(l);
@@ -1117,8 +1140,10 @@ hipError_t LaunchFolds(const Layer &l, const Work &w, const Shape &shape, int to
   case 1: return LaunchExperts<ND, ONE, GC, 1, ZP, T>(l, w, shape, tokens, Y, choice, s);
   case 2: return LaunchExperts<ND, ONE, GC, 2, ZP, T>(l, w, shape, tokens, Y, choice, s);
   case 4: return LaunchExperts<ND, ONE, GC, 4, ZP, T>(l, w, shape, tokens, Y, choice, s);
-  default: return LaunchExperts<ND, ONE, GC, 8, ZP, T>(l, w, shape, tokens, Y, choice, s);
+  default: break;
   }
+  if constexpr (GC < 4) return LaunchExperts<ND, ONE, GC, 8, ZP, T>(l, w, shape, tokens, Y, choice, s);
+  else return hipErrorInvalidValue;  // PickShape gives eight folds no four groups
 }
 
 template <typename T>
