@@ -66,6 +66,19 @@ __device__ __forceinline__ floatx4 Mfma(const Fragment<true> &w, const Fragment<
   return p;
 }
 
+// Workgroup -> tile: an XCD (blockIdx % 8) takes a contiguous run of an order that
+// walks groups of 4 row tiles column tile by column tile.
+__device__ __forceinline__ void TileOf(int L, int tiles_m, int tiles_n, int &tm, int &tn) {
+  const int tiles = tiles_m * tiles_n;
+  if (tiles % 8 == 0) L = (L & 7) * (tiles / 8) + (L >> 3);
+  constexpr int kGM = 4;
+  const int group = L / (kGM * tiles_n);
+  const int gm = min(kGM, tiles_m - group * kGM);
+  const int rem = L - group * kGM * tiles_n;
+  tm = group * kGM + rem % gm;
+  tn = rem / gm;
+}
+
 // n (up to C) consecutive values of a row of Y; whole: all C, at an address
 // that 16 bytes (or the C values) divide.
 template <typename T, int C>
@@ -201,20 +214,8 @@ __global__ __launch_bounds__(64 * WM *WN) void Fp8TileKernel(
   const int c = lane & 15, qd = lane >> 4;
   const int wm = wave % WM, wn = wave / WM;
 
-  // Workgroup -> tile: an XCD (blockIdx % 8) takes a contiguous run of an order
-  // that walks groups of 4 row tiles column tile by column tile.
   int tm, tn;
-  {
-    const int tiles = tiles_m * tiles_n;
-    int L = static_cast<int>(blockIdx.x);
-    if (tiles % 8 == 0) L = (L & 7) * (tiles / 8) + (L >> 3);
-    constexpr int kGM = 4;
-    const int group = L / (kGM * tiles_n);
-    const int gm = min(kGM, tiles_m - group * kGM);
-    const int rem = L - group * kGM * tiles_n;
-    tm = group * kGM + rem % gm;
-    tn = rem / gm;
-  }
+  TileOf(static_cast<int>(blockIdx.x), tiles_m, tiles_n, tm, tn);
   const int b0 = static_cast<int>(blockIdx.y) * per_split;
   const int b1 = min(nb, b0 + per_split);
   Y += static_cast<int64_t>(blockIdx.y) * M * N;
@@ -308,6 +309,168 @@ __global__ __launch_bounds__(64 * WM *WN) void Fp8TileKernel(
   }
 }
 
+// ---- many rows, 16-bit Y: 256 x 256 tiles ---------------------------------------
+//
+// Eight wavefronts, two per SIMD, of 8 x 4 fragments. A block of K is 32 slots,
+// one MFMA each; between them go the fold of two slots before (its products have
+// left the matrix unit by then), the LDS reads of the next group and the copies
+// of the tile after next, in an order that sched_barrier keeps. The barrier that
+// makes the next tile visible stands before the last group, when this tile's
+// reads are done: the next tile's weight fragments are read in place, each
+// behind its last MFMA, so that the matrix unit does not wait at the block's end
+// (with the barrier between the blocks: 604 us at 8192 x 4096 x 14336).
+constexpr int kWideTile = 256;
+
+template <typename T>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void Fp8WideKernel(
+    const uint8_t *__restrict__ W, const float *__restrict__ SW, const uint8_t *__restrict__ A,
+    const float *__restrict__ SA, T *__restrict__ Y, int64_t M, int64_t N, int64_t lda, int nb,
+    int tiles_m, int tiles_n, int groups) {
+  constexpr int MI = 8, NJ = 4, WM = 2, WN = 4, kWaves = 8;
+  constexpr int kARecs = 32, kWRecs = 32;
+  constexpr int kStage = (kARecs + kWRecs) * kRec + 256 * kWaves;  // bytes; row scales last
+  extern __shared__ uint8_t lds[];
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int c = lane & 15, qd = lane >> 4;
+  const int wm = wave % WM, wn = wave / WM;
+  int tm, tn;
+  TileOf(static_cast<int>(blockIdx.x), tiles_m, tiles_n, tm, tn);
+  const int64_t m0 = static_cast<int64_t>(tm) * kWideTile;
+  const int64_t rows = min(M - m0, static_cast<int64_t>(kWideTile));
+  const int last_row = static_cast<int>(rows) - 1;
+
+  uint32_t a_off[4];
+  const uint8_t *w_src[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int rec = i * kWaves + wave;
+    a_off[i] = static_cast<uint32_t>(min(16 * (rec >> 1) + c, last_row) * lda + 64 * (rec & 1) + 16 * qd);
+    const int64_t g = min(static_cast<int64_t>(tn) * WN + (rec >> 3), static_cast<int64_t>(groups) - 1);
+    w_src[i] = W + (g * nb * 8 + (rec & 7)) * kRec;
+  }
+  const uint8_t *a_base = A + m0 * lda;
+  const uint32_t s_off = static_cast<uint32_t>(min(static_cast<int>(threadIdx.x), last_row) * nb * 4);
+  const float *sa_base = SA + m0 * nb;
+  const uint32_t l16 = static_cast<uint32_t>(lane) * 16;
+  // Copy n (0 .. 8) of block b into the stage at byte st.
+  auto copy = [&](auto nc, int b, uint32_t st) __attribute__((always_inline)) {
+    constexpr int n = decltype(nc)::value;
+    if constexpr (n < 4)
+      CopyToLds16S(a_base + static_cast<int64_t>(b) * kBlock, a_off[n],
+                   lds0 + st + (n * kWaves + wave) * kRec);
+    else if constexpr (n < 8)
+      CopyToLds16S(w_src[n - 4] + static_cast<int64_t>(b) * 8 * kRec, l16,
+                   lds0 + st + (kARecs + (n - 4) * kWaves + wave) * kRec);
+    else
+      CopyToLds4S(sa_base + b, s_off, lds0 + st + (kARecs + kWRecs) * kRec + wave * 256);
+  };
+  auto issue = [&](int b, uint32_t st) __attribute__((always_inline)) {
+    [&]<int... n>(std::integer_sequence<int, n...>) __attribute__((always_inline)) {
+      (copy(std::integral_constant<int, n>{}, b, st), ...);
+    }(std::make_integer_sequence<int, 9>{});
+  };
+  const uint8_t *a_at = lds + wm * MI * 2 * kRec + lane * 16;
+  const uint8_t *w_at = lds + (kARecs + wn * 8) * kRec + lane * 16;
+  const uint8_t *s_at = lds + (kARecs + kWRecs) * kRec + (wm * MI * 16 + c) * 4;
+  auto readA = [&](uint32_t st, int i) __attribute__((always_inline)) {
+    const uint8_t *p = a_at + st + 2 * i * kRec;
+    return Fragment<false>(*reinterpret_cast<const intx4 *>(p),
+                           *reinterpret_cast<const intx4 *>(p + kRec)).v;
+  };
+  auto readW = [&](uint32_t st, int j) __attribute__((always_inline)) {
+    const uint8_t *p = w_at + st + 2 * j * kRec;
+    return Fragment<false>(*reinterpret_cast<const intx4 *>(p),
+                           *reinterpret_cast<const intx4 *>(p + kRec)).v;
+  };
+  auto readS = [&](uint32_t st, int i) __attribute__((always_inline)) {
+    return *reinterpret_cast<const float *>(s_at + st + 64 * i);
+  };
+
+  floatx4 acc[MI][NJ], part[4];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int v = 0; v < 4; ++v) part[v] = floatx4{0.f, 0.f, 0.f, 0.f};
+  const int last = nb - 1;
+  const float *sw = SW + (min(static_cast<int64_t>(tn) * WN + wn, static_cast<int64_t>(groups) - 1) >> 1) * nb;
+  issue(0, 0);
+  WaitBarrier<0>();
+  issue(min(1, last), kStage);
+  intx8 wf[NJ], af[2];
+  float f[2], scale = sw[0];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) wf[j] = readW(0, j);
+  af[0] = readA(0, 0);
+  f[0] = readS(0, 0) * scale;
+  f[1] = 0.0f;
+
+  auto fold = [&](auto kc) __attribute__((always_inline)) {  // slot k of a block
+    constexpr int k = decltype(kc)::value, i = k / NJ, j = k % NJ;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) acc[i][j][v] = fmaf(part[k % 4][v], f[i % 2], acc[i][j][v]);
+  };
+  constexpr int kSlots = MI * NJ;
+  for (int b = 0; b < nb; ++b) {
+    const uint32_t st = (b & 1) * kStage, other = kStage - st;
+    const float next_scale = sw[min(b + 1, last)];
+    float s_next = 0.0f;
+    auto slot = [&](auto kc) __attribute__((always_inline)) {
+      constexpr int k = decltype(kc)::value, i = k / NJ, j = k % NJ;
+      if constexpr (k == kSlots - NJ) {
+        WaitBarrier<0>();  // block b + 1 is in LDS, block b's reads are done
+      }
+      part[k % 4] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+          wf[j], af[i % 2], floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+      if constexpr (i + 1 < MI) {
+        if constexpr (j == 0) af[(i + 1) % 2] = readA(st, i + 1);
+        if constexpr (j == 1) s_next = readS(st, i + 1);
+      } else {
+        if constexpr (j == 0) af[(i + 1) % 2] = readA(other, 0);
+        if constexpr (j == 1) s_next = readS(other, 0);
+        wf[j] = readW(other, j);
+      }
+      // Two slots back; the first two of a block are the last ones of the block
+      // before (of its products with f[1], still there).
+      if constexpr (k >= 2) fold(std::integral_constant<int, k - 2>{});
+      else fold(std::integral_constant<int, kSlots - 2 + k>{});
+      // The factor of group i + 1 takes the place of group i - 1's after its last fold.
+      if constexpr (j == 3) f[(i + 1) % 2] = s_next * (i + 1 < MI ? scale : next_scale);
+      // Block b + 2 into the stage that block b has left.
+      if constexpr (k >= kSlots - NJ) copy(std::integral_constant<int, k - (kSlots - NJ)>{}, min(b + 2, last), st);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    [&]<int... k>(std::integer_sequence<int, k...>) __attribute__((always_inline)) {
+      (slot(std::integral_constant<int, k>{}), ...);
+    }(std::make_integer_sequence<int, kSlots>{});
+    [&]<int... n>(std::integer_sequence<int, n...>) __attribute__((always_inline)) {
+      (copy(std::integral_constant<int, 4 + n>{}, min(b + 2, last), st), ...);
+    }(std::make_integer_sequence<int, 5>{});
+    scale = next_scale;
+  }
+  fold(std::integral_constant<int, kSlots - 2>{});
+  fold(std::integral_constant<int, kSlots - 1>{});
+  WaitBarrier<0>();  // no copy may land after this workgroup
+
+  const int64_t n = (static_cast<int64_t>(tn) * WN + wn) * 64 + 16 * qd;
+  const bool whole = n + 16 <= N && (N * static_cast<int64_t>(sizeof(T))) % 16 == 0;
+  if (n < N) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int64_t row = 16 * (wm * MI + i) + c;
+      float v[16];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[4 * j + u] = acc[i][j][u];
+      if (row < rows) StoreRow<T, 16>(Y + (m0 + row) * N + n, v, N - n, whole);
+    }
+  }
+}
+
 // Y = the sum of S partial products, in order.
 template <typename T>
 __global__ __launch_bounds__(256) void Fp8SumKernel(const float *__restrict__ P, T *__restrict__ Y,
@@ -369,7 +532,18 @@ hipError_t TileLaunch(const Weight &w, const TileShape &t, int64_t M, const uint
 template <bool EXACT, typename T>
 hipError_t TileT(const Weight &w, const TileShape &t, int64_t M, const uint8_t *A, int64_t lda,
                  const float *sa, T *Y, hipStream_t s) {
-  if (t.rows == 256) return TileLaunch<8, 2, 4, 2, EXACT, T>(w, t, M, A, lda, sa, Y, s);
+  if (t.rows == 256) {
+    if constexpr (EXACT) {
+      return TileLaunch<8, 2, 4, 2, EXACT, T>(w, t, M, A, lda, sa, Y, s);
+    } else {
+      const int64_t tiles_m = CeilDiv(M, 256), tiles_n = CeilDiv(w.N, 256);
+      hipLaunchKernelGGL((Fp8WideKernel<T>), dim3(static_cast<unsigned>(tiles_m * tiles_n)),
+                         dim3(512), 2 * (64 * kRec + 2048), s, w.W, w.scales, A, sa, Y, M, w.N, lda,
+                         static_cast<int>(w.nb), static_cast<int>(tiles_m),
+                         static_cast<int>(tiles_n), static_cast<int>(w.groups));
+      return hipGetLastError();
+    }
+  }
   return TileLaunch<4, 2, 2, 3, EXACT, T>(w, t, M, A, lda, sa, Y, s);
 }
 
