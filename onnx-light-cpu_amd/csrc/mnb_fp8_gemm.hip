@@ -314,11 +314,20 @@ __global__ __launch_bounds__(64 * WM *WN) void Fp8TileKernel(
 // Eight wavefronts, two per SIMD, of 8 x 4 fragments. A block of K is 32 slots,
 // one MFMA each; between them go the fold of two slots before (its products have
 // left the matrix unit by then), the LDS reads of the next group and the copies
-// of the tile after next, in an order that sched_barrier keeps. The barrier that
-// makes the next tile visible stands before the last group, when this tile's
-// reads are done: the next tile's weight fragments are read in place, each
-// behind its last MFMA, so that the matrix unit does not wait at the block's end
-// (with the barrier between the blocks: 604 us at 8192 x 4096 x 14336).
+// of the block after next, in an order that sched_barrier keeps.
+//  - The barrier that makes the next block visible stands before the last group,
+//    when this block's reads are done: the next block's weight fragments are
+//    read in place, each behind its last MFMA, so that the matrix unit does not
+//    wait at the block's end.
+//  - LDS holds two blocks, and the copies of one take about as long as a block's
+//    MFMAs (1.8 us), so most start half a block earlier: a barrier in the
+//    middle says that the weights and half of the rows have been read.
+//  - A workgroup goes through its tiles without a pause: the last blocks of one
+//    copy the first blocks of the next, and its stores run beside those.
+// Left is the power limit: with these operands moving, the clock falls to 1.6-1.7
+// GHz (1.55 with the copies switched off, 2.1 on constant operands).
+// 8192 x 4096 x 14336: 604 us with barriers between the blocks, 510 with them
+// inside, 460 so.
 constexpr int kWideTile = 256;
 
 template <typename T>
@@ -326,49 +335,56 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const uint8_t *__restrict__ W, const float *__restrict__ SW, const uint8_t *__restrict__ A,
     const float *__restrict__ SA, T *__restrict__ Y, int64_t M, int64_t N, int64_t lda, int nb,
     int tiles_m, int tiles_n, int groups) {
-  constexpr int MI = 8, NJ = 4, WM = 2, WN = 4, kWaves = 8;
+  constexpr int MI = 8, NJ = 4, WM = 2, WN = 4;
   constexpr int kARecs = 32, kWRecs = 32;
-  constexpr int kStage = (kARecs + kWRecs) * kRec + 256 * kWaves;  // bytes; row scales last
+  constexpr int kStage = (kARecs + kWRecs) * kRec + 2048;  // bytes; row scales last
   extern __shared__ uint8_t lds[];
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int c = lane & 15, qd = lane >> 4;
   const int wm = wave % WM, wn = wave / WM;
-  int tm, tn;
-  TileOf(static_cast<int>(blockIdx.x), tiles_m, tiles_n, tm, tn);
-  const int64_t m0 = static_cast<int64_t>(tm) * kWideTile;
-  const int64_t rows = min(M - m0, static_cast<int64_t>(kWideTile));
-  const int last_row = static_cast<int>(rows) - 1;
+  const int tiles = tiles_m * tiles_n, last = nb - 1;
 
-  uint32_t a_off[4];
-  const uint8_t *w_src[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int rec = i * kWaves + wave;
-    a_off[i] = static_cast<uint32_t>(min(16 * (rec >> 1) + c, last_row) * lda + 64 * (rec & 1) + 16 * qd);
-    const int64_t g = min(static_cast<int64_t>(tn) * WN + (rec >> 3), static_cast<int64_t>(groups) - 1);
-    w_src[i] = W + (g * nb * 8 + (rec & 7)) * kRec;
-  }
-  const uint8_t *a_base = A + m0 * lda;
-  const uint32_t s_off = static_cast<uint32_t>(min(static_cast<int>(threadIdx.x), last_row) * nb * 4);
-  const float *sa_base = SA + m0 * nb;
+  // A tile's copy sources. Copy n < 4 takes a record of row fragments 2 n, 2 n + 1,
+  // 2 n + 8 and 2 n + 9 (groups 2 n and 2 n + 1 of both halves of the tile), copies
+  // 4 .. 7 the weights', copy 8 the row scales.
+  struct Source {
+    uint32_t a_off[4], s_off;
+    const uint8_t *a, *w[4];
+    const float *sa;
+  };
   const uint32_t l16 = static_cast<uint32_t>(lane) * 16;
-  // Copy n (0 .. 8) of block b into the stage at byte st.
-  auto copy = [&](auto nc, int b, uint32_t st) __attribute__((always_inline)) {
+  const int frag = (wave >> 2) * 8 + ((wave >> 1) & 1), half = wave & 1;  // of copy 0
+  auto source = [&](int tile, Source &o) __attribute__((always_inline)) {
+    int tm, tn;
+    TileOf(tile, tiles_m, tiles_n, tm, tn);
+    const int64_t m0 = static_cast<int64_t>(tm) * kWideTile;
+    const int last_row = static_cast<int>(min(M - m0, static_cast<int64_t>(kWideTile))) - 1;
+    o.a = A + m0 * lda;
+    o.sa = SA + m0 * nb;
+    o.s_off = static_cast<uint32_t>(min(static_cast<int>(threadIdx.x), last_row) * nb * 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o.a_off[i] = static_cast<uint32_t>(min(16 * (frag + 2 * i) + c, last_row) * lda + 64 * half + 16 * qd);
+      const int g = min(tn * WN + i, groups - 1);
+      o.w[i] = W + (static_cast<int64_t>(g) * nb * 8 + wave) * kRec;
+    }
+  };
+  auto copy = [&](auto nc, const Source &o, int b, uint32_t st) __attribute__((always_inline)) {
     constexpr int n = decltype(nc)::value;
     if constexpr (n < 4)
-      CopyToLds16S(a_base + static_cast<int64_t>(b) * kBlock, a_off[n],
-                   lds0 + st + (n * kWaves + wave) * kRec);
+      CopyToLds16S(o.a + static_cast<int64_t>(b) * kBlock, o.a_off[n],
+                   lds0 + st + (2 * (frag + 2 * n) + half) * kRec);
     else if constexpr (n < 8)
-      CopyToLds16S(w_src[n - 4] + static_cast<int64_t>(b) * 8 * kRec, l16,
-                   lds0 + st + (kARecs + (n - 4) * kWaves + wave) * kRec);
+      CopyToLds16S(o.w[n - 4] + static_cast<int64_t>(b) * 8 * kRec, l16,
+                   lds0 + st + (kARecs + (n - 4) * 8 + wave) * kRec);
     else
-      CopyToLds4S(sa_base + b, s_off, lds0 + st + (kARecs + kWRecs) * kRec + wave * 256);
+      CopyToLds4S(o.sa + b, o.s_off, lds0 + st + (kARecs + kWRecs) * kRec + wave * 256);
   };
-  auto issue = [&](int b, uint32_t st) __attribute__((always_inline)) {
+  auto issue = [&](const Source &o, int b, uint32_t st) __attribute__((always_inline)) {
     [&]<int... n>(std::integer_sequence<int, n...>) __attribute__((always_inline)) {
-      (copy(std::integral_constant<int, n>{}, b, st), ...);
+      (copy(std::integral_constant<int, n>{}, o, b, st), ...);
     }(std::make_integer_sequence<int, 9>{});
   };
   const uint8_t *a_at = lds + wm * MI * 2 * kRec + lane * 16;
@@ -387,19 +403,27 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   auto readS = [&](uint32_t st, int i) __attribute__((always_inline)) {
     return *reinterpret_cast<const float *>(s_at + st + 64 * i);
   };
+  // The weight scales of this wavefront's columns of a tile.
+  auto scales_of = [&](int tile) __attribute__((always_inline)) {
+    int tm, tn;
+    TileOf(tile, tiles_m, tiles_n, tm, tn);
+    return SW + static_cast<int64_t>(min(tn * WN + wn, groups - 1) >> 1) * nb;
+  };
 
   floatx4 acc[MI][NJ], part[4];
+  const floatx4 zero{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int v = 0; v < 4; ++v) part[v] = zero;
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int v = 0; v < 4; ++v) part[v] = floatx4{0.f, 0.f, 0.f, 0.f};
-  const int last = nb - 1;
-  const float *sw = SW + (min(static_cast<int64_t>(tn) * WN + wn, static_cast<int64_t>(groups) - 1) >> 1) * nb;
-  issue(0, 0);
-  WaitBarrier<0>();
-  issue(min(1, last), kStage);
+    for (int j = 0; j < NJ; ++j) acc[i][j] = zero;
+  Source now, next;
+  source(static_cast<int>(blockIdx.x), now);
+  issue(now, 0, 0);
+  issue(now, 1, kStage);
+  const float *sw = scales_of(static_cast<int>(blockIdx.x));
+  WaitBarrier<9>();
   intx8 wf[NJ], af[2];
   float f[2], scale = sw[0];
 #pragma unroll
@@ -413,62 +437,92 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
     for (int v = 0; v < 4; ++v) acc[i][j][v] = fmaf(part[k % 4][v], f[i % 2], acc[i][j][v]);
   };
-  constexpr int kSlots = MI * NJ;
-  for (int b = 0; b < nb; ++b) {
-    const uint32_t st = (b & 1) * kStage, other = kStage - st;
-    const float next_scale = sw[min(b + 1, last)];
-    float s_next = 0.0f;
-    auto slot = [&](auto kc) __attribute__((always_inline)) {
-      constexpr int k = decltype(kc)::value, i = k / NJ, j = k % NJ;
-      if constexpr (k == kSlots - NJ) {
-        WaitBarrier<0>();  // block b + 1 is in LDS, block b's reads are done
+  constexpr int kSlots = MI * NJ, kMid = 16, kLast = kSlots - NJ;
+  uint32_t st = 0;
+  for (int tile = static_cast<int>(blockIdx.x); tile < tiles; tile += gridDim.x) {
+    // Behind the last tile its last block is copied again.
+    const bool more = tile + static_cast<int>(gridDim.x) < tiles;
+    const int next_tile = more ? tile + static_cast<int>(gridDim.x) : tile;
+    const float *sw_next = scales_of(next_tile);
+    source(next_tile, next);
+    for (int b = 0; b < nb; ++b) {
+      const uint32_t other = kStage - st;
+      // The block after next: of this tile or of the next one. No branch here: it
+      // would cost the registers of the slots' pinned order.
+      const bool ahead = b + 2 > last;
+      const int cb = ahead ? (more ? b + 2 - nb : last) : b + 2;
+      Source from;
+      from.a = ahead ? next.a : now.a;
+      from.sa = ahead ? next.sa : now.sa;
+      from.s_off = ahead ? next.s_off : now.s_off;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        from.a_off[i] = ahead ? next.a_off[i] : now.a_off[i];
+        from.w[i] = ahead ? next.w[i] : now.w[i];
       }
-      part[k % 4] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-          wf[j], af[i % 2], floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-      if constexpr (i + 1 < MI) {
-        if constexpr (j == 0) af[(i + 1) % 2] = readA(st, i + 1);
-        if constexpr (j == 1) s_next = readS(st, i + 1);
-      } else {
-        if constexpr (j == 0) af[(i + 1) % 2] = readA(other, 0);
-        if constexpr (j == 1) s_next = readS(other, 0);
-        wf[j] = readW(other, j);
-      }
-      // Two slots back; the first two of a block are the last ones of the block
-      // before (of its products with f[1], still there).
-      if constexpr (k >= 2) fold(std::integral_constant<int, k - 2>{});
-      else fold(std::integral_constant<int, kSlots - 2 + k>{});
-      // The factor of group i + 1 takes the place of group i - 1's after its last fold.
-      if constexpr (j == 3) f[(i + 1) % 2] = s_next * (i + 1 < MI ? scale : next_scale);
-      // Block b + 2 into the stage that block b has left.
-      if constexpr (k >= kSlots - NJ) copy(std::integral_constant<int, k - (kSlots - NJ)>{}, min(b + 2, last), st);
-      __builtin_amdgcn_sched_barrier(0);
-    };
-    [&]<int... k>(std::integer_sequence<int, k...>) __attribute__((always_inline)) {
-      (slot(std::integral_constant<int, k>{}), ...);
-    }(std::make_integer_sequence<int, kSlots>{});
-    [&]<int... n>(std::integer_sequence<int, n...>) __attribute__((always_inline)) {
-      (copy(std::integral_constant<int, 4 + n>{}, min(b + 2, last), st), ...);
-    }(std::make_integer_sequence<int, 5>{});
-    scale = next_scale;
-  }
-  fold(std::integral_constant<int, kSlots - 2>{});
-  fold(std::integral_constant<int, kSlots - 1>{});
-  WaitBarrier<0>();  // no copy may land after this workgroup
-
-  const int64_t n = (static_cast<int64_t>(tn) * WN + wn) * 64 + 16 * qd;
-  const bool whole = n + 16 <= N && (N * static_cast<int64_t>(sizeof(T))) % 16 == 0;
-  if (n < N) {
+      const float next_scale = *(b < last ? sw + b + 1 : sw_next);
+      float s_next = 0.0f;
+      auto slot = [&](auto kc) __attribute__((always_inline)) {
+        constexpr int k = decltype(kc)::value, i = k / NJ, j = k % NJ;
+        if constexpr (k == kMid) WaitBarrier<63>();  // LDS reads up to group 4 are done
+        // The next block is in LDS (six newer copies are on their way), this block's
+        // reads are done.
+        if constexpr (k == kLast) WaitBarrier<6>();
+        part[k % 4] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], af[i % 2], zero, 0, 0,
+                                                                      0, 0, 0, 0);
+        if constexpr (i + 1 < MI) {
+          if constexpr (j == 0) af[(i + 1) % 2] = readA(st, i + 1);
+          if constexpr (j == 1) s_next = readS(st, i + 1);
+        } else {
+          if constexpr (j == 0) af[(i + 1) % 2] = readA(other, 0);
+          if constexpr (j == 1) s_next = readS(other, 0);
+          wf[j] = readW(other, j);
+        }
+        // Two slots back; the first two of a block are the last ones of the block
+        // before (of its products with f[1], still there).
+        if constexpr (k >= 2) fold(std::integral_constant<int, k - 2>{});
+        else fold(std::integral_constant<int, kSlots - 2 + k>{});
+        // The factor of group i + 1 takes the place of group i - 1's after its last fold.
+        if constexpr (j == 3) f[(i + 1) % 2] = s_next * (i + 1 < MI ? scale : next_scale);
+        // The block after next into this block's stage: the weights and the first four
+        // groups of rows, then the others and the row scales.
+        if constexpr (k >= kMid && k < kMid + 4) copy(std::integral_constant<int, 4 + k - kMid>{}, from, cb, st);
+        if constexpr (k >= kMid + 4 && k < kMid + 6) copy(std::integral_constant<int, k - kMid - 4>{}, from, cb, st);
+        if constexpr (k >= kLast && k < kLast + 2) copy(std::integral_constant<int, 2 + k - kLast>{}, from, cb, st);
+        if constexpr (k == kLast + 2) copy(std::integral_constant<int, 8>{}, from, cb, st);
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      [&]<int... k>(std::integer_sequence<int, k...>) __attribute__((always_inline)) {
+        (slot(std::integral_constant<int, k>{}), ...);
+      }(std::make_integer_sequence<int, kSlots>{});
+      scale = next_scale;
+      st = other;
+    }
+    sw = sw_next;
+    now = next;
+    fold(std::integral_constant<int, kSlots - 2>{});
+    fold(std::integral_constant<int, kSlots - 1>{});
+    part[(kSlots - 2) % 4] = part[(kSlots - 1) % 4] = zero;  // the next block folds them again
+    int tm, tn;
+    TileOf(tile, tiles_m, tiles_n, tm, tn);
+    const int64_t m0 = static_cast<int64_t>(tm) * kWideTile;
+    const int64_t rows = min(M - m0, static_cast<int64_t>(kWideTile));
+    const int64_t n = (static_cast<int64_t>(tn) * WN + wn) * 64 + 16 * qd;
+    const bool whole = n + 16 <= N && (N * static_cast<int64_t>(sizeof(T))) % 16 == 0;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
       const int64_t row = 16 * (wm * MI + i) + c;
       float v[16];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j)
+      for (int j = 0; j < NJ; ++j) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) v[4 * j + u] = acc[i][j][u];
-      if (row < rows) StoreRow<T, 16>(Y + (m0 + row) * N + n, v, N - n, whole);
+        acc[i][j] = zero;
+      }
+      if (row < rows && n < N) StoreRow<T, 16>(Y + (m0 + row) * N + n, v, N - n, whole);
     }
   }
+  WaitBarrier<0>();  // no copy may land after this workgroup
 }
 
 // Y = the sum of S partial products, in order.
@@ -494,7 +548,7 @@ struct TileShape {
 // every CU has work (at least four blocks each).
 TileShape PickTile(const Weight &w, int64_t M) {
   TileShape t{256, 256, 1, static_cast<int>(w.nb)};
-  if (CeilDiv(M, 256) * CeilDiv(w.N, 256) >= w.num_cus) return t;
+  if (w.nb >= 2 && CeilDiv(M, 256) * CeilDiv(w.N, 256) >= w.num_cus) return t;
   t.rows = t.cols = 128;
   const int64_t tiles = CeilDiv(M, 128) * CeilDiv(w.N, 128);
   int64_t s = std::max<int64_t>(1, w.num_cus / tiles);
@@ -537,8 +591,9 @@ hipError_t TileT(const Weight &w, const TileShape &t, int64_t M, const uint8_t *
       return TileLaunch<8, 2, 4, 2, EXACT, T>(w, t, M, A, lda, sa, Y, s);
     } else {
       const int64_t tiles_m = CeilDiv(M, 256), tiles_n = CeilDiv(w.N, 256);
-      hipLaunchKernelGGL((Fp8WideKernel<T>), dim3(static_cast<unsigned>(tiles_m * tiles_n)),
-                         dim3(512), 2 * (64 * kRec + 2048), s, w.W, w.scales, A, sa, Y, M, w.N, lda,
+      const int64_t wgs = std::min<int64_t>(tiles_m * tiles_n, w.num_cus);
+      hipLaunchKernelGGL((Fp8WideKernel<T>), dim3(static_cast<unsigned>(wgs)), dim3(512),
+                         2 * (64 * kRec + 2048), s, w.W, w.scales, A, sa, Y, M, w.N, lda,
                          static_cast<int>(w.nb), static_cast<int>(tiles_m),
                          static_cast<int>(tiles_n), static_cast<int>(w.groups));
       return hipGetLastError();
