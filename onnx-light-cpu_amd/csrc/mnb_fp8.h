@@ -26,7 +26,18 @@ struct Weight {
   int num_cus;
 };
 
-// s_waitcnt vmcnt(N) lgkmcnt(0) and a workgroup barrier, nothing moved across.
+// s_waitcnt vmcnt(N) lgkmcnt(0), nothing moved across: all but the newest N of this
+// wavefront's copies are in LDS.
+template <int N>
+__device__ __forceinline__ void WaitCopies() {
+  __asm__ volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | ((N >> 4) << 14));
+  __builtin_amdgcn_sched_barrier(0);
+  __asm__ volatile("" ::: "memory");
+}
+
+// The same and a workgroup barrier.
 template <int N>
 __device__ __forceinline__ void WaitBarrier() {
   __asm__ volatile("" ::: "memory");

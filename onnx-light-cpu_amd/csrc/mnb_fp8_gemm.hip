@@ -79,6 +79,18 @@ __device__ __forceinline__ void TileOf(int L, int tiles_m, int tiles_n, int &tm,
   tn = rem / gm;
 }
 
+// Rows of A in LDS: 128 bytes each, the eight 16-byte units of row r at places
+// unit ^ ((r / 2) % 8). A copy takes eight whole rows (full cache lines: 55 bytes a
+// clock and CU; the fragments' own order, 16 rows of 64 bytes, 16), and a
+// fragment's read, 16 rows of one unit, meets every bank once.
+__device__ __forceinline__ uint32_t CopyUnit(int lane, int row) {  // source byte of a copying lane
+  return static_cast<uint32_t>(((lane & 7) ^ ((row >> 1) & 7)) * 16);
+}
+__device__ __forceinline__ uint32_t ReadUnit(int lane, int h) {  // a lane's half h of a fragment
+  const int c = lane & 15, q = lane >> 4;
+  return static_cast<uint32_t>(c * 128 + ((4 * h + q) ^ ((c >> 1) & 7)) * 16);
+}
+
 // n (up to C) consecutive values of a row of Y; whole: all C, at an address
 // that 16 bytes (or the C values) divide.
 template <typename T, int C>
@@ -103,8 +115,9 @@ __device__ __forceinline__ void StoreRow(T *p, const float *v, int64_t n, bool w
 // ---- few rows: the weights streamed once ------------------------------------
 //
 // A workgroup takes RG fragments (16 columns each) and all rows (MC fragments
-// of 16); its wavefronts take the blocks of K in turn and add up in LDS.
-template <int MC, int RG, int WAVES, bool EXACT, typename T>
+// of 16); its wavefronts take the blocks of K in turn, D of them in flight, and
+// add up in LDS.
+template <int MC, int RG, int WAVES, int D, bool EXACT, typename T>
 __global__ __launch_bounds__(64 * WAVES) void Fp8StreamKernel(
     const uint8_t *__restrict__ W, const float *__restrict__ SW, const uint8_t *__restrict__ A,
     const float *__restrict__ SA, T *__restrict__ Y, int M, int64_t N, int64_t lda, int nb) {
@@ -130,7 +143,6 @@ __global__ __launch_bounds__(64 * WAVES) void Fp8StreamKernel(
     float s[MC];
   };
   auto load = [&](int b, Block &o) __attribute__((always_inline)) {
-    b = min(b, nb - 1);
 #pragma unroll
     for (int r = 0; r < RG; ++r)
 #pragma unroll
@@ -163,15 +175,24 @@ __global__ __launch_bounds__(64 * WAVES) void Fp8StreamKernel(
       }
     }
   };
-  Block x, y;
-  if (wave < nb) load(wave, x);
-  for (int b = wave; b < nb; b += 2 * WAVES) {
-    load(b + WAVES, y);
-    multiply(x);
-    if (b + WAVES < nb) {
-      load(b + 2 * WAVES, x);
-      multiply(y);
+  // This wavefront's blocks wave, wave + WAVES, ..: n of them, none loaded twice.
+  Block x[D];
+  const int n = (nb - wave + WAVES - 1) / WAVES;
+#pragma unroll
+  for (int d = 0; d < D; ++d)
+    if (d < n) load(wave + d * WAVES, x[d]);
+  int i = 0;
+  for (; i + 2 * D <= n; i += D) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      multiply(x[d]);
+      load(wave + (i + d + D) * WAVES, x[d]);
     }
+  }
+#pragma unroll
+  for (int d = 0; d < 2 * D - 1; ++d) {
+    if (i + d < n) multiply(x[d % D]);
+    if (d < D - 1 && i + d + D < n) load(wave + (i + d + D) * WAVES, x[d]);
   }
 #pragma unroll
   for (int m = 0; m < MC; ++m)
@@ -190,12 +211,101 @@ __global__ __launch_bounds__(64 * WAVES) void Fp8StreamKernel(
   }
 }
 
+// 17 to 64 rows: the rows, and with them the weights and the row scales, pass
+// through LDS, each wavefront's own blocks NS deep, so that the rows are copied by
+// whole lines (gathered into registers they bound it: 32 us at 48 x 14336 x 4096).
+template <int MC, int WAVES, int NS, bool EXACT, typename T>
+__global__ __launch_bounds__(64 * WAVES) void Fp8StreamLdsKernel(
+    const uint8_t *__restrict__ W, const float *__restrict__ SW, const uint8_t *__restrict__ A,
+    const float *__restrict__ SA, T *__restrict__ Y, int M, int64_t N, int64_t lda, int nb) {
+  constexpr int kRows = 2 * kRec, kScales = kRows + 2 * MC * kRec;  // offsets in a stage
+  constexpr int kStage = kScales + 256, kOps = 2 + 2 * MC + 1;
+  static_assert(NS * kStage >= MC * 1024, "the sums reuse the stages");
+  extern __shared__ uint8_t lds[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int c = lane & 15, qd = lane >> 4;
+  const int64_t g = blockIdx.x >> 2;
+  const int j = blockIdx.x & 3;
+  const uint8_t *w = W + (g * nb * 8 + 2 * j) * kRec;
+  const float *sw = SW + (g >> 1) * nb;
+  uint32_t a_off[2 * MC];
+#pragma unroll
+  for (int i = 0; i < 2 * MC; ++i) {
+    const int row = 8 * i + (lane >> 3);
+    a_off[i] = static_cast<uint32_t>(min(row, M - 1) * lda) + CopyUnit(lane, row);
+  }
+  const uint32_t s_off = static_cast<uint32_t>(min(lane, M - 1) * nb * 4), l16 = lane * 16;
+  const uint8_t *mine = lds + wave * NS * kStage;
+  const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(mine));
+  auto issue = [&](int b, int stage) __attribute__((always_inline)) {
+    const uint32_t st = base + stage * kStage;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      CopyToLds16S(w + (static_cast<int64_t>(b) * 8 + h) * kRec, l16, st + h * kRec);
+#pragma unroll
+    for (int i = 0; i < 2 * MC; ++i)
+      CopyToLds16S(A + static_cast<int64_t>(b) * kBlock, a_off[i], st + kRows + i * kRec);
+    CopyToLds4S(SA + b, s_off, st + kScales);
+  };
+  floatx4 acc[MC];
+#pragma unroll
+  for (int m = 0; m < MC; ++m) acc[m] = floatx4{0.f, 0.f, 0.f, 0.f};
+  auto multiply = [&](int b, int stage) __attribute__((always_inline)) {
+    const uint8_t *st = mine + stage * kStage;
+    const float scale = sw[b];
+    const Fragment<EXACT> wf(*reinterpret_cast<const intx4 *>(st + l16),
+                             *reinterpret_cast<const intx4 *>(st + kRec + l16));
+#pragma unroll
+    for (int m = 0; m < MC; ++m) {
+      const uint8_t *at = st + kRows + 2 * m * kRec;
+      const Fragment<EXACT> af(*reinterpret_cast<const intx4 *>(at + ReadUnit(lane, 0)),
+                               *reinterpret_cast<const intx4 *>(at + ReadUnit(lane, 1)));
+      const float f = *reinterpret_cast<const float *>(st + kScales + (16 * m + c) * 4) * scale;
+      const floatx4 p = Mfma(wf, af);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) acc[m][v] = fmaf(p[v], f, acc[m][v]);
+    }
+  };
+  // This wavefront's blocks wave, wave + WAVES, ..: n of them.
+  const int n = (nb - wave + WAVES - 1) / WAVES;
+#pragma unroll
+  for (int p = 0; p < NS - 1; ++p)
+    if (p < n) issue(wave + p * WAVES, p);
+  int i = 0, stage = 0;
+  for (; i + NS - 1 < n; ++i) {
+    WaitCopies<kOps *(NS - 2)>();
+    issue(wave + (i + NS - 1) * WAVES, stage == 0 ? NS - 1 : stage - 1);
+    multiply(wave + i * WAVES, stage);
+    stage = stage + 1 == NS ? 0 : stage + 1;
+  }
+  WaitCopies<0>();
+  for (; i < n; ++i) {
+    multiply(wave + i * WAVES, stage);
+    stage = stage + 1 == NS ? 0 : stage + 1;
+  }
+  __syncthreads();
+  floatx4 *red = reinterpret_cast<floatx4 *>(lds);  // [WAVES][MC][64]
+#pragma unroll
+  for (int m = 0; m < MC; ++m) red[(wave * MC + m) * 64 + lane] = acc[m];
+  __syncthreads();
+  for (int m = wave; m < MC; m += WAVES) {
+    floatx4 sum = red[m * 64 + lane];
+    for (int u = 1; u < WAVES; ++u) sum += red[(u * MC + m) * 64 + lane];
+    const int row = 16 * m + c;
+    const int64_t col = 64 * g + 16 * qd + 4 * j;
+    if (row < M && col < N) {
+      const float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+      StoreRow<T, 4>(Y + row * N + col, v, N - col, N % 4 == 0);
+    }
+  }
+}
+
 // ---- many rows: tiles in LDS --------------------------------------------------
 //
 // WM x WN wavefronts of MI x NJ fragments: a tile of 16 MI WM rows and
-// 16 NJ WN columns. A and W reach LDS by direct copies in the fragments' own
-// order (the lanes of a copy gather the rows of A), so an LDS read is 1 KiB in
-// a row; NS tiles of 128 values of K are in flight.
+// 16 NJ WN columns, in LDS by direct copies (W in the fragments' own order); NS
+// tiles of 128 values of K are in flight.
 template <int MI, int NJ, int WM, int WN, int NS, bool EXACT, typename T>
 __global__ __launch_bounds__(64 * WM *WN) void Fp8TileKernel(
     const uint8_t *__restrict__ W, const float *__restrict__ SW, const uint8_t *__restrict__ A,
@@ -229,9 +339,8 @@ __global__ __launch_bounds__(64 * WM *WN) void Fp8TileKernel(
   int64_t w_off[kWC];
 #pragma unroll
   for (int i = 0; i < kAC; ++i) {
-    const int rec = i * kWaves + wave;  // fragment rec / 2, half rec % 2
-    const int row = min(16 * (rec >> 1) + c, last_row);
-    a_off[i] = static_cast<uint32_t>(row * lda + 64 * (rec & 1) + 16 * qd);
+    const int row = 8 * (i * kWaves + wave) + (lane >> 3);
+    a_off[i] = static_cast<uint32_t>(min(row, last_row) * lda) + CopyUnit(lane, row);
   }
 #pragma unroll
   for (int i = 0; i < kWC; ++i) {
@@ -271,7 +380,7 @@ __global__ __launch_bounds__(64 * WM *WN) void Fp8TileKernel(
     WaitBarrier<kOps *(NS - 2)>();
     issue(min(b + NS - 1, b1 - 1), stage == 0 ? NS - 1 : stage - 1);
     const uint8_t *st = lds + stage * kStage;
-    const intx4 *la = reinterpret_cast<const intx4 *>(st) + wm * MI * 128 + lane;
+    const uint8_t *la = st + wm * MI * 2 * kRec;
     const intx4 *lw = reinterpret_cast<const intx4 *>(st + kARecs * kRec) + wn * 512 + lane;
     const float *ls = reinterpret_cast<const float *>(st + (kARecs + kWRecs) * kRec) + wm * MI * 16 + c;
     const Fragment<EXACT> wf[NJ] = {{lw[0], lw[64]},
@@ -280,7 +389,8 @@ __global__ __launch_bounds__(64 * WM *WN) void Fp8TileKernel(
                                     {lw[384], lw[448]}};
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-      const Fragment<EXACT> af(la[128 * i], la[128 * i + 64]);
+      const Fragment<EXACT> af(*reinterpret_cast<const intx4 *>(la + 2 * i * kRec + ReadUnit(lane, 0)),
+                               *reinterpret_cast<const intx4 *>(la + 2 * i * kRec + ReadUnit(lane, 1)));
       const float f = ls[16 * i] * scale;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
@@ -346,16 +456,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int wm = wave % WM, wn = wave / WM;
   const int tiles = tiles_m * tiles_n, last = nb - 1;
 
-  // A tile's copy sources. Copy n < 4 takes a record of row fragments 2 n, 2 n + 1,
-  // 2 n + 8 and 2 n + 9 (groups 2 n and 2 n + 1 of both halves of the tile), copies
-  // 4 .. 7 the weights', copy 8 the row scales.
+  // A tile's copy sources. Copy n < 4 takes eight of rows 32 n .. 32 n + 31 and
+  // 128 + 32 n .. (groups 2 n and 2 n + 1 of both halves of the tile), copies 4 .. 7
+  // the weights', copy 8 the row scales.
   struct Source {
     uint32_t a_off[4], s_off;
     const uint8_t *a, *w[4];
     const float *sa;
   };
   const uint32_t l16 = static_cast<uint32_t>(lane) * 16;
-  const int frag = (wave >> 2) * 8 + ((wave >> 1) & 1), half = wave & 1;  // of copy 0
+  const int row0 = (wave >> 2) * 128 + (wave & 3) * 8;  // of copy 0
   auto source = [&](int tile, Source &o) __attribute__((always_inline)) {
     int tm, tn;
     TileOf(tile, tiles_m, tiles_n, tm, tn);
@@ -366,7 +476,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     o.s_off = static_cast<uint32_t>(min(static_cast<int>(threadIdx.x), last_row) * nb * 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      o.a_off[i] = static_cast<uint32_t>(min(16 * (frag + 2 * i) + c, last_row) * lda + 64 * half + 16 * qd);
+      const int row = row0 + 32 * i + (lane >> 3);
+      o.a_off[i] = static_cast<uint32_t>(min(row, last_row) * lda) + CopyUnit(lane, row);
       const int g = min(tn * WN + i, groups - 1);
       o.w[i] = W + (static_cast<int64_t>(g) * nb * 8 + wave) * kRec;
     }
@@ -375,7 +486,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     constexpr int n = decltype(nc)::value;
     if constexpr (n < 4)
       CopyToLds16S(o.a + static_cast<int64_t>(b) * kBlock, o.a_off[n],
-                   lds0 + st + (2 * (frag + 2 * n) + half) * kRec);
+                   lds0 + st + (row0 + 32 * n) * 128);
     else if constexpr (n < 8)
       CopyToLds16S(o.w[n - 4] + static_cast<int64_t>(b) * 8 * kRec, l16,
                    lds0 + st + (kARecs + (n - 4) * 8 + wave) * kRec);
@@ -387,13 +498,13 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       (copy(std::integral_constant<int, n>{}, o, b, st), ...);
     }(std::make_integer_sequence<int, 9>{});
   };
-  const uint8_t *a_at = lds + wm * MI * 2 * kRec + lane * 16;
+  const uint8_t *a_at0 = lds + wm * MI * 2 * kRec + ReadUnit(lane, 0);
+  const uint8_t *a_at1 = lds + wm * MI * 2 * kRec + ReadUnit(lane, 1);
   const uint8_t *w_at = lds + (kARecs + wn * 8) * kRec + lane * 16;
   const uint8_t *s_at = lds + (kARecs + kWRecs) * kRec + (wm * MI * 16 + c) * 4;
   auto readA = [&](uint32_t st, int i) __attribute__((always_inline)) {
-    const uint8_t *p = a_at + st + 2 * i * kRec;
-    return Fragment<false>(*reinterpret_cast<const intx4 *>(p),
-                           *reinterpret_cast<const intx4 *>(p + kRec)).v;
+    return Fragment<false>(*reinterpret_cast<const intx4 *>(a_at0 + st + 2 * i * kRec),
+                           *reinterpret_cast<const intx4 *>(a_at1 + st + 2 * i * kRec)).v;
   };
   auto readW = [&](uint32_t st, int j) __attribute__((always_inline)) {
     const uint8_t *p = w_at + st + 2 * j * kRec;
@@ -544,13 +655,15 @@ struct TileShape {
   int splits, per_split;
 };
 
-// Large tiles where they fill the chip, else 128 x 128 ones with K split so that
-// every CU has work (at least four blocks each).
+// Large tiles where they fill the chip; for up to 256 rows tiles of all of them,
+// so that the weights are read once; else 128 x 128 ones. K is split so that every
+// CU has work (at least four blocks each).
 TileShape PickTile(const Weight &w, int64_t M) {
   TileShape t{256, 256, 1, static_cast<int>(w.nb)};
   if (w.nb >= 2 && CeilDiv(M, 256) * CeilDiv(w.N, 256) >= w.num_cus) return t;
-  t.rows = t.cols = 128;
-  const int64_t tiles = CeilDiv(M, 128) * CeilDiv(w.N, 128);
+  t.rows = M > 128 && M <= 256 ? 256 : 128;
+  t.cols = 128;
+  const int64_t tiles = CeilDiv(M, t.rows) * CeilDiv(w.N, 128);
   int64_t s = std::max<int64_t>(1, w.num_cus / tiles);
   s = std::min<int64_t>(s, std::max<int64_t>(1, w.nb / 4));
   s = std::min<int64_t>(s, 8);
@@ -562,10 +675,21 @@ TileShape PickTile(const Weight &w, int64_t M) {
 template <int MC, typename T>
 hipError_t StreamT(const Weight &w, int M, const uint8_t *A, int64_t lda, const float *sa, void *Y,
                    hipStream_t s) {
-  constexpr int kWaves = 8, kRG = 1;
+  constexpr int kWaves = 8, kRG = 1, kDepth = MC <= 2 ? 4 : 3;
   const size_t lds = static_cast<size_t>(kWaves) * MC * kRG * 1024;
-  hipLaunchKernelGGL((Fp8StreamKernel<MC, kRG, kWaves, sizeof(T) == 4, T>),
+  hipLaunchKernelGGL((Fp8StreamKernel<MC, kRG, kWaves, kDepth, sizeof(T) == 4, T>),
                      dim3(static_cast<unsigned>(w.groups * 4 / kRG)), dim3(64 * kWaves), lds, s, w.W,
+                     w.scales, A, sa, static_cast<T *>(Y), M, w.N, lda, static_cast<int>(w.nb));
+  return hipGetLastError();
+}
+
+template <int MC, typename T>
+hipError_t StreamLdsT(const Weight &w, int M, const uint8_t *A, int64_t lda, const float *sa,
+                      void *Y, hipStream_t s) {
+  constexpr int kWaves = MC == 2 ? 8 : MC == 3 ? 6 : 4, NS = 3;
+  const size_t lds = static_cast<size_t>(kWaves) * NS * ((2 + 2 * MC) * kRec + 256);
+  hipLaunchKernelGGL((Fp8StreamLdsKernel<MC, kWaves, NS, sizeof(T) == 4, T>),
+                     dim3(static_cast<unsigned>(w.groups * 4)), dim3(64 * kWaves), lds, s, w.W,
                      w.scales, A, sa, static_cast<T *>(Y), M, w.N, lda, static_cast<int>(w.nb));
   return hipGetLastError();
 }
@@ -586,6 +710,9 @@ hipError_t TileLaunch(const Weight &w, const TileShape &t, int64_t M, const uint
 template <bool EXACT, typename T>
 hipError_t TileT(const Weight &w, const TileShape &t, int64_t M, const uint8_t *A, int64_t lda,
                  const float *sa, T *Y, hipStream_t s) {
+  if (t.rows == 256 && t.cols == 128) {
+    return TileLaunch<8, 2, 2, 3, EXACT, T>(w, t, M, A, lda, sa, Y, s);
+  }
   if (t.rows == 256) {
     if constexpr (EXACT) {
       return TileLaunch<8, 2, 4, 2, EXACT, T>(w, t, M, A, lda, sa, Y, s);
@@ -609,9 +736,9 @@ hipError_t ProductT(const Weight &w, int64_t M, const uint8_t *A, int64_t lda, c
     const int m = static_cast<int>(M);
     switch ((M + 15) / 16) {
     case 1: return StreamT<1, T>(w, m, A, lda, sa, Y, s);
-    case 2: return StreamT<2, T>(w, m, A, lda, sa, Y, s);
-    case 3: return StreamT<3, T>(w, m, A, lda, sa, Y, s);
-    default: return StreamT<4, T>(w, m, A, lda, sa, Y, s);
+    case 2: return StreamLdsT<2, T>(w, m, A, lda, sa, Y, s);
+    case 3: return StreamLdsT<3, T>(w, m, A, lda, sa, Y, s);
+    default: return StreamLdsT<4, T>(w, m, A, lda, sa, Y, s);
     }
   }
   const TileShape t = PickTile(w, M);
@@ -636,7 +763,8 @@ size_t WorkBytes(const Weight &w, int64_t M) {
 }
 
 const char *ProductKernelName(const Weight &w, int64_t M) {
-  if (M <= kStreamRows) return "Fp8StreamKernel";
+  if (M <= 16) return "Fp8StreamKernel";
+  if (M <= kStreamRows) return "Fp8StreamLdsKernel";
   return "Fp8TileKernel";
 }
 
