@@ -299,17 +299,18 @@ struct Pipe {
     for (int i = 0; i < kSharedPer; ++i) {
       const int s = SharedCopy(i);
       const bool powers = s == kDigitCopies;
-      // The column whose data this lane copies, and which 32 bytes of a digit's unit.
-      const int column = powers ? lane : ONE ? lane & 3 : (s >> 1) * 16 + (lane & 15);
-      const int part = ONE ? (lane >> 2) & 3 : lane >> 4, h = ONE ? lane >> 4 : s & 1;
+      // The column whose data this lane copies; of digits eight columns of 128 bytes
+      // (whole lines), the 16-byte unit x of column c at place x ^ ((c / 2) % 8).
+      const int column = powers ? lane : ONE ? lane >> 3 : s * 8 + (lane >> 3);
       const int c = column & 15, digit = c / kT, token = (column >> 4) * kT + c % kT;
       // Columns without a token keep what LDS holds: nothing reads their sums. One
       // lane is always on, so that every copy is issued and counted.
-      s_on[i] = (token < n && digit < ND && column < 16 * GC && (!ONE || lane < 32) &&
-                 (!ONE || !powers || lane == 0)) || lane == 0;
+      s_on[i] = (token < n && digit < ND && column < 16 * GC && (!ONE || !powers || lane == 0)) ||
+                lane == 0;
       const uint32_t row = row_of(token < n ? token : 0), units = static_cast<uint32_t>(f.units);
       s_off[i] = powers ? row * units * (XB * 4)
-                        : (row * ND + min(digit, ND - 1)) * units * kUnit + 32 * part + 16 * h;
+                        : (row * ND + min(digit, ND - 1)) * units * kUnit +
+                              ((lane & 7) ^ ((c >> 1) & 7)) * 16;
     }
   }
   __device__ __forceinline__ void Issue(const Fixed &f, int u, int stage) const {
@@ -404,9 +405,11 @@ struct Pipe {
 #pragma unroll
     for (int g = 0; g < GC; ++g) {
       if (GC > 1 && g >= groups) continue;
-      const uint8_t *dig = st + kDigits + 2 * g * kRec + (q * kCols + min(c, kCols - 1)) * 16;
-      const intx4 b0 = *reinterpret_cast<const intx4 *>(dig);
-      const intx4 b1 = *reinterpret_cast<const intx4 *>(dig + kCols * 64);
+      const int kept = min(c, kCols - 1);
+      const uint8_t *dig = st + kDigits + 2 * g * kRec + kept * kUnit;
+      const int flip = (kept >> 1) & 7;
+      const intx4 b0 = *reinterpret_cast<const intx4 *>(dig + ((2 * q) ^ flip) * 16);
+      const intx4 b1 = *reinterpret_cast<const intx4 *>(dig + ((2 * q + 1) ^ flip) * 16);
       float power[XB];
       const uint8_t *at = st + kPowers + (ONE ? 0 : (g * 16 + c) * XB * 4);
       if constexpr (XB == 1) {
