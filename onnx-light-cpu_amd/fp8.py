@@ -44,19 +44,15 @@ def _library():
     return _lib
 
 
-def _on(device, stream, call):
-    """call() with `device` and `stream` current: what it allocates, copies and
-    launches is ordered on that stream."""
+def _elsewhere(device, stream):
+    """What has to be made current for a call on `device` and `stream`, so that what
+    it allocates, copies and launches is ordered there; None where it is."""
     import torch
-    if stream is not None:
-        if stream.device != device:
-            raise ValueError(f"stream of {stream.device}, tensors on {device}")
-        with torch.cuda.stream(stream):
-            return call()
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return call()
-    return call()
+    if stream is None:
+        return None if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+    if stream.device != device:
+        raise ValueError(f"stream of {stream.device}, tensors on {device}")
+    return torch.cuda.stream(stream)
 
 
 def quantize_fp8(X, stream=None):
@@ -66,32 +62,33 @@ def quantize_fp8(X, stream=None):
     amax / 448 and code = 448 x / amax rounded to e4m3. A 2-D X may have any row
     stride."""
     import torch
-    L = _library()
-    if not X.is_cuda or _types.get(X.dtype, 17) == 17:
+    L = _lib or _library()
+    x_type = _types.get(X.dtype, 17)
+    if x_type == 17 or not X.is_cuda:
         raise ValueError(f"{QUANTIZE_PREFIX}: X must be a float32, float16 or bfloat16 device "
                          "tensor")
-    if X.dim() == 0 or X.shape[-1] == 0:
+    shape, device = X.shape, X.device
+    if not shape or shape[-1] == 0:
         raise ValueError(f"{QUANTIZE_PREFIX}: X must be [..., K] with K >= 1")
-
-    def call():
-        shape, device = X.shape, X.device
-        K = shape[-1]
-        x, ldx = X, K
-        if not X.is_contiguous():
-            if X.dim() == 2 and X.stride(1) == 1 and X.stride(0) >= K:
-                ldx = X.stride(0)
-            else:
-                x = X.contiguous()
-        M = x.numel() // K
-        codes = torch.empty(shape, dtype=torch.float8_e4m3fn, device=device)
-        scales = torch.empty(shape[:-1] + (-(-K // BLOCK),), dtype=torch.float32, device=device)
-        status = L.mnb_fp8_quantize(M, K, _types[x.dtype], x.data_ptr(), ldx, codes.data_ptr(),
-                                    scales.data_ptr(), _raw_stream(device))
-        if status != 0:
-            _check(status, "quantize_fp8")
-        return codes, scales
-
-    return _on(X.device, stream, call)
+    elsewhere = _elsewhere(device, stream)
+    if elsewhere is not None:
+        with elsewhere:
+            return quantize_fp8(X)
+    K = shape[-1]
+    ldx = K
+    if not X.is_contiguous():
+        if X.dim() == 2 and X.stride(1) == 1 and X.stride(0) >= K:
+            ldx = X.stride(0)
+        else:
+            X = X.contiguous()
+    codes = torch.empty(shape, dtype=torch.float8_e4m3fn, device=device)
+    scales = torch.empty(shape[:-1] + ((K + BLOCK - 1) // BLOCK,), dtype=torch.float32,
+                         device=device)
+    status = L.mnb_fp8_quantize(X.numel() // K, K, x_type, X.data_ptr(), ldx, codes.data_ptr(),
+                                scales.data_ptr(), _raw_stream(device))
+    if status != 0:
+        _check(status, "quantize_fp8")
+    return codes, scales
 
 
 class MatMulFp8:
@@ -107,6 +104,7 @@ class MatMulFp8:
         self._plan = ctypes.c_void_p()
         self._device = None
         self._works = {}  # by thread and stream
+        self._needs = {}  # workspace bytes by (rows, dtype)
 
     _stream_workspace = MatMulNBits._stream_workspace
 
@@ -156,7 +154,7 @@ class MatMulFp8:
         if self._plan:
             _library().mnb_fp8_plan_destroy(self._plan)
             self._plan = ctypes.c_void_p()
-        self._works = {}
+        self._works, self._needs = {}, {}
 
     def __del__(self):
         try:
@@ -178,12 +176,12 @@ class MatMulFp8:
         if a_type is None or device != self._device:
             raise ValueError(f"{PREFIX}: A must be a float8_e4m3fn, float32, float16 or bfloat16 "
                              f"tensor on {self._device}")
-        K, N = self.K, self.N
-        if A.dim() == 0 or A.shape[-1] != K:
-            raise ValueError(f"{PREFIX}: A must be [..., {K}], got {list(A.shape)}")
-        rows = A.shape[:-1]
+        K, N, shape = self.K, self.N, A.shape
+        if not shape or shape[-1] != K:
+            raise ValueError(f"{PREFIX}: A must be [..., {K}], got {list(shape)}")
+        rows = shape[:-1]
         if a_type == 17:
-            want = rows + (-(-K // BLOCK),)
+            want = rows + ((K + BLOCK - 1) // BLOCK,)
             if (scales is None or scales.shape != want or scales.dtype != torch.float32
                     or scales.device != device):
                 raise ValueError(f"{PREFIX}: codes need float32 scales {list(want)} on {device}")
@@ -200,25 +198,38 @@ class MatMulFp8:
                                 or out.device != device or out.data_ptr() % 16 != 0):
             raise ValueError(f"{PREFIX}: out must be contiguous {list(rows + (N,))} on {device}, "
                              "aligned to 16 bytes")
+        elsewhere = _elsewhere(device, stream)
+        if elsewhere is not None:
+            with elsewhere:
+                return self(A, scales, out, out_dtype)
+        if not A.is_contiguous():
+            A = A.contiguous()
+        address = A.data_ptr()
+        if address % 16 != 0:
+            A = A.clone()
+            address = A.data_ptr()
+        if scales is not None and not scales.is_contiguous():
+            scales = scales.contiguous()
+        M = A.numel() // K
+        if out is None:
+            out = torch.empty(rows + (N,), dtype=dtype, device=device)
+        need = self._needs.get((M, a_type))
+        if need is None:
+            need = self._remember(M, A.dtype)
+        work = self._stream_workspace(need, device) if need else None
+        status = _lib.mnb_fp8_run(self._plan, M, a_type, address,
+                                  None if scales is None else scales.data_ptr(), y_type,
+                                  out.data_ptr(), None if work is None else work.data_ptr(), need,
+                                  _raw_stream(device))
+        if status != 0:
+            _check(status, "run")
+        return out
 
-        def call():
-            a = A if A.is_contiguous() else A.contiguous()
-            if a.data_ptr() % 16 != 0:
-                a = a.clone()
-            s = scales if scales is None or scales.is_contiguous() else scales.contiguous()
-            M = a.numel() // K
-            y = out if out is not None else torch.empty(rows + (N,), dtype=dtype, device=device)
-            need = self.workspace_bytes(M, A.dtype)
-            work = self._stream_workspace(need, device) if need else None
-            status = _lib.mnb_fp8_run(self._plan, M, a_type, a.data_ptr(),
-                                      None if s is None else s.data_ptr(), y_type, y.data_ptr(),
-                                      None if work is None else work.data_ptr(), need,
-                                      _raw_stream(device))
-            if status != 0:
-                _check(status, "run")
-            return y
-
-        return _on(device, stream, call)
+    def _remember(self, M, dtype):
+        if len(self._needs) > 256:
+            self._needs = {}
+        need = self._needs[M, _types[dtype]] = self.workspace_bytes(M, dtype)
+        return need
 
     run = __call__
 

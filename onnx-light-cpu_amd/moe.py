@@ -13,7 +13,7 @@ import ctypes
 import numpy as np
 
 from . import MatMulNBits, _check, _raw_stream, library
-from .fp8 import _on
+from .fp8 import _elsewhere
 
 PREFIX = "onnx_light_cpu_amd::MatMulNBitsMoE"
 
@@ -69,6 +69,7 @@ class MatMulNBitsMoE:
         self._device = None
         self._router = False
         self._works = {}  # by thread and stream
+        self._needs = {}  # workspace bytes by (tokens, type)
 
     _stream_workspace = MatMulNBits._stream_workspace
 
@@ -148,7 +149,7 @@ class MatMulNBitsMoE:
         if self._plan:
             _library().mnb_moe_plan_destroy(self._plan)
             self._plan = ctypes.c_void_p()
-        self._works = {}
+        self._works, self._needs = {}, {}
 
     def __del__(self):
         try:
@@ -169,9 +170,10 @@ class MatMulNBitsMoE:
         if x_type is None or device != self._device:
             raise ValueError(f"{PREFIX}: X must be a float32, float16 or bfloat16 tensor on "
                              f"{self._device}")
-        if X.dim() == 0 or X.shape[-1] != d.hidden:
-            raise ValueError(f"{PREFIX}: X must be [..., {d.hidden}], got {list(X.shape)}")
-        rows = X.shape[:-1]
+        H, k, shape = d.hidden, d.top_k, X.shape
+        if not shape or shape[-1] != H:
+            raise ValueError(f"{PREFIX}: X must be [..., {H}], got {list(shape)}")
+        rows = shape[:-1]
         if logits is None:
             if not self._router:
                 raise ValueError(f"{PREFIX}: a layer without a router needs logits")
@@ -179,32 +181,39 @@ class MatMulNBitsMoE:
                 or logits.device != device):
             raise ValueError(f"{PREFIX}: logits must be float32 {list(rows) + [d.experts]} on "
                              f"{device}")
-        if out is not None and (out.shape != X.shape or out.dtype != X.dtype
+        if out is not None and (out.shape != shape or out.dtype != X.dtype
                                 or out.device != device or not out.is_contiguous()):
             raise ValueError(f"{PREFIX}: out must be contiguous, of X's shape, type and device")
-
-        def call():
-            x = X if X.is_contiguous() else X.contiguous()
-            l = logits if logits is None or logits.is_contiguous() else logits.contiguous()
-            y = out if out is not None else torch.empty(X.shape, dtype=X.dtype, device=device)
-            ids = weights = None
-            if routing:
-                ids = torch.empty(rows + (d.top_k,), dtype=torch.int32, device=device)
-                weights = torch.empty(rows + (d.top_k,), dtype=torch.float32, device=device)
-            T = x.numel() // d.hidden
-            need = self.workspace_bytes(T, X.dtype)
-            work = self._stream_workspace(need, device) if need else None
-            status = _lib.mnb_moe_run(self._plan, T, x_type, x.data_ptr(),
-                                      None if l is None else l.data_ptr(), y.data_ptr(),
-                                      None if ids is None else ids.data_ptr(),
-                                      None if weights is None else weights.data_ptr(),
-                                      None if work is None else work.data_ptr(), need,
-                                      _raw_stream(device))
-            if status != 0:
-                _check(status, "run")
-            return (y, ids, weights) if routing else y
-
-        return _on(device, stream, call)
+        elsewhere = _elsewhere(device, stream)
+        if elsewhere is not None:
+            with elsewhere:
+                return self(X, logits, routing, out)
+        if not X.is_contiguous():
+            X = X.contiguous()
+        if logits is not None and not logits.is_contiguous():
+            logits = logits.contiguous()
+        if out is None:
+            out = torch.empty(shape, dtype=X.dtype, device=device)
+        ids = weights = None
+        if routing:
+            ids = torch.empty(rows + (k,), dtype=torch.int32, device=device)
+            weights = torch.empty(rows + (k,), dtype=torch.float32, device=device)
+        T = X.numel() // H
+        need = self._needs.get((T, x_type))
+        if need is None:
+            if len(self._needs) > 256:
+                self._needs = {}
+            need = self._needs[T, x_type] = self.workspace_bytes(T, X.dtype)
+        work = self._stream_workspace(need, device) if need else None
+        status = _lib.mnb_moe_run(self._plan, T, x_type, X.data_ptr(),
+                                  None if logits is None else logits.data_ptr(), out.data_ptr(),
+                                  None if ids is None else ids.data_ptr(),
+                                  None if weights is None else weights.data_ptr(),
+                                  None if work is None else work.data_ptr(), need,
+                                  _raw_stream(device))
+        if status != 0:
+            _check(status, "run")
+        return (out, ids, weights) if routing else out
 
     run = __call__
 
