@@ -79,7 +79,8 @@ int mnb_fp8_run(const mnb_fp8_plan *plan, int64_t M, int32_t a_type, const void 
                 const float *dAScales, int32_t y_type, void *dY, void *dWorkspace,
                 size_t workspace_bytes, void *stream);
 
-/* Name of the kernel that multiplies M rows ("" for a bad plan or M == 0). */
+/* Name of the kernel that multiplies M rows into a 16-bit Y ("" for a bad plan or
+ * M == 0). */
 const char *mnb_fp8_kernel_name(const mnb_fp8_plan *plan, int64_t M);
 
 #ifdef __cplusplus

@@ -301,19 +301,24 @@ __global__ __launch_bounds__(64 * WAVES) void Fp8StreamLdsKernel(
   }
 }
 
-// ---- many rows: tiles in LDS --------------------------------------------------
+// ---- more rows: tiles of 32 MI rows and 64 WN columns ---------------------------
 //
-// WM x WN wavefronts of MI x NJ fragments: a tile of 16 MI WM rows and
-// 16 NJ WN columns, in LDS by direct copies (W in the fragments' own order); NS
-// tiles of 128 values of K are in flight.
-template <int MI, int NJ, int WM, int WN, int NS, bool EXACT, typename T>
-__global__ __launch_bounds__(64 * WM *WN) void Fp8TileKernel(
+// Two by WN wavefronts of MI x 4 fragments, and NS blocks of K in LDS (W in the
+// fragments' own order). A block is 4 MI slots, one fragment's product each;
+// between them go the fold of two slots before and the LDS reads of the next
+// group, in an order that sched_barrier keeps. The barrier that makes the next
+// block visible stands before the last group, when this block's reads are done:
+// its stage takes the copies of the block NS ahead, and the next block's weight
+// fragments are read behind their last use (with the barrier between the blocks
+// 47 us instead of TILE256 at 200 x 4096 x 28672).
+template <int MI, int WN, int NS, bool EXACT, typename T>
+__global__ __launch_bounds__(128 * WN) __attribute__((amdgpu_waves_per_eu(1, 1))) void Fp8TileKernel(
     const uint8_t *__restrict__ W, const float *__restrict__ SW, const uint8_t *__restrict__ A,
     const float *__restrict__ SA, T *__restrict__ Y, int64_t M, int64_t N, int64_t lda, int nb,
-    int tiles_m, int tiles_n, int groups, int per_split) {
-  static_assert(NJ == 4, "a wavefront takes one group of 64 columns");
-  constexpr int kWaves = WM * WN;
-  constexpr int kARecs = 2 * MI * WM, kWRecs = 8 * WN;
+    int tiles_m, int tiles_n, int groups) {
+  constexpr int NJ = 4, WM = 2, kWaves = WM * WN;
+  constexpr int kARecs = 2 * MI * WM, kWRecs = 8 * WN;  // of 1 KiB
+  constexpr int kAC = kARecs / kWaves, kWC = kWRecs / kWaves, kOps = kAC + kWC + 1;
   static_assert(kARecs % kWaves == 0 && kWRecs % kWaves == 0, "copies");
   static_assert(64 * kWaves >= 16 * MI * WM, "one row scale per thread");
   constexpr int kStage = (kARecs + kWRecs) * kRec + 256 * kWaves;  // bytes; row scales last
@@ -323,20 +328,18 @@ __global__ __launch_bounds__(64 * WM *WN) void Fp8TileKernel(
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int c = lane & 15, qd = lane >> 4;
   const int wm = wave % WM, wn = wave / WM;
-
   int tm, tn;
   TileOf(static_cast<int>(blockIdx.x), tiles_m, tiles_n, tm, tn);
-  const int b0 = static_cast<int>(blockIdx.y) * per_split;
-  const int b1 = min(nb, b0 + per_split);
-  Y += static_cast<int64_t>(blockIdx.y) * M * N;
+  const int splits = gridDim.y, split = blockIdx.y;
+  const int b0 = static_cast<int>(static_cast<int64_t>(nb) * split / splits);
+  const int last = static_cast<int>(static_cast<int64_t>(nb) * (split + 1) / splits) - 1;
+  Y += static_cast<int64_t>(split) * M * N;
   const int64_t m0 = static_cast<int64_t>(tm) * 16 * MI * WM;
   const int64_t rows = min(M - m0, static_cast<int64_t>(16 * MI * WM));
   const int last_row = static_cast<int>(rows) - 1;
 
-  // Copy sources: per-lane offsets from a base that walks K.
-  constexpr int kAC = kARecs / kWaves, kWC = kWRecs / kWaves;
   uint32_t a_off[kAC];
-  int64_t w_off[kWC];
+  const uint8_t *w_src[kWC];
 #pragma unroll
   for (int i = 0; i < kAC; ++i) {
     const int row = 8 * (i * kWaves + wave) + (lane >> 3);
@@ -345,62 +348,113 @@ __global__ __launch_bounds__(64 * WM *WN) void Fp8TileKernel(
 #pragma unroll
   for (int i = 0; i < kWC; ++i) {
     const int rec = i * kWaves + wave;  // group rec / 8 of the tile
-    const int64_t g = min(static_cast<int64_t>(tn) * WN + (rec >> 3), static_cast<int64_t>(groups) - 1);
-    w_off[i] = (g * nb * 8 + (rec & 7)) * kRec;
+    const int g = min(tn * WN + (rec >> 3), groups - 1);
+    w_src[i] = W + (static_cast<int64_t>(g) * nb * 8 + (rec & 7)) * kRec;
   }
   const uint8_t *a_base = A + m0 * lda;
-  const float *sa_base = SA + (m0 + min(static_cast<int>(threadIdx.x), last_row)) * nb;
+  const uint32_t s_off = static_cast<uint32_t>(min(static_cast<int>(threadIdx.x), last_row) * nb * 4);
+  const float *sa_base = SA + m0 * nb;
   const uint32_t l16 = static_cast<uint32_t>(lane) * 16;
-  auto issue = [&](int b, int stage) __attribute__((always_inline)) {
-    const uint32_t st = lds0 + stage * kStage;
+  auto issue = [&](int b, uint32_t stage) __attribute__((always_inline)) {
+    const uint32_t st = lds0 + stage;
 #pragma unroll
     for (int i = 0; i < kAC; ++i)
       CopyToLds16S(a_base + static_cast<int64_t>(b) * kBlock, a_off[i],
                    st + (i * kWaves + wave) * kRec);
 #pragma unroll
     for (int i = 0; i < kWC; ++i)
-      CopyToLds16S(W + w_off[i] + static_cast<int64_t>(b) * 8 * kRec, l16,
+      CopyToLds16S(w_src[i] + static_cast<int64_t>(b) * 8 * kRec, l16,
                    st + (kARecs + i * kWaves + wave) * kRec);
-    CopyToLds4(sa_base + b, st + (kARecs + kWRecs) * kRec + wave * 256);
+    CopyToLds4S(sa_base + b, s_off, st + (kARecs + kWRecs) * kRec + wave * 256);
   };
-  constexpr int kOps = kAC + kWC + 1;
+  const uint8_t *a_at0 = lds + wm * MI * 2 * kRec + ReadUnit(lane, 0);
+  const uint8_t *a_at1 = lds + wm * MI * 2 * kRec + ReadUnit(lane, 1);
+  const uint8_t *w_at = lds + (kARecs + wn * 8) * kRec + lane * 16;
+  const uint8_t *s_at = lds + (kARecs + kWRecs) * kRec + (wm * MI * 16 + c) * 4;
+  struct Raw {
+    intx4 lo, hi;
+  };
+  auto readA = [&](uint32_t st, int i) __attribute__((always_inline)) {
+    return Raw{*reinterpret_cast<const intx4 *>(a_at0 + st + 2 * i * kRec),
+               *reinterpret_cast<const intx4 *>(a_at1 + st + 2 * i * kRec)};
+  };
+  auto readW = [&](uint32_t st, int j) __attribute__((always_inline)) {
+    const uint8_t *p = w_at + st + 2 * j * kRec;
+    return Raw{*reinterpret_cast<const intx4 *>(p), *reinterpret_cast<const intx4 *>(p + kRec)};
+  };
+  auto readS = [&](uint32_t st, int i) __attribute__((always_inline)) {
+    return *reinterpret_cast<const float *>(s_at + st + 64 * i);
+  };
+  using Frag = Fragment<EXACT>;
 
-  floatx4 acc[MI][NJ];
+  floatx4 acc[MI][NJ], part[4];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int v = 0; v < 4; ++v) part[v] = floatx4{0.f, 0.f, 0.f, 0.f};
+  const float *sw = SW + static_cast<int64_t>(min(tn * WN + wn, groups - 1) >> 1) * nb;
+#pragma unroll
+  for (int p = 0; p < NS; ++p) issue(min(b0 + p, last), p * kStage);
+  WaitBarrier<kOps *(NS - 1)>();
+  float f[2], scale = sw[b0];
+  Raw raw_w[NJ], raw_a = readA(0, 0);
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) raw_w[j] = readW(0, j);
+  f[0] = readS(0, 0) * scale;
+  f[1] = 0.0f;
+  Frag af[2] = {Frag(raw_a.lo, raw_a.hi), Frag(raw_a.lo, raw_a.hi)};
+  Frag wf[NJ] = {Frag(raw_w[0].lo, raw_w[0].hi), Frag(raw_w[1].lo, raw_w[1].hi),
+                 Frag(raw_w[2].lo, raw_w[2].hi), Frag(raw_w[3].lo, raw_w[3].hi)};
 
+  auto fold = [&](auto kc) __attribute__((always_inline)) {  // slot k of a block
+    constexpr int k = decltype(kc)::value, i = k / NJ, j = k % NJ;
 #pragma unroll
-  for (int p = 0; p < NS - 1; ++p) issue(min(b0 + p, b1 - 1), p);
-  const float *sw = SW + (min(static_cast<int64_t>(tn) * WN + wn, static_cast<int64_t>(groups) - 1) >> 1) * nb;
-  int stage = 0;
-  for (int b = b0; b < b1; ++b) {
-    const float scale = sw[b];
-    WaitBarrier<kOps *(NS - 2)>();
-    issue(min(b + NS - 1, b1 - 1), stage == 0 ? NS - 1 : stage - 1);
-    const uint8_t *st = lds + stage * kStage;
-    const uint8_t *la = st + wm * MI * 2 * kRec;
-    const intx4 *lw = reinterpret_cast<const intx4 *>(st + kARecs * kRec) + wn * 512 + lane;
-    const float *ls = reinterpret_cast<const float *>(st + (kARecs + kWRecs) * kRec) + wm * MI * 16 + c;
-    const Fragment<EXACT> wf[NJ] = {{lw[0], lw[64]},
-                                    {lw[128], lw[192]},
-                                    {lw[256], lw[320]},
-                                    {lw[384], lw[448]}};
-#pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const Fragment<EXACT> af(*reinterpret_cast<const intx4 *>(la + 2 * i * kRec + ReadUnit(lane, 0)),
-                               *reinterpret_cast<const intx4 *>(la + 2 * i * kRec + ReadUnit(lane, 1)));
-      const float f = ls[16 * i] * scale;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const floatx4 p = Mfma(wf[j], af);
-#pragma unroll
-        for (int v = 0; v < 4; ++v) acc[i][j][v] = fmaf(p[v], f, acc[i][j][v]);
+    for (int v = 0; v < 4; ++v) acc[i][j][v] = fmaf(part[k % 4][v], f[i % 2], acc[i][j][v]);
+  };
+  constexpr int kSlots = MI * NJ, kLast = kSlots - NJ;
+  static_assert(MI % 2 == 0, "the row fragments' parity");
+  uint32_t st = 0;
+  for (int b = b0; b <= last; ++b) {
+    const uint32_t next = st + kStage == NS * kStage ? 0 : st + kStage;
+    const float next_scale = sw[min(b + 1, last)];
+    float s_next = 0.0f;
+    auto slot = [&](auto kc) __attribute__((always_inline)) {
+      constexpr int k = decltype(kc)::value, i = k / NJ, j = k % NJ;
+      // The next block is in LDS, this block's reads are done.
+      if constexpr (k == kLast) WaitBarrier<kOps *(NS - 2)>();
+      part[k % 4] = Mfma(wf[j], af[i % 2]);
+      if constexpr (j == 0) raw_a = i + 1 < MI ? readA(st, i + 1) : readA(next, 0);
+      if constexpr (j == 1) s_next = i + 1 < MI ? readS(st, i + 1) : readS(next, 0);
+      if constexpr (i + 1 == MI) {
+        raw_w[j] = readW(next, j);
+        if constexpr (!EXACT) wf[j] = Frag(raw_w[j].lo, raw_w[j].hi);
       }
+      // Two slots back; the first two of a block are the last ones of the block
+      // before (of its products with f[1], still there).
+      if constexpr (k >= 2) fold(std::integral_constant<int, k - 2>{});
+      else fold(std::integral_constant<int, kSlots - 2 + k>{});
+      if constexpr (j == 3) {
+        // The factor of group i + 1 takes the place of group i - 1's after its last fold.
+        f[(i + 1) % 2] = s_next * (i + 1 < MI ? scale : next_scale);
+        af[(i + 1) % 2] = Frag(raw_a.lo, raw_a.hi);
+      }
+      if constexpr (k == kLast) issue(min(b + NS, last), st);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    [&]<int... k>(std::integer_sequence<int, k...>) __attribute__((always_inline)) {
+      (slot(std::integral_constant<int, k>{}), ...);
+    }(std::make_integer_sequence<int, kSlots>{});
+    if constexpr (EXACT) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) wf[j] = Frag(raw_w[j].lo, raw_w[j].hi);
     }
-    stage = stage + 1 == NS ? 0 : stage + 1;
+    scale = next_scale;
+    st = next;
   }
+  fold(std::integral_constant<int, kSlots - 2>{});
+  fold(std::integral_constant<int, kSlots - 1>{});
   WaitBarrier<0>();  // no copy may land after this workgroup
 
   const int64_t n = (static_cast<int64_t>(tn) * WN + wn) * 64 + 16 * qd;
@@ -651,24 +705,21 @@ __global__ __launch_bounds__(256) void Fp8SumKernel(const float *__restrict__ P,
 constexpr int64_t kStreamRows = 64;
 
 struct TileShape {
-  int rows, cols;
-  int splits, per_split;
+  int rows, cols, splits;
 };
 
-// Large tiles where they fill the chip; for up to 256 rows tiles of all of them,
-// so that the weights are read once; else 128 x 128 ones. K is split so that every
-// CU has work (at least four blocks each).
-TileShape PickTile(const Weight &w, int64_t M) {
-  TileShape t{256, 256, 1, static_cast<int>(w.nb)};
-  if (w.nb >= 2 && CeilDiv(M, 256) * CeilDiv(w.N, 256) >= w.num_cus) return t;
-  t.rows = M > 128 && M <= 256 ? 256 : 128;
-  t.cols = 128;
-  const int64_t tiles = CeilDiv(M, t.rows) * CeilDiv(w.N, 128);
-  int64_t s = std::max<int64_t>(1, w.num_cus / tiles);
-  s = std::min<int64_t>(s, std::max<int64_t>(1, w.nb / 4));
-  s = std::min<int64_t>(s, 8);
-  t.per_split = static_cast<int>(CeilDiv(w.nb, s));
-  t.splits = static_cast<int>(CeilDiv(w.nb, t.per_split));
+// exact: an fp32 Y.
+TileShape PickTile(const Weight &w, int64_t M, bool exact) {
+  // 16-bit results: large tiles where they fill the chip; for 129 to 256 rows tiles
+  // of all of them, so that the weights are read once. Else 128 x 128.
+  TileShape t{128, 128, 1};
+  if (!exact && w.nb >= 2 && CeilDiv(M, 256) * CeilDiv(w.N, 256) >= w.num_cus)
+    return TileShape{256, 256, 1};
+  if (!exact && M > 128 && M <= 256) t.rows = 256;
+  // K is split so that every CU has work, of at least four blocks each.
+  const int64_t tiles = CeilDiv(M, t.rows) * CeilDiv(w.N, t.cols);
+  const int64_t s = std::min<int64_t>({w.num_cus / tiles, w.nb / 4, 8});
+  t.splits = static_cast<int>(std::max<int64_t>(1, s));
   return t;
 }
 
@@ -694,29 +745,24 @@ hipError_t StreamLdsT(const Weight &w, int M, const uint8_t *A, int64_t lda, con
   return hipGetLastError();
 }
 
-template <int MI, int WM, int WN, int NS, bool EXACT, typename T>
+template <int MI, int WN, int NS, bool EXACT, typename T>
 hipError_t TileLaunch(const Weight &w, const TileShape &t, int64_t M, const uint8_t *A, int64_t lda,
                       const float *sa, T *Y, hipStream_t s) {
-  const int64_t tiles_m = CeilDiv(M, 16 * MI * WM), tiles_n = CeilDiv(w.N, 64 * WN);
-  const size_t lds = static_cast<size_t>(NS) * ((2 * MI * WM + 8 * WN) * kRec + 256 * WM * WN);
-  hipLaunchKernelGGL((Fp8TileKernel<MI, 4, WM, WN, NS, EXACT, T>),
-                     dim3(static_cast<unsigned>(tiles_m * tiles_n), t.splits), dim3(64 * WM * WN),
-                     lds, s, w.W, w.scales, A, sa, Y, M, w.N, lda, static_cast<int>(w.nb),
+  const int64_t tiles_m = CeilDiv(M, 32 * MI), tiles_n = CeilDiv(w.N, 64 * WN);
+  const size_t lds = static_cast<size_t>(NS) * ((4 * MI + 8 * WN) * kRec + 512 * WN);
+  hipLaunchKernelGGL((Fp8TileKernel<MI, WN, NS, EXACT, T>),
+                     dim3(static_cast<unsigned>(tiles_m * tiles_n), t.splits), dim3(128 * WN), lds,
+                     s, w.W, w.scales, A, sa, Y, M, w.N, lda, static_cast<int>(w.nb),
                      static_cast<int>(tiles_m), static_cast<int>(tiles_n),
-                     static_cast<int>(w.groups), t.per_split);
+                     static_cast<int>(w.groups));
   return hipGetLastError();
 }
 
 template <bool EXACT, typename T>
 hipError_t TileT(const Weight &w, const TileShape &t, int64_t M, const uint8_t *A, int64_t lda,
                  const float *sa, T *Y, hipStream_t s) {
-  if (t.rows == 256 && t.cols == 128) {
-    return TileLaunch<8, 2, 2, 3, EXACT, T>(w, t, M, A, lda, sa, Y, s);
-  }
-  if (t.rows == 256) {
-    if constexpr (EXACT) {
-      return TileLaunch<8, 2, 4, 2, EXACT, T>(w, t, M, A, lda, sa, Y, s);
-    } else {
+  if constexpr (!EXACT) {
+    if (t.cols == 256) {
       const int64_t tiles_m = CeilDiv(M, 256), tiles_n = CeilDiv(w.N, 256);
       const int64_t wgs = std::min<int64_t>(tiles_m * tiles_n, w.num_cus);
       hipLaunchKernelGGL((Fp8WideKernel<T>), dim3(static_cast<unsigned>(wgs)), dim3(512),
@@ -725,8 +771,9 @@ hipError_t TileT(const Weight &w, const TileShape &t, int64_t M, const uint8_t *
                          static_cast<int>(tiles_n), static_cast<int>(w.groups));
       return hipGetLastError();
     }
+    if (t.rows == 256) return TileLaunch<8, 2, 3, EXACT, T>(w, t, M, A, lda, sa, Y, s);
   }
-  return TileLaunch<4, 2, 2, 3, EXACT, T>(w, t, M, A, lda, sa, Y, s);
+  return TileLaunch<4, 2, 4, EXACT, T>(w, t, M, A, lda, sa, Y, s);
 }
 
 template <typename T>
@@ -741,8 +788,8 @@ hipError_t ProductT(const Weight &w, int64_t M, const uint8_t *A, int64_t lda, c
     default: return StreamLdsT<4, T>(w, m, A, lda, sa, Y, s);
     }
   }
-  const TileShape t = PickTile(w, M);
   constexpr bool kExact = sizeof(T) == 4;
+  const TileShape t = PickTile(w, M, kExact);
   if (t.splits == 1) return TileT<kExact, T>(w, t, M, A, lda, sa, static_cast<T *>(Y), s);
   float *parts = static_cast<float *>(work);
   hipError_t e = TileT<kExact, float>(w, t, M, A, lda, sa, parts, s);
@@ -758,14 +805,14 @@ hipError_t ProductT(const Weight &w, int64_t M, const uint8_t *A, int64_t lda, c
 
 size_t WorkBytes(const Weight &w, int64_t M) {
   if (M <= kStreamRows) return 0;
-  const TileShape t = PickTile(w, M);
-  return t.splits == 1 ? 0 : static_cast<size_t>(t.splits) * M * w.N * sizeof(float);
+  const int splits = std::max(PickTile(w, M, false).splits, PickTile(w, M, true).splits);
+  return splits == 1 ? 0 : static_cast<size_t>(splits) * M * w.N * sizeof(float);
 }
 
 const char *ProductKernelName(const Weight &w, int64_t M) {
   if (M <= 16) return "Fp8StreamKernel";
   if (M <= kStreamRows) return "Fp8StreamLdsKernel";
-  return "Fp8TileKernel";
+  return PickTile(w, M, false).cols == 256 ? "Fp8WideKernel" : "Fp8TileKernel";
 }
 
 hipError_t LaunchProduct(const Weight &w, int64_t M, const uint8_t *A, int64_t lda,

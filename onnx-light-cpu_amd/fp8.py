@@ -74,14 +74,15 @@ def quantize_fp8(X, stream=None):
     if elsewhere is not None:
         with elsewhere:
             return quantize_fp8(X)
-    K = shape[-1]
-    ldx = K
-    if not X.is_contiguous():
+    K = ldx = shape[-1]
+    if X.is_contiguous():
+        codes = torch.empty_like(X, dtype=torch.float8_e4m3fn)
+    else:
         if X.dim() == 2 and X.stride(1) == 1 and X.stride(0) >= K:
             ldx = X.stride(0)
         else:
             X = X.contiguous()
-    codes = torch.empty(shape, dtype=torch.float8_e4m3fn, device=device)
+        codes = torch.empty(shape, dtype=torch.float8_e4m3fn, device=device)
     scales = torch.empty(shape[:-1] + ((K + BLOCK - 1) // BLOCK,), dtype=torch.float32,
                          device=device)
     status = L.mnb_fp8_quantize(X.numel() // K, K, x_type, X.data_ptr(), ldx, codes.data_ptr(),
