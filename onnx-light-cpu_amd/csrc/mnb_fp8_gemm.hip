@@ -301,9 +301,9 @@ __global__ __launch_bounds__(64 * WAVES) void Fp8StreamLdsKernel(
   }
 }
 
-// ---- more rows: tiles of 32 MI rows and 64 WN columns ---------------------------
+// ---- more rows: tiles of 16 MI WM rows and 64 WN columns ------------------------
 //
-// Two by WN wavefronts of MI x 4 fragments, and NS blocks of K in LDS (W in the
+// WM by WN wavefronts of MI x 4 fragments, and NS blocks of K in LDS (W in the
 // fragments' own order). A block is 4 MI slots, one fragment's product each;
 // between them go the fold of two slots before and the LDS reads of the next
 // group, in an order that sched_barrier keeps. The barrier that makes the next
@@ -311,12 +311,12 @@ __global__ __launch_bounds__(64 * WAVES) void Fp8StreamLdsKernel(
 // its stage takes the copies of the block NS ahead, and the next block's weight
 // fragments are read behind their last use (with the barrier between the blocks
 // 47 us instead of TILE256 at 200 x 4096 x 28672).
-template <int MI, int WN, int NS, bool EXACT, typename T>
-__global__ __launch_bounds__(128 * WN) __attribute__((amdgpu_waves_per_eu(1, 1))) void Fp8TileKernel(
+template <int MI, int WM, int WN, int NS, bool EXACT, typename T>
+__global__ __launch_bounds__(64 * WM *WN) void Fp8TileKernel(
     const uint8_t *__restrict__ W, const float *__restrict__ SW, const uint8_t *__restrict__ A,
     const float *__restrict__ SA, T *__restrict__ Y, int64_t M, int64_t N, int64_t lda, int nb,
     int tiles_m, int tiles_n, int groups) {
-  constexpr int NJ = 4, WM = 2, kWaves = WM * WN;
+  constexpr int NJ = 4, kWaves = WM * WN;
   constexpr int kARecs = 2 * MI * WM, kWRecs = 8 * WN;  // of 1 KiB
   constexpr int kAC = kARecs / kWaves, kWC = kWRecs / kWaves, kOps = kAC + kWC + 1;
   static_assert(kARecs % kWaves == 0 && kWRecs % kWaves == 0, "copies");
@@ -457,9 +457,10 @@ __global__ __launch_bounds__(128 * WN) __attribute__((amdgpu_waves_per_eu(1, 1))
   fold(std::integral_constant<int, kSlots - 1>{});
   WaitBarrier<0>();  // no copy may land after this workgroup
 
-  const int64_t n = (static_cast<int64_t>(tn) * WN + wn) * 64 + 16 * qd;
-  const bool whole = n + 16 <= N && (N * static_cast<int64_t>(sizeof(T))) % 16 == 0;
-  if (n < N) {
+  const int64_t n0 = static_cast<int64_t>(tn) * WN * 64, n = n0 + wn * 64 + 16 * qd;
+  if ((N * static_cast<int64_t>(sizeof(T))) % 16 == 0) {
+    if (n >= N) return;
+    const bool whole = n + 16 <= N;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
       const int64_t row = 16 * (wm * MI + i) + c;
@@ -470,7 +471,25 @@ __global__ __launch_bounds__(128 * WN) __attribute__((amdgpu_waves_per_eu(1, 1))
         for (int u = 0; u < 4; ++u) v[4 * j + u] = acc[i][j][u];
       if (row < rows) StoreRow<T, 16>(Y + (m0 + row) * N + n, v, N - n, whole);
     }
+    return;
   }
+  // Rows that no vector store fits pass through LDS and leave by consecutive values
+  // (333 x 2500 x 5001: 21 us; 35 where each lane stored its 16 one by one).
+  constexpr int kPitch = 64 * WN + 4;
+  static_assert(16 * MI * WM * kPitch * 4 <= NS * kStage, "the tile reuses the stages");
+  float *tile = reinterpret_cast<float *>(lds);
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      *reinterpret_cast<floatx4 *>(tile + (16 * (wm * MI + i) + c) * kPitch + wn * 64 + 16 * qd + 4 * j) =
+          acc[i][j];
+  __syncthreads();
+  for (int row = wave; row < rows; row += kWaves)
+#pragma unroll
+    for (int u = 0; u < WN; ++u)
+      if (n0 + 64 * u + lane < N)
+        Y[(m0 + row) * N + n0 + 64 * u + lane] = static_cast<T>(tile[row * kPitch + 64 * u + lane]);
 }
 
 // ---- many rows, 16-bit Y: 256 x 256 tiles ---------------------------------------
@@ -710,10 +729,10 @@ struct TileShape {
 
 // exact: an fp32 Y.
 TileShape PickTile(const Weight &w, int64_t M, bool exact) {
-  // 16-bit results: large tiles where they fill the chip; for 129 to 256 rows tiles
+  // 16-bit results: large tiles where they fill the chip (rows of whole vectors); for 129 to 256 rows tiles
   // of all of them, so that the weights are read once. Else 128 x 128.
   TileShape t{128, 128, 1};
-  if (!exact && w.nb >= 2 && CeilDiv(M, 256) * CeilDiv(w.N, 256) >= w.num_cus)
+  if (!exact && w.nb >= 2 && w.N % 8 == 0 && CeilDiv(M, 256) * CeilDiv(w.N, 256) >= w.num_cus)
     return TileShape{256, 256, 1};
   if (!exact && M > 128 && M <= 256) t.rows = 256;
   // K is split so that every CU has work, of at least four blocks each.
@@ -745,14 +764,14 @@ hipError_t StreamLdsT(const Weight &w, int M, const uint8_t *A, int64_t lda, con
   return hipGetLastError();
 }
 
-template <int MI, int WN, int NS, bool EXACT, typename T>
+template <int MI, int WM, int WN, int NS, bool EXACT, typename T>
 hipError_t TileLaunch(const Weight &w, const TileShape &t, int64_t M, const uint8_t *A, int64_t lda,
                       const float *sa, T *Y, hipStream_t s) {
-  const int64_t tiles_m = CeilDiv(M, 32 * MI), tiles_n = CeilDiv(w.N, 64 * WN);
-  const size_t lds = static_cast<size_t>(NS) * ((4 * MI + 8 * WN) * kRec + 512 * WN);
-  hipLaunchKernelGGL((Fp8TileKernel<MI, WN, NS, EXACT, T>),
-                     dim3(static_cast<unsigned>(tiles_m * tiles_n), t.splits), dim3(128 * WN), lds,
-                     s, w.W, w.scales, A, sa, Y, M, w.N, lda, static_cast<int>(w.nb),
+  const int64_t tiles_m = CeilDiv(M, 16 * MI * WM), tiles_n = CeilDiv(w.N, 64 * WN);
+  const size_t lds = static_cast<size_t>(NS) * ((2 * MI * WM + 8 * WN) * kRec + 256 * WM * WN);
+  hipLaunchKernelGGL((Fp8TileKernel<MI, WM, WN, NS, EXACT, T>),
+                     dim3(static_cast<unsigned>(tiles_m * tiles_n), t.splits), dim3(64 * WM * WN),
+                     lds, s, w.W, w.scales, A, sa, Y, M, w.N, lda, static_cast<int>(w.nb),
                      static_cast<int>(tiles_m), static_cast<int>(tiles_n),
                      static_cast<int>(w.groups));
   return hipGetLastError();
@@ -771,9 +790,9 @@ hipError_t TileT(const Weight &w, const TileShape &t, int64_t M, const uint8_t *
                          static_cast<int>(tiles_n), static_cast<int>(w.groups));
       return hipGetLastError();
     }
-    if (t.rows == 256) return TileLaunch<8, 2, 3, EXACT, T>(w, t, M, A, lda, sa, Y, s);
+    if (t.rows == 256) return TileLaunch<8, 2, 2, 3, EXACT, T>(w, t, M, A, lda, sa, Y, s);
   }
-  return TileLaunch<4, 2, 4, EXACT, T>(w, t, M, A, lda, sa, Y, s);
+  return TileLaunch<2, 4, 2, 4, EXACT, T>(w, t, M, A, lda, sa, Y, s);
 }
 
 template <typename T>
