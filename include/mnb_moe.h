@@ -76,7 +76,8 @@ int mnb_moe_plan_destroy(mnb_moe_plan *plan);
 int mnb_moe_plan_device_bytes(const mnb_moe_plan *plan, size_t *bytes);
 
 /* Device workspace (16-byte aligned) of a run of T tokens: their values in
- * fixed point, the logits and the choice, the chosen experts' rows. */
+ * fixed point, the logits and the choice, the chosen experts' rows. It is
+ * enough for any smaller T too. */
 int mnb_moe_workspace_bytes(const mnb_moe_plan *plan, int64_t T, int32_t x_type, size_t *bytes);
 
 /* Y [T, hidden] of X [T, hidden], both of x_type (MNB_TYPE_FLOAT, _FLOAT16 or

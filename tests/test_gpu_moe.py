@@ -201,6 +201,21 @@ def test_every_token_on_one_expert(pkg, cuda):
         _check(y, ref, err)
 
 
+def test_workspace_serves_every_launch_of_a_run(pkg, cuda):
+    """39 tokens of this layer need more than 64 (down in more parts), and a run of
+    103 ends with them."""
+    import torch
+    H, I, E = 3328, 2048, 16
+    x, router, ws = _problem(103, H, I, E, 128, False, "bfloat16", 43, cuda)
+    op = pkg.MatMulNBitsMoE(H, I, E, 1, block_size=128).prepare_device(router, *ws)
+    for dtype in (torch.bfloat16, torch.float32):
+        needs = [op.workspace_bytes(T, dtype) for T in range(130)]
+        assert needs == sorted(needs) and needs[0] == 0 and len(set(needs[64:])) == 1
+    print("case moe 64 + 39 tokens", flush=True)
+    y = op(x)
+    assert torch.equal(y[:64], op(x[:64])) and torch.equal(y[64:], op(x[64:]))
+
+
 def test_nonfinite_tokens_stay_alone(pkg, cuda):
     import torch
     for T in (3, 40):
