@@ -114,66 +114,40 @@ __device__ __forceinline__ void StoreRow(T *p, const float *v, int64_t n, bool w
 
 // ---- few rows: the weights streamed once ------------------------------------
 //
-// A workgroup takes RG fragments (16 columns each) and all rows (MC fragments
-// of 16); its wavefronts take the blocks of K in turn, D of them in flight, and
-// add up in LDS.
-template <int MC, int RG, int WAVES, int D, bool EXACT, typename T>
+// Up to 16 rows: a workgroup takes 16 columns and all rows, one fragment each; its
+// wavefronts take the blocks of K in turn, D of them in flight, and add up in LDS.
+template <int WAVES, int D, bool EXACT, typename T>
 __global__ __launch_bounds__(64 * WAVES) void Fp8StreamKernel(
     const uint8_t *__restrict__ W, const float *__restrict__ SW, const uint8_t *__restrict__ A,
     const float *__restrict__ SA, T *__restrict__ Y, int M, int64_t N, int64_t lda, int nb) {
-  extern __shared__ floatx4 red[];  // [WAVES][MC * RG][64]
+  __shared__ floatx4 red[WAVES][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int c = lane & 15, qd = lane >> 4;
-  const int64_t f0 = static_cast<int64_t>(blockIdx.x) * RG;
-  const int64_t g = f0 >> 2;
-  const int j0 = static_cast<int>(f0 & 3);
-  const uint8_t *w = W + (g * nb * 8 + 2 * j0) * kRec + lane * 16;
+  const int64_t g = blockIdx.x >> 2;
+  const int j = blockIdx.x & 3;
+  const uint8_t *w = W + (g * nb * 8 + 2 * j) * kRec + lane * 16;
   const float *sw = SW + (g >> 1) * nb;
-  const uint8_t *a[MC];
-  const float *sa[MC];
-#pragma unroll
-  for (int m = 0; m < MC; ++m) {
-    const int64_t row = min(16 * m + c, M - 1);
-    a[m] = A + row * lda + 16 * qd;
-    sa[m] = SA + row * nb;
-  }
+  const int64_t row = min(c, M - 1);
+  const uint8_t *a = A + row * lda + 16 * qd;
+  const float *sa = SA + row * nb;
   struct Block {
-    intx4 w[RG][2], a[MC][2];
-    float s[MC];
+    intx4 w[2], a[2];
+    float s;
   };
   auto load = [&](int b, Block &o) __attribute__((always_inline)) {
 #pragma unroll
-    for (int r = 0; r < RG; ++r)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        o.w[r][h] = *reinterpret_cast<const intx4 *>(
-            w + (static_cast<int64_t>(b) * 8 + 2 * r + h) * kRec);
-    const float scale = sw[b];
-#pragma unroll
-    for (int m = 0; m < MC; ++m) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        o.a[m][h] = *reinterpret_cast<const intx4 *>(a[m] + static_cast<int64_t>(b) * kBlock + 64 * h);
-      o.s[m] = sa[m][b] * scale;
+    for (int h = 0; h < 2; ++h) {
+      o.w[h] = *reinterpret_cast<const intx4 *>(w + (static_cast<int64_t>(b) * 8 + h) * kRec);
+      o.a[h] = *reinterpret_cast<const intx4 *>(a + static_cast<int64_t>(b) * kBlock + 64 * h);
     }
+    o.s = sa[b] * sw[b];
   };
-  floatx4 acc[MC][RG];
-#pragma unroll
-  for (int m = 0; m < MC; ++m)
-#pragma unroll
-    for (int r = 0; r < RG; ++r) acc[m][r] = floatx4{0.f, 0.f, 0.f, 0.f};
+  floatx4 acc{0.f, 0.f, 0.f, 0.f};
   auto multiply = [&](const Block &o) __attribute__((always_inline)) {
+    const floatx4 p = Mfma(Fragment<EXACT>(o.w[0], o.w[1]), Fragment<EXACT>(o.a[0], o.a[1]));
 #pragma unroll
-    for (int r = 0; r < RG; ++r) {
-      const Fragment<EXACT> w(o.w[r][0], o.w[r][1]);
-#pragma unroll
-      for (int m = 0; m < MC; ++m) {
-        const floatx4 p = Mfma(w, Fragment<EXACT>(o.a[m][0], o.a[m][1]));
-#pragma unroll
-        for (int v = 0; v < 4; ++v) acc[m][r][v] = fmaf(p[v], o.s[m], acc[m][r][v]);
-      }
-    }
+    for (int v = 0; v < 4; ++v) acc[v] = fmaf(p[v], o.s, acc[v]);
   };
   // This wavefront's blocks wave, wave + WAVES, ..: n of them, none loaded twice.
   Block x[D];
@@ -194,20 +168,15 @@ __global__ __launch_bounds__(64 * WAVES) void Fp8StreamKernel(
     if (i + d < n) multiply(x[d % D]);
     if (d < D - 1 && i + d + D < n) load(wave + (i + d + D) * WAVES, x[d]);
   }
-#pragma unroll
-  for (int m = 0; m < MC; ++m)
-#pragma unroll
-    for (int r = 0; r < RG; ++r) red[(wave * MC * RG + m * RG + r) * 64 + lane] = acc[m][r];
+  red[wave][lane] = acc;
   __syncthreads();
-  for (int t = wave; t < MC * RG; t += WAVES) {
-    floatx4 sum = red[t * 64 + lane];
-    for (int u = 1; u < WAVES; ++u) sum += red[(u * MC * RG + t) * 64 + lane];
-    const int m = t / RG * 16 + c, r = t % RG;
-    const int64_t n = 64 * g + 16 * qd + 4 * (j0 + r);
-    if (m < M && n < N) {
-      const float v[4] = {sum[0], sum[1], sum[2], sum[3]};
-      StoreRow<T, 4>(Y + m * N + n, v, N - n, N % 4 == 0);
-    }
+  if (wave > 0) return;
+  floatx4 sum = red[0][lane];
+  for (int u = 1; u < WAVES; ++u) sum += red[u][lane];
+  const int64_t col = 64 * g + 16 * qd + 4 * j;
+  if (c < M && col < N) {
+    const float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+    StoreRow<T, 4>(Y + c * N + col, v, N - col, N % 4 == 0);
   }
 }
 
@@ -310,7 +279,7 @@ __global__ __launch_bounds__(64 * WAVES) void Fp8StreamLdsKernel(
 // block visible stands before the last group, when this block's reads are done:
 // its stage takes the copies of the block NS ahead, and the next block's weight
 // fragments are read behind their last use (with the barrier between the blocks
-// 47 us instead of TILE256 at 200 x 4096 x 28672).
+// 47 us instead of 44 at 200 x 4096 x 28672).
 template <int MI, int WM, int WN, int NS, bool EXACT, typename T>
 __global__ __launch_bounds__(64 * WM *WN) void Fp8TileKernel(
     const uint8_t *__restrict__ W, const float *__restrict__ SW, const uint8_t *__restrict__ A,
@@ -485,11 +454,12 @@ __global__ __launch_bounds__(64 * WM *WN) void Fp8TileKernel(
       *reinterpret_cast<floatx4 *>(tile + (16 * (wm * MI + i) + c) * kPitch + wn * 64 + 16 * qd + 4 * j) =
           acc[i][j];
   __syncthreads();
-  for (int row = wave; row < rows; row += kWaves)
+  for (int row = wave; row < rows; row += kWaves) {
 #pragma unroll
     for (int u = 0; u < WN; ++u)
       if (n0 + 64 * u + lane < N)
         Y[(m0 + row) * N + n0 + 64 * u + lane] = static_cast<T>(tile[row * kPitch + 64 * u + lane]);
+  }
 }
 
 // ---- many rows, 16-bit Y: 256 x 256 tiles ---------------------------------------
@@ -729,8 +699,9 @@ struct TileShape {
 
 // exact: an fp32 Y.
 TileShape PickTile(const Weight &w, int64_t M, bool exact) {
-  // 16-bit results: large tiles where they fill the chip (rows of whole vectors); for 129 to 256 rows tiles
-  // of all of them, so that the weights are read once. Else 128 x 128.
+  // 16-bit results: large tiles where they fill the chip (rows of whole vectors); for
+  // 129 to 256 rows tiles of all of them, so that the weights are read once (200 x
+  // 4096 x 28672: 44 us, 48 with 128 rows). Else 128 x 128.
   TileShape t{128, 128, 1};
   if (!exact && w.nb >= 2 && w.N % 8 == 0 && CeilDiv(M, 256) * CeilDiv(w.N, 256) >= w.num_cus)
     return TileShape{256, 256, 1};
@@ -742,13 +713,12 @@ TileShape PickTile(const Weight &w, int64_t M, bool exact) {
   return t;
 }
 
-template <int MC, typename T>
+template <typename T>
 hipError_t StreamT(const Weight &w, int M, const uint8_t *A, int64_t lda, const float *sa, void *Y,
                    hipStream_t s) {
-  constexpr int kWaves = 8, kRG = 1, kDepth = MC <= 2 ? 4 : 3;
-  const size_t lds = static_cast<size_t>(kWaves) * MC * kRG * 1024;
-  hipLaunchKernelGGL((Fp8StreamKernel<MC, kRG, kWaves, kDepth, sizeof(T) == 4, T>),
-                     dim3(static_cast<unsigned>(w.groups * 4 / kRG)), dim3(64 * kWaves), lds, s, w.W,
+  constexpr int kWaves = 8, kDepth = 4;
+  hipLaunchKernelGGL((Fp8StreamKernel<kWaves, kDepth, sizeof(T) == 4, T>),
+                     dim3(static_cast<unsigned>(w.groups * 4)), dim3(64 * kWaves), 0, s, w.W,
                      w.scales, A, sa, static_cast<T *>(Y), M, w.N, lda, static_cast<int>(w.nb));
   return hipGetLastError();
 }
@@ -780,7 +750,7 @@ hipError_t TileLaunch(const Weight &w, const TileShape &t, int64_t M, const uint
 template <bool EXACT, typename T>
 hipError_t TileT(const Weight &w, const TileShape &t, int64_t M, const uint8_t *A, int64_t lda,
                  const float *sa, T *Y, hipStream_t s) {
-  if constexpr (!EXACT) {
+  if constexpr (sizeof(T) == 2) {  // whole K, so Y itself
     if (t.cols == 256) {
       const int64_t tiles_m = CeilDiv(M, 256), tiles_n = CeilDiv(w.N, 256);
       const int64_t wgs = std::min<int64_t>(tiles_m * tiles_n, w.num_cus);
@@ -790,6 +760,8 @@ hipError_t TileT(const Weight &w, const TileShape &t, int64_t M, const uint8_t *
                          static_cast<int>(tiles_n), static_cast<int>(w.groups));
       return hipGetLastError();
     }
+  }
+  if constexpr (!EXACT) {
     if (t.rows == 256) return TileLaunch<8, 2, 2, 3, EXACT, T>(w, t, M, A, lda, sa, Y, s);
   }
   return TileLaunch<2, 4, 2, 4, EXACT, T>(w, t, M, A, lda, sa, Y, s);
@@ -801,7 +773,7 @@ hipError_t ProductT(const Weight &w, int64_t M, const uint8_t *A, int64_t lda, c
   if (M <= kStreamRows) {
     const int m = static_cast<int>(M);
     switch ((M + 15) / 16) {
-    case 1: return StreamT<1, T>(w, m, A, lda, sa, Y, s);
+    case 1: return StreamT<T>(w, m, A, lda, sa, Y, s);
     case 2: return StreamLdsT<2, T>(w, m, A, lda, sa, Y, s);
     case 3: return StreamLdsT<3, T>(w, m, A, lda, sa, Y, s);
     default: return StreamLdsT<4, T>(w, m, A, lda, sa, Y, s);

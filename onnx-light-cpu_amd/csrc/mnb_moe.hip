@@ -15,9 +15,11 @@
 // integers (below 2^21); they are scaled and added up in fp32, column by column,
 // and the columns of a token join after the last block.
 //
-// Four launches: logits and the fixed-point tokens; the choice; gate/up with
-// the activation, whose rows leave in fixed point; down with the weighted sum
-// over the experts. No atomics: every sum has one fixed order.
+// Three to five launches: logits and the fixed-point tokens; the choice (of one
+// token the gate/up workgroups each make it); gate/up with the activation, whose
+// rows leave in fixed point; down, with the weighted sum over the experts where
+// few tokens' sums fit its workgroups, otherwise that sum on its own. Every sum of
+// floating-point values has one fixed order.
 #include "mnb_moe.h"
 
 #include <algorithm>
@@ -571,7 +573,7 @@ constexpr int WavesPerSimd(int gc, int folds) {
   return gc * folds >= 16 ? 2 : gc > 1 || folds == 8 ? 4 : 6;
 }
 
-// Third launch: workgroup (b, i) the channels of block b of entry i's expert, 16
+// Gate/up: workgroup (b, i) the channels of block b of entry i's expert, 16
 // (gate and up) for each of GROUPS wavefronts that share a pipe, or, with KS runs
 // of the units, for each of GROUPS * KS wavefronts with pipes of their own.
 template <int ND, bool ONE, int GC, int F, bool ZP, int GROUPS, int KS, int NS, bool CHOOSE>
@@ -720,7 +722,7 @@ __global__ __launch_bounds__(64 * GROUPS *KS, GROUPS == 8 ? WavesPerSimd(GC, F) 
   }
 }
 
-// Fourth launch, few tokens on few experts: a workgroup takes 16 columns of Y. The
+// Down, few tokens on few experts: a workgroup takes 16 columns of Y. The
 // items (segment, unit) of the layer are cut into eight equal runs, one for each
 // wavefront and its pipe, which adds each segment's rows, times the tokens'
 // weights, to sums of its own; they join in order.
@@ -814,23 +816,21 @@ __global__ __launch_bounds__(512) void MoeDownNarrowKernel(Matrix m, Fixed fh, P
   }
 }
 
-// Fourth launch: a workgroup takes 256 columns of Y and one run of the items: part
-// blockIdx.y % cuts of the units of one segment, or `many` whole segments (cuts = 1).
-// Every pair's row, times its weight, goes to parts [cuts][pairs][width].
+// Down otherwise: a workgroup takes 256 columns of Y and part blockIdx.y % cuts of the
+// units of one segment. Every pair's row, times its weight, goes to parts
+// [cuts][pairs][width].
 template <int ND, bool ONE, int GC, int F, bool ZP, int NS>
 __global__ __launch_bounds__(512, WavesPerSimd(GC, F)) void MoeDownKernel(Matrix m, Fixed fh, Plan plan,
                                                      float *__restrict__ parts, int pairs, int cuts,
-                                                     int many, int64_t width) {
+                                                     int64_t width) {
   using P = Pipe<ND, ONE, GC, 2, F, 1, ZP, 8, NS>;
   constexpr int kT = P::kT;
   extern __shared__ uint4 dynamic[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int total = __builtin_amdgcn_readfirstlane(plan.segment[0]);
   const int cut = blockIdx.y % cuts, units = static_cast<int>(m.units);
-  int seg = blockIdx.y / cuts * many;
-  const int end = min(total, seg + many);
-  if (seg >= end) return;
+  const int seg = blockIdx.y / cuts;
+  if (seg >= __builtin_amdgcn_readfirstlane(static_cast<int>(plan.segment[0]))) return;
   const int u0 = units * cut / cuts, u1 = units * (cut + 1) / cuts;
   if (u0 >= u1) return;
   const int c = lane & 15, q = lane >> 4;
@@ -839,54 +839,36 @@ __global__ __launch_bounds__(512, WavesPerSimd(GC, F)) void MoeDownKernel(Matrix
   float *out = parts + static_cast<int64_t>(cut) * pairs * width +
                static_cast<int64_t>(blockIdx.x) * 256 + wave * 32 + 4 * q;
   P pipe(reinterpret_cast<const uint8_t *>(dynamic), lane, wave);
-  auto enter = [&](int s) __attribute__((always_inline)) {
-    const uint32_t w = __builtin_amdgcn_readfirstlane(plan.segment[1 + s]);
-    pipe.Segment(m, Expert(w), group, fh, Count(w),
-                 [&](int i) { return plan.pair[Offset(w) + i]; });
-  };
-  // The next item to copy.
-  int next_seg = seg, next_u = u0;
-  auto issue = [&](int stage) __attribute__((always_inline)) {
-    pipe.Issue(fh, next_u, stage);
-    if (next_u + 1 < u1) {
-      ++next_u;
-    } else if (next_seg + 1 < end) {
-      next_u = u0;
-      enter(++next_seg);
-    }  // past the end: the last again
-  };
-  enter(seg);
+  const uint32_t now = __builtin_amdgcn_readfirstlane(plan.segment[1 + seg]);
+  const int n = Count(now), groups = (n + kT - 1) / kT;
+  pipe.Segment(m, Expert(now), group, fh, n, [&](int i) { return plan.pair[Offset(now) + i]; });
 #pragma unroll
-  for (int p = 0; p < NS - 1; ++p) issue(p);
+  for (int p = 0; p < NS - 1; ++p) pipe.Issue(fh, min(u0 + p, u1 - 1), p);
   int stage = 0;
-  for (; seg < end; ++seg) {
-    const uint32_t now = __builtin_amdgcn_readfirstlane(plan.segment[1 + seg]);
-    const int n = Count(now), groups = (n + kT - 1) / kT;
-    floatx4 acc[2][GC];
+  floatx4 acc[2][GC];
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+  for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int g = 0; g < GC; ++g) acc[r][g] = floatx4{0.f, 0.f, 0.f, 0.f};
-    for (int u = u0; u < u1; ++u) {
-      P::template Wait<P::kOps *(NS - 2)>();
-      issue(stage == 0 ? NS - 1 : stage - 1);
-      pipe.Multiply(stage, groups, acc);
-      stage = stage + 1 == NS ? 0 : stage + 1;
-    }
+    for (int g = 0; g < GC; ++g) acc[r][g] = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int u = u0; u < u1; ++u) {
+    P::template Wait<P::kOps *(NS - 2)>();
+    pipe.Issue(fh, min(u + NS - 1, u1 - 1), stage == 0 ? NS - 1 : stage - 1);
+    pipe.Multiply(stage, groups, acc);
+    stage = stage + 1 == NS ? 0 : stage + 1;
+  }
 #pragma unroll
-    for (int g = 0; g < GC; ++g) {
-      const int j = g * kT + c;
-      const bool on = c < kT && j < n;
-      const int at = Offset(now) + (on ? j : 0);
-      const float p = plan.weight[at];
-      float *to = out + plan.pair[at] * width;
+  for (int g = 0; g < GC; ++g) {
+    const int j = g * kT + c;
+    const bool on = c < kT && j < n;
+    const int at = Offset(now) + (on ? j : 0);
+    const float p = plan.weight[at];
+    float *to = out + plan.pair[at] * width;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        floatx4 y;
+    for (int r = 0; r < 2; ++r) {
+      floatx4 y;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) y[v] = p * JoinDigits<ND, ONE>(acc[r][g][v] * weight);
-        if (on) *reinterpret_cast<floatx4 *>(to + 16 * r) = y;
-      }
+      for (int v = 0; v < 4; ++v) y[v] = p * JoinDigits<ND, ONE>(acc[r][g][v] * weight);
+      if (on) *reinterpret_cast<floatx4 *>(to + 16 * r) = y;
     }
   }
   P::template Wait<0>();  // no copy may land after the workgroup
@@ -1008,7 +990,7 @@ struct Shape {
   bool choose;  // one token: the gate/up kernel makes its choice
   int groups;   // column groups per pass over an expert's rows
   int segments; // at most
-  int cuts, many;  // down: runs of 1 / cuts of a segment, or of `many` segments
+  int cuts;     // down: runs of 1 / cuts of a segment
 };
 
 Shape PickShape(const Layer &l, int tokens, int ND) {
@@ -1032,8 +1014,9 @@ Shape PickShape(const Layer &l, int tokens, int ND) {
   // Down: about two workgroups a CU, of at least four units.
   const double met = l.experts * (1.0 - std::pow(1.0 - static_cast<double>(l.top_k) / l.experts, tokens));
   const double blocks_down = std::max(1.0, met) * CeilDiv(l.hidden, 256);
-  s.cuts = s.many = 1;
-  while (blocks_down * s.cuts < 1.5 * l.num_cus && l.down.units >= 8 * s.cuts && s.cuts < 8) s.cuts *= 2;
+  s.cuts = 1;
+  while (blocks_down * s.cuts < 1.5 * l.num_cus && l.down.units >= 8 * s.cuts && s.cuts < 8)
+    s.cuts *= 2;
   return s;
 }
 
@@ -1107,9 +1090,9 @@ hipError_t LaunchDown(const Layer &l, const Work &w, const Shape &shape, int tok
   const int pairs = tokens * l.top_k;
   const int64_t width = PartWidth(l);
   const dim3 grid(static_cast<unsigned>(width / 256),
-                  static_cast<unsigned>(CeilDiv(shape.segments, shape.many) * shape.cuts));
+                  static_cast<unsigned>(shape.segments * shape.cuts));
   hipLaunchKernelGGL((MoeDownKernel<ND, ONE, GC, F, ZP, NS>), grid, dim3(512), P::kLds, s, l.down,
-                     w.fh, w.plan, w.parts, pairs, shape.cuts, shape.many, width);
+                     w.fh, w.plan, w.parts, pairs, shape.cuts, width);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((MoeSumKernel<T>),
