@@ -70,11 +70,12 @@ int mnb_fp8_workspace_bytes(const mnb_fp8_plan *plan, int64_t M, int32_t a_type,
 
 /* Y[M, N] of y_type (MNB_TYPE_FLOAT, _FLOAT16 or _BFLOAT16; sums in fp32,
  * rounded once; for a 16-bit Y the products within a group of eight are cut off
- * 2^-13 below the group's largest, about 1.4e-5 of Y) from dense rows dA [M, K] of a_type: MNB_TYPE_FLOAT8E4M3FN
- * codes with dAScales [M, ceil(K / 128)], or values of another type with
- * dAScales NULL, quantized as by mnb_fp8_quantize. dA 16-byte aligned
- * (MNB_ERR_BAD_SHAPE otherwise, as for the workspace), dY aligned to 16 bytes.
- * M == 0 is a no-op; M <= 2^30 and M * N <= 2^36. Asynchronous on `stream`. */
+ * 2^-13 below the group's largest, about 1.4e-5 of Y) from dense rows dA [M, K]
+ * of a_type: MNB_TYPE_FLOAT8E4M3FN codes with dAScales [M, ceil(K / 128)], or
+ * values of another type with dAScales NULL, quantized as by mnb_fp8_quantize.
+ * dA, dY and the workspace are aligned to 16 bytes (MNB_ERR_BAD_SHAPE otherwise);
+ * dY and the workspace overlap nothing else. M == 0 is a no-op; M <= 2^30 and
+ * M * N <= 2^36. Asynchronous on `stream`. */
 int mnb_fp8_run(const mnb_fp8_plan *plan, int64_t M, int32_t a_type, const void *dA,
                 const float *dAScales, int32_t y_type, void *dY, void *dWorkspace,
                 size_t workspace_bytes, void *stream);

@@ -85,7 +85,8 @@ int mnb_moe_workspace_bytes(const mnb_moe_plan *plan, int64_t T, int32_t x_type,
  * router's place, NULL to take the router's (MNB_ERR_NULL_POINTER where the
  * plan has none). A NaN logit counts as -inf. dIds (int32 [T, top_k]) and
  * dWeights (fp32 [T, top_k]) receive the choice, largest logit first, and p;
- * either may be NULL. T == 0 is a no-op; T <= 2^24. Asynchronous on `stream`. */
+ * either may be NULL. What a run writes overlaps nothing else. T == 0 is a no-op;
+ * T <= 2^24. Asynchronous on `stream`. */
 int mnb_moe_run(const mnb_moe_plan *plan, int64_t T, int32_t x_type, const void *dX,
                 const float *dLogits, void *dY, int32_t *dIds, float *dWeights, void *dWorkspace,
                 size_t workspace_bytes, void *stream);

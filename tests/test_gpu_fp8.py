@@ -88,6 +88,10 @@ SHAPES = [
     (64, 2048, 192), (65, 128, 64), (65, 1500, 701), (100, 4096, 512), (128, 130, 128),
     (129, 256, 129), (200, 4096, 2048), (255, 640, 300), (256, 256, 256), (257, 2304, 257),
     (333, 2500, 5001), (1000, 1024, 1), (1024, 512, 8192), (2049, 896, 8200),
+    # few blocks of K under several tiles a workgroup, one block, an odd width
+    (4096, 256, 8192), (4100, 300, 4104), (4096, 128, 4096), (2049, 896, 8201),
+    # 129 to 256 rows, K split and whole, and the last row and column of a tile alone
+    (131, 4000, 300), (250, 1000, 77), (254, 130, 20001), (16, 127, 4097), (64, 1025, 16),
 ]
 
 

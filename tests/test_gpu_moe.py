@@ -129,6 +129,27 @@ SHAPES = [
     (64, 300, 260, 1, 1, 16, True, "float32", False),
     (65, 256, 256, 12, 4, 32, True, "bfloat16", True),
     (150, 200, 140, 5, 2, 16, False, "float32", True),
+    # one token: of more experts than a workgroup chooses from, 32 of 256, on wide
+    # experts (down in parts), with few blocks and with many
+    (1, 260, 200, 300, 4, 16, True, "bfloat16", False),
+    (1, 128, 64, 256, 32, 64, False, "float32", False),
+    (1, 256, 8200, 9, 8, 32, True, "float32", True),
+    (1, 300, 8200, 9, 8, 16, False, "bfloat16", True),
+    (1, 512, 2200, 9, 8, 16, True, "float16", True),
+    (1, 33, 2200, 12, 8, 256, False, "float32", True),
+    # the last number of tokens whose sums stay in down's workgroups, and the next
+    (8, 512, 2200, 9, 3, 16, True, "bfloat16", True),
+    (8, 130, 700, 32, 32, 32, True, "float32", True),
+    (8, 256, 4400, 24, 8, 64, False, "float32", True),
+    (9, 512, 2200, 9, 3, 16, False, "float32", True),
+    # two and four column groups with every width of block
+    (64, 200, 260, 4, 2, 16, True, "bfloat16", True),
+    (64, 200, 260, 4, 2, 32, False, "bfloat16", True),
+    (64, 300, 130, 4, 2, 64, True, "float32", False),
+    (64, 130, 300, 3, 3, 128, True, "float32", True),
+    (48, 700, 200, 16, 4, 32, True, "bfloat16", True),
+    (24, 700, 333, 8, 2, 64, False, "float32", True),
+    (30, 256, 128, 16, 2, 16, True, "float32", True),
 ]
 
 
