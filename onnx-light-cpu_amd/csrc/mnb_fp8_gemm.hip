@@ -279,7 +279,12 @@ __global__ __launch_bounds__(64 * WAVES) void Fp8StreamLdsKernel(
 // block visible stands before the last group, when this block's reads are done:
 // its stage takes the copies of the block NS ahead, and the next block's weight
 // fragments are read behind their last use (with the barrier between the blocks
-// 47 us instead of 44 at 200 x 4096 x 28672).
+// 47 us instead of 44 at 200 x 4096 x 28672). Four wavefronts, one per SIMD, and
+// two workgroups a CU where LDS allows: one's waits are the other's work (300 x 4096
+// x 4096, fp32 Y: 31 us with 128 x 128 tiles of eight wavefronts and K in two parts,
+// 27 with 64 x 128 of four). What bounds it: the start and the end of a tile (10 us of
+// the 20 at 333 x 2500 x 5001, fp32 Y, with one block of K), then copies, LDS reads
+// and MFMAs about equally.
 template <int MI, int WM, int WN, int NS, bool EXACT, typename T>
 __global__ __launch_bounds__(64 * WM *WN) void Fp8TileKernel(
     const uint8_t *__restrict__ W, const float *__restrict__ SW, const uint8_t *__restrict__ A,
@@ -691,7 +696,19 @@ __global__ __launch_bounds__(256) void Fp8SumKernel(const float *__restrict__ P,
   }
 }
 
-constexpr int64_t kStreamRows = 64;
+// Whether M rows take the kernels that stream the weights. Their workgroups of 16
+// columns each read all rows; past one workgroup a CU, and with more rows, that
+// costs more than the tiles' longer start (us, stream and tile, bf16 Y, weights
+// not in a cache: 48 rows of K = 4096, N = 4096: 7 and 12, N = 14336: 28 and 21; 20
+// rows of the same: 7 and 10, 20 and 16; 16 rows of 8192 x 8192: 20 and 19; one row
+// of K = 4096, N = 28672: 27 and 24; of K = 14336, N = 4096 64 rows: 26 and 22, 48
+// rows 23 and 20, but 17 and 18 with the weights in the last cache).
+bool Streams(const Weight &w, int64_t M) {
+  if (M > 64) return false;
+  const int64_t mib = w.N * w.nb * kBlock >> 20;
+  if (w.N > 16 * static_cast<int64_t>(w.num_cus)) return mib < (M <= 8 ? 96 : M <= 16 ? 48 : 24);
+  return M <= 48 || mib < 48;
+}
 
 struct TileShape {
   int rows, cols, splits;
@@ -699,16 +716,22 @@ struct TileShape {
 
 // exact: an fp32 Y.
 TileShape PickTile(const Weight &w, int64_t M, bool exact) {
-  // 16-bit results: large tiles where they fill the chip (rows of whole vectors); for
-  // 129 to 256 rows tiles of all of them, so that the weights are read once (200 x
-  // 4096 x 28672: 44 us, 48 with 128 rows). Else 128 x 128.
-  TileShape t{128, 128, 1};
+  // 16-bit results: large tiles where they fill the chip (rows of whole vectors).
   if (!exact && w.nb >= 2 && w.N % 8 == 0 && CeilDiv(M, 256) * CeilDiv(w.N, 256) >= w.num_cus)
     return TileShape{256, 256, 1};
-  if (!exact && M > 128 && M <= 256) t.rows = 256;
-  // K is split so that every CU has work, of at least four blocks each.
+  // 64 x 128, two workgroups a CU. Larger ones take fewer reads of LDS and the
+  // caches: 128 rows where they still fill the chip (512 x 4096 x 14336, bf16: 48 us
+  // instead of 58), and all of 129 to 256 rows for 16-bit results where half the chip
+  // has one (250 x 4096 x 20480: 40 us instead of 49; with fewer the other half
+  // counts: 200 x 4096 x 14336: 39 instead of 30).
+  TileShape t{64, 128, 1};
+  if (!exact && M > 128 && M <= 256 && 2 * CeilDiv(w.N, 128) > w.num_cus) t.rows = 256;
+  else if (M > 64 && CeilDiv(M, 128) * CeilDiv(w.N, 128) >= w.num_cus) t.rows = 128;
+  // K is split so that every CU has work, of at least eight blocks each, ten for 16-bit
+  // results: the second launch takes as long (333 x 2048 x 2560, bf16: 13 us in two
+  // parts of eight, 10 whole; 65 x 2048 x 1024, fp32: 12 and 15).
   const int64_t tiles = CeilDiv(M, t.rows) * CeilDiv(w.N, t.cols);
-  const int64_t s = std::min<int64_t>({w.num_cus / tiles, w.nb / 4, 8});
+  const int64_t s = std::min<int64_t>({w.num_cus / tiles, w.nb / (exact ? 8 : 10), 8});
   t.splits = static_cast<int>(std::max<int64_t>(1, s));
   return t;
 }
@@ -747,10 +770,11 @@ hipError_t TileLaunch(const Weight &w, const TileShape &t, int64_t M, const uint
   return hipGetLastError();
 }
 
-template <bool EXACT, typename T>
+template <typename T>
 hipError_t TileT(const Weight &w, const TileShape &t, int64_t M, const uint8_t *A, int64_t lda,
                  const float *sa, T *Y, hipStream_t s) {
-  if constexpr (sizeof(T) == 2) {  // whole K, so Y itself
+  constexpr bool kExact = sizeof(T) == 4;
+  if constexpr (!kExact) {
     if (t.cols == 256) {
       const int64_t tiles_m = CeilDiv(M, 256), tiles_n = CeilDiv(w.N, 256);
       const int64_t wgs = std::min<int64_t>(tiles_m * tiles_n, w.num_cus);
@@ -760,17 +784,16 @@ hipError_t TileT(const Weight &w, const TileShape &t, int64_t M, const uint8_t *
                          static_cast<int>(tiles_n), static_cast<int>(w.groups));
       return hipGetLastError();
     }
+    if (t.rows == 256) return TileLaunch<8, 2, 2, 3, kExact, T>(w, t, M, A, lda, sa, Y, s);
   }
-  if constexpr (!EXACT) {
-    if (t.rows == 256) return TileLaunch<8, 2, 2, 3, EXACT, T>(w, t, M, A, lda, sa, Y, s);
-  }
-  return TileLaunch<2, 4, 2, 4, EXACT, T>(w, t, M, A, lda, sa, Y, s);
+  if (t.rows == 128) return TileLaunch<4, 2, 2, 2, kExact, T>(w, t, M, A, lda, sa, Y, s);
+  return TileLaunch<2, 2, 2, 3, kExact, T>(w, t, M, A, lda, sa, Y, s);
 }
 
 template <typename T>
 hipError_t ProductT(const Weight &w, int64_t M, const uint8_t *A, int64_t lda, const float *sa,
                     void *Y, void *work, hipStream_t s) {
-  if (M <= kStreamRows) {
+  if (Streams(w, M)) {
     const int m = static_cast<int>(M);
     switch ((M + 15) / 16) {
     case 1: return StreamT<T>(w, m, A, lda, sa, Y, s);
@@ -781,9 +804,10 @@ hipError_t ProductT(const Weight &w, int64_t M, const uint8_t *A, int64_t lda, c
   }
   constexpr bool kExact = sizeof(T) == 4;
   const TileShape t = PickTile(w, M, kExact);
-  if (t.splits == 1) return TileT<kExact, T>(w, t, M, A, lda, sa, static_cast<T *>(Y), s);
+  if (t.splits == 1) return TileT<T>(w, t, M, A, lda, sa, static_cast<T *>(Y), s);
   float *parts = static_cast<float *>(work);
-  hipError_t e = TileT<kExact, float>(w, t, M, A, lda, sa, parts, s);
+  // Larger tiles are never split: they fill half the chip.
+  hipError_t e = TileLaunch<2, 2, 2, 3, kExact, float>(w, t, M, A, lda, sa, parts, s);
   if (e != hipSuccess) return e;
   const int64_t mn = M * w.N;
   hipLaunchKernelGGL((Fp8SumKernel<T>),
@@ -795,14 +819,13 @@ hipError_t ProductT(const Weight &w, int64_t M, const uint8_t *A, int64_t lda, c
 } // namespace
 
 size_t WorkBytes(const Weight &w, int64_t M) {
-  if (M <= kStreamRows) return 0;
+  if (Streams(w, M)) return 0;
   const int splits = std::max(PickTile(w, M, false).splits, PickTile(w, M, true).splits);
   return splits == 1 ? 0 : static_cast<size_t>(splits) * M * w.N * sizeof(float);
 }
 
 const char *ProductKernelName(const Weight &w, int64_t M) {
-  if (M <= 16) return "Fp8StreamKernel";
-  if (M <= kStreamRows) return "Fp8StreamLdsKernel";
+  if (Streams(w, M)) return M <= 16 ? "Fp8StreamKernel" : "Fp8StreamLdsKernel";
   return PickTile(w, M, false).cols == 256 ? "Fp8WideKernel" : "Fp8TileKernel";
 }
 
