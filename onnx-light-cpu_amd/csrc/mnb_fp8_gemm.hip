@@ -702,12 +702,13 @@ __global__ __launch_bounds__(256) void Fp8SumKernel(const float *__restrict__ P,
 // not in a cache: 48 rows of K = 4096, N = 4096: 7 and 12, N = 14336: 28 and 21; 20
 // rows of the same: 7 and 10, 20 and 16; 16 rows of 8192 x 8192: 20 and 19; one row
 // of K = 4096, N = 28672: 27 and 24; of K = 14336, N = 4096 64 rows: 26 and 22, 48
-// rows 23 and 20, but 17 and 18 with the weights in the last cache).
+// rows 23 and 20, but 17 and 18 with the weights in the last cache; of K = 28672,
+// N = 4096 40 rows: 40 and 29).
 bool Streams(const Weight &w, int64_t M) {
   if (M > 64) return false;
   const int64_t mib = w.N * w.nb * kBlock >> 20;
   if (w.N > 16 * static_cast<int64_t>(w.num_cus)) return mib < (M <= 8 ? 96 : M <= 16 ? 48 : 24);
-  return M <= 48 || mib < 48;
+  return M <= 8 || mib < (M <= 48 ? 96 : 48);
 }
 
 struct TileShape {

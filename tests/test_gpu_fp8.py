@@ -94,6 +94,7 @@ SHAPES = [
     (131, 4000, 300), (250, 1000, 77), (254, 130, 20001), (16, 127, 4097), (64, 1025, 16),
     # up to 64 rows on large weights, in tiles
     (1, 4096, 28672), (12, 8192, 6400), (33, 3000, 9001), (64, 12800, 4096), (17, 1000, 30001),
+    (9, 28672, 4096),
     # tiles of 128 rows
     (300, 300, 14401), (600, 129, 7000), (257, 4096, 11000),
 ]
