@@ -316,3 +316,46 @@ def test_streams_threads_and_graph(pkg, cuda):
         eager = op(x)
         torch.cuda.synchronize()
         assert torch.equal(out, eager)
+
+
+def test_two_graphs_and_threads(pkg, cuda):
+    """Two captured calls of one object, with K in parts and without, replayed between
+    eager ones, and calls of four threads on one stream: each has a workspace of its
+    own."""
+    import threading
+    import torch
+    K, N = 4096, 640
+    _, _, W, sw = _problem(1, K, N, 29, cuda)
+    op = pkg.MatMulFp8(K, N).prepare_device(W, sw / 4096)
+    graphs = []
+    for m in (100, 5):
+        x = torch.randn(m, K, device=cuda)
+        op(x)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = op(x)
+        graphs.append((g, x, out))
+    for _ in range(3):
+        for g, x, out in graphs:
+            x.normal_()
+            g.replay()
+        for g, x, out in graphs:
+            eager = op(x)
+            torch.cuda.synchronize()
+            assert torch.equal(out, eager)
+    xs = [torch.randn(m, K, device=cuda) for m in (100, 70, 33, 257)]
+    want = [op(x) for x in xs]
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(i):
+        got[i] = [op(xs[i]) for _ in range(8)]
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for ys, w in zip(got, want):
+        assert all(torch.equal(y, w) for y in ys)

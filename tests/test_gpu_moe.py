@@ -398,3 +398,27 @@ def test_decoder_half_layer(pkg, orc, cuda):
     ref, err = _layer64(hidden, want_ids, want_p,
                         [_dense(v, n) for v, n in zip(ws, (H, H, I))], 128, U["float32"])
     _check(y, ref, err)
+
+
+def test_threads(pkg, cuda):
+    """Calls of four threads on one stream, each with a workspace of its own."""
+    import threading
+    import torch
+    x, router, ws = _problem(70, 256, 300, 12, 32, True, "float16", 37, cuda)
+    op = pkg.MatMulNBitsMoE(256, 300, 12, 3, block_size=32).prepare_device(router, *ws)
+    xs = [x[:1], x[1:9], x[9:40], x]
+    want = [op(v) for v in xs]
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(i):
+        got[i] = [op(xs[i]) for _ in range(8)]
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for ys, w in zip(got, want):
+        assert all(torch.equal(y, w) for y in ys)
