@@ -997,12 +997,21 @@ Shape PickShape(const Layer &l, int tokens, int ND) {
   Shape s;
   s.entries = std::min(tokens * l.top_k, l.experts);
   const int64_t blocks = s.entries * CeilDiv(l.intermediate, 128);  // of 128 channels
-  s.narrow = tokens <= kNarrowTokens && blocks < 2 * l.num_cus;
-  s.split = s.narrow && 4 * blocks <= 2 * l.num_cus;
-  // A workgroup's choice among more experts takes longer than a launch of its own.
+  // Narrow workgroups, and down with the sum over the experts, where blocks of 128
+  // channels leave CUs idle (us, narrow and not; one token of hidden 4096, experts of
+  // 14336: 1 chosen 35 and 50, 2 chosen 50 and 57, 4 chosen 91 and 85; 2 tokens of
+  // 4096 x 2048, 2 of 16: 26 and 40; 4 tokens of 2048 x 1024, 4 of 64: 32 and 30; 8
+  // tokens, 6 of 64: 54 and 44).
+  s.narrow = tokens <= kNarrowTokens && blocks < (tokens == 1 ? l.num_cus : 3 * l.num_cus / 8);
+  // The units over four wavefronts each: one token of 2048 x 1024, 6 of 64: 19 us,
+  // 23 without; one of 4096 x 14336, 2 of 8, does not fill them: 49 both.
+  s.split = s.narrow && 2 * blocks <= l.num_cus;
+  // A workgroup's choice among more experts takes longer than a launch of its own (6 of
+  // 64: 19 us, 21 with a launch).
   s.choose = tokens == 1 && l.experts <= 256;
   // What most experts' tokens fill: their mean share and two standard deviations
-  // of even choices.
+  // of even choices (32 tokens of 4096 x 4096, 2 of 8: four groups 62 us, one 84; 64
+  // of 2048 x 1024, 8 of 64: two 81, one 92).
   const int group = tokens == 1 ? 1 : ND == 3 ? kTokens<3> : kTokens<2>;
   const double mean = static_cast<double>(tokens) * l.top_k / l.experts;
   const double most = std::min<double>(tokens, mean + 2.0 * std::sqrt(mean));
@@ -1011,7 +1020,8 @@ Shape PickShape(const Layer &l, int tokens, int ND) {
              : most <= 2 * group || l.folds == 8     ? 2
                                                      : 4;
   s.segments = s.entries + tokens * l.top_k / (s.groups * group);
-  // Down: about two workgroups a CU, of at least four units.
+  // Down: about two workgroups a CU, of at least four units (32 tokens of 4096 x 4096,
+  // 2 of 8: 62 us, 68 with whole rows; 4 of 4096 x 14336: 120 and 180).
   const double met = l.experts * (1.0 - std::pow(1.0 - static_cast<double>(l.top_k) / l.experts, tokens));
   const double blocks_down = std::max(1.0, met) * CeilDiv(l.hidden, 256);
   s.cuts = 1;
@@ -1115,11 +1125,15 @@ template <int ND, bool ONE, int GC, int F, bool ZP, typename T>
 hipError_t LaunchExperts(const Layer &l, const Work &w, const Shape &shape, int tokens, T *Y,
                          const Choice &choice, hipStream_t s) {
   const int pairs = tokens * l.top_k;
-  hipError_t e;
+  hipError_t e = hipSuccess;
   if constexpr (GC == 1) {
     if (shape.narrow) {
-      if (shape.split) e = LaunchGateUpC<ND, ONE, GC, F, ZP, 2, 4>(l, w, shape, pairs, choice, s);
-      else e = LaunchGateUpC<ND, ONE, GC, F, ZP, 2, 1>(l, w, shape, pairs, choice, s);
+      bool split = true;
+      if constexpr (ONE) {  // several tokens' narrow layers are always small enough
+        split = shape.split;
+        if (!split) e = LaunchGateUpC<ND, ONE, GC, F, ZP, 2, 1>(l, w, shape, pairs, choice, s);
+      }
+      if (split) e = LaunchGateUpC<ND, ONE, GC, F, ZP, 2, 4>(l, w, shape, pairs, choice, s);
       return e != hipSuccess ? e : LaunchDownNarrow<ND, ONE, F, ZP, T>(l, w, shape, tokens, Y, s);
     }
   }

@@ -142,6 +142,11 @@ SHAPES = [
     (8, 130, 700, 32, 32, 32, True, "float32", True),
     (8, 256, 4400, 24, 8, 64, False, "float32", True),
     (9, 512, 2200, 9, 3, 16, False, "float32", True),
+    # several tokens on either side of narrow workgroups
+    (4, 300, 1000, 64, 4, 128, True, "bfloat16", True),
+    (2, 640, 2000, 16, 2, 32, False, "float32", True),
+    (8, 200, 120, 100, 12, 16, True, "float32", False),
+    (8, 200, 120, 100, 11, 64, True, "bfloat16", True),
     # two and four column groups with every width of block
     (64, 200, 260, 4, 2, 16, True, "bfloat16", True),
     (64, 200, 260, 4, 2, 32, False, "bfloat16", True),
