@@ -456,8 +456,8 @@ __global__ __launch_bounds__(64 * WM *WN) void Fp8TileKernel(
   for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
-      *reinterpret_cast<floatx4 *>(tile + (16 * (wm * MI + i) + c) * kPitch + wn * 64 + 16 * qd + 4 * j) =
-          acc[i][j];
+      *reinterpret_cast<floatx4 *>(tile + (16 * (wm * MI + i) + c) * kPitch + wn * 64 + 16 * qd +
+                                   4 * j) = acc[i][j];
   __syncthreads();
   for (int row = wave; row < rows; row += kWaves) {
 #pragma unroll
@@ -645,9 +645,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         if constexpr (j == 3) f[(i + 1) % 2] = s_next * (i + 1 < MI ? scale : next_scale);
         // The block after next into this block's stage: the weights and the first four
         // groups of rows, then the others and the row scales.
-        if constexpr (k >= kMid && k < kMid + 4) copy(std::integral_constant<int, 4 + k - kMid>{}, from, cb, st);
-        if constexpr (k >= kMid + 4 && k < kMid + 6) copy(std::integral_constant<int, k - kMid - 4>{}, from, cb, st);
-        if constexpr (k >= kLast && k < kLast + 2) copy(std::integral_constant<int, 2 + k - kLast>{}, from, cb, st);
+        if constexpr (k >= kMid && k < kMid + 4)
+          copy(std::integral_constant<int, 4 + k - kMid>{}, from, cb, st);
+        if constexpr (k >= kMid + 4 && k < kMid + 6)
+          copy(std::integral_constant<int, k - kMid - 4>{}, from, cb, st);
+        if constexpr (k >= kLast && k < kLast + 2)
+          copy(std::integral_constant<int, 2 + k - kLast>{}, from, cb, st);
         if constexpr (k == kLast + 2) copy(std::integral_constant<int, 8>{}, from, cb, st);
         __builtin_amdgcn_sched_barrier(0);
       };

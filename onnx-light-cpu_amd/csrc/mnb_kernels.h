@@ -46,13 +46,7 @@ __device__ __forceinline__ void CopyToLds16S(const void *sbase, uint32_t voff, u
                    : "s"(lds_base), "v"(voff), "s"(sbase)
                    : "memory", "m0");
 }
-// Copies 4 bytes per lane from src to LDS byte lds_base + 4 lane (as CopyToLds16).
-__device__ __forceinline__ void CopyToLds4(const void *src, uint32_t lds_base) {
-  __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
-                   :
-                   : "s"(lds_base), "v"(src)
-                   : "memory", "m0");
-}
+// The same with 4 bytes per lane, landing at lds_base + 4 lane.
 __device__ __forceinline__ void CopyToLds4S(const void *sbase, uint32_t voff, uint32_t lds_base) {
   __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
                    :

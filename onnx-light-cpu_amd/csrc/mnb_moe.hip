@@ -577,7 +577,8 @@ constexpr int WavesPerSimd(int gc, int folds) {
 // (gate and up) for each of GROUPS wavefronts that share a pipe, or, with KS runs
 // of the units, for each of GROUPS * KS wavefronts with pipes of their own.
 template <int ND, bool ONE, int GC, int F, bool ZP, int GROUPS, int KS, int NS, bool CHOOSE>
-__global__ __launch_bounds__(64 * GROUPS *KS, GROUPS == 8 ? WavesPerSimd(GC, F) : 1) void MoeGateUpKernel(
+__global__ __launch_bounds__(64 * GROUPS *KS,
+                             GROUPS == 8 ? WavesPerSimd(GC, F) : 1) void MoeGateUpKernel(
     Matrix m, Fixed fx, Fixed fh, const int32_t *__restrict__ pair_expert,
     const float *__restrict__ pair_weight, Plan plan, int pairs, int top_k, bool by_expert,
     Choice choice) {
@@ -1022,7 +1023,8 @@ Shape PickShape(const Layer &l, int tokens, int ND) {
   s.segments = s.entries + tokens * l.top_k / (s.groups * group);
   // Down: about two workgroups a CU, of at least four units (32 tokens of 4096 x 4096,
   // 2 of 8: 62 us, 68 with whole rows; 4 of 4096 x 14336: 120 and 180).
-  const double met = l.experts * (1.0 - std::pow(1.0 - static_cast<double>(l.top_k) / l.experts, tokens));
+  const double share = static_cast<double>(l.top_k) / l.experts;
+  const double met = l.experts * (1.0 - std::pow(1.0 - share, tokens));
   const double blocks_down = std::max(1.0, met) * CeilDiv(l.hidden, 256);
   s.cuts = 1;
   while (blocks_down * s.cuts < 1.5 * l.num_cus && l.down.units >= 8 * s.cuts && s.cuts < 8)
