@@ -115,7 +115,9 @@ __device__ __forceinline__ void StoreRow(T *p, const float *v, int64_t n, bool w
 // ---- few rows: the weights streamed once ------------------------------------
 //
 // Up to 16 rows: a workgroup takes 16 columns and all rows, one fragment each; its
-// wavefronts take the blocks of K in turn, D of them in flight, and add up in LDS.
+// wavefronts take the blocks of K in turn, D of them in flight, and add up in LDS. One
+// row of 4096 x 6144: 6.3 to 7.6 us, a launch and two round trips (3.3 TB/s); of 14336 x
+// 4096 13 us (4.6 TB/s).
 template <int WAVES, int D, bool EXACT, typename T>
 __global__ __launch_bounds__(64 * WAVES) void Fp8StreamKernel(
     const uint8_t *__restrict__ W, const float *__restrict__ SW, const uint8_t *__restrict__ A,
@@ -182,7 +184,8 @@ __global__ __launch_bounds__(64 * WAVES) void Fp8StreamKernel(
 
 // 17 to 64 rows: the rows, and with them the weights and the row scales, pass
 // through LDS, each wavefront's own blocks NS deep, so that the rows are copied by
-// whole lines (gathered into registers they bound it: 32 us at 48 x 14336 x 4096).
+// whole lines (gathered into registers they bound it: 32 us at 48 x 14336 x 4096, 16.6
+// so). Bound by those rows, which every 16 columns read again.
 template <int MC, int WAVES, int NS, bool EXACT, typename T>
 __global__ __launch_bounds__(64 * WAVES) void Fp8StreamLdsKernel(
     const uint8_t *__restrict__ W, const float *__restrict__ SW, const uint8_t *__restrict__ A,

@@ -575,7 +575,10 @@ constexpr int WavesPerSimd(int gc, int folds) {
 
 // Gate/up: workgroup (b, i) the channels of block b of entry i's expert, 16
 // (gate and up) for each of GROUPS wavefronts that share a pipe, or, with KS runs
-// of the units, for each of GROUPS * KS wavefronts with pipes of their own.
+// of the units, for each of GROUPS * KS wavefronts with pipes of their own. Bound by
+// reading: 64 tokens of 4096 x 14336, 2 of 8 experts, 105 us (4.8 TB/s; about 10 less
+// without the products), one token 25 us (5.1 TB/s); one of 2048 x 1024, 6 of 64, 9 us,
+// its launch and two round trips.
 template <int ND, bool ONE, int GC, int F, bool ZP, int GROUPS, int KS, int NS, bool CHOOSE>
 __global__ __launch_bounds__(64 * GROUPS *KS,
                              GROUPS == 8 ? WavesPerSimd(GC, F) : 1) void MoeGateUpKernel(
@@ -726,7 +729,8 @@ __global__ __launch_bounds__(64 * GROUPS *KS,
 // Down, few tokens on few experts: a workgroup takes 16 columns of Y. The
 // items (segment, unit) of the layer are cut into eight equal runs, one for each
 // wavefront and its pipe, which adds each segment's rows, times the tokens'
-// weights, to sums of its own; they join in order.
+// weights, to sums of its own; they join in order. One token of 4096 x 14336, 2 of 8:
+// 20 us, 3.1 TB/s; neither copies eight deep nor sixteen wavefronts changed that.
 template <int ND, bool ONE, int F, bool ZP, int NS, typename T>
 __global__ __launch_bounds__(512) void MoeDownNarrowKernel(Matrix m, Fixed fh, Plan plan,
                                                            T *__restrict__ Y, int pairs,
@@ -819,7 +823,7 @@ __global__ __launch_bounds__(512) void MoeDownNarrowKernel(Matrix m, Fixed fh, P
 
 // Down otherwise: a workgroup takes 256 columns of Y and part blockIdx.y % cuts of the
 // units of one segment. Every pair's row, times its weight, goes to parts
-// [cuts][pairs][width].
+// [cuts][pairs][width]. 64 tokens of 4096 x 14336, 2 of 8: 53 us, 4.8 TB/s.
 template <int ND, bool ONE, int GC, int F, bool ZP, int NS>
 __global__ __launch_bounds__(512, WavesPerSimd(GC, F)) void MoeDownKernel(Matrix m, Fixed fh, Plan plan,
                                                      float *__restrict__ parts, int pairs, int cuts,
