@@ -667,7 +667,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     now = next;
     fold(std::integral_constant<int, kSlots - 2>{});
     fold(std::integral_constant<int, kSlots - 1>{});
-    part[(kSlots - 2) % 4] = part[(kSlots - 1) % 4] = zero;  // the next block folds them again
+    // The next tile's first block folds them again, by a factor of its own: this tile's
+    // last one may be infinite or NaN, and 0 times that would stay in the next tile's sums.
+    part[(kSlots - 2) % 4] = part[(kSlots - 1) % 4] = zero;
+    f[1] = 0.0f;
     int tm, tn;
     TileOf(tile, tiles_m, tiles_n, tm, tn);
     const int64_t m0 = static_cast<int64_t>(tm) * kWideTile;

@@ -359,3 +359,39 @@ def test_two_graphs_and_threads(pkg, cuda):
     torch.cuda.synchronize()
     for ys, w in zip(got, want):
         assert all(torch.equal(y, w) for y in ys)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("M,K,N", [(4100, 512, 8192), (5000, 256, 4096)])
+def test_nonfinite_rows_stay_alone_among_wide_tiles(pkg, cuda, M, K, N, dtype):
+    """An infinity or a NaN at every place of a tile, under as many tiles as make a
+    workgroup go from a group of four row tiles (1024 rows) to the next: the rows of the
+    other groups keep their bits. The bad block is the last one, then the first."""
+    import torch
+    dtype = getattr(torch, dtype)
+    A, sa, W, sw = _problem(M, K, N, 41, cuda)
+    sa, inf, nan = sa / 4096, float("inf"), float("nan")
+    op = pkg.MatMulFp8(K, N).prepare_device(W, sw)
+    clean = op(A, scales=sa, out_dtype=dtype)
+    x = torch.randn(M, K, device=cuda).to(dtype)
+    clean_rows = op(x)
+    print(f"case fp8 wide nonfinite M={M} K={K} N={N} {op.kernel_name(M)}", flush=True)
+    group = torch.arange(M, device=cuda) // 1024 % 2
+    for odd, value, block in ((0, nan, -1), (1, inf, -1), (0, inf, 0), (1, nan, 0)):
+        bad, keep = group == odd, group != odd
+        k = 128 * block if block < 0 else 5
+        codes, scales = A.view(torch.uint8).clone(), sa.clone()
+        scales[bad, block] = value
+        codes[bad, k] = 0x7F  # as quantize_fp8 leaves it
+        y = op(codes.view(A.dtype), scales=scales, out_dtype=dtype)
+        assert torch.equal(y[keep], clean[keep]) and bool(y[bad].isnan().all())
+        dirty = x.clone()
+        dirty[bad, k] = value
+        y = op(dirty)
+        assert torch.equal(y[keep], clean_rows[keep]) and bool(y[bad].isnan().all())
+    # a finite scale whose product with the weight's passes fp32
+    bad, keep = group == 0, group == 1
+    scales = sa / 1024
+    scales[bad, -1] = 2.0 ** 127
+    y = pkg.MatMulFp8(K, N).prepare_device(W, sw * 1024)(A, scales=scales, out_dtype=dtype)
+    assert torch.equal(y[keep], clean[keep])
