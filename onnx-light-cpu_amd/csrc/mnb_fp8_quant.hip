@@ -83,7 +83,7 @@ __global__ __launch_bounds__(kThreads) void QuantizeKernel(const T *__restrict__
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = x[i] * 448.0f / amax;
+    for (int i = 0; i < 8; ++i) q[i] = x[i] / amax;  // 0 where x is finite (448 x may not be)
   }
   if ((threadIdx.x & 15) == 0) S[item] = amax / 448.0f;
   int lo = 0, hi = 0;
@@ -145,7 +145,7 @@ hipError_t QuantizeT(int64_t M, int64_t K, const void *X, int64_t ldx, uint8_t *
   const bool vec = K % 8 == 0 && (ldx * sizeof(T)) % 16 == 0 && ldq % 8 == 0 &&
                    reinterpret_cast<uintptr_t>(X) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(Q) % 8 == 0;
-  // Launches of at most 2^26 workgroups: a grid's threads stay below 2^32.
+  // Launches of at most 2^27 items, 16 lanes each: a grid's threads stay below 2^32.
   const int64_t rows = std::max<int64_t>(1, (int64_t{1} << 27) / nb);
   for (int64_t m = 0; m < M; m += rows) {
     const int64_t n = std::min(rows, M - m);

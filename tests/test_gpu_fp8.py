@@ -395,3 +395,20 @@ def test_nonfinite_rows_stay_alone_among_wide_tiles(pkg, cuda, M, K, N, dtype):
     scales[bad, -1] = 2.0 ** 127
     y = pkg.MatMulFp8(K, N).prepare_device(W, sw * 1024)(A, scales=scales, out_dtype=dtype)
     assert torch.equal(y[keep], clean[keep])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+def test_quantize_largest_value_beside_an_infinity(pkg, cuda, dtype):
+    """A block with an infinity: its infinities become NaN, every finite value 0."""
+    import torch
+    dtype = getattr(torch, dtype)
+    big, inf = torch.finfo(dtype).max, float("inf")
+    x = torch.zeros(2, 300, dtype=dtype, device=cuda)
+    x[0, :4] = torch.tensor([big, inf, -big, 1.0])
+    x[1, 256:260] = torch.tensor([-inf, big, -1.0, -big])
+    print("case quantize largest beside infinity", dtype, flush=True)
+    q, s = pkg.quantize_fp8(x)
+    q = q.double()
+    assert s[0].isinf().tolist() == [True, False, False] and bool(q[0, 1].isnan())
+    assert s[1].isinf().tolist() == [False, False, True] and bool(q[1, 256].isnan())
+    assert q[0, [0, 2, 3]].tolist() == [0, 0, 0] and q[1, 257:260].tolist() == [0, 0, 0]
