@@ -706,18 +706,25 @@ __global__ __launch_bounds__(256) void Fp8SumKernel(const float *__restrict__ P,
 }
 
 // Whether M rows take the kernels that stream the weights. Their workgroups of 16
-// columns each read all rows; past one workgroup a CU, and with more rows, that
-// costs more than the tiles' longer start (us, stream and tile, bf16 Y, weights
-// not in a cache: 48 rows of K = 4096, N = 4096: 7 and 12, N = 14336: 28 and 21; 20
-// rows of the same: 7 and 10, 20 and 16; 16 rows of 8192 x 8192: 20 and 19; one row
-// of K = 4096, N = 28672: 27 and 24; of K = 14336, N = 4096 64 rows: 26 and 22, 48
-// rows 23 and 20, but 17 and 18 with the weights in the last cache; of K = 28672,
-// N = 4096 40 rows: 40 and 29).
+// columns each read all rows, M K bytes, and the more of them a CU has (r, rounded up)
+// the earlier the tiles' longer start is paid for: r r M K decides, up to 256 KiB of it
+// where up to 16 rows are gathered into registers, up to 448 KiB where they pass through
+// LDS; from r = 6, or 3, on the tiles are as fast or faster whatever K.
+// us, stream and tile, bf16 Y, weights not in a cache:
+//   N = 4096 (r = 1): K = 14336 16 rows 16 and 17, 32 rows 18 and 18, 33 rows 19 and 19,
+//     48 rows 23 and 20, 64 rows 26 and 22; K = 20480 17 rows 20 and 21, 32 rows 24 and
+//     22; K = 28672 9 rows 26 and 27, 16 rows 32 and 27; K = 8192 64 rows 16 and 16
+//   N = 1024: K = 16384 9 rows 11 and 13, 16 rows 15 and 14, 33 rows 15 and 14
+//   r = 2: 4096 x 8192 (K x N) 32 rows 13 and 13, 64 rows 17 and 16; 8192 x 5120 8 rows 13
+//     and 13, 16 rows 17 and 14
+//   r = 3: 2048 x 12288 16 rows 9 and 10, 32 rows 11 and 11; 1024 x 12288 48 rows 8 and 7
+//   r = 4: 4096 x 14336 1 row 15 and 16, 8 rows 16 and 15; 1024 x 14336 64 rows 13 and 7
+//   r = 5: 2048 x 20480 1 row 10 and 13, 16 rows 12 and 12
+//   r = 6: 4096 x 24576 1 row 23 and 22; 2048 x 24576 1 row 12 and 13, 4 rows 13 and 12
 bool Streams(const Weight &w, int64_t M) {
   if (M > 64) return false;
-  const int64_t mib = w.N * w.nb * kBlock >> 20;
-  if (w.N > 16 * static_cast<int64_t>(w.num_cus)) return mib < (M <= 8 ? 96 : M <= 16 ? 48 : 24);
-  return M <= 8 || mib < (M <= 48 ? 96 : 48);
+  const int64_t r = CeilDiv(w.groups * 4, w.num_cus), bytes = r * r * M * w.nb * kBlock;
+  return M <= 16 ? r <= 5 && bytes <= 256 << 10 : r <= 2 && bytes <= 448 << 10;
 }
 
 struct TileShape {

@@ -412,3 +412,27 @@ def test_quantize_largest_value_beside_an_infinity(pkg, cuda, dtype):
     assert s[0].isinf().tolist() == [True, False, False] and bool(q[0, 1].isnan())
     assert s[1].isinf().tolist() == [False, False, True] and bool(q[1, 256].isnan())
     assert q[0, [0, 2, 3]].tolist() == [0, 0, 0] and q[1, 257:260].tolist() == [0, 0, 0]
+
+
+@pytest.mark.parametrize("M,K,N,name", [
+    # columns that give a CU one workgroup: the rows' bytes decide
+    (16, 14336, 4096, "Fp8StreamKernel"), (32, 14336, 4096, "Fp8StreamLdsKernel"),
+    (33, 14336, 4096, "Fp8TileKernel"), (48, 14336, 4096, "Fp8TileKernel"),
+    (16, 28672, 4096, "Fp8TileKernel"), (9, 28672, 4096, "Fp8StreamKernel"),
+    (41, 11008, 1000, "Fp8StreamLdsKernel"), (64, 7168, 256, "Fp8StreamLdsKernel"),
+    # several workgroups a CU: the earlier, the more
+    (1, 4096, 6144, "Fp8StreamKernel"), (16, 8192, 5120, "Fp8TileKernel"),
+    (28, 4096, 8192, "Fp8StreamLdsKernel"), (64, 1024, 14336, "Fp8TileKernel"),
+    (1, 2048, 20480, "Fp8StreamKernel"), (1, 2048, 24576, "Fp8TileKernel")])
+def test_few_rows_by_their_bytes(pkg, cuda, M, K, N, name):
+    """The kernel of few rows follows from how often how many bytes of them are read."""
+    import torch
+    assert torch.cuda.get_device_properties(cuda).multi_processor_count == 256
+    A, sa, W, sw = _problem(M, K, N, M + K + N, cuda)
+    op = pkg.MatMulFp8(K, N).prepare_device(W, sw)
+    print(f"case fp8 M={M} K={K} N={N} {op.kernel_name(M)}", flush=True)
+    assert op.kernel_name(M) == name
+    ref, mag = _expect(A, sa, W, sw)
+    _within(op(A, scales=sa), ref, mag, K)
+    for dtype in (torch.bfloat16, torch.float16):
+        _within(op(A, scales=sa / 4096, out_dtype=dtype), ref / 4096, mag / 4096, K)
