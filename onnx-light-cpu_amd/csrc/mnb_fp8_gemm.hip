@@ -733,8 +733,12 @@ struct TileShape {
 
 // exact: an fp32 Y.
 TileShape PickTile(const Weight &w, int64_t M, bool exact) {
-  // 16-bit results: large tiles where they fill the chip (rows of whole vectors).
-  if (!exact && w.nb >= 2 && w.N % 8 == 0 && CeilDiv(M, 256) * CeilDiv(w.N, 256) >= w.num_cus)
+  // 16-bit results: large tiles where they fill the chip (rows of whole vectors), of
+  // rows that fill half a tile at least (K = 4096, N = 65536, us, in these tiles and in
+  // those below: 1 row 62 and 52, 40 rows 65 and 60, 128 rows 67 and 63, 129 rows 67 and
+  // 87; N = 128256: 1 row 123 and 93, 128 rows 136 and 124, 129 rows 133 and 167).
+  if (!exact && M > 128 && w.nb >= 2 && w.N % 8 == 0 &&
+      CeilDiv(M, 256) * CeilDiv(w.N, 256) >= w.num_cus)
     return TileShape{256, 256, 1};
   // 64 x 128, two workgroups a CU. Larger ones take fewer reads of LDS and the
   // caches: 128 rows where they still fill the chip (512 x 4096 x 14336, bf16: 48 us

@@ -436,3 +436,18 @@ def test_few_rows_by_their_bytes(pkg, cuda, M, K, N, name):
     _within(op(A, scales=sa), ref, mag, K)
     for dtype in (torch.bfloat16, torch.float16):
         _within(op(A, scales=sa / 4096, out_dtype=dtype), ref / 4096, mag / 4096, K)
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 2048, 66000), (40, 2048, 66000), (100, 300, 65300),
+                                   (129, 300, 65300), (260, 256, 33000)])
+def test_few_rows_of_very_wide_weights(pkg, cuda, M, K, N):
+    """Weights as wide as a vocabulary: few rows are not spread over tiles of 256 rows."""
+    import torch
+    A, sa, W, sw = _problem(M, K, N, M + K + N, cuda)
+    op = pkg.MatMulFp8(K, N).prepare_device(W, sw)
+    print(f"case fp8 M={M} K={K} N={N} {op.kernel_name(M)}", flush=True)
+    assert M > 128 or op.kernel_name(M) != "Fp8WideKernel"
+    ref, mag = _expect(A, sa, W, sw)
+    _within(op(A, scales=sa), ref, mag, K)
+    for dtype in (torch.bfloat16, torch.float16):
+        _within(op(A, scales=sa / 4096, out_dtype=dtype), ref / 4096, mag / 4096, K)
