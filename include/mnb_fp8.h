@@ -69,8 +69,10 @@ int mnb_fp8_plan_device_bytes(const mnb_fp8_plan *plan, size_t *bytes);
 int mnb_fp8_workspace_bytes(const mnb_fp8_plan *plan, int64_t M, int32_t a_type, size_t *bytes);
 
 /* Y[M, N] of y_type (MNB_TYPE_FLOAT, _FLOAT16 or _BFLOAT16; sums in fp32,
- * rounded once; for a 16-bit Y the products within a group of eight are cut off
- * 2^-13 below the group's largest, about 1.4e-5 of Y) from dense rows dA [M, K]
+ * rounded once; for _FLOAT and _FLOAT16 of exact products; for _BFLOAT16 a product
+ * is cut off 2^-13 below the largest of its group of eight along K, so that Y loses
+ * up to 7 2^-13 of the sum of the products' magnitudes: about 1.4e-5 of Y where they
+ * are of one size, all of a small product beside a large one) from dense rows dA [M, K]
  * of a_type: MNB_TYPE_FLOAT8E4M3FN codes with dAScales [M, ceil(K / 128)], or
  * values of another type with dAScales NULL, quantized as by mnb_fp8_quantize.
  * dA, dY and the workspace are aligned to 16 bytes (MNB_ERR_BAD_SHAPE otherwise);
@@ -80,7 +82,7 @@ int mnb_fp8_run(const mnb_fp8_plan *plan, int64_t M, int32_t a_type, const void 
                 const float *dAScales, int32_t y_type, void *dY, void *dWorkspace,
                 size_t workspace_bytes, void *stream);
 
-/* Name of the kernel that multiplies M rows into a 16-bit Y ("" for a bad plan or
+/* Name of the kernel that multiplies M rows into a bfloat16 Y ("" for a bad plan or
  * M == 0). */
 const char *mnb_fp8_kernel_name(const mnb_fp8_plan *plan, int64_t M);
 

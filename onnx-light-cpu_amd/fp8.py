@@ -168,7 +168,8 @@ class MatMulFp8:
         """Y[..., N] on A's device. A: float8_e4m3fn codes [..., K] with scales
         float32 [..., ceil(K / 128)] (as quantize_fp8 gives them), or a float32,
         float16 or bfloat16 tensor, quantized first. Y's type: out's, out_dtype,
-        else A's (float32 for codes)."""
+        else A's (float32 for codes). Products are exact for a float32 or float16 Y; a
+        bfloat16 Y loses up to 7 2^-13 of the sum of their magnitudes (mnb_fp8.h)."""
         import torch
         if not self._plan:
             raise ValueError(f"{PREFIX}: prepare() was not called")
@@ -242,7 +243,7 @@ class MatMulFp8:
         return n.value
 
     def kernel_name(self, M: int) -> str:
-        """The kernel that multiplies M rows."""
+        """The kernel that multiplies M rows into a bfloat16 Y."""
         return _library().mnb_fp8_kernel_name(self._plan, M).decode()
 
     def device_bytes(self) -> int:

@@ -451,3 +451,36 @@ def test_few_rows_of_very_wide_weights(pkg, cuda, M, K, N):
     _within(op(A, scales=sa), ref, mag, K)
     for dtype in (torch.bfloat16, torch.float16):
         _within(op(A, scales=sa / 4096, out_dtype=dtype), ref / 4096, mag / 4096, K)
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 1024, 256), (16, 1000, 100), (40, 2048, 64),
+                                   (100, 1024, 512), (200, 1024, 20000), (300, 512, 14400),
+                                   (4096, 256, 4096)])
+def test_products_beside_larger_ones(pkg, cuda, M, K, N):
+    """Outlier channels whose products cancel: every eighth value of K is 448, of
+    alternating sign in A, the values between are integers of magnitude 3 at most, so
+    that Y consists of products 2^14 and more below their neighbours. All products are
+    integers and a block's magnitudes add up to less than 2^23, so that no fp32 sum of
+    them rounds in whatever order: Y in fp32 is exact, in fp16 rounded once. A bfloat16
+    Y loses up to 7 2^-13 of the magnitudes (_within)."""
+    import torch
+    g = torch.Generator(device=cuda)
+    g.manual_seed(M + N)
+
+    def small(rows):
+        return torch.randint(-3, 4, (rows, K), device=cuda, generator=g).float()
+
+    A, W = small(M), small(N)
+    k = torch.arange(0, K, 8, device=cuda)
+    A[:, k] = torch.where(k // 8 % 2 == 0, 448.0, -448.0)
+    W[:, k] = 448.0
+    A, W = A.to(torch.float8_e4m3fn), W.to(torch.float8_e4m3fn)
+    sa = torch.full((M, -(-K // 128)), 2.0 ** -10, device=cuda)
+    sw = torch.ones(-(-N // 128), -(-K // 128), device=cuda)
+    op = pkg.MatMulFp8(K, N).prepare_device(W, sw)
+    print(f"case fp8 outliers M={M} K={K} N={N} {op.kernel_name(M)}", flush=True)
+    ref, mag = _expect(A, sa, W, sw)
+    assert torch.equal(op(A, scales=sa).double(), ref)
+    assert torch.equal(op(A, scales=sa, out_dtype=torch.float16), ref.half())
+    worst = _within(op(A, scales=sa, out_dtype=torch.bfloat16), ref, mag, K)
+    print(f"  bfloat16: worst / bound {worst:.3f}", flush=True)
