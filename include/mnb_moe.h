@@ -20,10 +20,10 @@
  *
  * Activations enter the products in fixed point: each token's (or expert
  * row's) block of 128 values is scaled by a power of two and rounded to 22 bits
- * (fp32 X) or 14 (16-bit X) below its largest magnitude, the 4-bit weights are
- * exact integers, and each weight block's sum is exact before it is scaled and
- * added up in fp32. A block that holds an infinity or a NaN makes the token's
- * products NaN.
+ * below its largest magnitude (at most 2^-22 of that, or of 2^-90 where that is
+ * larger), the 4-bit weights are exact integers, and each weight block's sum is exact
+ * before it is scaled and added up in fp32. A block that holds an infinity or a NaN
+ * makes the token's products NaN.
  *
  * Conventions of mnb.h hold (device pointers, void* streams, status codes,
  * checks before any HIP call, immutable plans, runs on distinct outputs and

@@ -54,7 +54,7 @@ hipError_t LaunchRelayout(const mnb_moe_weight &src, int64_t N, int64_t K, int b
                           hipStream_t s);
 
 // Bytes of the workspace of one launch of T <= kMaxTokens tokens.
-size_t WorkBytes(const Layer &l, int T, int32_t x_type);
+size_t WorkBytes(const Layer &l, int T);
 hipError_t LaunchLayer(const Layer &l, int T, int32_t x_type, const void *X, const float *logits,
                        void *Y, int32_t *ids, float *weights, void *work, hipStream_t s);
 

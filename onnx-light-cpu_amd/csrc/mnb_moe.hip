@@ -4,13 +4,18 @@
 // they meet, 4.25 bits a value; what a CU does per weight has to stay small.
 // The products are exact integers on the int8 MFMA:
 //
-//   x = 2^s (256^2 d2 + 256 d1 + d0), digits in [-128, 127] (two digits for
-//   16-bit activations), one power of two for each block of 128 values,
+//   x = 2^s (256^2 d2 + 256 d1 + d0), digits in [-128, 127], one power of two for
+//   each block of 128 values, 22 bits below the block's largest magnitude. A float16
+//   value keeps all its bits down to 2^-11 of that magnitude, a bfloat16 one down to
+//   2^-14; smaller ones, and fp32 values and experts' rows, are off by at most 2^-22 of
+//   it, as much as four fp32 additions to the largest value's product. (With two digits
+//   for 16-bit activations, 14 bits, the values beside an outlier of 2^12 times their
+//   size kept two.)
 //   w = scale (q - z), q - z in a byte by three or four operations on four
 //   weights at once, without conversions.
 //
 // A token's digits are columns of one MFMA tile: 16 columns hold five tokens of
-// three digits or eight of two, so the digits cost no extra matrix instruction,
+// three digits, so the digits of few tokens cost no extra matrix instruction,
 // and the rows of a tile are 16 weight rows. A weight block's sums are exact
 // integers (below 2^21); they are scaled and added up in fp32, column by column,
 // and the columns of a token join after the last block.
@@ -33,14 +38,17 @@ namespace {
 typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
+// Digits of a value.
+constexpr int kND = 3;
+
 // Columns of a tile per digit: the tokens of one column group. ONE: a group of
 // one token, whose digits alone are kept and copied.
-template <int ND, bool ONE = false>
-constexpr int kTokens = ONE ? 1 : ND == 3 ? 5 : 8;
+template <bool ONE>
+constexpr int kTokens = ONE ? 1 : 16 / kND;
 
 // ---- fixed point ---------------------------------------------------------------
 
-// Rows in fixed point: digits [rows][ND][units * 128] and the powers of two of
+// Rows in fixed point: digits [rows][kND][units * 128] and the powers of two of
 // each unit's `scales` parts [rows][units][scales].
 struct Fixed {
   int8_t *dig;
@@ -53,7 +61,6 @@ struct Fixed {
 // 16, or of the 16 / scales that share a part. The unit's 128 bytes of a digit
 // lie as the weight layout takes them, 16 for each half of the unit and lane
 // group: the eight of i at 64 (i / 8) + 16 (i % 4) + 8 (i / 4 % 2).
-template <int ND>
 __device__ __forceinline__ void StoreUnit(const Fixed &f, int64_t row, int64_t unit, int i,
                                           const float (&x)[8]) {
   // As integers, magnitudes order like their values, infinity above them and NaN on top.
@@ -65,10 +72,10 @@ __device__ __forceinline__ void StoreUnit(const Fixed &f, int64_t row, int64_t u
     top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 16)));
   const bool finite = top < 0x7F800000u;
   // 2^e <= amax < 2^(e + 1), at least 2^-90: smaller values count against that.
-  // The largest magnitude becomes at most 2^22 (2^14 for two digits), so that
-  // the top digit with its carries stays in a byte.
+  // The largest magnitude becomes at most 2^22, so that the top digit with its
+  // carries stays in a byte.
   const int e = finite ? max(static_cast<int>(top >> 23) - 127, -90) : 0;
-  constexpr int kBits = ND == 3 ? 21 : 13;
+  constexpr int kBits = 8 * kND - 3;
   int n[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j)
@@ -77,17 +84,17 @@ __device__ __forceinline__ void StoreUnit(const Fixed &f, int64_t row, int64_t u
     f.power[(row * f.units + unit) * f.scales + i / part] =
         finite ? ldexpf(1.0f, e - kBits) : __uint_as_float(0x7FC00000u);
 #pragma unroll
-  for (int d = 0; d < ND; ++d) {
+  for (int d = 0; d < kND; ++d) {
     uint32_t lo = 0, hi = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int digit = d + 1 < ND ? static_cast<int>(static_cast<int8_t>(n[j])) : n[j];
+      const int digit = d + 1 < kND ? static_cast<int>(static_cast<int8_t>(n[j])) : n[j];
       n[j] = (n[j] - digit) >> 8;
       const uint32_t b = static_cast<uint32_t>(digit) & 0xFFu;
       if (j < 4) lo |= b << (8 * j);
       else hi |= b << (8 * (j - 4));
     }
-    *reinterpret_cast<uint2 *>(f.dig + ((row * ND + d) * f.units + unit) * kUnit + 64 * (i >> 3) +
+    *reinterpret_cast<uint2 *>(f.dig + ((row * kND + d) * f.units + unit) * kUnit + 64 * (i >> 3) +
                                16 * (i & 3) + 8 * ((i >> 2) & 1)) = make_uint2(lo, hi);
   }
 }
@@ -98,7 +105,7 @@ __device__ __forceinline__ void StoreUnit(const Fixed &f, int64_t row, int64_t u
 // 64 bits (the choice is a comparison of sums: it shall not hang on their
 // order). The others: 16 lanes per (token, unit). VEC: H a multiple of 4, rows of
 // X and R aligned to four values.
-template <int ND, int RT, bool VEC, typename T>
+template <int RT, bool VEC, typename T>
 __global__ __launch_bounds__(256) void MoePrepKernel(const T *__restrict__ X,
                                                      const float *__restrict__ R, float *logits,
                                                      Fixed fx, int tokens, int64_t H, int E,
@@ -157,7 +164,7 @@ __global__ __launch_bounds__(256) void MoePrepKernel(const T *__restrict__ X,
   float x[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) x[j] = k0 + j < H ? static_cast<float>(X[row * H + k0 + j]) : 0.0f;
-  StoreUnit<ND>(fx, row, unit, tid & 15, x);
+  StoreUnit(fx, row, unit, tid & 15, x);
 }
 
 // ---- second launch: the choice ------------------------------------------------
@@ -253,10 +260,10 @@ __global__ __launch_bounds__(256) void MoeRouteKernel(const float *__restrict__ 
 // NS units are in flight by direct global -> LDS copies, so what keeps the memory
 // busy needs no registers. F weight blocks per unit, XB parts of it with powers
 // of two of their own.
-template <int ND, bool ONE, int GC, int R, int F, int XB, bool ZP, int SHARE, int NS>
+template <bool ONE, int GC, int R, int F, int XB, bool ZP, int SHARE, int NS>
 struct Pipe {
   static_assert(!ONE || GC == 1, "one token, one column group");
-  static constexpr int kT = kTokens<ND, ONE>;
+  static constexpr int kT = kTokens<ONE>;
   static constexpr int kCols = ONE ? 4 : 16;  // kept columns of a group
   static constexpr int kFolds = F > XB ? F : XB;
   static constexpr int kMeta = MetaBytes(F, ZP);
@@ -309,11 +316,11 @@ struct Pipe {
       // Columns without a token keep what LDS holds: nothing reads their sums. One
       // lane is always on, so that every copy is issued and counted.
       // A wavefront without a copy of its own repeats one lane of the last.
-      s_on[i] = (token < n && digit < ND && column < 16 * GC && (!ONE || !powers || lane == 0) &&
+      s_on[i] = (token < n && digit < kND && column < 16 * GC && (!ONE || !powers || lane == 0) &&
                  i * SHARE + ws < kShared) || lane == 0;
       const uint32_t row = row_of(token < n ? token : 0), units = static_cast<uint32_t>(f.units);
       s_off[i] = powers ? row * units * (XB * 4)
-                        : (row * ND + min(digit, ND - 1)) * units * kUnit +
+                        : (row * kND + min(digit, kND - 1)) * units * kUnit +
                               ((lane & 7) ^ ((c >> 1) & 7)) * 16;
     }
   }
@@ -475,19 +482,18 @@ __device__ __forceinline__ float LanesUp(float v) {
 
 // The sum of a token's digit columns (kTokens apart), in the column of digit 0
 // (garbage in the others): v holds this lane's column times 256^digit.
-template <int ND, bool ONE>
+template <bool ONE>
 __device__ __forceinline__ float JoinDigits(float v) {
-  constexpr int kT = kTokens<ND, ONE>;
-  if constexpr (ND == 2) return LanesUp<kT>(v) + v;
-  else return (LanesUp<2 * kT>(v) + LanesUp<kT>(v)) + v;
+  constexpr int kT = kTokens<ONE>;
+  return (LanesUp<2 * kT>(v) + LanesUp<kT>(v)) + v;
 }
 
 // What a column's sum counts for: 256^digit, and 1/16 without zero points (the
 // weights' bytes hold 16 times their value there).
-template <int ND, bool ONE, bool ZP>
+template <bool ONE, bool ZP>
 __device__ __forceinline__ float ColumnWeight(int lane) {
-  const int digit = (lane & 15) / kTokens<ND, ONE>;
-  if (digit >= ND) return 0.0f;
+  const int digit = (lane & 15) / kTokens<ONE>;
+  if (digit >= kND) return 0.0f;
   const float w = digit == 0 ? 1.0f : digit == 1 ? 256.0f : 65536.0f;
   return ZP ? w : w * 0.0625f;
 }
@@ -579,13 +585,13 @@ constexpr int WavesPerSimd(int gc, int folds) {
 // reading: 64 tokens of 4096 x 14336, 2 of 8 experts, 105 us (4.8 TB/s; about 10 less
 // without the products), one token 25 us (5.1 TB/s); one of 2048 x 1024, 6 of 64, 9 us,
 // its launch and two round trips.
-template <int ND, bool ONE, int GC, int F, bool ZP, int GROUPS, int KS, int NS, bool CHOOSE>
+template <bool ONE, int GC, int F, bool ZP, int GROUPS, int KS, int NS, bool CHOOSE>
 __global__ __launch_bounds__(64 * GROUPS *KS,
                              GROUPS == 8 ? WavesPerSimd(GC, F) : 1) void MoeGateUpKernel(
     Matrix m, Fixed fx, Fixed fh, const int32_t *__restrict__ pair_expert,
     const float *__restrict__ pair_weight, Plan plan, int pairs, int top_k, bool by_expert,
     Choice choice) {
-  using P = Pipe<ND, ONE, GC, 2, F, 1, ZP, KS == 1 ? GROUPS : 1, NS>;
+  using P = Pipe<ONE, GC, 2, F, 1, ZP, KS == 1 ? GROUPS : 1, NS>;
   constexpr int kT = P::kT, kChannels = 16 * GROUPS, kWaves = GROUPS * KS;
   constexpr int kPipes = KS == 1 ? 1 : kWaves;
   static_assert(kPipes * P::kLds >= GC * kT * kChannels * 4 + (KS - 1) * GROUPS * GC * 2048,
@@ -646,7 +652,7 @@ __global__ __launch_bounds__(64 * GROUPS *KS,
   const int n = __builtin_amdgcn_readfirstlane(shared_n);
   if (n == 0) return;
   const int c = lane & 15, q = lane >> 4;
-  const float weight = ColumnWeight<ND, ONE, ZP>(lane);
+  const float weight = ColumnWeight<ONE, ZP>(lane);
   const int cg = wave % GROUPS, ks = wave / GROUPS;
   P pipe(reinterpret_cast<const uint8_t *>(dynamic) + (KS == 1 ? 0 : wave * P::kLds), lane,
          KS == 1 ? wave : 0);
@@ -705,8 +711,8 @@ __global__ __launch_bounds__(64 * GROUPS *KS,
         floatx4 h;
 #pragma unroll
         for (int v = 0; v < 4; ++v)
-          h[v] = SiluMul(JoinDigits<ND, ONE>(acc[0][g][v] * weight),
-                         JoinDigits<ND, ONE>(acc[1][g][v] * weight));
+          h[v] = SiluMul(JoinDigits<ONE>(acc[0][g][v] * weight),
+                         JoinDigits<ONE>(acc[1][g][v] * weight));
         if (c < kT)
           *reinterpret_cast<floatx4 *>(hidden + (g * kT + c) * kChannels + 16 * cg + 4 * q) = h;
       }
@@ -720,7 +726,7 @@ __global__ __launch_bounds__(64 * GROUPS *KS,
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = hidden[i * kChannels + 8 * k + j];
       const int64_t k0 = static_cast<int64_t>(blockIdx.x) * (kChannels / 8) + k;  // eights of the row
-      StoreUnit<ND>(fh, list[t0 + i], k0 >> 4, static_cast<int>(k0 & 15), x);
+      StoreUnit(fh, list[t0 + i], k0 >> 4, static_cast<int>(k0 & 15), x);
     }
     __syncthreads();
   }
@@ -731,12 +737,12 @@ __global__ __launch_bounds__(64 * GROUPS *KS,
 // wavefront and its pipe, which adds each segment's rows, times the tokens'
 // weights, to sums of its own; they join in order. One token of 4096 x 14336, 2 of 8:
 // 20 us, 3.1 TB/s; neither copies eight deep nor sixteen wavefronts changed that.
-template <int ND, bool ONE, int F, bool ZP, int NS, typename T>
+template <bool ONE, int F, bool ZP, int NS, typename T>
 __global__ __launch_bounds__(512) void MoeDownNarrowKernel(Matrix m, Fixed fh, Plan plan,
                                                            T *__restrict__ Y, int pairs,
                                                            int most_segments, int tokens, int top_k,
                                                            int64_t H) {
-  using P = Pipe<ND, ONE, 1, 1, F, 4, ZP, 1, NS>;
+  using P = Pipe<ONE, 1, 1, F, 4, ZP, 1, NS>;
   constexpr int kT = P::kT;
   // The pipes' LDS, then sums [8][tokens][16], the pairs' weights, the segments and
   // the list of pairs.
@@ -761,7 +767,7 @@ __global__ __launch_bounds__(512) void MoeDownNarrowKernel(Matrix m, Fixed fh, P
   ++segments;
   const int i0 = items * wave / 8, i1 = items * (wave + 1) / 8;
   const int c = lane & 15, q = lane >> 4;
-  const float weight = ColumnWeight<ND, ONE, ZP>(lane);
+  const float weight = ColumnWeight<ONE, ZP>(lane);
   if (i0 < i1) {
     P pipe(lds + wave * P::kLds, lane, 0, blockIdx.x & 1);
     // The next item to copy.
@@ -795,7 +801,7 @@ __global__ __launch_bounds__(512) void MoeDownNarrowKernel(Matrix m, Fixed fh, P
         const uint32_t now = __builtin_amdgcn_readfirstlane(segments[seg]);
         floatx4 y;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) y[v] = JoinDigits<ND, ONE>(acc[0][0][v] * weight);
+        for (int v = 0; v < 4; ++v) y[v] = JoinDigits<ONE>(acc[0][0][v] * weight);
         acc[0][0] = floatx4{0.f, 0.f, 0.f, 0.f};
         if (c < kT && c < Count(now)) {
           const float p = weights[Offset(now) + c];
@@ -824,11 +830,11 @@ __global__ __launch_bounds__(512) void MoeDownNarrowKernel(Matrix m, Fixed fh, P
 // Down otherwise: a workgroup takes 256 columns of Y and part blockIdx.y % cuts of the
 // units of one segment. Every pair's row, times its weight, goes to parts
 // [cuts][pairs][width]. 64 tokens of 4096 x 14336, 2 of 8: 53 us, 4.8 TB/s.
-template <int ND, bool ONE, int GC, int F, bool ZP, int NS>
+template <bool ONE, int GC, int F, bool ZP, int NS>
 __global__ __launch_bounds__(512, WavesPerSimd(GC, F)) void MoeDownKernel(Matrix m, Fixed fh, Plan plan,
                                                      float *__restrict__ parts, int pairs, int cuts,
                                                      int64_t width) {
-  using P = Pipe<ND, ONE, GC, 2, F, 1, ZP, 8, NS>;
+  using P = Pipe<ONE, GC, 2, F, 1, ZP, 8, NS>;
   constexpr int kT = P::kT;
   extern __shared__ uint4 dynamic[];
   const int lane = threadIdx.x & 63;
@@ -839,7 +845,7 @@ __global__ __launch_bounds__(512, WavesPerSimd(GC, F)) void MoeDownKernel(Matrix
   const int u0 = units * cut / cuts, u1 = units * (cut + 1) / cuts;
   if (u0 >= u1) return;
   const int c = lane & 15, q = lane >> 4;
-  const float weight = ColumnWeight<ND, ONE, ZP>(lane);
+  const float weight = ColumnWeight<ONE, ZP>(lane);
   const int64_t group = min(static_cast<int64_t>(blockIdx.x) * 8 + wave, m.groups - 1);
   float *out = parts + static_cast<int64_t>(cut) * pairs * width +
                static_cast<int64_t>(blockIdx.x) * 256 + wave * 32 + 4 * q;
@@ -872,7 +878,7 @@ __global__ __launch_bounds__(512, WavesPerSimd(GC, F)) void MoeDownKernel(Matrix
     for (int r = 0; r < 2; ++r) {
       floatx4 y;
 #pragma unroll
-      for (int v = 0; v < 4; ++v) y[v] = p * JoinDigits<ND, ONE>(acc[r][g][v] * weight);
+      for (int v = 0; v < 4; ++v) y[v] = p * JoinDigits<ONE>(acc[r][g][v] * weight);
       if (on) *reinterpret_cast<floatx4 *>(to + 16 * r) = y;
     }
   }
@@ -998,7 +1004,7 @@ struct Shape {
   int cuts;     // down: runs of 1 / cuts of a segment
 };
 
-Shape PickShape(const Layer &l, int tokens, int ND) {
+Shape PickShape(const Layer &l, int tokens) {
   Shape s;
   s.entries = std::min(tokens * l.top_k, l.experts);
   const int64_t blocks = s.entries * CeilDiv(l.intermediate, 128);  // of 128 channels
@@ -1017,7 +1023,7 @@ Shape PickShape(const Layer &l, int tokens, int ND) {
   // What most experts' tokens fill: their mean share and two standard deviations
   // of even choices (32 tokens of 4096 x 4096, 2 of 8: four groups 62 us, one 84; 64
   // of 2048 x 1024, 8 of 64: two 81, one 92).
-  const int group = tokens == 1 ? 1 : ND == 3 ? kTokens<3> : kTokens<2>;
+  const int group = tokens == 1 ? 1 : kTokens<false>;
   const double mean = static_cast<double>(tokens) * l.top_k / l.experts;
   const double most = std::min<double>(tokens, mean + 2.0 * std::sqrt(mean));
   // Four groups of 16-wide blocks would not fit the registers.
@@ -1038,7 +1044,7 @@ Shape PickShape(const Layer &l, int tokens, int ND) {
 
 int64_t PartWidth(const Layer &l) { return CeilDiv(l.hidden, 256) * 256; }
 
-Work Split(const Layer &l, int T, int ND, void *base) {
+Work Split(const Layer &l, int T, void *base) {
   Work w;
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -1047,12 +1053,12 @@ Work Split(const Layer &l, int T, int ND, void *base) {
     return p;
   };
   const size_t pairs = static_cast<size_t>(T) * l.top_k;
-  const Shape shape = PickShape(l, T, ND);
+  const Shape shape = PickShape(l, T);
   auto fixed = [&](size_t rows, int64_t units, int scales) {
     Fixed f;
     f.units = units;
     f.scales = scales;
-    f.dig = reinterpret_cast<int8_t *>(take(rows * ND * units * kUnit));
+    f.dig = reinterpret_cast<int8_t *>(take(rows * kND * units * kUnit));
     f.power = reinterpret_cast<float *>(take(rows * units * scales * 4));
     return f;
   };
@@ -1070,44 +1076,44 @@ Work Split(const Layer &l, int T, int ND, void *base) {
   return w;
 }
 
-template <int ND, bool ONE, int GC, int F, bool ZP, int GROUPS, int KS, bool CHOOSE>
+template <bool ONE, int GC, int F, bool ZP, int GROUPS, int KS, bool CHOOSE>
 hipError_t LaunchGateUp(const Layer &l, const Work &w, const Shape &shape, int pairs,
                         const Choice &choice, hipStream_t s) {
   constexpr int NS = KS > 1 && ONE ? 4 : GC == 1 && GROUPS == 8 ? 2 : 3;
-  using P = Pipe<ND, ONE, GC, 2, F, 1, ZP, KS == 1 ? GROUPS : 1, NS>;
+  using P = Pipe<ONE, GC, 2, F, 1, ZP, KS == 1 ? GROUPS : 1, NS>;
   const dim3 grid(static_cast<unsigned>(l.gate_up.groups / GROUPS),
                   static_cast<unsigned>(shape.entries + (CHOOSE ? 0 : 1)));
-  hipLaunchKernelGGL((MoeGateUpKernel<ND, ONE, GC, F, ZP, GROUPS, KS, NS, CHOOSE>), grid,
+  hipLaunchKernelGGL((MoeGateUpKernel<ONE, GC, F, ZP, GROUPS, KS, NS, CHOOSE>), grid,
                      dim3(64 * GROUPS * KS), (KS == 1 ? 1 : GROUPS * KS) * P::kLds, s, l.gate_up,
                      w.fx, w.fh, w.pair_expert, w.pair_weight, w.plan, pairs, l.top_k,
                      pairs >= l.experts, choice);
   return hipGetLastError();
 }
 
-template <int ND, bool ONE, int F, bool ZP, typename T>
+template <bool ONE, int F, bool ZP, typename T>
 hipError_t LaunchDownNarrow(const Layer &l, const Work &w, const Shape &shape, int tokens, T *Y,
                             hipStream_t s) {
   constexpr int NS = ONE ? 5 : 3;
-  using P = Pipe<ND, ONE, 1, 1, F, 4, ZP, 1, NS>;
+  using P = Pipe<ONE, 1, 1, F, 4, ZP, 1, NS>;
   const int pairs = tokens * l.top_k;
   const size_t lds = static_cast<size_t>(8) * P::kLds + 8 * tokens * 16 * sizeof(float) + pairs * 6 +
                      (shape.segments + 1) * 4;
-  hipLaunchKernelGGL((MoeDownNarrowKernel<ND, ONE, F, ZP, NS, T>),
+  hipLaunchKernelGGL((MoeDownNarrowKernel<ONE, F, ZP, NS, T>),
                      dim3(static_cast<unsigned>(2 * l.down.groups)), dim3(512), lds, s, l.down, w.fh,
                      w.plan, Y, pairs, shape.segments, tokens, l.top_k, l.hidden);
   return hipGetLastError();
 }
 
-template <int ND, bool ONE, int GC, int F, bool ZP, typename T>
+template <bool ONE, int GC, int F, bool ZP, typename T>
 hipError_t LaunchDown(const Layer &l, const Work &w, const Shape &shape, int tokens, T *Y,
                       hipStream_t s) {
   constexpr int NS = GC == 1 ? 2 : 3;
-  using P = Pipe<ND, ONE, GC, 2, F, 1, ZP, 8, NS>;
+  using P = Pipe<ONE, GC, 2, F, 1, ZP, 8, NS>;
   const int pairs = tokens * l.top_k;
   const int64_t width = PartWidth(l);
   const dim3 grid(static_cast<unsigned>(width / 256),
                   static_cast<unsigned>(shape.segments * shape.cuts));
-  hipLaunchKernelGGL((MoeDownKernel<ND, ONE, GC, F, ZP, NS>), grid, dim3(512), P::kLds, s, l.down,
+  hipLaunchKernelGGL((MoeDownKernel<ONE, GC, F, ZP, NS>), grid, dim3(512), P::kLds, s, l.down,
                      w.fh, w.plan, w.parts, pairs, shape.cuts, width);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
@@ -1117,17 +1123,17 @@ hipError_t LaunchDown(const Layer &l, const Work &w, const Shape &shape, int tok
   return hipGetLastError();
 }
 
-template <int ND, bool ONE, int GC, int F, bool ZP, int GROUPS, int KS>
+template <bool ONE, int GC, int F, bool ZP, int GROUPS, int KS>
 hipError_t LaunchGateUpC(const Layer &l, const Work &w, const Shape &shape, int pairs,
                          const Choice &choice, hipStream_t s) {
   if constexpr (ONE) {
     if (shape.choose)
-      return LaunchGateUp<ND, ONE, GC, F, ZP, GROUPS, KS, true>(l, w, shape, pairs, choice, s);
+      return LaunchGateUp<ONE, GC, F, ZP, GROUPS, KS, true>(l, w, shape, pairs, choice, s);
   }
-  return LaunchGateUp<ND, ONE, GC, F, ZP, GROUPS, KS, false>(l, w, shape, pairs, choice, s);
+  return LaunchGateUp<ONE, GC, F, ZP, GROUPS, KS, false>(l, w, shape, pairs, choice, s);
 }
 
-template <int ND, bool ONE, int GC, int F, bool ZP, typename T>
+template <bool ONE, int GC, int F, bool ZP, typename T>
 hipError_t LaunchExperts(const Layer &l, const Work &w, const Shape &shape, int tokens, T *Y,
                          const Choice &choice, hipStream_t s) {
   const int pairs = tokens * l.top_k;
@@ -1137,34 +1143,33 @@ hipError_t LaunchExperts(const Layer &l, const Work &w, const Shape &shape, int 
       bool split = true;
       if constexpr (ONE) {  // several tokens' narrow layers are always small enough
         split = shape.split;
-        if (!split) e = LaunchGateUpC<ND, ONE, GC, F, ZP, 2, 1>(l, w, shape, pairs, choice, s);
+        if (!split) e = LaunchGateUpC<ONE, GC, F, ZP, 2, 1>(l, w, shape, pairs, choice, s);
       }
-      if (split) e = LaunchGateUpC<ND, ONE, GC, F, ZP, 2, 4>(l, w, shape, pairs, choice, s);
-      return e != hipSuccess ? e : LaunchDownNarrow<ND, ONE, F, ZP, T>(l, w, shape, tokens, Y, s);
+      if (split) e = LaunchGateUpC<ONE, GC, F, ZP, 2, 4>(l, w, shape, pairs, choice, s);
+      return e != hipSuccess ? e : LaunchDownNarrow<ONE, F, ZP, T>(l, w, shape, tokens, Y, s);
     }
   }
-  e = LaunchGateUpC<ND, ONE, GC, F, ZP, 8, 1>(l, w, shape, pairs, choice, s);
-  return e != hipSuccess ? e : LaunchDown<ND, ONE, GC, F, ZP, T>(l, w, shape, tokens, Y, s);
+  e = LaunchGateUpC<ONE, GC, F, ZP, 8, 1>(l, w, shape, pairs, choice, s);
+  return e != hipSuccess ? e : LaunchDown<ONE, GC, F, ZP, T>(l, w, shape, tokens, Y, s);
 }
 
-template <int ND, bool ONE, int GC, bool ZP, typename T>
+template <bool ONE, int GC, bool ZP, typename T>
 hipError_t LaunchFolds(const Layer &l, const Work &w, const Shape &shape, int tokens, T *Y,
                        const Choice &choice, hipStream_t s) {
   switch (l.folds) {
-  case 1: return LaunchExperts<ND, ONE, GC, 1, ZP, T>(l, w, shape, tokens, Y, choice, s);
-  case 2: return LaunchExperts<ND, ONE, GC, 2, ZP, T>(l, w, shape, tokens, Y, choice, s);
-  case 4: return LaunchExperts<ND, ONE, GC, 4, ZP, T>(l, w, shape, tokens, Y, choice, s);
+  case 1: return LaunchExperts<ONE, GC, 1, ZP, T>(l, w, shape, tokens, Y, choice, s);
+  case 2: return LaunchExperts<ONE, GC, 2, ZP, T>(l, w, shape, tokens, Y, choice, s);
+  case 4: return LaunchExperts<ONE, GC, 4, ZP, T>(l, w, shape, tokens, Y, choice, s);
   default: break;
   }
-  if constexpr (GC < 4) return LaunchExperts<ND, ONE, GC, 8, ZP, T>(l, w, shape, tokens, Y, choice, s);
+  if constexpr (GC < 4) return LaunchExperts<ONE, GC, 8, ZP, T>(l, w, shape, tokens, Y, choice, s);
   else return hipErrorInvalidValue;  // PickShape gives eight folds no four groups
 }
 
 template <typename T>
 hipError_t LaunchLayerT(const Layer &l, int tokens, const void *X, const float *logits, void *Y,
                         int32_t *ids, float *weights, void *work, hipStream_t s) {
-  constexpr int ND = sizeof(T) == 4 ? 3 : 2;
-  const Work w = Split(l, tokens, ND, work);
+  const Work w = Split(l, tokens, work);
   constexpr int kRT = 4;
   const int router_wgs =
       logits ? 0 : l.experts * (tokens == 1 ? 1 : static_cast<int>(CeilDiv(tokens, kRT)));
@@ -1172,7 +1177,7 @@ hipError_t LaunchLayerT(const Layer &l, int tokens, const void *X, const float *
       static_cast<unsigned>(router_wgs + CeilDiv(tokens * l.gate_up.units, 16));
   const bool vec = l.hidden % 4 == 0 && reinterpret_cast<uintptr_t>(X) % (4 * sizeof(T)) == 0;
   auto launch_prep = [&](auto rt, auto v) {
-    hipLaunchKernelGGL((MoePrepKernel<ND, decltype(rt)::value, decltype(v)::value, T>), dim3(prep),
+    hipLaunchKernelGGL((MoePrepKernel<decltype(rt)::value, decltype(v)::value, T>), dim3(prep),
                        dim3(256), 0, s, static_cast<const T *>(X), l.router, w.logits, w.fx, tokens,
                        l.hidden, l.experts, router_wgs);
   };
@@ -1182,7 +1187,7 @@ hipError_t LaunchLayerT(const Layer &l, int tokens, const void *X, const float *
   else vec ? launch_prep(Several{}, std::true_type{}) : launch_prep(Several{}, std::false_type{});
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const Shape shape = PickShape(l, tokens, ND);
+  const Shape shape = PickShape(l, tokens);
   const Choice choice{logits ? logits : w.logits, ids, weights, l.experts, l.normalize};
   if (!shape.choose) {
     hipLaunchKernelGGL(MoeRouteKernel, dim3(static_cast<unsigned>(tokens)), dim3(256), 0, s,
@@ -1195,8 +1200,8 @@ hipError_t LaunchLayerT(const Layer &l, int tokens, const void *X, const float *
   auto experts = [&](auto groups, auto one) {
     constexpr int GC = decltype(groups)::value;
     constexpr bool kOne = decltype(one)::value;
-    return l.zeros ? LaunchFolds<ND, kOne, GC, true, T>(l, w, shape, tokens, y, choice, s)
-                   : LaunchFolds<ND, kOne, GC, false, T>(l, w, shape, tokens, y, choice, s);
+    return l.zeros ? LaunchFolds<kOne, GC, true, T>(l, w, shape, tokens, y, choice, s)
+                   : LaunchFolds<kOne, GC, false, T>(l, w, shape, tokens, y, choice, s);
   };
   if (tokens == 1) return experts(std::integral_constant<int, 1>{}, std::true_type{});
   switch (shape.groups) {
@@ -1240,9 +1245,7 @@ hipError_t LaunchRelayout(const mnb_moe_weight &src, int64_t N, int64_t K, int b
   return hipSuccess;
 }
 
-size_t WorkBytes(const Layer &l, int T, int32_t x_type) {
-  return Split(l, T, x_type == MNB_TYPE_FLOAT ? 3 : 2, nullptr).bytes;
-}
+size_t WorkBytes(const Layer &l, int T) { return Split(l, T, nullptr).bytes; }
 
 hipError_t LaunchLayer(const Layer &l, int T, int32_t x_type, const void *X, const float *logits,
                        void *Y, int32_t *ids, float *weights, void *work, hipStream_t s) {

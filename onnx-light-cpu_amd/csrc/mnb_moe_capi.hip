@@ -9,10 +9,9 @@ struct mnb_moe_plan {
   int device;
   void *mem[5];  // gate/up records and meta; down's; router
   size_t bytes;
-  // Workspace of up to t + 1 tokens a launch, with 16-bit and with fp32 activations.
-  // A launch of fewer tokens can need more (down is cut into more parts), and the
-  // last launch of a long run may have any number.
-  size_t work[2][mnb::moe::kMaxTokens];
+  // Workspace of up to t + 1 tokens a launch. A launch of fewer tokens can need more
+  // (down is cut into more parts), and the last launch of a long run may have any number.
+  size_t work[mnb::moe::kMaxTokens];
 };
 
 namespace {
@@ -35,8 +34,8 @@ int Fail(const char *what, hipError_t e, int status) {
   return status;
 }
 
-size_t RunBytes(const mnb_moe_plan *p, int64_t T, int32_t x_type) {
-  return p->work[x_type == MNB_TYPE_FLOAT][std::min<int64_t>(T, kMaxTokens) - 1];
+size_t RunBytes(const mnb_moe_plan *p, int64_t T) {
+  return p->work[std::min<int64_t>(T, kMaxTokens) - 1];
 }
 
 void FreePlan(mnb_moe_plan *p) {
@@ -99,11 +98,8 @@ int Create(const mnb_moe_desc *d, const float *router, const mnb_moe_weight *gat
   l.gate_up.units = CeilDiv(d->hidden, kUnit);
   l.down.groups = CeilDiv(d->hidden, 32);
   l.down.units = CeilDiv(d->intermediate, kUnit);
-  for (const int32_t type : {MNB_TYPE_FLOAT16, MNB_TYPE_FLOAT})
-    for (int t = 0; t < kMaxTokens; ++t) {
-      size_t *work = p->work[type == MNB_TYPE_FLOAT];
-      work[t] = std::max(mnb::moe::WorkBytes(l, t + 1, type), t > 0 ? work[t - 1] : 0);
-    }
+  for (int t = 0; t < kMaxTokens; ++t)
+    p->work[t] = std::max(mnb::moe::WorkBytes(l, t + 1), t > 0 ? p->work[t - 1] : 0);
   const size_t up = static_cast<size_t>(d->experts) * l.gate_up.groups * l.gate_up.units;
   const size_t dn = static_cast<size_t>(d->experts) * l.down.groups * l.down.units;
   const size_t rec = kRecords * kRec, meta = mnb::moe::MetaBytes(l.folds, l.zeros);
@@ -221,7 +217,7 @@ int mnb_moe_workspace_bytes(const mnb_moe_plan *plan, int64_t T, int32_t x_type,
   if (plan == nullptr || bytes == nullptr) return MNB_ERR_NULL_POINTER;
   if (!FloatType(x_type)) return MNB_ERR_BAD_ATTRIBUTE;
   if (T < 0 || T > kMaxRun) return MNB_ERR_BAD_SHAPE;
-  *bytes = T == 0 ? 0 : RunBytes(plan, T, x_type);
+  *bytes = T == 0 ? 0 : RunBytes(plan, T);
   return MNB_OK;
 }
 
@@ -239,7 +235,7 @@ int mnb_moe_run(const mnb_moe_plan *plan, int64_t T, int32_t x_type, const void 
   if (!Aligned(dX, size) || !Aligned(dY, size) || !Aligned(dLogits, 4) || !Aligned(dIds, 4) ||
       !Aligned(dWeights, 4) || !Aligned(dWorkspace, 16))
     return MNB_ERR_BAD_SHAPE;
-  if (dWorkspace == nullptr || workspace_bytes < RunBytes(plan, T, x_type))
+  if (dWorkspace == nullptr || workspace_bytes < RunBytes(plan, T))
     return MNB_ERR_WORKSPACE;
   int cur = -1;
   if (hipGetDevice(&cur) != hipSuccess || cur != plan->device) return MNB_ERR_NO_DEVICE;

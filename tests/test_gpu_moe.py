@@ -427,3 +427,62 @@ def test_threads(pkg, cuda):
     torch.cuda.synchronize()
     for ys, w in zip(got, want):
         assert all(torch.equal(y, w) for y in ys)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("T,H,I,E,bs,zp", [
+    (1, 256, 128, 4, 32, True), (1, 512, 4224, 8, 128, False), (4, 256, 128, 4, 16, False),
+    (8, 384, 200, 4, 128, True), (9, 384, 200, 8, 64, True), (30, 256, 128, 4, 32, False),
+    (64, 256, 300, 4, 256, True)])
+def test_outliers_leave_the_other_values(pkg, cuda, T, H, I, E, bs, zp, dtype):
+    """Every 128th activation is 2^12, every 128th channel of the experts 2^12 times as
+    large, and their weights are zero: the result is that of the other values.
+
+    Beside 2^12 the fixed point's step is 2^-9. The other activations are multiples of
+    2^-6 below 2: exact. Their products are off by the fp32 scalings and additions
+    alone, (blocks + 4) 2^-24 of the digits' magnitudes: a value's digits add up to at
+    most four times its size and two halves of a digit, 2^8 steps. The experts' rows
+    are off by half a step, 2^-22 of their block's largest, more. The rest is
+    _layer64's."""
+    import torch
+    g = torch.Generator(device=cuda)
+    g.manual_seed(T + H + I)
+    x = torch.randint(-127, 128, (T, H), device=cuda, generator=g).float() / 64
+    x[:, ::128] = torch.where(torch.arange(T, device=cuda) % 2 == 0, 4096.0, -4096.0)[:, None]
+    x = x.to(getattr(torch, dtype))
+    _, _, ws = _problem(1, H, I, E, bs, zp, "float32", 7, cuda)
+    for B, S, Z in ws:
+        if Z is not None:
+            Z.fill_(0x88)
+        row = B.flatten(2)  # zero weights for every 128th value
+        row[:, :, ::64] = row[:, :, ::64] & 0xF0 | 8
+        B.copy_(row.reshape(B.shape))
+    ws[1][1][:, ::128] *= 4096.0
+    dense = [_dense(w, n) for w, n in zip(ws, (H, H, I))]
+    logits = torch.randn(T, E, device=cuda, generator=g)
+    ids, p = _choice(logits, 2, True)
+    op = pkg.MatMulNBitsMoE(H, I, E, 2, block_size=bs).prepare_device(None, *ws)
+    y = op(x, logits=logits)
+    print(f"case moe outliers T={T} H={H} I={I} E={E} bs={bs} zp={zp} {dtype}", flush=True)
+    v = x.double()
+    ref, err = torch.zeros_like(v), torch.zeros_like(v)
+
+    def product(v, ve, W, exact):
+        Wt, top = W.t().contiguous(), _blocks(v.abs() + ve)
+        digits = 4 * (v.abs() + ve) + 2.0 ** -13 * top
+        off = ve + (0 if exact else 2.0 ** -22 * top) + (-(-v.shape[1] // bs) + 4) * 2.0 ** -24 * digits
+        return v @ Wt, off @ Wt.abs()
+
+    for e in sorted(set(ids.flatten().tolist())):
+        t, s = torch.nonzero(ids == e, as_tuple=True)
+        zero = torch.zeros_like(v[t])
+        gate, ge = product(v[t], zero, dense[0][e], True)
+        up, ue = product(v[t], zero, dense[1][e], True)
+        silu = gate * torch.sigmoid(gate)
+        se = 1.1 * ge + 2.0 ** -20 * (silu.abs() + 1.1 * ge)
+        h, he = silu * up, se * (up.abs() + ue) + silu.abs() * ue
+        d, de = product(h, he + 2.0 ** -23 * (h.abs() + he), dense[2][e], False)
+        w = p[t, s][:, None]
+        ref[t] += w * d
+        err[t] += w * de + w * 2.0 ** -18 * (d.abs() + de)
+    print(f"  worst / bound {_check(y, ref, err):.3f}", flush=True)
