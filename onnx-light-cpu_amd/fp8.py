@@ -9,6 +9,7 @@ errors, and no CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import math
 
 import numpy as np
 
@@ -53,6 +54,19 @@ def _elsewhere(device, stream):
     if stream.device != device:
         raise ValueError(f"stream of {stream.device}, tensors on {device}")
     return torch.cuda.stream(stream)
+
+
+def _laid_out(shape, want):
+    """Whether values of `shape` lie in memory as those of `want`: axes of 1 apart, the
+    same one, or with neighbouring axes joined into one."""
+    want = [n for n in want if n != 1]
+    for n in shape:
+        joined = 1
+        while joined < n and want:
+            joined *= want.pop(0)
+        if joined != n:
+            return False
+    return not want
 
 
 def quantize_fp8(X, stream=None):
@@ -110,23 +124,32 @@ class MatMulFp8:
     _stream_workspace = MatMulNBits._stream_workspace
 
     # -- constants ---------------------------------------------------------
-    def _check_sizes(self, w, s):
+    def _check_sizes(self, W, scales):
         if self.K <= 0 or self.N <= 0:
             return  # the C ABI reports it
-        blocks = -(-self.N // BLOCK) * -(-self.K // BLOCK)
+        blocks = [-(-self.N // BLOCK), -(-self.K // BLOCK)]
+        w, s = math.prod(W.shape), math.prod(scales.shape)
         if w != self.N * self.K:
             raise ValueError(f"{PREFIX}: W has {w} values, expected N*K = {self.N * self.K}")
-        if s != blocks:
-            raise ValueError(f"{PREFIX}: scales has {s} elements, expected {blocks}")
+        if s != blocks[0] * blocks[1]:
+            raise ValueError(f"{PREFIX}: scales has {s} elements, expected "
+                             f"{blocks[0] * blocks[1]}")
+        if not _laid_out(W.shape, [self.N, self.K]):
+            raise ValueError(f"{PREFIX}: W must be [N, K] = {[self.N, self.K]}, got "
+                             f"{list(W.shape)}")
+        if not _laid_out(scales.shape, blocks):
+            raise ValueError(f"{PREFIX}: scales must be [ceil(N / 128), ceil(K / 128)] = {blocks}, "
+                             f"got {list(scales.shape)}")
 
     def prepare(self, W, scales):
         """Uploads host (numpy) constants once, to the current device: W uint8
-        (e4m3 codes) [N, K], scales float32 [ceil(N / 128), ceil(K / 128)]."""
+        (e4m3 codes) [N, K], scales float32 [ceil(N / 128), ceil(K / 128)] (axes may be
+        joined, as in flat arrays)."""
         import torch
         self.release()
         W = np.ascontiguousarray(W, dtype=np.uint8)
         scales = np.ascontiguousarray(scales, dtype=np.float32)
-        self._check_sizes(W.size, scales.size)
+        self._check_sizes(W, scales)
         _check(_library().mnb_fp8_plan_create(self.K, self.N, _host_ptr(W), _host_ptr(scales),
                                               ctypes.byref(self._plan)), "prepare")
         self._device = torch.device("cuda", torch.cuda.current_device())
@@ -142,7 +165,7 @@ class MatMulFp8:
             raise ValueError(f"{PREFIX}: W must be a float8_e4m3fn or uint8 device tensor")
         if scales.device != W.device or scales.dtype != torch.float32:
             raise ValueError(f"{PREFIX}: scales must be a float32 tensor on W's device")
-        self._check_sizes(W.numel(), scales.numel())
+        self._check_sizes(W, scales)
         with torch.cuda.device(W.device):
             w, s = W.contiguous(), scales.contiguous()
             _check(_library().mnb_fp8_plan_create_device(self.K, self.N, _dev_ptr(w), _dev_ptr(s),

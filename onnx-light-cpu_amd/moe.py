@@ -9,11 +9,12 @@ first axis. There is no CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import math
 
 import numpy as np
 
 from . import MatMulNBits, _check, _raw_stream, library
-from .fp8 import _elsewhere
+from .fp8 import _elsewhere, _laid_out
 
 PREFIX = "onnx_light_cpu_amd::MatMulNBitsMoE"
 
@@ -74,23 +75,27 @@ class MatMulNBitsMoE:
     _stream_workspace = MatMulNBits._stream_workspace
 
     # -- constants ---------------------------------------------------------
-    def _check_sizes(self, router, gate, up, down, size):
+    def _check_sizes(self, router, gate, up, down):
         d = self.desc
         if min(d.hidden, d.intermediate, d.experts) <= 0 or d.block_size < 2:
             return  # the C ABI reports it
+        arrays = []
         for name, w, n, k in (("gate", gate, d.intermediate, d.hidden),
                               ("up", up, d.intermediate, d.hidden),
                               ("down", down, d.hidden, d.intermediate)):
             nb = -(-k // d.block_size)
-            want = (d.experts * n * nb * (d.block_size // 2), d.experts * n * nb,
-                    d.experts * n * ((nb + 1) // 2))
-            for what, a, count in zip(("B", "scales", "zero_points"), w, want):
-                if a is not None and size(a) != count:
-                    raise ValueError(f"{PREFIX}: {name}'s {what} has {size(a)} elements, "
-                                     f"expected {count}")
-        if router is not None and size(router) != d.experts * d.hidden:
-            raise ValueError(f"{PREFIX}: router has {size(router)} elements, expected "
-                             f"{d.experts * d.hidden}")
+            for what, a, last in zip(("B", "scales", "zero_points"), w,
+                                     ([nb, d.block_size // 2], [nb], [(nb + 1) // 2])):
+                arrays.append((f"{name}'s {what}", a, [d.experts, n] + last))
+        arrays.append(("router", router, [d.experts, d.hidden]))
+        arrays = [(name, a, want) for name, a, want in arrays if a is not None]
+        for name, a, want in arrays:
+            if math.prod(a.shape) != math.prod(want):
+                raise ValueError(f"{PREFIX}: {name} has {math.prod(a.shape)} elements, expected "
+                                 f"{math.prod(want)}")
+        for name, a, want in arrays:
+            if not _laid_out(a.shape, want):
+                raise ValueError(f"{PREFIX}: {name} must be {want}, got {list(a.shape)}")
 
     def _weights(self, gate, up, down):
         ws = [tuple(w) + (None,) * (3 - len(w)) for w in (gate, up, down)]
@@ -104,14 +109,15 @@ class MatMulNBitsMoE:
         down: (B, scales, zero_points or None), MatMulNBits weights with the experts
         as first axis, gate and up [experts, intermediate, ...] over hidden, down
         [experts, hidden, ...] over intermediate; router float32 [experts, hidden],
-        or None where every call brings its logits."""
+        or None where every call brings its logits. Axes may be joined, as in flat
+        arrays."""
         import torch
         self.release()
         ws = [tuple(None if a is None else np.ascontiguousarray(a, dtype=t)
                     for a, t in zip(w, (np.uint8, np.float32, np.uint8)))
               for w in self._weights(gate, up, down)]
         r = None if router is None else np.ascontiguousarray(router, dtype=np.float32)
-        self._check_sizes(r, *ws, lambda a: a.size)
+        self._check_sizes(r, *ws)
         self._create("mnb_moe_plan_create", r, ws, lambda a: a.ctypes.data)
         self._device = torch.device("cuda", torch.cuda.current_device())
         return self
@@ -130,7 +136,7 @@ class MatMulNBitsMoE:
                                      "points uint8 tensors on one device")
         if router is not None and (router.dtype != torch.float32 or router.device != device):
             raise ValueError(f"{PREFIX}: router must be a float32 tensor on the weights' device")
-        self._check_sizes(router, *ws, lambda a: a.numel())
+        self._check_sizes(router, *ws)
         with torch.cuda.device(device):
             ws = [tuple(None if a is None else a.contiguous() for a in w) for w in ws]
             r = None if router is None else router.contiguous()

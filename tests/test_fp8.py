@@ -75,3 +75,22 @@ def test_python_refusals(pkg):
         op.prepare_device(torch.zeros(8, 8, dtype=torch.uint8), torch.zeros(1, 1))
     with pytest.raises(ValueError, match="bad shape"):
         pkg.MatMulFp8(0, 8).prepare(np.zeros(1, np.uint8), np.zeros(1, np.float32))
+
+
+def test_shapes_of_constants(pkg):
+    """A weight or scales with the right number of values in the wrong order."""
+    import torch
+    op = pkg.MatMulFp8(256, 384)
+    W, S = np.zeros((384, 256), np.uint8), np.zeros((3, 2), np.float32)
+    for w, s, match in ((W.T, S, r"W must be \[N, K\] = \[384, 256\], got \[256, 384\]"),
+                        (W.reshape(192, 512), S, "W must be"), (W.reshape(768, 128), S, "W must"),
+                        (W, S.T, r"scales must be .* = \[3, 2\], got \[2, 3\]")):
+        with pytest.raises(ValueError, match=match):
+            op.prepare(w, s)
+    assert not op._plan
+    laid_out = pkg.fp8._laid_out
+    for shape in ((2, 3, 4), (6, 4), (2, 12), (24,), (1, 2, 3, 1, 4), (24, 1)):
+        assert laid_out(shape, [2, 3, 4])
+    for shape in ((3, 2, 4), (4, 6), (12, 2), (2, 4, 3), (2, 2, 6), (2, 3), (2, 3, 4, 2), ()):
+        assert not laid_out(shape, [2, 3, 4])
+    assert laid_out((1, 1), [1]) and laid_out((5,), [1, 5, 1]) and laid_out((), [1, 1])

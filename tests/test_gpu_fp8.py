@@ -484,3 +484,18 @@ def test_products_beside_larger_ones(pkg, cuda, M, K, N):
     assert torch.equal(op(A, scales=sa, out_dtype=torch.float16), ref.half())
     worst = _within(op(A, scales=sa, out_dtype=torch.bfloat16), ref, mag, K)
     print(f"  bfloat16: worst / bound {worst:.3f}", flush=True)
+
+
+def test_flat_constants(pkg, cuda):
+    """W and scales whose axes are joined give the same plan."""
+    import torch
+    A, sa, W, sw = _problem(5, 300, 200, 43, cuda)
+    want = pkg.MatMulFp8(300, 200).prepare_device(W, sw)(A, scales=sa)
+    flat = pkg.MatMulFp8(300, 200).prepare_device(W.reshape(-1), sw.reshape(1, -1))
+    host = pkg.MatMulFp8(300, 200).prepare(W.view(torch.uint8).cpu().numpy().reshape(-1),
+                                           sw.cpu().numpy().reshape(-1))
+    assert torch.equal(flat(A, scales=sa), want) and torch.equal(host(A, scales=sa), want)
+    with pytest.raises(ValueError, match="W must be"):
+        flat.prepare_device(W.view(torch.uint8).t(), sw)
+    with pytest.raises(ValueError, match="scales must be"):
+        flat.prepare_device(W, sw.t())

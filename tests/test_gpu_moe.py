@@ -486,3 +486,17 @@ def test_outliers_leave_the_other_values(pkg, cuda, T, H, I, E, bs, zp, dtype):
         ref[t] += w * d
         err[t] += w * de + w * 2.0 ** -18 * (d.abs() + de)
     print(f"  worst / bound {_check(y, ref, err):.3f}", flush=True)
+
+
+def test_joined_axes_of_constants(pkg, cuda):
+    """Weights with their axes joined give the same plan; other orders are refused."""
+    import torch
+    x, router, ws = _problem(3, 64, 96, 4, 32, True, "float32", 47, cuda)
+    want = pkg.MatMulNBitsMoE(64, 96, 4, 2).prepare_device(router, *ws)(x)
+    flat = [tuple(a.flatten(1) for a in w) for w in ws]
+    op = pkg.MatMulNBitsMoE(64, 96, 4, 2).prepare_device(router.reshape(-1), *flat)
+    assert torch.equal(op(x), want)
+    with pytest.raises(ValueError, match="router must be"):
+        op.prepare_device(router.t(), *ws)
+    with pytest.raises(ValueError, match="gate's scales must be"):
+        op.prepare_device(router, (ws[0][0], ws[0][1].transpose(1, 2), ws[0][2]), ws[1], ws[2])

@@ -95,3 +95,25 @@ def test_python_refusals(pkg):
         op.prepare_device(None, *(tuple(torch.from_numpy(a) for a in w) for w in (gate, gate, down)))
     with pytest.raises(ValueError, match="bad attribute"):
         pkg.MatMulNBitsMoE(64, 32, 4, 5).prepare(router, gate, gate, down)
+
+
+def test_shapes_of_constants(pkg):
+    """Weights, zero points and a router with the right number of elements in the wrong
+    order."""
+    op = pkg.MatMulNBitsMoE(64, 128, 4, 2)
+    up = (np.zeros((4, 128, 2, 16), np.uint8), np.zeros((4, 128, 2), np.float32),
+          np.zeros((4, 128, 1), np.uint8))
+    down = (np.zeros((4, 64, 4, 16), np.uint8), np.zeros((4, 64, 4), np.float32),
+            np.zeros((4, 64, 2), np.uint8))
+    router = np.zeros((4, 64), np.float32)
+    for args, match in (
+            ((router, down, up, down), r"gate's B must be \[4, 128, 2, 16\], got \[4, 64, 4, 16\]"),
+            ((router, up, up, (up[0],) + down[1:]), "down's B must be"),
+            ((router, up, (up[0].transpose(1, 0, 2, 3),) + up[1:], down), "up's B must be"),
+            ((router, up, up, (down[0], down[1].transpose(0, 2, 1), down[2])),
+             r"down's scales must be \[4, 64, 4\], got \[4, 4, 64\]"),
+            ((router, up, up, down[:2] + (down[2].transpose(0, 2, 1),)), "down's zero_points must"),
+            ((router.T, up, up, down), r"router must be \[4, 64\], got \[64, 4\]")):
+        with pytest.raises(ValueError, match=match):
+            op.prepare(*args)
+    assert not op._plan
