@@ -1010,19 +1010,22 @@ Shape PickShape(const Layer &l, int tokens) {
   const int64_t blocks = s.entries * CeilDiv(l.intermediate, 128);  // of 128 channels
   // Narrow workgroups, and down with the sum over the experts, where blocks of 128
   // channels leave CUs idle (us, narrow and not; one token of hidden 4096, experts of
-  // 14336: 1 chosen 35 and 50, 2 chosen 50 and 57, 4 chosen 91 and 85; 2 tokens of
-  // 4096 x 2048, 2 of 16: 26 and 40; 4 tokens of 2048 x 1024, 4 of 64: 32 and 30; 8
-  // tokens, 6 of 64: 54 and 44).
+  // 14336: 1 chosen 35 and 48, 2 chosen 52 and 61, 4 chosen 92 and 86; 2 tokens of
+  // 4096 x 2048, 2 of 16: 25 and 41; 4 tokens of 2048 x 1024, 4 of 64: 33 and 30; 8
+  // tokens, 6 of 64: 65 and 44).
   s.narrow = tokens <= kNarrowTokens && blocks < (tokens == 1 ? l.num_cus : 3 * l.num_cus / 8);
   // The units over four wavefronts each: one token of 2048 x 1024, 6 of 64: 19 us,
-  // 23 without; one of 4096 x 14336, 2 of 8, does not fill them: 49 both.
+  // 23 without; one of 4096 x 14336, 2 of 8, whose workgroups fill the chip: 64, 52 without.
   s.split = s.narrow && 2 * blocks <= l.num_cus;
   // A workgroup's choice among more experts takes longer than a launch of its own (6 of
   // 64: 19 us, 21 with a launch).
   s.choose = tokens == 1 && l.experts <= 256;
   // What most experts' tokens fill: their mean share and two standard deviations
-  // of even choices (32 tokens of 4096 x 4096, 2 of 8: four groups 62 us, one 84; 64
-  // of 2048 x 1024, 8 of 64: two 81, one 92).
+  // of even choices (us with one, two and four groups: 32 tokens of 4096 x 4096, 2 of 8:
+  // 100, 79 and 77; 64 of 2048 x 1024, 8 of 64: 123, 116 and 105, 8 of 128: 149, 145 and
+  // 162; 24 of 2048 x 1408, 4 of 60: 75, 85 and 90). Where two experts are chosen by half
+  // of the tokens each, the same number is the best of the three, or within 1% of it:
+  // 151, 123 and 108; 159, 138 and 120, 193, 165 and 169; 77, 77 and 82.
   const int group = tokens == 1 ? 1 : kTokens<false>;
   const double mean = static_cast<double>(tokens) * l.top_k / l.experts;
   const double most = std::min<double>(tokens, mean + 2.0 * std::sqrt(mean));
@@ -1032,7 +1035,7 @@ Shape PickShape(const Layer &l, int tokens) {
                                                      : 4;
   s.segments = s.entries + tokens * l.top_k / (s.groups * group);
   // Down: about two workgroups a CU, of at least four units (32 tokens of 4096 x 4096,
-  // 2 of 8: 62 us, 68 with whole rows; 4 of 4096 x 14336: 120 and 180).
+  // 2 of 8: 77 us, 83 with whole rows; 4 of 4096 x 14336: 112 and 167).
   const double share = static_cast<double>(l.top_k) / l.experts;
   const double met = l.experts * (1.0 - std::pow(1.0 - share, tokens));
   const double blocks_down = std::max(1.0, met) * CeilDiv(l.hidden, 256);
