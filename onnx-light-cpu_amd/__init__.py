@@ -645,5 +645,5 @@ class NodeKernel:
             pass
 
 
-from .fp8 import MatMulFp8, quantize_fp8  # noqa: E402,F401  (they use the names above)
+from .fp8 import MatMulFp8, quantize_fp8, release_workspaces  # noqa: E402,F401  (use the above)
 from .moe import MatMulNBitsMoE  # noqa: E402,F401

@@ -21,6 +21,15 @@ QUANTIZE_PREFIX = "onnx_light_cpu_amd::QuantizeFp8"
 
 _lib = None
 _types = None  # torch dtype -> MNB_TYPE_* of include/mnb_fp8.h
+# Workspaces by thread and stream, of all objects: their calls there run one after
+# another, and a model has hundreds of them (8192 rows of K = 14336: 117 MB a call).
+_shared_works = {}
+
+
+def release_workspaces():
+    """Gives the workspaces that MatMulFp8 and MatMulNBitsMoE calls share back to torch's
+    allocator; the next calls have new ones."""
+    _shared_works.clear()
 
 
 def _library():
@@ -118,9 +127,9 @@ class MatMulFp8:
         self.K, self.N = int(K), int(N)
         self._plan = ctypes.c_void_p()
         self._device = None
-        self._works = {}  # by thread and stream
         self._needs = {}  # workspace bytes by (rows, dtype)
 
+    _works = _shared_works
     _stream_workspace = MatMulNBits._stream_workspace
 
     # -- constants ---------------------------------------------------------
@@ -178,7 +187,7 @@ class MatMulFp8:
         if self._plan:
             _library().mnb_fp8_plan_destroy(self._plan)
             self._plan = ctypes.c_void_p()
-        self._works, self._needs = {}, {}
+        self._needs = {}
 
     def __del__(self):
         try:

@@ -14,7 +14,7 @@ import math
 import numpy as np
 
 from . import MatMulNBits, _check, _raw_stream, library
-from .fp8 import _elsewhere, _laid_out
+from .fp8 import _elsewhere, _laid_out, _shared_works
 
 PREFIX = "onnx_light_cpu_amd::MatMulNBitsMoE"
 
@@ -69,9 +69,9 @@ class MatMulNBitsMoE:
         self._plan = ctypes.c_void_p()
         self._device = None
         self._router = False
-        self._works = {}  # by thread and stream
         self._needs = {}  # workspace bytes by (tokens, type)
 
+    _works = _shared_works
     _stream_workspace = MatMulNBits._stream_workspace
 
     # -- constants ---------------------------------------------------------
@@ -155,7 +155,7 @@ class MatMulNBitsMoE:
         if self._plan:
             _library().mnb_moe_plan_destroy(self._plan)
             self._plan = ctypes.c_void_p()
-        self._works, self._needs = {}, {}
+        self._needs = {}
 
     def __del__(self):
         try:

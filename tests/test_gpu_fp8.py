@@ -499,3 +499,35 @@ def test_flat_constants(pkg, cuda):
         flat.prepare_device(W.view(torch.uint8).t(), sw)
     with pytest.raises(ValueError, match="scales must be"):
         flat.prepare_device(W, sw.t())
+
+
+def test_objects_share_a_workspace(pkg, cuda):
+    """Objects that run one after another on a stream take turns at one workspace; two
+    streams and a released object change no result, and it can be given back."""
+    import torch
+    pkg.release_workspaces()
+    K, N, M = 1000, 640, 500
+    ops, xs = [], []
+    for i in range(6):
+        _, _, W, sw = _problem(1, K, N, 51 + i, cuda)
+        ops.append(pkg.MatMulFp8(K, N).prepare_device(W, sw / 4096))
+        xs.append(torch.randn(M, K, device=cuda))
+    out = [torch.empty(M, N, device=cuda) for _ in ops]
+    need = ops[0].workspace_bytes(M, torch.float32)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for op, x, y in zip(ops, xs, out):
+        op(x, out=y)
+    assert need >= M * K and torch.cuda.memory_allocated() - before <= need + 512
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [op(x, stream=streams[i % 2]) for i, (op, x) in enumerate(zip(ops, xs))]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, out))
+    ops[0].release()
+    assert torch.equal(ops[1](xs[1]), out[1])
+    del got
+    torch.cuda.synchronize()
+    pkg.release_workspaces()
+    assert torch.cuda.memory_allocated() <= before
+    assert torch.equal(ops[2](xs[2]), out[2])

@@ -500,3 +500,29 @@ def test_joined_axes_of_constants(pkg, cuda):
         op.prepare_device(router.t(), *ws)
     with pytest.raises(ValueError, match="gate's scales must be"):
         op.prepare_device(router, (ws[0][0], ws[0][1].transpose(1, 2), ws[0][2]), ws[1], ws[2])
+
+
+def test_layers_share_a_workspace(pkg, cuda):
+    """Layers that run one after another on a stream take turns at one workspace, which
+    the 8-bit products have too."""
+    import torch
+    pkg.release_workspaces()
+    layers = []
+    for i in range(4):
+        x, router, ws = _problem(40, 256, 384, 8, 32, True, "bfloat16", 61 + i, cuda)
+        layers.append((pkg.MatMulNBitsMoE(256, 384, 8, 2).prepare_device(router, *ws), x,
+                       torch.empty_like(x)))
+    W = torch.ones(256, 300, device=cuda).to(torch.float8_e4m3fn)
+    proj = pkg.MatMulFp8(300, 256).prepare_device(W, torch.ones(2, 3, device=cuda))
+    v, o = torch.ones(100, 300, device=cuda), torch.empty(100, 256, device=cuda)
+    need = layers[0][0].workspace_bytes(40, torch.bfloat16)
+    assert need > proj.workspace_bytes(100, torch.float32) > 0
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for op, x, y in layers:
+        op(x, out=y)
+        proj(v, out=o)
+    assert torch.cuda.memory_allocated() - before <= need + 512
+    for op, x, y in layers:
+        assert torch.equal(op(x), y)
+    assert bool((o == 300).all())
