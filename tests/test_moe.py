@@ -117,3 +117,20 @@ def test_shapes_of_constants(pkg):
         with pytest.raises(ValueError, match=match):
             op.prepare(*args)
     assert not op._plan
+
+
+@pytest.mark.parametrize("hidden,intermediate", [
+    ((1 << 18) + 1, 32), (64, (1 << 18) + 1), (1 << 18, (1 << 16) + 1), ((1 << 16) + 1, 1 << 18)])
+def test_width_limits(pkg, lib, hidden, intermediate):
+    """One past each width's limit, which keeps offsets in 32 bits, and past the
+    product's, with both widths inside theirs."""
+    assert _create(pkg, lib, hidden=hidden, intermediate=intermediate) == SHAPE
+
+
+@pytest.mark.parametrize("hidden,intermediate", [(1 << 18, 1 << 16), (1 << 16, 1 << 18)])
+def test_widths_at_their_limits(pkg, lib, hidden, intermediate):
+    """The limits themselves pass the description's check: what is refused next is
+    the missing weight."""
+    ws = _weights(pkg)
+    ws[2] = None
+    assert _create(pkg, lib, ws, hidden=hidden, intermediate=intermediate) == NULLP
