@@ -10,7 +10,8 @@
  * shorter. It stands beside the 4-bit MatMulNBits of mnb.h (the same weight
  * layout [N, K], prepared plan, status codes and rules on streams and
  * workspaces); no ONNX operator has this contract, so it is not in the node
- * registration table. The reference has no counterpart.
+ * registration table. The reference has no counterpart. A block's two scales are
+ * multiplied in fp32 first, so their product has to be in fp32's range.
  *
  * Conventions of mnb.h hold: device pointers on the plan's device, streams as
  * void* (NULL = the default stream), every entry point returns an mnb_status,

@@ -192,8 +192,9 @@ __global__ __launch_bounds__(64 * WAVES) void Fp8StreamKernel(
 
 // 17 to 64 rows: the rows, and with them the weights and the row scales, pass
 // through LDS, each wavefront's own blocks NS deep, so that the rows are copied by
-// whole lines (gathered into registers they bound it: 32 us at 48 x 14336 x 4096, 16.6
-// so). Bound by those rows, which every 16 columns read again.
+// whole lines (gathered into registers they bound it: 32 us at 48 x 14336 x 4096 with the
+// weights in the last cache, 16.6 so). Bound by those rows, which every 16 columns read
+// again: 32 x 14336 x 4096 18 us, 3.3 TB/s of weights, 17 rows 14.5.
 template <int MC, int WAVES, int NS, bool EXACT, typename T>
 __global__ __launch_bounds__(64 * WAVES) void Fp8StreamLdsKernel(
     const uint8_t *__restrict__ W, const float *__restrict__ SW, const uint8_t *__restrict__ A,
@@ -293,7 +294,8 @@ __global__ __launch_bounds__(64 * WAVES) void Fp8StreamLdsKernel(
 // 47 us instead of 44 at 200 x 4096 x 28672). Four wavefronts, one per SIMD, and
 // two workgroups a CU where LDS allows: one's waits are the other's work (300 x 4096
 // x 4096, fp32 Y: 31 us with 128 x 128 tiles of eight wavefronts and K in two parts,
-// 27 with 64 x 128 of four). What bounds it: the start and the end of a tile (10 us of
+// 27 with 64 x 128 of four; 8192 x 4096 x 14336, 128 x 128: fp32 Y 903 us, fp16 Y 830,
+// 1.16 PFLOP/s). What bounds it: the start and the end of a tile (10 us of
 // the 20 at 333 x 2500 x 5001, fp32 Y, with one block of K), then copies, LDS reads
 // and MFMAs about equally.
 template <int MI, int WM, int WN, int NS, bool EXACT, typename T>
@@ -496,7 +498,8 @@ __global__ __launch_bounds__(64 * WM *WN) void Fp8TileKernel(
 // Left is the power limit: with these operands moving, the clock falls to 1.6-1.7
 // GHz (1.55 with the copies switched off, 2.1 on constant operands).
 // 8192 x 4096 x 14336: 604 us with barriers between the blocks, 510 with them
-// inside, 460 so.
+// inside, 460 with copies half a block earlier, 437 with rows copied by whole lines,
+// 418 so (2.30 PFLOP/s).
 constexpr int kWideTile = 256;
 
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void Fp8WideKernel(

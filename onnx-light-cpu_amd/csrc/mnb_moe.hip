@@ -582,9 +582,10 @@ constexpr int WavesPerSimd(int gc, int folds) {
 // Gate/up: workgroup (b, i) the channels of block b of entry i's expert, 16
 // (gate and up) for each of GROUPS wavefronts that share a pipe, or, with KS runs
 // of the units, for each of GROUPS * KS wavefronts with pipes of their own. Bound by
-// reading: 64 tokens of 4096 x 14336, 2 of 8 experts, 105 us (4.8 TB/s; about 10 less
-// without the products), one token 25 us (5.1 TB/s); one of 2048 x 1024, 6 of 64, 9 us,
-// its launch and two round trips.
+// reading: one token of 4096 x 14336, 2 of 8 experts, 25 us (5.1 TB/s); one of 2048 x
+// 1024, 6 of 64, 9 to 11 us, its launch and two round trips; 64 tokens of 4096 x 14336
+// 119 us, 4.2 TB/s counting each weight once: experts of more than 20 tokens, one in
+// ten of even choices, read theirs twice.
 template <bool ONE, int GC, int F, bool ZP, int GROUPS, int KS, int NS, bool CHOOSE>
 __global__ __launch_bounds__(64 * GROUPS *KS,
                              GROUPS == 8 ? WavesPerSimd(GC, F) : 1) void MoeGateUpKernel(
@@ -829,7 +830,8 @@ __global__ __launch_bounds__(512) void MoeDownNarrowKernel(Matrix m, Fixed fh, P
 
 // Down otherwise: a workgroup takes 256 columns of Y and part blockIdx.y % cuts of the
 // units of one segment. Every pair's row, times its weight, goes to parts
-// [cuts][pairs][width]. 64 tokens of 4096 x 14336, 2 of 8: 53 us, 4.8 TB/s.
+// [cuts][pairs][width]. 64 tokens of 4096 x 14336, 2 of 8: 55 us where no expert has
+// more than 20 tokens (4.5 TB/s), 72 where one or two have.
 template <bool ONE, int GC, int F, bool ZP, int NS>
 __global__ __launch_bounds__(512, WavesPerSimd(GC, F)) void MoeDownKernel(Matrix m, Fixed fh, Plan plan,
                                                      float *__restrict__ parts, int pairs, int cuts,
