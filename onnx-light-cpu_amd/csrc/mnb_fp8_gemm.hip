@@ -719,7 +719,8 @@ __global__ __launch_bounds__(256) void Fp8SumKernel(const float *__restrict__ P,
 // columns each read all rows, M K bytes, and the more of them a CU has (r, rounded up)
 // the earlier the tiles' longer start is paid for: r r M K decides, up to 256 KiB of it
 // where up to 16 rows are gathered into registers, up to 448 KiB where they pass through
-// LDS; from r = 6, or 3, on the tiles are as fast or faster whatever K.
+// LDS. From r = 6, or 3, on the tiles lose 1 us at the few K and M where they lose at
+// all, and gain more elsewhere.
 // us, stream and tile, bf16 Y, weights not in a cache:
 //   N = 4096 (r = 1): K = 14336 16 rows 16 and 17, 32 rows 18 and 18, 33 rows 19 and 19,
 //     48 rows 23 and 20, 64 rows 26 and 22; K = 20480 17 rows 20 and 21, 32 rows 24 and

@@ -10,7 +10,8 @@ the sum of magnitudes, which the same sum bounds. _layer64 carries these bounds
 through the layer: through silu (slope at most 1.1), the product with up, the
 second rounding, down, and the weighted sum; the choice's weights are off by at
 most 2^-19 (fp32 exp, one ulp, and a sum of at most E terms). The output's own
-rounding is at most half a step of it.
+rounding is at most half a step of it. (16-bit types are rounded to 2^-22 too:
+test_outliers_leave_the_other_values holds them to that.)
 """
 import ctypes
 
