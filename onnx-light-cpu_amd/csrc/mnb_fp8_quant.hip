@@ -1,6 +1,7 @@
 // Rows to e4m3 with a scale for each block of 128, the weight layout of the
 // 8-bit product, and the padding of ragged code rows.
 #include "mnb_fp8.h"
+#include "mnb_values.h"
 
 namespace mnb {
 namespace fp8 {
@@ -8,43 +9,7 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <typename T>
-__device__ __forceinline__ float ToFloat(T v) {
-  return static_cast<float>(v);
-}
-
-// Eight values at p (n of them exist), zeros behind them.
-template <typename T, bool VEC>
-__device__ __forceinline__ void Load8(const T *p, int n, float (&x)[8]) {
-  if constexpr (VEC) {
-    if (n <= 0) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-      return;
-    }
-    typedef T Vec __attribute__((ext_vector_type(16 / sizeof(T))));
-#pragma unroll
-    for (int v = 0; v < static_cast<int>(sizeof(T)) / 2; ++v) {
-      const Vec q = reinterpret_cast<const Vec *>(p)[v];
-#pragma unroll
-      for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i)
-        x[v * static_cast<int>(16 / sizeof(T)) + i] = ToFloat(q[i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = i < n ? ToFloat(p[i]) : 0.0f;
-  }
-}
-
-// One (row, block) item per 16 lanes, eight values a lane. The quotient
-// 448 x / amax is correctly rounded to fp32 (for fp32 x up to rare double
-// roundings of a 2^-47 residue), since half-way codes are common among 16-bit rows
-// and a reciprocal's rounding would push them to either side: with
-// a = amax 2^-e in [1, 2) and r the rounded 1 / a, q0 = t r is off by at most
-// two units, its remainder t - q0 a is exact in one fma, and q0 + remainder r
-// rounds to the nearest (Markstein). t = 448 x 2^-e carries its own rounding
-// error along for fp32 rows. Four to six operations a value instead of a
-// division's eleven; bound by memory.
+// One (row, block) item per 16 lanes, eight values a lane; bound by memory.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(kThreads) void QuantizeKernel(const T *__restrict__ X,
                                                            uint8_t *__restrict__ Q,
@@ -58,46 +23,20 @@ __global__ __launch_bounds__(kThreads) void QuantizeKernel(const T *__restrict__
   const int n = static_cast<int>(min(int64_t{8}, K - k0));  // <= 0 past the row
   float x[8];
   Load8<T, VEC>(X + row * ldx + k0, n, x);
-  // As integers, magnitudes order like their values, infinity above them and NaN on top.
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+  uint32_t top = TopBits(x);
 #pragma unroll
   for (int off = 8; off >= 1; off >>= 1)
     top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 16)));
-  const uint32_t least = static_cast<uint32_t>(127 - 100) << 23;  // 2^-100
-  const float amax = __uint_as_float(max(top, least));
-  const int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-  float q[8];
-  if (top < 0x7F800000u) {
-    const float a = ldexpf(amax, -e);
-    const float r = 1.0f / a;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float xs = ldexpf(x[i], -e);
-      const float t = xs * 448.0f;
-      const float q0 = t * r;
-      float rem = fmaf(-q0, a, t);
-      if constexpr (sizeof(T) == 4) rem += fmaf(xs, 448.0f, -t);
-      q[i] = fmaf(rem, r, q0);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = x[i] / amax;  // 0 where x is finite (448 x may not be)
-  }
+  float amax;
+  const int2 code = BlockCodes<sizeof(T) == 4>(x, top, &amax);
   if ((threadIdx.x & 15) == 0) S[item] = amax / 448.0f;
-  int lo = 0, hi = 0;
-  lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], lo, false);
-  lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
-  hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], hi, false);
-  hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], hi, true);
   uint8_t *out = Q + row * ldq + k0;
   if constexpr (VEC) {
-    if (k0 < ldq) *reinterpret_cast<int2 *>(out) = make_int2(lo, hi);
+    if (k0 < ldq) *reinterpret_cast<int2 *>(out) = code;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (k0 + i < ldq) out[i] = static_cast<uint8_t>((i < 4 ? lo : hi) >> (8 * (i & 3)));
+      if (k0 + i < ldq) out[i] = static_cast<uint8_t>((i < 4 ? code.x : code.y) >> (8 * (i & 3)));
   }
 }
 

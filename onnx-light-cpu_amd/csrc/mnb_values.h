@@ -1,0 +1,107 @@
+// Loads, stores and 8-bit codes of rows in fp32, fp16 or bf16, shared by the
+// kernels that take them.
+#pragma once
+
+#include "mnb_kernels.h"
+
+namespace mnb {
+
+typedef float floatx4v __attribute__((ext_vector_type(4)));
+
+// Eight values at p (n of them exist), zeros behind them. VEC: p is aligned to 16
+// bytes, and all eight exist or none.
+template <typename T, bool VEC>
+__device__ __forceinline__ void Load8(const T *p, int n, float (&x)[8]) {
+  if constexpr (VEC) {
+    if (n <= 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+      return;
+    }
+    typedef T Vec __attribute__((ext_vector_type(16 / sizeof(T))));
+#pragma unroll
+    for (int v = 0; v < static_cast<int>(sizeof(T)) / 2; ++v) {
+      const Vec q = reinterpret_cast<const Vec *>(p)[v];
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i)
+        x[v * static_cast<int>(16 / sizeof(T)) + i] = static_cast<float>(q[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i < n ? static_cast<float>(p[i]) : 0.0f;
+  }
+}
+
+// Eight values to p, each rounded to T, n of them.
+template <typename T, bool VEC>
+__device__ __forceinline__ void Store8(T *p, int n, const float (&x)[8]) {
+  if constexpr (VEC) {
+    if (n <= 0) return;
+    typedef T Vec __attribute__((ext_vector_type(16 / sizeof(T))));
+#pragma unroll
+    for (int v = 0; v < static_cast<int>(sizeof(T)) / 2; ++v) {
+      Vec q;
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i)
+        q[i] = static_cast<T>(x[v * static_cast<int>(16 / sizeof(T)) + i]);
+      reinterpret_cast<Vec *>(p)[v] = q;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[i] = static_cast<T>(x[i]);
+  }
+}
+
+// The bits of the largest magnitude: as integers, magnitudes order like their
+// values, infinity above them and NaN on top.
+__device__ __forceinline__ uint32_t TopBits(const float (&x)[8]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+  return top;
+}
+
+// Four e4m3 codes of four values, ties to even.
+__device__ __forceinline__ int Codes4(float a, float b, float c, float d) {
+  int v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
+}
+
+// Codes of eight values of a row's block of 128 whose largest magnitude has the
+// bits `top`: 448 x / amax, amax at least 2^-100. FP32: the values are fp32, not
+// widened 16-bit ones. The quotient is correctly rounded to fp32 (for fp32 x up to
+// rare double roundings of a 2^-47 residue), since half-way codes are common among
+// 16-bit rows and a reciprocal's rounding would push them to either side: with
+// a = amax 2^-e in [1, 2) and r the rounded 1 / a, q0 = t r is off by at most
+// two units, its remainder t - q0 a is exact in one fma, and q0 + remainder r
+// rounds to the nearest (Markstein). t = 448 x 2^-e carries its own rounding
+// error along for fp32 rows. Four to six operations a value instead of a
+// division's eleven.
+template <bool FP32>
+__device__ __forceinline__ int2 BlockCodes(const float (&x)[8], uint32_t top, float *amax_out) {
+  const uint32_t least = static_cast<uint32_t>(127 - 100) << 23;  // 2^-100
+  const float amax = __uint_as_float(max(top, least));
+  const int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+  float q[8];
+  if (top < 0x7F800000u) {
+    const float a = ldexpf(amax, -e);
+    const float r = 1.0f / a;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float xs = ldexpf(x[i], -e);
+      const float t = xs * 448.0f;
+      const float q0 = t * r;
+      float rem = fmaf(-q0, a, t);
+      if constexpr (FP32) rem += fmaf(xs, 448.0f, -t);
+      q[i] = fmaf(rem, r, q0);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = x[i] / amax;  // 0 where x is finite (448 x may not be)
+  }
+  *amax_out = amax;
+  return make_int2(Codes4(q[0], q[1], q[2], q[3]), Codes4(q[4], q[5], q[6], q[7]));
+}
+
+} // namespace mnb

@@ -267,6 +267,14 @@ class MatMulFp8:
 
     run = __call__
 
+    def run_rmsnorm(self, X, gamma, eps: float = 1e-5, residual=None, out_dtype=None, stream=None):
+        """Y = this projection of rms_norm_fp8(X, gamma, eps, residual), the norm's input
+        of a decoder layer; of X's type, or out_dtype. With a residual: (Y, X + residual)."""
+        from .norm import rms_norm_fp8
+        codes, scales, *total = rms_norm_fp8(X, gamma, eps, residual=residual, stream=stream)
+        Y = self(codes, scales=scales, out_dtype=out_dtype or X.dtype, stream=stream)
+        return (Y, total[0]) if total else Y
+
     def workspace_bytes(self, M: int, dtype) -> int:
         """Device workspace of a call of M rows of `dtype` (mnb_fp8_workspace_bytes)."""
         n = ctypes.c_size_t()

@@ -1,0 +1,103 @@
+"""RMS norm with the residual's addition (include/mnb_norm.h).
+
+``rms_norm_fp8`` makes the e4m3 rows that ``MatMulFp8`` multiplies,
+``rms_norm`` rows of X's own type, as ``MatMulNBitsMoE`` takes them; with a
+residual both return the sum too, which the next residual addition needs.
+``MatMulNBits.run_rmsnorm`` and ``MatMulFp8.run_rmsnorm`` take the norm with their
+product. There is no CPU fallback.
+"""
+from __future__ import annotations
+
+import ctypes
+
+from . import _check, _raw_stream, library
+from .fp8 import BLOCK, _elsewhere
+
+PREFIX = "onnx_light_cpu_amd::RmsNorm"
+
+_lib = None
+_types = None  # torch dtype -> MNB_TYPE_* of include/mnb_fp8.h
+
+
+def _library():
+    """libmnb.so with the norm's signature."""
+    global _lib, _types
+    if _lib is None:
+        import torch
+        L = library()
+        vp, i64, i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
+        L.mnb_rms_norm.argtypes = [i64, i64, i32, vp, i64, vp, i64, vp, ctypes.c_float, i32, vp,
+                                   vp, vp, vp]
+        _types = {torch.float32: 1, torch.float16: 10, torch.bfloat16: 16}
+        _lib = L
+    return _lib
+
+
+def _rows(X, K):
+    """(X, values between its rows), a copy where its rows are not evenly apart."""
+    if X.is_contiguous():
+        return X, K
+    if X.dim() == 2 and X.stride(1) == 1 and X.stride(0) >= K:
+        return X, X.stride(0)
+    return X.contiguous(), K
+
+
+def _run(X, gamma, epsilon, residual, codes, stream):
+    import torch
+    L = _lib or _library()
+    dtype, device, shape = X.dtype, X.device, X.shape
+    x_type = _types.get(dtype)
+    if x_type is None or not X.is_cuda:
+        raise ValueError(f"{PREFIX}: X must be a float32, float16 or bfloat16 device tensor")
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"{PREFIX}: X must be [..., K] with K >= 1")
+    K = shape[-1]
+    if gamma.shape != (K,) or gamma.dtype != torch.float32 or gamma.device != device:
+        raise ValueError(f"{PREFIX}: gamma must be float32 [{K}] on {device}")
+    if residual is not None and (residual.shape != shape or residual.dtype != dtype
+                                 or residual.device != device):
+        raise ValueError(f"{PREFIX}: residual must be of X's shape, type and device")
+    if not 0.0 <= epsilon < float("inf"):
+        raise ValueError(f"{PREFIX}: epsilon must be finite and not negative, got {epsilon}")
+    elsewhere = _elsewhere(device, stream)
+    if elsewhere is not None:
+        with elsewhere:
+            return _run(X, gamma, epsilon, residual, codes, None)
+    X, ldx = _rows(X, K)
+    gamma = gamma.contiguous()
+    total, ldr = None, 0
+    if residual is not None:
+        residual, ldr = _rows(residual, K)
+        total = torch.empty(shape, dtype=dtype, device=device)
+    scales = None
+    if codes:
+        Y = torch.empty(shape, dtype=torch.float8_e4m3fn, device=device)
+        scales = torch.empty(shape[:-1] + ((K + BLOCK - 1) // BLOCK,), dtype=torch.float32,
+                             device=device)
+    else:
+        Y = torch.empty(shape, dtype=dtype, device=device)
+    status = L.mnb_rms_norm(X.numel() // K, K, x_type, X.data_ptr(), ldx,
+                            None if total is None else residual.data_ptr(), ldr, gamma.data_ptr(),
+                            epsilon, 17 if codes else x_type, Y.data_ptr(),
+                            scales.data_ptr() if codes else None,
+                            None if total is None else total.data_ptr(), _raw_stream(device))
+    if status != 0:
+        _check(status, "rms_norm")
+    return Y, scales, total
+
+
+def rms_norm(X, gamma, epsilon: float = 1e-5, residual=None, stream=None):
+    """Y [..., K] = h / sqrt(mean(h^2) + epsilon) * gamma of X's type, h = X + residual
+    rounded to it; X a float32, float16 or bfloat16 device tensor, residual the same
+    or None, gamma float32 [K]. With a residual: (Y, h). 2-D inputs may have any row
+    stride."""
+    Y, _, total = _run(X, gamma, epsilon, residual, False, stream)
+    return Y if total is None else (Y, total)
+
+
+def rms_norm_fp8(X, gamma, epsilon: float = 1e-5, residual=None, stream=None):
+    """(codes float8_e4m3fn [..., K], scales float32 [..., ceil(K / 128)]) of the fp32
+    norm that rms_norm rounds, as quantize_fp8 makes them; with a residual: (codes,
+    scales, h)."""
+    Y, scales, total = _run(X, gamma, epsilon, residual, True, stream)
+    return (Y, scales) if total is None else (Y, scales, total)

@@ -1,0 +1,173 @@
+"""The RMS norm on the GPU, against its definition in 64 bits.
+
+Tolerances, fixed before the first run. A thread adds up the squares of at most 8 n
+values, n the units that it holds (4, or K / 8192 of a longer row), then a tree of 6
+and a sum of 16 add to them: with half a unit (2^-24) lost in each of these and in
+each square, the sum is off by (8 n + 23) 2^-24 relative, its root by half of that,
+and division, root, reciprocal and two products add 2^-24 (2^-23 for the root
+and the reciprocal) each. With n <= 6 here that is below 2^-18 of y. The output's
+rounding is half a step (eps / 2) of the value more. A code stands for y within
+2^-4 of it or, below e4m3's normal values, half its least step, 2^-10, of the scale.
+"""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+FP32 = 2.0 ** -18
+
+
+def _problem(M, K, dtype, device, seed=0):
+    import torch
+    g = torch.Generator(device=device)
+    g.manual_seed(seed)
+    x, r = (torch.randn(M, K, device=device, generator=g)
+            * torch.exp(torch.randn(M, 1, device=device, generator=g)) for _ in range(2))
+    gamma = 1.0 + 0.3 * torch.randn(K, device=device, generator=g)
+    return x.to(dtype), r.to(dtype), gamma
+
+
+def _norm64(h, gamma, eps):
+    import torch
+    h = h.double()
+    return h / torch.sqrt((h * h).mean(dim=-1, keepdim=True) + eps) * gamma.double()
+
+
+def _check_codes(codes, scales, y):
+    """Codes and scales [M, nb] against y [M, K] in 64 bits."""
+    import torch
+    M, K = y.shape
+    nb = -(-K // 128)
+    pad = torch.nn.functional.pad(y, (0, nb * 128 - K)).reshape(M, nb, 128)
+    want = pad.abs().amax(dim=-1).clamp(min=2.0 ** -100) / 448.0
+    assert codes.dtype == torch.float8_e4m3fn and scales.dtype == torch.float32
+    assert ((scales.double() - want).abs() <= (FP32 + 2.0 ** -23) * want).all()
+    s = scales.double().repeat_interleave(128, dim=1)[:, :K]
+    got = codes.float().double() * s
+    tol = (2.0 ** -4 + 2 * FP32) * y.abs() + (2.0 ** -10 + 2 * FP32) * s
+    assert ((got - y).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("M,K", [(1, 1), (1, 8), (2, 7), (3, 127), (5, 128), (2, 129), (3, 1000),
+                                 (4, 1001), (1, 4096), (600, 512), (530, 2048), (520, 4104),
+                                 (7, 8192), (2, 16392), (3, 32768), (2, 32776), (1, 40001)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm(pkg, cuda, M, K, dtype, residual):
+    import torch
+    dtype = getattr(torch, dtype)
+    x, r, gamma = _problem(M, K, dtype, cuda, M + K)
+    r = r if residual else None
+    h = x if r is None else (x.float() + r.float()).to(dtype)
+    y = _norm64(h, gamma, 1e-5)
+    Y = pkg.rms_norm(x, gamma, 1e-5, residual=r)
+    C = pkg.rms_norm_fp8(x, gamma, 1e-5, residual=r)
+    if residual:
+        Y, H = Y
+        assert torch.equal(H, h) and torch.equal(C[2], h)
+    assert Y.dtype == dtype
+    info = torch.finfo(dtype)
+    tol = (info.eps / 2 + FP32) * y.abs() + info.smallest_normal * info.eps
+    assert ((Y.double() - y).abs() <= tol).all()
+    _check_codes(C[0], C[1], y)
+
+
+@pytest.mark.parametrize("K", [512, 513])
+def test_strided_rows(pkg, cuda, K):
+    """Rows of a wider tensor, on any side; the values beside them do not count."""
+    import torch
+    x, r, gamma = _problem(9, K, torch.bfloat16, cuda, 3)
+    wide, wide_r = (torch.full((9, K + 24), float("nan"), dtype=torch.bfloat16, device=cuda)
+                    for _ in range(2))
+    wide[:, 8:8 + K] = x
+    wide_r[:, 16:16 + K] = r
+    want = pkg.rms_norm_fp8(x, gamma, residual=r)
+    got = pkg.rms_norm_fp8(wide[:, 8:8 + K], gamma, residual=wide_r[:, 16:16 + K])
+    for a, b in zip(got, want):
+        assert torch.equal(a.float(), b.float())
+    shaped = pkg.rms_norm(x.reshape(3, 3, K).transpose(0, 1), gamma)
+    assert torch.equal(shaped, pkg.rms_norm(x, gamma).reshape(3, 3, K).transpose(0, 1))
+
+
+def test_special_rows(pkg, cuda):
+    """Zeros give zeros, an infinity or a NaN spoils its own row alone."""
+    import torch
+    x, _, gamma = _problem(6, 384, torch.float32, cuda, 4)
+    x[1] = 0.0
+    x[2, 5] = float("inf")
+    x[3, 200] = float("nan")
+    Y = pkg.rms_norm(x, gamma)
+    codes, scales = pkg.rms_norm_fp8(x, gamma)
+    assert (Y[1] == 0).all() and (codes[1].float() == 0).all()
+    # 1 / sqrt(inf) = 0: the infinity becomes NaN, its row's other values 0
+    assert Y[2, 5].isnan() and Y[3].isnan().all() and codes[3].float().isnan().all()
+    assert (scales[2] * codes[2].float().reshape(3, 128)[:, 5])[0].isnan()
+    good = [0, 4, 5]
+    y = _norm64(x[good], gamma, 1e-5)
+    assert ((Y[good].double() - y).abs() <= (2.0 ** -24 + FP32) * y.abs()).all()
+    _check_codes(codes[good], scales[good], y)
+
+
+def test_epsilon_and_empty(pkg, cuda):
+    import torch
+    x, r, gamma = _problem(2, 64, torch.float32, cuda, 5)
+    y = _norm64(x * 1e-3, gamma, 0.25)
+    Y = pkg.rms_norm(x * 1e-3, gamma, 0.25)
+    assert ((Y.double() - y).abs() <= 2 * FP32 * y.abs()).all()
+    assert pkg.rms_norm(x[:0], gamma).shape == (0, 64)
+    codes, scales, h = pkg.rms_norm_fp8(x[:0], gamma, residual=r[:0])
+    assert codes.shape == (0, 64) and scales.shape == (0, 1) and h.shape == (0, 64)
+
+
+def test_refusals(pkg, cuda):
+    import torch
+    x, r, gamma = _problem(2, 64, torch.float32, cuda, 6)
+    for args, kwargs, match in (((x, gamma.half()), {}, "gamma"), ((x, gamma[:63]), {}, "gamma"),
+                                ((x, gamma.cpu()), {}, "gamma"), ((x, gamma, -1.0), {}, "epsilon"),
+                                ((x, gamma, float("nan")), {}, "epsilon"),
+                                ((x, gamma), {"residual": r.half()}, "residual"),
+                                ((x, gamma), {"residual": r[:1]}, "residual"),
+                                ((x[:, :0], gamma), {}, "K >= 1")):
+        for f in (pkg.rms_norm, pkg.rms_norm_fp8):
+            with pytest.raises(ValueError, match=match):
+                f(*args, **kwargs)
+
+
+def test_stream_and_graph(pkg, cuda):
+    """On another stream, and captured: replays read the inputs of their time."""
+    import torch
+    x, r, gamma = _problem(33, 1024, torch.bfloat16, cuda, 7)
+    want = pkg.rms_norm_fp8(x, gamma, residual=r)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = pkg.rms_norm_fp8(x, gamma, residual=r, stream=side)
+    side.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a.float(), b.float())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = pkg.rms_norm_fp8(x, gamma, residual=r)
+    for k in range(3):
+        x.copy_(_problem(33, 1024, torch.bfloat16, cuda, 20 + k)[0])
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, pkg.rms_norm_fp8(x, gamma, residual=r)):
+            assert torch.equal(a.float(), b.float())
+
+
+def test_norm_of_a_projection(pkg, cuda):
+    """MatMulFp8.run_rmsnorm is the norm and the product, and returns the sum."""
+    import torch
+    g = torch.Generator(device=cuda)
+    g.manual_seed(8)
+    K, N = 512, 384
+    W = (torch.randn(N, K, device=cuda, generator=g) * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+    s = torch.rand(3, 4, device=cuda, generator=g) + 0.5
+    op = pkg.MatMulFp8(K, N).prepare_device(W, s)
+    x, r, gamma = _problem(17, K, torch.bfloat16, cuda, 9)
+    codes, scales, h = pkg.rms_norm_fp8(x, gamma, residual=r)
+    Y, H = op.run_rmsnorm(x, gamma, residual=r)
+    assert torch.equal(H, h)
+    assert torch.equal(Y, op(codes, scales=scales, out_dtype=torch.bfloat16))
+    Y = op.run_rmsnorm(x.reshape(17, 1, K), gamma, out_dtype=torch.float32)
+    codes, scales = pkg.rms_norm_fp8(x, gamma)
+    assert torch.equal(Y.reshape(17, N), op(codes, scales=scales))
