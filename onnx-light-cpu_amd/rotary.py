@@ -1,0 +1,186 @@
+"""Rotary positions with several axes (include/mnb_rotary.h).
+
+``Rotary`` turns the query and key heads of a QKV projection by their tokens'
+positions: one axis for text, three (time, row, column) for images and video.
+The frequencies are kept as turns in 64-bit fixed point, so that the angle of a
+far position is as exact as that of a near one. There is no CPU fallback.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from fractions import Fraction
+
+from . import _check, _raw_stream, library
+from .fp8 import _elsewhere
+
+PREFIX = "onnx_light_cpu_amd::Rotary"
+MAX_PAIRS, MAX_AXES = 256, 8
+_TWO_PI = 2 * Fraction("3.14159265358979323846264338327950288419716939937510582097494")
+
+_lib = None
+_types = None  # torch dtype -> MNB_TYPE_* of include/mnb_fp8.h
+_positions = None  # torch dtype -> MNB_TYPE_* of include/mnb_rotary.h
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [("head_dim", ctypes.c_int32), ("rotary_dim", ctypes.c_int32),
+                ("axes", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("turns", ctypes.POINTER(ctypes.c_uint64)), ("axis", ctypes.POINTER(ctypes.c_uint8))]
+
+
+class RotaryHeads(ctypes.Structure):
+    _fields_ = [("heads", ctypes.c_int32), ("x", ctypes.c_void_p),
+                ("x_token_stride", ctypes.c_int64), ("x_head_stride", ctypes.c_int64),
+                ("y", ctypes.c_void_p), ("y_token_stride", ctypes.c_int64),
+                ("y_head_stride", ctypes.c_int64)]
+
+
+def _library():
+    """libmnb.so with the rotation's signature."""
+    global _lib, _types, _positions
+    if _lib is None:
+        import torch
+        L = library()
+        vp, i64, i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
+        heads = ctypes.POINTER(RotaryHeads)
+        L.mnb_rotary.argtypes = [ctypes.POINTER(RotaryDesc), i64, i32, vp, i64, i32, heads, heads,
+                                 vp]
+        _types = {torch.float32: 1, torch.float16: 10, torch.bfloat16: 16}
+        _positions = {torch.int32: 6, torch.int64: 7}
+        _lib = L
+    return _lib
+
+
+class Rotary:
+    """Rotation of the first `rotary_dim` values (default: all) of heads of `head_dim`.
+
+    sections: how many of the rotary_dim / 2 frequencies each axis has, in their
+    order (default: one axis); axes: or each frequency's axis. inv_freq: the
+    frequencies in radians a position (default: base ** (-2 j / rotary_dim)).
+    Pair j is (x[j], x[j + rotary_dim / 2]), or (x[2j], x[2j + 1]) if interleaved.
+    Calls of one object on several streams or threads may overlap."""
+
+    op_type = "Rotary"
+
+    def __init__(self, head_dim: int, sections=None, base: float = 10000.0, rotary_dim=None,
+                 interleaved: bool = False, inv_freq=None, axes=None):
+        self.head_dim = int(head_dim)
+        self.rotary_dim = self.head_dim if rotary_dim is None else int(rotary_dim)
+        pairs = self.rotary_dim // 2
+        if (self.rotary_dim % 2 or not 1 <= pairs <= MAX_PAIRS
+                or not self.rotary_dim <= self.head_dim <= 4096):
+            raise ValueError(f"{PREFIX}: rotary_dim must be even, 2 .. {2 * MAX_PAIRS} and at most "
+                             f"head_dim (at most 4096), got {self.rotary_dim} of {self.head_dim}")
+        if sections is not None and axes is not None:
+            raise ValueError(f"{PREFIX}: sections or axes, not both")
+        if axes is None:
+            sections = (pairs,) if sections is None else tuple(int(n) for n in sections)
+            if min(sections, default=-1) < 0 or sum(sections) != pairs:
+                raise ValueError(f"{PREFIX}: sections must add up to rotary_dim / 2 = {pairs}, got "
+                                 f"{list(sections)}")
+            axes = [a for a, n in enumerate(sections) for _ in range(n)]
+            self.axes = len(sections)
+        else:
+            axes = [int(a) for a in axes]
+            if len(axes) != pairs or min(axes) < 0:
+                raise ValueError(f"{PREFIX}: axes must be one axis for each of the {pairs} "
+                                 "frequencies")
+            self.axes = max(axes) + 1
+        if self.axes > MAX_AXES:
+            raise ValueError(f"{PREFIX}: at most {MAX_AXES} axes, got {self.axes}")
+        if inv_freq is None:
+            if not 0.0 < base < math.inf:
+                raise ValueError(f"{PREFIX}: base must be positive, got {base}")
+            inv_freq = [math.exp(-2.0 * j / self.rotary_dim * math.log(base))
+                        for j in range(pairs)]
+        self.inv_freq = [float(f) for f in inv_freq]
+        if len(self.inv_freq) != pairs or not all(map(math.isfinite, self.inv_freq)):
+            raise ValueError(f"{PREFIX}: inv_freq must be {pairs} finite numbers")
+        # 2^64 f / (2 pi) modulo 2^64, from the double exactly
+        turns = [round(Fraction(f) / _TWO_PI * 2 ** 64) % 2 ** 64 for f in self.inv_freq]
+        self._turns = (ctypes.c_uint64 * pairs)(*turns)
+        self._axis = (ctypes.c_uint8 * pairs)(*axes)
+        self.desc = RotaryDesc(self.head_dim, self.rotary_dim, self.axes, int(bool(interleaved)),
+                               self._turns, self._axis)
+
+    def _heads(self, x, y):
+        """The C struct of x [T, H, D] and its result y, with addresses and strides."""
+        return RotaryHeads(x.shape[-2], x.data_ptr(), x.stride(0), x.stride(1), y.data_ptr(),
+                           y.stride(0), y.stride(1))
+
+    @staticmethod
+    def _flat(x):
+        """x [..., H, D] as [T, H, D] without a copy, or None."""
+        try:
+            y = x if x.dim() == 3 else x.view((math.prod(x.shape[:-2]),) + x.shape[-2:])
+        except RuntimeError:
+            return None
+        # axes of one value may have any stride: theirs counts for nothing
+        s = [d if n > 1 else y.shape[1] * y.shape[2] for n, d in zip(y.shape[:2], y.stride()[:2])]
+        if s[0] < y.shape[2] or s[1] < y.shape[2] or (y.shape[2] > 1 and y.stride(2) != 1):
+            return None
+        return y.as_strided(y.shape, (s[0], s[1], 1))
+
+    def __call__(self, Q, K, positions, out=None, stream=None):
+        """(Q', K') of Q [..., Hq, head_dim] and K [..., Hkv, head_dim] (float32, float16
+        or bfloat16 device tensors of one type, of any strides with whole heads; K may be
+        None: then Q' alone). positions: int32 or int64, [...] the tokens' axes, or [axes,
+        ...] where there are several. out: the results' tensors, which may be Q and K
+        themselves."""
+        import torch
+        L = _lib or _library()
+        device, dtype = Q.device, Q.dtype
+        x_type = _types.get(dtype)
+        if x_type is None or not Q.is_cuda:
+            raise ValueError(f"{PREFIX}: Q must be a float32, float16 or bfloat16 device tensor")
+        D, tokens = self.head_dim, Q.shape[:-2]
+        parts = [("Q", Q)] if K is None else [("Q", Q), ("K", K)]
+        for name, x in parts:
+            if x.dim() < 2 or x.shape[-1] != D or x.shape[:-2] != tokens:
+                raise ValueError(f"{PREFIX}: {name} must be [..., heads, {D}] of the same tokens, "
+                                 f"got {list(x.shape)}")
+            if x.dtype != dtype or x.device != device:
+                raise ValueError(f"{PREFIX}: {name} must be of Q's type and device")
+        want = tuple(tokens) if self.axes == 1 else (self.axes,) + tuple(tokens)
+        pos_type = _positions.get(positions.dtype)
+        if (pos_type is None or positions.device != device
+                or tuple(positions.shape) not in ((want, (1,) + want) if self.axes == 1 else (want,))):
+            raise ValueError(f"{PREFIX}: positions must be int32 or int64 {list(want)} on {device}, "
+                             f"got {positions.dtype} {list(positions.shape)}")
+        if out is not None:
+            out = (out,) if K is None and isinstance(out, torch.Tensor) else tuple(out)
+            if len(out) != len(parts):
+                raise ValueError(f"{PREFIX}: out must be {len(parts)} tensors")
+            for (name, x), y in zip(parts, out):
+                if (y.shape != x.shape or y.dtype != dtype or y.device != device
+                        or self._flat(y) is None):
+                    raise ValueError(f"{PREFIX}: out must have {name}'s shape, type and device, "
+                                     "and whole heads")
+        elsewhere = _elsewhere(device, stream)
+        if elsewhere is not None:
+            with elsewhere:
+                return self(Q, K, positions, out)
+        heads, results, keep = [], [], []
+        for i, (name, x) in enumerate(parts):
+            flat = self._flat(x)
+            if flat is None:
+                flat = self._flat(x.contiguous())
+            y = torch.empty(x.shape, dtype=dtype, device=device) if out is None else out[i]
+            flat_y = self._flat(y)
+            if flat_y.data_ptr() == flat.data_ptr() and flat_y.stride() != flat.stride():
+                flat = flat.contiguous()
+            keep.append(flat)
+            heads.append(self._heads(flat, flat_y))
+            results.append(y)
+        T = math.prod(tokens)
+        positions = positions.contiguous()
+        status = L.mnb_rotary(ctypes.byref(self.desc), T, pos_type, positions.data_ptr(), T, x_type,
+                              ctypes.byref(heads[0]),
+                              ctypes.byref(heads[1]) if K is not None else None,
+                              _raw_stream(device))
+        if status != 0:
+            _check(status, "rotary")
+        return results[0] if K is None else tuple(results)
+
+    run = __call__
