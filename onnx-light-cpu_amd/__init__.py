@@ -646,6 +646,7 @@ class NodeKernel:
 
 
 from .fp8 import MatMulFp8, quantize_fp8, release_workspaces  # noqa: E402,F401  (use the above)
+from .kv import Fp8KVCache  # noqa: E402,F401
 from .moe import MatMulNBitsMoE  # noqa: E402,F401
 from .norm import rms_norm, rms_norm_fp8  # noqa: E402,F401
 from .rotary import Rotary  # noqa: E402,F401

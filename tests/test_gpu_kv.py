@@ -1,0 +1,600 @@
+"""The 8-bit cache and its attention on the GPU, against definitions in 64 bits.
+
+Tolerances, fixed before the first run. What append writes is exact: scales are
+powers of two, so a code is the value's own rounding. For an output of attend, with
+p the exact weights, A = sum p |v| and S the largest |scale| sum |q k| of the
+row's keys:
+  - a score adds D exact products in fp32 (half a unit, 2^-24, lost in each addition
+    of magnitudes up to S), is scaled twice and shifted; a fp32 query is two fp16 terms,
+    2^-22 of each value; together (D + 16) 2^-24 S + 2^-22 S, and the exponent's
+    own rounding, 2^-24 of at most (S + 128) / ln 2, twice. A weight is off by that,
+    and by 2^-21 for the hardware's exponential;
+  - the weights of a row are divided by their sum, which has the same errors: twice;
+  - a weight is rounded to fp16, 2^-11 relative, for 16-bit queries, to 2^-22 for fp32,
+    and where it is below fp16's normal values to 2^-39 of the largest times its value
+    scale: n 2^-38 max|v| for n keys, max|v| by channel;
+  - sums of n weighted values in fp32: n 2^-24 A; joins and the division, 2^-20 A;
+  - the output's rounding, half a step (eps / 2) of the value.
+"""
+import itertools
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- definitions ------------------------------------------------------------
+
+def _e4m3(v):
+    """v (float64) rounded to the nearest e4m3 value, ties to even."""
+    import torch
+    e = torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -7))).clamp(min=-6.0)
+    step = torch.exp2(e - 3.0)
+    return torch.round(v / step) * step
+
+
+def _spans(tokens, lengths, starts):
+    """[(first row, rows, length)] of each sequence."""
+    B = len(lengths)
+    if starts is None:
+        n = tokens // B
+        return [(b * n, n, max(0, lengths[b])) for b in range(B)]
+    return [(starts[b], starts[b + 1] - starts[b], max(0, lengths[b])) for b in range(B)]
+
+
+def _append64(values, scales, X, table, spans, page):
+    """values [pages, H, page, D] (code values) and scales [pages, H], in 64 bits, in place."""
+    import torch
+    for b, (row, n, length) in enumerate(spans):
+        at = length - n
+        rows = X[row + max(0, -at):row + n].double()
+        at = max(0, at)
+        while len(rows):
+            p, slot = at // page, at % page
+            part, rows = rows[:page - slot], rows[page - slot:]
+            at += len(part)
+            if p >= len(table[b]) or not 0 <= table[b][p] < len(values):
+                continue
+            p = table[b][p]
+            finite = torch.where(part.isfinite(), part, 0.0)
+            amax = finite.abs().amax(dim=(0, 2))
+            e = torch.ceil(torch.log2(amax / 448.0)).clamp(min=-64.0)
+            scale = torch.exp2(e)
+            if slot:
+                scale = torch.maximum(scale, scales[p])
+                values[p] = torch.where(values[p].isnan(), values[p],
+                                        _e4m3(values[p] * (scales[p] / scale)[:, None, None]))
+            scales[p] = scale
+            q = _e4m3(finite / scale[:, None])
+            q = torch.where(part.isfinite(), q, math.nan)
+            values[p, :, slot:slot + len(part)] = q.transpose(0, 1)
+
+
+def _attend64(Q, k, v, table, spans, scale, window, dtype):
+    """(y, tolerance) in 64 bits; k, v [pages, H, page, D] values."""
+    import torch
+    T, Hq, D = Q.shape
+    H, page = k.shape[1:3]
+    eps = torch.finfo(dtype).eps
+    y, tol = torch.zeros(T, Hq, D, dtype=torch.float64), torch.zeros(T, Hq, D, dtype=torch.float64)
+    for b, (row, n, length) in enumerate(spans):
+        for i in range(n):
+            pos = length - n + i
+            keys = [t for t in range(max(0, pos - window + 1) if window else 0, pos + 1)
+                    if t // page < len(table[b]) and 0 <= table[b][t // page] < len(k)]
+            if not keys:
+                continue
+            at = torch.tensor([[table[b][t // page], t % page] for t in keys]).t()
+            for h in range(Hq):
+                kk, vv = k[at[0], h * H // Hq, at[1]], v[at[0], h * H // Hq, at[1]]
+                q = Q[row + i, h].double()
+                s = scale * (kk @ q)
+                p = torch.softmax(s, dim=0)
+                S = abs(scale) * (kk.abs() @ q.abs()).max().item()
+                A = p @ vv.abs()
+                m = len(keys)
+                e = 2 * ((D + 16) * 2.0 ** -24 * S + 2.0 ** -22 * S + 2.0 ** -22 * (S + 128)
+                         + 2.0 ** -21)
+                w = 2.0 ** -22 if dtype == torch.float32 else 2.0 ** -11
+                y[row + i, h] = p @ vv
+                tol[row + i, h] = ((e + w + m * 2.0 ** -24 + 2.0 ** -20) * A
+                                   + m * 2.0 ** -38 * vv.abs().amax(dim=0))
+    tol += eps / 2 * (y.abs() + tol) + torch.finfo(dtype).smallest_normal * eps
+    return y, tol
+
+
+# ---- problems ---------------------------------------------------------------
+
+def _rand(shape, seed, device, size=1.0):
+    import torch
+    g = torch.Generator(device=device)
+    g.manual_seed(seed)
+    return torch.randn(shape, device=device, generator=g) * size
+
+
+def _table(B, width, spare, seed):
+    """A table of different pages in no order, and how many pages there are."""
+    import torch
+    g = torch.Generator()
+    g.manual_seed(seed)
+    pages = B * width + spare
+    return torch.randperm(pages, generator=g)[:B * width].reshape(B, width).tolist(), pages
+
+
+def _cache(pkg, pages, H, page, D, device, seed, exponents=(-8, -3)):
+    """A cache of random values and what they are; some scales no powers of two."""
+    import torch
+    tensors = []
+    for n in range(2):
+        codes = (_rand((pages, H, page, D), seed + n, device, 100.0).clamp(-448, 448)
+                 .to(torch.float8_e4m3fn))
+        g = torch.Generator(device=device)
+        g.manual_seed(seed + 5 + n)
+        e = torch.randint(*exponents, (pages, H), device=device, generator=g)
+        tensors += [codes, torch.exp2(e.double()).float() * 1.25 ** (n * (seed % 2))]
+    return pkg.Fp8KVCache.from_tensors(tensors[0], tensors[2], tensors[1], tensors[3])
+
+
+def _values(codes, scales=None):
+    v = codes.cpu().float().double()
+    return v if scales is None else v * scales.cpu().double()[..., None, None]
+
+
+def _i32(x, device):
+    import torch
+    return None if x is None else torch.tensor(x, dtype=torch.int32, device=device)
+
+
+def _check_attend(pkg, cuda, Hq, H, D, page, lengths, news, dtype, window=0, seed=0, ragged=True,
+                  scale=None, spoil=None, q_size=1.0, exponents=(-8, -3), max_tokens=None):
+    """attend against the definition; unseen slots and pages hold NaN codes. spoil(table,
+    cache, Q): changes before the call."""
+    import torch
+    dtype = getattr(torch, dtype)
+    B, T = len(lengths), sum(news)
+    width = max(1, -(-max(lengths) // page))
+    table, pages = _table(B, width, 2, seed)
+    cache = _cache(pkg, pages, H, page, D, cuda, seed, exponents)
+    Q = _rand((T, Hq, D), seed + 9, cuda, q_size).to(dtype)
+    hold = torch.zeros(pages, page, dtype=torch.bool, device=cuda)
+    for b in range(B):
+        for t in range(lengths[b]):
+            hold[table[b][t // page], t % page] = True
+    for codes in (cache.k, cache.v):
+        codes.view(torch.uint8).masked_fill_(~hold[:, None, :, None], 0x7F)
+    if spoil is not None:
+        spoil(table, cache, Q)
+    starts = [sum(news[:b]) for b in range(B + 1)] if ragged else None
+    got = cache.attend(Q, _i32(table, cuda), _i32(lengths, cuda), starts=_i32(starts, cuda),
+                       scale=scale, window=window, max_tokens=max_tokens)
+    y, tol = _attend64(Q.cpu(), _values(cache.k, cache.k_scales), _values(cache.v, cache.v_scales),
+                       table, _spans(T, lengths, starts), D ** -0.5 if scale is None else scale,
+                       window, dtype)
+    assert got.dtype == dtype and got.shape == Q.shape
+    got = got.cpu().double()
+    nan = y.isnan()
+    assert torch.equal(got.isnan(), nan)
+    assert ((got - y).abs() <= tol)[~nan].all()
+    return got
+
+
+# ---- attention --------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("D", [16, 48, 64, 80, 128, 144, 256])
+@pytest.mark.parametrize("Hq,H", [(1, 1), (6, 2), (20, 1)])
+def test_one_token(pkg, cuda, D, Hq, H, dtype):
+    _check_attend(pkg, cuda, Hq, H, D, 32, [100, 7, 1, 33], [1] * 4, dtype, seed=D + Hq)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("length", [1, 15, 16, 17, 63, 64, 65, 127, 300])
+def test_lengths_and_pages(pkg, cuda, page, length):
+    _check_attend(pkg, cuda, 4, 2, 64, page, [length], [1], "bfloat16", seed=length, ragged=False)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("D", [64, 112, 256])
+@pytest.mark.parametrize("Hq,H,news", [(2, 2, [2, 17, 40]), (8, 2, [5, 1, 9]), (7, 1, [30, 3, 1])])
+def test_several_tokens(pkg, cuda, Hq, H, D, news, dtype):
+    _check_attend(pkg, cuda, Hq, H, D, 32, [70, 17, 130], news, dtype, seed=D + Hq)
+
+
+@pytest.mark.parametrize("window", [1, 2, 16, 63, 64, 65, 100, 1000, 1 << 40])
+@pytest.mark.parametrize("news", [[1, 1], [40, 90]])
+def test_windows(pkg, cuda, window, news):
+    _check_attend(pkg, cuda, 4, 2, 64, 32, [200, 90], news, "float16", window=window, seed=window % 91)
+
+
+@pytest.mark.parametrize("news,lengths", [([3, 1, 2], [3, 0, 1]), ([1, 1], [0, 0]), ([5, 70], [2, 0]),
+                                          ([0, 4, 0], [10, 4, 0]), ([1], [1])])
+@pytest.mark.parametrize("window", [0, 2])
+def test_empty_rows(pkg, cuda, news, lengths, window):
+    """Sequences of no tokens, of fewer tokens than rows, and of no rows."""
+    got = _check_attend(pkg, cuda, 4, 2, 64, 16, lengths, news, "float32", window=window, seed=3)
+    row = 0
+    for n, length in zip(news, lengths):
+        for i in range(n):
+            assert (got[row + i] == 0).all() == (length - n + i < 0)
+        row += n
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("news", [[1], [3], [150]])
+@pytest.mark.parametrize("D", [64, 128])
+def test_long(pkg, cuda, news, dtype, D):
+    """Long enough for the keys to be shared out over workgroups."""
+    _check_attend(pkg, cuda, 2, 1, D, 64, [2500], news, dtype, seed=D)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("q_size,scale", [(1e-4, 1e3), (300.0, 1e-3), (30.0, None), (1.0, 0.0),
+                                          (1.0, -0.2)])
+def test_sizes_of_queries(pkg, cuda, q_size, scale, dtype):
+    """Sharp and flat weights; queries that fp16 alone could not hold."""
+    _check_attend(pkg, cuda, 4, 2, 64, 32, [150, 3], [1, 3], dtype, seed=5, q_size=q_size,
+                  scale=scale)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_sizes_of_values(pkg, cuda, dtype):
+    """Pages of very different scales: their weights have to keep up."""
+    _check_attend(pkg, cuda, 2, 1, 64, 16, [130], [5], dtype, seed=6, exponents=(-30, 20),
+                  scale=1e-6)
+
+
+def test_huge_queries(pkg, cuda):
+    """fp32 and bf16 queries far beyond fp16's range, undone by the scale."""
+    for dtype in ("float32", "bfloat16"):
+        _check_attend(pkg, cuda, 2, 1, 64, 16, [40], [2], dtype, seed=7, q_size=1e20, scale=1e-21)
+
+
+# ---- what must leave no trace ---------------------------------------------------
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("window", [0, 20])
+@pytest.mark.parametrize("news", [[4], [40]])
+def test_nan_in_later_tokens(pkg, cuda, D, news, window):
+    """A NaN value reaches the rows that see it and no others, by channel; a NaN key
+    the whole of those rows."""
+    import torch
+
+    def spoil(table, cache, Q):
+        for which, t, d in (("v", 97, 3), ("v", 98, 5), ("k", 99, 1), ("v", 70, 7)):
+            code = getattr(cache, which).view(torch.uint8)
+            code[table[0][t // 32], 0, t % 32, d] = 0xFF
+
+    got = _check_attend(pkg, cuda, 4, 2, D, 32, [100], news, "bfloat16", window=window, seed=8,
+                        spoil=spoil)
+    first = got[news[0] - 4]  # position 96: sees none of the last three
+    assert first[:2, [3, 5]].isfinite().all() and first[2:].isfinite().all()
+    assert got[news[0] - 3, :2, 3].isnan().all() and got[news[0] - 1, :2].isnan().all()
+
+
+def test_infinite_queries(pkg, cuda):
+    """A row whose query is not finite is its own trouble."""
+    import torch
+
+    def spoil(table, cache, Q):
+        Q[1, 0, 3] = float("inf")
+        Q[2, 1, 0] = float("nan")
+
+    import torch as _t
+    dtype, lengths = _t.float32, [60]
+    clean = _check_attend(pkg, cuda, 2, 1, 64, 32, lengths, [4], "float32", seed=9)
+    table, pages = _table(1, 2, 2, 9)
+    cache = _cache(pkg, pages, 1, 32, 64, cuda, 9)
+    Q = _rand((4, 2, 64), 18, cuda).to(dtype)
+    spoil(table, cache, Q)
+    got = cache.attend(Q, _i32(table, cuda), _i32(lengths, cuda)).cpu().double()
+    assert got[2, 1].isnan().all() and not got[1, 0].isfinite().all()
+    good = torch.ones(4, 2, dtype=torch.bool)
+    good[1, 0] = good[2, 1] = False
+    assert torch.equal(got[good], clean[good])
+
+
+@pytest.mark.parametrize("news", [[1, 1], [30, 60]])
+def test_pages_outside_the_cache(pkg, cuda, news):
+    """Pages that the cache does not have are not seen: nothing is read there."""
+    import torch
+
+    def spoil(table, cache, Q):
+        table[0][1], table[0][2], table[1][0] = -1, cache.pages, -2 ** 31
+        table[1][1] = 2 ** 31 - 1
+
+    _check_attend(pkg, cuda, 4, 2, 64, 32, [100, 90], news, "float16", seed=10, spoil=spoil)
+    # every page of one sequence: a row of nothing
+    def gone(table, cache, Q):
+        table[0][:] = [cache.pages] * len(table[0])
+
+    got = _check_attend(pkg, cuda, 4, 2, 64, 32, [100, 90], news, "float32", seed=11, spoil=gone)
+    assert (got[:news[0]] == 0).all()
+    assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("lengths,starts", [
+    ([10 ** 9, -5], [0, 3, 6]), ([2 ** 31 - 1, -2 ** 31], [0, 3, 6]), ([20, 20], [0, 100, 200]),
+    ([20, 20], [-5, 2, -7]), ([20, 20], [6, 3, 0]), ([20, 20], [2 ** 31 - 1, -2 ** 31, 5])])
+def test_lengths_and_starts_out_of_range(pkg, cuda, lengths, starts):
+    """What the device memory holds may be anything: rows outside stay as they are."""
+    import torch
+    table, pages = _table(2, 2, 1, 12)
+    cache = _cache(pkg, pages, 1, 32, 64, cuda, 12)
+    Q = _rand((6, 2, 64), 13, cuda)
+    args = (_i32(table, cuda), _i32(lengths, cuda))
+    out = torch.full_like(Q, 7.0)
+    cache.attend(Q, *args, starts=_i32(starts, cuda), out=out)
+    cache.append(Q[:, :1], Q[:, 1:], *args, starts=_i32(starts, cuda))
+    cache.attend(Q, *args, out=out)
+    torch.cuda.synchronize()
+    if starts == [0, 100, 200]:
+        # one sequence of six rows
+        want = cache.attend(Q, args[0][:1], args[1][:1])
+        out = torch.full_like(Q, 7.0)
+        cache.attend(Q, *args, starts=_i32(starts, cuda), out=out)
+        assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("split", [False, True])
+def test_rows_of_no_sequence(pkg, cuda, split):
+    """Rows before the first, behind the last sequence: kept in out, 0 without it."""
+    import torch
+    width = 40 if split else 1
+    table, pages = _table(2, width, 0, 14)
+    cache = _cache(pkg, pages, 2, 64, 64, cuda, 14)
+    Q = _rand((10, 4, 64), 15, cuda).to(torch.bfloat16)
+    lengths = [64 * width, 64 * width - 3]
+    args = (_i32(table, cuda), _i32(lengths, cuda))
+    out = torch.full_like(Q, 7.0)
+    cache.attend(Q, *args, starts=_i32([2, 5, 7], cuda), out=out)
+    fresh = cache.attend(Q, *args, starts=_i32([2, 5, 7], cuda), max_tokens=3)
+    assert (out[:2] == 7).all() and (out[7:] == 7).all()
+    assert (fresh[:2] == 0).all() and (fresh[7:] == 0).all()
+    assert torch.equal(out[2:7], fresh[2:7])
+    alone = cache.attend(Q[2:5], args[0][:1], args[1][:1])
+    assert ((alone.float() - out[2:5].float()).abs() <= 2.0 ** -6 * alone.float().abs().amax()).all()
+
+
+# ---- append -----------------------------------------------------------------
+
+def _check_append(pkg, cuda, cache, state, X, table, lengths, starts, page):
+    """One append, on both sides; everything else stays as it was, bit for bit."""
+    import torch
+    spans = _spans(X[0].shape[0], lengths, starts)
+    cache.append(*X, _i32(table, cuda), _i32(lengths, cuda), starts=_i32(starts, cuda))
+    for (values, scales), x, codes, s in zip(state, X, (cache.k, cache.v),
+                                             (cache.k_scales, cache.v_scales)):
+        _append64(values, scales, x.cpu(), table, spans, page)
+        assert torch.equal(s.cpu().double(), scales)
+        got = _values(codes)
+        assert torch.equal(got.isnan(), values.isnan())
+        assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(values))
+
+
+def _state(cache):
+    return [[_values(cache.k), cache.k_scales.cpu().double()],
+            [_values(cache.v), cache.v_scales.cpu().double()]]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("H,D", [(1, 16), (3, 80), (2, 128), (2, 256)])
+def test_append(pkg, cuda, dtype, page, H, D):
+    """A prompt, tokens one by one with values that grow, and a chunk, of two
+    sequences: the scales and codes of every step."""
+    import torch
+    dtype = getattr(torch, dtype)
+    table, pages = _table(2, 4 * 64 // page + 2, 1, 20)
+    cache = _cache(pkg, pages, H, page, D, cuda, 20)
+    state = _state(cache)
+    lengths = [0, 0]
+    for step, news in enumerate([[20, 37], [1, 1], [1, 1], [1, 0], [70, 30], [1, 1]]):
+        lengths = [a + b for a, b in zip(lengths, news)]
+        starts = [0, news[0], sum(news)]
+        X = [_rand((sum(news), H, D), 30 + 2 * step + n, cuda, 4.0 ** step).to(dtype) for n in (0, 1)]
+        _check_append(pkg, cuda, cache, state, X, table, lengths, starts, page)
+
+
+def test_append_borders_of_scales(pkg, cuda):
+    """Magnitudes just below, at and above 448 times a power of two, zeros, fp32's
+    ends, ties of codes, infinities and NaN."""
+    import torch
+    tops = [448.0, math.nextafter(448.0, 500.0), 0.0, 2.0 ** -55, 448 * 2.0 ** -64, 2.0 ** -140, 1.75,
+            3.4e38, float("inf"), float("nan"), 1.0]
+    table, pages = _table(len(tops), 1, 0, 21)
+    cache = _cache(pkg, pages, 1, 16, 16, cuda, 21)
+    X = []
+    for n in range(2):
+        x = _rand((len(tops), 1, 16), 22 + n, cuda, 1e-3).abs()
+        for i, top in enumerate(tops):
+            top = torch.tensor(top, dtype=torch.float32).item()
+            x[i] = torch.nan_to_num(x[i] * (top if 0 < top < 1e38 else 1.0))
+            x[i, 0, 5] = top
+            # halves of a code's last place: 1.0625 and 1.1875 lie between two codes
+            x[i, 0, 6:8] = torch.tensor([1.0625, -1.1875], device=cuda) * (0.5 if top == 1.0 else 0)
+        X.append(x.contiguous())
+    _check_append(pkg, cuda, cache, _state(cache), X, table, [1] * len(tops), None, 16)
+
+
+def test_append_of_strided_and_batched_rows(pkg, cuda):
+    """Views of a QKV projection's rows, misaligned rows, [sequences, tokens, ...]."""
+    import torch
+    H, D, page, T = 2, 48, 16, 12
+    table, pages = _table(3, 2, 0, 23)
+    qkv = _rand((T, 8 + 2 * H, D), 24, cuda).to(torch.bfloat16)
+    k, v = qkv[:, 8:8 + H], qkv[:, 8 + H:]
+    odd = torch.zeros(T * H * D + 1, dtype=torch.bfloat16, device=cuda)[1:].view(T, H, D)
+    odd.copy_(k)
+    lengths = [4, 20, 3]
+    codes = []
+    for K, V in ((k.contiguous(), v.contiguous()), (k, v), (odd, v),
+                 (k.reshape(3, 4, H, D), v.reshape(3, 4, H, D)),
+                 (k.transpose(0, 1).contiguous().transpose(0, 1), v)):
+        cache = _cache(pkg, pages, H, page, D, cuda, 25)
+        cache.append(K, V, _i32(table, cuda), _i32(lengths, cuda))
+        codes.append([t.view(torch.uint8) for t in (cache.k, cache.v)]
+                     + [cache.k_scales, cache.v_scales])
+    for other in codes[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(codes[0], other))
+
+
+def test_append_outside_the_table_and_cache(pkg, cuda):
+    """Positions below 0 or past the table, pages outside: dropped; the rest is written."""
+    import torch
+    H, D, page = 1, 32, 16
+    table, pages = _table(3, 2, 1, 26)
+    table[1][0], table[2][1] = -1, pages
+    cache = _cache(pkg, pages, H, page, D, cuda, 26)
+    X = [_rand((60, H, D), 27 + n, cuda) for n in range(2)]
+    _check_append(pkg, cuda, cache, _state(cache), X, table, [10, 25, 45], None, page)
+
+
+def test_append_twice_is_append_once(pkg, cuda):
+    import torch
+    table, pages = _table(2, 3, 0, 28)
+    cache = _cache(pkg, pages, 2, 32, 64, cuda, 28)
+    X = [_rand((10, 2, 64), 29 + n, cuda, 100.0) for n in range(2)]
+    args = (*X, _i32(table, cuda), _i32([40, 66], cuda))
+    cache.append(*args)
+    once = [cache.k.clone(), cache.v.clone(), cache.k_scales.clone(), cache.v_scales.clone()]
+    cache.append(*args)
+    for a, b in zip(once, (cache.k, cache.v, cache.k_scales, cache.v_scales)):
+        assert torch.equal(a.float(), b.float())
+
+
+# ---- streams, graphs, sizes ---------------------------------------------------
+
+def test_offsets_past_32_bits(pkg, cuda):
+    """A cache of more than 4 GiB of codes: pages at its very end."""
+    import torch
+    pages, H, page, D = 40000, 4, 256, 128  # 5.2 GB of keys, as much of values
+    cache = pkg.Fp8KVCache(pages, H, D, page)
+    table = [[pages - 1, 3], [pages - 2, 32768]]
+    lengths = [300, 260]
+    X = [_rand((520, H, D), 40 + n, cuda) for n in range(2)]
+    starts = [0, 300, 520]
+    lengths[1] = 220
+    cache.append(*X, _i32(table, cuda), _i32(lengths, cuda), starts=_i32(starts, cuda))
+    small = pkg.Fp8KVCache(4, H, D, page)
+    small.append(*X, _i32([[0, 1], [2, 3]], cuda), _i32(lengths, cuda), starts=_i32(starts, cuda))
+    for p, r in ((pages - 1, 0), (3, 1), (pages - 2, 2)):
+        assert torch.equal(cache.k[p].float(), small.k[r].float())
+        assert torch.equal(cache.v_scales[p], small.v_scales[r])
+    assert (cache.k_scales > 0).sum().item() == 3 * H
+    Q = _rand((2, 8, D), 42, cuda)
+    got = cache.attend(Q, _i32(table, cuda), _i32(lengths, cuda))
+    want = small.attend(Q, _i32([[0, 1], [2, 3]], cuda), _i32(lengths, cuda))
+    assert torch.equal(got, want)
+    del cache
+    torch.cuda.empty_cache()
+
+
+def test_streams_and_threads(pkg, cuda):
+    """Calls that overlap, each with a workspace of its own."""
+    import threading
+
+    import torch
+    table, pages = _table(3, 30, 0, 43)
+    cache = _cache(pkg, pages, 2, 64, 64, cuda, 43)
+    args = (_i32(table, cuda), _i32([1900, 1500, 3], cuda))
+    Qs = [_rand((3, 4, 64), 44 + n, cuda) for n in range(4)]
+    want = [cache.attend(Q, *args) for Q in Qs]
+    torch.cuda.synchronize()
+    got = [[] for _ in Qs]
+
+    def work(n):
+        stream = torch.cuda.Stream()
+        for _ in range(20):
+            got[n].append(cache.attend(Qs[n], *args, stream=stream))
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for n in range(4):
+        assert len(got[n]) == 20 and all(torch.equal(y, want[n]) for y in got[n])
+
+
+def test_graphs(pkg, cuda):
+    """A captured append and attention replayed as the sequences grow; two graphs on
+    one cache do not share a workspace."""
+    import torch
+    H, Hq, D, page = 2, 8, 64, 64
+    table, pages = _table(2, 40, 0, 50)
+    cache, plain = (_cache(pkg, pages, H, page, D, cuda, 50) for _ in range(2))
+    table_, lengths = _i32(table, cuda), _i32([2400, 60], cuda)
+    K, V = (_rand((2, H, D), 51 + n, cuda).to(torch.bfloat16) for n in range(2))
+    Q = _rand((2, Hq, D), 53, cuda).to(torch.bfloat16)
+    R = _rand((2, Hq, D), 54, cuda).to(torch.bfloat16)
+    for c in (cache, plain):
+        c.append(K, V, table_, lengths)
+        c.attend(Q, table_, lengths)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for q in (Q, R):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            cache.append(K, V, table_, lengths)
+            outs.append(cache.attend(q, table_, lengths))
+        graphs.append(graph)
+    for step in range(4):
+        lengths += 1
+        for n, x in enumerate((K, V, Q, R)):
+            x.copy_(_rand(x.shape, 60 + 4 * step + n, cuda, 2.0 ** step))
+        plain.append(K, V, table_, lengths)
+        want = [plain.attend(q, table_, lengths) for q in (Q, R)]
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(cache.k.float(), plain.k.float())
+        assert torch.equal(cache.v_scales, plain.v_scales)
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_same_bits_again(pkg, cuda):
+    import torch
+    table, pages = _table(2, 32, 0, 70)
+    cache = _cache(pkg, pages, 2, 64, 128, cuda, 70)
+    for n in (1, 6, 200):
+        Q = _rand((2 * n, 8, 128), 71, cuda).to(torch.bfloat16)
+        args = (Q, _i32(table, cuda), _i32([2048, 1111], cuda))
+        want = cache.attend(*args)
+        assert all(torch.equal(cache.attend(*args), want) for _ in range(5))
+
+
+def test_shapes_of_queries(pkg, cuda):
+    """[sequences, tokens, heads, head_dim], strides, and rows of nothing."""
+    import torch
+    table, pages = _table(2, 3, 0, 72)
+    cache = _cache(pkg, pages, 2, 32, 64, cuda, 72)
+    args = (_i32(table, cuda), _i32([90, 40], cuda))
+    qkv = _rand((2, 3, 12, 64), 73, cuda).to(torch.float16)
+    Q = qkv[:, :, :8]
+    want = cache.attend(Q.contiguous().reshape(6, 8, 64), *args)
+    assert torch.equal(cache.attend(Q, *args).reshape(6, 8, 64), want)
+    swapped = Q.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(cache.attend(swapped, *args).reshape(6, 8, 64), want)
+    assert cache.attend(Q[:, :0], *args).shape == (2, 0, 8, 64)
+    none = cache.attend(Q[:0], args[0][:0], args[1][:0])
+    assert none.shape == (0, 3, 8, 64)
+    out = torch.empty(6, 8, 64, dtype=torch.float16, device=cuda)
+    assert cache.attend(want, *args, out=out) is out
+
+
+def test_values_come_back(pkg, cuda):
+    """A sequence of one token: its value, whatever the query. Its weight w is 2^14 but
+    for the rounding of a difference; an fp32 value is multiplied by two fp16 terms, w (1 +
+    2^-22) at most, divided by w as a product with a reciprocal (two roundings, 2^-24
+    each, and 2^-24 of the sum): within 2^-21. The one term of a 16-bit Y is off by as little."""
+    import torch
+    for dtype, D in itertools.product((torch.float32, torch.bfloat16), (64, 256)):
+        cache = pkg.Fp8KVCache(3, 2, D, 16)
+        v = (torch.randint(-7, 8, (1, 2, D), device=cuda) * 2.0).to(dtype)
+        table, lengths = _i32([[1]], cuda), _i32([1], cuda)
+        cache.append(v * 0.5, v, table, lengths)
+        y = cache.attend(_rand((1, 6, D), 80, cuda).to(dtype), table, lengths)
+        v = v.repeat_interleave(3, dim=1)
+        assert ((y - v).abs() <= (2.0 ** -21 if dtype == torch.float32 else 0.0) * v.abs()).all()
