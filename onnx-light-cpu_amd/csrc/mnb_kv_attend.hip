@@ -28,6 +28,7 @@ namespace {
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half4v __attribute__((ext_vector_type(4)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+typedef float floatx16v __attribute__((ext_vector_type(16)));
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 64;          // tokens of a step
@@ -60,10 +61,9 @@ __device__ __forceinline__ void Transpose4(const uint32_t (&in)[4], uint32_t (&o
   out[3] = __builtin_amdgcn_perm(CD, AB, 0x07060302);
 }
 
-// 0xFF in the place of each NaN code (0x7F or 0xFF).
-__device__ __forceinline__ uint32_t NanBytes(uint32_t w) {
-  const uint32_t top = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-  return (top >> 7) * 0xFFu;
+// 0x80 in the place of each NaN code (0x7F or 0xFF), 0 in the others'.
+__device__ __forceinline__ uint32_t NanTops(uint32_t w) {
+  return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
 }
 
 __device__ __forceinline__ float MaxGroups(float v) {
@@ -83,6 +83,58 @@ __device__ __forceinline__ float Log2Scale(float w) {
   int e;
   const float m = frexpf(w, &e);  // w = m 2^e, 0.5 <= m < 1
   return static_cast<float>(e - 1) + log2f(2.0f * m);
+}
+
+// The power of two by which a row of queries with this largest magnitude is
+// multiplied; fp16 rows are taken as they are.
+template <typename T>
+__device__ __forceinline__ int QueryShift(uint32_t top) {
+  return std::is_same<T, _Float16>::value ? 0 : RangeExponent(__uint_as_float(top), 14);
+}
+
+// What turns a dot product of such a row with key codes into log2 of a weight, but for
+// the codes' scale. Its sign is in the queries, so that the largest product is the largest
+// weight; it is never 0, so that an unseen token's -inf stays that.
+__device__ __forceinline__ float QueryScale(float scale, int shift) {
+  return ldexpf(fabsf(scale) * 1.44269504f, -shift);
+}
+
+__device__ __forceinline__ float ScoreScale(float query, float key) {
+  return fmaxf(query * key, 0x1p-126f);
+}
+
+template <int TERMS>
+__device__ __forceinline__ void SplitQuery(const float (&f)[8], int shift, float sign,
+                                           half8v (&q)[TERMS]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float v = ldexpf(f[e] * sign, shift);
+    const _Float16 hi = static_cast<_Float16>(v);
+    q[0][e] = hi;
+    if constexpr (TERMS == 2) q[1][e] = static_cast<_Float16>(v - static_cast<float>(hi));
+  }
+}
+
+// The weights 2^(scale s + add) of eight scores as fp16 terms, and their sum before that rounding:
+// beside a page of far larger values a page's weights may be lost for the values'
+// sum, but never for their own.
+template <int TERMS>
+__device__ __forceinline__ float Weights(const float (&s)[8], float scale, float add,
+                                         half8v (&p)[TERMS]) {
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float w = Exp2(fmaf(s[i], scale, add));
+    sum += w;
+    const _Float16 hi = static_cast<_Float16>(w);
+    p[0][i] = hi;
+    if constexpr (TERMS == 2) p[1][i] = static_cast<_Float16>(w - static_cast<float>(hi));
+  }
+  return sum;
+}
+
+__device__ __forceinline__ half8v ReadLds(uint32_t at) {
+  return *(const __attribute__((address_space(3))) half8v *)at;
 }
 
 // The tokens that a tile of rows looks at, and how they are shared out.
@@ -139,16 +191,15 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
   half8v q[MT][KS][2][kTerms];
   float cq[MT];   // what turns a dot product with key codes into log2 weights
   int pos[MT];
-  int64_t out[MT];  // row of Y, -1 for none
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     const int64_t r = row0 + 16 * t + col;
     const bool there = r < rows;
-    const int i = there ? static_cast<int>(r / group) : 0, g = static_cast<int>(r - static_cast<int64_t>(i) * group);
+    const int i = there ? static_cast<int>(r / group) : 0;
+    const int g = there ? static_cast<int>(r - static_cast<int64_t>(i) * group) : 0;
     pos[t] = there ? span.first + i : -1;
-    out[t] = there ? static_cast<int64_t>(span.row + i) * a.q_heads + h * group + g : -1;
     const T *x = static_cast<const T *>(a.q.x) + (span.row + i) * a.q.token_stride +
-                 (h * group + (there ? g : 0)) * a.q.head_stride;
+                 (h * group + g) * a.q.head_stride;
     float f[KS][2][8];
     uint32_t top = 0;
 #pragma unroll
@@ -159,25 +210,16 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
         Load8<T, true>(x + d, there ? c.dim - d : 0, f[j][half]);
         top = max(top, TopBits(f[j][half]));
       }
-    int shift = 0;
-    if constexpr (!std::is_same<T, _Float16>::value) {
-      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
-      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
-      shift = RangeExponent(__uint_as_float(top), 14);
-    }
-    cq[t] = ldexpf(a.scale * 1.44269504f, -shift);
+    top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
+    top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+    const int shift = QueryShift<T>(top);
+    cq[t] = QueryScale(a.scale, shift);
+    const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
     for (int j = 0; j < KS; ++j)
 #pragma unroll
       for (int half = 0; half < 2; ++half)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float v = ldexpf(f[j][half][e], shift);
-          const _Float16 hi = static_cast<_Float16>(v);
-          q[t][j][half][0][e] = hi;
-          if constexpr (kTerms == 2)
-            q[t][j][half][1][e] = static_cast<_Float16>(v - static_cast<float>(hi));
-        }
+        SplitQuery<kTerms>(f[j][half], shift, sign, q[t][j][half]);
   }
 
   floatx4v o[MT][VD];
@@ -225,7 +267,7 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
         for (int x = 0; x < VW; ++x) vw[sub][i][x] = w[x];
       }
       const float sk = c.scales[0][at], sv = c.scales[1][at];
-      ks[sub] = good ? sk : 0.0f;
+      ks[sub] = good ? sk : 1.0f;
       ev[sub] = good ? Log2Scale(sv) : -kInf;
       inv[sub] = good ? 1.0f / sv : 0.0f;
     }
@@ -254,22 +296,22 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
     float alpha[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      float top = -kInf;
+      float top = -kInf, scale[4];
 #pragma unroll
       for (int sub = 0; sub < 4; ++sub) {
-        const float scale = cq[t] * ks[sub];
+        scale[sub] = ScoreScale(cq[t], ks[sub]);
+        if (edge) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float y = fmaf(acc[t][sub][i], scale, ev[sub]);
-          if (edge) {
+          for (int i = 0; i < 4; ++i) {
             const int tok = t0 + 16 * sub + 4 * grp + i;
             const bool seen = tok <= pos[t] && tok < reach.end && ev[sub] != -kInf &&
                               (a.window == 0 || tok > pos[t] - a.window);
-            y = seen ? y : -kInf;
+            acc[t][sub][i] = seen ? acc[t][sub][i] : -kInf;
           }
-          acc[t][sub][i] = y;
-          top = fmaxf(top, y);
         }
+        const float most = fmaxf(fmaxf(acc[t][sub][0], acc[t][sub][1]),
+                                 fmaxf(acc[t][sub][2], acc[t][sub][3]));
+        top = fmaxf(top, fmaf(most, scale[sub], ev[sub]));
       }
       top = fmaxf(m[t], MaxGroups(top));
       const float use = top == -kInf ? 0.0f : top;
@@ -282,7 +324,7 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
         float part = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float w = Exp2(acc[t][sub][i] - (use - kShift));
+          const float w = Exp2(fmaf(acc[t][sub][i], scale[sub], ev[sub] - use + kShift));
           part += w;
           const _Float16 hi = static_cast<_Float16>(w);
           p[t][sub >> 1][0][4 * (sub & 1) + i] = hi;
@@ -324,7 +366,7 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
 #pragma unroll
             for (int y = 0; y < VW; ++y) {
               w[x][i][y] = seen ? w[x][i][y] : 0u;
-              nan |= NanBytes(w[x][i][y]);
+              nan |= NanTops(w[x][i][y]);
             }
           }
         if (__any(nan != 0)) {
@@ -347,7 +389,7 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
             for (int x = 0; x < 2; ++x) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const uint32_t bytes = NanBytes(w[x][i][y]);
+                const uint32_t bytes = (NanTops(w[x][i][y]) >> 7) * 0xFFu;
                 w[x][i][y] &= ~bytes;
                 flag[x][i] = bytes & 0x38383838u;  // 1.0
               }
@@ -446,55 +488,426 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
   }
 }
 
-// Joins the splits of a row: one wavefront per row, four values of it a lane.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void JoinKernel(Attend a, Work work) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
-  const Span span = SpanOf(a.batch, blockIdx.y, a.cache.page_shift);
-  if (i >= static_cast<int64_t>(span.count) * a.q_heads) return;
-  const int64_t row = static_cast<int64_t>(span.row) * a.q_heads + i;
-  const int64_t step = static_cast<int64_t>(a.batch.tokens) * a.q_heads;
-  const int d = 4 * (threadIdx.x & 63);
-  const bool there = d < a.cache.dim;
-  float top = -kInf;
-  for (int s = 0; s < work.splits; ++s) top = fmaxf(top, work.ml[s * step + row].x);
-  const float use = top == -kInf ? 0.0f : top;
-  float sum = 0.0f;
-  floatx4v v = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < work.splits; ++s) {
-    const float2 ml = work.ml[s * step + row];
-    if (ml.y == 0.0f) continue;
-    const float by = Exp2(ml.x - use);
-    sum = fmaf(ml.y, by, sum);
-    if (!there) continue;
-    const floatx4v part =
-        *reinterpret_cast<const floatx4v *>(work.parts + (s * step + row) * a.cache.dim + d);
+// Many rows: 32 queries to a wavefront, NW wavefronts to a workgroup, on tiles of 64
+// tokens that the workgroup widens to fp16 once, in LDS, for all of them. MFMAs of
+// 32 x 32 halve what a product reads of LDS; V is laid out transposed, in the order
+// of tokens that a lane's weights have. The next tile's codes are in registers
+// while a tile is multiplied, and are widened into the other half of LDS.
+// grid (heads, row tiles x splits, sequences): heads lie next to each other, so that a head's
+// workgroups share an XCD's cache where there are eight; late rows, which see the
+// most keys, come first.
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work, int row_tiles) {
+  constexpr int kTerms = Terms<T>();
+  constexpr int kThreadsT = 64 * NW;
+  constexpr int KP = DP / 16;                  // 16-code pieces of a key, steps of Q K^T
+  constexpr int DT = DP / 32;                  // tiles of O^T
+  constexpr int kUnits = 4 * DP;               // 16-byte pieces of a tile's keys, of its values
+  constexpr int kEach = (kUnits + kThreadsT - 1) / kThreadsT;
+  constexpr int kMask = DP / 8 < 16 ? DP / 8 - 1 : 15;
+  const Cache &c = a.cache;
+  const int s = blockIdx.z, h = blockIdx.x;
+  const int split = blockIdx.y % work.splits, tile = row_tiles - 1 - blockIdx.y / work.splits;
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Span span = SpanOf(a.batch, s, c.page_shift);
+  const int group = a.q_heads / c.heads;
+  const int64_t rows = static_cast<int64_t>(span.count) * group;
+  const int64_t row0 = static_cast<int64_t>(tile) * (32 * NW);
+  if (row0 >= rows) return;
+  const int64_t row1 = min(row0 + 32 * NW, rows) - 1;
+  const Reach reach = ReachOf(span, static_cast<int>(row0 / group), static_cast<int>(row1 / group),
+                              a.window);
+  const int tiles = reach.end > reach.begin ? (reach.end - reach.begin + kTile - 1) / kTile : 0;
+  const int each = (tiles + work.splits - 1) / work.splits;
+  const int tile0 = split * each, tile1 = min(tiles, tile0 + each);
+
+  // Two tiles of keys, [token][unit ^ token], and two of values, [d][unit ^ (d / 4) ^ d],
+  // units of eight values: neighbouring lanes' units lie in different banks.
+  constexpr uint32_t kHalf = kTile * DP * 2;
+  __shared__ __attribute__((aligned(16))) uint8_t tiles_of[4 * kHalf];
+  __shared__ float4 info[2][4];                 // 16 tokens' key scale, log2 and inverse of the
+                                                // values', whether they are seen at all
+  // NaN values are kept apart: a tile's tokens that have one, by d, and whether any has.
+  // Of four neighbouring tiles, for one is made while the last's readers may be reading.
+  __shared__ uint32_t nans[4][DP][2], any_nan[4];
+
+  // This wavefront's rows.
+  const int64_t r0 = row0 + 32 * wave, r = r0 + col;
+  const bool there = r < rows, busy = r0 < rows;
+  const int i0 = there ? static_cast<int>(r / group) : 0;
+  const int g = there ? static_cast<int>(r - static_cast<int64_t>(i0) * group) : 0;
+  const int pos = there ? span.first + i0 : -1;
+  const int pmin = span.first + static_cast<int>(r0 / group);
+  const int pmax = span.first + static_cast<int>(min(r0 + 31, rows - 1) / group);
+  half8v q[KP][kTerms];
+  float cq;
+  {
+    const T *x = static_cast<const T *>(a.q.x) + (span.row + i0) * a.q.token_stride +
+                 (h * group + g) * a.q.head_stride;
+    float f[KP][8];
+    uint32_t top = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = fmaf(part[e], by, v[e]);
+    for (int j = 0; j < KP; ++j) {
+      const int d = 16 * j + 8 * half;
+      Load8<T, true>(x + d, there ? c.dim - d : 0, f[j]);
+      top = max(top, TopBits(f[j]));
+    }
+    top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+    const int shift = QueryShift<T>(top);
+    cq = QueryScale(a.scale, shift);
+    const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
+#pragma unroll
+    for (int j = 0; j < KP; ++j) SplitQuery<kTerms>(f[j], shift, sign, q[j]);
+  }
+
+  // What a thread brings of each tile: 16 codes of a key, four of four tokens' values.
+  uint4v kw[kEach];
+  uint32_t vw[kEach][4];
+  uint32_t kid[kEach], vid[kEach], sid = 0;
+  float sk = 1.0f, sv = 1.0f;
+  const auto page_of = [&](int tok) {
+    return tok < reach.end ? PageOf(a.batch, s, tok >> c.page_shift) : ~0u;
+  };
+  const auto find = [&](int n) {  // the pages of tile n
+    const int t0 = reach.begin + kTile * n;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int u = tid + k * kThreadsT;
+      kid[k] = page_of(t0 + u / KP);
+      vid[k] = page_of(t0 + 4 * (u / (DP / 4)));
+    }
+    if (tid < 4) sid = page_of(t0 + 16 * tid);
+  };
+  uint32_t sid_now = ~0u;   // the page of sk and sv
+  bool vgood[kEach];
+  const auto load = [&](int n) {  // its codes and scales; pages outside the cache: of page 0
+    const int t0 = reach.begin + kTile * n, page = (1 << c.page_shift) - 1;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int u = tid + k * kThreadsT;
+      if (kUnits % kThreadsT != 0 && u >= kUnits) break;
+      const int kt = u / KP, kd = 16 * (u - kt * KP);
+      const int64_t kat = static_cast<int64_t>(kid[k] < c.pages ? kid[k] : 0) * c.heads + h;
+      kw[k] = *reinterpret_cast<const uint4v *>(
+          c.codes[0] + ((kat << c.page_shift) + ((t0 + kt) & page)) * c.dim + (kd < c.dim ? kd : 0));
+      const int vt = 4 * (u / (DP / 4)), vd = 4 * (u % (DP / 4));
+      vgood[k] = vid[k] < c.pages;
+      const int64_t vat = static_cast<int64_t>(vgood[k] ? vid[k] : 0) * c.heads + h;
+      const uint8_t *v = c.codes[1] + ((vat << c.page_shift) + ((t0 + vt) & page)) * c.dim +
+                         (vd < c.dim ? vd : 0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) vw[k][e] = *reinterpret_cast<const uint32_t *>(v + e * c.dim);
+    }
+    if (tid < 4) {
+      sid_now = sid;
+      const int64_t at = static_cast<int64_t>(sid < c.pages ? sid : 0) * c.heads + h;
+      sk = c.scales[0][at];
+      sv = c.scales[1][at];
+    }
+  };
+  const auto store = [&](int n) {  // into half n & 1 of LDS
+    const int t0 = reach.begin + kTile * n, to = n & 1;
+    const bool part_seen = t0 + kTile > reach.end || (a.window > 0 && t0 <= reach.pmin - a.window);
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int u = tid + k * kThreadsT;
+      if (kUnits % kThreadsT != 0 && u >= kUnits) break;
+      const int kt = u / KP, x = 2 * (u - kt * KP);
+      half8v *row = reinterpret_cast<half8v *>(tiles_of + to * kHalf) + kt * (DP / 8);
+      row[x ^ (kt & kMask)] = Widen8(kw[k][0], kw[k][1]);
+      row[(x + 1) ^ (kt & kMask)] = Widen8(kw[k][2], kw[k][3]);
+      // A weight of 0 does not undo a NaN: values of tokens that no row sees are cleared.
+      const int quad = u / (DP / 4), d = 4 * (u % (DP / 4));
+      if (part_seen || !vgood[k]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int tok = t0 + 4 * quad + e;
+          const bool seen = vgood[k] && tok < reach.end &&
+                            (a.window == 0 || tok > reach.pmin - a.window);
+          vw[k][e] = seen ? vw[k][e] : 0u;
+        }
+      }
+      const uint32_t nan = NanTops(vw[k][0]) | NanTops(vw[k][1]) | NanTops(vw[k][2]) |
+                           NanTops(vw[k][3]);
+      if (nan != 0) {
+        any_nan[n & 3] = 1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t tops = NanTops(vw[k][e]);
+          const int tok = 4 * quad + e;
+#pragma unroll 1
+          for (int x = 0; x < 4; ++x)
+            if ((tops >> (8 * x)) & 0x80u)
+              atomicOr(&nans[n & 3][d + x][tok >> 5], 1u << (tok & 31));
+          vw[k][e] &= ~((tops >> 7) * 0xFFu);
+        }
+      }
+      uint32_t turned[4];
+      Transpose4(vw[k], turned);
+      // Four tokens 4 quad .. of a group of 16 are the first or the second half of the
+      // eight that a lane with half = quad % 2 has weights of.
+      const int unit = 2 * (quad >> 2) + (quad & 1), part = (quad >> 1) & 1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const half2v lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(turned[e]), 1.0f,
+                                                                   false);
+        const half2v hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(turned[e]), 1.0f,
+                                                                   true);
+        const int swap = ((d >> 2) ^ (d + e)) & 7;
+        half4v *at = reinterpret_cast<half4v *>(tiles_of + (2 + to) * kHalf +
+                                                ((d + e) * (kTile / 8) + (unit ^ swap)) * 16);
+        at[part] = half4v{lo[0], lo[1], hi[0], hi[1]};
+      }
+    }
+    if (tid < 4) {
+      const bool good = sid_now < c.pages;
+      info[to][tid] = good ? make_float4(sk, Log2Scale(sv), 1.0f / sv, 1.0f)
+                           : make_float4(1.0f, -kInf, 0.0f, 0.0f);
+    }
+  };
+  const auto clear = [&](int n) {  // the record of tile n's NaN
+    for (int d = tid; d < DP; d += kThreadsT) nans[n & 3][d][0] = nans[n & 3][d][1] = 0;
+    if (tid == 0) any_nan[n & 3] = 0;
+  };
+
+  floatx16v o[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
+  float m = -kInf, l = 0.0f;
+
+  // Where this lane reads: the other tokens, values and half lie at constant distances.
+  const uint32_t base = static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)tiles_of));
+  uint32_t kat[KP], vat[4];
+#pragma unroll
+  for (int k = 0; k < KP; ++k)
+    kat[k] = base + (col * (DP / 8) + ((2 * k + half) ^ (col & kMask))) * 16;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    vat[j] = base + 2 * kHalf + (col * (kTile / 8) + ((2 * j + half) ^ (((col >> 2) ^ col) & 7))) * 16;
+
+  // One tile against this wavefront's rows; edge: some row does not see some token of it.
+  const auto step = [&](bool edge, int n) {
+    const int from = n & 1, t0 = reach.begin + kTile * n;
+    const uint32_t off = from ? kHalf : 0;
+    const auto seen = [&](int j) {  // token j of the tile, by this lane's row
+      const int tok = t0 + j;
+      return tok <= pos && tok < reach.end && info[from][j >> 4].w != 0.0f &&
+             (a.window == 0 || tok > pos - a.window);
+    };
+    floatx16v sc[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[j][e] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KP; ++k) {
+        const half8v kf = ReadLds(kat[k] + off + j * (32 * DP * 2));
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term)
+          sc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[k][term], sc[j], 0, 0, 0);
+      }
+    }
+    if (edge) {
+      __asm__ volatile("");  // a branch: as selects this would take as long as the rest
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          sc[j][e] = seen(32 * j + 8 * (e >> 2) + 4 * half + (e & 3)) ? sc[j][e] : -kInf;
+    }
+    float4 in[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) in[j] = info[from][j];
+    float top = -kInf, scale[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      scale[j] = ScoreScale(cq, in[j].x);
+      float most = -kInf;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, sc[j >> 1][8 * (j & 1) + e]);
+      top = fmaxf(top, fmaf(most, scale[j], in[j].y));
+    }
+    top = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
+    const float use = top == -kInf ? 0.0f : top;
+    const float alpha = Exp2(m - use);
+    const bool grew = top != m;
+    m = top;
+    half8v p[4][kTerms];
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = sc[j >> 1][8 * (j & 1) + e];
+      sum = fmaf(Weights<kTerms>(y, scale[j], in[j].y - use + kShift, p[j]), in[j].z, sum);
+    }
+    l = fmaf(l, alpha, sum);
+    if (__any(grew)) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= alpha;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const half8v v = ReadLds(vat[j] + off + d * (32 * kTile * 2));
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term)
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[j][term], o[d], 0, 0, 0);
+      }
+    if (any_nan[n & 3] != 0) {
+      uint32_t sees[2] = {~0u, ~0u};
+      if (edge) {
+        sees[0] = sees[1] = 0;
+        for (int j = 0; j < kTile; ++j) sees[j >> 5] |= seen(j) ? 1u << (j & 31) : 0u;
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t *w = nans[n & 3][32 * d + 8 * (e >> 2) + 4 * half + (e & 3)];
+          if (((w[0] & sees[0]) | (w[1] & sees[1])) != 0) o[d][e] = __builtin_nanf("");
+        }
+    }
+  };
+
+  if (tile0 < tile1) {
+    for (int n = 0; n < 4; ++n) clear(n);
+    __syncthreads();
+    find(tile0);
+    load(tile0);
+    find(tile0 + 1);
+    store(tile0);
+    load(tile0 + 1);
+    find(tile0 + 2);
+    __syncthreads();
+  }
+  for (int n = tile0; n < tile1; ++n) {
+    const int t0 = reach.begin + kTile * n;
+    if (n + 1 < tile1) {
+      store(n + 1);
+      load(n + 2);
+      find(n + 3);
+    }
+    clear(n + 3);
+    if (busy && t0 <= pmax && (a.window == 0 || t0 + kTile - 1 > pmin - a.window)) {
+      const bool edge = t0 + kTile - 1 > pmin || t0 + kTile > reach.end ||
+                        (a.window > 0 && t0 <= pmax - a.window) ||
+                        info[n & 1][0].w * info[n & 1][1].w * info[n & 1][2].w *
+                                info[n & 1][3].w == 0.0f;
+      step(__builtin_amdgcn_readfirstlane(edge), n);
+    }
+    __syncthreads();
   }
   if (!there) return;
-  const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
-  T *y = static_cast<T *>(a.y) + row * a.cache.dim + d;
+  l += __shfl_xor(l, 32);
+  const int64_t at = static_cast<int64_t>(span.row + i0) * a.q_heads + h * group + g;
+  const float by = work.splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+  const int64_t part = static_cast<int64_t>(split) * a.batch.tokens * a.q_heads + at;
+  if (work.splits > 1 && half == 0) work.ml[part] = make_float2(m, l);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(v[e] * by);
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int d0 = 32 * d + 8 * (e >> 2) + 4 * half;
+      if (d0 >= c.dim) continue;
+      if (work.splits > 1) {
+        *reinterpret_cast<floatx4v *>(work.parts + part * c.dim + d0) =
+            floatx4v{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+      } else {
+        typedef T Vec __attribute__((ext_vector_type(4)));
+        const Vec y = {static_cast<T>(o[d][e] * by), static_cast<T>(o[d][e + 1] * by),
+                       static_cast<T>(o[d][e + 2] * by), static_cast<T>(o[d][e + 3] * by)};
+        *reinterpret_cast<Vec *>(static_cast<T *>(a.y) + at * c.dim + d0) = y;
+      }
+    }
+}
+
+// Joins the splits of a row. PER threads to a row, four values of it each; where one
+// row has more threads than its width, they take every n-th split. A workgroup
+// per row (PER 256) hides the reads of many splits, a wavefront (PER 64) is enough for few.
+template <typename T, int PER>
+__global__ __launch_bounds__(kThreads) void JoinKernel(Attend a, Work work) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * (kThreads / PER) + threadIdx.x / PER;
+  const Span span = SpanOf(a.batch, blockIdx.y, a.cache.page_shift);
+  if (i >= static_cast<int64_t>(span.count) * a.q_heads) return;  // PER 256: all threads
+  const int64_t row = static_cast<int64_t>(span.row) * a.q_heads + i;
+  const int64_t step = static_cast<int64_t>(a.batch.tokens) * a.q_heads;
+  const int dim = a.cache.dim, lane = threadIdx.x & 63;
+  const int wide = dim <= 64 ? 16 : dim <= 128 ? 32 : 64;  // threads that hold a row
+  const int t = threadIdx.x % PER, first = t / wide, stride = PER / wide, d = 4 * (t % wide);
+  // Every wavefront finds the maximum: a lane per split, 64 at most.
+  float2 ml = lane < work.splits ? work.ml[lane * step + row] : make_float2(-kInf, 0.0f);
+  float top = ml.x;
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+  const float use = top == -kInf ? 0.0f : top;
+  const float by = ml.y == 0.0f ? 0.0f : Exp2(ml.x - use);
+  float sum = ml.y * by;
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
+  floatx4v v = {0.0f, 0.0f, 0.0f, 0.0f};
+  const float *part = work.parts + row * dim + (d < dim ? d : 0);
+  for (int s0 = 0; s0 < work.splits; s0 += stride) {
+    const int s = s0 + first;
+    const float w = __shfl(by, s & 63);
+    if (s < work.splits && w != 0.0f) {  // else it saw nothing, and wrote nothing
+      const floatx4v p = *reinterpret_cast<const floatx4v *>(part + s * step * dim);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = fmaf(p[e], w, v[e]);
+    }
+  }
+  for (int off = wide; off < 64; off *= 2)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], off);
+  if constexpr (PER > 64) {
+    __shared__ floatx4v sums[PER / 64][64];
+    sums[threadIdx.x >> 6][lane] = v;
+    __syncthreads();
+    if (threadIdx.x >= wide) return;
+#pragma unroll
+    for (int w = 1; w < PER / 64; ++w) v += sums[w][lane];
+  } else if (lane >= wide) {
+    return;
+  }
+  if (d >= dim) return;
+  const float over = sum == 0.0f ? 0.0f : 1.0f / sum;
+  T *y = static_cast<T *>(a.y) + row * dim + d;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(v[e] * over);
 }
 
 // How a call is launched.
 struct Plan {
-  int mt, row_tiles, splits;
+  int mt;      // AttendSplitKernel's tiles of 16 rows, or
+  int waves;   // AttendTileKernel's wavefronts; 0: the other
+  int row_tiles, splits;
 };
 
 Plan PlanOf(const Cache &c, const Batch &b, int32_t q_heads, int32_t x_type) {
-  Plan p;
+  Plan p{1, 0, 1, 1};
   const int64_t rows = static_cast<int64_t>(b.max_tokens) * (q_heads / c.heads);
-  // Two tiles of fp32 queries 256 wide leave no registers for the keys.
-  p.mt = rows > 16 && (c.dim <= 128 || x_type != MNB_TYPE_FLOAT) ? 2 : 1;
-  p.row_tiles = static_cast<int>(CeilDiv(rows, 16 * p.mt));
-  // Workgroups for three on each CU, each with a tile for every wavefront at least.
+  const bool fp32 = x_type == MNB_TYPE_FLOAT;
+  int64_t per = 16, least = kWaves, goal = 3 * 256;
+  if (rows > 32 && c.dim <= 128) {
+    p.waves = rows > 128 && !fp32 ? 8 : 4;
+    per = 32 * p.waves;
+    goal = 256 * (8 / p.waves);
+    least = 8;
+  } else if (rows > 16 && (c.dim <= 128 || !fp32)) {
+    // Two tiles of fp32 queries 256 wide leave no registers for the keys.
+    p.mt = 2;
+    per = 32;
+  }
+  p.row_tiles = static_cast<int>(CeilDiv(rows, per));
   const int64_t groups = static_cast<int64_t>(b.sequences) * c.heads * p.row_tiles;
   const int64_t tiles = CeilDiv(static_cast<int64_t>(b.width) << c.page_shift, kTile);
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(64, tiles / kWaves));
-  p.splits = static_cast<int>(std::min(most, std::max<int64_t>(1, 3 * 256 / groups)));
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(64, tiles / least));
+  p.splits = static_cast<int>(std::min(most, std::max<int64_t>(1, goal / groups)));
   return p;
 }
 
@@ -506,8 +919,20 @@ hipError_t Split(const Attend &a, const Work &w, const Plan &p, hipStream_t s) {
   return hipGetLastError();
 }
 
+template <typename T, int DP, int NW>
+hipError_t Tile(const Attend &a, const Work &w, const Plan &p, hipStream_t s) {
+  const dim3 grid(a.cache.heads, static_cast<unsigned>(p.row_tiles * p.splits), a.batch.sequences);
+  hipLaunchKernelGGL((AttendTileKernel<T, DP, NW>), grid, dim3(64 * NW), 0, s, a, w, p.row_tiles);
+  return hipGetLastError();
+}
+
 template <typename T, int DP>
 hipError_t SplitDim(const Attend &a, const Work &w, const Plan &p, hipStream_t s) {
+  if constexpr (DP <= 128) {
+    if constexpr (Terms<T>() == 1)
+      if (p.waves == 8) return Tile<T, DP, 8>(a, w, p, s);
+    if (p.waves == 4) return Tile<T, DP, 4>(a, w, p, s);
+  }
   if constexpr (DP <= 128 || Terms<T>() == 1)
     if (p.mt == 2) return Split<T, DP, 2>(a, w, p, s);
   return Split<T, DP, 1>(a, w, p, s);
@@ -530,10 +955,14 @@ hipError_t LaunchT(const Attend &a, int32_t x_type, void *work, hipStream_t s) {
                  : a.cache.dim <= 128 ? SplitDim<T, 128>(a, w, p, s)
                                       : SplitDim<T, 256>(a, w, p, s);
   if (e != hipSuccess || p.splits == 1) return e;
-  const dim3 grid(static_cast<unsigned>(
-                      CeilDiv(static_cast<int64_t>(a.batch.max_tokens) * a.q_heads, kWaves)),
-                  a.batch.sequences);
-  hipLaunchKernelGGL((JoinKernel<T>), grid, dim3(kThreads), 0, s, a, w);
+  const int64_t rows = static_cast<int64_t>(a.batch.max_tokens) * a.q_heads;
+  if (p.splits > 8) {
+    const dim3 grid(static_cast<unsigned>(rows), a.batch.sequences);
+    hipLaunchKernelGGL((JoinKernel<T, kThreads>), grid, dim3(kThreads), 0, s, a, w);
+  } else {
+    const dim3 grid(static_cast<unsigned>(CeilDiv(rows, kWaves)), a.batch.sequences);
+    hipLaunchKernelGGL((JoinKernel<T, 64>), grid, dim3(kThreads), 0, s, a, w);
+  }
   return hipGetLastError();
 }
 
