@@ -66,10 +66,23 @@ __device__ __forceinline__ uint32_t NanTops(uint32_t w) {
   return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
 }
 
-__device__ __forceinline__ float MaxGroups(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
+// The larger of lanes l and l ^ 32, l and l ^ 16, without a round trip through LDS: of a
+// register swapped with itself one result has the lower lanes' values everywhere, the other
+// the upper ones'.
+__device__ __forceinline__ float MaxHalves(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
+
+__device__ __forceinline__ float MaxRows(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// The largest of the lanes with the same column of a 16 x 16 result.
+__device__ __forceinline__ float MaxGroups(float v) { return MaxHalves(MaxRows(v)); }
 
 __device__ __forceinline__ float SumGroups(float v) {
   v += __shfl_xor(v, 16);
@@ -133,8 +146,19 @@ __device__ __forceinline__ float Weights(const float (&s)[8], float scale, float
   return sum;
 }
 
+// The same number, of which the compiler knows nothing.
+__device__ __forceinline__ uint32_t Opaque(uint32_t v) {
+  __asm__ volatile("" : "+v"(v));
+  return v;
+}
+
 __device__ __forceinline__ half8v ReadLds(uint32_t at) {
   return *(const __attribute__((address_space(3))) half8v *)at;
+}
+
+template <typename V>
+__device__ __forceinline__ void WriteLds(uint32_t at, V v) {
+  *(__attribute__((address_space(3))) V *)at = v;
 }
 
 // The tokens that a tile of rows looks at, and how they are shared out.
@@ -525,21 +549,25 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
   // Two tiles of keys, [token][unit ^ token], and two of values, [d][unit ^ (d / 4) ^ d],
   // units of eight values: neighbouring lanes' units lie in different banks.
   constexpr uint32_t kHalf = kTile * DP * 2;
-  __shared__ __attribute__((aligned(16))) uint8_t tiles_of[4 * kHalf];
-  __shared__ float4 info[2][4];                 // 16 tokens' key scale, log2 and inverse of the
-                                                // values', whether they are seen at all
+  __shared__ __attribute__((aligned(256))) uint8_t tiles_of[4 * kHalf];
+  // Of 16 tokens: the keys' scale, log2 and inverse of the values'.
+  __shared__ float4 info[4][4];
   // NaN values are kept apart: a tile's tokens that have one, by d, and whether any has.
-  // Of four neighbouring tiles, for one is made while the last's readers may be reading.
+  // Four tiles' records, for one is made while readers of others are behind.
   __shared__ uint32_t nans[4][DP][2], any_nan[4];
+
+  const uint32_t base = static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)tiles_of));
 
   // This wavefront's rows.
   const int64_t r0 = row0 + 32 * wave, r = r0 + col;
-  const bool there = r < rows, busy = r0 < rows;
+  const bool there = r < rows;
   const int i0 = there ? static_cast<int>(r / group) : 0;
   const int g = there ? static_cast<int>(r - static_cast<int64_t>(i0) * group) : 0;
   const int pos = there ? span.first + i0 : -1;
-  const int pmin = span.first + static_cast<int>(r0 / group);
-  const int pmax = span.first + static_cast<int>(min(r0 + 31, rows - 1) / group);
+  const int pmin = __builtin_amdgcn_readfirstlane(span.first + static_cast<int>(r0 / group));
+  const int pmax = __builtin_amdgcn_readfirstlane(
+      span.first + static_cast<int>(min(r0 + 31, rows - 1) / group));
   half8v q[KP][kTerms];
   float cq;
   {
@@ -561,69 +589,104 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
     for (int j = 0; j < KP; ++j) SplitQuery<kTerms>(f[j], shift, sign, q[j]);
   }
 
-  // What a thread brings of each tile: 16 codes of a key, four of four tokens' values.
+  // What a thread brings of each tile: 16 codes of a key, four of four tokens' values. All
+  // that a wavefront brings at a time is of one group of 16 tokens, and so of one page.
+  // Values are brought a tile later than keys, when their weights are made.
   uint4v kw[kEach];
   uint32_t vw[kEach][4];
-  uint32_t kid[kEach], vid[kEach], sid = 0;
-  float sk = 1.0f, sv = 1.0f;
-  const auto page_of = [&](int tok) {
-    return tok < reach.end ? PageOf(a.batch, s, tok >> c.page_shift) : ~0u;
-  };
+  uint32_t id[kEach];                           // page of the group's next keys; ~0: none
+  uint32_t kid[kEach], vid[kEach];              // of the keys and the values that are held
+  int64_t kfrom[kEach], vfrom[kEach];           // where their group begins
+  float sk[kEach], sv[kEach];                   // the keys' page's scales
+  int grp[kEach];
+  uint32_t koff[kEach], voff[kEach], kto[kEach], vto[kEach];
+  const uint32_t dim = c.dim, slots = (1u << c.page_shift) - 1;
+  const int64_t head = static_cast<int64_t>(h << c.page_shift) * dim;
+  const int32_t *table = a.batch.table + static_cast<int64_t>(s) * a.batch.width;
+  // The index of a vector load whose address is the same in all lanes: a scalar load
+  // would be waited for with the next read of LDS.
+  const uint32_t lane0 = Opaque(0);
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const uint32_t u = tid + k * kThreadsT;
+    grp[k] = __builtin_amdgcn_readfirstlane(u / DP);
+    kid[k] = vid[k] = ~0u;
+    kfrom[k] = vfrom[k] = 0;
+    const uint32_t kt = u / KP, kd = 16 * (u % KP), quad = u / (DP / 4), vd = 4 * (u % (DP / 4));
+    koff[k] = kt % 16 * dim + (kd < dim ? kd : 0);
+    voff[k] = 4 * (quad % 4) * dim + (vd < dim ? vd : 0);
+    // The key's second unit is its first ^ 1. Four tokens 4 quad .. of a group of 16 are the
+    // first or the second half of the eight that a lane with half = quad % 2 has
+    // weights of; value vd + e goes e rows further, to unit ^ e.
+    kto[k] = (kt * (DP / 8) + (2 * (u % KP) ^ (kt & kMask))) * 16;
+    vto[k] = 2 * kHalf + 8 * (quad / 2 % 2) +
+             16 * (vd * (kTile / 8) + ((2 * (quad / 4) + quad % 2) ^ (((vd >> 2) ^ vd) & 7)));
+  }
   const auto find = [&](int n) {  // the pages of tile n
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int tok = reach.begin + kTile * n + 16 * grp[k];
+      const int32_t *at = table + (min(tok, reach.end - 1) >> c.page_shift);
+      id[k] = tok < reach.end ? at[lane0] : ~0u;
+    }
+  };
+  const auto load_keys = [&](int n) {  // and their scales; of page 0 where there are none
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      vid[k] = kid[k];
+      vfrom[k] = kfrom[k];
+      kid[k] = __builtin_amdgcn_readfirstlane(id[k]);
+      const uint32_t page = kid[k] < c.pages ? kid[k] : 0;
+      const uint32_t slot = (reach.begin + kTile * n + 16 * grp[k]) & slots;
+      kfrom[k] = static_cast<int64_t>(page) * (static_cast<uint32_t>(c.heads << c.page_shift) * dim) +
+                 head + slot * dim;
+      if (kUnits % kThreadsT != 0 && grp[k] >= 4) break;
+      kw[k] = *reinterpret_cast<const uint4v *>(c.codes[0] + kfrom[k] + koff[k]);
+      if ((64 * wave + k * kThreadsT) % DP == 0) {
+        const int64_t at = static_cast<int64_t>(page) * c.heads + h;
+        sk[k] = c.scales[0][at + lane0];
+        sv[k] = c.scales[1][at + lane0];
+      }
+    }
+  };
+  const auto load_values = [&]() {
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      if (kUnits % kThreadsT != 0 && grp[k] >= 4) break;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        vw[k][e] = *reinterpret_cast<const uint32_t *>(c.codes[1] + vfrom[k] + (voff[k] + e * dim));
+    }
+  };
+  const auto store_keys = [&](int n) {  // into half n & 1 of the keys' LDS
+    const uint32_t off = base + (n & 1 ? kHalf : 0);
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      if (kUnits % kThreadsT != 0 && grp[k] >= 4) break;
+      const bool good = kid[k] < c.pages;
+      if (!good) kw[k] = uint4v{0, 0, 0, 0};  // no NaN: the info's -inf does the rest
+      WriteLds(off + kto[k], Widen8(kw[k][0], kw[k][1]));
+      WriteLds((off + kto[k]) ^ 16, Widen8(kw[k][2], kw[k][3]));
+      if ((64 * wave + k * kThreadsT) % DP == 0 && lane == 0)
+        info[n & 3][grp[k]] = good ? make_float4(sk[k], Log2Scale(sv[k]), 1.0f / sv[k], 0.0f)
+                                   : make_float4(1.0f, -kInf, 0.0f, 0.0f);
+    }
+  };
+  const auto store_values = [&](int n) {
     const int t0 = reach.begin + kTile * n;
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-      const int u = tid + k * kThreadsT;
-      kid[k] = page_of(t0 + u / KP);
-      vid[k] = page_of(t0 + 4 * (u / (DP / 4)));
-    }
-    if (tid < 4) sid = page_of(t0 + 16 * tid);
-  };
-  uint32_t sid_now = ~0u;   // the page of sk and sv
-  bool vgood[kEach];
-  const auto load = [&](int n) {  // its codes and scales; pages outside the cache: of page 0
-    const int t0 = reach.begin + kTile * n, page = (1 << c.page_shift) - 1;
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-      const int u = tid + k * kThreadsT;
-      if (kUnits % kThreadsT != 0 && u >= kUnits) break;
-      const int kt = u / KP, kd = 16 * (u - kt * KP);
-      const int64_t kat = static_cast<int64_t>(kid[k] < c.pages ? kid[k] : 0) * c.heads + h;
-      kw[k] = *reinterpret_cast<const uint4v *>(
-          c.codes[0] + ((kat << c.page_shift) + ((t0 + kt) & page)) * c.dim + (kd < c.dim ? kd : 0));
-      const int vt = 4 * (u / (DP / 4)), vd = 4 * (u % (DP / 4));
-      vgood[k] = vid[k] < c.pages;
-      const int64_t vat = static_cast<int64_t>(vgood[k] ? vid[k] : 0) * c.heads + h;
-      const uint8_t *v = c.codes[1] + ((vat << c.page_shift) + ((t0 + vt) & page)) * c.dim +
-                         (vd < c.dim ? vd : 0);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) vw[k][e] = *reinterpret_cast<const uint32_t *>(v + e * c.dim);
-    }
-    if (tid < 4) {
-      sid_now = sid;
-      const int64_t at = static_cast<int64_t>(sid < c.pages ? sid : 0) * c.heads + h;
-      sk = c.scales[0][at];
-      sv = c.scales[1][at];
-    }
-  };
-  const auto store = [&](int n) {  // into half n & 1 of LDS
-    const int t0 = reach.begin + kTile * n, to = n & 1;
+    const uint32_t off = base + (n & 1 ? kHalf : 0);
     const bool part_seen = t0 + kTile > reach.end || (a.window > 0 && t0 <= reach.pmin - a.window);
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
-      const int u = tid + k * kThreadsT;
-      if (kUnits % kThreadsT != 0 && u >= kUnits) break;
-      const int kt = u / KP, x = 2 * (u - kt * KP);
-      half8v *row = reinterpret_cast<half8v *>(tiles_of + to * kHalf) + kt * (DP / 8);
-      row[x ^ (kt & kMask)] = Widen8(kw[k][0], kw[k][1]);
-      row[(x + 1) ^ (kt & kMask)] = Widen8(kw[k][2], kw[k][3]);
+      if (kUnits % kThreadsT != 0 && grp[k] >= 4) break;
       // A weight of 0 does not undo a NaN: values of tokens that no row sees are cleared.
-      const int quad = u / (DP / 4), d = 4 * (u % (DP / 4));
-      if (part_seen || !vgood[k]) {
+      const bool good = vid[k] < c.pages;
+      if (part_seen || !good) {
+        const uint32_t u = Opaque(tid) + k * kThreadsT;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int tok = t0 + 4 * quad + e;
-          const bool seen = vgood[k] && tok < reach.end &&
+          const int tok = t0 + static_cast<int>(4 * (u / (DP / 4))) + e;
+          const bool seen = good && tok < reach.end &&
                             (a.window == 0 || tok > reach.pmin - a.window);
           vw[k][e] = seen ? vw[k][e] : 0u;
         }
@@ -631,97 +694,115 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
       const uint32_t nan = NanTops(vw[k][0]) | NanTops(vw[k][1]) | NanTops(vw[k][2]) |
                            NanTops(vw[k][3]);
       if (nan != 0) {
+        const uint32_t u = Opaque(tid) + k * kThreadsT;
         any_nan[n & 3] = 1;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t tops = NanTops(vw[k][e]);
-          const int tok = 4 * quad + e;
+          const int tok = 4 * (u / (DP / 4)) + e;
 #pragma unroll 1
           for (int x = 0; x < 4; ++x)
             if ((tops >> (8 * x)) & 0x80u)
-              atomicOr(&nans[n & 3][d + x][tok >> 5], 1u << (tok & 31));
+              atomicOr(&nans[n & 3][4 * (u % (DP / 4)) + x][tok >> 5], 1u << (tok & 31));
           vw[k][e] &= ~((tops >> 7) * 0xFFu);
         }
       }
       uint32_t turned[4];
       Transpose4(vw[k], turned);
-      // Four tokens 4 quad .. of a group of 16 are the first or the second half of the
-      // eight that a lane with half = quad % 2 has weights of.
-      const int unit = 2 * (quad >> 2) + (quad & 1), part = (quad >> 1) & 1;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const half2v lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(turned[e]), 1.0f,
                                                                    false);
         const half2v hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(turned[e]), 1.0f,
                                                                    true);
-        const int swap = ((d >> 2) ^ (d + e)) & 7;
-        half4v *at = reinterpret_cast<half4v *>(tiles_of + (2 + to) * kHalf +
-                                                ((d + e) * (kTile / 8) + (unit ^ swap)) * 16);
-        at[part] = half4v{lo[0], lo[1], hi[0], hi[1]};
+        WriteLds(((off + vto[k]) ^ (16 * e)) + e * (kTile * 2), half4v{lo[0], lo[1], hi[0], hi[1]});
       }
-    }
-    if (tid < 4) {
-      const bool good = sid_now < c.pages;
-      info[to][tid] = good ? make_float4(sk, Log2Scale(sv), 1.0f / sv, 1.0f)
-                           : make_float4(1.0f, -kInf, 0.0f, 0.0f);
     }
   };
   const auto clear = [&](int n) {  // the record of tile n's NaN
-    for (int d = tid; d < DP; d += kThreadsT) nans[n & 3][d][0] = nans[n & 3][d][1] = 0;
-    if (tid == 0) any_nan[n & 3] = 0;
+    const int at = static_cast<int>(Opaque(tid));
+    for (int d = at; d < DP; d += kThreadsT) nans[n & 3][d][0] = nans[n & 3][d][1] = 0;
+    if (at == 0) any_nan[n & 3] = 0;
   };
 
-  floatx16v o[DT];
+  floatx16v o[DT], sc[2];
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
+  half8v p[4][kTerms];
   float m = -kInf, l = 0.0f;
 
   // Where this lane reads: the other tokens, values and half lie at constant distances.
-  const uint32_t base = static_cast<uint32_t>(
-      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)tiles_of));
   uint32_t kat[KP], vat[4];
 #pragma unroll
   for (int k = 0; k < KP; ++k)
     kat[k] = base + (col * (DP / 8) + ((2 * k + half) ^ (col & kMask))) * 16;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    vat[j] = base + 2 * kHalf + (col * (kTile / 8) + ((2 * j + half) ^ (((col >> 2) ^ col) & 7))) * 16;
+    vat[j] = base + 2 * kHalf +
+             (col * (kTile / 8) + ((2 * j + half) ^ (((col >> 2) ^ col) & 7))) * 16;
 
-  // One tile against this wavefront's rows; edge: some row does not see some token of it.
-  const auto step = [&](bool edge, int n) {
-    const int from = n & 1, t0 = reach.begin + kTile * n;
-    const uint32_t off = from ? kHalf : 0;
-    const auto seen = [&](int j) {  // token j of the tile, by this lane's row
-      const int tok = t0 + j;
-      return tok <= pos && tok < reach.end && info[from][j >> 4].w != 0.0f &&
-             (a.window == 0 || tok > pos - a.window);
+  // sc = K(n) Q^T and o += V(n - 1)^T P^T, or the first alone. Left to itself the compiler
+  // waits for each operand when it reads it (40 MFMAs' time); here kAhead are on their way.
+  const auto multiply = [&](auto values, int n) {
+    constexpr int kFirst = 2 * KP, kAll = kFirst + (decltype(values)::value ? 4 * DT : 0);
+    constexpr int kAhead = 6;
+    const uint32_t koff = n & 1 ? kHalf : 0, voff = kHalf - koff;
+    half8v x[kAhead];
+    const auto read = [&](int i) {
+      if (i < kFirst)
+        x[i % kAhead] = ReadLds(kat[i >> 1] + koff + (i & 1) * (32 * DP * 2));
+      else
+        x[i % kAhead] = ReadLds(vat[(i - kFirst) / DT] + voff +
+                                (i - kFirst) % DT * (32 * kTile * 2));
     };
-    floatx16v sc[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) sc[j][e] = 0.0f;
 #pragma unroll
-      for (int k = 0; k < KP; ++k) {
-        const half8v kf = ReadLds(kat[k] + off + j * (32 * DP * 2));
+    for (int i = 0; i < kAhead; ++i) read(i);
 #pragma unroll
-        for (int term = 0; term < kTerms; ++term)
-          sc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[k][term], sc[j], 0, 0, 0);
+    for (int i = 0; i < kAll; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int term = 0; term < kTerms; ++term) {
+        if (i < kFirst) {
+          sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[i % kAhead], q[i >> 1][term],
+                                                             sc[i & 1], 0, 0, 0);
+        } else {
+          const int j = (i - kFirst) / DT, d = (i - kFirst) % DT;
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[i % kAhead], p[j][term], o[d], 0, 0, 0);
+        }
       }
+      if (i + kAhead < kAll) read(i + kAhead);
     }
-    if (edge) {
-      __asm__ volatile("");  // a branch: as selects this would take as long as the rest
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // This lane's row sees token j of tile n, where it is of a page, if low < j <= high.
+  const auto high = [&](int n) { return min(pos, reach.end - 1) - (reach.begin + kTile * n); };
+  const auto low = [&](int n) {
+    return a.window > 0 ? pos - a.window - (reach.begin + kTile * n) : -1;
+  };
+  const auto weights = [&](int n) {  // p, l and m from sc
+    const int t0 = reach.begin + kTile * n;
+    float4 in[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) in[j] = info[n & 3][j];
+    // Whether some row does not see some token.
+    if (t0 + kTile - 1 > pmin || t0 + kTile > reach.end ||
+        (a.window > 0 && t0 <= pmax - a.window)) {
+      const int hi = high(n) - 4 * half, lo = low(n) - 4 * half;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          sc[j][e] = seen(32 * j + 8 * (e >> 2) + 4 * half + (e & 3)) ? sc[j][e] : -kInf;
+        for (int e = 0; e < 16; ++e) {
+          const int tok = 32 * j + 8 * (e >> 2) + (e & 3);
+          sc[j][e] = tok <= hi && tok > lo ? sc[j][e] : -kInf;
+        }
+      __asm__ volatile("");  // a branch: as selects this would take as long as the rest
     }
-    float4 in[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) in[j] = info[from][j];
     float top = -kInf, scale[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -731,12 +812,11 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
       for (int e = 0; e < 8; ++e) most = fmaxf(most, sc[j >> 1][8 * (j & 1) + e]);
       top = fmaxf(top, fmaf(most, scale[j], in[j].y));
     }
-    top = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
+    top = fmaxf(m, MaxHalves(top));
     const float use = top == -kInf ? 0.0f : top;
     const float alpha = Exp2(m - use);
     const bool grew = top != m;
     m = top;
-    half8v p[4][kTerms];
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -744,64 +824,75 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = sc[j >> 1][8 * (j & 1) + e];
       sum = fmaf(Weights<kTerms>(y, scale[j], in[j].y - use + kShift, p[j]), in[j].z, sum);
+      // Made here, not where they are used: there the matrix instructions would wait, and
+      // what they are made of would take registers.
+#pragma unroll
+      for (int term = 0; term < kTerms; ++term) __asm__ volatile("" : "+v"(p[j][term]));
     }
     l = fmaf(l, alpha, sum);
+    __asm__ volatile("" : "+v"(l));
     if (__any(grew)) {
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] *= alpha;
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const half8v v = ReadLds(vat[j] + off + d * (32 * kTile * 2));
-#pragma unroll
-        for (int term = 0; term < kTerms; ++term)
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[j][term], o[d], 0, 0, 0);
-      }
+  };
+  const auto spoil = [&](int n) {  // NaN values of tile n, to the rows that see them
     if (any_nan[n & 3] != 0) {
-      uint32_t sees[2] = {~0u, ~0u};
-      if (edge) {
-        sees[0] = sees[1] = 0;
-        for (int j = 0; j < kTile; ++j) sees[j >> 5] |= seen(j) ? 1u << (j & 31) : 0u;
-      }
+      const auto to = [](int j) {  // the tokens up to j
+        return j < 0 ? uint64_t{0} : j >= 63 ? ~uint64_t{0} : (uint64_t{2} << j) - 1;
+      };
+      const uint64_t seen = to(high(n)) & ~to(low(n));
+      const uint32_t sees[2] = {static_cast<uint32_t>(seen), static_cast<uint32_t>(seen >> 32)};
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const uint32_t *w = nans[n & 3][32 * d + 8 * (e >> 2) + 4 * half + (e & 3)];
           if (((w[0] & sees[0]) | (w[1] & sees[1])) != 0) o[d][e] = __builtin_nanf("");
+          __builtin_amdgcn_sched_barrier(0);  // one condition at a time: all would take 128 SGPRs
         }
     }
   };
 
   if (tile0 < tile1) {
+    // Where a SIMD has two of the wavefronts, one multiplies while the other makes
+    // weights and widens codes: the second is half a step behind, and so, to be in time
+    // for the first, brings its share of a tile a step ahead.
+    const bool second = NW == 8 && wave >= 4;
     for (int n = 0; n < 4; ++n) clear(n);
-    __syncthreads();
     find(tile0);
-    load(tile0);
+    load_keys(tile0);
     find(tile0 + 1);
-    store(tile0);
-    load(tile0 + 1);
+    __syncthreads();
+    store_keys(tile0);
+    load_keys(tile0 + 1);
+    load_values();
     find(tile0 + 2);
+    int ahead = tile0;
+    const auto bring = [&]() {  // the keys of tile ahead + 1, the values of tile ahead
+      store_keys(ahead + 1);
+      store_values(ahead);
+      load_keys(ahead + 2);
+      load_values();
+      find(ahead + 3);
+      ++ahead;
+    };
     __syncthreads();
-  }
-  for (int n = tile0; n < tile1; ++n) {
-    const int t0 = reach.begin + kTile * n;
-    if (n + 1 < tile1) {
-      store(n + 1);
-      load(n + 2);
-      find(n + 3);
+    if (second) {
+      bring();
+      __syncthreads();
     }
-    clear(n + 3);
-    if (busy && t0 <= pmax && (a.window == 0 || t0 + kTile - 1 > pmin - a.window)) {
-      const bool edge = t0 + kTile - 1 > pmin || t0 + kTile > reach.end ||
-                        (a.window > 0 && t0 <= pmax - a.window) ||
-                        info[n & 1][0].w * info[n & 1][1].w * info[n & 1][2].w *
-                                info[n & 1][3].w == 0.0f;
-      step(__builtin_amdgcn_readfirstlane(edge), n);
+    multiply(std::false_type{}, tile0);
+    for (int n = tile0; n < tile1; ++n) {
+      __syncthreads();
+      weights(n);
+      bring();
+      if (!second) clear(n + 2);
+      __syncthreads();
+      multiply(std::true_type{}, n + 1);  // the scores of tile1 are not used
+      spoil(n);
     }
-    __syncthreads();
+    if (NW == 8 && !second) __syncthreads();
   }
   if (!there) return;
   l += __shfl_xor(l, 32);
