@@ -9,10 +9,10 @@
 //
 // e4m3 codes are exact in fp16, so the products are fp16 MFMAs on the codes
 // themselves. A page's key scale multiplies its scores. Its value scale w goes
-// into the exponent: with y = s log2(e) + log2(w) and m the running maximum of y,
-// P = 2^(y - m + 14) is the token's weight times its value scale, at most 2^14 and
-// with full fp16 precision down to 2^-28 of the largest; the sum of the weights
-// alone takes P / w. Then O / l needs no further scale.
+// into the exponent: with y = s log2(e) + log2(w) and m a running maximum of y,
+// P = 2^(y - m + 14) is the token's weight times its value scale, with full fp16
+// precision down to 2^-28 of the largest; the sum of the weights alone takes P / w. Then
+// O / l needs no further scale.
 // Queries are scaled by a power of two to below 2^15 and rounded to one fp16 term
 // (exact for fp16, and for bf16 down to 2^-31 of the row's largest magnitude) or,
 // fp32, to two (22 bits); P likewise is one term or, fp32, two.
@@ -35,7 +35,9 @@ constexpr int kTile = 64;          // tokens of a step
 constexpr int kWaves = 4;          // of a workgroup: each takes every fourth tile of its part
 constexpr int kThreads = 64 * kWaves;
 constexpr float kInf = __builtin_inff();
-constexpr float kShift = 14.0f;    // P's largest value is 2^14
+constexpr float kShift = 14.0f;    // P is 2^14 where y is m: AttendSplitKernel
+constexpr float kTileShift = 12.0f;  // 2^12: AttendTileKernel, whose m may be behind
+constexpr float kMost = 65504.0f;  // fp16's largest value
 
 template <typename T>
 constexpr int Terms() { return sizeof(T) == 4 ? 2 : 1; }
@@ -676,6 +678,9 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
     const int t0 = reach.begin + kTile * n;
     const uint32_t off = base + (n & 1 ? kHalf : 0);
     const bool part_seen = t0 + kTile > reach.end || (a.window > 0 && t0 <= reach.pmin - a.window);
+    // Some rows see a token that others do not: elsewhere NaN may go the way of all values.
+    const bool mixed = t0 + kTile - 1 > reach.pmin ||
+                       (a.window > 0 && t0 <= reach.pmax - a.window);
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
       if (kUnits % kThreadsT != 0 && grp[k] >= 4) break;
@@ -691,8 +696,9 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
           vw[k][e] = seen ? vw[k][e] : 0u;
         }
       }
-      const uint32_t nan = NanTops(vw[k][0]) | NanTops(vw[k][1]) | NanTops(vw[k][2]) |
-                           NanTops(vw[k][3]);
+      uint32_t nan = 0;
+      if (mixed)
+        nan = NanTops(vw[k][0]) | NanTops(vw[k][1]) | NanTops(vw[k][2]) | NanTops(vw[k][3]);
       if (nan != 0) {
         const uint32_t u = Opaque(tid) + k * kThreadsT;
         any_nan[n & 3] = 1;
@@ -719,10 +725,9 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
       }
     }
   };
-  const auto clear = [&](int n) {  // the record of tile n's NaN
-    const int at = static_cast<int>(Opaque(tid));
-    for (int d = at; d < DP; d += kThreadsT) nans[n & 3][d][0] = nans[n & 3][d][1] = 0;
-    if (at == 0) any_nan[n & 3] = 0;
+  const auto clear = [&](int n) {  // the record of tile n's NaN, by one wavefront
+    for (int d = lane; d < DP; d += 64) nans[n & 3][d][0] = nans[n & 3][d][1] = 0;
+    any_nan[n & 3] = 0;
   };
 
   floatx16v o[DT], sc[2];
@@ -803,38 +808,53 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
         }
       __asm__ volatile("");  // a branch: as selects this would take as long as the rest
     }
-    float top = -kInf, scale[4];
+    float scale[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      scale[j] = ScoreScale(cq, in[j].x);
-      float most = -kInf;
+    for (int j = 0; j < 4; ++j) scale[j] = ScoreScale(cq, in[j].x);
+    float part[4];
+    const auto make = [&](float top) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) most = fmaxf(most, sc[j >> 1][8 * (j & 1) + e]);
-      top = fmaxf(top, fmaf(most, scale[j], in[j].y));
-    }
-    top = fmaxf(m, MaxHalves(top));
-    const float use = top == -kInf ? 0.0f : top;
-    const float alpha = Exp2(m - use);
-    const bool grew = top != m;
-    m = top;
-    float sum = 0.0f;
+      for (int j = 0; j < 4; ++j) {
+        float y[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float y[8];
+        for (int e = 0; e < 8; ++e) y[e] = sc[j >> 1][8 * (j & 1) + e];
+        part[j] = Weights<kTerms>(y, scale[j], in[j].y - top + kTileShift, p[j]);
+      }
+    };
+    // The maximum that earlier tiles left does, as long as no eight weights add up to what
+    // fp16 cannot hold (a NaN fails this too, as at the first tile); else the
+    // tile's own is found, and a factor of 2 left above it.
+    make(m);
+    const bool fits = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) <= kMost &&
+                      part[0] + part[1] + part[2] + part[3] < kInf;
+    if (__any(!fits)) {
+      __asm__ volatile("");
+      float top = -kInf;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = sc[j >> 1][8 * (j & 1) + e];
-      sum = fmaf(Weights<kTerms>(y, scale[j], in[j].y - use + kShift, p[j]), in[j].z, sum);
-      // Made here, not where they are used: there the matrix instructions would wait, and
-      // what they are made of would take registers.
+      for (int j = 0; j < 4; ++j) {
+        float most = -kInf;
 #pragma unroll
-      for (int term = 0; term < kTerms; ++term) __asm__ volatile("" : "+v"(p[j][term]));
-    }
-    l = fmaf(l, alpha, sum);
-    __asm__ volatile("" : "+v"(l));
-    if (__any(grew)) {
+        for (int e = 0; e < 8; ++e) most = fmaxf(most, sc[j >> 1][8 * (j & 1) + e]);
+        top = fmaxf(top, fmaf(most, scale[j], in[j].y));
+      }
+      top = MaxHalves(top) + 1.0f;
+      const float next = fmaxf(m, top), use = next == -kInf ? 0.0f : next;
+      const float alpha = Exp2(m - use);
+      m = next;
+      make(use);
+      l *= alpha;
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] *= alpha;
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) l = fmaf(part[j], in[j].z, l);
+    // Made here, not where they are used: there the matrix instructions would wait, and what
+    // they are made of would take registers.
+    __asm__ volatile("" : "+v"(l));
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int term = 0; term < kTerms; ++term) __asm__ volatile("" : "+v"(p[j][term]));
   };
   const auto spoil = [&](int n) {  // NaN values of tile n, to the rows that see them
     if (any_nan[n & 3] != 0) {
@@ -859,7 +879,8 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
     // weights and widens codes: the second is half a step behind, and so, to be in time
     // for the first, brings its share of a tile a step ahead.
     const bool second = NW == 8 && wave >= 4;
-    for (int n = 0; n < 4; ++n) clear(n);
+    if (wave == 0)
+      for (int n = 0; n < 4; ++n) clear(n);
     find(tile0);
     load_keys(tile0);
     find(tile0 + 1);
@@ -887,7 +908,7 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
       __syncthreads();
       weights(n);
       bring();
-      if (!second) clear(n + 2);
+      if (wave == 0 && any_nan[(n + 2) & 3] != 0) clear(n + 2);
       __syncthreads();
       multiply(std::true_type{}, n + 1);  // the scores of tile1 are not used
       spoil(n);

@@ -11,8 +11,9 @@ row's keys:
     and by 2^-21 for the hardware's exponential;
   - the weights of a row are divided by their sum, which has the same errors: twice;
   - a weight is rounded to fp16, 2^-11 relative, for 16-bit queries, to 2^-22 for fp32,
-    and where it is below fp16's normal values to 2^-39 of the largest times its value
-    scale: n 2^-38 max|v| for n keys, max|v| by channel;
+    and where it is below fp16's normal values by 2^-25 at most; the largest weight (times its
+    value scale) is 2^14 for few rows, for many 2^12 or, as a factor of 2 is left above it
+    when it is found, 2^11 at least: 2^-36 of it, n 2^-35 max|v| for n keys, max|v| by channel;
   - sums of n weighted values in fp32: n 2^-24 A; joins and the division, 2^-20 A;
   - the output's rounding, half a step (eps / 2) of the value.
 """
@@ -99,7 +100,7 @@ def _attend64(Q, k, v, table, spans, scale, window, dtype):
                 w = 2.0 ** -22 if dtype == torch.float32 else 2.0 ** -11
                 y[row + i, h] = p @ vv
                 tol[row + i, h] = ((e + w + m * 2.0 ** -24 + 2.0 ** -20) * A
-                                   + m * 2.0 ** -38 * vv.abs().amax(dim=0))
+                                   + m * 2.0 ** -35 * vv.abs().amax(dim=0))
     tol += eps / 2 * (y.abs() + tol) + torch.finfo(dtype).smallest_normal * eps
     return y, tol
 
