@@ -18,8 +18,6 @@ struct Part {
 };
 
 struct Args {
-  uint64_t turns[kMaxPairs];
-  uint8_t axis[kMaxPairs];
   Part part[2];
   const void *pos;
   int64_t axis_stride, T;
@@ -27,6 +25,14 @@ struct Args {
   int32_t head_dim, pairs;
   int32_t tokens;         // a workgroup's
   bool pos64, interleaved;
+};
+
+// Frequencies travel with the launch, so that a call depends on no memory but its tensors;
+// a launch with 64 of them is 1.7 KiB shorter than one with 256.
+template <int PAIRS>
+struct Frequencies {
+  uint64_t turns[PAIRS];
+  uint8_t axis[PAIRS];
 };
 
 // cos and sin of `turn` 2^-64 turns. The nearest quarter turn goes off in
@@ -55,17 +61,17 @@ __device__ __forceinline__ float2 CosSin(uint64_t turn) {
 // heads (one 64-bit product, 30 operations a pair), then turns the heads: an
 // item is one head's eight pairs, two loads and two stores of 16 bytes for 16-bit
 // types. Memory bounds it.
-template <typename T, bool VEC>
-__global__ __launch_bounds__(kThreads) void RotaryKernel(Args a) {
+template <typename T, bool VEC, int PAIRS>
+__global__ __launch_bounds__(kThreads) void RotaryKernel(Args a, Frequencies<PAIRS> f) {
   extern __shared__ float2 table[];  // [tokens][pairs]
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tokens;
   const int tokens = static_cast<int>(min(static_cast<int64_t>(a.tokens), a.T - t0));
   for (int i = threadIdx.x; i < tokens * a.pairs; i += kThreads) {
     const int t = i / a.pairs, j = i - t * a.pairs;
-    const int64_t at = a.axis[j] * a.axis_stride + t0 + t;
+    const int64_t at = f.axis[j] * a.axis_stride + t0 + t;
     const int64_t p = a.pos64 ? static_cast<const int64_t *>(a.pos)[at]
                               : static_cast<const int32_t *>(a.pos)[at];
-    table[i] = CosSin(static_cast<uint64_t>(p) * a.turns[j]);
+    table[i] = CosSin(static_cast<uint64_t>(p) * f.turns[j]);
   }
   __syncthreads();
   const int rot = (a.pairs + 7) / 8;                       // items of a head that turn,
@@ -127,8 +133,11 @@ bool VecPart(const Part &p, int64_t size) {
          p.yt * size % 16 == 0 && p.yh * size % 16 == 0;
 }
 
-template <typename T>
-hipError_t Launch(Args &a, hipStream_t s) {
+template <typename T, int PAIRS>
+hipError_t LaunchFor(Args &a, const mnb_rotary_desc &d, hipStream_t s) {
+  Frequencies<PAIRS> f;
+  std::copy_n(d.turns, a.pairs, f.turns);
+  std::copy_n(d.axis, a.pairs, f.axis);
   const int items = a.heads * ((a.pairs + 7) / 8 + (a.head_dim - 2 * a.pairs + 15) / 16);
   // About two items a thread; the table of cos and sin has one entry a thread or
   // little more. Few tokens are shared by several workgroups.
@@ -140,10 +149,15 @@ hipError_t Launch(Args &a, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(groups), split);
   const size_t lds = sizeof(float2) * a.tokens * a.pairs;
   if (vec)
-    hipLaunchKernelGGL((RotaryKernel<T, true>), grid, dim3(kThreads), lds, s, a);
+    hipLaunchKernelGGL((RotaryKernel<T, true, PAIRS>), grid, dim3(kThreads), lds, s, a, f);
   else
-    hipLaunchKernelGGL((RotaryKernel<T, false>), grid, dim3(kThreads), lds, s, a);
+    hipLaunchKernelGGL((RotaryKernel<T, false, PAIRS>), grid, dim3(kThreads), lds, s, a, f);
   return hipGetLastError();
+}
+
+template <typename T>
+hipError_t Launch(Args &a, const mnb_rotary_desc &d, hipStream_t s) {
+  return a.pairs <= 64 ? LaunchFor<T, 64>(a, d, s) : LaunchFor<T, kMaxPairs>(a, d, s);
 }
 
 int CheckHeads(const mnb_rotary_heads *h, int64_t head_dim, uintptr_t size) {
@@ -181,11 +195,8 @@ extern "C" int mnb_rotary(const mnb_rotary_desc *desc, int64_t T, int32_t pos_ty
     return MNB_ERR_BAD_SHAPE;
   Args a;
   a.pairs = R / 2;
-  for (int j = 0; j < a.pairs; ++j) {
+  for (int j = 0; j < a.pairs; ++j)
     if (desc->axis[j] >= desc->axes) return MNB_ERR_BAD_ATTRIBUTE;
-    a.turns[j] = desc->turns[j];
-    a.axis[j] = desc->axis[j];
-  }
   const uintptr_t size = x_type == MNB_TYPE_FLOAT ? 4 : 2;
   if (T == 0) return MNB_OK;
   a.heads0 = query->heads;
@@ -221,9 +232,9 @@ extern "C" int mnb_rotary(const mnb_rotary_desc *desc, int64_t T, int32_t pos_ty
   }
   const hipStream_t s = static_cast<hipStream_t>(stream);
   switch (x_type) {
-  case MNB_TYPE_FLOAT16: e = Launch<_Float16>(a, s); break;
-  case MNB_TYPE_BFLOAT16: e = Launch<__bf16>(a, s); break;
-  default: e = Launch<float>(a, s);
+  case MNB_TYPE_FLOAT16: e = Launch<_Float16>(a, *desc, s); break;
+  case MNB_TYPE_BFLOAT16: e = Launch<__bf16>(a, *desc, s); break;
+  default: e = Launch<float>(a, *desc, s);
   }
   if (e == hipSuccess) return MNB_OK;
   SetLastHipError("rotary positions", e);

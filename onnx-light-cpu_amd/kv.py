@@ -173,31 +173,31 @@ class Fp8KVCache:
             table = table.contiguous()
         if not lengths.is_contiguous():
             lengths = lengths.contiguous()
-        if starts is not None and not starts.is_contiguous():
-            starts = starts.contiguous()
+        B, width = table.shape
         shape = X.shape
         tokens = shape[0] if len(shape) == 3 else shape[0] * shape[1]
-        batch = KvBatch(table.shape[0], tokens, 0 if starts is None else max_tokens or 0,
-                        table.shape[1], table.data_ptr(), lengths.data_ptr(),
-                        None if starts is None else starts.data_ptr())
-        return batch, (table, lengths, starts)
+        if starts is None:
+            return KvBatch(B, tokens, 0, width, table.data_ptr(), lengths.data_ptr(),
+                           None), (table, lengths)
+        if not starts.is_contiguous():
+            starts = starts.contiguous()
+        return KvBatch(B, tokens, max_tokens or 0, width, table.data_ptr(), lengths.data_ptr(),
+                       starts.data_ptr()), (table, lengths, starts)
 
     @staticmethod
     def _rows(X):
         """(the C struct of X [..., heads, head_dim], the tensor it points into): X, or a
         copy where its rows are not evenly apart or not aligned to 16 bytes."""
-        shape, strides = X.shape, X.stride()
-        H, D = shape[-2:]
-        sh = strides[-2] if H > 1 else D
+        shape, strides, address, even = X.shape, X.stride(), X.data_ptr(), True
         if len(shape) == 3:
-            st = strides[0] if shape[0] > 1 else H * D
-            even = True
+            n, H, D = shape
+            st = strides[0] if n > 1 else H * D
         else:
-            n, t = shape[:2]
+            n, t, H, D = shape
             st = strides[1] if t > 1 else strides[0] if n > 1 else H * D
             even = n <= 1 or t <= 1 or strides[0] == t * strides[1]
+        sh = strides[-2] if H > 1 else D
         each = 16 // X.element_size()
-        address = X.data_ptr()
         if (not even or strides[-1] != 1 or st < D or sh < D or st % each or sh % each
                 or address % 16 != 0):
             X = X.clone() if X.is_contiguous() else X.contiguous()
@@ -262,8 +262,10 @@ class Fp8KVCache:
         q, X = self._rows(Q)
         batch, keep = self._batch(Q, table, lengths, starts, max_tokens)
         if out is None:
-            make = torch.empty if starts is None else torch.zeros
-            out = make(Q.shape, dtype=Q.dtype, device=self.device)
+            if starts is not None:
+                out = torch.zeros(Q.shape, dtype=Q.dtype, device=self.device)
+            else:
+                out = torch.empty_like(Q, memory_format=torch.contiguous_format)
         key = (batch.sequences, batch.tokens, batch.max_tokens, batch.table_width, heads, x_type,
                starts is None)
         need = self._needs.get(key)

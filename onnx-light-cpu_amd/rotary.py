@@ -9,14 +9,14 @@ from __future__ import annotations
 
 import ctypes
 import math
-from fractions import Fraction
-
 from . import _check, _raw_stream, library
 from .fp8 import _elsewhere
 
 PREFIX = "onnx_light_cpu_amd::Rotary"
 MAX_PAIRS, MAX_AXES = 256, 8
-_TWO_PI = 2 * Fraction("3.14159265358979323846264338327950288419716939937510582097494")
+# 2^256 / (2 pi), of pi's first 60 digits
+_PI_DIGITS = 314159265358979323846264338327950288419716939937510582097494
+_PER_TURN = 2 ** 256 * 10 ** 59 // (2 * _PI_DIGITS)
 
 _lib = None
 _types = None  # torch dtype -> MNB_TYPE_* of include/mnb_fp8.h
@@ -97,30 +97,39 @@ class Rotary:
         self.inv_freq = [float(f) for f in inv_freq]
         if len(self.inv_freq) != pairs or not all(map(math.isfinite, self.inv_freq)):
             raise ValueError(f"{PREFIX}: inv_freq must be {pairs} finite numbers")
-        # 2^64 f / (2 pi) modulo 2^64, from the double exactly
-        turns = [round(Fraction(f) / _TWO_PI * 2 ** 64) % 2 ** 64 for f in self.inv_freq]
+        # f / (2 pi) modulo 1 in units of 2^-64, from the double as the ratio that it is
+        turns = []
+        for f in self.inv_freq:
+            over, under = f.as_integer_ratio()
+            turns.append(((over * _PER_TURN // under >> 191) + 1 >> 1) % 2 ** 64)
         self._turns = (ctypes.c_uint64 * pairs)(*turns)
         self._axis = (ctypes.c_uint8 * pairs)(*axes)
         self.desc = RotaryDesc(self.head_dim, self.rotary_dim, self.axes, int(bool(interleaved)),
                                self._turns, self._axis)
 
-    def _heads(self, x, y):
-        """The C struct of x [T, H, D] and its result y, with addresses and strides."""
-        return RotaryHeads(x.shape[-2], x.data_ptr(), x.stride(0), x.stride(1), y.data_ptr(),
-                           y.stride(0), y.stride(1))
-
     @staticmethod
-    def _flat(x):
-        """x [..., H, D] as [T, H, D] without a copy, or None."""
-        try:
-            y = x if x.dim() == 3 else x.view((math.prod(x.shape[:-2]),) + x.shape[-2:])
-        except RuntimeError:
+    def _strides(x):
+        """(between tokens, between heads) of x [..., H, D] in values, None where its heads
+        are not whole or its tokens not evenly apart."""
+        shape, strides = x.shape, x.stride()
+        H, D = shape[-2:]
+        sh = strides[-2] if H > 1 else D
+        if len(shape) == 3:
+            st = strides[0] if shape[0] > 1 else H * D
+        else:
+            st = apart = 0
+            for n, d in zip(shape[-3::-1], strides[-3::-1]):  # the axes of tokens, last first
+                if n == 1:
+                    continue
+                if st == 0:
+                    st = apart = d
+                elif d != apart:
+                    return None
+                apart *= n
+            st = st or H * D
+        if st < D or sh < D or (D > 1 and strides[-1] != 1):
             return None
-        # axes of one value may have any stride: theirs counts for nothing
-        s = [d if n > 1 else y.shape[1] * y.shape[2] for n, d in zip(y.shape[:2], y.stride()[:2])]
-        if s[0] < y.shape[2] or s[1] < y.shape[2] or (y.shape[2] > 1 and y.stride(2) != 1):
-            return None
-        return y.as_strided(y.shape, (s[0], s[1], 1))
+        return st, sh
 
     def __call__(self, Q, K, positions, out=None, stream=None):
         """(Q', K') of Q [..., Hq, head_dim] and K [..., Hkv, head_dim] (float32, float16
@@ -142,11 +151,12 @@ class Rotary:
                                  f"got {list(x.shape)}")
             if x.dtype != dtype or x.device != device:
                 raise ValueError(f"{PREFIX}: {name} must be of Q's type and device")
-        want = tuple(tokens) if self.axes == 1 else (self.axes,) + tuple(tokens)
-        pos_type = _positions.get(positions.dtype)
+        pos_type, where = _positions.get(positions.dtype), positions.shape
+        want = (self.axes,) + tokens
         if (pos_type is None or positions.device != device
-                or tuple(positions.shape) not in ((want, (1,) + want) if self.axes == 1 else (want,))):
-            raise ValueError(f"{PREFIX}: positions must be int32 or int64 {list(want)} on {device}, "
+                or (where != want and (self.axes > 1 or where != tokens))):
+            want = list(want if self.axes > 1 else tokens)
+            raise ValueError(f"{PREFIX}: positions must be int32 or int64 {want} on {device}, "
                              f"got {positions.dtype} {list(positions.shape)}")
         if out is not None:
             out = (out,) if K is None and isinstance(out, torch.Tensor) else tuple(out)
@@ -154,27 +164,34 @@ class Rotary:
                 raise ValueError(f"{PREFIX}: out must be {len(parts)} tensors")
             for (name, x), y in zip(parts, out):
                 if (y.shape != x.shape or y.dtype != dtype or y.device != device
-                        or self._flat(y) is None):
+                        or (y.numel() and self._strides(y) is None)):
                     raise ValueError(f"{PREFIX}: out must have {name}'s shape, type and device, "
                                      "and whole heads")
         elsewhere = _elsewhere(device, stream)
         if elsewhere is not None:
             with elsewhere:
                 return self(Q, K, positions, out)
+        T = tokens[0] if len(tokens) == 1 else math.prod(tokens)
+        if T == 0:
+            results = [torch.empty_like(x) for _, x in parts] if out is None else out
+            return results[0] if K is None else tuple(results)
         heads, results, keep = [], [], []
         for i, (name, x) in enumerate(parts):
-            flat = self._flat(x)
-            if flat is None:
-                flat = self._flat(x.contiguous())
-            y = torch.empty(x.shape, dtype=dtype, device=device) if out is None else out[i]
-            flat_y = self._flat(y)
-            if flat_y.data_ptr() == flat.data_ptr() and flat_y.stride() != flat.stride():
-                flat = flat.contiguous()
-            keep.append(flat)
-            heads.append(self._heads(flat, flat_y))
+            strides = self._strides(x)
+            y = torch.empty_like(x) if out is None else out[i]
+            to = self._strides(y)
+            if to is None:  # empty_like kept an order of axes
+                y = torch.empty(x.shape, dtype=dtype, device=device)
+                to = self._strides(y)
+            address, address_y = x.data_ptr(), y.data_ptr()
+            if strides is None or (address == address_y and strides != to):
+                x = x.clone(memory_format=torch.contiguous_format)
+                keep.append(x)
+                strides, address = self._strides(x), x.data_ptr()
+            heads.append(RotaryHeads(x.shape[-2], address, *strides, address_y, *to))
             results.append(y)
-        T = math.prod(tokens)
-        positions = positions.contiguous()
+        if not positions.is_contiguous():
+            positions = positions.contiguous()
         status = L.mnb_rotary(ctypes.byref(self.desc), T, pos_type, positions.data_ptr(), T, x_type,
                               ctypes.byref(heads[0]),
                               ctypes.byref(heads[1]) if K is not None else None,
