@@ -9,10 +9,11 @@
 //
 // e4m3 codes are exact in fp16, so the products are fp16 MFMAs on the codes
 // themselves. A page's key scale multiplies its scores. Its value scale w goes
-// into the exponent: with y = s log2(e) + log2(w) and m a running maximum of y,
-// P = 2^(y - m + 14) is the token's weight times its value scale, with full fp16
-// precision down to 2^-28 of the largest; the sum of the weights alone takes P / w. Then
-// O / l needs no further scale.
+// into the exponent: with y = s log2(e) + log2(w) and m near the maximum of y so far,
+// P = 2^(y - m + 12) is the token's weight times its value scale, with full fp16
+// precision down to 2^-25 of the largest; the sum of the weights alone takes P / w. Then
+// O / l needs no further scale. m is the maximum that earlier tiles left, and a factor of 2
+// above it, until a tile has weights that fp16 might not hold.
 // Queries are scaled by a power of two to below 2^15 and rounded to one fp16 term
 // (exact for fp16, and for bf16 down to 2^-31 of the row's largest magnitude) or,
 // fp32, to two (22 bits); P likewise is one term or, fp32, two.
@@ -35,9 +36,7 @@ constexpr int kTile = 64;          // tokens of a step
 constexpr int kWaves = 4;          // of a workgroup: each takes every fourth tile of its part
 constexpr int kThreads = 64 * kWaves;
 constexpr float kInf = __builtin_inff();
-constexpr float kShift = 14.0f;    // P is 2^14 where y is m: AttendSplitKernel
-constexpr float kTileShift = 12.0f;  // 2^12: AttendTileKernel, whose m may be behind
-constexpr float kMost = 65504.0f;  // fp16's largest value
+constexpr float kShift = 12.0f;    // P is 2^12 where y is m
 
 template <typename T>
 constexpr int Terms() { return sizeof(T) == 4 ? 2 : 1; }
@@ -133,6 +132,17 @@ __device__ __forceinline__ void SplitQuery(const float (&f)[8], int shift, float
 // The weights 2^(scale s + add) of eight scores as fp16 terms, and their sum before that rounding:
 // beside a page of far larger values a page's weights may be lost for the values'
 // sum, but never for their own.
+// Whether fp16 holds all weights that add up to these sums; a NaN fails too, as it does
+// in a row's first tile.
+__device__ __forceinline__ bool Fits(const float (&sum)[4]) {
+  return fmaxf(fmaxf(sum[0], sum[1]), fmaxf(sum[2], sum[3])) <= 65504.0f &&
+         sum[0] + sum[1] + sum[2] + sum[3] < kInf;
+}
+
+__device__ __forceinline__ float FromLane(float v, int lane) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
+}
+
 template <int TERMS>
 __device__ __forceinline__ float Weights(const float (&s)[8], float scale, float add,
                                          half8v (&p)[TERMS]) {
@@ -258,46 +268,74 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
     for (int d = 0; d < VD; ++d) o[t][d] = floatx4v{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  for (int step = split * each + wave; step < tile1; step += kWaves) {
-    const int t0 = reach.begin + kTile * step;
-    // Every token is seen by every row, unless the tile lies at an edge.
-    bool edge = t0 + kTile - 1 > reach.pmin || t0 + kTile > reach.end ||
-                (a.window > 0 && t0 <= reach.pmax - a.window);
-    uint4v kw[4][KS];
-    uint32_t vw[4][4][VW];
-    float ks[4], ev[4], inv[4];
+  // A tile is four groups of 16 tokens, each of one page; lanes 16 j .. look up group j's
+  // page and scales. Keys are asked for as soon as the last tile's are multiplied,
+  // values likewise, into the same registers, and pages a tile earlier.
+  uint4v kw[4][KS];
+  uint32_t vw[4][4][VW];
+  uint32_t id[4];  // pages of what kw holds or will hold, ~0 for none
+  float sk = 1.0f, sv = 1.0f;
+  const uint32_t dim = c.dim, slots = (1u << c.page_shift) - 1;
+  const uint32_t head = static_cast<uint32_t>(h << c.page_shift) * dim;
+  const uint32_t apart = static_cast<uint32_t>(c.heads << c.page_shift) * dim;
+  const int32_t *table = a.batch.table + static_cast<int64_t>(s) * a.batch.width;
+  // Past head_dim the query is 0: any of a key's codes will do; and rows of O^T lie there
+  // that are not stored.
+  uint32_t koff[KS];
+#pragma unroll
+  for (int j = 0; j < KS; ++j)
+    koff[j] = col * dim + (64 * j + 16 * grp < dim ? 64 * j + 16 * grp : 0);
+  const uint32_t voff = 4 * grp * dim + (VD * col < dim ? VD * col : 0);
+  const auto find = [&](int step) {
+    const int tok = reach.begin + kTile * step + 16 * grp;
+    const uint32_t page = table[min(tok, reach.end - 1) >> c.page_shift];
+    return step < tile1 && tok < reach.end && page < c.pages ? page : ~0u;
+  };
+  const auto spread = [&](uint32_t page) {
+#pragma unroll
+    for (int sub = 0; sub < 4; ++sub) id[sub] = __builtin_amdgcn_readlane(page, 16 * sub);
+  };
+  const auto where = [&](int step, int sub) {  // codes before a group's; page 0's for none
+    const uint32_t slot = (reach.begin + kTile * step + 16 * sub) & slots;
+    return static_cast<int64_t>(id[sub] != ~0u ? id[sub] : 0) * apart + (head + slot * dim);
+  };
+  const auto load_keys = [&](int step) {
 #pragma unroll
     for (int sub = 0; sub < 4; ++sub) {
-      const int ts = t0 + 16 * sub;
-      uint32_t id = ts < reach.end ? PageOf(a.batch, s, ts >> c.page_shift) : ~0u;
-      const bool good = id < c.pages;
-      edge |= !good;
-      id = good ? id : 0u;  // in bounds; nothing of it counts
-      const int64_t at = static_cast<int64_t>(id) * c.heads + h;
-      const int slot = ts & ((1 << c.page_shift) - 1);
-      const int64_t base = ((at << c.page_shift) + slot) * c.dim;
-      const uint8_t *kp = c.codes[0] + base + col * c.dim;
-      const uint8_t *vp = c.codes[1] + base + 4 * grp * c.dim;
+      const uint8_t *k = c.codes[0] + where(step, sub);
 #pragma unroll
-      for (int j = 0; j < KS; ++j) {
-        // Past head_dim the query is 0: any of this key's codes will do.
-        const int d = 64 * j + 16 * grp;
-        kw[sub][j] = *reinterpret_cast<const uint4v *>(kp + (d < c.dim ? d : 0));
-      }
-      // Past head_dim lie rows of O^T that are not stored.
-      const int d = VD * col < c.dim ? VD * col : 0;
+      for (int j = 0; j < KS; ++j) kw[sub][j] = *reinterpret_cast<const uint4v *>(k + koff[j]);
+    }
+  };
+  const auto load_values = [&](int step) {
+#pragma unroll
+    for (int sub = 0; sub < 4; ++sub) {
+      const uint8_t *v = c.codes[1] + where(step, sub);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t *w = reinterpret_cast<const uint32_t *>(vp + i * c.dim + d);
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(v + (voff + i * dim));
 #pragma unroll
         for (int x = 0; x < VW; ++x) vw[sub][i][x] = w[x];
       }
-      const float sk = c.scales[0][at], sv = c.scales[1][at];
-      ks[sub] = good ? sk : 1.0f;
-      ev[sub] = good ? Log2Scale(sv) : -kInf;
-      inv[sub] = good ? 1.0f / sv : 0.0f;
     }
-
+  };
+  const auto load_scales = [&](uint32_t page) {
+    const int64_t at = static_cast<int64_t>(page != ~0u ? page : 0) * c.heads + h;
+    sk = c.scales[0][at];
+    sv = c.scales[1][at];
+  };
+  int step = split * each + wave;
+  uint32_t page = ~0u, next = ~0u;  // this lane's group's, of this and the next tile
+  if (step < tile1) {
+    page = find(step);
+    next = find(step + kWaves);
+    spread(page);
+    load_keys(step);
+    load_scales(page);
+    load_values(step);
+  }
+  for (; step < tile1; step += kWaves) {
+    const int t0 = reach.begin + kTile * step;
     floatx4v acc[MT][4];
 #pragma unroll
     for (int sub = 0; sub < 4; ++sub) {
@@ -316,68 +354,92 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
                                                                    acc[t][sub], 0, 0, 0);
         }
     }
+    // The scales' part in scores and weights, made by the lanes that hold them.
+    const bool there = page != ~0u;
+    const float lane_ks = there ? sk : 1.0f, lane_ev = there ? Log2Scale(sv) : -kInf;
+    const float lane_inv = there ? 1.0f / sv : 0.0f;
+    const bool whole = __all(there);
+    float ks[4], ev[4], inv[4];
+#pragma unroll
+    for (int sub = 0; sub < 4; ++sub) {
+      ks[sub] = FromLane(lane_ks, 16 * sub);
+      ev[sub] = FromLane(lane_ev, 16 * sub);
+      inv[sub] = FromLane(lane_inv, 16 * sub);
+    }
+    const bool more = step + kWaves < tile1;
+    if (more) {
+      spread(next);
+      load_keys(step + kWaves);
+      load_scales(next);
+    }
+    page = next;
+    // Before the next values: loads end in their order, and the wait for this one must
+    // not be one for those.
+    if (more) next = find(step + 2 * kWaves);
 
+    // Some row does not see some token.
+    const bool edge = !whole || t0 + kTile - 1 > reach.pmin || t0 + kTile > reach.end ||
+                      (a.window > 0 && t0 <= reach.pmax - a.window);
     half8v p[MT][2][kTerms];
-    bool grew = false;
-    float alpha[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      float top = -kInf, scale[4];
+      if (edge) {
+        const int hi = min(pos[t], reach.end - 1) - (t0 + 4 * grp);
+        const int lo = a.window > 0 ? pos[t] - a.window - (t0 + 4 * grp) : -64;
 #pragma unroll
-      for (int sub = 0; sub < 4; ++sub) {
-        scale[sub] = ScoreScale(cq[t], ks[sub]);
-        if (edge) {
+        for (int sub = 0; sub < 4; ++sub)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int tok = t0 + 16 * sub + 4 * grp + i;
-            const bool seen = tok <= pos[t] && tok < reach.end && ev[sub] != -kInf &&
-                              (a.window == 0 || tok > pos[t] - a.window);
+            const int tok = 16 * sub + i;
+            const bool seen = tok <= hi && tok > lo && ev[sub] != -kInf;
             acc[t][sub][i] = seen ? acc[t][sub][i] : -kInf;
           }
-        }
-        const float most = fmaxf(fmaxf(acc[t][sub][0], acc[t][sub][1]),
-                                 fmaxf(acc[t][sub][2], acc[t][sub][3]));
-        top = fmaxf(top, fmaf(most, scale[sub], ev[sub]));
+        __asm__ volatile("");  // a branch, not selects
       }
-      top = fmaxf(m[t], MaxGroups(top));
-      const float use = top == -kInf ? 0.0f : top;
-      alpha[t] = Exp2(m[t] - use);
-      grew |= top != m[t];
-      m[t] = top;
-      float sum = 0.0f;
+      float scale[4], part[4];
 #pragma unroll
-      for (int sub = 0; sub < 4; ++sub) {
-        float part = 0.0f;
+      for (int sub = 0; sub < 4; ++sub) scale[sub] = ScoreScale(cq[t], ks[sub]);
+      const auto make = [&](float top) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float w = Exp2(fmaf(acc[t][sub][i], scale[sub], ev[sub] - use + kShift));
-          part += w;
-          const _Float16 hi = static_cast<_Float16>(w);
-          p[t][sub >> 1][0][4 * (sub & 1) + i] = hi;
-          if constexpr (kTerms == 2)
-            p[t][sub >> 1][1][4 * (sub & 1) + i] =
-                static_cast<_Float16>(w - static_cast<float>(hi));
+        for (int sub = 0; sub < 4; ++sub) {
+          const float add = ev[sub] - top + kShift;
+          part[sub] = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float w = Exp2(fmaf(acc[t][sub][i], scale[sub], add));
+            part[sub] += w;
+            const _Float16 hi = static_cast<_Float16>(w);
+            p[t][sub >> 1][0][4 * (sub & 1) + i] = hi;
+            if constexpr (kTerms == 2)
+              p[t][sub >> 1][1][4 * (sub & 1) + i] =
+                  static_cast<_Float16>(w - static_cast<float>(hi));
+          }
         }
-        sum = fmaf(part, inv[sub], sum);
+      };
+      make(m[t]);
+      if (__any(!Fits(part))) {
+        float top = -kInf;
+#pragma unroll
+        for (int sub = 0; sub < 4; ++sub) {
+          const float most = fmaxf(fmaxf(acc[t][sub][0], acc[t][sub][1]),
+                                   fmaxf(acc[t][sub][2], acc[t][sub][3]));
+          top = fmaxf(top, fmaf(most, scale[sub], ev[sub]));
+        }
+        top = fmaxf(m[t], MaxGroups(top) + 1.0f);
+        const float use = top == -kInf ? 0.0f : top;
+        const float alpha = Exp2(m[t] - use);
+        m[t] = top;
+        make(use);
+        l[t] *= alpha;
+#pragma unroll
+        for (int d = 0; d < VD; ++d) o[t][d] *= alpha;
       }
-      l[t] = fmaf(l[t], alpha[t], sum);
-    }
-    if (__any(grew)) {
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int d = 0; d < VD; ++d) o[t][d] *= alpha[t];
+      for (int sub = 0; sub < 4; ++sub) l[t] = fmaf(part[sub], inv[sub], l[t]);
     }
 
 #pragma unroll
     for (int pair = 0; pair < 2; ++pair) {
-      uint32_t w[2][4][VW];
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int y = 0; y < VW; ++y) w[x][i][y] = vw[2 * pair + x][i][y];
       if (edge) {
         // A weight of 0 does not undo a NaN: values of tokens that no row sees are
         // cleared, and NaN values that some rows may see are kept apart.
@@ -391,8 +453,8 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
                               (a.window == 0 || tok > reach.pmin - a.window);
 #pragma unroll
             for (int y = 0; y < VW; ++y) {
-              w[x][i][y] = seen ? w[x][i][y] : 0u;
-              nan |= NanTops(w[x][i][y]);
+              vw[2 * pair + x][i][y] = seen ? vw[2 * pair + x][i][y] : 0u;
+              nan |= NanTops(vw[2 * pair + x][i][y]);
             }
           }
         if (__any(nan != 0)) {
@@ -402,12 +464,10 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int tok = t0 + 32 * pair + 16 * x + 4 * grp + i;
-                seen[t][4 * x + i] = acc[t][2 * pair + x][i] == -kInf || tok > pos[t]
+              for (int i = 0; i < 4; ++i)
+                seen[t][4 * x + i] = acc[t][2 * pair + x][i] == -kInf
                                          ? static_cast<_Float16>(0.0f)
                                          : static_cast<_Float16>(1.0f);
-              }
 #pragma unroll
           for (int y = 0; y < VW; ++y) {
             uint32_t flag[2][4], turned[2][4];
@@ -415,8 +475,9 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
             for (int x = 0; x < 2; ++x) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const uint32_t bytes = (NanTops(w[x][i][y]) >> 7) * 0xFFu;
-                w[x][i][y] &= ~bytes;
+                uint32_t &w = vw[2 * pair + x][i][y];
+                const uint32_t bytes = (NanTops(w) >> 7) * 0xFFu;
+                w &= ~bytes;
                 flag[x][i] = bytes & 0x38383838u;  // 1.0
               }
               Transpose4(flag[x], turned[x]);
@@ -441,7 +502,8 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
         uint32_t turned[2][4];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const uint32_t in[4] = {w[x][0][y], w[x][1][y], w[x][2][y], w[x][3][y]};
+          const uint32_t in[4] = {vw[2 * pair + x][0][y], vw[2 * pair + x][1][y],
+                                  vw[2 * pair + x][2][y], vw[2 * pair + x][3][y]};
           Transpose4(in, turned[x]);
         }
 #pragma unroll
@@ -456,6 +518,7 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
         }
       }
     }
+    if (more) load_values(step + kWaves);
   }
 
   // The wavefronts' parts, one tile of 16 rows at a time. A lane holds values VD (4 grp
@@ -818,16 +881,11 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
         float y[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = sc[j >> 1][8 * (j & 1) + e];
-        part[j] = Weights<kTerms>(y, scale[j], in[j].y - top + kTileShift, p[j]);
+        part[j] = Weights<kTerms>(y, scale[j], in[j].y - top + kShift, p[j]);
       }
     };
-    // The maximum that earlier tiles left does, as long as no eight weights add up to what
-    // fp16 cannot hold (a NaN fails this too, as at the first tile); else the
-    // tile's own is found, and a factor of 2 left above it.
     make(m);
-    const bool fits = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) <= kMost &&
-                      part[0] + part[1] + part[2] + part[3] < kInf;
-    if (__any(!fits)) {
+    if (__any(!Fits(part))) {
       __asm__ volatile("");
       float top = -kInf;
 #pragma unroll
@@ -1005,15 +1063,16 @@ Plan PlanOf(const Cache &c, const Batch &b, int32_t q_heads, int32_t x_type) {
   const int64_t rows = static_cast<int64_t>(b.max_tokens) * (q_heads / c.heads);
   const bool fp32 = x_type == MNB_TYPE_FLOAT;
   int64_t per = 16, least = kWaves, goal = 3 * 256;
-  if (rows > 32 && c.dim <= 128) {
+  if (rows > (fp32 ? 32 : 64) && c.dim <= 128) {
     p.waves = rows > 128 && !fp32 ? 8 : 4;
     per = 32 * p.waves;
     goal = 256 * (8 / p.waves);
     least = 8;
   } else if (rows > 16 && (c.dim <= 128 || !fp32)) {
     // Two tiles of fp32 queries 256 wide leave no registers for the keys.
-    p.mt = 2;
-    per = 32;
+    p.mt = fp32 || c.dim > 128 ? 2 : static_cast<int>(std::min<int64_t>(4, CeilDiv(rows, 16)));
+    per = 16 * p.mt;
+    least = kWaves * p.mt;  // a part's sums are as large as its keys
   }
   p.row_tiles = static_cast<int>(CeilDiv(rows, per));
   const int64_t groups = static_cast<int64_t>(b.sequences) * c.heads * p.row_tiles;
@@ -1044,6 +1103,10 @@ hipError_t SplitDim(const Attend &a, const Work &w, const Plan &p, hipStream_t s
     if constexpr (Terms<T>() == 1)
       if (p.waves == 8) return Tile<T, DP, 8>(a, w, p, s);
     if (p.waves == 4) return Tile<T, DP, 4>(a, w, p, s);
+  }
+  if constexpr (DP <= 128 && Terms<T>() == 1) {
+    if (p.mt == 3) return Split<T, DP, 3>(a, w, p, s);
+    if (p.mt == 4) return Split<T, DP, 4>(a, w, p, s);
   }
   if constexpr (DP <= 128 || Terms<T>() == 1)
     if (p.mt == 2) return Split<T, DP, 2>(a, w, p, s);

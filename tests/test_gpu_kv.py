@@ -352,9 +352,13 @@ def test_rows_of_no_sequence(pkg, cuda, split):
     fresh = cache.attend(Q, *args, starts=_i32([2, 5, 7], cuda), max_tokens=3)
     assert (out[:2] == 7).all() and (out[7:] == 7).all()
     assert (fresh[:2] == 0).all() and (fresh[7:] == 0).all()
-    assert torch.equal(out[2:7], fresh[2:7])
     alone = cache.attend(Q[2:5], args[0][:1], args[1][:1])
-    assert ((alone.float() - out[2:5].float()).abs() <= 2.0 ** -6 * alone.float().abs().amax()).all()
+    # Other bounds may choose another kernel: each result is off by half a step (2^-8) of its
+    # value, and by 2^-10 of the largest value for its weights' rounding (2^-11) and sums.
+    most = _values(cache.v, cache.v_scales).abs().max().item()
+    for a, b in ((out[2:7], fresh[2:7]), (out[2:5], alone)):
+        a, b = a.float(), b.float()
+        assert ((a - b).abs() <= 2.0 ** -8 * (a.abs() + b.abs()) + 2.0 ** -9 * most).all()
 
 
 # ---- append -----------------------------------------------------------------
