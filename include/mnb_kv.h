@@ -82,7 +82,7 @@ int mnb_kv_workspace_bytes(const mnb_kv_cache *cache, const mnb_kv_batch *batch,
                            int32_t x_type, size_t *bytes);
 
 /* Y [tokens, heads, head_dim], dense, of Q's type, aligned to 16 bytes: for row i of sequence b
- * at position p and query head h, the softmax over the keys t <= p (and t > p -
+ * at position p and query head h (tokens * heads at most 2^27), the softmax over the keys t <= p (and t > p -
  * window, where window > 0; beyond 2^30 it counts as 0) of scale * q . k_t, times v; heads is a multiple of
  * kv_heads, and query heads h use cache head h / (heads / kv_heads). A row that
  * sees no key, or only scores of -inf, is 0; unseen keys and values leave no trace, NaN

@@ -189,15 +189,40 @@ __device__ __forceinline__ Reach ReachOf(const Span &span, int rows_first, int r
   return r;
 }
 
-// A part of a row: parts[split][row][dim] sums, ml[split][row] = {maximum, sum}.
-struct Work {
-  float *parts;
+// Parts of rows, of `splits` shares of the keys: sums [dim], maximum and sum of weights.
+struct Parts {
+  float *sums;
   float2 *ml;
   int splits;
 };
 
+// Sequences with at most `few` rows to a cache head are AttendSplitKernel's, whose parts
+// lie [split][sequence][few_tokens][q_heads]; the others AttendTileKernel's, [split][token]
+// [q_heads].
+struct Work {
+  Parts part, tile_part;
+  int64_t few;
+  int32_t few_tokens;
+};
+
+// Rows of a sequence to a cache head.
+__device__ __forceinline__ int64_t RowsOf(const Attend &a, const Span &span) {
+  return static_cast<int64_t>(min(span.count, a.batch.max_tokens)) * (a.q_heads / a.cache.heads);
+}
+
+// A row's place among the parts, of split 0, and the distance to the next split's.
+__device__ __forceinline__ int64_t PartOf(const Attend &a, const Work &w, int s, int i, int head) {
+  return (static_cast<int64_t>(s) * w.few_tokens + i) * a.q_heads + head;
+}
+__device__ __forceinline__ int64_t PartStep(const Attend &a, const Work &w) {
+  return static_cast<int64_t>(a.batch.sequences) * w.few_tokens * a.q_heads;
+}
+__device__ __forceinline__ int64_t TilePartStep(const Attend &a) {
+  return static_cast<int64_t>(a.batch.tokens) * a.q_heads;
+}
+
 // DP: head_dim rounded up to 64, 128 or 256; MT: tiles of 16 queries.
-// grid (splits, heads x row tiles, sequences). A row is a token's query head of
+// grid (heads x row tiles x splits, sequences). A row is a token's query head of
 // this cache head: row r is token r / group, head r % group.
 template <typename T, int DP, int MT>
 __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work work, int row_tiles) {
@@ -206,20 +231,21 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
   constexpr int VD = DP / 16;      // values of a token that a lane holds, tiles of O^T
   constexpr int VW = VD / 4;       // the same in words
   const Cache &c = a.cache;
-  const int s = blockIdx.z, split = blockIdx.x;
-  const int h = blockIdx.y / row_tiles, tile = blockIdx.y - h * row_tiles;
+  const int s = blockIdx.y, split = blockIdx.x % work.part.splits;
+  const int h = blockIdx.x / work.part.splits / row_tiles;
+  const int tile = blockIdx.x / work.part.splits - h * row_tiles;
   const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Span span = SpanOf(a.batch, s, c.page_shift);
   const int group = a.q_heads / c.heads;
-  const int64_t rows = static_cast<int64_t>(span.count) * group;
+  const int64_t rows = RowsOf(a, span);
   const int64_t row0 = static_cast<int64_t>(tile) * (16 * MT);
-  if (row0 >= rows) return;
+  if (row0 >= rows || rows > work.few) return;
   const int64_t row1 = min(row0 + 16 * MT, rows) - 1;
   const Reach reach = ReachOf(span, static_cast<int>(row0 / group), static_cast<int>(row1 / group),
                               a.window);
   const int tiles = reach.end > reach.begin ? (reach.end - reach.begin + kTile - 1) / kTile : 0;
-  const int each = (tiles + work.splits - 1) / work.splits;
+  const int each = (tiles + work.part.splits - 1) / work.part.splits;
   const int tile1 = min(tiles, (split + 1) * each);
 
   // Queries. A lane's values for the two MFMAs of piece j are the halves of 16
@@ -561,15 +587,15 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
     }
     const int i = static_cast<int>(row / group), g = static_cast<int>(row - static_cast<int64_t>(i) * group);
     const int64_t at = static_cast<int64_t>(span.row + i) * a.q_heads + h * group + g;
-    if (work.splits == 1) {
+    if (work.part.splits == 1) {
       const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
       T *y = static_cast<T *>(a.y) + at * c.dim + d0;
 #pragma unroll
       for (int d = 0; d < VD; ++d) y[d] = static_cast<T>(v[d] * by);
     } else {
-      const int64_t part = static_cast<int64_t>(split) * a.batch.tokens * a.q_heads + at;
-      if (d0 == 0) work.ml[part] = make_float2(top, sum);
-      float *y = work.parts + part * c.dim + d0;
+      const int64_t part = PartOf(a, work, s, i, h * group + g) + split * PartStep(a, work);
+      if (d0 == 0) work.part.ml[part] = make_float2(top, sum);
+      float *y = work.part.sums + part * c.dim + d0;
       if (sum != 0.0f)
 #pragma unroll
         for (int d = 0; d < VD; ++d) y[d] = v[d];
@@ -582,9 +608,9 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
 // 32 x 32 halve what a product reads of LDS; V is laid out transposed, in the order
 // of tokens that a lane's weights have. The next tile's codes are in registers
 // while a tile is multiplied, and are widened into the other half of LDS.
-// grid (heads, row tiles x splits, sequences): heads lie next to each other, so that a head's
-// workgroups share an XCD's cache where there are eight; late rows, which see the
-// most keys, come first.
+// grid (row tiles x splits x heads, sequences): heads lie next to each other, so that a
+// head's workgroups share an XCD's cache where there are eight; late rows, which see
+// the most keys, come first.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work, int row_tiles) {
   constexpr int kTerms = Terms<T>();
@@ -595,20 +621,21 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
   constexpr int kEach = (kUnits + kThreadsT - 1) / kThreadsT;
   constexpr int kMask = DP / 8 < 16 ? DP / 8 - 1 : 15;
   const Cache &c = a.cache;
-  const int s = blockIdx.z, h = blockIdx.x;
-  const int split = blockIdx.y % work.splits, tile = row_tiles - 1 - blockIdx.y / work.splits;
+  const int s = blockIdx.y, h = blockIdx.x % a.cache.heads, rest = blockIdx.x / a.cache.heads;
+  const int split = rest % work.tile_part.splits;
+  const int tile = row_tiles - 1 - rest / work.tile_part.splits;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Span span = SpanOf(a.batch, s, c.page_shift);
   const int group = a.q_heads / c.heads;
-  const int64_t rows = static_cast<int64_t>(span.count) * group;
+  const int64_t rows = RowsOf(a, span);
   const int64_t row0 = static_cast<int64_t>(tile) * (32 * NW);
-  if (row0 >= rows) return;
+  if (row0 >= rows || rows <= work.few) return;
   const int64_t row1 = min(row0 + 32 * NW, rows) - 1;
   const Reach reach = ReachOf(span, static_cast<int>(row0 / group), static_cast<int>(row1 / group),
                               a.window);
   const int tiles = reach.end > reach.begin ? (reach.end - reach.begin + kTile - 1) / kTile : 0;
-  const int each = (tiles + work.splits - 1) / work.splits;
+  const int each = (tiles + work.tile_part.splits - 1) / work.tile_part.splits;
   const int tile0 = split * each, tile1 = min(tiles, tile0 + each);
 
   // Two tiles of keys, [token][unit ^ token], and two of values, [d][unit ^ (d / 4) ^ d],
@@ -976,17 +1003,17 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
   if (!there) return;
   l += __shfl_xor(l, 32);
   const int64_t at = static_cast<int64_t>(span.row + i0) * a.q_heads + h * group + g;
-  const float by = work.splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-  const int64_t part = static_cast<int64_t>(split) * a.batch.tokens * a.q_heads + at;
-  if (work.splits > 1 && half == 0) work.ml[part] = make_float2(m, l);
+  const float by = work.tile_part.splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+  const int64_t part = split * TilePartStep(a) + at;
+  if (work.tile_part.splits > 1 && half == 0) work.tile_part.ml[part] = make_float2(m, l);
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int e = 0; e < 16; e += 4) {
       const int d0 = 32 * d + 8 * (e >> 2) + 4 * half;
       if (d0 >= c.dim) continue;
-      if (work.splits > 1) {
-        *reinterpret_cast<floatx4v *>(work.parts + part * c.dim + d0) =
+      if (work.tile_part.splits > 1) {
+        *reinterpret_cast<floatx4v *>(work.tile_part.sums + part * c.dim + d0) =
             floatx4v{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
       } else {
         typedef T Vec __attribute__((ext_vector_type(4)));
@@ -999,19 +1026,39 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
 
 // Joins the splits of a row. PER threads to a row, four values of it each; where one
 // row has more threads than its width, they take every n-th split. A workgroup
-// per row (PER 256) hides the reads of many splits, a wavefront (PER 64) is enough for few.
+// per row (PER 256) hides the reads of many splits (32 rows of 32 splits: 28 us with a
+// wavefront, 4.6 with four), a wavefront (PER 64) is enough for few splits or many rows.
 template <typename T, int PER>
-__global__ __launch_bounds__(kThreads) void JoinKernel(Attend a, Work work) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * (kThreads / PER) + threadIdx.x / PER;
-  const Span span = SpanOf(a.batch, blockIdx.y, a.cache.page_shift);
-  if (i >= static_cast<int64_t>(span.count) * a.q_heads) return;  // PER 256: all threads
-  const int64_t row = static_cast<int64_t>(span.row) * a.q_heads + i;
-  const int64_t step = static_cast<int64_t>(a.batch.tokens) * a.q_heads;
+__global__ __launch_bounds__(kThreads) void JoinKernel(Attend a, Work work, int64_t row0) {
+  const int64_t row = row0 + static_cast<int64_t>(blockIdx.x) * (kThreads / PER) +
+                      __builtin_amdgcn_readfirstlane(threadIdx.x / PER);
+  const int token = static_cast<int>(row / a.q_heads);
+  if (token >= a.batch.tokens) return;  // PER 256: all threads
+  int s = 0;
+  if (a.batch.starts == nullptr) {
+    s = token / a.batch.each;
+  } else {  // the last sequence that starts at this token or before
+    for (int to = a.batch.sequences; to - s > 1;) {
+      const int mid = (s + to) / 2;
+      if (a.batch.starts[mid] <= token) s = mid;
+      else to = mid;
+    }
+  }
+  const Span span = SpanOf(a.batch, s, a.cache.page_shift);
+  const int i = token - span.row;
+  if (i < 0 || i >= min(span.count, a.batch.max_tokens)) return;
+  const bool tile = RowsOf(a, span) > work.few;
+  const Parts &parts = tile ? work.tile_part : work.part;
+  const int splits = parts.splits;
+  if (splits == 1) return;  // written where it was computed
+  const int head = static_cast<int>(row - static_cast<int64_t>(token) * a.q_heads);
+  const int64_t at = tile ? row : PartOf(a, work, s, i, head);
+  const int64_t step = tile ? TilePartStep(a) : PartStep(a, work);
   const int dim = a.cache.dim, lane = threadIdx.x & 63;
   const int wide = dim <= 64 ? 16 : dim <= 128 ? 32 : 64;  // threads that hold a row
   const int t = threadIdx.x % PER, first = t / wide, stride = PER / wide, d = 4 * (t % wide);
   // Every wavefront finds the maximum: a lane per split, 64 at most.
-  float2 ml = lane < work.splits ? work.ml[lane * step + row] : make_float2(-kInf, 0.0f);
+  float2 ml = lane < splits ? parts.ml[lane * step + at] : make_float2(-kInf, 0.0f);
   float top = ml.x;
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
@@ -1021,12 +1068,12 @@ __global__ __launch_bounds__(kThreads) void JoinKernel(Attend a, Work work) {
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
   floatx4v v = {0.0f, 0.0f, 0.0f, 0.0f};
-  const float *part = work.parts + row * dim + (d < dim ? d : 0);
-  for (int s0 = 0; s0 < work.splits; s0 += stride) {
-    const int s = s0 + first;
-    const float w = __shfl(by, s & 63);
-    if (s < work.splits && w != 0.0f) {  // else it saw nothing, and wrote nothing
-      const floatx4v p = *reinterpret_cast<const floatx4v *>(part + s * step * dim);
+  const float *part = parts.sums + at * dim + (d < dim ? d : 0);
+  for (int s0 = 0; s0 < splits; s0 += stride) {
+    const int i0 = s0 + first;
+    const float w = __shfl(by, i0 & 63);
+    if (i0 < splits && w != 0.0f) {  // else it saw nothing, and wrote nothing
+      const floatx4v p = *reinterpret_cast<const floatx4v *>(part + i0 * step * dim);
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = fmaf(p[e], w, v[e]);
     }
@@ -1051,40 +1098,60 @@ __global__ __launch_bounds__(kThreads) void JoinKernel(Attend a, Work work) {
   for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(v[e] * over);
 }
 
-// How a call is launched.
+// How a call is launched: for sequences of at most `few` rows to a cache head
+// AttendSplitKernel with mt tiles of 16, for others AttendTileKernel with `waves`
+// wavefronts. Of sequences that all have as many rows only one of the two has any (mt or
+// waves is 0), ragged ones may have both.
 struct Plan {
-  int mt;      // AttendSplitKernel's tiles of 16 rows, or
-  int waves;   // AttendTileKernel's wavefronts; 0: the other
-  int row_tiles, splits;
+  int mt = 0, row_tiles = 0, splits = 1;
+  int waves = 0, tile_row_tiles = 0, tile_splits = 1;
+  int64_t few = 0;
+  int32_t few_tokens = 0;
 };
 
 Plan PlanOf(const Cache &c, const Batch &b, int32_t q_heads, int32_t x_type) {
-  Plan p{1, 0, 1, 1};
-  const int64_t rows = static_cast<int64_t>(b.max_tokens) * (q_heads / c.heads);
-  const bool fp32 = x_type == MNB_TYPE_FLOAT;
-  int64_t per = 16, least = kWaves, goal = 3 * 256;
-  if (rows > (fp32 ? 32 : 64) && c.dim <= 128) {
+  Plan p;
+  const int64_t group = q_heads / c.heads, rows = b.max_tokens * group;
+  const bool fp32 = x_type == MNB_TYPE_FLOAT, tiles = c.dim <= 128;
+  // Two tiles of fp32 queries 256 wide leave no registers for the keys.
+  const int most_mt = fp32 ? (tiles ? 2 : 1) : tiles ? 4 : 2;
+  const int64_t key_tiles = CeilDiv(static_cast<int64_t>(b.width) << c.page_shift, kTile);
+  const auto parts = [&](int64_t groups, int64_t goal, int64_t least) {
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(64, key_tiles / least));
+    return static_cast<int>(std::min(most, std::max<int64_t>(1, goal / groups)));
+  };
+  int64_t few = rows;
+  if (tiles && rows > 16 * most_mt) {
+    // Where ragged sequences are long or short, the short ones are taken to be decoded.
+    p.few = few = b.starts == nullptr ? 0 : group <= 16 ? 16 : 32;
     p.waves = rows > 128 && !fp32 ? 8 : 4;
-    per = 32 * p.waves;
-    goal = 256 * (8 / p.waves);
-    least = 8;
-  } else if (rows > 16 && (c.dim <= 128 || !fp32)) {
-    // Two tiles of fp32 queries 256 wide leave no registers for the keys.
-    p.mt = fp32 || c.dim > 128 ? 2 : static_cast<int>(std::min<int64_t>(4, CeilDiv(rows, 16)));
-    per = 16 * p.mt;
-    least = kWaves * p.mt;  // a part's sums are as large as its keys
+    const int64_t per = 32 * p.waves;
+    p.tile_row_tiles = static_cast<int>(CeilDiv(rows, per));
+    const int64_t filled = b.starts == nullptr ? b.sequences * p.tile_row_tiles
+                                               : CeilDiv(b.tokens * group, per);
+    // One workgroup of eight wavefronts fits a CU, or two of four, or one for fp32. Four tiles
+    // at least are worth a part (32 to 128 tokens of one sequence over 4096: 25 to 33 us, 30 to
+    // 36 with eight, 27 to 32 with two); eight of fp32 (128 tokens: 39 us, 51 with four).
+    p.tile_splits = parts(filled * c.heads, fp32 || p.waves == 8 ? 256 : 512, fp32 ? 8 : 4);
+  } else {
+    p.few = INT64_MAX;
   }
-  p.row_tiles = static_cast<int>(CeilDiv(rows, per));
-  const int64_t groups = static_cast<int64_t>(b.sequences) * c.heads * p.row_tiles;
-  const int64_t tiles = CeilDiv(static_cast<int64_t>(b.width) << c.page_shift, kTile);
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(64, tiles / least));
-  p.splits = static_cast<int>(std::min(most, std::max<int64_t>(1, goal / groups)));
+  p.few_tokens = static_cast<int32_t>(few / group);
+  if (few > 0) {
+    p.mt = static_cast<int>(std::min<int64_t>(most_mt, CeilDiv(few, 16)));
+    p.row_tiles = static_cast<int>(CeilDiv(few, 16 * p.mt));
+    // Workgroups for three on each CU; a part's sums are as large as mt tiles of keys for
+    // each of its wavefronts.
+    p.splits = parts(static_cast<int64_t>(b.sequences) * c.heads * p.row_tiles, 3 * 256,
+                     kWaves * p.mt);
+  }
   return p;
 }
 
 template <typename T, int DP, int MT>
 hipError_t Split(const Attend &a, const Work &w, const Plan &p, hipStream_t s) {
-  const dim3 grid(p.splits, static_cast<unsigned>(a.cache.heads * p.row_tiles), a.batch.sequences);
+  const dim3 grid(static_cast<unsigned>(a.cache.heads) * p.row_tiles * p.splits,
+                  a.batch.sequences);
   hipLaunchKernelGGL((AttendSplitKernel<T, DP, MT>), grid, dim3(kThreads), 0, s, a, w,
                      p.row_tiles);
   return hipGetLastError();
@@ -1092,61 +1159,87 @@ hipError_t Split(const Attend &a, const Work &w, const Plan &p, hipStream_t s) {
 
 template <typename T, int DP, int NW>
 hipError_t Tile(const Attend &a, const Work &w, const Plan &p, hipStream_t s) {
-  const dim3 grid(a.cache.heads, static_cast<unsigned>(p.row_tiles * p.splits), a.batch.sequences);
-  hipLaunchKernelGGL((AttendTileKernel<T, DP, NW>), grid, dim3(64 * NW), 0, s, a, w, p.row_tiles);
+  const dim3 grid(static_cast<unsigned>(a.cache.heads) * p.tile_row_tiles * p.tile_splits,
+                  a.batch.sequences);
+  hipLaunchKernelGGL((AttendTileKernel<T, DP, NW>), grid, dim3(64 * NW), 0, s, a, w,
+                     p.tile_row_tiles);
   return hipGetLastError();
 }
 
 template <typename T, int DP>
-hipError_t SplitDim(const Attend &a, const Work &w, const Plan &p, hipStream_t s) {
+hipError_t LaunchDim(const Attend &a, const Work &w, const Plan &p, hipStream_t s) {
+  hipError_t e = hipSuccess;
   if constexpr (DP <= 128) {
+    if (p.waves == 4) e = Tile<T, DP, 4>(a, w, p, s);
     if constexpr (Terms<T>() == 1)
-      if (p.waves == 8) return Tile<T, DP, 8>(a, w, p, s);
-    if (p.waves == 4) return Tile<T, DP, 4>(a, w, p, s);
+      if (p.waves == 8) e = Tile<T, DP, 8>(a, w, p, s);
   }
+  if (e != hipSuccess) return e;
   if constexpr (DP <= 128 && Terms<T>() == 1) {
     if (p.mt == 3) return Split<T, DP, 3>(a, w, p, s);
     if (p.mt == 4) return Split<T, DP, 4>(a, w, p, s);
   }
   if constexpr (DP <= 128 || Terms<T>() == 1)
     if (p.mt == 2) return Split<T, DP, 2>(a, w, p, s);
-  return Split<T, DP, 1>(a, w, p, s);
+  if (p.mt == 1) return Split<T, DP, 1>(a, w, p, s);
+  return e;
 }
 
-size_t Round256(size_t v) { return (v + 255) / 256 * 256; }
+// Where a call's parts lie in the workspace.
+struct Layout {
+  size_t ml = 0, tile_sums = 0, tile_ml = 0, total = 0;
+};
 
-size_t PartBytes(const Cache &c, const Batch &b, int32_t q_heads, int splits) {
-  return Round256(sizeof(float) * splits * b.tokens * q_heads * c.dim);
+Layout LayoutOf(const Cache &c, const Batch &b, int32_t q_heads, const Plan &p) {
+  Layout l;
+  const auto round = [](size_t v) { return (v + 255) / 256 * 256; };
+  const auto rows = [&](int splits, size_t tokens) {
+    return splits > 1 ? static_cast<size_t>(splits) * tokens * q_heads : 0;
+  };
+  const size_t few = rows(p.splits, static_cast<size_t>(b.sequences) * p.few_tokens);
+  const size_t many = rows(p.tile_splits, b.tokens);
+  l.ml = round(few * c.dim * sizeof(float));
+  l.tile_sums = l.ml + round(few * sizeof(float2));
+  l.tile_ml = l.tile_sums + round(many * c.dim * sizeof(float));
+  l.total = l.tile_ml + round(many * sizeof(float2));
+  return l;
 }
 
 template <typename T>
 hipError_t LaunchT(const Attend &a, int32_t x_type, void *work, hipStream_t s) {
   const Plan p = PlanOf(a.cache, a.batch, a.q_heads, x_type);
-  const Work w{static_cast<float *>(work),
-               reinterpret_cast<float2 *>(static_cast<char *>(work) +
-                                          PartBytes(a.cache, a.batch, a.q_heads, p.splits)),
-               p.splits};
-  hipError_t e = a.cache.dim <= 64    ? SplitDim<T, 64>(a, w, p, s)
-                 : a.cache.dim <= 128 ? SplitDim<T, 128>(a, w, p, s)
-                                      : SplitDim<T, 256>(a, w, p, s);
-  if (e != hipSuccess || p.splits == 1) return e;
-  const int64_t rows = static_cast<int64_t>(a.batch.max_tokens) * a.q_heads;
-  if (p.splits > 8) {
-    const dim3 grid(static_cast<unsigned>(rows), a.batch.sequences);
-    hipLaunchKernelGGL((JoinKernel<T, kThreads>), grid, dim3(kThreads), 0, s, a, w);
-  } else {
-    const dim3 grid(static_cast<unsigned>(CeilDiv(rows, kWaves)), a.batch.sequences);
-    hipLaunchKernelGGL((JoinKernel<T, 64>), grid, dim3(kThreads), 0, s, a, w);
+  const Layout l = LayoutOf(a.cache, a.batch, a.q_heads, p);
+  char *const at = static_cast<char *>(work);
+  const Work w{{reinterpret_cast<float *>(at), reinterpret_cast<float2 *>(at + l.ml), p.splits},
+               {reinterpret_cast<float *>(at + l.tile_sums),
+                reinterpret_cast<float2 *>(at + l.tile_ml), p.tile_splits},
+               p.few,
+               p.few_tokens};
+  const hipError_t e = a.cache.dim <= 64    ? LaunchDim<T, 64>(a, w, p, s)
+                       : a.cache.dim <= 128 ? LaunchDim<T, 128>(a, w, p, s)
+                                            : LaunchDim<T, 256>(a, w, p, s);
+  const int splits = std::max(p.splits, p.tile_splits);
+  if (e != hipSuccess || splits == 1) return e;
+  // Rows at a time, so that a grid's threads stay below 2^32.
+  const int64_t rows = static_cast<int64_t>(a.batch.tokens) * a.q_heads, most = int64_t{1} << 23;
+  for (int64_t r = 0; r < rows; r += most) {
+    const int64_t n = std::min(most, rows - r);
+    if (splits > 8 && rows <= 1024)
+      hipLaunchKernelGGL((JoinKernel<T, kThreads>), dim3(static_cast<unsigned>(n)), dim3(kThreads),
+                         0, s, a, w, r);
+    else
+      hipLaunchKernelGGL((JoinKernel<T, 64>), dim3(static_cast<unsigned>(CeilDiv(n, kWaves))),
+                         dim3(kThreads), 0, s, a, w, r);
+    const hipError_t j = hipGetLastError();
+    if (j != hipSuccess) return j;
   }
-  return hipGetLastError();
+  return hipSuccess;
 }
 
 } // namespace
 
 size_t AttendWorkBytes(const Cache &c, const Batch &b, int32_t q_heads, int32_t x_type) {
-  const Plan p = PlanOf(c, b, q_heads, x_type);
-  if (p.splits == 1) return 0;
-  return PartBytes(c, b, q_heads, p.splits) + sizeof(float2) * p.splits * b.tokens * q_heads;
+  return LayoutOf(c, b, q_heads, PlanOf(c, b, q_heads, x_type)).total;
 }
 
 hipError_t LaunchAttend(const Attend &a, int32_t x_type, void *work, hipStream_t s) {

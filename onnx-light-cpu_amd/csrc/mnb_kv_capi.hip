@@ -69,8 +69,9 @@ int CheckRows(const mnb_kv_rows *r, int64_t dim, int32_t x_type, Rows *rows) {
   return MNB_OK;
 }
 
-int CheckHeads(const mnb_kv_cache *c, int32_t heads) {
+int CheckHeads(const mnb_kv_cache *c, const mnb_kv_batch *b, int32_t heads) {
   if (heads < 1 || heads > (1 << 16) || heads % c->kv_heads != 0) return MNB_ERR_BAD_SHAPE;
+  if (b->tokens * heads > int64_t{1} << 27) return MNB_ERR_BAD_SHAPE;  // a grid's threads
   return MNB_OK;
 }
 
@@ -117,7 +118,7 @@ int mnb_kv_workspace_bytes(const mnb_kv_cache *cache, const mnb_kv_batch *batch,
   int st = CheckShape(cache, batch, &c, &b);
   if (st != MNB_OK) return st;
   if (!FloatType(x_type)) return MNB_ERR_BAD_ATTRIBUTE;
-  if ((st = CheckHeads(cache, heads)) != MNB_OK) return st;
+  if ((st = CheckHeads(cache, batch, heads)) != MNB_OK) return st;
   *bytes = b.sequences == 0 || b.tokens == 0 ? 0 : AttendWorkBytes(c, b, heads, x_type);
   return MNB_OK;
 }
@@ -130,7 +131,7 @@ int mnb_kv_attend(const mnb_kv_cache *cache, const mnb_kv_batch *batch, int32_t 
   if (st != MNB_OK) return st;
   if (!FloatType(x_type) || !(scale == scale) || scale - scale != 0.0f || window < 0)
     return MNB_ERR_BAD_ATTRIBUTE;
-  if ((st = CheckHeads(cache, heads)) != MNB_OK) return st;
+  if ((st = CheckHeads(cache, batch, heads)) != MNB_OK) return st;
   if (a.batch.sequences == 0 || a.batch.tokens == 0) return MNB_OK;
   if ((st = CheckPointers(cache, batch)) != MNB_OK ||
       (st = CheckRows(q, a.cache.dim, x_type, &a.q)) != MNB_OK)

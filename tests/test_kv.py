@@ -71,7 +71,8 @@ def test_pointers_and_strides(pkg, lib, change, status):
 
 
 @pytest.mark.parametrize("change,status", [
-    ({"heads": 0}, SHAPE), ({"heads": 3}, SHAPE), ({"heads": (1 << 16) + 2}, SHAPE)])
+    ({"heads": 0}, SHAPE), ({"heads": 3}, SHAPE), ({"heads": (1 << 16) + 2}, SHAPE),
+    ({"heads": 18, "batch": {"tokens": 1 << 23}}, SHAPE)])
 def test_heads(pkg, lib, change, status):
     bad = dict(change, cache={"k": None})
     assert _call(pkg, lib, **bad)[1:] == (status, status)
