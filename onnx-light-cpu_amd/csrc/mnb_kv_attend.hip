@@ -1069,13 +1069,19 @@ __global__ __launch_bounds__(kThreads) void JoinKernel(Attend a, Work work, int6
   for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
   floatx4v v = {0.0f, 0.0f, 0.0f, 0.0f};
   const float *part = parts.sums + at * dim + (d < dim ? d : 0);
-  for (int s0 = 0; s0 < splits; s0 += stride) {
-    const int i0 = s0 + first;
-    const float w = __shfl(by, i0 & 63);
-    if (i0 < splits && w != 0.0f) {  // else it saw nothing, and wrote nothing
-      const floatx4v p = *reinterpret_cast<const floatx4v *>(part + i0 * step * dim);
+  for (int s0 = 0; s0 < splits; s0 += 4 * stride) {
+    floatx4v p[4];  // asked for before it is known which splits saw anything
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = fmaf(p[e], w, v[e]);
+    for (int x = 0; x < 4; ++x)
+      p[x] = *reinterpret_cast<const floatx4v *>(
+          part + min(s0 + x * stride + first, splits - 1) * step * dim);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int i0 = s0 + x * stride + first;
+      const float w = __shfl(by, i0 & 63);
+      if (i0 >= splits || w == 0.0f) continue;  // it saw nothing, and wrote nothing
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = fmaf(p[x][e], w, v[e]);
     }
   }
   for (int off = wide; off < 64; off *= 2)

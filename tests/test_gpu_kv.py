@@ -229,6 +229,34 @@ def test_long(pkg, cuda, news, dtype, D):
     _check_attend(pkg, cuda, 2, 1, D, 64, [2500], news, dtype, seed=D)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("window", [0, 900])
+def test_prompts_beside_decoded_sequences(pkg, cuda, window, dtype):
+    """One call of sequences with one row and with many, both long enough to be shared out,
+    and an empty slot."""
+    _check_attend(pkg, cuda, 4, 1, 64, 64, [2100, 1500, 0, 700, 1300], [60, 1, 1, 3, 20], dtype,
+                  window=window, seed=16, max_tokens=60)
+
+
+@pytest.mark.parametrize("max_tokens", [1, 3, 20])
+def test_max_tokens_too_small(pkg, cuda, max_tokens):
+    """Rows past what the caller gave as the most are left out, in bounds; the others of
+    their sequence, and other sequences, are not the worse for it."""
+    import torch
+    table, pages = _table(2, 30, 1, 17)
+    cache = _cache(pkg, pages, 2, 64, 64, cuda, 17)
+    Q = _rand((45, 8, 64), 18, cuda)
+    args = (_i32(table, cuda), _i32([1900, 1800], cuda))
+    starts = _i32([0, 40, 45], cuda)
+    want = cache.attend(Q, *args, starts=starts)
+    got = cache.attend(Q, *args, starts=starts, max_tokens=max_tokens, out=torch.full_like(Q, 7.0))
+    most = _values(cache.v, cache.v_scales).abs().max().item()
+    for row, n in ((0, 40), (40, 5)):
+        seen = min(n, max_tokens)
+        assert ((got - want)[row:row + seen].abs() <= 2.0 ** -16 * most).all()
+        assert (got[row + seen:row + n] == 7.0).all()
+
+
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("q_size,scale", [(1e-4, 1e3), (300.0, 1e-3), (30.0, None), (1.0, 0.0),
                                           (1.0, -0.2)])
