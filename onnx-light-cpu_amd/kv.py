@@ -39,11 +39,12 @@ class KvRows(ctypes.Structure):
 
 _lib = None
 _types = None  # torch dtype -> MNB_TYPE_* of include/mnb_fp8.h
+_int32 = _current_device = None  # torch.int32, torch's query of the current device
 
 
 def _library():
     """libmnb.so with the cache's signatures."""
-    global _lib, _types
+    global _lib, _types, _int32, _current_device
     if _lib is None:
         import torch
         L = library()
@@ -55,6 +56,7 @@ def _library():
         L.mnb_kv_attend.argtypes = [cache, batch, i32, i32, rows, ctypes.c_float, i64, vp, vp, sz,
                                     vp]
         _types = {torch.float32: 1, torch.float16: 10, torch.bfloat16: 16}
+        _int32, _current_device = torch.int32, torch._C._cuda_getDevice
         _lib = L
     return _lib
 
@@ -120,75 +122,83 @@ class Fp8KVCache:
             raise ValueError(f"{PREFIX}: kv_heads must be 1 .. 1024 and pages 1 .. 2^31 - 1, got "
                              f"{kv_heads} and {pages}")
 
+    # The calls hold these tensors' addresses: they cannot be replaced.
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    k_scales = property(lambda self: self._tensors[2])
+    v_scales = property(lambda self: self._tensors[3])
+
     def _set(self, k, v, k_scales, v_scales):
-        self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
+        self._tensors = (k, v, k_scales, v_scales)
         self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.device = k.device
         self._cache = KvCache(self.pages, self.kv_heads, self.page_size, self.head_dim,
                               k.data_ptr(), v.data_ptr(), k_scales.data_ptr(),
                               v_scales.data_ptr())
+        self._cache_ref = ctypes.byref(self._cache)
         self._needs = {}  # workspace bytes by the call's sizes
 
     _works = _shared_works
     _stream_workspace = MatMulNBits._stream_workspace
 
     # -- what the calls share ----------------------------------------------
-    def _check_tokens(self, X, name, heads=None):
-        shape = X.shape
-        if (X.dim() not in (3, 4) or shape[-1] != self.head_dim
+    # The smallest calls are bound by these functions, not by their 4 us of kernels: an
+    # attribute of a tensor costs 50 to 100 ns, so each is read once.
+    def _check_tokens(self, shape, dtype, device, name, heads):
+        if (len(shape) not in (3, 4) or shape[-1] != self.head_dim
                 or (heads is not None and shape[-2] != heads)):
             raise ValueError(f"{PREFIX}: {name} must be [..., "
                              f"{'heads' if heads is None else heads}, {self.head_dim}], got "
                              f"{list(shape)}")
-        if X.dtype not in _types or X.device != self.device:
+        if dtype not in _types or device != self.device:
             raise ValueError(f"{PREFIX}: {name} must be a float32, float16 or bfloat16 tensor on "
                              f"{self.device}")
 
-    def _check_sequences(self, X, table, lengths, starts, max_tokens):
-        import torch
-        i32, device, shape = torch.int32, self.device, X.shape
-        if table.dim() != 2 or table.dtype != i32 or table.device != device:
+    def _batch(self, shape, table, lengths, starts, max_tokens):
+        """(the C struct of the sequences of tokens of this shape, what it points to)."""
+        device = self.device
+        sizes = table.shape
+        if len(sizes) != 2 or table.dtype != _int32 or table.device != device:
             raise ValueError(f"{PREFIX}: table must be int32 [sequences, width] on {device}")
-        B = table.shape[0]
-        if lengths.shape != (B,) or lengths.dtype != i32 or lengths.device != device:
+        B, width = sizes
+        if lengths.shape != (B,) or lengths.dtype != _int32 or lengths.device != device:
             raise ValueError(f"{PREFIX}: lengths must be int32 [{B}] on {device}")
+        each = 0
+        if len(shape) == 3:
+            tokens = even = shape[0]
+            if starts is None and (even % B if B else even):
+                even = -1
+        else:
+            tokens, even = shape[0] * shape[1], 0 if shape[0] == B else -1
+        if max_tokens is not None and max_tokens < 0:
+            raise ValueError(f"{PREFIX}: max_tokens must not be negative, got {max_tokens}")
+        first = None
         if starts is not None:
             if len(shape) != 3:
                 raise ValueError(f"{PREFIX}: with starts, tokens must be [tokens, heads, "
                                  f"{self.head_dim}], got {list(shape)}")
-            if starts.shape != (B + 1,) or starts.dtype != i32 or starts.device != device:
+            if starts.shape != (B + 1,) or starts.dtype != _int32 or starts.device != device:
                 raise ValueError(f"{PREFIX}: starts must be int32 [{B + 1}] on {device}")
-        elif shape[0] != B if len(shape) == 4 else (shape[0] % B if B else shape[0]):
+            if not starts.is_contiguous():
+                starts = starts.contiguous()
+            first, each = starts.data_ptr(), max_tokens or 0
+        elif even < 0:
             raise ValueError(f"{PREFIX}: {list(shape[:-2])} tokens are not the same number for each "
                              f"of {B} sequences")
-        if max_tokens is not None and max_tokens < 0:
-            raise ValueError(f"{PREFIX}: max_tokens must not be negative, got {max_tokens}")
         if device.type != "cuda":
             raise ValueError(f"{PREFIX}: the cache is on {device}; there is no CPU fallback")
-
-    @staticmethod
-    def _batch(X, table, lengths, starts, max_tokens):
-        """(the C struct of the sequences, what it points to)."""
         if not table.is_contiguous():
             table = table.contiguous()
         if not lengths.is_contiguous():
             lengths = lengths.contiguous()
-        B, width = table.shape
-        shape = X.shape
-        tokens = shape[0] if len(shape) == 3 else shape[0] * shape[1]
-        if starts is None:
-            return KvBatch(B, tokens, 0, width, table.data_ptr(), lengths.data_ptr(),
-                           None), (table, lengths)
-        if not starts.is_contiguous():
-            starts = starts.contiguous()
-        return KvBatch(B, tokens, max_tokens or 0, width, table.data_ptr(), lengths.data_ptr(),
-                       starts.data_ptr()), (table, lengths, starts)
+        return KvBatch(B, tokens, each, width, table.data_ptr(), lengths.data_ptr(),
+                       first), (table, lengths, starts)
 
     @staticmethod
-    def _rows(X):
+    def _rows(X, shape):
         """(the C struct of X [..., heads, head_dim], the tensor it points into): X, or a
         copy where its rows are not evenly apart or not aligned to 16 bytes."""
-        shape, strides, address, even = X.shape, X.stride(), X.data_ptr(), True
+        strides, address, even = X.stride(), X.data_ptr(), True
         if len(shape) == 3:
             n, H, D = shape
             st = strides[0] if n > 1 else H * D
@@ -197,9 +207,9 @@ class Fp8KVCache:
             st = strides[1] if t > 1 else strides[0] if n > 1 else H * D
             even = n <= 1 or t <= 1 or strides[0] == t * strides[1]
         sh = strides[-2] if H > 1 else D
-        each = 16 // X.element_size()
-        if (not even or strides[-1] != 1 or st < D or sh < D or st % each or sh % each
-                or address % 16 != 0):
+        # 8 values of any of the types are whole 16 bytes
+        if (not even or strides[-1] != 1 or st < D or sh < D or st % 8 or sh % 8
+                or address % 16):
             X = X.clone() if X.is_contiguous() else X.contiguous()
             st, sh, address = H * D, D, X.data_ptr()
         return KvRows(address, st, sh), X
@@ -211,20 +221,22 @@ class Fp8KVCache:
         scale is the least power of two that its largest magnitude allows; it grows
         as the page fills, and then the page's codes are rounded again."""
         L = _lib or _library()
-        self._check_tokens(K, "K", self.kv_heads)
-        self._check_tokens(V, "V", self.kv_heads)
-        if K.dtype != V.dtype or K.shape != V.shape:
+        shape, dtype, device = K.shape, K.dtype, K.device
+        self._check_tokens(shape, dtype, device, "K", self.kv_heads)
+        if V.shape != shape or V.dtype != dtype or V.device != device:
+            self._check_tokens(V.shape, V.dtype, V.device, "V", self.kv_heads)
             raise ValueError(f"{PREFIX}: K and V must be of one shape and type")
-        self._check_sequences(K, table, lengths, starts, max_tokens)
-        elsewhere = _elsewhere(self.device, stream)
-        if elsewhere is not None:
-            with elsewhere:
-                return self.append(K, V, table, lengths, starts, max_tokens)
-        k, K = self._rows(K)
-        v, V = self._rows(V)
-        batch, keep = self._batch(K, table, lengths, starts, max_tokens)
-        status = L.mnb_kv_append(ctypes.byref(self._cache), ctypes.byref(batch), _types[K.dtype],
-                                 ctypes.byref(k), ctypes.byref(v), _raw_stream(self.device))
+        if stream is not None or (device.index is not None and device.index != _current_device()):
+            self._batch(shape, table, lengths, starts, max_tokens)  # its refusals first
+            elsewhere = _elsewhere(device, stream)
+            if elsewhere is not None:
+                with elsewhere:
+                    return self.append(K, V, table, lengths, starts, max_tokens)
+        batch, keep = self._batch(shape, table, lengths, starts, max_tokens)
+        k, K = self._rows(K, shape)
+        v, V = self._rows(V, shape)
+        status = L.mnb_kv_append(self._cache_ref, ctypes.byref(batch), _types[dtype],
+                                 ctypes.byref(k), ctypes.byref(v), _raw_stream(device))
         if status != 0:
             _check(status, "append")
         return self
@@ -238,8 +250,9 @@ class Fp8KVCache:
         that sees nothing is 0. Rows of no sequence are 0, or stay as they are in out."""
         import torch
         L = _lib or _library()
-        self._check_tokens(Q, "Q")
-        heads, x_type = Q.shape[-2], _types[Q.dtype]
+        shape, dtype, device = Q.shape, Q.dtype, Q.device
+        self._check_tokens(shape, dtype, device, "Q", None)
+        heads, x_type = shape[-2], _types[dtype]
         if heads == 0 or heads % self.kv_heads:
             raise ValueError(f"{PREFIX}: Q's heads must be a multiple of {self.kv_heads}, got "
                              f"{heads}")
@@ -249,21 +262,21 @@ class Fp8KVCache:
             scale = self.head_dim ** -0.5
         elif not math.isfinite(scale):
             raise ValueError(f"{PREFIX}: scale must be finite, got {scale}")
-        if out is not None and (out.shape != Q.shape or out.dtype != Q.dtype
-                                or out.device != self.device or not out.is_contiguous()
-                                or out.data_ptr() % 16 != 0):
+        if out is not None and (out.shape != shape or out.dtype != dtype or out.device != device
+                                or not out.is_contiguous() or out.data_ptr() % 16 != 0):
             raise ValueError(f"{PREFIX}: out must be contiguous, of Q's shape, type and device, "
                              "aligned to 16 bytes")
-        self._check_sequences(Q, table, lengths, starts, max_tokens)
-        elsewhere = _elsewhere(self.device, stream)
-        if elsewhere is not None:
-            with elsewhere:
-                return self.attend(Q, table, lengths, starts, max_tokens, scale, window, out)
-        q, X = self._rows(Q)
-        batch, keep = self._batch(Q, table, lengths, starts, max_tokens)
+        if stream is not None or (device.index is not None and device.index != _current_device()):
+            self._batch(shape, table, lengths, starts, max_tokens)  # its refusals first
+            elsewhere = _elsewhere(device, stream)
+            if elsewhere is not None:
+                with elsewhere:
+                    return self.attend(Q, table, lengths, starts, max_tokens, scale, window, out)
+        batch, keep = self._batch(shape, table, lengths, starts, max_tokens)
+        q, X = self._rows(Q, shape)
         if out is None:
             if starts is not None:
-                out = torch.zeros(Q.shape, dtype=Q.dtype, device=self.device)
+                out = torch.zeros(shape, dtype=dtype, device=device)
             else:
                 out = torch.empty_like(Q, memory_format=torch.contiguous_format)
         key = (batch.sequences, batch.tokens, batch.max_tokens, batch.table_width, heads, x_type,
@@ -273,14 +286,14 @@ class Fp8KVCache:
             if len(self._needs) > 256:
                 self._needs = {}
             n = ctypes.c_size_t()
-            _check(L.mnb_kv_workspace_bytes(ctypes.byref(self._cache), ctypes.byref(batch), heads,
-                                            x_type, ctypes.byref(n)), "workspace_bytes")
+            _check(L.mnb_kv_workspace_bytes(self._cache_ref, ctypes.byref(batch), heads, x_type,
+                                            ctypes.byref(n)), "workspace_bytes")
             need = self._needs[key] = n.value
-        work = self._stream_workspace(need, self.device) if need else None
-        status = L.mnb_kv_attend(ctypes.byref(self._cache), ctypes.byref(batch), heads, x_type,
+        work = self._stream_workspace(need, device) if need else None
+        status = L.mnb_kv_attend(self._cache_ref, ctypes.byref(batch), heads, x_type,
                                  ctypes.byref(q), scale, window, out.data_ptr(),
                                  None if work is None else work.data_ptr(), need,
-                                 _raw_stream(self.device))
+                                 _raw_stream(device))
         if status != 0:
             _check(status, "attend")
         return out

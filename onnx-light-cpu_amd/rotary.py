@@ -106,12 +106,13 @@ class Rotary:
         self._axis = (ctypes.c_uint8 * pairs)(*axes)
         self.desc = RotaryDesc(self.head_dim, self.rotary_dim, self.axes, int(bool(interleaved)),
                                self._turns, self._axis)
+        self._ref = ctypes.byref(self.desc)
 
     @staticmethod
-    def _strides(x):
+    def _strides(x, shape):
         """(between tokens, between heads) of x [..., H, D] in values, None where its heads
         are not whole or its tokens not evenly apart."""
-        shape, strides = x.shape, x.stride()
+        strides = x.stride()
         H, D = shape[-2:]
         sh = strides[-2] if H > 1 else D
         if len(shape) == 3:
@@ -139,32 +140,32 @@ class Rotary:
         themselves."""
         import torch
         L = _lib or _library()
-        device, dtype = Q.device, Q.dtype
+        device, dtype, D = Q.device, Q.dtype, self.head_dim
         x_type = _types.get(dtype)
         if x_type is None or not Q.is_cuda:
             raise ValueError(f"{PREFIX}: Q must be a float32, float16 or bfloat16 device tensor")
-        D, tokens = self.head_dim, Q.shape[:-2]
-        parts = [("Q", Q)] if K is None else [("Q", Q), ("K", K)]
-        for name, x in parts:
-            if x.dim() < 2 or x.shape[-1] != D or x.shape[:-2] != tokens:
+        shapes = (Q.shape,) if K is None else (Q.shape, K.shape)
+        tokens = shapes[0][:-2]
+        for name, shape in zip("QK", shapes):
+            if len(shape) < 2 or shape[-1] != D or shape[:-2] != tokens:
                 raise ValueError(f"{PREFIX}: {name} must be [..., heads, {D}] of the same tokens, "
-                                 f"got {list(x.shape)}")
-            if x.dtype != dtype or x.device != device:
-                raise ValueError(f"{PREFIX}: {name} must be of Q's type and device")
+                                 f"got {list(shape)}")
+        if K is not None and (K.dtype != dtype or K.device != device):
+            raise ValueError(f"{PREFIX}: K must be of Q's type and device")
         pos_type, where = _positions.get(positions.dtype), positions.shape
-        want = (self.axes,) + tokens
         if (pos_type is None or positions.device != device
-                or (where != want and (self.axes > 1 or where != tokens))):
-            want = list(want if self.axes > 1 else tokens)
+                or (where != (self.axes,) + tokens and (self.axes > 1 or where != tokens))):
+            want = ([] if self.axes == 1 else [self.axes]) + list(tokens)
             raise ValueError(f"{PREFIX}: positions must be int32 or int64 {want} on {device}, "
-                             f"got {positions.dtype} {list(positions.shape)}")
+                             f"got {positions.dtype} {list(where)}")
+        parts = (Q,) if K is None else (Q, K)
         if out is not None:
             out = (out,) if K is None and isinstance(out, torch.Tensor) else tuple(out)
             if len(out) != len(parts):
                 raise ValueError(f"{PREFIX}: out must be {len(parts)} tensors")
-            for (name, x), y in zip(parts, out):
-                if (y.shape != x.shape or y.dtype != dtype or y.device != device
-                        or (y.numel() and self._strides(y) is None)):
+            for name, shape, y in zip("QK", shapes, out):
+                if (y.shape != shape or y.dtype != dtype or y.device != device
+                        or (y.numel() and self._strides(y, shape) is None)):
                     raise ValueError(f"{PREFIX}: out must have {name}'s shape, type and device, "
                                      "and whole heads")
         elsewhere = _elsewhere(device, stream)
@@ -173,26 +174,26 @@ class Rotary:
                 return self(Q, K, positions, out)
         T = tokens[0] if len(tokens) == 1 else math.prod(tokens)
         if T == 0:
-            results = [torch.empty_like(x) for _, x in parts] if out is None else out
+            results = [torch.empty_like(x) for x in parts] if out is None else out
             return results[0] if K is None else tuple(results)
         heads, results, keep = [], [], []
-        for i, (name, x) in enumerate(parts):
-            strides = self._strides(x)
-            y = torch.empty_like(x) if out is None else out[i]
-            to = self._strides(y)
-            if to is None:  # empty_like kept an order of axes
-                y = torch.empty(x.shape, dtype=dtype, device=device)
-                to = self._strides(y)
-            address, address_y = x.data_ptr(), y.data_ptr()
+        for x, shape in zip(parts, shapes):
+            strides, address = self._strides(x, shape), x.data_ptr()
+            if out is None:
+                y = torch.empty_like(x, memory_format=torch.contiguous_format)
+                to, address_y = (shape[-2] * D, D), y.data_ptr()
+            else:
+                y = out[len(results)]
+                to, address_y = self._strides(y, shape), y.data_ptr()
             if strides is None or (address == address_y and strides != to):
                 x = x.clone(memory_format=torch.contiguous_format)
                 keep.append(x)
-                strides, address = self._strides(x), x.data_ptr()
-            heads.append(RotaryHeads(x.shape[-2], address, *strides, address_y, *to))
+                strides, address = (shape[-2] * D, D), x.data_ptr()
+            heads.append(RotaryHeads(shape[-2], address, *strides, address_y, *to))
             results.append(y)
         if not positions.is_contiguous():
             positions = positions.contiguous()
-        status = L.mnb_rotary(ctypes.byref(self.desc), T, pos_type, positions.data_ptr(), T, x_type,
+        status = L.mnb_rotary(self._ref, T, pos_type, positions.data_ptr(), T, x_type,
                               ctypes.byref(heads[0]),
                               ctypes.byref(heads[1]) if K is not None else None,
                               _raw_stream(device))
