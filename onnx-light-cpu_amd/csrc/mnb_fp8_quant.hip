@@ -30,14 +30,7 @@ __global__ __launch_bounds__(kThreads) void QuantizeKernel(const T *__restrict__
   float amax;
   const int2 code = BlockCodes<sizeof(T) == 4>(x, top, &amax);
   if ((threadIdx.x & 15) == 0) S[item] = amax / 448.0f;
-  uint8_t *out = Q + row * ldq + k0;
-  if constexpr (VEC) {
-    if (k0 < ldq) *reinterpret_cast<int2 *>(out) = code;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (k0 + i < ldq) out[i] = static_cast<uint8_t>((i < 4 ? code.x : code.y) >> (8 * (i & 3)));
-  }
+  StoreCodes8<VEC>(Q + row * ldq + k0, static_cast<int>(min(int64_t{8}, ldq - k0)), code);
 }
 
 __global__ __launch_bounds__(kThreads) void PadKernel(const uint8_t *__restrict__ A,

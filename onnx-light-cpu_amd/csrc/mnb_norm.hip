@@ -86,14 +86,7 @@ __global__ __launch_bounds__(kMaxThreads) void RmsNormKernel(Args a) {
       const int2 code = BlockCodes<true>(y, top, &amax);
       if (n <= 0) return;
       if ((t & 15) == 0) a.scales[row * nb + k0 / kBlock] = amax / 448.0f;
-      uint8_t *out = static_cast<uint8_t *>(a.Y) + row * a.K + k0;
-      if constexpr (VEC) {
-        *reinterpret_cast<int2 *>(out) = code;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < n) out[i] = static_cast<uint8_t>((i < 4 ? code.x : code.y) >> (8 * (i & 3)));
-      }
+      StoreCodes8<VEC>(static_cast<uint8_t *>(a.Y) + row * a.K + k0, n, code);
     } else {
       Store8<T, VEC>(static_cast<T *>(a.Y) + row * a.K + k0, n, y);
     }

@@ -4,52 +4,75 @@
 
 #include "mnb_kernels.h"
 
+#include <type_traits>
+
 namespace mnb {
 
 typedef float floatx4v __attribute__((ext_vector_type(4)));
+
+// 16 bytes of values, at an address that is aligned to 16 bytes or to a value only:
+// global memory takes wide accesses at any such address, and the compiler makes them of this.
+template <typename T, bool ALIGNED>
+struct Wide {
+  typedef T Vec __attribute__((ext_vector_type(16 / sizeof(T))));
+  typedef T Loose __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+  typedef std::conditional_t<ALIGNED, Vec, Loose> Type;
+  static constexpr int kValues = 16 / sizeof(T);
+};
 
 // Eight values at p (n of them exist), zeros behind them. VEC: p is aligned to 16
 // bytes, and all eight exist or none.
 template <typename T, bool VEC>
 __device__ __forceinline__ void Load8(const T *p, int n, float (&x)[8]) {
-  if constexpr (VEC) {
-    if (n <= 0) {
+  typedef Wide<T, VEC> W;
+  if (n >= 8) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-      return;
+    for (int v = 0; v < 8 / W::kValues; ++v) {
+      const typename W::Type q = reinterpret_cast<const typename W::Type *>(p)[v];
+#pragma unroll
+      for (int i = 0; i < W::kValues; ++i) x[v * W::kValues + i] = static_cast<float>(q[i]);
     }
-    typedef T Vec __attribute__((ext_vector_type(16 / sizeof(T))));
-#pragma unroll
-    for (int v = 0; v < static_cast<int>(sizeof(T)) / 2; ++v) {
-      const Vec q = reinterpret_cast<const Vec *>(p)[v];
-#pragma unroll
-      for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i)
-        x[v * static_cast<int>(16 / sizeof(T)) + i] = static_cast<float>(q[i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = i < n ? static_cast<float>(p[i]) : 0.0f;
+    return;
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = !VEC && i < n ? static_cast<float>(p[i]) : 0.0f;
 }
 
 // Eight values to p, each rounded to T, n of them.
 template <typename T, bool VEC>
 __device__ __forceinline__ void Store8(T *p, int n, const float (&x)[8]) {
-  if constexpr (VEC) {
-    if (n <= 0) return;
-    typedef T Vec __attribute__((ext_vector_type(16 / sizeof(T))));
+  typedef Wide<T, VEC> W;
+  if (n >= 8) {
 #pragma unroll
-    for (int v = 0; v < static_cast<int>(sizeof(T)) / 2; ++v) {
-      Vec q;
+    for (int v = 0; v < 8 / W::kValues; ++v) {
+      typename W::Type q;
 #pragma unroll
-      for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i)
-        q[i] = static_cast<T>(x[v * static_cast<int>(16 / sizeof(T)) + i]);
-      reinterpret_cast<Vec *>(p)[v] = q;
+      for (int i = 0; i < W::kValues; ++i) q[i] = static_cast<T>(x[v * W::kValues + i]);
+      reinterpret_cast<typename W::Type *>(p)[v] = q;
     }
-  } else {
+    return;
+  }
+  if constexpr (!VEC) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (i < n) p[i] = static_cast<T>(x[i]);
+  }
+}
+
+// Eight codes to p, n of them.
+template <bool VEC>
+__device__ __forceinline__ void StoreCodes8(uint8_t *p, int n, int2 code) {
+  typedef int Pair __attribute__((ext_vector_type(2)));
+  typedef int Loose __attribute__((ext_vector_type(2), aligned(1)));
+  typedef std::conditional_t<VEC, Pair, Loose> Type;
+  if (n >= 8) {
+    *reinterpret_cast<Type *>(p) = Type{code.x, code.y};
+    return;
+  }
+  if constexpr (!VEC) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[i] = static_cast<uint8_t>((i < 4 ? code.x : code.y) >> (8 * (i & 3)));
   }
 }
 
