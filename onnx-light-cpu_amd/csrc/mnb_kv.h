@@ -51,6 +51,42 @@ __host__ __device__ inline Span SpanOf(const Batch &b, int s, int page_shift) {
   return r;
 }
 
+// Ragged sequences share a launch: of workgroups `unit` 0 .. UnitsOf - 1, each sequence
+// has those from its first row times `rows`, in blocks of 2^shift, plus `more` for every sequence
+// before it. That are no fewer than its own rows touch (more: 1 where they are counted from the
+// sequence's first, 2 where blocks lie anywhere), and the launch grows with the
+// rows and the sequences, not with their product.
+struct Units {
+  int32_t rows, shift, more;
+};
+
+inline int64_t UnitsOf(const Batch &b, const Units &u) {
+  return (static_cast<int64_t>(b.tokens) * u.rows >> u.shift) +
+         static_cast<int64_t>(b.sequences) * u.more;
+}
+
+#ifdef __HIPCC__
+// The sequence that has this unit, and its first one. All lanes of a wavefront call it: they
+// look at 64 sequences at a time.
+__device__ inline int SequenceOf(const Batch &b, const Units &u, int64_t unit, int64_t *first) {
+  const auto from = [&](int s) {
+    const int row = min(max(b.starts[s], 0), b.tokens);
+    return (static_cast<int64_t>(row) * u.rows >> u.shift) + static_cast<int64_t>(s) * u.more;
+  };
+  const int lane = threadIdx.x & 63;
+  int lo = 0, hi = b.sequences;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) / 64, s = lo + lane * step;
+    const int before = __popcll(__ballot(s < hi && from(min(s, hi - 1)) <= unit));
+    lo += max(before - 1, 0) * step;
+    hi = min(hi, lo + step);
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  *first = from(lo);
+  return lo;
+}
+#endif
+
 // Page of a sequence's position block p < width, or a number that is no page's.
 __host__ __device__ inline uint32_t PageOf(const Batch &b, int s, int p) {
   return static_cast<uint32_t>(b.table[static_cast<int64_t>(s) * b.width + p]);

@@ -51,18 +51,27 @@ __device__ __forceinline__ float PageScale(uint32_t top) {
   return __uint_as_float(static_cast<uint32_t>(max(e, -64) + 127) << 23);
 }
 
+__host__ __device__ inline Units PageUnits(const Cache &c) { return {1, c.page_shift, 2}; }
+
 // One workgroup per page that a sequence's new rows reach, head, and keys or
 // values: it alone writes that page, so nothing is atomic. An item is sixteen
 // values of a row; the rows are read for their largest magnitude and again, from
 // the caches, for their codes.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void AppendKernel(Cache c, Batch b, Rows k, Rows v) {
-  const int s = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1;
+  int s = blockIdx.z, nth = blockIdx.x;  // of the pages that this sequence's rows reach
+  const int h = blockIdx.y >> 1, which = blockIdx.y & 1;
+  if (b.starts != nullptr) {
+    int64_t unit;
+    s = SequenceOf(b, PageUnits(c), blockIdx.x, &unit);
+    nth = blockIdx.x - static_cast<int>(unit);
+    if (nth < 0) return;
+  }
   const Span span = SpanOf(b, s, c.page_shift);
   const int page = 1 << c.page_shift;
   const int first = max(span.first, 0);
   if (first >= span.end) return;
-  const int p = (first >> c.page_shift) + static_cast<int>(blockIdx.x);
+  const int p = (first >> c.page_shift) + nth;
   const int64_t begin = static_cast<int64_t>(p) << c.page_shift;
   if (begin >= span.end) return;
   const int lo = max(first - static_cast<int>(begin), 0);  // the new tokens' slots
@@ -120,7 +129,9 @@ hipError_t Launch(const Cache &c, const Batch &b, const Rows &k, const Rows &v, 
   const int64_t page = int64_t{1} << c.page_shift;
   // Pages that max_tokens neighbouring positions reach at most; the table has no more.
   const int64_t reach = std::min<int64_t>((b.max_tokens + page - 2) / page + 1, b.width);
-  const dim3 grid(static_cast<unsigned>(reach), 2u * c.heads, b.sequences);
+  const dim3 grid(
+      static_cast<unsigned>(b.starts == nullptr ? reach : UnitsOf(b, PageUnits(c))), 2u * c.heads,
+      b.starts == nullptr ? b.sequences : 1);
   hipLaunchKernelGGL((AppendKernel<T>), grid, dim3(kThreads), 0, s, c, b, k, v);
   return hipGetLastError();
 }

@@ -221,19 +221,35 @@ __device__ __forceinline__ int64_t TilePartStep(const Attend &a) {
   return static_cast<int64_t>(a.batch.tokens) * a.q_heads;
 }
 
+// Tiles of `per` rows, a power of two, of ragged sequences.
+__host__ __device__ inline Units RowUnits(const Cache &c, int q_heads, int per) {
+  return {q_heads / c.heads, 31 - __builtin_clz(per), 1};
+}
+
 // DP: head_dim rounded up to 64, 128 or 256; MT: tiles of 16 queries.
 // grid (heads x row tiles x splits, sequences). A row is a token's query head of
 // this cache head: row r is token r / group, head r % group.
 template <typename T, int DP, int MT>
-__global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work work, int row_tiles) {
+__global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work work, int row_tiles,
+                                                              int64_t unit0) {
   constexpr int kTerms = Terms<T>();
   constexpr int KS = DP / 64;      // 16-byte pieces of a key that a lane holds
   constexpr int VD = DP / 16;      // values of a token that a lane holds, tiles of O^T
   constexpr int VW = VD / 4;       // the same in words
   const Cache &c = a.cache;
-  const int s = blockIdx.y, split = blockIdx.x % work.part.splits;
-  const int h = blockIdx.x / work.part.splits / row_tiles;
-  const int tile = blockIdx.x / work.part.splits - h * row_tiles;
+  const int split = blockIdx.x % work.part.splits, rest = blockIdx.x / work.part.splits;
+  int s = blockIdx.y, h, tile;
+  if (row_tiles > 0) {
+    h = rest / row_tiles;
+    tile = rest - h * row_tiles;
+  } else {  // units of ragged sequences
+    h = rest % c.heads;
+    const int64_t unit = unit0 + rest / c.heads;
+    int64_t first;
+    s = SequenceOf(a.batch, RowUnits(a.cache, a.q_heads, 16 * MT), unit, &first);
+    tile = static_cast<int>(unit - first);
+    if (tile < 0) return;
+  }
   const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Span span = SpanOf(a.batch, s, c.page_shift);
@@ -612,7 +628,8 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
 // head's workgroups share an XCD's cache where there are eight; late rows, which see
 // the most keys, come first.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work, int row_tiles) {
+__global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work, int row_tiles,
+                                                             int64_t unit0) {
   constexpr int kTerms = Terms<T>();
   constexpr int kThreadsT = 64 * NW;
   constexpr int KP = DP / 16;                  // 16-code pieces of a key, steps of Q K^T
@@ -621,16 +638,23 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
   constexpr int kEach = (kUnits + kThreadsT - 1) / kThreadsT;
   constexpr int kMask = DP / 8 < 16 ? DP / 8 - 1 : 15;
   const Cache &c = a.cache;
-  const int s = blockIdx.y, h = blockIdx.x % a.cache.heads, rest = blockIdx.x / a.cache.heads;
+  const int h = blockIdx.x % a.cache.heads, rest = blockIdx.x / a.cache.heads;
   const int split = rest % work.tile_part.splits;
-  const int tile = row_tiles - 1 - rest / work.tile_part.splits;
+  int s = blockIdx.y, late = rest / work.tile_part.splits;  // tiles behind this one
+  if (row_tiles == 0) {  // units of ragged sequences
+    const int64_t unit = unit0 + late;
+    int64_t first;
+    s = SequenceOf(a.batch, RowUnits(a.cache, a.q_heads, 32 * NW), unit, &first);
+    late = static_cast<int>(unit - first);
+  }
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Span span = SpanOf(a.batch, s, c.page_shift);
   const int group = a.q_heads / c.heads;
   const int64_t rows = RowsOf(a, span);
+  const int tile = static_cast<int>(CeilDiv(rows, 32 * NW)) - 1 - late;
+  if (tile < 0 || late < 0 || rows <= work.few) return;
   const int64_t row0 = static_cast<int64_t>(tile) * (32 * NW);
-  if (row0 >= rows || rows <= work.few) return;
   const int64_t row1 = min(row0 + 32 * NW, rows) - 1;
   const Reach reach = ReachOf(span, static_cast<int>(row0 / group), static_cast<int>(row1 / group),
                               a.window);
@@ -1154,22 +1178,42 @@ Plan PlanOf(const Cache &c, const Batch &b, int32_t q_heads, int32_t x_type) {
   return p;
 }
 
+// Ragged sequences' units, `each` workgroups to one, so many at a time that a grid's
+// threads stay below 2^32.
+template <typename L>
+hipError_t InUnits(const Attend &a, const Units &u, unsigned each, const L &launch) {
+  const int64_t units = UnitsOf(a.batch, u), most = (1 << 22) / each;
+  for (int64_t i = 0; i < units; i += most) {
+    const hipError_t e = launch(dim3(each * static_cast<unsigned>(std::min(most, units - i))), 0, i);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
 template <typename T, int DP, int MT>
 hipError_t Split(const Attend &a, const Work &w, const Plan &p, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(a.cache.heads) * p.row_tiles * p.splits,
-                  a.batch.sequences);
-  hipLaunchKernelGGL((AttendSplitKernel<T, DP, MT>), grid, dim3(kThreads), 0, s, a, w,
-                     p.row_tiles);
-  return hipGetLastError();
+  const unsigned each = static_cast<unsigned>(a.cache.heads) * p.splits;
+  const auto launch = [&](dim3 grid, int row_tiles, int64_t unit0) {
+    hipLaunchKernelGGL((AttendSplitKernel<T, DP, MT>), grid, dim3(kThreads), 0, s, a, w, row_tiles,
+                       unit0);
+    return hipGetLastError();
+  };
+  if (a.batch.starts == nullptr || p.row_tiles == 1)
+    return launch(dim3(each * p.row_tiles, a.batch.sequences), p.row_tiles, 0);
+  return InUnits(a, RowUnits(a.cache, a.q_heads, 16 * MT), each, launch);
 }
 
 template <typename T, int DP, int NW>
 hipError_t Tile(const Attend &a, const Work &w, const Plan &p, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(a.cache.heads) * p.tile_row_tiles * p.tile_splits,
-                  a.batch.sequences);
-  hipLaunchKernelGGL((AttendTileKernel<T, DP, NW>), grid, dim3(64 * NW), 0, s, a, w,
-                     p.tile_row_tiles);
-  return hipGetLastError();
+  const unsigned each = static_cast<unsigned>(a.cache.heads) * p.tile_splits;
+  const auto launch = [&](dim3 grid, int row_tiles, int64_t unit0) {
+    hipLaunchKernelGGL((AttendTileKernel<T, DP, NW>), grid, dim3(64 * NW), 0, s, a, w, row_tiles,
+                       unit0);
+    return hipGetLastError();
+  };
+  if (a.batch.starts == nullptr)
+    return launch(dim3(each * p.tile_row_tiles, a.batch.sequences), p.tile_row_tiles, 0);
+  return InUnits(a, RowUnits(a.cache, a.q_heads, 32 * NW), each, launch);
 }
 
 template <typename T, int DP>

@@ -238,6 +238,21 @@ def test_prompts_beside_decoded_sequences(pkg, cuda, window, dtype):
                   window=window, seed=16, max_tokens=60)
 
 
+def _many(B):
+    """Rows and lengths of B sequences: one row, mostly, or none, and a few prompts."""
+    news = [0 if b % 11 == 3 else 75 if b == B - 30 else 20 if b % 50 == 7 else 1 for b in range(B)]
+    return news, [n + (b * 7) % 40 - 1 if b % 9 else n for b, n in enumerate(news)]
+
+
+@pytest.mark.parametrize("D,dtype", [(64, "bfloat16"), (128, "float32"), (256, "bfloat16"),
+                                     (256, "float32")])
+@pytest.mark.parametrize("B,max_tokens", [(64, None), (65, 75), (150, None)])
+def test_many_sequences(pkg, cuda, B, max_tokens, D, dtype):
+    """More sequences than a wavefront has lanes."""
+    news, lengths = _many(B)
+    _check_attend(pkg, cuda, 4, 1, D, 16, lengths, news, dtype, seed=19, max_tokens=max_tokens)
+
+
 @pytest.mark.parametrize("max_tokens", [1, 3, 20])
 def test_max_tokens_too_small(pkg, cuda, max_tokens):
     """Rows past what the caller gave as the most are left out, in bounds; the others of
@@ -481,6 +496,17 @@ def test_append_outside_the_table_and_cache(pkg, cuda):
     cache = _cache(pkg, pages, H, page, D, cuda, 26)
     X = [_rand((60, H, D), 27 + n, cuda) for n in range(2)]
     _check_append(pkg, cuda, cache, _state(cache), X, table, [10, 25, 45], None, page)
+
+
+@pytest.mark.parametrize("B", [64, 65, 150])
+def test_append_of_many_sequences(pkg, cuda, B):
+    news, lengths = _many(B)
+    H, D, page = 2, 32, 16
+    table, pages = _table(B, 8, 1, 33)
+    cache = _cache(pkg, pages, H, page, D, cuda, 33)
+    X = [_rand((sum(news), H, D), 34 + n, cuda) for n in range(2)]
+    _check_append(pkg, cuda, cache, _state(cache), X, table, lengths,
+                  [sum(news[:b]) for b in range(B + 1)], page)
 
 
 def test_append_twice_is_append_once(pkg, cuda):
