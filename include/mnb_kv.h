@@ -7,7 +7,8 @@
  * of any length. The scales that mnb_kv_append makes are powers of two (e4m3's
  * precision does not depend on where in its range a value lies, so they lose
  * nothing, and a page whose scale grows is re-rounded exactly, but for values that become
- * subnormal); mnb_kv_attend takes any positive ones.
+ * subnormal); mnb_kv_attend takes any from 2^-100 up, and 0 for a page whose
+ * codes are 0.
  *
  * It stands between the QKV projection (mnb.h, mnb_fp8.h), whose rows
  * mnb_rotary turns in place, and the output projection. ONNX's Attention-24 is
@@ -48,7 +49,8 @@ typedef struct mnb_kv_cache {
  * starts beyond `tokens` count as `tokens`; positions that the table does
  * not reach and pages outside the cache are neither written nor seen. Rows of no
  * sequence are left as they are. A page that two sequences append to in one call
- * holds codes of either; any number may read one. */
+ * has codes and a scale of either, as has one that one sequence reaches twice; any
+ * number may read one. */
 typedef struct mnb_kv_batch {
   int64_t sequences;    /* 0 .. 65535 */
   int64_t tokens;       /* rows of the call's tensors, at most 2^24 */
@@ -81,12 +83,13 @@ int mnb_kv_append(const mnb_kv_cache *cache, const mnb_kv_batch *batch, int32_t 
 int mnb_kv_workspace_bytes(const mnb_kv_cache *cache, const mnb_kv_batch *batch, int32_t heads,
                            int32_t x_type, size_t *bytes);
 
-/* Y [tokens, heads, head_dim], dense, of Q's type, aligned to 16 bytes: for row i of sequence b
- * at position p and query head h (tokens * heads at most 2^27), the softmax over the keys t <= p (and t > p -
- * window, where window > 0; beyond 2^30 it counts as 0) of scale * q . k_t, times v; heads is a multiple of
- * kv_heads, and query heads h use cache head h / (heads / kv_heads). A row that
- * sees no key, or only scores of -inf, is 0; unseen keys and values leave no trace, NaN
- * and infinities among them. Products are exact up to 2^-22 of q's largest magnitude
+/* Y [tokens, heads, head_dim], dense, of Q's type, aligned to 16 bytes, overlapping
+ * nothing else: for row i of sequence b at position p and query head h (tokens *
+ * heads at most 2^27), the softmax over the keys t <= p (and t > p - window, where
+ * window > 0; beyond 2^30 it counts as 0) of scale * q . k_t, times v; heads is a
+ * multiple of kv_heads, and query heads h use cache head h / (heads / kv_heads). A row
+ * that sees no key, or only scores of -inf, is 0; unseen keys and values leave no trace,
+ * NaN and infinities among them. Products are exact up to 2^-22 of q's largest magnitude
  * (fp32 q; fp16 and bf16 q: exact), the weights have 22 bits for an fp32 Y and 11
  * otherwise, sums are fp32. The value scales of one head and sequence lie within 2^100 of
  * each other. Runs on the current device, asynchronous on `stream`. */

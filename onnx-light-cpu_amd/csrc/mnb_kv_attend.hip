@@ -92,6 +92,9 @@ __device__ __forceinline__ float SumGroups(float v) {
 
 __device__ __forceinline__ float Exp2(float v) { return __builtin_amdgcn_exp2f(v); }
 
+// A page of zeros may have the scale 0: its values are 0, its tokens weigh what they do.
+__device__ __forceinline__ float ValueScale(float w) { return w == 0.0f ? 0x1p-64f : w; }
+
 // log2 of a positive scale: an integer exactly for a power of two.
 __device__ __forceinline__ float Log2Scale(float w) {
   int e;
@@ -398,8 +401,9 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
     }
     // The scales' part in scores and weights, made by the lanes that hold them.
     const bool there = page != ~0u;
-    const float lane_ks = there ? sk : 1.0f, lane_ev = there ? Log2Scale(sv) : -kInf;
-    const float lane_inv = there ? 1.0f / sv : 0.0f;
+    const float value = ValueScale(sv);
+    const float lane_ks = there ? sk : 1.0f, lane_ev = there ? Log2Scale(value) : -kInf;
+    const float lane_inv = there ? 1.0f / value : 0.0f;
     const bool whole = __all(there);
     float ks[4], ev[4], inv[4];
 #pragma unroll
@@ -783,9 +787,11 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
       if (!good) kw[k] = uint4v{0, 0, 0, 0};  // no NaN: the info's -inf does the rest
       WriteLds(off + kto[k], Widen8(kw[k][0], kw[k][1]));
       WriteLds((off + kto[k]) ^ 16, Widen8(kw[k][2], kw[k][3]));
-      if ((64 * wave + k * kThreadsT) % DP == 0 && lane == 0)
-        info[n & 3][grp[k]] = good ? make_float4(sk[k], Log2Scale(sv[k]), 1.0f / sv[k], 0.0f)
+      if ((64 * wave + k * kThreadsT) % DP == 0 && lane == 0) {
+        const float value = ValueScale(sv[k]);
+        info[n & 3][grp[k]] = good ? make_float4(sk[k], Log2Scale(value), 1.0f / value, 0.0f)
                                    : make_float4(1.0f, -kInf, 0.0f, 0.0f);
+      }
     }
   };
   const auto store_values = [&](int n) {

@@ -27,8 +27,8 @@ _shared_works = {}
 
 
 def release_workspaces():
-    """Gives the workspaces that MatMulFp8 and MatMulNBitsMoE calls share back to torch's
-    allocator; the next calls have new ones."""
+    """Gives the workspaces that MatMulFp8, MatMulNBitsMoE and Fp8KVCache calls share back to
+    torch's allocator; the next calls have new ones."""
     _shared_works.clear()
 
 

@@ -91,8 +91,8 @@ class Fp8KVCache:
 
     @classmethod
     def from_tensors(cls, k, v, k_scales, v_scales):
-        """A cache of tensors that exist (held, not copied); scales may be any positive
-        numbers, append makes powers of two."""
+        """A cache of tensors that exist (held, not copied); scales may be any
+        numbers from 2^-100 up, or 0 for a page of codes of 0; append makes powers of two."""
         import torch
         if k.dim() != 4:
             raise ValueError(f"{PREFIX}: k must be [pages, kv_heads, page_size, head_dim], got "

@@ -288,6 +288,21 @@ def test_sizes_of_values(pkg, cuda, dtype):
                   scale=1e-6)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("news", [[1, 3], [40, 90]])
+def test_pages_of_zeros(pkg, cuda, news, dtype):
+    """Scales of 0, as a quantizer may give a page of zeros: its tokens still have their
+    weights."""
+    def zeros(table, cache, Q):
+        for p in (table[0][1], table[1][0], table[1][3]):
+            cache.v[p].zero_()
+            cache.v_scales[p] = 0.0
+        for p in (table[0][0], table[1][3], table[1][4]):
+            cache.k_scales[p] = 0.0
+
+    _check_attend(pkg, cuda, 4, 2, 64, 32, [110, 200], news, dtype, seed=35, spoil=zeros)
+
+
 def test_huge_queries(pkg, cuda):
     """fp32 and bf16 queries far beyond fp16's range, undone by the scale."""
     for dtype in ("float32", "bfloat16"):
