@@ -132,9 +132,6 @@ __device__ __forceinline__ void SplitQuery(const float (&f)[8], int shift, float
   }
 }
 
-// The weights 2^(scale s + add) of eight scores as fp16 terms, and their sum before that rounding:
-// beside a page of far larger values a page's weights may be lost for the values'
-// sum, but never for their own.
 // Whether fp16 holds all weights that add up to these sums; a NaN fails too, as it does
 // in a row's first tile.
 __device__ __forceinline__ bool Fits(const float (&sum)[4]) {
@@ -146,6 +143,9 @@ __device__ __forceinline__ float FromLane(float v, int lane) {
   return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
 }
 
+// The weights 2^(scale s + add) of eight scores as fp16 terms, and their sum before that rounding:
+// beside a page of far larger values a page's weights may be lost for the values'
+// sum, but never for their own.
 template <int TERMS>
 __device__ __forceinline__ float Weights(const float (&s)[8], float scale, float add,
                                          half8v (&p)[TERMS]) {
@@ -229,9 +229,16 @@ __host__ __device__ inline Units RowUnits(const Cache &c, int q_heads, int per) 
   return {q_heads / c.heads, 31 - __builtin_clz(per), 1};
 }
 
-// DP: head_dim rounded up to 64, 128 or 256; MT: tiles of 16 queries.
-// grid (heads x row tiles x splits, sequences). A row is a token's query head of
-// this cache head: row r is token r / group, head r % group.
+// Few rows: each key and value is read once, by one wavefront, from memory straight into
+// the registers that the MFMAs take, with no LDS between; the row's heads and drafted
+// tokens share it. DP: head_dim rounded up to 64, 128 or 256; MT: tiles of 16 queries.
+// grid (heads x row tiles x splits, sequences), or (row tiles of all sequences x heads x
+// splits) where row_tiles is 0. A row is a token's query head of this cache head: row r is
+// token r / group, head r % group.
+// Memory bounds it: 32 sequences at 16384 tokens, 8 heads of 128, bf16, take 188 us (1.08 GB,
+// 5.7 TB/s; a copy reaches 4.7), 16 drafted tokens of 8
+// sequences there 114 with widening and weights in the way. One sequence at 8192 tokens has a
+// workgroup on each CU, each with two tiles a wavefront: 8.3 us, of which 3.6 are its bytes'.
 template <typename T, int DP, int MT>
 __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work work, int row_tiles,
                                                               int64_t unit0) {
@@ -628,9 +635,14 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
 // 32 x 32 halve what a product reads of LDS; V is laid out transposed, in the order
 // of tokens that a lane's weights have. The next tile's codes are in registers
 // while a tile is multiplied, and are widened into the other half of LDS.
-// grid (row tiles x splits x heads, sequences): heads lie next to each other, so that a
+// grid (row tiles x splits x heads, sequences), or (row tiles of all sequences x splits x
+// heads) where row_tiles is 0: heads lie next to each other, so that a
 // head's workgroups share an XCD's cache where there are eight; late rows, which see
 // the most keys, come first.
+// The matrix instructions bound it: 2048 bf16 tokens of 32 heads of 128 over 16384 keys take
+// 547 us, 0.94 PFLOP/s (a large library product reaches 1.2). The weights, their exponentials
+// first, take nearly as long as a tile's products, and run on the SIMD's other wavefront
+// meanwhile; with the halves of a workgroup not half a step apart it took 772.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work, int row_tiles,
                                                              int64_t unit0) {
@@ -1055,9 +1067,10 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
 }
 
 // Joins the splits of a row. PER threads to a row, four values of it each; where one
-// row has more threads than its width, they take every n-th split. A workgroup
-// per row (PER 256) hides the reads of many splits (32 rows of 32 splits: 28 us with a
-// wavefront, 4.6 with four), a wavefront (PER 64) is enough for few splits or many rows.
+// row has more threads than its width, they take every n-th split. All parts of a row
+// are asked for at once: it is bound by two trips to memory, 4 us. A workgroup per row
+// (PER 256) is sooner for few rows of many splits (attention of one token over 8192: 11.1 us in
+// all, 12.5 with a wavefront), a wavefront (PER 64) for many rows (3500: 37.0, 41.7).
 template <typename T, int PER>
 __global__ __launch_bounds__(kThreads) void JoinKernel(Attend a, Work work, int64_t row0) {
   const int64_t row = row0 + static_cast<int64_t>(blockIdx.x) * (kThreads / PER) +
@@ -1149,7 +1162,9 @@ Plan PlanOf(const Cache &c, const Batch &b, int32_t q_heads, int32_t x_type) {
   Plan p;
   const int64_t group = q_heads / c.heads, rows = b.max_tokens * group;
   const bool fp32 = x_type == MNB_TYPE_FLOAT, tiles = c.dim <= 128;
-  // Two tiles of fp32 queries 256 wide leave no registers for the keys.
+  // Up to 64 rows AttendSplitKernel is as fast as AttendTileKernel over long caches (16 drafted
+  // tokens of 8 sequences at 16384: 114 and 112 us) and starts sooner. Two tiles of fp32
+  // queries 256 wide leave no registers for the keys.
   const int most_mt = fp32 ? (tiles ? 2 : 1) : tiles ? 4 : 2;
   const int64_t key_tiles = CeilDiv(static_cast<int64_t>(b.width) << c.page_shift, kTile);
   const auto parts = [&](int64_t groups, int64_t goal, int64_t least) {
@@ -1160,6 +1175,9 @@ Plan PlanOf(const Cache &c, const Batch &b, int32_t q_heads, int32_t x_type) {
   if (tiles && rows > 16 * most_mt) {
     // Where ragged sequences are long or short, the short ones are taken to be decoded.
     p.few = few = b.starts == nullptr ? 0 : group <= 16 ? 16 : 32;
+    // Eight wavefronts share a tile's widening (2048 tokens over 16384: 547 us, 631 with
+    // four); 128 rows leave half of them without any (4 x 32 tokens over 8192: 46 us, 58 with
+    // eight), and two terms of fp32 need the registers.
     p.waves = rows > 128 && !fp32 ? 8 : 4;
     const int64_t per = 32 * p.waves;
     p.tile_row_tiles = static_cast<int>(CeilDiv(rows, per));
@@ -1176,8 +1194,9 @@ Plan PlanOf(const Cache &c, const Batch &b, int32_t q_heads, int32_t x_type) {
   if (few > 0) {
     p.mt = static_cast<int>(std::min<int64_t>(most_mt, CeilDiv(few, 16)));
     p.row_tiles = static_cast<int>(CeilDiv(few, 16 * p.mt));
-    // Workgroups for three on each CU; a part's sums are as large as mt tiles of keys for
-    // each of its wavefronts.
+    // Workgroups for three on each CU, which fit (for two or six the times are the same,
+    // within 1%; six have twice the parts); a part's sums are as large as mt tiles of keys
+    // for each of its wavefronts.
     p.splits = parts(static_cast<int64_t>(b.sequences) * c.heads * p.row_tiles, 3 * 256,
                      kWaves * p.mt);
   }

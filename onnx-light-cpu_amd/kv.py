@@ -74,8 +74,8 @@ class Fp8KVCache:
     [sequences, width], the pages of each sequence in their order; lengths: int32
     [sequences], each sequence's tokens with those of the call, which are its last;
     starts: int32 [sequences + 1], the first row of each sequence where they have
-    different numbers of rows, and the end; max_tokens: the largest number (it bounds
-    the launch; without it, all rows might be one sequence's). All are device tensors
+    different numbers of rows, and the end; max_tokens: the largest number (kernels are
+    chosen by it; without it, all rows might be one sequence's). All are device tensors
     but max_tokens: a captured call can be replayed as they change."""
 
     op_type = "Fp8KVCache"
