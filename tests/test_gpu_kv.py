@@ -12,8 +12,8 @@ row's keys:
   - the weights of a row are divided by their sum, which has the same errors: twice;
   - a weight is rounded to fp16, 2^-11 relative, for 16-bit queries, to 2^-22 for fp32,
     and where it is below fp16's normal values by 2^-25 at most; the largest weight (times its
-    value scale) is 2^14 for few rows, for many 2^12 or, as a factor of 2 is left above it
-    when it is found, 2^11 at least: 2^-36 of it, n 2^-35 max|v| for n keys, max|v| by channel;
+    value scale) is 2^12 or, as a factor of 2 is left above it when it is found, 2^11 at
+    least: 2^-36 of it, n 2^-35 max|v| for n keys, max|v| by channel;
   - sums of n weighted values in fp32: n 2^-24 A; joins and the division, 2^-20 A;
   - the output's rounding, half a step (eps / 2) of the value.
 """
