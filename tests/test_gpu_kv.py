@@ -564,6 +564,28 @@ def test_offsets_past_32_bits(pkg, cuda):
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("ragged,max_tokens", [(False, None), (True, 1), (True, None)])
+def test_most_sequences(pkg, cuda, ragged, max_tokens):
+    """As many sequences as a call may have, of one token each: its value comes back. A code is
+    off by half a step (2^-4) of the value or of the least normal (2^-6 scale); scores are
+    below 128, so a weight and the sum are off by 2^-11 (above), and everything else by less."""
+    import torch
+    B, D, page = 65535, 16, 16
+    cache = pkg.Fp8KVCache(B, 1, D, page, device=cuda)
+    g = torch.Generator(device=cuda)
+    g.manual_seed(36)
+    table = torch.randperm(B, device=cuda, generator=g).int()[:, None]
+    lengths = torch.ones(B, dtype=torch.int32, device=cuda)
+    starts = torch.arange(B + 1, dtype=torch.int32, device=cuda) if ragged else None
+    K, V, Q = (_rand((B, 1, D), 37 + n, cuda).clamp(-4, 4) for n in range(3))
+    cache.append(K, V, table, lengths, starts=starts, max_tokens=max_tokens)
+    got = cache.attend(Q, table, lengths, starts=starts, max_tokens=max_tokens)
+    scale = cache.v_scales[table[:, 0].long()][:, :, None]
+    held = cache.v[table[:, 0].long(), :, 0].float() * scale
+    assert ((held - V).abs() <= 2.0 ** -4 * V.abs() + 2.0 ** -10 * scale).all()
+    assert ((got - held).abs() <= 2.0 ** -10 * held.abs()).all()
+
+
 def test_streams_and_threads(pkg, cuda):
     """Calls that overlap, each with a workspace of its own."""
     import threading
@@ -626,6 +648,41 @@ def test_graphs(pkg, cuda):
         assert torch.equal(cache.k.float(), plain.k.float())
         assert torch.equal(cache.v_scales, plain.v_scales)
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_graph_of_ragged_calls(pkg, cuda):
+    """A captured ragged call replayed as rows go from one sequence to another, to none, and
+    as lengths and pages change."""
+    import torch
+    H, Hq, D, page, T = 2, 8, 64, 16, 64
+    table, pages = _table(3, 100, 0, 55)
+    cache, plain = (_cache(pkg, pages, H, page, D, cuda, 55) for _ in range(2))
+    table_, lengths, starts = _i32(table, cuda), _i32([1500, 300, 64], cuda), _i32([0, 60, 61, 64], cuda)
+    K, V = (_rand((T, H, D), 56 + n, cuda).to(torch.bfloat16) for n in range(2))
+    Q = _rand((T, Hq, D), 58, cuda).to(torch.bfloat16)
+    args = (table_, lengths, starts)
+    for c in (cache, plain):
+        c.append(K, V, *args)
+        c.attend(Q, *args)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.append(K, V, *args)
+        got = cache.attend(Q, *args)
+    for s, l, swap in (([0, 60, 61, 64], [1500, 300, 64], False), ([0, 1, 2, 64], [1501, 301, 130], False),
+                       ([5, 5, 64, 64], [1501, 360, 0], True), ([0, 64, 64, 64], [20, 0, 130], False),
+                       ([0, 0, 0, 0], [1600, 1600, 1600], False), ([0, 20, 41, 64], [1600, 21, 24], True)):
+        starts.copy_(_i32(s, cuda))
+        lengths.copy_(_i32(l, cuda))
+        if swap:
+            table_.copy_(table_.flip(0).clone())
+        plain.append(K, V, *args)
+        want = plain.attend(Q, *args)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(cache.k.float().nan_to_num(), plain.k.float().nan_to_num())
+        assert torch.equal(cache.k_scales, plain.k_scales)
+        assert torch.equal(got, want)
 
 
 def test_same_bits_again(pkg, cuda):
