@@ -111,23 +111,24 @@ class Rotary:
     @staticmethod
     def _strides(x, shape):
         """(between tokens, between heads) of x [..., H, D] in values, None where its heads
-        are not whole or its tokens not evenly apart."""
+        are not whole or its tokens not evenly apart, or the same memory several times."""
         strides = x.stride()
         H, D = shape[-2:]
         sh = strides[-2] if H > 1 else D
         if len(shape) == 3:
             st = strides[0] if shape[0] > 1 else H * D
         else:
-            st = apart = 0
+            st = apart = None
             for n, d in zip(shape[-3::-1], strides[-3::-1]):  # the axes of tokens, last first
                 if n == 1:
                     continue
-                if st == 0:
+                if st is None:
                     st = apart = d
                 elif d != apart:
                     return None
                 apart *= n
-            st = st or H * D
+            if st is None:
+                st = H * D
         if st < D or sh < D or (D > 1 and strides[-1] != 1):
             return None
         return st, sh

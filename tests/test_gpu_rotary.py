@@ -132,6 +132,28 @@ def test_views_in_place_and_shapes(pkg, cuda, D):
     assert torch.equal(qkv[:, Hq + Hkv:], v)
 
 
+def test_expanded_tokens(pkg, cuda):
+    """One row for several tokens (stride 0, of the inner or the outer axis): read as their
+    copies are; a result that would lie on itself is refused."""
+    import torch
+    D = 64
+    op = pkg.Rotary(D)
+    q, k = _heads(3, 4, D, torch.bfloat16, cuda, 13), _heads(3, 2, D, torch.bfloat16, cuda, 14)
+    for axis, shape in ((1, (3, 2)), (0, (2, 3))):
+        pos = torch.arange(6, device=cuda).reshape(shape) * 13
+        Q, K = (x.unsqueeze(axis).expand(*shape, *x.shape[1:]) for x in (q, k))
+        want = op(Q.contiguous(), K.contiguous(), pos)
+        for a, b in zip(op(Q, K, pos), want):
+            assert torch.equal(a, b)
+        fresh = [torch.empty(shape + x.shape[1:], dtype=x.dtype, device=cuda) for x in (q, k)]
+        for a, b in zip(op(Q, K, pos, out=fresh), want):
+            assert torch.equal(a, b)
+        with pytest.raises(ValueError, match="whole heads"):
+            op(Q, K, pos, out=(fresh[0], K))
+        with pytest.raises(ValueError, match="whole heads"):
+            op(Q, K, pos, out=(Q, fresh[1]))
+
+
 def test_many_tokens(pkg, cuda):
     """More tokens than a workgroup has, against the same tokens a few at a time."""
     import torch

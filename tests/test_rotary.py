@@ -102,6 +102,33 @@ def test_python_refusals(pkg, kwargs, match):
         pkg.Rotary(**kwargs)
 
 
+def test_strides_of_tokens_of_several_axes(pkg):
+    """Token axes that can be walked with one stride, and those that cannot: expanded ones (a
+    stride of 0, innermost or not), transposed and sliced ones. Every value that the strides
+    lead to is the tensor's own."""
+    import torch
+    H, D = 4, 8
+    x = torch.arange(6 * H * D, dtype=torch.float32).reshape(2, 3, H, D)
+    row = x[0, :, None]  # [3, 1, H, D]
+    cases = [(x, True), (x.view(6, H, D), True), (x.view(1, 2, 3, H, D), True), (x[:, :1], True),
+             (x[:, 1:2], True), (x[:, 0], True), (x[:1], True), (x[:1, :1], True), (x[..., :2, :], True),
+             (x.view(2, 3, 1, H, D), True), (x[0, 0], True),
+             (x.transpose(0, 1), False), (x[:, :2], False), (x[:, ::2], False),
+             (row.expand(3, 2, H, D), False), (row.expand(3, 5, H, D)[:1], False),
+             (row[:1].expand(3, 2, H, D), False), (x[:1].expand(2, 3, H, D), False),
+             (row[None].expand(2, 3, 1, H, D), False), (row[:, :, None].expand(3, 1, 2, H, D), False),
+             (x[0, :1].expand(3, H, D), False), (x[0, :, :1].expand(3, H, D), False),
+             (x[0, 0].expand(3, H, D), False)]
+    for n, (t, even) in enumerate(cases):
+        got = pkg.Rotary._strides(t, t.shape)
+        assert (got is not None) == even, (n, t.shape, t.stride(), got)
+        if got is not None:
+            T = t.numel() // (t.shape[-2] * D)
+            at = (torch.arange(T)[:, None, None] * got[0] + torch.arange(t.shape[-2])[:, None] * got[1]
+                  + torch.arange(D) + t.storage_offset())
+            assert torch.equal(x.flatten()[at], t.reshape(T, -1, D)), n
+
+
 def test_no_cpu_fallback(pkg):
     import torch
     with pytest.raises(ValueError, match="device tensor"):
