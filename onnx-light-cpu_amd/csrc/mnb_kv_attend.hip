@@ -16,7 +16,10 @@
 // above it, until a tile has weights that fp16 might not hold.
 // Queries are scaled by a power of two to below 2^15 and rounded to one fp16 term
 // (exact for fp16, and for bf16 down to 2^-31 of the row's largest magnitude) or,
-// fp32, to two (22 bits); P likewise is one term or, fp32, two.
+// fp32, to two (22 bits). P is two terms (22 bits) for fp32 and fp16 results: one, of 11
+// bits, is as coarse as an fp16 result itself, and made its error 1.4 times its own
+// rounding's (2048 tokens over 16384: 733 us, 552 with one; a token of each of 32 sequences
+// there 193 and 194). It is one for bf16, whose results have 8 bits: there it adds 1%.
 #include "mnb_kv.h"
 #include "mnb_values.h"
 
@@ -40,6 +43,10 @@ constexpr float kShift = 12.0f;    // P is 2^12 where y is m
 
 template <typename T>
 constexpr int Terms() { return sizeof(T) == 4 ? 2 : 1; }
+
+// Terms of a weight.
+template <typename T>
+constexpr int WeightTerms() { return std::is_same<T, __bf16>::value ? 1 : 2; }
 
 // Two codes' words -> the eight values, in order.
 __device__ __forceinline__ half8v Widen8(uint32_t lo, uint32_t hi) {
@@ -242,7 +249,7 @@ __host__ __device__ inline Units RowUnits(const Cache &c, int q_heads, int per) 
 template <typename T, int DP, int MT>
 __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work work, int row_tiles,
                                                               int64_t unit0) {
-  constexpr int kTerms = Terms<T>();
+  constexpr int kTerms = Terms<T>(), kWeights = WeightTerms<T>();
   constexpr int KS = DP / 64;      // 16-byte pieces of a key that a lane holds
   constexpr int VD = DP / 16;      // values of a token that a lane holds, tiles of O^T
   constexpr int VW = VD / 4;       // the same in words
@@ -433,7 +440,7 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
     // Some row does not see some token.
     const bool edge = !whole || t0 + kTile - 1 > reach.pmin || t0 + kTile > reach.end ||
                       (a.window > 0 && t0 <= reach.pmax - a.window);
-    half8v p[MT][2][kTerms];
+    half8v p[MT][2][kWeights];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
       if (edge) {
@@ -463,7 +470,7 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
             part[sub] += w;
             const _Float16 hi = static_cast<_Float16>(w);
             p[t][sub >> 1][0][4 * (sub & 1) + i] = hi;
-            if constexpr (kTerms == 2)
+            if constexpr (kWeights == 2)
               p[t][sub >> 1][1][4 * (sub & 1) + i] =
                   static_cast<_Float16>(w - static_cast<float>(hi));
           }
@@ -565,7 +572,7 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
 #pragma unroll
           for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int term = 0; term < kTerms; ++term)
+            for (int term = 0; term < kWeights; ++term)
               o[t][4 * y + b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p[t][pair][term],
                                                                        o[t][4 * y + b], 0, 0, 0);
         }
@@ -646,7 +653,7 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work, int row_tiles,
                                                              int64_t unit0) {
-  constexpr int kTerms = Terms<T>();
+  constexpr int kTerms = Terms<T>(), kWeights = WeightTerms<T>();
   constexpr int kThreadsT = 64 * NW;
   constexpr int KP = DP / 16;                  // 16-code pieces of a key, steps of Q K^T
   constexpr int DT = DP / 32;                  // tiles of O^T
@@ -867,7 +874,7 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
-  half8v p[4][kTerms];
+  half8v p[4][kWeights];
   float m = -kInf, l = 0.0f;
 
   // Where this lane reads: the other tokens, values and half lie at constant distances.
@@ -903,15 +910,16 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
 #pragma unroll
     for (int i = 0; i < kAll; ++i) {
       __builtin_amdgcn_sched_barrier(0);
+      if (i < kFirst) {
 #pragma unroll
-      for (int term = 0; term < kTerms; ++term) {
-        if (i < kFirst) {
+        for (int term = 0; term < kTerms; ++term)
           sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[i % kAhead], q[i >> 1][term],
                                                              sc[i & 1], 0, 0, 0);
-        } else {
-          const int j = (i - kFirst) / DT, d = (i - kFirst) % DT;
+      } else {
+        const int j = (i - kFirst) / DT, d = (i - kFirst) % DT;
+#pragma unroll
+        for (int term = 0; term < kWeights; ++term)
           o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[i % kAhead], p[j][term], o[d], 0, 0, 0);
-        }
       }
       if (i + kAhead < kAll) read(i + kAhead);
     }
@@ -950,7 +958,7 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
         float y[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = sc[j >> 1][8 * (j & 1) + e];
-        part[j] = Weights<kTerms>(y, scale[j], in[j].y - top + kShift, p[j]);
+        part[j] = Weights<kWeights>(y, scale[j], in[j].y - top + kShift, p[j]);
       }
     };
     make(m);
@@ -981,7 +989,7 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int term = 0; term < kTerms; ++term) __asm__ volatile("" : "+v"(p[j][term]));
+      for (int term = 0; term < kWeights; ++term) __asm__ volatile("" : "+v"(p[j][term]));
   };
   const auto spoil = [&](int n) {  // NaN values of tile n, to the rows that see them
     if (any_nan[n & 3] != 0) {

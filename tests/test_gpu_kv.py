@@ -303,6 +303,27 @@ def test_pages_of_zeros(pkg, cuda, news, dtype):
     _check_attend(pkg, cuda, 4, 2, 64, 32, [110, 200], news, dtype, seed=35, spoil=zeros)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("news,lengths", [([1, 1, 1, 1], [2, 3, 4, 7]), ([9], [12]), ([40], [40]),
+                                          ([150], [150])])
+def test_weights_of_float16_rows(pkg, cuda, D, news, lengths):
+    """A float16 result is as exact as its own rounding: half a step of the value, and what an
+    fp32 result may be off by (its weights have 22 bits as well). Positive values, so that no
+    weight's rounding is undone by another's, of few keys."""
+    import torch
+    page, B = 16, len(lengths)
+    table, pages = _table(B, -(-max(lengths) // page), 1, D)
+    cache = _cache(pkg, pages, 1, page, D, cuda, D)
+    cache.v.view(torch.uint8).bitwise_and_(0x7F)
+    Q = _rand((sum(news), 4, D), D + 1, cuda, 0.3).to(torch.float16)
+    starts = [sum(news[:b]) for b in range(B + 1)]
+    got = cache.attend(Q, _i32(table, cuda), _i32(lengths, cuda), starts=_i32(starts, cuda))
+    y, tol = _attend64(Q.cpu(), _values(cache.k, cache.k_scales), _values(cache.v, cache.v_scales),
+                       table, _spans(len(Q), lengths, starts), D ** -0.5, 0, torch.float32)
+    half = torch.exp2(torch.floor(torch.log2(y.abs() + tol)).clamp(min=-14.0) - 11.0)
+    assert ((got.cpu().double() - y).abs() <= half + tol).all()
+
+
 def test_huge_queries(pkg, cuda):
     """fp32 and bf16 queries far beyond fp16's range, undone by the scale."""
     for dtype in ("float32", "bfloat16"):
