@@ -7,8 +7,8 @@
  * of any length. The scales that mnb_kv_append makes are powers of two (e4m3's
  * precision does not depend on where in its range a value lies, so they lose
  * nothing, and a page whose scale grows is re-rounded exactly, but for values that become
- * subnormal); mnb_kv_attend takes any from 2^-100 up, and 0 for a page whose
- * codes are 0.
+ * subnormal); mnb_kv_attend takes any from 2^-100 to 2^100, powers of two to 2^120, and
+ * 0 for a page whose codes are 0.
  *
  * It stands between the QKV projection (mnb.h, mnb_fp8.h), whose rows
  * mnb_rotary turns in place, and the output projection. ONNX's Attention-24 is

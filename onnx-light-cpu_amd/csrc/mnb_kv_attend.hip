@@ -41,6 +41,12 @@ constexpr int kThreads = 64 * kWaves;
 constexpr float kInf = __builtin_inff();
 constexpr float kShift = 12.0f;    // P is 2^12 where y is m
 
+// The weights' sums count P / w in units of 2^16. P is below 65504 / 4 on average (Fits), so
+// 2^30 tokens of the least scale, 2^-100, stay below 2^128, and one of the largest that append
+// makes, 2^120, whose P is 2^11, is 2^-125. (An exponent that an instruction can hold: as a
+// factor it took two registers more, and 16 drafted tokens of 8 sequences at 16384 121 us for 113.)
+__device__ __forceinline__ float InSumUnits(float v) { return ldexpf(v, -16); }
+
 template <typename T>
 constexpr int Terms() { return sizeof(T) == 4 ? 2 : 1; }
 
@@ -417,7 +423,7 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
     const bool there = page != ~0u;
     const float value = ValueScale(sv);
     const float lane_ks = there ? sk : 1.0f, lane_ev = there ? Log2Scale(value) : -kInf;
-    const float lane_inv = there ? 1.0f / value : 0.0f;
+    const float lane_inv = there ? InSumUnits(1.0f / value) : 0.0f;
     const bool whole = __all(there);
     float ks[4], ev[4], inv[4];
 #pragma unroll
@@ -625,7 +631,7 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
       const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
       T *y = static_cast<T *>(a.y) + at * c.dim + d0;
 #pragma unroll
-      for (int d = 0; d < VD; ++d) y[d] = static_cast<T>(v[d] * by);
+      for (int d = 0; d < VD; ++d) y[d] = static_cast<T>(InSumUnits(v[d]) * by);
     } else {
       const int64_t part = PartOf(a, work, s, i, h * group + g) + split * PartStep(a, work);
       if (d0 == 0) work.part.ml[part] = make_float2(top, sum);
@@ -689,7 +695,7 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
   // units of eight values: neighbouring lanes' units lie in different banks.
   constexpr uint32_t kHalf = kTile * DP * 2;
   __shared__ __attribute__((aligned(256))) uint8_t tiles_of[4 * kHalf];
-  // Of 16 tokens: the keys' scale, log2 and inverse of the values'.
+  // Of 16 tokens: the keys' scale, log2 and inverse (in sum units) of the values'.
   __shared__ float4 info[4][4];
   // NaN values are kept apart: a tile's tokens that have one, by d, and whether any has.
   // Four tiles' records, for one is made while readers of others are behind.
@@ -808,8 +814,9 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
       WriteLds((off + kto[k]) ^ 16, Widen8(kw[k][2], kw[k][3]));
       if ((64 * wave + k * kThreadsT) % DP == 0 && lane == 0) {
         const float value = ValueScale(sv[k]);
-        info[n & 3][grp[k]] = good ? make_float4(sk[k], Log2Scale(value), 1.0f / value, 0.0f)
-                                   : make_float4(1.0f, -kInf, 0.0f, 0.0f);
+        info[n & 3][grp[k]] =
+            good ? make_float4(sk[k], Log2Scale(value), InSumUnits(1.0f / value), 0.0f)
+                 : make_float4(1.0f, -kInf, 0.0f, 0.0f);
       }
     }
   };
@@ -1067,8 +1074,9 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
             floatx4v{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
       } else {
         typedef T Vec __attribute__((ext_vector_type(4)));
-        const Vec y = {static_cast<T>(o[d][e] * by), static_cast<T>(o[d][e + 1] * by),
-                       static_cast<T>(o[d][e + 2] * by), static_cast<T>(o[d][e + 3] * by)};
+        Vec y;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) y[x] = static_cast<T>(InSumUnits(o[d][e + x]) * by);
         *reinterpret_cast<Vec *>(static_cast<T *>(a.y) + at * c.dim + d0) = y;
       }
     }
@@ -1152,7 +1160,7 @@ __global__ __launch_bounds__(kThreads) void JoinKernel(Attend a, Work work, int6
   const float over = sum == 0.0f ? 0.0f : 1.0f / sum;
   T *y = static_cast<T *>(a.y) + row * dim + d;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(v[e] * over);
+  for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(InSumUnits(v[e]) * over);
 }
 
 // How a call is launched: for sequences of at most `few` rows to a cache head

@@ -324,6 +324,26 @@ def test_weights_of_float16_rows(pkg, cuda, D, news, lengths):
     assert ((got.cpu().double() - y).abs() <= half + tol).all()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("news", [1, 100, 150])
+@pytest.mark.parametrize("exponent", [-100, -64, 0, 100, 120])
+def test_ends_of_value_scales(pkg, cuda, exponent, news, dtype):
+    """The least and the largest value scales, 2^18 keys of one weight: the weights' sum, which
+    is divided by the scale, neither overflows nor vanishes. Values of 1, so that all sums are
+    whole multiples of one power of two: only the division and Y round."""
+    import torch
+    page, D, width = 256, 64, 1024
+    cache = pkg.Fp8KVCache(1, 1, D, page, device=cuda)
+    cache.k.view(torch.uint8).fill_(0x38)  # 1.0
+    cache.v.view(torch.uint8).fill_(0x38)
+    cache.k_scales.fill_(1.0)
+    cache.v_scales.fill_(2.0 ** exponent)
+    table = torch.zeros(1, width, dtype=torch.int32, device=cuda)  # one page for all
+    Q = _rand((news, 1, D), 90, cuda).to(getattr(torch, dtype))
+    got = cache.attend(Q, table, _i32([width * page], cuda), scale=0.0).double()
+    assert ((got - 2.0 ** exponent).abs() <= 2.0 ** (exponent - 22)).all()
+
+
 def test_huge_queries(pkg, cuda):
     """fp32 and bf16 queries far beyond fp16's range, undone by the scale."""
     for dtype in ("float32", "bfloat16"):
