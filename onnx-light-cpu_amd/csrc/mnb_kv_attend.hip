@@ -115,6 +115,13 @@ __device__ __forceinline__ float Log2Scale(float w) {
   return static_cast<float>(e - 1) + log2f(2.0f * m);
 }
 
+// What a page's scales add to the scores of its tokens: log2 of the values', or something that
+// is not below infinity where they are no numbers (a negative one of values is none).
+__device__ __forceinline__ float ScoreAdd(float key, float value) {
+  return fabsf(key) < kInf ? Log2Scale(value) : __builtin_nanf("");
+}
+__device__ __forceinline__ bool NoScale(float add) { return !(add < kInf); }
+
 // The power of two by which a row of queries with this largest magnitude is
 // multiplied; fp16 rows are taken as they are.
 template <typename T>
@@ -422,9 +429,17 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
     // The scales' part in scores and weights, made by the lanes that hold them.
     const bool there = page != ~0u;
     const float value = ValueScale(sv);
-    const float lane_ks = there ? sk : 1.0f, lane_ev = there ? Log2Scale(value) : -kInf;
-    const float lane_inv = there ? InSumUnits(1.0f / value) : 0.0f;
-    const bool whole = __all(there);
+    const float lane_ks = there ? sk : 1.0f;
+    float lane_ev = there ? ScoreAdd(sk, value) : -kInf;
+    float lane_inv = there ? InSumUnits(1.0f / value) : 0.0f;
+    // Some row does not see some token.
+    const bool edge = !__all(there) || t0 + kTile - 1 > reach.pmin || t0 + kTile > reach.end ||
+                      (a.window > 0 && t0 <= reach.pmax - a.window);
+    // Scales that are no numbers reach the rows that see their tokens, through the scores.
+    const bool lane_none = edge && NoScale(lane_ev);
+    const uint64_t none = __ballot(lane_none);
+    lane_ev = lane_none ? 0.0f : lane_ev;
+    lane_inv = lane_none ? 0.0f : lane_inv;
     float ks[4], ev[4], inv[4];
 #pragma unroll
     for (int sub = 0; sub < 4; ++sub) {
@@ -443,9 +458,6 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
     // not be one for those.
     if (more) next = find(step + 2 * kWaves);
 
-    // Some row does not see some token.
-    const bool edge = !whole || t0 + kTile - 1 > reach.pmin || t0 + kTile > reach.end ||
-                      (a.window > 0 && t0 <= reach.pmax - a.window);
     half8v p[MT][2][kWeights];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
@@ -461,6 +473,14 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
             acc[t][sub][i] = seen ? acc[t][sub][i] : -kInf;
           }
         __asm__ volatile("");  // a branch, not selects
+        if (none != 0) {
+#pragma unroll
+          for (int sub = 0; sub < 4; ++sub)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if ((none >> (16 * sub) & 1) != 0 && acc[t][sub][i] != -kInf)
+                acc[t][sub][i] = __builtin_nanf("");
+        }
       }
       float scale[4], part[4];
 #pragma unroll
@@ -815,7 +835,7 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
       if ((64 * wave + k * kThreadsT) % DP == 0 && lane == 0) {
         const float value = ValueScale(sv[k]);
         info[n & 3][grp[k]] =
-            good ? make_float4(sk[k], Log2Scale(value), InSumUnits(1.0f / value), 0.0f)
+            good ? make_float4(sk[k], ScoreAdd(sk[k], value), InSumUnits(1.0f / value), 0.0f)
                  : make_float4(1.0f, -kInf, 0.0f, 0.0f);
       }
     }
@@ -954,6 +974,15 @@ __global__ __launch_bounds__(64 * NW) void AttendTileKernel(Attend a, Work work,
           sc[j][e] = tok <= hi && tok > lo ? sc[j][e] : -kInf;
         }
       __asm__ volatile("");  // a branch: as selects this would take as long as the rest
+      // Scales that are no numbers reach the rows that see their tokens, through the scores.
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (NoScale(in[j].y)) {
+#pragma unroll
+          for (int e = 8 * (j & 1); e < 8 * (j & 1) + 8; ++e)
+            sc[j >> 1][e] = sc[j >> 1][e] == -kInf ? -kInf : __builtin_nanf("");
+          in[j].y = in[j].z = 0.0f;
+        }
     }
     float scale[4];
 #pragma unroll

@@ -372,6 +372,46 @@ def test_nan_in_later_tokens(pkg, cuda, D, news, window):
     assert got[news[0] - 3, :2, 3].isnan().all() and got[news[0] - 1, :2].isnan().all()
 
 
+@pytest.mark.parametrize("dtype,D", [("bfloat16", 64), ("float16", 128), ("float32", 128),
+                                     ("bfloat16", 256)])
+@pytest.mark.parametrize("news", [[1, 2], [40, 30], [150, 9]])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, -1.0])
+def test_scales_of_unseen_pages(pkg, cuda, news, bad, dtype, D):
+    """Pages that lie before the window, in its first tile, hold anything: codes and scales."""
+    lengths, window, page = [300, 180], 37, 16
+
+    def spoil(table, cache, Q):
+        for b, (n, length) in enumerate(zip(news, lengths)):
+            for p in range((length - n - window + 1) // page):
+                for codes, scales in ((cache.k, cache.k_scales), (cache.v, cache.v_scales)):
+                    codes.view(torch.uint8)[table[b][p]] = 0x7F
+                    scales[table[b][p]] = bad
+
+    import torch
+    got = _check_attend(pkg, cuda, 4, 2, D, page, lengths, news, dtype, window=window, seed=45,
+                        spoil=spoil)
+    assert got.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype,D", [("bfloat16", 64), ("float32", 128), ("bfloat16", 256)])
+@pytest.mark.parametrize("window", [0, 50])
+@pytest.mark.parametrize("new", [40, 150])
+@pytest.mark.parametrize("which", ["k_scales", "v_scales"])
+def test_nan_scales_of_later_pages(pkg, cuda, which, new, window, dtype, D):
+    """A page whose scale is NaN is the trouble of the rows that see it, and of no other."""
+    length, page, at = 170, 16, 10
+
+    def spoil(table, cache, Q):
+        getattr(cache, which)[table[0][at], 0] = math.nan
+
+    got = _check_attend(pkg, cuda, 4, 2, D, page, [length], [new], dtype, window=window, seed=46,
+                        spoil=spoil)
+    for i in range(new):
+        pos = length - new + i
+        sees = pos >= at * page and (window == 0 or pos - window < (at + 1) * page - 1)
+        assert got[i, :2].isnan().all() == sees and got[i, 2:].isfinite().all()
+
+
 def test_infinite_queries(pkg, cuda):
     """A row whose query is not finite is its own trouble."""
     import torch
