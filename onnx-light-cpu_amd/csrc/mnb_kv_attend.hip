@@ -436,10 +436,8 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
     const bool edge = !__all(there) || t0 + kTile - 1 > reach.pmin || t0 + kTile > reach.end ||
                       (a.window > 0 && t0 <= reach.pmax - a.window);
     // Scales that are no numbers reach the rows that see their tokens, through the scores.
-    const bool lane_none = edge && NoScale(lane_ev);
-    const uint64_t none = __ballot(lane_none);
-    lane_ev = lane_none ? 0.0f : lane_ev;
-    lane_inv = lane_none ? 0.0f : lane_inv;
+    const uint64_t none = edge ? __ballot(NoScale(lane_ev)) : 0;
+    if (none != 0 && NoScale(lane_ev)) lane_ev = lane_inv = 0.0f;
     float ks[4], ev[4], inv[4];
 #pragma unroll
     for (int sub = 0; sub < 4; ++sub) {
