@@ -126,7 +126,7 @@ __device__ __forceinline__ bool NoScale(float add) { return !(add < kInf); }
 // multiplied; fp16 rows are taken as they are.
 template <typename T>
 __device__ __forceinline__ int QueryShift(uint32_t top) {
-  return std::is_same<T, _Float16>::value ? 0 : RangeExponent(__uint_as_float(top), 14);
+  return std::is_same<T, _Float16>::value ? 0 : SplitExponent(__uint_as_float(top), 14);
 }
 
 // What turns a dot product of such a row with key codes into log2 of a weight, but for
@@ -148,7 +148,10 @@ __device__ __forceinline__ void SplitQuery(const float (&f)[8], int shift, float
     const float v = ldexpf(f[e] * sign, shift);
     const _Float16 hi = static_cast<_Float16>(v);
     q[0][e] = hi;
-    if constexpr (TERMS == 2) q[1][e] = static_cast<_Float16>(v - static_cast<float>(hi));
+    if constexpr (TERMS == 2) {
+      const float rest = v - static_cast<float>(hi);
+      q[1][e] = static_cast<_Float16>(rest == rest ? rest : 0.0f);  // an infinity has none
+    }
   }
 }
 

@@ -434,6 +434,30 @@ def test_infinite_queries(pkg, cuda):
     assert torch.equal(got[good], clean[good])
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("new", [3, 40, 150])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_scores_of_minus_infinity(pkg, cuda, D, new, dtype):
+    """A query with an infinity where all keys are negative: only scores of -inf, a row of
+    0, however large the query's other values; where all are positive, NaN."""
+    import torch
+    dtype, length, page = getattr(torch, dtype), 160, 32
+    table, pages = _table(1, 5, 1, 47)
+    cache = _cache(pkg, pages, 1, page, D, cuda, 47)
+    cache.k.view(torch.uint8)[..., 3] = 0xB8  # -1.0
+    cache.k.view(torch.uint8)[..., 4] = 0x38  # 1.0
+    Q = _rand((new, 4, D), 48, cuda).to(dtype)
+    Q[:, 1, 3] = math.inf
+    Q[:, 2, 3] = math.inf
+    Q[:, 2, 5:9] = 60000.0 if dtype == torch.float16 else 1e6
+    Q[:, 3, 4] = math.inf
+    args = (_i32(table, cuda), _i32([length], cuda))
+    got = cache.attend(Q, *args)
+    assert got[:, 0].isfinite().all() and (got[:, 1:3] == 0).all() and got[:, 3].isnan().all()
+    got = cache.attend(Q, *args, scale=-0.1)  # the signs the other way round
+    assert got[:, 0].isfinite().all() and got[:, 1:3].isnan().all() and (got[:, 3] == 0).all()
+
+
 @pytest.mark.parametrize("news", [[1, 1], [30, 60]])
 def test_pages_outside_the_cache(pkg, cuda, news):
     """Pages that the cache does not have are not seen: nothing is read there."""
