@@ -72,9 +72,10 @@ typedef struct mnb_kv_rows {
  * A page's scale is the least power of two, 2^-64 at least, that brings the
  * largest magnitude of its tokens to 448 or below, with s the scale that it had: a page
  * that begins with a new token starts anew, one that is continued takes no less
- * than s, and if it takes more its codes are re-rounded, code * s / scale. Codes
- * are rounded to nearest, ties to even. Infinities and NaN become NaN codes and
- * do not count for the scale. Runs on the current device, asynchronous on `stream`. */
+ * than s, power of two or not, and if it takes more its codes are re-rounded, code * s /
+ * scale. Codes are x / scale in fp32 (exact for powers of two) rounded to nearest, ties to
+ * even. Infinities and NaN become NaN codes and do not count for the scale. Runs on the
+ * current device, asynchronous on `stream`. */
 int mnb_kv_append(const mnb_kv_cache *cache, const mnb_kv_batch *batch, int32_t x_type,
                   const mnb_kv_rows *k, const mnb_kv_rows *v, void *stream);
 

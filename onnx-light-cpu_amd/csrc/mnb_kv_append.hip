@@ -24,11 +24,17 @@ __device__ __forceinline__ bool Finite(float x) {
   return (__float_as_uint(x) & 0x7FFFFFFFu) < 0x7F800000u;
 }
 
-// Sixteen codes of x times `by`, NaN where x is not finite.
-__device__ __forceinline__ uint4 Codes16(const float (&x)[16], float by) {
+// Sixteen codes of x / scale, NaN where x is not finite; by is 1 / scale. A scale that a page had
+// may be no power of two, and its reciprocal's rounding would move halves of a code's last
+// place to either side: the quotient's remainder, exact in one fma, corrects it.
+__device__ __forceinline__ uint4 Codes16(const float (&x)[16], float scale, float by) {
   float y[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) y[i] = Finite(x[i]) ? x[i] * by : __builtin_nanf("");
+  if ((__float_as_uint(scale) & 0x7FFFFFu) != 0) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) y[i] = fmaf(fmaf(-y[i], scale, x[i]), by, y[i]);
+  }
   uint4 r;
   r.x = Codes4(y[0], y[1], y[2], y[3]);
   r.y = Codes4(y[4], y[5], y[6], y[7]);
@@ -121,7 +127,7 @@ __global__ __launch_bounds__(kThreads) void AppendKernel(Cache c, Batch b, Rows 
     const int t = u / per, d = 16 * (u - t * per);
     float f[16];
     Load16(x + t * rows.token_stride + d, f);
-    reinterpret_cast<uint4 *>(codes)[lo * per + u] = Codes16(f, by);
+    reinterpret_cast<uint4 *>(codes)[lo * per + u] = Codes16(f, scale, by);
   }
   if (threadIdx.x == 0) c.scales[which][at] = scale;
 }

@@ -93,7 +93,7 @@ class Fp8KVCache:
     def from_tensors(cls, k, v, k_scales, v_scales):
         """A cache of tensors that exist (held, not copied); scales may be any
         numbers from 2^-100 to 2^100 (powers of two to 2^120), or 0 for a page of codes of
-        0; append makes powers of two."""
+        0. append makes powers of two, but a page that it continues keeps a larger scale."""
         import torch
         if k.dim() != 4:
             raise ValueError(f"{PREFIX}: k must be [pages, kv_heads, page_size, head_dim], got "

@@ -585,6 +585,27 @@ def test_append_borders_of_scales(pkg, cuda):
     _check_append(pkg, cuda, cache, _state(cache), X, table, [1] * len(tops), None, 16)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("scale", [1.0, 1.25, 1.375, 1.75, 1.1, 3.0 * 2.0 ** -9])
+def test_append_beside_other_scales(pkg, cuda, scale, dtype):
+    """A continued page keeps a scale that is no power of two: codes are the fp32 quotients',
+    halves of a code's last place to the even one."""
+    import torch
+    D, page = 64, 16
+    scale = torch.tensor(scale, dtype=torch.float32)
+    cache = pkg.Fp8KVCache(1, 1, D, page, device=cuda)
+    for s in (cache.k_scales, cache.v_scales):
+        s.fill_(scale.item())
+    # 17 / 16 and on: between two codes, at eight powers of two, below 448
+    halves = (torch.arange(17, 32, 2)[:, None] / 16 * torch.exp2(torch.arange(-2.0, 6.0))).reshape(1, D)
+    X = [(sign * halves * scale).to(getattr(torch, dtype)).repeat(4, 1)[:, None] for sign in (1, -1)]
+    cache.append(*(x.to(cuda) for x in X), _i32([[0]], cuda), _i32([9], cuda))
+    for x, codes, s in zip(X, (cache.k, cache.v), (cache.k_scales, cache.v_scales)):
+        assert s.item() == scale.item()
+        want = _e4m3((x.float() / scale).double())
+        assert torch.equal(_values(codes)[0, 0, 5:9], want[:, 0])
+
+
 def test_append_of_strided_and_batched_rows(pkg, cuda):
     """Views of a QKV projection's rows, misaligned rows, [sequences, tokens, ...]."""
     import torch
