@@ -144,17 +144,29 @@ hipError_t LaunchFor(Args &a, const mnb_rotary_desc &d, hipStream_t s) {
   // little more. Few tokens are shared by several workgroups. (6144 tokens and 64, 40 heads:
   // 23.0 and 4.3 us; four times as many items 23.5 and 5.2, a quarter 23.3 and 4.6.)
   a.tokens = std::max(1, std::min(2 * kThreads / items, 2 * kThreads / a.pairs));
-  const int64_t groups = (a.T + a.tokens - 1) / a.tokens;
   const int split = std::min(64, std::max(1, a.tokens * items / (2 * kThreads)));
   const bool vec = a.pairs % 8 == 0 && a.head_dim % 8 == 0 &&
                    VecPart(a.part[0], sizeof(T)) && VecPart(a.part[1], sizeof(T));
-  const dim3 grid(static_cast<unsigned>(groups), split);
   const size_t lds = sizeof(float2) * a.tokens * a.pairs;
-  if (vec)
-    hipLaunchKernelGGL((RotaryKernel<T, true, PAIRS>), grid, dim3(kThreads), lds, s, a, f);
-  else
-    hipLaunchKernelGGL((RotaryKernel<T, false, PAIRS>), grid, dim3(kThreads), lds, s, a, f);
-  return hipGetLastError();
+  // Tokens at a time, so that a grid's threads stay below 2^32.
+  const int64_t most = (int64_t{1} << 23) * a.tokens;
+  for (int64_t t = 0; t < a.T; t += most) {
+    Args b = a;
+    b.T = std::min(most, a.T - t);
+    b.pos = static_cast<const char *>(a.pos) + t * (a.pos64 ? 8 : 4);
+    for (Part &p : b.part) {
+      p.x = static_cast<const T *>(p.x) + t * p.xt;
+      p.y = static_cast<T *>(p.y) + t * p.yt;
+    }
+    const dim3 grid(static_cast<unsigned>((b.T + b.tokens - 1) / b.tokens), split);
+    if (vec)
+      hipLaunchKernelGGL((RotaryKernel<T, true, PAIRS>), grid, dim3(kThreads), lds, s, b, f);
+    else
+      hipLaunchKernelGGL((RotaryKernel<T, false, PAIRS>), grid, dim3(kThreads), lds, s, b, f);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 template <typename T>

@@ -168,6 +168,27 @@ def test_many_tokens(pkg, cuda):
     assert empty[0].shape == (0, 2, 64)
 
 
+def test_most_tokens(pkg, cuda):
+    """As many tokens as a call may have, each with so many heads that a workgroup has only
+    one: more workgroups than one launch takes. Against the same tokens a few at a time."""
+    import torch
+    T, H, D = 2 ** 24, 300, 2
+    op = pkg.Rotary(D, sections=(0, 1))
+    g = torch.Generator(device=cuda)
+    g.manual_seed(15)
+    x = torch.empty(T, H, D, dtype=torch.float16, device=cuda)  # 20 GB
+    x.view(-1, 4)[:] = torch.randn(4, device=cuda, generator=g).half()
+    x[:, :, 0] += (torch.arange(T, device=cuda) % 1009)[:, None].half() / 1024
+    pos = torch.randint(0, 10 ** 6, (2, T), dtype=torch.int32, device=cuda, generator=g)
+    at = torch.tensor([0, 1, 2 ** 23 - 1, 2 ** 23, 2 ** 23 + 1, T - 2, T - 1], device=cuda)
+    want = op(x[at], x[at, :1], pos[:, at])
+    K = x[:, :1].clone()
+    assert op(x, K, pos, out=(x, K))[0] is x
+    assert torch.equal(x[at], want[0]) and torch.equal(K[at], want[1])
+    del x, K
+    torch.cuda.empty_cache()
+
+
 def test_refusals(pkg, cuda):
     import torch
     op = pkg.Rotary(64, sections=(16, 16))
