@@ -1219,8 +1219,11 @@ Plan PlanOf(const Cache &c, const Batch &b, int32_t q_heads, int32_t x_type) {
   };
   int64_t few = rows;
   if (tiles && rows > 16 * most_mt) {
-    // Where ragged sequences are long or short, the short ones are taken to be decoded.
-    p.few = few = b.starts == nullptr ? 0 : group <= 16 ? 16 : 32;
+    // Where ragged sequences are long or short, the short ones are taken to be decoded. Tokens of
+    // more than 32 rows are sooner in the launch that there is for the prompts (48 heads on
+    // one, 8 sequences at 2000 tokens beside a prompt of 200: 56 us, 65 apart; 64 on each of two, 64
+    // sequences at 16000: 517, 715): then nothing is left for AttendSplitKernel, and it is not launched.
+    p.few = few = b.starts == nullptr || group > 32 ? 0 : group <= 16 ? 16 : 32;
     // Eight wavefronts share a tile's widening (2048 tokens over 16384: 547 us, 631 with
     // four); 128 rows leave half of them without any (4 x 32 tokens over 8192: 46 us, 58 with
     // eight), and two terms of fp32 need the registers.

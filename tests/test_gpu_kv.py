@@ -238,6 +238,15 @@ def test_prompts_beside_decoded_sequences(pkg, cuda, window, dtype):
                   window=window, seed=16, max_tokens=60)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("group", [17, 32, 33, 40, 48, 64, 65, 72])
+def test_many_heads_beside_a_prompt(pkg, cuda, group, dtype):
+    """Ragged calls with many query heads to a cache head: one token's rows are as many as a
+    tile of few rows, or more than any; long enough to be shared out."""
+    _check_attend(pkg, cuda, 2 * group, 2, 32, 64, [700, 1100, 0, 330], [12, 1, 1, 2], dtype,
+                  seed=group, max_tokens=12)
+
+
 def _many(B):
     """Rows and lengths of B sequences: one row, mostly, or none, and a few prompts."""
     news = [0 if b % 11 == 3 else 75 if b == B - 30 else 20 if b % 50 == 7 else 1 for b in range(B)]
