@@ -65,6 +65,30 @@ def _elsewhere(device, stream):
     return torch.cuda.stream(stream)
 
 
+_no_gradient = None  # the autograd function below
+
+
+def _without_gradient(prefix, call, *inputs):
+    """call()'s results, new tensors, for an operator without a gradient and inputs of
+    which some require one: backward() raises there instead of stopping without a word."""
+    global _no_gradient
+    if _no_gradient is None:
+        import torch
+
+        class NoGradient(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, prefix, call, *inputs):
+                ctx.prefix = prefix
+                return call()
+
+            @staticmethod
+            def backward(ctx, *gradients):
+                raise RuntimeError(f"{ctx.prefix}: the operator has no gradient")
+
+        _no_gradient = NoGradient
+    return _no_gradient.apply(prefix, call, *inputs)
+
+
 def _laid_out(shape, want):
     """Whether values of `shape` lie in memory as those of `want`: axes of 1 apart, the
     same one, or with neighbouring axes joined into one."""
@@ -269,8 +293,12 @@ class MatMulFp8:
 
     def run_rmsnorm(self, X, gamma, eps: float = 1e-5, residual=None, out_dtype=None, stream=None):
         """Y = this projection of rms_norm_fp8(X, gamma, eps, residual), the norm's input
-        of a decoder layer; of X's type, or out_dtype. With a residual: (Y, X + residual)."""
-        from .norm import rms_norm_fp8
+        of a decoder layer; of X's type, or out_dtype. With a residual: (Y, X + residual).
+        It has no gradient: backward() through a result raises."""
+        from .norm import _wants_gradient, rms_norm_fp8
+        if _wants_gradient(X, gamma, residual):
+            return _without_gradient("onnx_light_cpu_amd::MatMulFp8", lambda: self.run_rmsnorm(
+                X, gamma, eps, residual, out_dtype, stream), X, gamma, residual)
         codes, scales, *total = rms_norm_fp8(X, gamma, eps, residual=residual, stream=stream)
         Y = self(codes, scales=scales, out_dtype=out_dtype or X.dtype, stream=stream)
         return (Y, total[0]) if total else Y

@@ -4,7 +4,8 @@
 each page of tokens and head. ``append`` writes a call's new tokens, ``attend`` is
 the causal attention of their queries over the cache, from one token of each
 sequence to chunks of prompts, in one call for all sequences. Between them and a
-QKV projection stands ``Rotary``. There is no CPU fallback.
+QKV projection stands ``Rotary``. There is no CPU fallback, and no gradient: the cache
+holds values alone, and backward() through a result of ``attend`` raises.
 """
 from __future__ import annotations
 
@@ -12,7 +13,7 @@ import ctypes
 import math
 
 from . import MatMulNBits, _check, _raw_stream, library
-from .fp8 import _elsewhere, _shared_works
+from .fp8 import _elsewhere, _shared_works, _without_gradient
 
 PREFIX = "onnx_light_cpu_amd::Fp8KVCache"
 PAGE_SIZES = (16, 32, 64, 128, 256)
@@ -267,6 +268,11 @@ class Fp8KVCache:
                                 or not out.is_contiguous() or out.data_ptr() % 16 != 0):
             raise ValueError(f"{PREFIX}: out must be contiguous, of Q's shape, type and device, "
                              "aligned to 16 bytes")
+        if Q.requires_grad and torch.is_grad_enabled():
+            if out is not None:
+                raise ValueError(f"{PREFIX}: with out, Q must not require a gradient")
+            return _without_gradient(PREFIX, lambda: self.attend(
+                Q, table, lengths, starts, max_tokens, scale, window, stream=stream), Q)
         if stream is not None or (device.index is not None and device.index != _current_device()):
             self._batch(shape, table, lengths, starts, max_tokens)  # its refusals first
             elsewhere = _elsewhere(device, stream)

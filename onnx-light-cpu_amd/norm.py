@@ -4,14 +4,14 @@
 ``rms_norm`` rows of X's own type, as ``MatMulNBitsMoE`` takes them; with a
 residual both return the sum too, which the next residual addition needs.
 ``MatMulNBits.run_rmsnorm`` and ``MatMulFp8.run_rmsnorm`` take the norm with their
-product. There is no CPU fallback.
+product. There is no CPU fallback, and no gradient: backward() through a result raises.
 """
 from __future__ import annotations
 
 import ctypes
 
 from . import _check, _raw_stream, library
-from .fp8 import BLOCK, _elsewhere
+from .fp8 import BLOCK, _elsewhere, _without_gradient
 
 PREFIX = "onnx_light_cpu_amd::RmsNorm"
 _INF = float("inf")
@@ -32,6 +32,14 @@ def _library():
         _types = {torch.float32: 1, torch.float16: 10, torch.bfloat16: 16}
         _lib = L
     return _lib
+
+
+def _wants_gradient(X, gamma, residual):
+    if (X.requires_grad or gamma.requires_grad
+            or (residual is not None and residual.requires_grad)):
+        import torch
+        return torch.is_grad_enabled()
+    return False
 
 
 def _rows(X, K):
@@ -62,6 +70,9 @@ def _run(X, gamma, epsilon, residual, codes, stream):
         raise ValueError(f"{PREFIX}: residual must be of X's shape, type and device")
     if not 0.0 <= epsilon < _INF:
         raise ValueError(f"{PREFIX}: epsilon must be finite and not negative, got {epsilon}")
+    if _wants_gradient(X, gamma, residual):
+        return _without_gradient(PREFIX, lambda: _run(X, gamma, epsilon, residual, codes, stream),
+                                 X, gamma, residual)
     elsewhere = _elsewhere(device, stream)
     if elsewhere is not None:
         with elsewhere:

@@ -3,14 +3,15 @@
 ``Rotary`` turns the query and key heads of a QKV projection by their tokens'
 positions: one axis for text, three (time, row, column) for images and video.
 The frequencies are kept as turns in 64-bit fixed point, so that the angle of a
-far position is as exact as that of a near one. There is no CPU fallback.
+far position is as exact as that of a near one. There is no CPU fallback, and no gradient:
+backward() through a result raises.
 """
 from __future__ import annotations
 
 import ctypes
 import math
 from . import _check, _raw_stream, library
-from .fp8 import _elsewhere
+from .fp8 import _elsewhere, _without_gradient
 
 PREFIX = "onnx_light_cpu_amd::Rotary"
 MAX_PAIRS, MAX_AXES = 256, 8
@@ -169,6 +170,10 @@ class Rotary:
                         or (y.numel() and self._strides(y, shape) is None)):
                     raise ValueError(f"{PREFIX}: out must have {name}'s shape, type and device, "
                                      "and whole heads")
+        if (Q.requires_grad or (K is not None and K.requires_grad)) and torch.is_grad_enabled():
+            if out is not None:
+                raise ValueError(f"{PREFIX}: with out, Q and K must not require a gradient")
+            return _without_gradient(PREFIX, lambda: self(Q, K, positions, stream=stream), *parts)
         elsewhere = _elsewhere(device, stream)
         if elsewhere is not None:
             with elsewhere:

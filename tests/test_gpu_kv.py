@@ -864,3 +864,29 @@ def test_values_come_back(pkg, cuda):
         y = cache.attend(_rand((1, 6, D), 80, cuda).to(dtype), table, lengths)
         v = v.repeat_interleave(3, dim=1)
         assert ((y - v).abs() <= (2.0 ** -21 if dtype == torch.float32 else 0.0) * v.abs()).all()
+
+
+def test_no_gradient(pkg, cuda):
+    """Queries that require a gradient have their results; backward() says that there is none."""
+    import torch
+    table, pages = _table(2, 3, 0, 74)
+    cache = _cache(pkg, pages, 2, 32, 64, cuda, 74)
+    args = (_i32(table, cuda), _i32([90, 40], cuda))
+    Q = _rand((6, 8, 64), 75, cuda)
+    K = _rand((6, 2, 64), 76, cuda)
+    cache.append(K, K, *args)
+    want = cache.attend(Q, *args, window=30, scale=0.3)
+    Q.requires_grad_()
+    K.requires_grad_()
+    cache.append(K, K, *args)  # the cache holds values alone
+    assert not cache.k_scales.requires_grad
+    got = cache.attend(Q, *args, window=30, scale=0.3)
+    assert torch.equal(got, want) and got.requires_grad
+    with pytest.raises(RuntimeError, match="no gradient"):
+        got.sum().backward()
+    with pytest.raises(ValueError, match="must not require a gradient"):
+        cache.attend(Q, *args, out=torch.empty_like(want))
+    with torch.no_grad():
+        out = torch.empty_like(want)
+        assert cache.attend(Q, *args, window=30, scale=0.3, out=out) is out
+    assert torch.equal(out, want) and not out.requires_grad and Q.grad is None

@@ -171,3 +171,33 @@ def test_norm_of_a_projection(pkg, cuda):
     Y = op.run_rmsnorm(x.reshape(17, 1, K), gamma, out_dtype=torch.float32)
     codes, scales = pkg.rms_norm_fp8(x, gamma)
     assert torch.equal(Y.reshape(17, N), op(codes, scales=scales))
+
+
+@pytest.mark.parametrize("which", ["x", "gamma", "residual"])
+def test_no_gradient(pkg, cuda, which):
+    """What requires a gradient is taken, with the same results; backward() says that there is
+    none, and nothing is recorded where none is wanted."""
+    import torch
+    x, r, gamma = _problem(3, 256, torch.float32, cuda, 10)
+    W = torch.ones(128, 256, device=cuda).to(torch.float8_e4m3fn)
+    op = pkg.MatMulFp8(256, 128).prepare_device(W, torch.ones(1, 2, device=cuda))
+    calls = (lambda: pkg.rms_norm(x, gamma, residual=r), lambda: op.run_rmsnorm(x, gamma, residual=r),
+             lambda: pkg.rms_norm_fp8(x, gamma, residual=r)[1:],
+             lambda: (pkg.rms_norm(x, gamma, residual=r, stream=torch.cuda.current_stream())[0],))
+    want = [call() for call in calls]
+    {"x": x, "gamma": gamma, "residual": r}[which].requires_grad_()
+    for call, ys in zip(calls, want):
+        got = call()
+        assert len(got) == len(ys) and all(torch.equal(a, b) for a, b in zip(got, ys))
+        for y in got:
+            assert y.requires_grad
+            with pytest.raises(RuntimeError, match="no gradient"):
+                (y * 2.0).sum().backward(retain_graph=True)
+        with torch.no_grad():
+            assert not any(y.requires_grad for y in call())
+    if which != "residual":
+        y = pkg.rms_norm(x, gamma)
+        y += 1.0  # a result may be changed in place
+        with pytest.raises(RuntimeError, match="no gradient"):
+            y.sum().backward()
+    assert x.grad is None and gamma.grad is None

@@ -226,3 +226,33 @@ def test_stream_and_graph(pkg, cuda):
         torch.cuda.synchronize()
         want = op(q, k, pos)
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+def test_no_gradient(pkg, cuda):
+    """Q and K that require a gradient are turned all the same; backward() says that there is
+    none, and their own memory is not written behind the graph's back."""
+    import torch
+    op = pkg.Rotary(64)
+    q, k = _heads(5, 4, 64, torch.float32, cuda, 16), _heads(5, 2, 64, torch.float32, cuda, 17)
+    pos = torch.arange(5, device=cuda)
+    want = op(q, k, pos)
+    for leaf in (q, k):
+        leaf.requires_grad_()
+        got = op(q, k, pos)
+        assert all(torch.equal(a, b) and a.requires_grad for a, b in zip(got, want))
+        for y in got:
+            with pytest.raises(RuntimeError, match="no gradient"):
+                y.sum().backward(retain_graph=True)
+        with pytest.raises(ValueError, match="must not require a gradient"):
+            op(q, k, pos, out=(torch.empty_like(q), torch.empty_like(k)))
+        with torch.no_grad():
+            assert not op(q, k, pos)[0].requires_grad
+        leaf.requires_grad_(False)
+    q.requires_grad_()
+    alone = op(q, None, pos)
+    assert torch.equal(alone, want[0])
+    with pytest.raises(RuntimeError, match="no gradient"):
+        alone.sum().backward()
+    with torch.no_grad():
+        op(q, k, pos, out=(q, k))
+    assert torch.equal(q, want[0])
