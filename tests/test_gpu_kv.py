@@ -421,6 +421,76 @@ def test_nan_scales_of_later_pages(pkg, cuda, which, new, window, dtype, D):
         assert got[i, :2].isnan().all() == sees and got[i, 2:].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Hq,new,length,window", [(1, 600, 632, 0), (1, 600, 1000, 300), (1, 120, 400, 290),
+                                                  (4, 150, 400, 290), (4, 150, 182, 0)])
+def test_nan_in_many_tiles(pkg, cuda, Hq, new, length, window, D, dtype):
+    """NaN values in tile after tile that some of a workgroup's rows see and others do not,
+    five to nine of them: rows and channels of each are its own."""
+    def spoil(table, cache, Q):
+        v = cache.v.view(torch.uint8)
+        for t in range(5, length, 61):
+            v[table[0][t // 32], 0, t % 32, t * 7 % D] = 0x7F
+
+    import torch
+    got = _check_attend(pkg, cuda, Hq, 1, D, 32, [length], [new], dtype, window=window, seed=49,
+                        spoil=spoil)
+    assert got.isnan().any() and got.isfinite().any(dim=2).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("new", [100, 150])
+@pytest.mark.parametrize("q_size,scale,exponents", [(1e-4, 1e3, (-8, -3)), (300.0, 1e-3, (-8, -3)),
+                                                    (30.0, None, (-8, -3)), (1.0, 0.0, (-8, -3)),
+                                                    (1.0, -0.2, (-8, -3)), (1.0, 1e-6, (-30, 20))])
+def test_sizes_of_queries_and_values_of_prompts(pkg, cuda, q_size, scale, exponents, new, dtype):
+    """Sharp and flat weights, negative scales and pages of very different ones, where rows are
+    many: more than 64 and more than 128 to a cache head. Values up to 448 2^19 pass float16's
+    largest, 65504: from half a step above it, 65520, on a result is an infinity, and a result
+    that is within its tolerance of 65520 may be."""
+    import torch
+    dtype, page, D = getattr(torch, dtype), 16, 64
+    table, pages = _table(1, -(-(new + 30) // page), 2, 50)
+    cache = _cache(pkg, pages, 2, page, D, cuda, 50, exponents)
+    Q = _rand((new, 2, D), 59, cuda, q_size).to(dtype)
+    got = cache.attend(Q, _i32(table, cuda), _i32([new + 30], cuda), scale=scale).cpu().double()
+    y, tol = _attend64(Q.cpu(), _values(cache.k, cache.k_scales), _values(cache.v, cache.v_scales),
+                       table, [(0, new, new + 30)], D ** -0.5 if scale is None else scale, 0, dtype)
+    good = (got - y).abs() <= tol
+    if dtype == torch.float16:
+        inf = got == torch.copysign(torch.full_like(y, math.inf), y)
+        good = torch.where(y.abs() - tol >= 65520.0, inf, good | (inf & (y.abs() + tol >= 65520.0)))
+    assert good.all()
+
+
+@pytest.mark.parametrize("new", [100, 150])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_huge_queries_of_prompts(pkg, cuda, new, dtype):
+    _check_attend(pkg, cuda, 1, 1, 64, 16, [new + 30], [new], dtype, seed=51, q_size=1e20,
+                  scale=1e-21)
+
+
+@pytest.mark.parametrize("new", [100, 150])
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+def test_infinite_queries_of_prompts(pkg, cuda, new, dtype):
+    """Rows whose queries are not finite leave the others' bits alone."""
+    import torch
+    dtype = getattr(torch, dtype)
+    table, pages = _table(1, 6, 0, 52)
+    cache = _cache(pkg, pages, 1, 32, 64, cuda, 52)
+    args = (_i32(table, cuda), _i32([180], cuda))
+    Q = _rand((new, 2, 64), 53, cuda).to(dtype)
+    want = cache.attend(Q, *args)
+    bad = torch.zeros(new, 2, dtype=torch.bool, device=cuda)
+    for row, head, value in ((1, 0, math.inf), (2, 1, math.nan), (40, 0, -math.inf), (99, 1, math.nan)):
+        Q[row, head, row % 64] = value
+        bad[row, head] = True
+    got = cache.attend(Q, *args)
+    assert torch.equal(got[~bad], want[~bad])
+    assert got[2, 1].isnan().all() and got[99, 1].isnan().all()
+
+
 def test_infinite_queries(pkg, cuda):
     """A row whose query is not finite is its own trouble."""
     import torch
@@ -507,6 +577,57 @@ def test_lengths_and_starts_out_of_range(pkg, cuda, lengths, starts):
         out = torch.full_like(Q, 7.0)
         cache.attend(Q, *args, starts=_i32(starts, cuda), out=out)
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("lengths,starts", [
+    ([10 ** 9, -5], [0, 3, 6]), ([2 ** 31 - 1, -2 ** 31], [0, 3, 6]), ([20, 30], [0, 100, 200]),
+    ([20, 30], [-5, 2, 4]), ([70, 64], [1, 4, 9]), ([2, 0], [0, 3, 5]), ([20, 20], [-5, 2, -7]),
+    ([20, 20], [6, 3, 0]), ([20, 20], [2 ** 31 - 1, -2 ** 31, 5])])
+def test_rows_and_pages_outside_of_all_spans(pkg, cuda, lengths, starts):
+    """starts are held to 0 .. tokens, positions to the table: what lies outside stays as it
+    is, bit for bit, and the rows inside are those of a call of their own. (Falling starts may
+    leave rows out.)"""
+    import torch
+    page, width, T = 32, 2, 6
+    table, pages = _table(2, width, 1, 77)
+    cache = _cache(pkg, pages, 1, page, 64, cuda, 77)
+    X = [_rand((T, 1, 64), 78 + n, cuda) for n in range(2)]
+    Q = _rand((T, 2, 64), 80, cuda)
+    falling = any(a > b for a, b in zip(starts, starts[1:]))
+    spans = []
+    for b in range(2):
+        row = min(max(starts[b], 0), T)
+        spans.append((row, max(0, min(starts[b + 1], T) - row), max(0, lengths[b])))
+    args = (_i32(table, cuda), _i32(lengths, cuda))
+    state, before = _state(cache), [cache.k.view(torch.uint8).clone(), cache.v.view(torch.uint8).clone(),
+                                    cache.k_scales.clone(), cache.v_scales.clone()]
+    cache.append(*X, *args, starts=_i32(starts, cuda))
+    touched = torch.zeros(pages, dtype=torch.bool, device=cuda)
+    for b, (row, n, length) in enumerate(spans):
+        for i in range(n):
+            if 0 <= length - n + i < width * page:
+                touched[table[b][(length - n + i) // page]] = True
+    after = (cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scales, cache.v_scales)
+    for a, b in zip(before, after):
+        assert torch.equal(a[~touched], b[~touched])
+    if not falling:
+        for (values, scales), x, codes, s in zip(state, X, (cache.k, cache.v),
+                                                 (cache.k_scales, cache.v_scales)):
+            _append64(values, scales, x.cpu(), table, spans, page)
+            assert torch.equal(_values(codes), values) and torch.equal(s.cpu().double(), scales)
+
+    out = torch.full_like(Q, 7.0)
+    cache.attend(Q, *args, starts=_i32(starts, cuda), out=out)
+    inside = torch.zeros(T, dtype=torch.bool, device=cuda)
+    most = _values(cache.v, cache.v_scales).abs().max().item()
+    for b, (row, n, length) in enumerate(spans):
+        inside[row:row + n] = True
+        for i in range(0 if falling else n):
+            sees = min(length - n + i, width * page - 1) + 1
+            want = (cache.attend(Q[row + i:row + i + 1], args[0][b:b + 1], _i32([sees], cuda))[0]
+                    if sees > 0 else torch.zeros(2, 64, device=cuda))
+            assert ((out[row + i] - want).abs() <= 2.0 ** -16 * most).all()
+    assert (out[~inside] == 7.0).all()
 
 
 @pytest.mark.parametrize("split", [False, True])

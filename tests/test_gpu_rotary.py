@@ -86,6 +86,26 @@ def test_far_positions(pkg, cuda, pos):
     assert ((Q.cpu().double() - y).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("pos", [2 ** 31 - 1, 2 ** 40 + 12345, 2 ** 62, 2 ** 63 - 1, -2 ** 63, -7])
+def test_turns_of_far_positions(pkg, cuda, pos, interleaved):
+    """The angle is the position times the frequency as the object holds it, in units of 2^-64 of
+    a turn, with no rounding: the same tolerance at any position."""
+    import torch
+    op = pkg.Rotary(128, interleaved=interleaved)
+    q = _heads(1, 2, 128, torch.float32, cuda, 18)
+    got = op(q, None, torch.tensor([pos], device=cuda)).cpu().double()
+    x = q.cpu().double()
+    for j in range(64):
+        angle = float(Fraction(op._turns[j] * pos % 2 ** 64, 2 ** 64) * TWO_PI)
+        i0, i1 = (2 * j, 2 * j + 1) if interleaved else (j, j + 64)
+        u, v = x[0, :, i0], x[0, :, i1]
+        for i, y in ((i0, u * math.cos(angle) - v * math.sin(angle)),
+                     (i1, v * math.cos(angle) + u * math.sin(angle))):
+            tol = 2.0 ** -21 * (u.abs() + v.abs()) + 2.0 ** -24 * y.abs()
+            assert ((got[0, :, i] - y).abs() <= tol).all(), j
+
+
 def test_axes_by_sections_and_by_list(pkg, cuda):
     import torch
     T, D = 6, 64

@@ -77,6 +77,18 @@ def test_turns_are_frequencies_over_two_pi(pkg):
     assert r._turns[3] == 0
 
 
+def test_turns_are_the_nearest(pkg):
+    """Half a unit of 2^-64 of a turn is all that a frequency, a double, loses: 2^-65 |p| turns at
+    position p."""
+    from fractions import Fraction
+    two_pi = 2 * Fraction("3.14159265358979323846264338327950288419716939937510582097494")
+    for r in (pkg.Rotary(128), pkg.Rotary(64, base=5e5),
+              pkg.Rotary(8, inv_freq=[1e-9, 3.0, -2.5e4, 1e12])):
+        for f, turn in zip(r.inv_freq, r._turns):
+            off = (Fraction(f) / two_pi * 2 ** 64 - turn) % 2 ** 64
+            assert min(off, 2 ** 64 - off) <= Fraction(1, 2) + Fraction(1, 1000)
+
+
 def test_axes_of_frequencies(pkg):
     assert list(pkg.Rotary(16, sections=(2, 3, 3))._axis) == [0, 0, 1, 1, 1, 2, 2, 2]
     r = pkg.Rotary(16, rotary_dim=8, axes=(0, 1, 2, 0))
