@@ -183,7 +183,8 @@ class Fp8KVCache:
                 raise ValueError(f"{PREFIX}: starts must be int32 [{B + 1}] on {device}")
             if not starts.is_contiguous():
                 starts = starts.contiguous()
-            first, each = starts.data_ptr(), max_tokens or 0
+            # the C struct's field would cut a larger number to its low 64 bits
+            first, each = starts.data_ptr(), min(max_tokens or 0, tokens)
         elif even < 0:
             raise ValueError(f"{PREFIX}: {list(shape[:-2])} tokens are not the same number for each "
                              f"of {B} sequences")
@@ -260,6 +261,7 @@ class Fp8KVCache:
                              f"{heads}")
         if window < 0:
             raise ValueError(f"{PREFIX}: window must not be negative, got {window}")
+        window = min(window, 2 ** 31)  # more than any table reaches, and the C argument holds
         if scale is None:
             scale = self.head_dim ** -0.5
         elif not math.isfinite(scale):

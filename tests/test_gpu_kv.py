@@ -1011,3 +1011,18 @@ def test_no_gradient(pkg, cuda):
         out = torch.empty_like(want)
         assert cache.attend(Q, *args, window=30, scale=0.3, out=out) is out
     assert torch.equal(out, want) and not out.requires_grad and Q.grad is None
+
+
+@pytest.mark.parametrize("more", [2 ** 31, 2 ** 63, 2 ** 64, 2 ** 64 + 1, 10 ** 30])
+def test_numbers_past_64_bits(pkg, cuda, more):
+    """A window and a largest number of tokens beyond anything mean no limit, whatever is left of
+    them in 64 bits."""
+    import torch
+    table, pages = _table(2, 30, 0, 81)
+    cache = _cache(pkg, pages, 2, 64, 64, cuda, 81)
+    Q = _rand((7, 4, 64), 82, cuda)
+    args = (Q, _i32(table, cuda), _i32([1900, 60], cuda))
+    starts = _i32([0, 3, 7], cuda)
+    want = cache.attend(*args, starts=starts)
+    assert torch.equal(cache.attend(*args, starts=starts, window=more), want)
+    assert torch.equal(cache.attend(*args, starts=starts, max_tokens=more), want)
