@@ -90,10 +90,10 @@ int mnb_kv_workspace_bytes(const mnb_kv_cache *cache, const mnb_kv_batch *batch,
  * window > 0; beyond 2^30 it counts as 0) of scale * q . k_t, times v; heads is a
  * multiple of kv_heads, and query heads h use cache head h / (heads / kv_heads). A row
  * that sees no key, or only scores of -inf, is 0; unseen keys and values leave no trace,
- * NaN and infinities among them, in their scales too. Products are exact up to 2^-22 of q's largest magnitude
- * (fp32 q; fp16 and bf16 q: exact), the weights have 22 bits for an fp32 or fp16 Y and 11
- * for a bf16 one, sums are fp32. The value scales of one head and sequence lie within 2^100 of
- * each other. Runs on the current device, asynchronous on `stream`. */
+ * NaN and infinities among them, in their scales too. Products are exact for fp16 q, up to
+ * 2^-31 of q's largest magnitude for bf16 and up to 2^-22 for fp32; the weights have 22 bits
+ * for an fp32 or fp16 Y and 11 for a bf16 one; sums are fp32. The value scales of one head and
+ * sequence lie within 2^100 of each other. Runs on the current device, asynchronous on `stream`. */
 int mnb_kv_attend(const mnb_kv_cache *cache, const mnb_kv_batch *batch, int32_t heads,
                   int32_t x_type, const mnb_kv_rows *q, float scale, int64_t window, void *dY,
                   void *dWorkspace, size_t workspace_bytes, void *stream);

@@ -14,8 +14,11 @@
  * The reference has no counterpart.
  *
  * A frequency is given in turns: f_j / (2 pi) modulo 1, in units of 2^-64. A
- * position times it is the angle modulo a turn with no rounding at all, for any
- * 64-bit position, where fp32 angles lose a bit with each doubling.
+ * position times it is the angle modulo a turn with no rounding, for any 64-bit
+ * position. What is rounded is the frequency, by 2^-65 of a turn at most, which moves the
+ * angle of position p by 2^-65 |p| turns: less than fp32 results show up to |p| = 2^38,
+ * where fp32 angles lose a bit with each doubling from 1 on. cos and sin are off by less
+ * than 2^-23.
  *
  * Conventions of mnb.h hold (device pointers, void* streams, status codes,
  * checks before any HIP call).

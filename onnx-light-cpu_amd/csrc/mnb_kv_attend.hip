@@ -259,9 +259,10 @@ __host__ __device__ inline Units RowUnits(const Cache &c, int q_heads, int per) 
 // splits) where row_tiles is 0. A row is a token's query head of this cache head: row r is
 // token r / group, head r % group.
 // Memory bounds it: 32 sequences at 16384 tokens, 8 heads of 128, bf16, take 188 us (1.08 GB,
-// 5.7 TB/s; a copy reaches 4.7), 16 drafted tokens of 8
-// sequences there 114 with widening and weights in the way. One sequence at 8192 tokens has a
-// workgroup on each CU, each with two tiles a wavefront: 8.3 us, of which 3.6 are its bytes'.
+// 5.7 TB/s; a copy reaches 4.7), 16 drafted tokens of 8 sequences there 114 with widening and
+// weights in the way, one wavefront on a SIMD and, bf16, 20 spilled registers. One sequence at
+// 8192 tokens has a workgroup on each CU, each with two tiles a wavefront: 8.3 us, of which 3.6
+// are its bytes'.
 template <typename T, int DP, int MT>
 __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work work, int row_tiles,
                                                               int64_t unit0) {
@@ -674,7 +675,7 @@ __global__ __launch_bounds__(kThreads) void AttendSplitKernel(Attend a, Work wor
 // head's workgroups share an XCD's cache where there are eight; late rows, which see
 // the most keys, come first.
 // The matrix instructions bound it: 2048 bf16 tokens of 32 heads of 128 over 16384 keys take
-// 547 us, 0.94 PFLOP/s (a large library product reaches 1.2). The weights, their exponentials
+// 549 us, 0.94 PFLOP/s (a large library product reaches 1.2). The weights, their exponentials
 // first, take nearly as long as a tile's products, and run on the SIMD's other wavefront
 // meanwhile; with the halves of a workgroup not half a step apart it took 772.
 template <typename T, int DP, int NW>
@@ -1220,19 +1221,23 @@ Plan PlanOf(const Cache &c, const Batch &b, int32_t q_heads, int32_t x_type) {
   int64_t few = rows;
   if (tiles && rows > 16 * most_mt) {
     // Where ragged sequences are long or short, the short ones are taken to be decoded. Tokens of
-    // more than 32 rows are sooner in the launch that there is for the prompts (48 heads on
-    // one, 8 sequences at 2000 tokens beside a prompt of 200: 56 us, 65 apart; 64 on each of two, 64
-    // sequences at 16000: 517, 715): then nothing is left for AttendSplitKernel, and it is not launched.
+    // more than 32 rows are sooner in the launch that there is for the prompts (48 heads on one,
+    // 8 sequences at 2000 tokens beside a prompt of 200: 56 us, 65 apart; 64 on each of two, 64
+    // sequences at 16000: 517, 715): then nothing is left for AttendSplitKernel, and it is not
+    // launched.
     p.few = few = b.starts == nullptr || group > 32 ? 0 : group <= 16 ? 16 : 32;
-    // Eight wavefronts share a tile's widening (2048 tokens over 16384: 547 us, 631 with
+    // Eight wavefronts share a tile's widening (2048 tokens over 16384: 549 us, 631 with
     // four); 128 rows leave half of them without any (4 x 32 tokens over 8192: 46 us, 58 with
-    // eight), and two terms of fp32 need the registers.
+    // eight). fp32 keeps four: ragged calls, few long tiles, gain from narrow ones (a prompt of
+    // 200 beside 8 decoded sequences at 2000: 55 us, 76 with eight), prompts alone would from
+    // wide ones (1024 tokens over 8192: 358 us, 335; at head_dim 64 227, 176).
     p.waves = rows > 128 && !fp32 ? 8 : 4;
     const int64_t per = 32 * p.waves;
     p.tile_row_tiles = static_cast<int>(CeilDiv(rows, per));
     const int64_t filled = b.starts == nullptr ? b.sequences * p.tile_row_tiles
                                                : CeilDiv(b.tokens * group, per);
-    // One workgroup of eight wavefronts fits a CU, or two of four, or one for fp32. Four tiles
+    // One workgroup of eight wavefronts fits a CU, or two of four, or one of 128-wide fp32 or
+    // fp16 (301 and 259 registers). Four tiles
     // at least are worth a part (32 to 128 tokens of one sequence over 4096: 25 to 33 us, 30 to
     // 36 with eight, 27 to 32 with two); eight of fp32 (128 tokens: 39 us, 51 with four).
     p.tile_splits = parts(filled * c.heads, fp32 || p.waves == 8 ? 256 : 512, fp32 ? 8 : 4);
@@ -1243,9 +1248,12 @@ Plan PlanOf(const Cache &c, const Batch &b, int32_t q_heads, int32_t x_type) {
   if (few > 0) {
     p.mt = static_cast<int>(std::min<int64_t>(most_mt, CeilDiv(few, 16)));
     p.row_tiles = static_cast<int>(CeilDiv(few, 16 * p.mt));
-    // Workgroups for three on each CU, which fit (for two or six the times are the same,
-    // within 1%; six have twice the parts); a part's sums are as large as mt tiles of keys
-    // for each of its wavefronts.
+    // Three workgroups to a CU, where mt 1 lets two stay at a time and others one: short calls
+    // do not depend on it, long ones want as many as stay or fewer, those that divide badly
+    // more (for one, two, three and six to a CU, us: 16 drafted tokens of 8 sequences at 16384
+    // 80, 96, 114, 127; a token of 32 there 185, 193, 193, 195; of 16 at 8192 and head_dim 256,
+    // 16 heads on 4, 51, 56, 62, 87; of 12 at 8192 43, 40, 39, 41). A part's sums are as large
+    // as mt tiles of keys for each of its wavefronts.
     p.splits = parts(static_cast<int64_t>(b.sequences) * c.heads * p.row_tiles, 3 * 256,
                      kWaves * p.mt);
   }

@@ -27,8 +27,8 @@ struct Args {
 // units stays in registers between the sum of its squares and its second use, one
 // read of X and R and one write of each result; NV == 0: longer rows are read
 // again (h from where it was stored). Many rows are bound by memory: 8192 rows of 4096,
-// bf16, with residual and codes take 43 us (236 MB, 5.4 TB/s), 333 fp32 rows of 2500
-// 4.5. Few are one round trip to memory and the sum's: one row of 4096 3.0 us.
+// bf16, with residual and codes take 48 us (236 MB, 4.9 TB/s; 43 over and over, where the
+// last cache holds most of them), 333 fp32 rows of 2500 4.4. Few are one round trip to memory and the sum's: one row of 4096 3.0 us.
 template <typename T, bool VEC, bool CODES, int NV>
 __global__ __launch_bounds__(kMaxThreads) void RmsNormKernel(Args a) {
   constexpr int kUnits = NV > 0 ? NV : 1;
@@ -111,7 +111,7 @@ hipError_t Launch(Args a, int64_t M, hipStream_t s) {
   const int waves = static_cast<int>(std::min<int64_t>(kMaxThreads / 64, (units + 63) / 64));
   int threads = 64 * waves;
   // Many rows: fewer threads with more units each, so that a CU holds several rows (8192 rows
-  // of 4096: 43.3 us, 46.4 with a unit a thread; 600 rows 6.5 and 6.7). Few rows are done
+  // of 4096, over and over: 43.3 us, 46.4 with a unit a thread; 600 rows 6.5 and 6.7). Few rows are done
   // sooner with a unit a thread (256 rows of 8192: 5.7 us, 8.6 with four).
   if (M > 512)
     while (threads > 256 && (threads / 2) % 64 == 0 && units <= 4 * (threads / 2)) threads /= 2;

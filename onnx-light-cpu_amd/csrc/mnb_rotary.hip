@@ -60,8 +60,9 @@ __device__ __forceinline__ float2 CosSin(uint64_t turn) {
 // A workgroup first makes the cos and sin of its tokens in LDS, once for all
 // heads (one 64-bit product, 30 operations a pair), then turns the heads: an
 // item is one head's eight pairs, two loads and two stores of 16 bytes for 16-bit
-// types. Memory bounds it: 6144 tokens of 40 heads of 128, bf16, take 23 us (126 MB,
-// 5.5 TB/s); 64 tokens 4.3, which is the launch and three trips to memory one after another.
+// types. Memory bounds it: 6144 tokens of 40 heads of 128, bf16, take 24 us (126 MB,
+// 5.1 TB/s; 21 over and over, from the last cache in part); 64 tokens 4.3, which is the launch
+// and three trips to memory one after another.
 template <typename T, bool VEC, int PAIRS>
 __global__ __launch_bounds__(kThreads) void RotaryKernel(Args a, Frequencies<PAIRS> f) {
   extern __shared__ float2 table[];  // [tokens][pairs]
@@ -141,8 +142,8 @@ hipError_t LaunchFor(Args &a, const mnb_rotary_desc &d, hipStream_t s) {
   std::copy_n(d.axis, a.pairs, f.axis);
   const int items = a.heads * ((a.pairs + 7) / 8 + (a.head_dim - 2 * a.pairs + 15) / 16);
   // About two items a thread; the table of cos and sin has one entry a thread or
-  // little more. Few tokens are shared by several workgroups. (6144 tokens and 64, 40 heads:
-  // 23.0 and 4.3 us; four times as many items 23.5 and 5.2, a quarter 23.3 and 4.6.)
+  // little more. Few tokens are shared by several workgroups. (6144 tokens and 64, 40 heads,
+  // over and over: 23.0 and 4.3 us; four times as many items 23.5 and 5.2, a quarter 23.3 and 4.6.)
   a.tokens = std::max(1, std::min(2 * kThreads / items, 2 * kThreads / a.pairs));
   const int split = std::min(64, std::max(1, a.tokens * items / (2 * kThreads)));
   const bool vec = a.pairs % 8 == 0 && a.head_dim % 8 == 0 &&

@@ -2,9 +2,10 @@
 
 ``Rotary`` turns the query and key heads of a QKV projection by their tokens'
 positions: one axis for text, three (time, row, column) for images and video.
-The frequencies are kept as turns in 64-bit fixed point, so that the angle of a
-far position is as exact as that of a near one. There is no CPU fallback, and no gradient:
-backward() through a result raises.
+The frequencies are kept as turns in 64-bit fixed point: the product with a position is
+not rounded, and the frequency's own rounding moves position p by 2^-65 |p| turns, less than
+fp32 results show up to 2^38. There is no CPU fallback, and no gradient: backward() through
+a result raises.
 """
 from __future__ import annotations
 
@@ -139,7 +140,7 @@ class Rotary:
         or bfloat16 device tensors of one type, of any strides with whole heads; K may be
         None: then Q' alone). positions: int32 or int64, [...] the tokens' axes, or [axes,
         ...] where there are several. out: the results' tensors, which may be Q and K
-        themselves."""
+        themselves, and overlap nothing else."""
         import torch
         L = _lib or _library()
         device, dtype, D = Q.device, Q.dtype, self.head_dim
