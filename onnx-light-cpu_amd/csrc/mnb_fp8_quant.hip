@@ -27,8 +27,9 @@ __global__ __launch_bounds__(kThreads) void QuantizeKernel(const T *__restrict__
 #pragma unroll
   for (int off = 8; off >= 1; off >>= 1)
     top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 16)));
-  float amax;
-  const int2 code = BlockCodes<sizeof(T) == 4>(x, top, &amax);
+  float amax, q[8];
+  BlockQuotients<sizeof(T) == 4>(x, top, q, &amax);
+  const int2 code = Codes8(q);
   if ((threadIdx.x & 15) == 0) S[item] = amax / 448.0f;
   StoreCodes8<VEC>(Q + row * ldq + k0, static_cast<int>(min(int64_t{8}, ldq - k0)), code);
 }

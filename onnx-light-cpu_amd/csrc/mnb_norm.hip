@@ -22,6 +22,58 @@ struct Args {
   float epsilon;
 };
 
+// v rounded to fp32 such that a second rounding, to a code, is that of v itself: to the neighbour
+// with an odd last bit, if it is none.
+__device__ __forceinline__ float RoundToOdd(double v) {
+  const float f = static_cast<float>(v);
+  const double rest = v - static_cast<double>(f);
+  const uint32_t u = __float_as_uint(f);
+  if (rest == 0.0 || f == 0.0f || (u & 1) != 0) return f;
+  return __uint_as_float((rest > 0.0) == (f > 0.0f) ? u + 1 : u - 1);
+}
+
+// Codes of eight values h g of a block of 128 that 16 lanes hold, the nearest to 448 h g /
+// amax. The row's factor norm is in y = h g norm as in amax, which has the bits `top`, and drops
+// out. In fp32 the quotient is off by seven half units, 2^-24, at most: two each of y and amax, the
+// reciprocal's two and its product's. `less` and `more` hold it between them: 8 half units below
+// what was computed and 10 above it. Only where their codes differ, in one of 2^16, can it matter: a
+// wavefront that has such a code computes them again in 64 bits, where products and the middle
+// between two codes are exact. 8192 rows of 4096 take what they took with fp32 codes alone (44 us
+// over and over), rows of 16384, whose registers it raises from 69 to 90, 50 us for 46 (2000).
+__device__ __forceinline__ int2 NearestCodes(const float (&y)[8], const float (&h)[8],
+                                             const float (&g)[8], uint32_t top, float *amax) {
+  *amax = __uint_as_float(max(top, kLeastAmax));
+  const float by = 448.0f / *amax * (1.0f - 0x1p-21f);
+  float less[8], more[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    less[i] = y[i] * by;
+    more[i] = less[i] * (1.0f + 0x1.2p-20f);
+  }
+  int2 code = Codes8(less);
+  const int2 other = Codes8(more);
+  if (__any(code.x != other.x || code.y != other.y)) {
+    double most = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = fmax(most, fabs(static_cast<double>(h[i]) * g[i]));
+#pragma unroll
+    for (int off = 8; off >= 1; off >>= 1) most = fmax(most, __shfl_xor(most, off, 16));
+    float q[8];
+    if (top > kLeastAmax && top < 0x7F800000u) {
+      const double over = 1.0 / most;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // the nearest quotient, as in BlockQuotients
+        const double t = static_cast<double>(h[i]) * g[i] * 448.0, q0 = t * over;
+        q[i] = RoundToOdd(fma(fma(-q0, most, t), over, q0));
+      }
+    } else {
+      BlockQuotients<true>(y, top, q, amax);
+    }
+    code = Codes8(q);
+  }
+  return code;
+}
+
 // One workgroup per row; thread t holds the units of eight values t, t + T, ...,
 // so that a block of 128 is 16 neighbouring lanes. NV > 0: a row of at most NV T
 // units stays in registers between the sum of its squares and its second use, one
@@ -63,29 +115,35 @@ __global__ __launch_bounds__(kMaxThreads) void RmsNormKernel(Args a) {
   }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
+  double total = sum;
   if (threads > 64) {
     __shared__ float part[kMaxThreads / 64];
     if ((t & 63) == 0) part[t >> 6] = sum;
     __syncthreads();
-    sum = 0.0f;
-    for (int w = 0; w < threads / 64; ++w) sum += part[w];
+    total = 0.0;
+    for (int w = 0; w < threads / 64; ++w) total += part[w];
   }
-  const float norm = 1.0f / sqrtf(sum / static_cast<float>(a.K) + a.epsilon);
+  // One rounding for the factor that all values of the row share.
+  const float norm = static_cast<float>(
+      rsqrt(total / static_cast<double>(a.K) + static_cast<double>(a.epsilon)));
   const int64_t nb = (a.K + kBlock - 1) / kBlock;
   const auto finish = [&](int j, float(&y)[8]) {
     const int64_t k0 = 8 * (static_cast<int64_t>(j) * threads + t);
     const int n = static_cast<int>(min(int64_t{8}, a.K - k0));
-    float g[8];
+    float g[8], h[8];
     Load8<float, VEC>(a.gamma + k0, n, g);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = n > i ? y[i] * norm * g[i] : 0.0f;
+    for (int i = 0; i < 8; ++i) {
+      h[i] = y[i];
+      y[i] = n > i ? y[i] * norm * g[i] : 0.0f;
+    }
     if constexpr (CODES) {
       uint32_t top = TopBits(y);
 #pragma unroll
       for (int off = 8; off >= 1; off >>= 1)
         top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 16)));
       float amax;
-      const int2 code = BlockCodes<true>(y, top, &amax);
+      const int2 code = NearestCodes(y, h, g, top, &amax);
       if (n <= 0) return;
       if ((t & 15) == 0) a.scales[row * nb + k0 / kBlock] = amax / 448.0f;
       StoreCodes8<VEC>(static_cast<uint8_t *>(a.Y) + row * a.K + k0, n, code);

@@ -91,8 +91,8 @@ __device__ __forceinline__ int Codes4(float a, float b, float c, float d) {
   return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
 }
 
-// Codes of eight values of a row's block of 128 whose largest magnitude has the
-// bits `top`: 448 x / amax, amax at least 2^-100. FP32: the values are fp32, not
+// What the codes of eight values of a row's block of 128 are rounded from, the block's largest
+// magnitude having the bits `top`: 448 x / amax, amax at least 2^-100. FP32: the values are fp32, not
 // widened 16-bit ones. The quotient is correctly rounded to fp32 (for fp32 x up to
 // rare double roundings of a 2^-47 residue), since half-way codes are common among
 // 16-bit rows and a reciprocal's rounding would push them to either side: with
@@ -101,12 +101,13 @@ __device__ __forceinline__ int Codes4(float a, float b, float c, float d) {
 // rounds to the nearest (Markstein). t = 448 x 2^-e carries its own rounding
 // error along for fp32 rows. Four to six operations a value instead of a
 // division's eleven.
+constexpr uint32_t kLeastAmax = static_cast<uint32_t>(127 - 100) << 23;  // 2^-100
+
 template <bool FP32>
-__device__ __forceinline__ int2 BlockCodes(const float (&x)[8], uint32_t top, float *amax_out) {
-  const uint32_t least = static_cast<uint32_t>(127 - 100) << 23;  // 2^-100
-  const float amax = __uint_as_float(max(top, least));
+__device__ __forceinline__ void BlockQuotients(const float (&x)[8], uint32_t top, float (&q)[8],
+                                               float *amax_out) {
+  const float amax = __uint_as_float(max(top, kLeastAmax));
   const int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-  float q[8];
   if (top < 0x7F800000u) {
     const float a = ldexpf(amax, -e);
     const float r = 1.0f / a;
@@ -124,6 +125,9 @@ __device__ __forceinline__ int2 BlockCodes(const float (&x)[8], uint32_t top, fl
     for (int i = 0; i < 8; ++i) q[i] = x[i] / amax;  // 0 where x is finite (448 x may not be)
   }
   *amax_out = amax;
+}
+
+__device__ __forceinline__ int2 Codes8(const float (&q)[8]) {
   return make_int2(Codes4(q[0], q[1], q[2], q[3]), Codes4(q[4], q[5], q[6], q[7]));
 }
 

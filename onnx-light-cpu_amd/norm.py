@@ -110,8 +110,8 @@ def rms_norm(X, gamma, epsilon: float = 1e-5, residual=None, stream=None):
 
 
 def rms_norm_fp8(X, gamma, epsilon: float = 1e-5, residual=None, stream=None):
-    """(codes float8_e4m3fn [..., K], scales float32 [..., ceil(K / 128)]) of the fp32
-    norm that rms_norm rounds, as quantize_fp8 makes them; with a residual: (codes,
-    scales, h)."""
+    """(codes float8_e4m3fn [..., K], scales float32 [..., ceil(K / 128)]) of the norm that
+    rms_norm rounds, in quantize_fp8's format: the codes nearest to 448 times its unrounded
+    values over their block's largest; with a residual: (codes, scales, h)."""
     Y, scales, total = _run(X, gamma, epsilon, residual, True, stream)
     return (Y, scales) if total is None else (Y, scales, total)

@@ -201,3 +201,44 @@ def test_no_gradient(pkg, cuda, which):
         with pytest.raises(RuntimeError, match="no gradient"):
             y.sum().backward()
     assert x.grad is None and gamma.grad is None
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("M,K", [(1, 4096), (4096, 2048), (600, 5000), (64, 40001)])
+def test_codes_are_the_nearest(pkg, cuda, M, K, dtype):
+    """Every code is the one nearest to 448 y / amax as 64 bits have it, unless that lies
+    within 2^-45 of the middle of two: 64 bits themselves do not decide there. (The row's own
+    factor is y's and amax's, and drops out.)"""
+    import torch
+    x, r, gamma = _problem(M, K, getattr(torch, dtype), cuda, 11)
+    codes, _, h = pkg.rms_norm_fp8(x, gamma, residual=r)
+    nb = -(-K // 128)
+    u = torch.nn.functional.pad(h.double() * gamma.double(), (0, nb * 128 - K)).reshape(M, nb, 128)
+    q = 448.0 * u / u.abs().amax(dim=-1, keepdim=True)
+    step = torch.exp2(torch.floor(torch.log2(q.abs().clamp(min=2.0 ** -7))).clamp(min=-6.0) - 3.0)
+    got = torch.nn.functional.pad(codes.float(), (0, nb * 128 - K)).reshape(M, nb, 128).double()
+    assert ((got - q).abs() <= step / 2 + 2.0 ** -45 * q.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("K", [128, 512, 4096, 9999, 32776])
+def test_factor_of_a_row(pkg, cuda, K, dtype):
+    """Rows of powers of two, whose squares and their sums (below 2^24) are exact: a value of 1 is
+    the row's factor, rounded once, half a unit, 2^-24; a scale is four times it over 448, rounded
+    again. Of 16-bit results half a step more."""
+    import torch
+    dtype = getattr(torch, dtype)
+    g = torch.Generator(device=cuda)
+    g.manual_seed(13)
+    share = torch.rand(700, 1, device=cuda, generator=g)  # another mean for each row
+    x = torch.where(torch.rand(700, K, device=cuda, generator=g) < share, 1.0, 2.0)
+    x[:, ::128] = -4.0
+    ones = torch.ones(K, device=cuda)
+    norm = torch.rsqrt((x.double() ** 2).mean(dim=1, keepdim=True) + 2.0 ** -16)
+    Y = pkg.rms_norm(x.to(dtype), ones, 2.0 ** -16).double()
+    half = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -24)
+    want = x.double() * norm
+    assert ((Y - want).abs() <= (2.0 ** -24 + half) * want.abs()).all()
+    _, scales = pkg.rms_norm_fp8(x.to(dtype), ones, 2.0 ** -16)
+    want = 4.0 * norm / 448.0
+    assert ((scales.double() - want).abs() <= (2.0 ** -23 + 2.0 ** -48) * want).all()
