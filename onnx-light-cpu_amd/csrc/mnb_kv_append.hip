@@ -63,7 +63,7 @@ __host__ __device__ inline Units PageUnits(const Cache &c) { return {1, c.page_s
 // values: it alone writes that page, so nothing is atomic. An item is sixteen
 // values of a row; the rows are read for their largest magnitude and again, from
 // the caches, for their codes. Memory bounds prompts: 2 x 4001 tokens of 8 heads of
-// 128, bf16, take 12.4 us (33 MB read, 16 written: 4.0 TB/s). A token of each of 64 sequences takes
+// 128, bf16, take 12.6 us (33 MB read, 16 written: 3.9 TB/s). A token of each of 64 sequences takes
 // 4.6: table, old scale and rows are three trips to memory, a page that grows a fourth.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void AppendKernel(Cache c, Batch b, Rows k, Rows v) {
