@@ -80,7 +80,8 @@ __device__ __forceinline__ int2 NearestCodes(const float (&y)[8], const float (&
 // read of X and R and one write of each result; NV == 0: longer rows are read
 // again (h from where it was stored). Many rows are bound by memory: 8192 rows of 4096,
 // bf16, with residual and codes take 48 us (236 MB, 4.9 TB/s; 43 over and over, where the
-// last cache holds most of them), 333 fp32 rows of 2500 4.4. Few are one round trip to memory and the sum's: one row of 4096 3.1 us.
+// last cache holds most of them), 333 fp32 rows of 2500 4.4. Few are one round trip to memory
+// and the sum's: one row of 4096 3.1 us.
 template <typename T, bool VEC, bool CODES, int NV>
 __global__ __launch_bounds__(kMaxThreads) void RmsNormKernel(Args a) {
   constexpr int kUnits = NV > 0 ? NV : 1;
